@@ -5,6 +5,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <algorithm>
@@ -315,6 +316,12 @@ int check_device_errors(fo_ctx *ctx) {
     FO_CUDA(cudaMemcpy(&bits, ctx->dev_err, sizeof bits, cudaMemcpyDeviceToHost), "cudaMemcpy(error word)");
     if (bits) {
         cudaMemset(ctx->dev_err, 0, sizeof bits);
+        if (!(bits & ~(FO_DEVERR_PAGED | FO_DEVERR_POSITION | FO_DEVERR_VALUE))) {
+            if (bits & FO_DEVERR_PAGED)
+                return fail(FO_ERR_INVALID, "a paged call's page table, lengths or row ranges do not fit its buffers");
+            if (bits & FO_DEVERR_POSITION) return fail(FO_ERR_INVALID, "a rotary position lies outside its table");
+            return fail(FO_ERR_NONFINITE, "a value appended to a paged cache is not finite");
+        }
         return fail(FO_ERR_CUDA, "a kernel wait exceeded its time limit and the kernel unwound (bits 0x%x)", bits);
     }
     return FO_OK;
@@ -1695,6 +1702,205 @@ int fo_draft_attend(fo_draft_kv *kv, const float *q, int64_t bases, int64_t wind
         FO_CUDA(cudaStreamSynchronize(st), "cudaStreamSynchronize");
     }
     return FO_OK;
+}
+
+// ------------------------------------------- rotary positions, paged cache
+namespace {
+
+// Rows of heads that a call reads, or writes (every element apart).
+int check_rows(const fo_rows *r, const char *name, int64_t rows, int64_t dim, bool written) {
+    if (!r || !r->data) return fail(FO_ERR_INVALID, "%s: null pointer", name);
+    if (r->dtype != FO_DT_F32 && r->dtype != FO_DT_BF16) return fail(FO_ERR_INVALID, "%s: unknown type %d", name, r->dtype);
+    if (r->heads < 1) return fail(FO_ERR_INVALID, "%s: head count must be positive", name);
+    if (r->row_stride < 0 || r->head_stride < 0) return fail(FO_ERR_INVALID, "%s: negative stride", name);
+    if (reinterpret_cast<uintptr_t>(r->data) % (r->dtype == FO_DT_F32 ? 4 : 2) != 0)
+        return fail(FO_ERR_INVALID, "%s: misaligned for its type", name);
+    if (written) {
+        const bool rows_outer = (rows <= 1 || r->row_stride >= (r->heads - 1) * r->head_stride + dim) &&
+                                (r->heads <= 1 || r->head_stride >= dim);
+        const bool heads_outer = (r->heads <= 1 || r->head_stride >= (rows - 1) * r->row_stride + dim) &&
+                                 (rows <= 1 || r->row_stride >= dim);
+        if (!rows_outer && !heads_outer) return fail(FO_ERR_INVALID, "%s: rows overlap", name);
+    }
+    return FO_OK;
+}
+
+int check_rope(const fo_rope_spec *r, int64_t head_dim) {
+    if (!r || !r->table) return fail(FO_ERR_INVALID, "rope: null table");
+    if (reinterpret_cast<uintptr_t>(r->table) & 7) return fail(FO_ERR_INVALID, "rope: table must be 8-byte aligned");
+    if (r->positions < 1) return fail(FO_ERR_INVALID, "rope: table without positions");
+    if (r->rot_dim < 2 || r->rot_dim % 2 != 0 || r->rot_dim > head_dim)
+        return fail(FO_ERR_INVALID, "rope: rot_dim must be even and at most the head's width");
+    if (r->layout != FO_ROPE_INTERLEAVED && r->layout != FO_ROPE_HALF)
+        return fail(FO_ERR_INVALID, "rope: unknown layout %d", r->layout);
+    if (reinterpret_cast<uintptr_t>(r->row_positions) & 3) return fail(FO_ERR_INVALID, "rope: misaligned positions");
+    return FO_OK;
+}
+
+int check_paged(const fo_paged_kv *kv, const fo_paged_batch *b) {
+    if (!kv || !b) return fail(FO_ERR_INVALID, "paged cache: null descriptor");
+    if (kv->page_size != 16 && kv->page_size != 32 && kv->page_size != 64 && kv->page_size != 128)
+        return fail(FO_ERR_INVALID, "paged cache: page_size must be 16, 32, 64 or 128");
+    if (kv->head_dim != 64 && kv->head_dim != 128) return fail(FO_ERR_INVALID, "paged cache: head_dim must be 64 or 128");
+    if (kv->format != FO_PAGED_I8 && kv->format != FO_PAGED_E4M3)
+        return fail(FO_ERR_INVALID, "paged cache: unknown format %d", kv->format);
+    if (kv->n_kv_heads < 1 || kv->n_kv_heads > 4096) return fail(FO_ERR_INVALID, "paged cache: KV heads must be 1..4096");
+    if (kv->n_pages < 1 || kv->n_pages > INT32_MAX) return fail(FO_ERR_INVALID, "paged cache: pages must be 1..2^31 - 1");
+    if (!kv->k_codes || !kv->v_codes || !kv->k_scales || !kv->v_scales)
+        return fail(FO_ERR_INVALID, "paged cache: null pool pointer");
+    if (!aligned16(kv->k_codes) || !aligned16(kv->v_codes))
+        return fail(FO_ERR_INVALID, "paged cache: codes must be 16-byte aligned");
+    if (!aligned4(kv->k_scales) || !aligned4(kv->v_scales))
+        return fail(FO_ERR_INVALID, "paged cache: misaligned scales");
+    if (b->n_seqs < 0 || b->n_seqs > 65535 || b->max_rows < 0 || b->max_rows > INT32_MAX || b->total_rows < 0 ||
+        b->total_rows > INT32_MAX)
+        return fail(FO_ERR_INVALID, "paged batch: at most 65,535 sequences and 2^31 - 1 rows");
+    if (!b->row_start && b->total_rows != b->n_seqs * b->max_rows)
+        return fail(FO_ERR_INVALID, "paged batch: total_rows must be n_seqs * max_rows");
+    if (b->n_seqs > 0) {
+        if (!b->page_table || !b->lens) return fail(FO_ERR_INVALID, "paged batch: null page table or lengths");
+        if (b->table_stride < 1 || b->table_stride > INT32_MAX / kv->page_size)
+            return fail(FO_ERR_INVALID, "paged batch: a sequence has 1 page to 2^31 - 1 positions");
+        if (!aligned4(b->page_table) || !aligned4(b->lens) || !aligned4(b->row_start))
+            return fail(FO_ERR_INVALID, "paged batch: misaligned integers");
+    }
+    return FO_OK;
+}
+
+#define FO_TRY(call)                  \
+    do {                              \
+        const int st_ = (call);       \
+        if (st_ != FO_OK) return st_; \
+    } while (0)
+
+}  // namespace
+
+int fo_rope_table(fo_ctx *ctx, float *table, int64_t positions, int32_t rot_dim, fo_rope_scaling s) {
+    if (!table || reinterpret_cast<uintptr_t>(table) % 8 != 0)
+        return fail(FO_ERR_INVALID, "fo_rope_table: the table must be an 8-byte aligned device pointer");
+    if (positions < 1 || positions > INT32_MAX || rot_dim < 2 || rot_dim % 2 != 0 || rot_dim > 256)
+        return fail(FO_ERR_INVALID, "fo_rope_table: positions must be positive, rot_dim even and at most 256");
+    if (!(s.theta > 1.0) || !std::isfinite(s.theta)) return fail(FO_ERR_INVALID, "fo_rope_table: theta must be above 1");
+    if (s.scaling < FO_ROPE_PLAIN || s.scaling > FO_ROPE_YARN)
+        return fail(FO_ERR_INVALID, "fo_rope_table: unknown scaling %d", s.scaling);
+    if (s.scaling != FO_ROPE_PLAIN && (!(s.factor > 0.0) || !std::isfinite(s.factor)))
+        return fail(FO_ERR_INVALID, "fo_rope_table: factor must be positive");
+    if (s.scaling == FO_ROPE_YARN &&
+        (!(s.original_positions > 0.0) || !(s.beta_slow > 0.0) || !(s.beta_fast >= s.beta_slow) ||
+         !(s.attention_factor >= 0.0)))
+        return fail(FO_ERR_INVALID, "fo_rope_table: YARN wants original positions, beta_fast >= beta_slow > 0 and "
+                                    "attention_factor >= 0");
+    if (!ctx) return fail(FO_ERR_INVALID, "null context");
+    DeviceGuard guard(ctx->device);
+    cudaError_t e = fo_launch_rope_table(table, positions, rot_dim, &s, ctx->stream);
+    return e == cudaSuccess ? FO_OK : cuda_fail(e, "rope table launch");
+}
+
+int fo_rope(fo_ctx *ctx, const fo_rows *x, const fo_rows *out, int64_t rows, int32_t head_dim,
+            const fo_rope_spec *rope, int32_t transpose) {
+    if (rows < 0 || rows > INT32_MAX) return fail(FO_ERR_INVALID, "fo_rope: rows must be 0..2^31 - 1");
+    if (head_dim < 2 || head_dim > 256) return fail(FO_ERR_INVALID, "fo_rope: head_dim must be 2..256");
+    FO_TRY(check_rows(x, "fo_rope x", rows, head_dim, false));
+    FO_TRY(check_rows(out, "fo_rope out", rows, head_dim, true));
+    if (x->heads != out->heads || x->dtype != out->dtype)
+        return fail(FO_ERR_INVALID, "fo_rope: x and out must have one type and as many heads");
+    FO_TRY(check_rope(rope, head_dim));
+    const bool in_place = x->data == out->data;
+    if (in_place && (x->row_stride != out->row_stride || x->head_stride != out->head_stride))
+        return fail(FO_ERR_INVALID, "fo_rope: in place, x and out must be laid out alike");
+    if (!ctx) return fail(FO_ERR_INVALID, "null context");
+    DeviceGuard guard(ctx->device);
+    fo_rope_launch a = {};
+    a.x = *x;
+    a.out = *out;
+    a.rows = rows;
+    a.rope = *rope;
+    a.err = ctx->dev_err;
+    a.head_dim = head_dim;
+    a.transpose = transpose != 0;
+    a.in_place = in_place;
+    cudaError_t e = fo_launch_rope(&a, ctx->stream);
+    return e == cudaSuccess ? FO_OK : cuda_fail(e, "rope launch");
+}
+
+int fo_paged_append(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch *batch, const fo_rows *k,
+                    const fo_rows *v, const fo_rows *q, const fo_rows *q_out, const fo_rope_spec *rope) {
+    FO_TRY(check_paged(kv, batch));
+    const int64_t rows = batch->total_rows;
+    FO_TRY(check_rows(k, "fo_paged_append k", rows, kv->head_dim, false));
+    FO_TRY(check_rows(v, "fo_paged_append v", rows, kv->head_dim, false));
+    if (k->heads != kv->n_kv_heads || v->heads != kv->n_kv_heads)
+        return fail(FO_ERR_INVALID, "fo_paged_append: k and v must have the cache's heads");
+    if (k->dtype != v->dtype) return fail(FO_ERR_INVALID, "fo_paged_append: k and v must have one type");
+    if (rope) FO_TRY(check_rope(rope, kv->head_dim));
+    if ((q != nullptr) != (q_out != nullptr)) return fail(FO_ERR_INVALID, "fo_paged_append: q needs q_out");
+    bool in_place = false;
+    if (q) {
+        if (!rope) return fail(FO_ERR_INVALID, "fo_paged_append: queries are taken to be rotated, without rope there is nothing to do");
+        FO_TRY(check_rows(q, "fo_paged_append q", rows, kv->head_dim, false));
+        FO_TRY(check_rows(q_out, "fo_paged_append q_out", rows, kv->head_dim, true));
+        if (q->heads != q_out->heads || q->dtype != q_out->dtype || q->dtype != k->dtype)
+            return fail(FO_ERR_INVALID, "fo_paged_append: q and q_out must have one type, the keys', and as many heads");
+        in_place = q->data == q_out->data;
+        if (in_place && (q->row_stride != q_out->row_stride || q->head_stride != q_out->head_stride))
+            return fail(FO_ERR_INVALID, "fo_paged_append: in place, q and q_out must be laid out alike");
+    }
+    if (!ctx) return fail(FO_ERR_INVALID, "null context");
+    if (rows == 0) return FO_OK;
+    DeviceGuard guard(ctx->device);
+    fo_append_launch a = {};
+    a.kv = *kv;
+    a.batch = *batch;
+    a.k = *k;
+    a.v = *v;
+    a.err = ctx->dev_err;
+    if (rope) {
+        a.rope = *rope;
+        a.rotate = 1;
+    }
+    if (q) {
+        a.q.x = *q;
+        a.q.out = *q_out;
+        a.q.rows = rows;
+        a.q.rope = *rope;
+        a.q.err = ctx->dev_err;
+        a.q.head_dim = kv->head_dim;
+        a.q.in_place = in_place;
+    }
+    cudaError_t e = fo_launch_paged_append(&a, ctx->stream);
+    return e == cudaSuccess ? FO_OK : cuda_fail(e, "paged append launch");
+}
+
+int fo_paged_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch *batch, const fo_rows *q,
+                       const float *sinks, float scale, int64_t window, const fo_rows *out, float *lse) {
+    FO_TRY(check_paged(kv, batch));
+    const int64_t rows = batch->total_rows;
+    FO_TRY(check_rows(q, "fo_paged_attention q", rows, kv->head_dim, false));
+    FO_TRY(check_rows(out, "fo_paged_attention out", rows, kv->head_dim, true));
+    if (q->heads != out->heads || q->dtype != out->dtype)
+        return fail(FO_ERR_INVALID, "fo_paged_attention: q and out must have one type and as many heads");
+    if (q->heads % kv->n_kv_heads != 0 || q->heads > 65535)
+        return fail(FO_ERR_INVALID, "fo_paged_attention: query heads must be a multiple of the KV heads");
+    if (batch->max_rows > FO_PAGED_MAX_ROWS)
+        return fail(FO_ERR_INVALID, "fo_paged_attention: at most %d rows a sequence", FO_PAGED_MAX_ROWS);
+    if (!std::isfinite(scale)) return fail(FO_ERR_INVALID, "fo_paged_attention: scale must be finite");
+    if (window < 0) return fail(FO_ERR_INVALID, "fo_paged_attention: negative window");
+    if (!aligned4(sinks) || !aligned4(lse)) return fail(FO_ERR_INVALID, "fo_paged_attention: misaligned sinks or lse");
+    if (!ctx) return fail(FO_ERR_INVALID, "null context");
+    if (rows == 0) return FO_OK;
+    DeviceGuard guard(ctx->device);
+    fo_paged_attention_launch a = {};
+    a.kv = *kv;
+    a.batch = *batch;
+    a.q = *q;
+    a.out = *out;
+    a.sinks = sinks;
+    a.lse = lse;
+    a.scale = scale;
+    a.window = window;
+    a.err = ctx->dev_err;
+    cudaError_t e = fo_launch_paged_attention(&a, ctx->stream);
+    return e == cudaSuccess ? FO_OK : cuda_fail(e, "paged attention launch");
 }
 
 }  // extern "C"

@@ -6,6 +6,8 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include "../../include/fo_attention.h"
+
 #ifdef __cplusplus
 extern "C" {
 #endif
@@ -188,6 +190,54 @@ cudaError_t fo_launch_draft_attend(const int8_t *key_codes, const float *key_sca
                                    const float *value_scales, int64_t capacity, const float *q, int64_t start,
                                    int64_t n, const float *chain_keys, const float *chain_values, int64_t chain,
                                    float *part, unsigned *counters, float *out, cudaStream_t stream);
+
+// Device error bits of the rotary and paged-cache kernels: a page table,
+// length or row range that does not fit its buffers; a rotary position
+// outside its table; a value that is not finite.
+#define FO_DEVERR_PAGED 4u
+#define FO_DEVERR_POSITION 8u
+#define FO_DEVERR_VALUE 16u
+
+// Rotation of rows of heads (rope.cu); the launcher fills in the last line.
+struct fo_rope_launch {
+    fo_rows x, out;
+    int64_t rows;
+    fo_rope_spec rope;
+    unsigned *err;
+    int32_t head_dim, transpose, in_place;
+    int32_t slots, head_blocks, block_x;
+};
+cudaError_t fo_launch_rope_table(float *table, int64_t positions, int32_t rot_dim, const fo_rope_scaling *scaling,
+                                 cudaStream_t stream);
+cudaError_t fo_launch_rope(const fo_rope_launch *args, cudaStream_t stream);
+
+// Appending rows to the paged cache (paged_append.cu): k and v into their
+// pages (k rotated when rotate is set), and the queries' rotation (q.rows 0:
+// none).
+struct fo_append_launch {
+    fo_paged_kv kv;
+    fo_paged_batch batch;
+    fo_rows k, v;
+    fo_rope_spec rope;
+    fo_rope_launch q;
+    unsigned *err;
+    int32_t rotate;
+};
+cudaError_t fo_launch_paged_append(const fo_append_launch *args, cudaStream_t stream);
+
+// Attention over the paged cache (paged_attention.cu).
+#define FO_PAGED_MAX_ROWS 64  // rows of one sequence
+struct fo_paged_attention_launch {
+    fo_paged_kv kv;
+    fo_paged_batch batch;
+    fo_rows q, out;
+    const float *sinks;
+    float *lse;
+    float scale;
+    int64_t window;
+    unsigned *err;
+};
+cudaError_t fo_launch_paged_attention(const fo_paged_attention_launch *args, cudaStream_t stream);
 
 // The bounded-wait self-test kernel (selftest.cu).
 cudaError_t fo_launch_bounded_wait(unsigned *err, unsigned long long limit_ns, cudaStream_t stream);

@@ -1,0 +1,167 @@
+// paged.cuh -- device helpers shared by the rotary kernels and the paged
+// 8-bit KV cache (rope.cu, paged_append.cu, paged_attention.cu): rows of
+// heads in FP32 or BF16, a batch's sequences, and the 8-bit codes.
+#pragma once
+
+#include <float.h>
+
+#include "fo_common.cuh"
+#include "fo_kernels.h"
+
+namespace fo {
+
+// ------------------------------------------------------------- row elements
+// Ordinary loads: fo_rope may write the rows that it reads.
+template <typename T>
+__device__ __forceinline__ float load1(const T *p);
+template <>
+__device__ __forceinline__ float load1<float>(const float *p) { return *p; }
+template <>
+__device__ __forceinline__ float load1<uint16_t>(const uint16_t *p) { return bf16_f32(*p); }
+
+// Eight adjacent elements; p 16-byte aligned.
+template <typename T>
+__device__ __forceinline__ void load8(const T *p, float *x);
+template <>
+__device__ __forceinline__ void load8<float>(const float *p, float *x) {
+    const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+}
+template <>
+__device__ __forceinline__ void load8<uint16_t>(const uint16_t *p, float *x) {
+    const uint4 a = *reinterpret_cast<const uint4 *>(p);
+    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        x[2 * i] = __uint_as_float(w[i] << 16);
+        x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+    }
+}
+
+// Two floats as a BF16 pair, each rounded to nearest even (NaN stays NaN).
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+__device__ __forceinline__ void store1(float *p, float x) { *p = x; }
+__device__ __forceinline__ void store1(uint16_t *p, float x) { *p = (uint16_t)bf16_pair(x, 0.0f); }
+__device__ __forceinline__ void store8(float *p, const float *x) {
+    reinterpret_cast<float4 *>(p)[0] = make_float4(x[0], x[1], x[2], x[3]);
+    reinterpret_cast<float4 *>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
+}
+__device__ __forceinline__ void store8(uint16_t *p, const float *x) {
+    *reinterpret_cast<uint4 *>(p) =
+        make_uint4(bf16_pair(x[0], x[1]), bf16_pair(x[2], x[3]), bf16_pair(x[4], x[5]), bf16_pair(x[6], x[7]));
+}
+
+// ---------------------------------------------------------------- rotation
+// A pair's two results, every product and sum rounded on its own.
+__device__ __forceinline__ float rot_first(float a, float b, float2 cs) {
+    return __fsub_rn(__fmul_rn(a, cs.x), __fmul_rn(b, cs.y));
+}
+__device__ __forceinline__ float rot_second(float a, float b, float2 cs) {
+    return __fadd_rn(__fmul_rn(b, cs.x), __fmul_rn(a, cs.y));
+}
+
+// ---------------------------------------------------------------- sequences
+// Sequence b of a batch: its rows [first, first + n) and its positions.  What
+// does not fit its buffers (rows out of order or beyond total_rows, more than
+// max_rows; a length beyond the page table) raises FO_DEVERR_PAGED and leaves
+// the sequence without rows, or without positions.
+struct Sequence {
+    int64_t first, len;
+    int n;
+};
+__device__ __forceinline__ Sequence load_sequence(const fo_paged_batch &b, int page_size, int64_t seq, unsigned *err) {
+    Sequence s;
+    s.len = __ldg(b.lens + seq);
+    if (b.row_start) {
+        const int64_t r0 = __ldg(b.row_start + seq), r1 = __ldg(b.row_start + seq + 1);
+        s.first = r0;
+        s.n = (int)(r1 - r0);
+        if (r0 < 0 || r1 < r0 || r1 > b.total_rows || r1 - r0 > b.max_rows) {
+            atomicOr(err, FO_DEVERR_PAGED);
+            s.first = 0;
+            s.n = 0;
+        }
+    } else {
+        s.first = seq * b.max_rows;
+        s.n = (int)b.max_rows;
+    }
+    if (s.len > b.table_stride * page_size) {
+        atomicOr(err, FO_DEVERR_PAGED);
+        s.len = 0;
+    }
+    if (s.len < 0) s.len = 0;
+    return s;
+}
+
+// The pool's page number for a sequence's page j (0 and the error word for
+// one outside the pool).
+__device__ __forceinline__ int64_t page_of(const fo_paged_batch &b, int64_t n_pages, int64_t seq, int64_t j,
+                                           unsigned *err, bool &valid) {
+    const int64_t p = __ldg(b.page_table + seq * b.table_stride + j);
+    valid = p >= 0 && p < n_pages;
+    if (!valid) atomicOr(err, FO_DEVERR_PAGED);
+    return valid ? p : 0;
+}
+
+// -------------------------------------------------------------------- codes
+__device__ __forceinline__ float code_max(int format) { return format == FO_PAGED_I8 ? 127.0f : 448.0f; }
+
+// A value against its block's scale, x / scale rounded once, saturated to the
+// largest code (so is an infinity); NaN, and anything in a block of scale 0,
+// gives 0.
+__device__ __forceinline__ float scaled(float x, float scale, float top) {
+    const float y = __fdiv_rn(x, scale);
+    return scale > 0.0f && x == x ? fminf(fmaxf(y, -top), top) : 0.0f;
+}
+
+// Four codes from four values within the codes' range, rounded to nearest
+// even.
+template <int FORMAT>
+__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
+    if constexpr (FORMAT == FO_PAGED_I8) {
+        const uint32_t x = (uint32_t)__float2int_rn(a) & 255u, y = (uint32_t)__float2int_rn(b) & 255u;
+        const uint32_t z = (uint32_t)__float2int_rn(c) & 255u, w = (uint32_t)__float2int_rn(d);
+        return x | y << 8 | z << 16 | w << 24;
+    } else {
+        uint32_t r;
+        asm("{\n\t.reg .b16 lo, hi;\n\t"
+            "cvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\t"
+            "cvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\t"
+            "mov.b32 %0, {lo, hi};\n\t}"
+            : "=r"(r)
+            : "f"(a), "f"(b), "f"(c), "f"(d));
+        return r;
+    }
+}
+
+// Two FP8 codes as an FP16 pair (exact); the low byte's in the low half.
+__device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t pair) {
+    uint32_t r;
+    asm("{\n\t.reg .b16 lo;\n\tcvt.u16.u32 lo, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\t}" : "=r"(r) : "r"(pair));
+    return r;
+}
+__device__ __forceinline__ float2 f16x2_f32x2(uint32_t h) {
+    float2 f;
+    asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.f32.f16 %0, lo;\n\tcvt.f32.f16 %1, hi;\n\t}"
+        : "=f"(f.x), "=f"(f.y)
+        : "r"(h));
+    return f;
+}
+
+// Four codes as floats (exact).
+template <int FORMAT>
+__device__ __forceinline__ void decode4(uint32_t w, float *f) {
+    if constexpr (FORMAT == FO_PAGED_I8) {
+        s8x4_f32(w, f);
+    } else {
+        const float2 lo = f16x2_f32x2(e4m3x2_f16x2(w & 0xFFFFu)), hi = f16x2_f32x2(e4m3x2_f16x2(w >> 16));
+        f[0] = lo.x, f[1] = lo.y, f[2] = hi.x, f[3] = hi.y;
+    }
+}
+
+}  // namespace fo

@@ -1,0 +1,155 @@
+// paged_rope.cuh -- the rotation of rows of heads as a device function: the
+// whole of fo_rope's kernel (rope.cu) and the queries' part of the paged
+// append (paged_append.cu).
+#pragma once
+
+#include "paged.cuh"
+
+namespace fo {
+
+constexpr int ROPE_THREADS = 256;
+constexpr int ROPE_HEADS = 4;  // heads a thread takes, with one read of its table entries
+
+// Work of one row: a slot is eight adjacent elements of a head (interleaved
+// layout, and elements that pass unrotated), or eight pairs (half layout:
+// two groups of eight elements rot_dim / 2 apart); without 16-byte alignment
+// (VEC false) one pair or one passing element.
+__host__ __device__ inline int rope_slots(const fo_rope_launch &a, bool vec, bool half) {
+    const int rot = a.rope.rot_dim, pass = a.in_place ? 0 : a.head_dim - rot;
+    if (!vec) return rot / 2 + pass;
+    return half ? rot / 16 + pass / 8 : (rot + pass + 7) / 8;
+}
+
+// Chooses between whole 16-byte groups and single elements, and the block's
+// width; returns whether groups are used.
+inline bool rope_shape(fo_rope_launch *a) {
+    const int64_t unit = a->x.dtype == FO_DT_F32 ? 4 : 8;  // elements in 16 bytes
+    auto ok = [&](const fo_rows &r) {
+        return (reinterpret_cast<uintptr_t>(r.data) & 15) == 0 && r.row_stride % unit == 0 && r.head_stride % unit == 0;
+    };
+    const bool half = a->rope.layout == FO_ROPE_HALF;
+    const bool vec = ok(a->x) && ok(a->out) && a->head_dim % 8 == 0 && (!half || a->rope.rot_dim % 16 == 0);
+    a->slots = rope_slots(*a, vec, half);
+    a->head_blocks = (a->x.heads + ROPE_HEADS - 1) / ROPE_HEADS;
+    const int64_t width = (int64_t)a->slots * a->head_blocks;
+    a->block_x = (int)(width < ROPE_THREADS ? (width < 1 ? 1 : width) : ROPE_THREADS);
+    return vec;
+}
+
+// Block `block` of the rotation; `position(row, padded)` gives a row's
+// position, or sets padded (the row is copied as it is).
+template <typename T, bool HALF, bool VEC, typename Position>
+__device__ __forceinline__ void rope_block(const fo_rope_launch &a, int64_t block, Position position) {
+    // Threads x over (head block, slot), y over rows; the block's shape is
+    // recomputed from block_x so that it also runs inside a 1-D block.
+    const int t = threadIdx.y * blockDim.x + threadIdx.x;
+    const int rows_per_block = ROPE_THREADS / a.block_x;
+    const int ty = t / a.block_x, tx = t - ty * a.block_x;
+    const int64_t row = block * rows_per_block + ty;
+    if (ty >= rows_per_block || row >= a.rows) return;
+    bool padded;
+    const int64_t p = position(row, padded);
+    const bool inside = p >= 0 && p < a.rope.positions;
+    if (!inside && !padded && tx == 0) atomicOr(a.err, FO_DEVERR_POSITION);
+    const int rot = a.rope.rot_dim, h2 = rot / 2;
+    const float2 *entries = reinterpret_cast<const float2 *>(a.rope.table) + (inside ? p : 0) * h2;
+    auto entry = [&](int pair) {
+        float2 cs = __ldg(entries + pair);
+        if (!inside) cs = padded ? make_float2(1.0f, 0.0f) : make_float2(NAN, NAN);
+        if (a.transpose) cs.y = -cs.y;
+        return cs;
+    };
+    const T *xr = static_cast<const T *>(a.x.data) + row * a.x.row_stride;
+    T *yr = static_cast<T *>(a.out.data) + row * a.out.row_stride;
+    const int width = a.slots * a.head_blocks;
+    for (int w = tx; w < width; w += a.block_x) {
+        const int hb = w / a.slots, slot = w - hb * a.slots;
+        // Heads hb, hb + head_blocks, ..: neighbouring threads take
+        // neighbouring heads.
+        if constexpr (VEC && HALF) {
+            const int pairs8 = rot / 16;
+            if (slot < pairs8) {
+                const int d = slot * 8;
+                float x0[ROPE_HEADS][8], x1[ROPE_HEADS][8];
+#pragma unroll
+                for (int k = 0; k < ROPE_HEADS; k++) {
+                    const int h = hb + k * a.head_blocks;
+                    if (h < a.x.heads) {
+                        load8(xr + h * a.x.head_stride + d, x0[k]);
+                        load8(xr + h * a.x.head_stride + d + h2, x1[k]);
+                    }
+                }
+                float2 cs[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) cs[e] = entry(d + e);
+#pragma unroll
+                for (int k = 0; k < ROPE_HEADS; k++) {
+                    const int h = hb + k * a.head_blocks;
+                    if (h < a.x.heads) {
+                        float y0[8], y1[8];
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            y0[e] = rot_first(x0[k][e], x1[k][e], cs[e]);
+                            y1[e] = rot_second(x0[k][e], x1[k][e], cs[e]);
+                        }
+                        store8(yr + h * a.out.head_stride + d, y0);
+                        store8(yr + h * a.out.head_stride + d + h2, y1);
+                    }
+                }
+            } else {
+                const int d = rot + (slot - pairs8) * 8;
+#pragma unroll
+                for (int k = 0; k < ROPE_HEADS; k++) {
+                    const int h = hb + k * a.head_blocks;
+                    float x[8];
+                    if (h < a.x.heads) {
+                        load8(xr + h * a.x.head_stride + d, x);
+                        store8(yr + h * a.out.head_stride + d, x);
+                    }
+                }
+            }
+        } else if constexpr (VEC) {
+            const int d = slot * 8;
+            float x[ROPE_HEADS][8];
+#pragma unroll
+            for (int k = 0; k < ROPE_HEADS; k++) {
+                const int h = hb + k * a.head_blocks;
+                if (h < a.x.heads) load8(xr + h * a.x.head_stride + d, x[k]);
+            }
+            float2 cs[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) cs[e] = d + 2 * e < rot ? entry(d / 2 + e) : make_float2(1.0f, 0.0f);
+#pragma unroll
+            for (int k = 0; k < ROPE_HEADS; k++) {
+                const int h = hb + k * a.head_blocks;
+                if (h < a.x.heads) {
+                    float y[8];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const bool turn = d + 2 * e < rot;  // a passing element keeps its bits
+                        y[2 * e] = turn ? rot_first(x[k][2 * e], x[k][2 * e + 1], cs[e]) : x[k][2 * e];
+                        y[2 * e + 1] = turn ? rot_second(x[k][2 * e], x[k][2 * e + 1], cs[e]) : x[k][2 * e + 1];
+                    }
+                    store8(yr + h * a.out.head_stride + d, y);
+                }
+            }
+        } else {
+            const bool pair = slot < h2;
+            const int d0 = !pair ? rot + slot - h2 : HALF ? slot : 2 * slot;
+            const int d1 = HALF ? slot + h2 : 2 * slot + 1;
+            const float2 cs = pair ? entry(slot) : make_float2(1.0f, 0.0f);
+            for (int h = hb; h < a.x.heads; h += a.head_blocks) {
+                const float u = load1(xr + h * a.x.head_stride + d0);
+                if (pair) {
+                    const float v = load1(xr + h * a.x.head_stride + d1);
+                    store1(yr + h * a.out.head_stride + d0, rot_first(u, v, cs));
+                    store1(yr + h * a.out.head_stride + d1, rot_second(u, v, cs));
+                } else {
+                    store1(yr + h * a.out.head_stride + d0, u);
+                }
+            }
+        }
+    }
+}
+
+}  // namespace fo

@@ -90,6 +90,43 @@ class PrefillOptions(ctypes.Structure):
         return cls(EXP_EXACT, 0, SOFTMAX_ONLINE, SOFTMAX_ONLINE)
 
 
+class Rows(ctypes.Structure):
+    """fo_rows: rows of heads in device memory."""
+    _fields_ = [("data", ctypes.c_void_p), ("row_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
+                ("heads", ctypes.c_int32), ("dtype", ctypes.c_int32)]
+
+
+class RopeScaling(ctypes.Structure):
+    """fo_rope_scaling"""
+    _fields_ = [("theta", ctypes.c_double), ("scaling", ctypes.c_int32), ("factor", ctypes.c_double),
+                ("original_positions", ctypes.c_double), ("beta_fast", ctypes.c_double),
+                ("beta_slow", ctypes.c_double), ("attention_factor", ctypes.c_double)]
+
+
+class RopeSpec(ctypes.Structure):
+    """fo_rope_spec"""
+    _fields_ = [("table", ctypes.c_void_p), ("positions", ctypes.c_int64), ("row_positions", ctypes.c_void_p),
+                ("rot_dim", ctypes.c_int32), ("layout", ctypes.c_int32)]
+
+
+class PagedPool(ctypes.Structure):
+    """fo_paged_kv"""
+    _fields_ = [("k_codes", ctypes.c_void_p), ("v_codes", ctypes.c_void_p), ("k_scales", ctypes.c_void_p),
+                ("v_scales", ctypes.c_void_p), ("n_pages", ctypes.c_int64), ("page_size", ctypes.c_int32),
+                ("n_kv_heads", ctypes.c_int32), ("head_dim", ctypes.c_int32), ("format", ctypes.c_int32)]
+
+
+class PagedSequences(ctypes.Structure):
+    """fo_paged_batch"""
+    _fields_ = [("page_table", ctypes.c_void_p), ("lens", ctypes.c_void_p), ("row_start", ctypes.c_void_p),
+                ("table_stride", ctypes.c_int64), ("n_seqs", ctypes.c_int64), ("max_rows", ctypes.c_int64),
+                ("total_rows", ctypes.c_int64)]
+
+
+ROPE_LAYOUTS = {"interleaved": 0, "half": 1}
+ROPE_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
+PAGED_I8, PAGED_E4M3 = 0, 1
+
 EXPORTS = [
     "fo_version", "fo_last_error", "fo_ctx_create", "fo_ctx_destroy", "fo_ctx_synchronize", "fo_ctx_last_ms",
     "fo_attention", "fo_attention_prefill_bf16", "fo_convert_bf16", "fo_kv_seal", "fo_kv_destroy",
@@ -103,7 +140,8 @@ EXPORTS = [
     "fo_attention_prefill_bf16_rows", "fo_attention_prefill_bf16_rows_split", "fo_i8_seal", "fo_i8_destroy", "fo_i8_bytes", "fo_i8_records",
     "fo_i8_decode_batch", "fo_draft_kv_create", "fo_draft_kv_destroy", "fo_draft_kv_push", "fo_draft_kv_len",
     "fo_draft_kv_bytes", "fo_draft_kv_records", "fo_draft_attend", "fo_peer_block_register",
-    "fo_peer_block_destroy", "fo_sharded_prefill_bf16_peers",
+    "fo_peer_block_destroy", "fo_sharded_prefill_bf16_peers", "fo_rope_table", "fo_rope", "fo_paged_append",
+    "fo_paged_attention",
 ]
 
 _lib: Optional[ctypes.CDLL] = None
@@ -176,6 +214,10 @@ def lib() -> ctypes.CDLL:
         "fo_peer_block_register": (I, [P, P, I32, I32, P, I64, ctypes.POINTER(P)]),
         "fo_peer_block_destroy": (I, [P]),
         "fo_sharded_prefill_bf16_peers": (I, [P, P, P, P, P, I64, I64, I64, Geometry, P, PrefillOptions, I32]),
+        "fo_rope_table": (I, [P, P, I64, I32, RopeScaling]),
+        "fo_rope": (I, [P, P, P, I64, I32, P, I32]),
+        "fo_paged_append": (I, [P, P, P, P, P, P, P, P]),
+        "fo_paged_attention": (I, [P, P, P, P, P, ctypes.c_float, I64, P, P]),
     }
     for name, (res, args) in sigs.items():
         fn = getattr(L, name)
@@ -668,6 +710,181 @@ def static_scratch_status(stream=None):
     """fo_decode_static_scratch_status: raises CudaError if a bounded device
     wait of a static-scratch decode gave up since the last check."""
     check(lib().fo_decode_static_scratch_status(stream))
+
+
+# ------------------------------------------------ rotary positions, paged cache
+_ROW_TYPES = None  # torch dtype -> FO_DT_*
+_stream_contexts = {}
+
+
+def _torch():
+    global _ROW_TYPES
+    import torch
+    if _ROW_TYPES is None:
+        _ROW_TYPES = {torch.float32: 0, torch.bfloat16: 1}
+    return torch
+
+
+def stream_context(device: int) -> Context:
+    """The context of torch's current stream on `device` (made at its first
+    use, so a stream that is to be captured runs once before)."""
+    stream = _torch()._C._cuda_getCurrentRawStream(device)
+    ctx = _stream_contexts.get((device, stream))
+    if ctx is None:
+        ctx = _stream_contexts[(device, stream)] = Context(device, stream or None)
+    return ctx
+
+
+def _rows(t, name: str) -> Rows:
+    """A CUDA tensor [rows][heads][head_dim] as fo_rows; rows and heads in any
+    strides."""
+    if _ROW_TYPES is None:
+        _torch()
+    kind = _ROW_TYPES.get(t.dtype)
+    if kind is None or not t.is_cuda or t.dim() != 3:
+        raise FoError(f"{name} must be a CUDA tensor [rows][heads][head_dim] of float32 or bfloat16")
+    shape, stride = t.shape, t.stride()
+    if stride[2] != 1:
+        raise FoError(f"{name}: a head's values must be adjacent")
+    return Rows(t.data_ptr(), stride[0], stride[1], shape[1], kind)
+
+
+def _device_ints(t, name: str):
+    if not _on_device(t) or not t.is_contiguous() or str(t.dtype) != "torch.int32":
+        raise FoError(f"{name} must be a contiguous CUDA tensor of int32")
+    return t.data_ptr()
+
+
+def rope_table(table, theta=10000.0, scaling="none", factor=1.0, original_positions=0, beta_fast=32.0, beta_slow=1.0,
+               attention_factor=0.0, ctx=None):
+    """fo_rope_table: fills the CUDA tensor `table` [positions][rot_dim / 2][2]
+    with {cos, sin}; scaling "none", "linear", "ntk" or "yarn"."""
+    if not _on_device(table) or not table.is_contiguous() or table.dim() != 3 or table.shape[2] != 2 or \
+            str(table.dtype) != "torch.float32":
+        raise FoError("a rope table is a contiguous float32 CUDA tensor [positions][rot_dim / 2][2]")
+    ctx = ctx or stream_context(table.device.index)
+    check(lib().fo_rope_table(ctx.handle, table.data_ptr(), table.shape[0], 2 * table.shape[1],
+                              RopeScaling(theta, ROPE_SCALINGS[scaling], factor, original_positions, beta_fast,
+                                          beta_slow, attention_factor)))
+    return table
+
+
+class Rope:
+    """A rope table and the layout of the pairs that it turns."""
+
+    def __init__(self, table, layout="interleaved"):
+        if not _on_device(table) or not table.is_contiguous() or table.dim() != 3 or table.shape[2] != 2 or \
+                str(table.dtype) != "torch.float32":
+            raise FoError("a rope table is a contiguous float32 CUDA tensor [positions][rot_dim / 2][2]")
+        self.table = table
+        self.spec = (table.data_ptr(), table.shape[0], 2 * table.shape[1], ROPE_LAYOUTS[layout])
+
+    def at(self, positions, rows: int) -> RopeSpec:
+        table, n, rot_dim, layout = self.spec
+        if positions is None:
+            return RopeSpec(table, n, None, rot_dim, layout)
+        if positions.numel() != rows:
+            raise FoError("one position for each row")
+        return RopeSpec(table, n, _device_ints(positions, "positions"), rot_dim, layout)
+
+
+def rope(x, out, rope: Rope, positions=None, inverse=False, ctx=None):
+    """fo_rope: rows x [rows][heads][head_dim] rotated into `out` (x itself is
+    allowed) at `positions` [rows] int32 (None: the row's number).  inverse:
+    the transposed rotation, which takes a gradient back."""
+    a, b = _rows(x, "x"), _rows(out, "out")
+    if x.shape != out.shape:
+        raise FoError("rope: x and out must have one shape")
+    spec = rope.at(positions, x.shape[0])
+    ctx = ctx or stream_context(x.device.index)
+    check(lib().fo_rope(ctx.handle, ctypes.byref(a), ctypes.byref(b), x.shape[0], x.shape[2], ctypes.byref(spec),
+                        1 if inverse else 0))
+    return out
+
+
+class PagedKv:
+    """The pool of a paged 8-bit cache (fo_paged_kv): codes [pages][kv heads]
+    [page size][head dim] of int8 or float8_e4m3fn, scales [pages][kv heads]
+    float32, all contiguous CUDA tensors of the caller's."""
+
+    def __init__(self, k_codes, v_codes, k_scales, v_scales):
+        torch = _torch()
+        formats = {torch.int8: PAGED_I8, torch.float8_e4m3fn: PAGED_E4M3}
+        if k_codes.dtype not in formats or v_codes.dtype != k_codes.dtype:
+            raise FoError("paged codes must be int8 or float8_e4m3fn, keys and values alike")
+        if k_codes.dim() != 4 or k_codes.shape != v_codes.shape:
+            raise FoError("paged codes must be [pages][kv heads][page size][head dim], keys and values alike")
+        for t in (k_scales, v_scales):
+            if t.dtype != torch.float32 or t.shape != k_codes.shape[:2]:
+                raise FoError("paged scales must be float32 [pages][kv heads]")
+        for t in (k_codes, v_codes, k_scales, v_scales):
+            if not t.is_cuda or not t.is_contiguous():
+                raise FoError("paged codes and scales must be contiguous CUDA tensors")
+        self.keep = (k_codes, v_codes, k_scales, v_scales)
+        n_pages, kv_heads, page_size, self.head_dim = k_codes.shape
+        self.device = k_codes.device.index
+        self.pool = PagedPool(k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
+                              n_pages, page_size, kv_heads, self.head_dim, formats[k_codes.dtype])
+
+
+class PagedBatch:
+    """The sequences of paged calls (fo_paged_batch): page_table [seqs][pages]
+    and lens [seqs] int32, lens counting the call's rows; `rows` of each
+    sequence, or at most, with row_start [seqs + 1] int32, as many as that
+    says.  The tensors are the caller's and may change between calls."""
+
+    def __init__(self, page_table, lens, rows=1, row_start=None):
+        if page_table.dim() != 2 or page_table.shape[0] != lens.numel():
+            raise FoError("page_table must be [seqs][pages], with one length for each")
+        if row_start is not None and row_start.numel() != lens.numel() + 1:
+            raise FoError("row_start must have one entry more than there are sequences")
+        self.keep = (page_table, lens, row_start)
+        n = lens.numel()
+        self.sequences = PagedSequences(_device_ints(page_table, "page_table"), _device_ints(lens, "lens"),
+                                        None if row_start is None else _device_ints(row_start, "row_start"),
+                                        page_table.shape[1], n, rows, n * rows)
+
+    def of(self, rows: int) -> PagedSequences:
+        self.sequences.total_rows = rows
+        return self.sequences
+
+
+def paged_append(kv: PagedKv, batch: PagedBatch, k, v, rope: Optional[Rope] = None, positions=None, q=None,
+                 q_out=None, ctx=None):
+    """fo_paged_append: rows k, v [rows][kv heads][head dim] into the batch's
+    pages, keys rotated on the way when `rope` is given (at `positions`, else
+    at their place in the cache), and queries q rotated into q_out."""
+    rk, rv = _rows(k, "k"), _rows(v, "v")
+    if k.shape[2] != kv.head_dim or v.shape != k.shape:
+        raise FoError("paged_append: k and v must be [rows][kv heads][head dim] of the cache")
+    rows = k.shape[0]
+    rq = ro = spec = None
+    if rope is not None:
+        spec = ctypes.byref(rope.at(positions, rows))
+    if q is not None:
+        if q_out is None or q.shape != q_out.shape or q.shape[0] != rows or q.shape[2] != kv.head_dim:
+            raise FoError("paged_append: q and q_out must be [rows][heads][head dim]")
+        rq, ro = ctypes.byref(_rows(q, "q")), ctypes.byref(_rows(q_out, "q_out"))
+    ctx = ctx or stream_context(kv.device)
+    check(lib().fo_paged_append(ctx.handle, ctypes.byref(kv.pool), ctypes.byref(batch.of(rows)), ctypes.byref(rk),
+                                ctypes.byref(rv), rq, ro, spec))
+
+
+def paged_attention(kv: PagedKv, batch: PagedBatch, q, out, sinks=None, scale=None, window=0, lse=None, ctx=None):
+    """fo_paged_attention: q [rows][heads][head dim] over the batch's cached
+    positions into `out`; scale None: 1 / sqrt(head dim)."""
+    rq, ro = _rows(q, "q"), _rows(out, "out")
+    if q.shape[2] != kv.head_dim or out.shape != q.shape:
+        raise FoError("paged_attention: q and out must be [rows][heads][head dim] of the cache's width")
+    for t, n, name in ((sinks, q.shape[1], "sinks"), (lse, q.shape[0] * q.shape[1], "lse")):
+        if t is not None and (not t.is_cuda or not t.is_contiguous() or t.numel() != n or t.element_size() != 4):
+            raise FoError(f"paged_attention: {name} must be a contiguous float32 CUDA tensor of {n}")
+    ctx = ctx or stream_context(kv.device)
+    check(lib().fo_paged_attention(ctx.handle, ctypes.byref(kv.pool), ctypes.byref(batch.of(q.shape[0])),
+                                   ctypes.byref(rq), None if sinks is None else sinks.data_ptr(),
+                                   kv.head_dim ** -0.5 if scale is None else scale, window, ctypes.byref(ro),
+                                   None if lse is None else lse.data_ptr()))
+    return out
 
 
 class _DeviceArray:

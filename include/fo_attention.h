@@ -46,6 +46,9 @@
  *   fo_decode_static_scratch_status  and its device error report
  *   fo_i8_*                        BASELINE config 4's INT8 KV format
  *   fo_selftest_bounded_wait       the kernels' bounded-wait failure path
+ *   fo_rope_table, fo_rope         rotary positions from a table, by position
+ *   fo_paged_append, fo_paged_attention  an 8-bit KV cache in pages shared by many
+ *                                  sequences: append with rotation, verify-row attention
  *
  * Conventions (mirroring the reference's, src/kernels/attention/mod.rs:159-195
  * and src/quant/kv.rs:248-295):
@@ -441,6 +444,133 @@ int fo_draft_kv_records(const fo_draft_kv *kv, const int8_t **key_codes, const f
  * [16][64].  bases <= fo_draft_kv_len; at least one row attended. */
 int fo_draft_attend(fo_draft_kv *kv, const float *q, int64_t bases, int64_t window, const float *chain_keys,
                     const float *chain_values, int64_t chain, float *output, int mem);
+
+/* ------------------------------------------------------------------------
+ * Rotary positions and a paged 8-bit KV cache (no counterpart in the
+ * reference, whose caches are one contiguous allocation per page of text).
+ *
+ * These calls take DEVICE pointers only, launch on the context's stream and
+ * return; none synchronizes, and after its first call on a context none
+ * allocates, so they can be captured in CUDA graphs.  What the device alone
+ * can see (a page number outside the pool, a rotary position outside the
+ * table, a value that is not finite) goes to the context's error word, which
+ * fo_ctx_synchronize reports and clears; no such input reads or writes out
+ * of bounds. */
+
+#define FO_DT_F32 0
+#define FO_DT_BF16 1
+
+/* Rows of heads in device memory: element (row, head, d) at
+ * data[row * row_stride + head * head_stride + d] (strides in elements, the
+ * head's own values adjacent).  Rows may be a part of wider ones (a
+ * projection's) and heads may come before rows. */
+typedef struct {
+    void *data;
+    int64_t row_stride;
+    int64_t head_stride;
+    int32_t heads;
+    int32_t dtype; /* FO_DT_* */
+} fo_rows;
+
+/* Which two elements of a head form rotated pair i of rot_dim / 2. */
+#define FO_ROPE_INTERLEAVED 0 /* 2 i and 2 i + 1 */
+#define FO_ROPE_HALF 1        /* i and i + rot_dim / 2 */
+
+/* How a table's positions are scaled for contexts longer than the model's. */
+#define FO_ROPE_PLAIN 0
+#define FO_ROPE_LINEAR 1 /* every frequency divided by factor */
+#define FO_ROPE_NTK 2    /* theta * factor^(rot_dim / (rot_dim - 2)) */
+#define FO_ROPE_YARN 3   /* by parts: see fo_rope_table */
+
+typedef struct {
+    double theta;
+    int32_t scaling;            /* FO_ROPE_PLAIN .. FO_ROPE_YARN */
+    double factor;              /* > 0; 1 leaves every scaling without effect */
+    double original_positions;  /* YARN: positions the model was trained on */
+    double beta_fast, beta_slow; /* YARN: turns over those positions (32 and 1) */
+    double attention_factor;    /* YARN: the table's magnitude; 0 is 0.1 ln(factor) + 1 */
+} fo_rope_scaling;
+
+typedef struct {
+    const float *table;           /* [positions][rot_dim / 2]{cos, sin} */
+    int64_t positions;
+    const int32_t *row_positions; /* position of each row; NULL: the row's number (fo_rope) or its place in the cache */
+    int32_t rot_dim;              /* even, at most the head's width; the rest of a head is not rotated */
+    int32_t layout;               /* FO_ROPE_INTERLEAVED | FO_ROPE_HALF */
+} fo_rope_spec;
+
+/* Fills table [positions][rot_dim / 2]{cos, sin}: the cosine and sine, each
+ * rounded once from FP64, of position * f_i with f_i = theta^(-2 i / rot_dim)
+ * scaled as asked.  YARN (Peng et al., 2023) keeps the pairs that turn more
+ * than beta_fast times over original_positions, divides by factor the
+ * frequencies of those that turn less than beta_slow times, ramps linearly
+ * over the pairs between, and multiplies the table by attention_factor. */
+int fo_rope_table(fo_ctx *ctx, float *table, int64_t positions, int32_t rot_dim, fo_rope_scaling scaling);
+
+/* Rotates `rows` rows of x into out (the same memory, laid out alike, is
+ * allowed; any other overlap is not): pair (a, b) at a row's position becomes
+ * (a cos - b sin, b cos + a sin), in FP32 with each product and sum rounded,
+ * then rounded once to out's type.  With transpose set the sine's sign is
+ * turned: the gradient with respect to x of a gradient given for the rotated
+ * rows.  head_dim is at most 256, x and out of one type and as many heads.
+ * A row whose position lies outside the table becomes NaN where it would be
+ * rotated, and the error word says so. */
+int fo_rope(fo_ctx *ctx, const fo_rows *x, const fo_rows *out, int64_t rows, int32_t head_dim,
+            const fo_rope_spec *rope, int32_t transpose);
+
+#define FO_PAGED_I8 0   /* codes -127..127 */
+#define FO_PAGED_E4M3 1 /* FP8 e4m3, finite codes only */
+
+/* The pool of a paged cache: n_pages pages of page_size (16, 32, 64 or 128)
+ * positions, every head's keys of a page adjacent, one FP32 scale per (page,
+ * KV head) of keys and of values; a key is code * scale.  Caller-owned, codes
+ * 16-byte aligned.  head_dim is 64 or 128. */
+typedef struct {
+    void *k_codes, *v_codes;   /* [n_pages][n_kv_heads][page_size][head_dim] */
+    float *k_scales, *v_scales; /* [n_pages][n_kv_heads] */
+    int64_t n_pages;
+    int32_t page_size, n_kv_heads, head_dim, format;
+} fo_paged_kv;
+
+/* Sequences of a call and its rows.  Sequence b holds lens[b] positions, THE
+ * CALL'S ROWS INCLUDED: its n rows are the last n positions, lens[b] - n ..
+ * lens[b] - 1.  row_start NULL: every sequence has max_rows rows, sequence
+ * b's from row b * max_rows; otherwise sequence b's rows are row_start[b] ..
+ * row_start[b + 1] - 1, at most max_rows of them and none beyond total_rows.
+ * A row whose position is negative (a padded slot of a captured graph has
+ * lens 0) stores nothing and attends to nothing.  Position p of sequence b
+ * is in page page_table[b * table_stride + p / page_size], p % page_size. */
+typedef struct {
+    const int32_t *page_table; /* [n_seqs][table_stride] */
+    const int32_t *lens;       /* [n_seqs] */
+    const int32_t *row_start;  /* [n_seqs + 1] or NULL */
+    int64_t table_stride, n_seqs, max_rows, total_rows;
+} fo_paged_batch;
+
+/* Appends the rows of k and v [total_rows][n_kv_heads][head_dim] to the
+ * sequences' pages, and rotates rows: k on its way into the cache and q into
+ * q_out (q and q_out NULL: no queries; rope NULL: nothing is rotated, and q
+ * must be NULL).  The rows that fall into one page share the page's scale: a
+ * page whose first position is among them takes max |x| / 127 (int8) or
+ * / 448 (e4m3) of its new rows; a page that holds earlier positions keeps
+ * its scale unless the new rows need a larger one, and then its earlier codes
+ * are rounded again against that.  code = x / scale, rounded to nearest even.
+ * Pages that sequences share must not be appended to.  A value that is not
+ * finite takes no part in the scale; infinities are stored as the largest
+ * code, NaN as zero, and the error word says so. */
+int fo_paged_append(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch *batch, const fo_rows *k,
+                    const fo_rows *v, const fo_rows *q, const fo_rows *q_out, const fo_rope_spec *rope);
+
+/* Attention of the batch's query rows over their sequences' cached positions:
+ * the row at position p sees positions 0 .. p, or the newest `window` of them
+ * (0: all).  q and out have one type and n_heads heads, a multiple of
+ * n_kv_heads (query head h reads KV head h / (n_heads / n_kv_heads)).  With
+ * s_j = scale * q . k_j: out = sum_j exp(s_j) v_j / (sum_j exp(s_j) +
+ * exp(sinks[head])), sinks NULL: without that term; lse (NULL: not wanted)
+ * [total_rows][n_heads] = ln sum_j exp(s_j).  A row that sees nothing gives 0
+ * and -infinity.  max_rows is at most 64. */
+int fo_paged_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch *batch, const fo_rows *q,
+                       const float *sinks, float scale, int64_t window, const fo_rows *out, float *lse);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,580 @@
+"""The rotary operators and the paged 8-bit KV cache on the GPU
+(fo_rope_table, fo_rope, fo_paged_append, fo_paged_attention) against plain
+float64 implementations (tests/paged_reference.py).
+
+Bounds.  A rotation has two products and a sum, each rounded: 3 * 2^-24 of
+|a c| + |b s|.  BF16 output lies between the roundings to BF16 of the exact
+result less and plus the FP32 bound (rounding is monotonic).  An append's codes and scales are equal to the documented float32 steps.  An
+attention's score s = scale * sum q k is off by at most d = 2^-17 of the score's
+sum of magnitudes (FP32 sums of at most 128 products, queries held to 22 bits),
+which moves a probability by a factor e^d and the output by at most 4 d max|v|;
+FP32 probabilities, sums and divisions add 2^-18 max|v|; with BF16 rows the
+probabilities carry 11 bits, 2^-11 max|v|."""
+
+import math
+
+import numpy as np
+import pytest
+
+import fo_cuda as F
+import paged_reference as R
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+DTYPES = {"f32": torch.float32, "bf16": torch.bfloat16}
+
+
+def dev(x):
+    return torch.from_numpy(np.ascontiguousarray(x)).cuda()
+
+
+def rows_of(rng, rows, heads, dim, dtype, order="rows", pad=0):
+    """Random rows as (CUDA tensor in some order of memory, its float64 values)."""
+    x = torch.from_numpy(rng.standard_normal((rows, heads + pad, dim)).astype(np.float32)).to(DTYPES[dtype])
+    if order == "heads":  # heads before rows
+        t = x.transpose(0, 1).contiguous().cuda().transpose(0, 1)[:, :heads]
+    else:
+        t = x.cuda()[:, :heads]
+    return t, x[:, :heads].double().numpy()
+
+
+def plain_table(positions, rot, theta=10000.0):
+    f = theta ** (-2.0 * np.arange(rot // 2) / rot)
+    a = np.arange(positions)[:, None] * f
+    return np.stack((np.cos(a), np.sin(a)), -1).astype(np.float32)
+
+
+def within(got, exact, bound, dtype):
+    """Whether every value of `got` is a value within `bound` of the exact one, rounded to the type."""
+    low, high = (torch.from_numpy(np.asarray(x)).to(torch.float64) for x in (exact - bound, exact + bound))
+    if dtype == "bf16":
+        low, high = low.to(torch.bfloat16).double(), high.to(torch.bfloat16).double()
+    got = torch.from_numpy(got)
+    return bool(((got >= low) & (got <= high)).all())
+
+
+# ----------------------------------------------------------------- the table
+@pytest.mark.parametrize("scaling", ["none", "linear", "ntk", "yarn"])
+@pytest.mark.parametrize("rot", [2, 24, 64, 128])
+def test_rope_table(scaling, rot):
+    n, theta, factor, original = 70001, 10000.0, 4.0, 4096
+    i = np.arange(rot // 2)
+    f, m = theta ** (-2.0 * i / rot), 1.0
+    if scaling == "linear":
+        f = f / factor
+    elif scaling == "ntk" and rot > 2:
+        f = (theta * factor ** (rot / (rot - 2))) ** (-2.0 * i / rot)
+    elif scaling == "yarn":
+        at = lambda turns: rot * math.log(original / (turns * 2 * math.pi)) / (2 * math.log(theta))  # noqa: E731
+        low, high = max(math.floor(at(32)), 0), min(math.ceil(at(1)), rot - 1)
+        ramp = np.clip((i - low) / max(high - low, 0.001), 0, 1)
+        f, m = f / factor * ramp + f * (1 - ramp), 0.1 * math.log(factor) + 1
+    a = np.arange(n)[:, None] * f
+    expected = np.stack((np.cos(a), np.sin(a)), -1) * m
+    table = torch.empty(n, rot // 2, 2, device="cuda")
+    F.rope_table(table, theta, scaling, factor, original)
+    got = table.cpu().numpy().astype(np.float64)
+    # Half a unit of FP32, and FP64 angles off by some units of 70,000.
+    assert np.abs(got - expected).max() <= 2.0 ** -24 * m + 1e-10
+
+
+# -------------------------------------------------------------------- rotation
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("rows,heads,dim,rot,order,pad,shift", [
+    (1, 1, 64, 64, "rows", 0, 0),
+    (7, 24, 64, 32, "rows", 8, 0),     # the temporal half, a part of wider rows
+    (33, 5, 128, 128, "heads", 0, 0),  # heads before rows
+    (19, 3, 128, 24, "rows", 1, 0),    # pairs that no group of eight divides
+    (11, 2, 80, 80, "rows", 0, 0),
+    (6, 3, 66, 34, "rows", 0, 0),      # a width that no group of eight divides
+    (5, 9, 64, 64, "rows", 0, 1),      # off a 16-byte boundary
+    (300, 40, 128, 64, "rows", 0, 0),
+])
+def test_rope(layout, dtype, rows, heads, dim, rot, order, pad, shift):
+    rng = np.random.default_rng(rows * 1000 + dim + rot)
+    x, xv = rows_of(rng, rows, heads, dim, dtype, order, pad)
+    if shift:
+        flat = torch.empty(x.numel() + shift, dtype=x.dtype, device="cuda")
+        flat[shift:].view(x.shape).copy_(x)
+        x = flat[shift:].view(x.shape)
+    table = plain_table(500, rot)
+    positions = rng.integers(0, 500, rows).astype(np.int32)
+    rope = F.Rope(dev(table), layout)
+    for inverse in (False, True):
+        for where in (dev(positions), None):
+            at = positions if where is not None else np.arange(rows)
+            expected = R.rotate(xv, table, at, layout, inverse)
+            out = torch.full((rows, heads, dim), 7.0, dtype=x.dtype, device="cuda")
+            F.rope(x, out, rope, positions=where, inverse=inverse)
+            got = out.double().cpu().numpy()
+            bound = 3 * 2.0 ** -24 * R.rotate(np.abs(xv), np.abs(table) * [1, -1], at, layout).max()
+            assert within(got, expected, bound, dtype)
+            assert np.array_equal(got[..., rot:], xv[..., rot:])
+            # In place the same bits.
+            own = x.clone(memory_format=torch.preserve_format)
+            F.rope(own, own, rope, positions=where, inverse=inverse)
+            assert torch.equal(own, out)
+
+
+def test_rope_transpose_is_the_gradient():
+    """sum w * rope(x) changes by <transposed rotation of w, dx>: against central differences, which a linear map
+    meets to rounding (FP32 values of some 10: differences over a step of 1/4 are good to 1e-4)."""
+    rng = np.random.default_rng(5)
+    x, w = rng.standard_normal((2, 3, 4, 64)).astype(np.float32)
+    table = plain_table(64, 32) * np.float32(1.25)
+    positions = dev(np.array([3, 60, 21], np.int32))
+    for layout in ("interleaved", "half"):
+        rope = F.Rope(dev(table), layout)
+        g = F.rope(dev(w), torch.empty(3, 4, 64, device="cuda"), rope, positions, inverse=True).cpu().numpy()
+
+        def value(z):
+            y = F.rope(dev(z), torch.empty(3, 4, 64, device="cuda"), rope, positions)
+            return float((y.double().cpu() * torch.from_numpy(w).double()).sum())
+
+        for i in [(0, 0, 0), (0, 1, 17), (1, 3, 31), (2, 2, 16), (2, 0, 40), (1, 1, 1)]:
+            up, down = x.copy(), x.copy()
+            up[i] += 0.25
+            down[i] -= 0.25
+            assert abs((value(up) - value(down)) / 0.5 - g[i]) < 1e-4
+
+
+def test_rope_position_outside_the_table():
+    ctx = F.Context(0)
+    x = torch.ones(3, 2, 64, device="cuda")
+    out = torch.zeros_like(x)
+    F.rope(x, out, F.Rope(dev(plain_table(10, 32))), dev(np.array([9, 10, -1], np.int32)), ctx=ctx)
+    with pytest.raises(F.FoError, match="outside its table"):
+        ctx.synchronize()
+    ctx.synchronize()  # reported once
+    got = out.cpu().numpy()
+    assert np.isfinite(got[0]).all() and np.isnan(got[1:, :, :32]).all() and (got[1:, :, 32:] == 1).all()
+    ctx.close()
+
+
+# ----------------------------------------------------------------- paged cache
+class Cache:
+    """A pool with random contents, its pages handed out in any order; what no sequence holds is garbage (NaN codes
+    and scales)."""
+
+    def __init__(self, rng, fmt, dim, page, kv_heads, lens, spare=2, extra_positions=0):
+        self.fmt, self.lens, self.page = fmt, list(lens), page
+        per = [-(-(max(n, 0) + extra_positions) // page) for n in lens]
+        width = max(max(per), 1)
+        order = rng.permutation(sum(per) + spare)
+        self.table = np.full((len(lens), width), -7, np.int32)  # what is not read may be anything
+        at = 0
+        for b, n in enumerate(per):
+            self.table[b, :n] = order[at:at + n]
+            at += n
+        shape = (sum(per) + spare, kv_heads, page, dim)
+        garbage = 0x7F if fmt == "e4m3" else 0x55
+        self.codes = [np.full(shape, garbage, np.uint8) for _ in range(2)]
+        self.scales = [np.full(shape[:2], np.nan, np.float32) for _ in range(2)]
+        for b, n in enumerate(lens):
+            for p in range(0, n, page):
+                pg, m = self.table[b, p // page], min(page, n - p)
+                for i in range(2):
+                    x = rng.standard_normal((kv_heads, m, dim)).astype(np.float32)
+                    scale = np.abs(x).max((1, 2)) / R.TOP[fmt] * rng.uniform(0.5, 2.0, kv_heads).astype(np.float32)
+                    scale = np.maximum(scale, np.abs(x).max((1, 2)) / R.TOP[fmt]).astype(np.float32)
+                    self.codes[i][pg, :, :m] = R.encode(np.clip(x / scale[:, None, None], -R.TOP[fmt], R.TOP[fmt]), fmt)
+                    self.scales[i][pg] = scale
+
+    def on_device(self):
+        kind = torch.int8 if self.fmt == "i8" else torch.float8_e4m3fn
+        self.dev = [dev(c).view(kind) for c in self.codes] + [dev(s) for s in self.scales]
+        return F.PagedKv(*self.dev)
+
+    def batch(self, rows, ragged):
+        start = None
+        if ragged:
+            start = dev(np.concatenate(([0], np.cumsum(rows))).astype(np.int32))
+        return F.PagedBatch(dev(self.table), dev(np.array(self.lens, np.int32)), rows=max(rows), row_start=start)
+
+    def values(self, i, b):
+        """float64 [kv heads][positions][dim] of sequence b's keys (0) or values (1)."""
+        n = self.lens[b]
+        pages = self.table[b, :-(-n // self.page)]
+        x = R.decode(self.codes[i][pages], self.fmt) * self.scales[i][pages].astype(np.float64)[..., None, None]
+        return x.transpose(1, 0, 2, 3).reshape(x.shape[1], -1, x.shape[3])[:, :n]
+
+    def check(self, codes_equal_where=None):
+        for i in range(2):
+            got = self.dev[i].view(torch.uint8).cpu().numpy()
+            assert np.array_equal(got, self.codes[i])
+            assert np.array_equal(self.dev[2 + i].cpu().numpy().view(np.uint32), self.scales[i].view(np.uint32))
+
+
+def attention_case(seed, fmt, dim, page, kv_heads, group, dtype, lens, rows, window=0, sinks=True, ragged=False,
+                   scale=None, q_scale=1.0, order="rows", pad=0, ctx=None):
+    rng = np.random.default_rng(seed)
+    cache = Cache(rng, fmt, dim, page, kv_heads, lens)
+    kv, batch = cache.on_device(), cache.batch(rows, ragged)
+    heads, total = kv_heads * group, sum(rows)
+    q, _ = rows_of(rng, total, heads, dim, dtype, order, pad)
+    q = (q * q_scale).to(q.dtype) if q_scale != 1.0 else q
+    qv = q.double().cpu().numpy()
+    sk = rng.standard_normal(heads).astype(np.float32) if sinks else None
+    out = torch.full((total, heads, dim), 9.0, dtype=q.dtype, device="cuda")
+    lse = torch.full((total, heads), 9.0, device="cuda")
+    F.paged_attention(kv, batch, q, out, sinks=None if sk is None else dev(sk), scale=scale, window=window, lse=lse,
+                      ctx=ctx)
+    got, got_lse = out.double().cpu().numpy(), lse.double().cpu().numpy()
+    at = 0
+    for b, n in enumerate(rows):
+        k, v = cache.values(0, b), cache.values(1, b)
+        top = np.abs(v).max(initial=0.0)
+        for r in range(n):
+            o, z, size = R.attend(qv[at], k, v, lens[b] - n + r, window, sk, dim ** -0.5 if scale is None else scale)
+            d = 2.0 ** -17 * size
+            bound = 4 * d * top + 2.0 ** -18 * top
+            if dtype == "bf16":
+                bound = bound + 2.0 ** -11 * top
+            assert within(got[at], o, bound, dtype), (b, r, np.abs(got[at] - o).max(), bound)
+            if lens[b] - n + r < 0:
+                assert np.isneginf(got_lse[at]).all() and (got[at] == 0).all()
+            else:
+                assert (np.abs(got_lse[at] - z) <= d + 2.0 ** -20 * (1 + np.abs(z))).all()
+            at += 1
+    return out, lse
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+def test_attention_lengths(fmt, dtype, dim, page):
+    """One row each against lengths around every edge: none, one, a page's and a tile's end."""
+    lens = [0, 1, 2, 15, 16, 17, 63, 64, 65, 127, 128, 129, 200, 777]
+    attention_case(1, fmt, dim, page, 2, 2, dtype, lens, [1] * len(lens))
+
+
+@pytest.mark.parametrize("group", [1, 2, 3, 5, 8, 16])
+@pytest.mark.parametrize("rows", [1, 2, 5, 8])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attention_groups_and_rows(group, rows, dtype):
+    lens = [300, rows - 1, rows, 70]  # the second has a row that sees nothing
+    attention_case(2, "i8", 64, 32, 3, group, dtype, lens, [rows] * 4)
+    attention_case(3, "e4m3", 128, 64, 1, group, dtype, lens, [rows] * 4, sinks=False)
+
+
+@pytest.mark.parametrize("rows", [17, 64])
+def test_attention_many_rows(rows):
+    attention_case(4, "i8", 64, 16, 2, 4, "bf16", [400, 64], [rows] * 2)
+    attention_case(4, "e4m3", 128, 16, 1, 4, "f32", [90], [rows])
+
+
+@pytest.mark.parametrize("window", [1, 2, 63, 64, 65, 200, 5000])
+def test_attention_window(window):
+    lens = [1, 64, 129, 700]
+    attention_case(5, "i8", 64, 16, 2, 4, "bf16", lens, [1] * 4, window=window)
+    attention_case(6, "e4m3", 128, 32, 2, 2, "f32", lens, [4] * 4, window=window)
+
+
+def test_attention_ragged_rows():
+    attention_case(7, "i8", 128, 32, 2, 4, "bf16", [500, 90, 3, 1200, 7], [1, 5, 0, 3, 7], ragged=True)
+    attention_case(7, "e4m3", 64, 16, 4, 2, "f32", [500, 90, 0, 2], [2, 0, 1, 8], ragged=True, window=100)
+
+
+def test_attention_orders_of_memory():
+    for order in ("rows", "heads"):
+        attention_case(8, "i8", 64, 64, 2, 3, "bf16", [333, 40], [3, 3], order=order, pad=5)
+        attention_case(8, "e4m3", 128, 64, 2, 3, "f32", [333, 40], [3, 3], order=order, pad=5)
+
+
+def test_attention_one_long_sequence_and_many_short_ones():
+    attention_case(9, "i8", 64, 64, 8, 2, "f32", [16384], [5])
+    attention_case(9, "e4m3", 128, 128, 2, 4, "bf16", [9000, 1, 30, 5000], [1] * 4)
+    lens = [int(n) for n in np.random.default_rng(0).integers(0, 150, 300)]
+    attention_case(10, "i8", 64, 16, 2, 2, "bf16", lens, [1] * 300)
+
+
+def test_attention_scales_of_queries():
+    """Queries far from 1 (their magnitude must not matter to how they are held), and a peaked softmax."""
+    attention_case(11, "i8", 64, 32, 2, 2, "f32", [500], [2], q_scale=1e-6, scale=1e5)
+    attention_case(11, "i8", 128, 32, 2, 2, "bf16", [500], [2], q_scale=2.0 ** 20, scale=2.0 ** -21)
+    attention_case(12, "e4m3", 64, 32, 2, 2, "f32", [500], [2], scale=3.0)
+    attention_case(13, "i8", 64, 32, 2, 2, "f32", [70], [1], q_scale=0.0)
+    attention_case(13, "i8", 64, 32, 2, 2, "bf16", [70], [1], scale=-0.3)
+
+
+def test_attention_pages_of_very_different_scales():
+    """A page whose values are 2^40 times another's: what it adds to small outputs is exact to its own size."""
+    rng = np.random.default_rng(14)
+    cache = Cache(rng, "i8", 64, 16, 1, [64])
+    cache.scales[1][cache.table[0, 1]] *= 2.0 ** 40
+    cache.scales[1][cache.table[0, 2]] *= 2.0 ** -40
+    cache.scales[0][cache.table[0, 1]] = 0.0  # a page of zero keys
+    kv, batch = cache.on_device(), cache.batch([1], False)
+    q, qv = rows_of(rng, 1, 2, 64, "f32")
+    out = torch.empty(1, 2, 64, device="cuda")
+    F.paged_attention(kv, batch, q, out)
+    k, v = cache.values(0, 0), cache.values(1, 0)
+    o, _, _ = R.attend(qv[0], k, v, 63, 0, None, 0.125)
+    got = out.double().cpu().numpy()[0]
+    assert (np.abs(got - o) <= 2.0 ** -14 * np.abs(v).max()).all()
+    # Without that page in sight, the others' accuracy is their own.
+    F.paged_attention(kv, batch, q, out, window=32)
+    o, _, _ = R.attend(qv[0], k, v, 63, 32, None, 0.125)
+    assert (np.abs(out.double().cpu().numpy()[0] - o) <= 2.0 ** -14 * np.abs(v[:, 32:]).max()).all()
+
+
+def test_attention_results_do_not_change_between_runs():
+    a = attention_case(15, "i8", 64, 64, 8, 2, "bf16", [5000, 300, 8000], [1] * 3)
+    b = attention_case(15, "i8", 64, 64, 8, 2, "bf16", [5000, 300, 8000], [1] * 3)
+    assert torch.equal(a[0], b[0]) and torch.equal(a[1], b[1])
+
+
+def test_attention_reports_bad_tables_and_lengths():
+    rng = np.random.default_rng(16)
+    cache = Cache(rng, "i8", 64, 16, 1, [40, 40])
+    q, _ = rows_of(rng, 2, 1, 64, "f32")
+    out = torch.empty(2, 1, 64, device="cuda")
+    for change in ("page", "length"):
+        ctx = F.Context(0)
+        if change == "page":
+            cache.table[1, 1] = 1 << 30
+        else:
+            cache.table[1, 1] = 0
+            cache.lens[1] = 49  # a page more than its table has
+        F.paged_attention(cache.on_device(), cache.batch([1, 1], False), q, out, ctx=ctx)
+        with pytest.raises(F.FoError, match="page table"):
+            ctx.synchronize()
+        ctx.synchronize()
+        o, _, _ = R.attend(q.double().cpu().numpy()[0], cache.values(0, 0), cache.values(1, 0), 39, 0, None, 0.125)
+        assert np.abs(out.double().cpu().numpy()[0] - o).max() < 1e-4  # the other sequence is whole
+        ctx.close()
+    ctx = F.Context(0)
+    cache.lens[1] = 40
+    batch = F.PagedBatch(dev(cache.table), dev(np.array(cache.lens, np.int32)), rows=2,
+                         row_start=dev(np.array([0, 1, 5], np.int32)))
+    F.paged_attention(cache.on_device(), batch, q, out, ctx=ctx)
+    with pytest.raises(F.FoError, match="row ranges"):
+        ctx.synchronize()
+    ctx.close()
+
+
+# --------------------------------------------------------------------- append
+def append_case(seed, fmt, dim, page, kv_heads, dtype, held, rows, layout="interleaved", rot=None, heads=0,
+                ragged=False, order="rows", pad=0, positions=False, size=1.0):
+    """Rows appended to sequences that hold `held` positions each."""
+    rng = np.random.default_rng(seed)
+    room = max(rows)
+    cache = Cache(rng, fmt, dim, page, kv_heads, held, extra_positions=room)
+    cache.lens = [n + m for n, m in zip(held, rows)]
+    total = sum(rows)
+    k, kx = rows_of(rng, total, kv_heads, dim, dtype, order, pad)
+    v, vx = rows_of(rng, total, kv_heads, dim, dtype, order, pad)
+    k, v = (k * size).to(k.dtype), (v * size).to(v.dtype)
+    kx, vx = k.double().cpu().numpy(), v.double().cpu().numpy()
+    kv, batch = cache.on_device(), cache.batch(rows, ragged)
+    rope = where = q = q_out = None
+    at = np.array([n + r for n, m in zip(held, rows) for r in range(m)])
+    if rot:
+        table = plain_table(4000, rot)
+        rope = F.Rope(dev(table), layout)
+        if positions:
+            at = rng.integers(0, 4000, total)
+            where = dev(at.astype(np.int32))
+        if heads:
+            q, qx = rows_of(rng, total, heads, dim, dtype, order, pad)
+            q_out = torch.full((total, heads, dim), 5.0, dtype=q.dtype, device="cuda")
+        kx = R.rotate(kx, table, at, layout, dtype=np.float32)
+    F.paged_append(kv, batch, k, v, rope=rope, positions=where, q=q, q_out=q_out)
+    R.append(cache.codes[0], cache.scales[0], kx.astype(np.float32), rows, cache.lens, cache.table, fmt)
+    R.append(cache.codes[1], cache.scales[1], vx.astype(np.float32), rows, cache.lens, cache.table, fmt)
+    cache.check()
+    if heads:
+        expected = torch.from_numpy(R.rotate(qx, table, at, layout, dtype=np.float32)).to(q.dtype)
+        assert torch.equal(q_out.cpu(), expected)
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+def test_append_steps(fmt, dtype, dim, page):
+    """Single rows and some at every place of a page, with scales that grow and that stay."""
+    held = [0, 1, page - 1, page, page + 1, 3 * page - 2]
+    for rows in (1, 3, 8):
+        append_case(20, fmt, dim, page, 2, dtype, held, [rows] * 6, rot=dim, heads=4)
+    append_case(21, fmt, dim, page, 2, dtype, held, [1] * 6, size=9.0)
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("page", [16, 128])
+def test_append_prompts(fmt, dtype, dim, page):
+    append_case(22, fmt, dim, page, 3, dtype, [0, 5, page], [300] * 3, rot=dim // 2, layout="half", heads=6)
+    append_case(23, fmt, dim, page, 1, dtype, [0, 7, 90, 0], [211, 1, 50, 0], rot=dim, heads=2, ragged=True, size=30.0)
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "half"])
+@pytest.mark.parametrize("rot", [2, 24, 32, 64])
+def test_append_rotations(layout, rot):
+    for rows in (2, 40):
+        append_case(24, "i8", 64, 32, 2, "f32", [10, 31], [rows] * 2, layout=layout, rot=rot, heads=3)
+        append_case(25, "e4m3", 64, 32, 2, "bf16", [10, 31], [rows] * 2, layout=layout, rot=rot, heads=3,
+                    positions=True, order="heads", pad=1)
+
+
+def test_append_ragged_and_orders():
+    append_case(26, "i8", 64, 16, 2, "bf16", [0, 9, 100, 3], [8, 0, 1, 5], ragged=True, rot=64, heads=2, pad=3)
+    append_case(27, "e4m3", 128, 64, 2, "f32", [0, 9, 100, 3, 64], [500, 1, 2, 0, 129], ragged=True, rot=128, heads=2,
+                order="heads")
+
+
+def test_append_again_after_a_rejected_draft():
+    """Lengths taken back and appended to again: the page keeps its (larger) scale, a page begun anew does not."""
+    rng = np.random.default_rng(28)
+    cache = Cache(rng, "i8", 64, 16, 1, [10], extra_positions=40)
+    kv = cache.on_device()
+    for n, m, size in [(20, 10, 50.0), (14, 4, 1.0), (17, 3, 1.0), (16, 1, 0.1), (18, 2, 0.01)]:
+        cache.lens = [n]
+        k, kx = rows_of(rng, m, 1, 64, "f32")
+        k, kx = k * size, (k * size).cpu().numpy()
+        F.paged_append(kv, cache.batch([m], False), k, k)
+        R.append(cache.codes[0], cache.scales[0], kx, [m], cache.lens, cache.table, "i8")
+        R.append(cache.codes[1], cache.scales[1], kx, [m], cache.lens, cache.table, "i8")
+        cache.check()
+
+
+def test_append_padded_slots_and_zeros():
+    """Padded slots (length 0) store nothing; blocks of zeros have scale 0 and grow from it."""
+    rng = np.random.default_rng(29)
+    cache = Cache(rng, "e4m3", 64, 16, 1, [0, 3, 2], extra_positions=20)
+    kv = cache.on_device()
+    table = plain_table(50, 64)
+    k = torch.zeros(3, 1, 64, device="cuda")
+    k[2] = 4.0
+    q, _ = rows_of(rng, 3, 2, 64, "f32")
+    q_out = torch.empty_like(q)
+    cache.lens = [0, 1, 3]
+    ctx = F.Context(0)
+    F.paged_append(kv, cache.batch([1] * 3, False), k, k, rope=F.Rope(dev(table)), q=q, q_out=q_out, ctx=ctx)
+    ctx.synchronize()
+    kx = R.rotate(k.cpu().numpy(), table, np.array([0, 0, 2]), "interleaved", dtype=np.float32)
+    R.append(cache.codes[0], cache.scales[0], kx, [1] * 3, cache.lens, cache.table, "e4m3")
+    R.append(cache.codes[1], cache.scales[1], k.cpu().numpy(), [1] * 3, cache.lens, cache.table, "e4m3")
+    cache.check()
+    assert cache.scales[0][cache.table[1, 0], 0] == 0
+    assert torch.equal(q_out[0], q[0])
+    ctx.close()
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("rows", [2, 40])
+def test_append_values_that_are_not_finite(fmt, rows):
+    rng = np.random.default_rng(30)
+    cache = Cache(rng, fmt, 64, 32, 2, [5], extra_positions=rows)
+    cache.lens = [5 + rows]
+    kv = cache.on_device()
+    k, kx = rows_of(rng, rows, 2, 64, "f32")
+    k[0, 0, 3], k[1, 1, 9], k[1, 0, 7] = math.nan, math.inf, -math.inf
+    ctx = F.Context(0)
+    F.paged_append(kv, cache.batch([rows], False), k, k, ctx=ctx)
+    with pytest.raises(F.NonFiniteError, match="not finite"):
+        ctx.synchronize()
+    ctx.synchronize()
+    for i in range(2):
+        R.append(cache.codes[i], cache.scales[i], k.cpu().numpy(), [rows], cache.lens, cache.table, fmt)
+    cache.check()
+    ctx.close()
+
+
+def test_append_reports_bad_pages():
+    rng = np.random.default_rng(31)
+    cache = Cache(rng, "i8", 64, 16, 1, [3, 3], extra_positions=4)
+    kv = cache.on_device()
+    cache.lens = [4, 4]
+    good = cache.table.copy()
+    cache.table[1, 0] = -1
+    ctx = F.Context(0)
+    k, kx = rows_of(rng, 2, 1, 64, "f32")
+    F.paged_append(kv, cache.batch([1, 1], False), k, k, ctx=ctx)
+    with pytest.raises(F.FoError, match="page table"):
+        ctx.synchronize()
+    for i in range(2):
+        R.append(cache.codes[i], cache.scales[i], kx.astype(np.float32)[:1], [1], [4], good[:1], "i8")
+    cache.check()  # the other sequence's row is in, nothing else changed
+    ctx.close()
+
+
+# -------------------------------------------------------------------- together
+def test_steps_on_a_side_stream_and_in_a_graph():
+    """A decode loop as a program runs it: append with rotation and attend, captured once, replayed with the lengths
+    moved on, on a stream of its own; each step against the plain forms of the cache as it then is."""
+    rng = np.random.default_rng(32)
+    dim, page, kv_heads, heads = 64, 16, 2, 4
+    cache = Cache(rng, "i8", dim, page, kv_heads, [30, 5], extra_positions=8)
+    table = plain_table(100, dim)
+    side = torch.cuda.Stream()
+    k, v = (torch.zeros(2, kv_heads, dim, device="cuda", dtype=torch.bfloat16) for _ in range(2))
+    q, q_out, out = (torch.zeros(2, heads, dim, device="cuda", dtype=torch.bfloat16) for _ in range(3))
+    kv, rope = cache.on_device(), F.Rope(dev(table))
+    lens = dev(np.array([30, 5], np.int32))
+    batch = F.PagedBatch(dev(cache.table), lens, rows=1)
+    scratch = [t.clone() for t in cache.dev]
+
+    def step():
+        lens.add_(1)
+        F.paged_append(kv, batch, k, v, rope=rope, q=q, q_out=q_out)
+        F.paged_attention(kv, batch, q_out, out)
+
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        step()  # the stream's context is made here
+    torch.cuda.synchronize()
+    for t, s in zip(cache.dev, scratch):
+        t.copy_(s)
+    lens.copy_(dev(np.array([30, 5], np.int32)))
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        step()
+    for i in range(6):
+        x = [torch.from_numpy(rng.standard_normal(t.shape).astype(np.float32)).to(t.dtype) for t in (k, v, q)]
+        for t, s in zip((k, v, q), x):
+            t.copy_(s)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(side):
+            graph.replay()
+        torch.cuda.synchronize()
+        cache.lens = [31 + i, 6 + i]
+        at = np.array([30 + i, 5 + i])
+        kx = R.rotate(x[0].double().numpy(), table, at, "interleaved", dtype=np.float32)
+        R.append(cache.codes[0], cache.scales[0], kx, [1, 1], cache.lens, cache.table, "i8")
+        R.append(cache.codes[1], cache.scales[1], x[1].float().numpy(), [1, 1], cache.lens, cache.table, "i8")
+        cache.check()
+        for b in range(2):
+            o, _, size = R.attend(q_out[b].double().cpu().numpy(), cache.values(0, b), cache.values(1, b),
+                                  cache.lens[b] - 1, 0, None, dim ** -0.5)
+            top = np.abs(cache.values(1, b)).max()
+            bound = (4 * 2.0 ** -17 * size + 2.0 ** -18 + 2.0 ** -11) * top
+            assert within(out[b].double().cpu().numpy(), o, bound, "bf16")
+
+
+def test_offsets_beyond_32_bits():
+    """A pool of more than 2^32 bytes: the last pages are appended to and read."""
+    page, kv_heads, dim = 128, 8, 128
+    pages = (1 << 32) // (page * kv_heads * dim) + 40
+    codes = [torch.zeros(pages, kv_heads, page, dim, dtype=torch.int8, device="cuda") for _ in range(2)]
+    scales = [torch.zeros(pages, kv_heads, device="cuda") for _ in range(2)]
+    kv = F.PagedKv(*codes, *scales)
+    table = dev(np.arange(pages - 1, pages - 4, -1, dtype=np.int32)[None, :])
+    rng = np.random.default_rng(33)
+    k, kx = rows_of(rng, 300, kv_heads, dim, "f32")
+    v, vx = rows_of(rng, 300, kv_heads, dim, "f32")
+    batch = F.PagedBatch(table, dev(np.array([300], np.int32)), rows=300)
+    F.paged_append(kv, batch, k, v)
+    q, qv = rows_of(rng, 1, kv_heads, dim, "f32")
+    out = torch.empty(1, kv_heads, dim, device="cuda")
+    F.paged_attention(kv, F.PagedBatch(table, dev(np.array([300], np.int32))), q, out)
+    o, _, _ = R.attend(qv[0], kx.transpose(1, 0, 2), vx.transpose(1, 0, 2), 299, 0, None, dim ** -0.5)
+    # Codes of 8 bits: half a step of max / 127 in every key and value.
+    step = max(np.abs(kx).max(), np.abs(vx).max()) / 254
+    assert np.abs(out.double().cpu().numpy()[0] - o).max() <= step * (1 + 4 * np.abs(qv).sum(-1).max() * dim ** -0.5)
+    assert int(sum((c != 0).any(dim=(1, 2, 3)).sum() for c in codes)) == 6  # three pages each, nothing else
