@@ -158,6 +158,10 @@ struct fo_ctx {
     // Head-sharded prefill: the gathers' stream and its events.
     cudaStream_t comm = nullptr;
     std::vector<cudaEvent_t> comm_ev;
+    // Paged attention: the blocks' unfinished parts and their counters, of one
+    // size for all calls, made by the first.
+    DevBuf paged_parts;
+    int sms = 0;
 };
 
 struct fo_kv_cache {
@@ -499,6 +503,7 @@ int fo_ctx_destroy(fo_ctx *ctx) {
     ctx->host_append_pages.release();
     ctx->i8_pages.release();
     ctx->host_i8_pages.release();
+    ctx->paged_parts.release();
     if (ctx->flags) cudaFree(ctx->flags);
     if (ctx->dev_err) cudaFree(ctx->dev_err);
     if (ctx->ev0) cudaEventDestroy(ctx->ev0);
@@ -1899,7 +1904,19 @@ int fo_paged_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch 
     a.scale = scale;
     a.window = window;
     a.err = ctx->dev_err;
-    cudaError_t e = fo_launch_paged_attention(&a, ctx->stream);
+    if (!ctx->sms) {
+        int sms = 0;
+        FO_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, ctx->device), "cudaDeviceGetAttribute");
+        const size_t parts = (size_t)2 * sms * FO_PAGED_QUERIES;
+        FO_CUDA(ctx->paged_parts.ensure(parts * (128 + 2) * 4 + (size_t)sms * 4), "cudaMalloc(paged attention parts)");
+        FO_CUDA(cudaMemsetAsync(ctx->paged_parts.ptr, 0, ctx->paged_parts.bytes, ctx->stream), "cudaMemset(parts)");
+        ctx->sms = sms;
+    }
+    const size_t parts = (size_t)2 * ctx->sms * FO_PAGED_QUERIES;
+    a.part_o = (float *)ctx->paged_parts.ptr;
+    a.part_ml = a.part_o + parts * 128;
+    a.counters = (unsigned *)(a.part_ml + parts * 2);
+    cudaError_t e = fo_launch_paged_attention(&a, ctx->sms, ctx->stream);
     return e == cudaSuccess ? FO_OK : cuda_fail(e, "paged attention launch");
 }
 

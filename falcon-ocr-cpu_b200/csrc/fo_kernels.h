@@ -236,8 +236,16 @@ struct fo_paged_attention_launch {
     float scale;
     int64_t window;
     unsigned *err;
+    // Scratch of the context: a block's two unfinished parts and a counter.
+    float *part_o;       // [2 sms][FO_PAGED_QUERIES][head_dim]
+    float *part_ml;      // [2 sms][FO_PAGED_QUERIES][2]
+    unsigned *counters;  // [sms], zero between calls
+    // Filled in by the launcher: query heads per KV head, queries that a block
+    // holds, warps that share a tile, and what 16-byte accesses may be used for.
+    int32_t group, queries, col_groups, q_vec, out_vec, evict_first;
 };
-cudaError_t fo_launch_paged_attention(const fo_paged_attention_launch *args, cudaStream_t stream);
+#define FO_PAGED_QUERIES 64  // queries that a block holds at most
+cudaError_t fo_launch_paged_attention(const fo_paged_attention_launch *args, int sms, cudaStream_t stream);
 
 // The bounded-wait self-test kernel (selftest.cu).
 cudaError_t fo_launch_bounded_wait(unsigned *err, unsigned long long limit_ns, cudaStream_t stream);
