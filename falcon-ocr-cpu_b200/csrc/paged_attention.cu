@@ -8,19 +8,20 @@
 // of its KV head, so the call is bound by HBM: positions x KV heads x 2 D
 // bytes.
 //
-// Work is a line of tiles, 64 positions of one KV head of one sequence (and
-// one group of its queries, where there are more than a block holds), the
-// tiles of a (sequence, KV head) adjacent.  Each of at most one block per SM
+// Work is a line of tiles, 16 KB of one KV head of one sequence (64 or 128
+// positions; and one group of its queries, where there are more than a block
+// holds), the tiles of a (sequence, KV head) adjacent.  Each of at most one block per SM
 // takes an equal piece of the line, wherever sequences begin and end, so
 // uneven lengths leave no SM behind and one long sequence is spread over all
 // of them.  A block that holds only part of a (sequence, KV head) leaves its
 // maximum, sum and output in scratch, and the last block of those that share
 // it (a counter in scratch) joins the parts in order.
 //
-// In a block a producer warp walks the page table one step ahead and copies
+// In a block four producer warps walk the page table a step ahead and copy
 // tiles into a ring in shared memory with TMA (swizzled, so that the reads
-// below meet no bank conflicts); eight consumer warps take tiles in turn, each
-// with its own running maximum and sum, and are joined at a piece's end.  A
+// below meet no bank conflicts); eight consumer warps, two to a tile, a half
+// each, take tiles in turn, each with its own running maximum and sum, and are
+// joined at a piece's end.  A
 // consumer computes S^T = K Q^T and O^T += V^T P^T on m16n8k16 tensor
 // instructions with the codes as the A operand: an int8 or FP8 code is an
 // FP16 number exactly, and a scale multiplies a finished sum, so nothing of the
@@ -42,25 +43,31 @@
 
 namespace fo {
 
-constexpr int PA_TILE = 64;        // positions of a tile
-constexpr int PA_CONSUMERS = 8;    // consumer warps
-constexpr int PA_THREADS = 32 * (PA_CONSUMERS + 4);  // and a warpgroup for the producer warp
+constexpr int PA_CONSUMERS = 8;  // consumer warps
+constexpr int PA_PRODUCERS = 4;  // producer warps
+constexpr int PA_STAGES = 12;    // tiles in the ring
+// A parity wait cannot tell a barrier's phase from the one two before it.
+// Every slot of the ring is filled by one producer warp only and emptied by
+// one group of consumer warps only, each of which passes its phases one by one.
+static_assert(PA_STAGES % PA_PRODUCERS == 0 && PA_STAGES % (PA_CONSUMERS / 2) == 0, "owners of the ring's slots");
+constexpr int PA_THREADS = 32 * (PA_CONSUMERS + PA_PRODUCERS);
 // Registers a thread: launched with 168 (65,536 over 384 threads), the
-// producer's warpgroup gives up what the consumers' two take:
-// 128 * 56 + 256 * 224 = 384 * 168.
-constexpr int PA_LAUNCH_REGS = 168, PA_PRODUCER_REGS = 56, PA_CONSUMER_REGS = 224;
+// producers' warpgroup gives up what the consumers' two take:
+// 128 * 72 + 256 * 216 = 384 * 168.
+constexpr int PA_LAUNCH_REGS = 168, PA_PRODUCER_REGS = 72, PA_CONSUMER_REGS = 216;
 static_assert(128 * PA_PRODUCER_REGS + 256 * PA_CONSUMER_REGS == PA_THREADS * PA_LAUNCH_REGS, "register split");
 constexpr float PA_P_BITS = 10.0f;  // probabilities are held times 2^10
 constexpr float PA_LOG2E = 1.4426950408889634f, PA_LN2 = 0.6931471805599453f;
 
 template <int D>
 struct PaShape {
-    static constexpr int TILE_BYTES = PA_TILE * D;
+    static constexpr int TILE_BYTES = 8192;        // of keys, and of values
+    static constexpr int TILE = TILE_BYTES / D;    // positions
+    static constexpr int HALF = TILE / 2;          // a consumer warp's
     static constexpr int STAGE = 2 * TILE_BYTES;
-    static constexpr int STAGES = D == 64 ? 20 : 10;  // 160 KB of tiles
-    static constexpr int COMB_LD = D + 4;             // a column of the joining buffer, in floats
+    static constexpr int COMB_LD = 64 + 4;         // a column of the joining buffer (64 dimensions), in floats
     static constexpr int COMB = PA_CONSUMERS * 8 * COMB_LD * 4;
-    static constexpr int SMEM = 1024 + STAGES * STAGE + COMB;
+    static constexpr int SMEM = 1024 + PA_STAGES * STAGE + COMB;
 };
 
 // The row of eight that a fragment's row g stands for: such that a K
@@ -112,19 +119,21 @@ struct PaWork {
     int tiles;   // per KV head and group of queries (one at least, so that rows that see nothing are written)
     int groups;  // groups of `queries` queries
 };
+template <int TILE>
 __device__ __forceinline__ PaWork pa_work(const fo_paged_attention_launch &a, int64_t seq) {
     PaWork w;
     w.s = load_sequence(a.batch, a.kv.page_size, seq, a.err);
     const int64_t p0 = max64(w.s.len - w.s.n, 0);
     w.low = a.window > 0 ? (int)max64(p0 + 1 - a.window, 0) : 0;
-    w.t0 = w.low / PA_TILE;
-    w.tiles = max((int)((w.s.len + PA_TILE - 1) / PA_TILE) - w.t0, 1);
+    w.t0 = w.low / TILE;
+    w.tiles = max((int)((w.s.len + TILE - 1) / TILE) - w.t0, 1);
     w.groups = (w.s.n * a.group + a.queries - 1) / a.queries;
     return w;
 }
 
 // A place in the line: a sequence, a unit of it (KV head, group of queries)
 // and a tile of the unit.
+template <int TILE>
 struct PaCursor {
     PaWork w;
     int seq, unit, tile;
@@ -140,14 +149,14 @@ struct PaCursor {
         unit = 0;
         do {
             if (++seq >= a.batch.n_seqs) return;
-            w = pa_work(a, seq);
+            w = pa_work<TILE>(a, seq);
         } while (w.groups == 0);
     }
 };
 
 struct PaShared {
-    uint64_t full[20], empty[20];
-    float scales[20][8];  // keys' of a tile's pages, then values'
+    uint64_t full[PA_STAGES], empty[PA_STAGES];
+    float scales[PA_STAGES][16];  // keys' of a tile's pages, then values'
     float ml[PA_CONSUMERS][16][2];
     long long warp_sum[PA_THREADS / 32];
     long long begin_base;
@@ -183,7 +192,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                            const __grid_constant__ fo_paged_attention_launch a) {
     using Shape = PaShape<D>;
-    constexpr int STAGES = Shape::STAGES;
+    constexpr int STAGES = PA_STAGES;
+    constexpr int TILE = Shape::TILE, HALF = Shape::HALF;
+    constexpr int STEPS = HALF / 16;       // m16 steps of a consumer's half
     constexpr int KW = D / 16;             // words of a K row per lane
     constexpr int VW = D / 32;             // words of a V row per lane
     constexpr int MT = D / 16;             // m16 tiles of the output's dimensions
@@ -195,20 +206,20 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     uint8_t *tiles = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(pa_smem) + 1023) & ~uintptr_t(1023));
     float *comb = reinterpret_cast<float *>(tiles + STAGES * Shape::STAGE);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const int key_groups = PA_CONSUMERS / a.col_groups;
+    const int key_groups = PA_CONSUMERS / 2 / a.col_groups;
 
     // This block's piece [begin, end) of the line, and where it begins.
     if (tid == 0) {
         for (int i = 0; i < STAGES; i++) {
             sm100::mbar_init(&sh.full[i], 1);
-            sm100::mbar_init(&sh.empty[i], a.col_groups);
+            sm100::mbar_init(&sh.empty[i], 2 * a.col_groups);
         }
         sm100::mbar_fence_init();
         sh.abort = 0;
     }
     auto work_of = [&](int64_t seq) -> long long {
         if (seq >= a.batch.n_seqs) return 0;
-        const PaWork w = pa_work(a, seq);
+        const PaWork w = pa_work<TILE>(a, seq);
         return (long long)w.tiles * w.groups * a.kv.n_kv_heads;
     };
     long long all, mine = work_of(tid);
@@ -234,9 +245,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         before = pa_scan(mine, sh, chunk);
     }
     __syncthreads();
-    PaCursor at;
+    PaCursor<TILE> at;
     at.seq = sh.begin_seq;
-    at.w = pa_work(a, at.seq);
+    at.w = pa_work<TILE>(a, at.seq);
     long long base = sh.begin_base;  // the line's number of at's sequence's first tile
     {
         const int in = (int)(begin - base);
@@ -245,44 +256,57 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     }
     const int count = (int)(end - begin);
     const int page = a.kv.page_size;
-    const int pages = page >= PA_TILE ? 1 : PA_TILE / page;  // of a tile
+    const int pages = page >= TILE ? 1 : TILE / page;  // of a tile
 
     if (warp >= PA_CONSUMERS) {
         // ------------------------------------------------------------ producer
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PA_PRODUCER_REGS));
-        if (warp > PA_CONSUMERS) return;
-        // Page numbers and scales are fetched a batch of 32 pages at a time, the
-        // numbers two batches ahead of the copies and the scales one.
+        // Each producer warp issues every PA_PRODUCERS-th tile of the block's: one
+        // warp's wait, expectation and two copies take about 500 cycles, more
+        // than a tile's share of HBM's time.  Page numbers and scales are fetched
+        // a batch of 32 pages at a time, the numbers two batches ahead of the
+        // copies and the scales one.
+        const int producer = warp - PA_CONSUMERS;
         const int per_batch = 32 / pages;
         const int j = lane % pages, off = lane / pages;
         struct Batch {
-            int n, head, row;  // tiles, KV head, and this lane's page: number (-1: none), first row in it
+            int first, n;   // the block's tiles first, first + PA_PRODUCERS, ..: n of them
+            int head, row;  // KV head, and this lane's page: its first row, its number (-1: none)
             int id;
             bool bad;
             float ks, vs;
         };
         int ahead = 0;  // tiles handed to batches
+        bool more = true;
         auto fetch_id = [&]() {
             Batch b;
-            b.n = min(min(per_batch, at.left()), count - ahead);
             b.id = -1;
             b.bad = false;
             b.row = 0;
             b.ks = b.vs = 0.0f;
-            if (b.n <= 0) return b;
-            b.head = at.head();
-            const int64_t pos = (int64_t)(at.w.t0 + at.tile + off) * PA_TILE + j * page;  // of a page's first copied row
-            const int64_t first = pos / page * page;
-            if (off < b.n && pos < at.w.s.len && first + page > at.w.low) {
-                b.id = __ldg(a.batch.page_table + at.seq * a.batch.table_stride + pos / page);
-                b.row = (int)(pos - first);
+            b.first = b.n = b.head = 0;
+            const int span = min(min(PA_PRODUCERS * per_batch, at.left()), count - ahead);
+            if (span <= 0) {
+                more = false;
+                return b;
             }
-            ahead += b.n;
-            at.advance(a, b.n);
+            const int skip = (producer - ahead % PA_PRODUCERS + PA_PRODUCERS) % PA_PRODUCERS;
+            b.first = ahead + skip;
+            b.n = (span - skip + PA_PRODUCERS - 1) / PA_PRODUCERS;
+            b.head = at.head();
+            // The first position that the page's copy holds.
+            const int64_t pos = (int64_t)(at.w.t0 + at.tile + skip + PA_PRODUCERS * off) * TILE + j * page;
+            const int64_t begins = pos / page * page;
+            if (off < b.n && pos < at.w.s.len && begins + page > at.w.low) {
+                b.id = __ldg(a.batch.page_table + at.seq * a.batch.table_stride + pos / page);
+                b.row = (int)(pos - begins);
+            }
+            ahead += span;
+            at.advance(a, span);
             return b;
         };
         auto fetch_scales = [&](Batch &b) {
-            if (b.n <= 0 || b.id == -1) return;
+            if (b.id == -1) return;
             b.bad = b.id < 0 || b.id >= a.kv.n_pages;
             if (b.bad) return;
             const int64_t tile = (int64_t)b.id * a.kv.n_kv_heads + b.head;
@@ -294,19 +318,20 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             sm100::tma_prefetch(&v_map);
         }
         const uint64_t policy = sm100::l2_evict_first();
-        const int rows = min(page, PA_TILE);
+        const int rows = min(page, TILE);
         const uint32_t bytes = (uint32_t)rows * D;
-        int issued = 0;
+        int last = -1;  // the last tile whose copies were issued
         bool ok = true;
         // The first page numbers are asked for together, the first scales while
         // the second numbers are on their way.
         Batch now = fetch_id(), next = fetch_id();
         fetch_scales(now);
-        while (now.n > 0 && ok) {
+        for (bool rest = true; rest && ok;) {
+            rest = more;
             Batch later = fetch_id();
             fetch_scales(next);
             for (int i = 0; i < now.n; i++) {
-                const int slot = issued % STAGES, round = issued / STAGES;
+                const int tile = now.first + PA_PRODUCERS * i, slot = tile % STAGES, round = tile / STAGES;
                 if (round > 0 && !sm100::mbar_wait(&sh.empty[slot], (round - 1) & 1, &sh.abort, a.err)) {
                     ok = false;
                     break;
@@ -336,19 +361,19 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                     // A page number outside the pool gives NaN; a page that no row
                     // sees has scales of 0.
                     sh.scales[slot][j] = now.bad ? NAN : now.ks;
-                    sh.scales[slot][4 + j] = now.bad ? NAN : now.vs;
+                    sh.scales[slot][8 + j] = now.bad ? NAN : now.vs;
                     if (now.bad) atomicOr(a.err, FO_DEVERR_PAGED);
                 }
                 __syncwarp();
                 if (lane == 0) sm100::mbar_arrive(&sh.full[slot]);
-                issued++;
+                last = tile;
             }
             now = next;
             next = later;
         }
         if (!ok && lane == 0) {
             // A consumer gave up: the copies in flight land before the block ends.
-            for (int i = max(issued - STAGES, 0); i < issued; i++)
+            for (int i = last; i >= 0 && i > last - STAGES; i -= PA_PRODUCERS)
                 sm100::mbar_wait_drain(&sh.full[i % STAGES], (i / STAGES) & 1);
         }
         return;
@@ -357,13 +382,13 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     // ---------------------------------------------------------------- consumers
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PA_CONSUMER_REGS));
     const int g = lane >> 2, t = lane & 3;
-    const int key_group = warp / a.col_groups, col_group = warp % a.col_groups;
+    const int col_group = warp % a.col_groups, half = warp / a.col_groups % 2, key_group = warp / a.col_groups / 2;
     const int kg = pa_key<D>(g), kt0 = pa_key<D>(2 * t), kt1 = pa_key<D>(2 * t + 1);
     // Byte offsets of this lane's pieces of a K row and of its V rows.
     const int k_off = D == 128 ? kg * 128 + ((t ^ kg) << 4) : kg * 64 + ((t ^ (kg >> 1 & 3)) << 4);
     const int v_off0 = D == 128 ? kt0 * 128 + ((g ^ kt0) << 4) : kt0 * 64 + (((g >> 1) ^ (kt0 >> 1 & 3)) << 4) + (g & 1) * 8;
     const int v_off1 = D == 128 ? kt1 * 128 + ((g ^ kt1) << 4) : kt1 * 64 + (((g >> 1) ^ (kt1 >> 1 & 3)) << 4) + (g & 1) * 8;
-    const int pages_shift = page == 16 ? 0 : page == 32 ? 1 : 2;  // log2 of the 16-row steps of a page's part of a tile
+    const int page_shift = 31 - __clz(min(page, TILE) / 16);  // log2 of the m16 steps of a page's part of a tile
     bool ok = true;
 
     for (int i = 0; i < count;) {
@@ -450,14 +475,22 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         int k = i + (key_group - i % key_groups + key_groups) % key_groups;
         for (; ok && k < i + n; k += key_groups) {
             const int slot = k % STAGES;
-            const int pos0 = (at.w.t0 + at.tile + (k - i)) * PA_TILE;
+            // The first position of this warp's half.
+            const int pos0 = (at.w.t0 + at.tile + (k - i)) * TILE + half * HALF;
             ok = sm100::mbar_wait(&sh.full[slot], (k / STAGES) & 1, &sh.abort, a.err);
             if (!ok) break;
-            uint8_t *kt = tiles + slot * Shape::STAGE, *vt = kt + Shape::TILE_BYTES;
+            if (pos0 > p_last || pos0 + HALF <= at.w.low) {
+                // No row sees any of it.
+                __syncwarp();
+                if (lane == 0) sm100::mbar_arrive(&sh.empty[slot]);
+                continue;
+            }
+            const uint8_t *kt = tiles + slot * Shape::STAGE + half * HALF * D;
+            uint8_t *vt = tiles + slot * Shape::STAGE + Shape::TILE_BYTES + half * HALF * D;
             // S^T: rows = keys, columns = queries.
-            float c[4][NT][4];
+            float c[STEPS][NT][4];
 #pragma unroll
-            for (int mt = 0; mt < 4; mt++) {
+            for (int mt = 0; mt < STEPS; mt++) {
                 uint32_t kw[2][KW];
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
@@ -479,15 +512,15 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                     for (int nt = 0; nt < NT; nt++) pa_mma(c[mt][nt], a0, a1, a2, a3, qf[nt][w][0], qf[nt][w][1]);
                 }
             }
-            const bool masked = pos0 + PA_TILE - 1 > p_first || pos0 < low_last;
+            const bool masked = pos0 + HALF - 1 > p_first || pos0 < low_last;
             // Scores, times log2 e; FP32 rows have a query's two terms in
             // neighbouring columns.
             float mx[NT][2];
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) mx[nt][0] = mx[nt][1] = -INFINITY;
 #pragma unroll
-            for (int mt = 0; mt < 4; mt++) {
-                const float ks = sh.scales[slot][mt >> pages_shift];
+            for (int mt = 0; mt < STEPS; mt++) {
+                const float ks = sh.scales[slot][(half * STEPS + mt) >> page_shift];
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
                     if constexpr (TERMS == 2) {
@@ -553,9 +586,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                 }
             }
             // Probabilities, transposed into B operands: rows = keys of V.
-            uint32_t pf[4][NT][2];
+            uint32_t pf[STEPS][NT][2];
 #pragma unroll
-            for (int mt = 0; mt < 4; mt++)
+            for (int mt = 0; mt < STEPS; mt++)
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++)
 #pragma unroll
@@ -578,9 +611,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             if constexpr (FORMAT == FO_PAGED_E4M3) {
                 // Rows beyond the sequence, or of pages that no row sees, may hold any
                 // bytes: an FP8 NaN times a probability of 0 would be NaN.
-                const int lo_row = max(at.w.low / page * page - pos0, 0), hi_row = (int)min64(s.len - pos0, PA_TILE);
-                if (lo_row > 0 || hi_row < PA_TILE) {
-                    for (int x = lane; x < Shape::TILE_BYTES / 16; x += 32) {
+                const int lo_row = max(at.w.low / page * page - pos0, 0), hi_row = (int)min64(s.len - pos0, HALF);
+                if (lo_row > 0 || hi_row < HALF) {
+                    for (int x = lane; x < HALF * D / 16; x += 32) {
                         const int row = x / (D / 16);
                         if (row < lo_row || row >= hi_row) reinterpret_cast<uint4 *>(vt)[x] = make_uint4(0, 0, 0, 0);
                     }
@@ -595,7 +628,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
 #pragma unroll
                     for (int e = 0; e < 4; e++) acc[d][nt][e] = 0.0f;
 #pragma unroll
-            for (int kk = 0; kk < 4; kk++) {
+            for (int kk = 0; kk < STEPS; kk++) {
                 uint32_t va[VW], vb[VW], vc[VW], vd[VW];
                 const uint8_t *row = vt + 16 * kk * D;
                 if constexpr (D == 128) {
@@ -621,9 +654,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                         for (int nt = 0; nt < NT; nt++)
                             pa_mma(acc[2 * w + b][nt], a0, a1, a2, a3, pf[kk][nt][0], pf[kk][nt][1]);
                     }
-                if (kk == 3 || ((kk + 1) & ((1 << pages_shift) - 1)) == 0) {
+                if (kk == STEPS - 1 || ((half * STEPS + kk + 1) & ((1 << page_shift) - 1)) == 0) {
                     // The end of a page: its scale.
-                    const float vs = sh.scales[slot][4 + (kk >> pages_shift)];
+                    const float vs = sh.scales[slot][8 + ((half * STEPS + kk) >> page_shift)];
 #pragma unroll
                     for (int d = 0; d < MT; d++)
 #pragma unroll
@@ -679,19 +712,22 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                 a.lse[(s.first + r) * a.q.heads + h] = ll == 0.0f ? -INFINITY : (mm + log2f(ll) - PA_P_BITS) * PA_LN2;
         };
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-            float *mine_at = comb + warp * 8 * Shape::COMB_LD;
+        for (int pass = 0; pass < NT * (D / 64); pass++) {
+            // An n8 tile's columns, 64 dimensions of them.
+            const int nt = pass / (D / 64), d64 = pass % (D / 64);
+            if (D == 64 || g / 4 == d64) {
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                float *col = mine_at + (2 * t + h) * Shape::COMB_LD + (D / 8) * g;
+                for (int h = 0; h < 2; h++) {
+                    float *col = comb + (warp * 8 + 2 * t + h) * Shape::COMB_LD + (D / 8) * g - 64 * d64;
 #pragma unroll
-                for (int d = 0; d < MT; d += 2)
-                    *reinterpret_cast<float4 *>(col + 2 * d) =
-                        make_float4(o[d][nt][h], o[d][nt][2 + h], o[d + 1][nt][h], o[d + 1][nt][2 + h]);
+                    for (int d = 0; d < MT; d += 2)
+                        *reinterpret_cast<float4 *>(col + 2 * d) =
+                            make_float4(o[d][nt][h], o[d][nt][2 + h], o[d + 1][nt][h], o[d + 1][nt][2 + h]);
+                }
             }
             pa_consumers_sync();
-            for (int x = tid; x < a.col_groups * QN * (D / 4); x += 32 * PA_CONSUMERS) {
-                const int quad = x % (D / 4), cq = x / (D / 4);
+            for (int x = tid; x < a.col_groups * QN * 16; x += 32 * PA_CONSUMERS) {
+                const int quad = x % 16, cq = x / 16;
                 const int cg = cq / QN, col = (cq - cg * QN) * TERMS;
                 const int qi = query_of(nt, 0) + (cg - col_group) * WARP_QUERIES + col / TERMS;
                 if (qi >= n_queries) continue;
@@ -717,11 +753,12 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                     v = make_float4(fmaf(u.x, f, v.x), fmaf(u.y, f, v.y), fmaf(u.z, f, v.z), fmaf(u.w, f, v.w));
                 }
                 if (lost) ll = NAN;
+                const int at_quad = 16 * d64 + quad;
                 if (c0 == c1) {
-                    write_out(qi, quad, v, mm, ll);
+                    write_out(qi, at_quad, v, mm, ll);
                 } else {
-                    *reinterpret_cast<float4 *>(a.part_o + (part * a.queries + qi) * D + 4 * quad) = v;
-                    if (quad == 0)
+                    *reinterpret_cast<float4 *>(a.part_o + (part * a.queries + qi) * D + 4 * at_quad) = v;
+                    if (at_quad == 0)
                         *reinterpret_cast<float2 *>(a.part_ml + (part * a.queries + qi) * 2) = make_float2(mm, ll);
                 }
             }
@@ -781,7 +818,7 @@ bool pa_map(CUtensorMap *map, const void *codes, const fo_paged_kv &kv) {
     const cuuint64_t rows = (cuuint64_t)kv.n_kv_heads * kv.page_size;
     cuuint64_t dims[3] = {(cuuint64_t)kv.head_dim, rows, (cuuint64_t)kv.n_pages};
     cuuint64_t strides[2] = {(cuuint64_t)kv.head_dim, rows * kv.head_dim};
-    cuuint32_t box[3] = {(cuuint32_t)kv.head_dim, (cuuint32_t)std::min(kv.page_size, PA_TILE), 1};
+    cuuint32_t box[3] = {(cuuint32_t)kv.head_dim, (cuuint32_t)std::min<int>(kv.page_size, 8192 / kv.head_dim), 1};
     cuuint32_t estr[3] = {1, 1, 1};
     return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void *>(codes), dims, strides, box, estr,
               CU_TENSOR_MAP_INTERLEAVE_NONE, kv.head_dim == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
@@ -841,11 +878,12 @@ extern "C" cudaError_t fo_launch_paged_attention(const fo_paged_attention_launch
     };
     a.q_vec = aligned(a.q, 16);
     a.out_vec = aligned(a.out, terms == 2 ? 16 : 8);
-    // No more blocks than the most tiles there can be for, a warp each.
+    // No more blocks than the most tiles there can be for, one for each group
+    // of consumer warps.
     const int64_t most = a.batch.n_seqs * a.kv.n_kv_heads * ((columns / terms + a.queries - 1) / a.queries) *
-                         ((a.batch.table_stride * a.kv.page_size + fo::PA_TILE - 1) / fo::PA_TILE);
-    const int64_t warps = fo::PA_CONSUMERS / a.col_groups;
-    const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(sms, (most + warps - 1) / warps));
+                         ((a.batch.table_stride * a.kv.page_size * a.kv.head_dim + 8191) / 8192);
+    const int64_t groups = fo::PA_CONSUMERS / 2 / a.col_groups;
+    const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(sms, (most + groups - 1) / groups));
     if (a.kv.head_dim == 64)
         return a.kv.format == FO_PAGED_I8 ? fo::launch_attention<64, FO_PAGED_I8>(a, nt, grid, stream)
                                           : fo::launch_attention<64, FO_PAGED_E4M3>(a, nt, grid, stream);
