@@ -17,23 +17,30 @@
 // maximum, sum and output in scratch, and the last block of those that share
 // it (a counter in scratch) joins the parts in order.
 //
-// In a block four producer warps walk the page table a step ahead and copy
+// In a block two producer warps walk the page table a step ahead and copy
 // tiles into a ring in shared memory with TMA (swizzled, so that the reads
 // below meet no bank conflicts); eight consumer warps, two to a tile, a half
-// each, take tiles in turn, each with its own running maximum and sum, and are
-// joined at a piece's end.  A
-// consumer computes S^T = K Q^T and O^T += V^T P^T on m16n8k16 tensor
-// instructions with the codes as the A operand: an int8 or FP8 code is an
-// FP16 number exactly, and a scale multiplies a finished sum, so nothing of the
-// cache is rounded.  The 5th-generation MMA reads its operands from shared
-// memory or TMEM, which would cost every tile a trip back through shared
-// memory after the conversion; a decode's few queries leave these instructions
-// far from bounding the kernel.  A query is held as FP16 relative to a
-// power of two near its largest element: BF16's 8 bits exactly, FP32 as the sum
-// of two terms (22 bits) in neighbouring columns.  Probabilities are scaled
-// by 2^10 so that FP16 holds those down to 2^-24 of the largest at full
-// precision; BF16 rows round them to FP16's 11 bits, three more than the
-// output has, FP32 rows carry a second term.  Sums, maxima and outputs are FP32.
+// each, take tiles in turn, each with its own running maximum and sum; and two
+// epilogue warps split the next (sequence, KV head)'s queries into operands
+// while the consumers are at this one's, join the consumers' parts, and write
+// or hand on the result, so that the consumers go from one to the next
+// without waiting for any of that.
+//
+// The codes themselves are the A operands of the tensor instructions: a
+// consumer computes S^T = K Q^T and O^T += V^T P^T on m16n8k32 products of
+// int8 (exact, 32-bit sums) or of e4m3 (exact products, FP32 sums), keys as
+// they lie, values through transposing shared-memory loads, so that nothing
+// of the cache is converted or rounded; a scale multiplies a finished sum.
+// Queries and probabilities are split into 8-bit terms, one product each.
+// int8: a query is a 23-bit integer relative to a power of two near its
+// largest element (three bytes), a probability one of 16 bits (BF16 rows, whose
+// output has 8) or 23 (FP32 rows) relative to its tile's largest.  e4m3: terms
+// of 4 bits, each what the ones before it leave: two for a BF16 query, which
+// hold it exactly, three for its probabilities (12 bits), twice three for
+// FP32 rows.  The 5th-generation MMA would want the few queries' side padded
+// and every score and output moved through TMEM; at a decode's few columns
+// these instructions take a small part of the time that HBM needs for a
+// tile.  Maxima, sums and outputs are FP32.
 #include "paged.cuh"
 #include "sm100.cuh"
 
@@ -44,46 +51,75 @@
 namespace fo {
 
 constexpr int PA_CONSUMERS = 8;  // consumer warps
-constexpr int PA_PRODUCERS = 4;  // producer warps
-constexpr int PA_STAGES = 12;    // tiles in the ring
+constexpr int PA_PRODUCERS = 2;  // producer warps
+constexpr int PA_EPILOGUES = 2;  // epilogue warps
+constexpr int PA_STAGES = 8;     // tiles in the ring
 // A parity wait cannot tell a barrier's phase from the one two before it.
 // Every slot of the ring is filled by one producer warp only and emptied by
 // one group of consumer warps only, each of which passes its phases one by one.
 static_assert(PA_STAGES % PA_PRODUCERS == 0 && PA_STAGES % (PA_CONSUMERS / 2) == 0, "owners of the ring's slots");
-constexpr int PA_THREADS = 32 * (PA_CONSUMERS + PA_PRODUCERS);
+constexpr int PA_THREADS = 32 * (PA_CONSUMERS + PA_PRODUCERS + PA_EPILOGUES);
 // Registers a thread: launched with 168 (65,536 over 384 threads), the
-// producers' warpgroup gives up what the consumers' two take:
-// 128 * 72 + 256 * 216 = 384 * 168.
-constexpr int PA_LAUNCH_REGS = 168, PA_PRODUCER_REGS = 72, PA_CONSUMER_REGS = 216;
-static_assert(128 * PA_PRODUCER_REGS + 256 * PA_CONSUMER_REGS == PA_THREADS * PA_LAUNCH_REGS, "register split");
-constexpr float PA_P_BITS = 10.0f;  // probabilities are held times 2^10
+// producers' and epilogues' warpgroup gives up what the consumers' two take:
+// 128 * 104 + 256 * 200 = 384 * 168.
+constexpr int PA_LAUNCH_REGS = 168, PA_OTHER_REGS = 104, PA_CONSUMER_REGS = 200;
+static_assert(128 * PA_OTHER_REGS + 256 * PA_CONSUMER_REGS == PA_THREADS * PA_LAUNCH_REGS, "register split");
 constexpr float PA_LOG2E = 1.4426950408889634f, PA_LN2 = 0.6931471805599453f;
 
-template <int D>
+template <int D, int FORMAT, int NT, bool F32>
 struct PaShape {
     static constexpr int TILE_BYTES = 8192;        // of keys, and of values
     static constexpr int TILE = TILE_BYTES / D;    // positions
     static constexpr int HALF = TILE / 2;          // a consumer warp's
     static constexpr int STAGE = 2 * TILE_BYTES;
-    static constexpr int COMB_LD = 64 + 4;         // a column of the joining buffer (64 dimensions), in floats
-    static constexpr int COMB = PA_CONSUMERS * 8 * COMB_LD * 4;
-    static constexpr int SMEM = 1024 + PA_STAGES * STAGE + COMB;
+    static constexpr int QT = FORMAT == FO_PAGED_I8 ? 3 : F32 ? 6 : 2;                // a query's terms
+    static constexpr int PT = FORMAT == FO_PAGED_I8 ? (F32 ? 3 : 2) : F32 ? 6 : 3;    // a probability's
+    static constexpr int PART_LD = D + 4;          // a column of a consumer's part, in floats
+    static constexpr int PARTS = PA_CONSUMERS * NT * 8 * PART_LD * 4;
+    static constexpr int Q_TILE = QT * (D / 32) * 32 * 8;  // an n8 tile of queries as operands
+    static int smem(int q_tiles) { return 1024 + PA_STAGES * STAGE + PARTS + q_tiles * Q_TILE; }
 };
 
-// The row of eight that a fragment's row g stands for: such that a K
-// fragment's and a V fragment's reads fall into different banks under the
-// tile's swizzle (128-byte rows: 128-byte swizzle; 64-byte rows: 64-byte).
+// The key of eight that a fragment's row g stands for: such that a K
+// fragment's reads fall into different banks under the tile's swizzle (128-byte
+// rows: 128-byte swizzle; 64-byte rows: 64-byte).  Rows 8 .. 15 of a fragment
+// stand for the keys 8 + pa_key(g ^ 4), so that the eight rows of a V load do too.
 template <int D>
-__device__ __forceinline__ int pa_key(int g) {
-    if constexpr (D == 128) return g & 1 ? (g - 1) ^ 5 : g;
-    return (0x65217430u >> (4 * g)) & 7;
+__host__ __device__ constexpr int pa_key(int g) {
+    return D == 128 ? g >> 1 | (g & 1) << 2 : g;
 }
 
-__device__ __forceinline__ void pa_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
-                                       uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+// Accumulators of int8 products start at 1.5 * 2^23's bits, so that read as
+// floats they are 1.5 * 2^23 + sum (sums here stay below 2^22).
+constexpr uint32_t PA_MAGIC = 0x4B400000u;
+constexpr float PA_MAGIC_F = 12582912.0f;
+
+// c += a b, a m16 x k32, b k32 x n8: int8 codes by signed or unsigned bytes.
+template <bool SIGNED>
+__device__ __forceinline__ void pa_imma(uint32_t (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                        uint32_t b0, uint32_t b1) {
+    if constexpr (SIGNED)
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+    else
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.u8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+            : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void pa_qmma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+                                        uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+// Two 16 x 16 matrices of bytes, transposed: lanes 0 .. 15 give the addresses
+// of the first one's rows, 16 .. 31 of the second's; r[0] and r[1] are its
+// columns g and g + 8, rows 4 t .. 4 t + 3.
+__device__ __forceinline__ void pa_load_transposed(uint32_t (&r)[4], uint32_t address) {
+    asm volatile("ldmatrix.sync.aligned.m16n16.x2.trans.shared.b8 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(address));
 }
 // An 8 x 8 matrix of 16-bit elements, two per lane along a row, transposed.
 __device__ __forceinline__ uint32_t pa_transpose(uint32_t x) {
@@ -91,25 +127,18 @@ __device__ __forceinline__ uint32_t pa_transpose(uint32_t x) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-__device__ __forceinline__ uint32_t pa_f16x2(float lo, float hi) {
+// Two floats as e4m3 (nearest even), lo in the low byte, and what is left.
+__device__ __forceinline__ uint32_t pa_e4m3x2(float &lo, float &hi) {
     uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    asm("{\n\t.reg .b16 x;\n\tcvt.rn.satfinite.e4m3x2.f32 x, %2, %1;\n\tcvt.u32.u16 %0, x;\n\t}"
+        : "=r"(r)
+        : "f"(lo), "f"(hi));
+    const float2 back = f16x2_f32x2(e4m3x2_f16x2(r));
+    lo -= back.x;
+    hi -= back.y;
     return r;
 }
-// Four codes as FP16 (exact): the low two and the high two.
-template <int FORMAT>
-__device__ __forceinline__ void pa_codes(uint32_t w, uint32_t &lo, uint32_t &hi) {
-    if constexpr (FORMAT == FO_PAGED_I8) {
-        // 1024 + (code + 128) has the code in its low bits; 1152 = 0x6480.
-        const uint32_t u = w ^ 0x80808080u;
-        const uint32_t a = __byte_perm(u, 0x64646464u, 0x4140), b = __byte_perm(u, 0x64646464u, 0x4342);
-        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(lo) : "r"(a), "r"(0x64806480u));
-        asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(hi) : "r"(b), "r"(0x64806480u));
-    } else {
-        lo = e4m3x2_f16x2(w & 0xFFFFu);
-        hi = e4m3x2_f16x2(w >> 16);
-    }
-}
+constexpr float PA_GROUP = 4096.0f;  // e4m3 terms 4 .. 6 stand for 2^-12 of their value
 
 // A sequence's share of the line of tiles.
 struct PaWork {
@@ -156,11 +185,15 @@ struct PaCursor {
 
 struct PaShared {
     uint64_t full[PA_STAGES], empty[PA_STAGES];
-    float scales[PA_STAGES][16];  // keys' of a tile's pages, then values'
+    uint64_t q_full, q_free;        // a segment's queries are there; have been taken
+    uint64_t part_full, part_free;  // its parts
+    float scales[PA_STAGES][16];    // keys' of a tile's pages, then values'
     float ml[PA_CONSUMERS][16][2];
+    float q_scale[FO_PAGED_QUERIES];
+    int q_pos[FO_PAGED_QUERIES];
     long long warp_sum[PA_THREADS / 32];
     long long begin_base;
-    int begin_seq, abort, last;
+    int begin_seq, abort;
 };
 
 // Sum of x over the block's earlier threads; `all` the whole block's.
@@ -185,26 +218,244 @@ __device__ __forceinline__ long long pa_scan(long long x, PaShared &sh, long lon
     return before + incl - x;
 }
 
-__device__ __forceinline__ void pa_consumers_sync() { asm volatile("bar.sync 1, %0;" ::"n"(32 * PA_CONSUMERS) : "memory"); }
+// The smallest whole number of at least total / n (FP64 holds what there can be
+// of tiles exactly; its quotient is off by one at most).
+__device__ __forceinline__ long long pa_share(long long total, int n) {
+    long long x = (long long)((double)total / n);
+    while (x * n < total) x++;
+    return x;
+}
 
-template <int D, int FORMAT, int NT, int TERMS>
+// The epilogue warps: `me` of PA_EPILOGUES takes every PA_EPILOGUES-th n8 tile of
+// queries to split into operands, and every such query to join and write.
+template <int D, int FORMAT, int NT, bool F32, int TILE>
+__device__ __forceinline__ void pa_epilogue(const fo_paged_attention_launch &a, PaShared &sh, PaCursor<TILE> at, int count,
+                                            long long begin, long long per, int me, float *parts, uint2 *q_ops) {
+    using Shape = PaShape<D, FORMAT, NT, F32>;
+    using T = typename std::conditional<F32, float, uint16_t>::type;
+    constexpr bool I8 = FORMAT == FO_PAGED_I8;
+    constexpr int KS = D / 32, QT = Shape::QT;
+    const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+
+    // A unit's queries as B operands: column g of an n8 tile, this lane's elements
+    // 16 t .. 16 t + 15 of each 64.
+    auto split = [&](const PaCursor<TILE> &u) {
+        const int q0 = u.group() * a.queries, head = u.head();
+        const int n_queries = min(u.w.s.n * a.group - q0, a.queries);
+        for (int tile = me; tile * 8 < n_queries; tile += PA_EPILOGUES) {
+            const int qi = tile * 8 + g;
+            const T *q = nullptr;
+            int r = 0;
+            if (qi < n_queries) {
+                r = (q0 + qi) / a.group;
+                q = static_cast<const T *>(a.q.data) + (u.w.s.first + r) * a.q.row_stride +
+                    (head * a.group + (q0 + qi) - r * a.group) * a.q.head_stride + 16 * t;
+            }
+            float x[KS / 2][16], top = 0.0f;
+            bool finite = true;
+#pragma unroll
+            for (int c = 0; c < KS / 2; c++) {
+                if (!q) {
+#pragma unroll
+                    for (int e = 0; e < 16; e++) x[c][e] = 0.0f;
+                } else if (a.q_vec) {
+                    load8(q + 64 * c, x[c]);
+                    load8(q + 64 * c + 8, x[c] + 8);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; e++) x[c][e] = load1(q + 64 * c + e);
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < KS / 2; c++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    top = fmaxf(top, fabsf(x[c][e]));
+                    finite &= fabsf(x[c][e]) <= FLT_MAX;
+                }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const unsigned all_finite = __ballot_sync(0xffffffffu, finite);
+            // A power of two near the largest element brings it to [2^21, 2^22)
+            // (int8) or [2^7, 2^8) (e4m3); in two factors, so that FP32's whole
+            // range of exponents can be brought there.
+            const int e = max((int)(__float_as_uint(top) >> 23), 1);
+            const float up = I8 ? 2097152.0f : 128.0f;
+            const float inv0 = __uint_as_float((uint32_t)(254 - (e + 1) / 2 - 63) << 23);
+            const float inv1 = __uint_as_float((uint32_t)(254 - (e - (e + 1) / 2) - 64) << 23);
+            if (t == 0) {
+                const bool good = (all_finite >> (lane & 28) & 15) == 15;
+                sh.q_scale[qi] = good ? __uint_as_float((uint32_t)e << 23) / up * a.scale * PA_LOG2E : NAN;
+                sh.q_pos[qi] = q ? (int)(u.w.s.len - u.w.s.n) + r : -1;
+            }
+            uint2 *to = q_ops + tile * (Shape::Q_TILE / 8) + lane;
+#pragma unroll
+            for (int c = 0; c < KS / 2; c++)
+#pragma unroll
+                for (int w = 0; w < 2; w++) {
+                    // Elements 8 w .. 8 w + 7: step 2 c + w.
+                    float y[8];
+#pragma unroll
+                    for (int i = 0; i < 8; i++) y[i] = x[c][8 * w + i] * inv0 * inv1 * up;
+                    if constexpr (I8) {
+                        uint32_t f[3][2];
+#pragma unroll
+                        for (int h = 0; h < 2; h++) {
+                            uint32_t z[4];
+#pragma unroll
+                            for (int i = 0; i < 4; i++) z[i] = (uint32_t)__float2int_rn(y[4 * h + i]);
+                            const uint32_t lo01 = __byte_perm(z[0], z[1], 0x5140), lo23 = __byte_perm(z[2], z[3], 0x5140);
+                            f[0][h] = __byte_perm(__byte_perm(z[0], z[1], 0x0062), __byte_perm(z[2], z[3], 0x0062), 0x5410);
+                            f[1][h] = __byte_perm(lo01, lo23, 0x7632);
+                            f[2][h] = __byte_perm(lo01, lo23, 0x5410);
+                        }
+#pragma unroll
+                        for (int i = 0; i < 3; i++) to[(i * KS + 2 * c + w) * 32] = make_uint2(f[i][0], f[i][1]);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < QT; i++) {
+                            if (i == 3) {
+#pragma unroll
+                                for (int j = 0; j < 8; j++) y[j] *= PA_GROUP;
+                            }
+                            uint32_t f[4];
+#pragma unroll
+                            for (int j = 0; j < 4; j++) f[j] = pa_e4m3x2(y[2 * j], y[2 * j + 1]);
+                            to[(i * KS + 2 * c + w) * 32] = make_uint2(f[0] | f[1] << 16, f[2] | f[3] << 16);
+                        }
+                    }
+                }
+        }
+        __syncwarp();
+        if (lane == 0) sm100::mbar_arrive(&sh.q_full);
+    };
+
+    PaCursor<TILE> next = at;
+    int next_i = 0;
+    split(next);
+    for (int i = 0, segment = 0; i < count; segment++) {
+        const int n = min(at.left(), count - i);
+        // The next unit's queries.
+        next_i += n;
+        next.advance(a, n);
+        if (next_i < count) {
+            if (!sm100::mbar_wait(&sh.q_free, segment & 1, &sh.abort, a.err)) return;
+            split(next);
+        }
+        const Sequence &s = at.w.s;
+        const int head = at.head(), q0 = at.group() * a.queries;
+        const int n_queries = min(s.n * a.group - q0, a.queries);
+        // The unit's tiles in the line, and the blocks that share it.
+        const long long unit_begin = begin + i - at.tile, unit_end = unit_begin + at.w.tiles;
+        const bool alone = unit_begin >= begin && unit_end <= begin + count;
+        int c0 = blockIdx.x, c1 = blockIdx.x;
+        if (!alone) {
+            c0 = (int)((double)unit_begin / (double)per);
+            c1 = (int)((double)(unit_end - 1) / (double)per);
+        }
+        if (!sm100::mbar_wait(&sh.part_full, segment & 1, &sh.abort, a.err)) return;
+
+        // One query's four dimensions at a time, from parts in shared memory or, at
+        // the last block to come, in scratch.
+        auto at_part = [&](int cta, int qi) { return (2 * (int64_t)cta + (cta == c0 ? 1 : 0)) * a.queries + qi; };
+        auto join = [&](bool scratch) {
+            for (int x = lane; x < (n_queries - me + PA_EPILOGUES - 1) / PA_EPILOGUES * (D / 4); x += 32) {
+                const int quad = x % (D / 4), qi = x / (D / 4) * PA_EPILOGUES + me;
+                const int tile = qi / 8, cg = tile % a.col_groups, nt = tile / a.col_groups, col = qi % 8;
+                const int parts_n = scratch ? c1 - c0 + 1 : PA_CONSUMERS / a.col_groups;
+                float mm = -INFINITY, ll = 0.0f;
+                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                bool lost = false;
+#pragma unroll 4
+                for (int j = 0; j < parts_n; j++) {
+                    const int w = j * a.col_groups + cg;
+                    float2 ml;
+                    float4 u;
+                    if (scratch) {
+                        ml = __ldcg(reinterpret_cast<const float2 *>(a.part_ml) + at_part(c0 + j, qi));
+                        u = __ldcg(reinterpret_cast<const float4 *>(a.part_o + at_part(c0 + j, qi) * D) + quad);
+                    } else {
+                        ml = *reinterpret_cast<const float2 *>(sh.ml[w][8 * nt + col]);
+                        u = *reinterpret_cast<const float4 *>(parts + ((w * NT + nt) * 8 + col) * Shape::PART_LD + 4 * quad);
+                    }
+                    lost |= ml.x != ml.x || ml.y != ml.y;
+                    if (ml.x == -INFINITY) continue;  // it has seen nothing
+                    const float top = fmaxf(mm, ml.x);
+                    const float f0 = sm100::ex2(mm - top), f1 = sm100::ex2(ml.x - top);
+                    mm = top;
+                    ll = fmaf(ml.y, f1, ll * f0);
+                    v = make_float4(fmaf(u.x, f1, v.x * f0), fmaf(u.y, f1, v.y * f0), fmaf(u.z, f1, v.z * f0),
+                                    fmaf(u.w, f1, v.w * f0));
+                }
+                if (lost) ll = NAN;
+                if (!scratch && !alone) {
+                    const int64_t at_me = at_part(blockIdx.x, qi);
+                    __stcg(reinterpret_cast<float4 *>(a.part_o + at_me * D) + quad, v);
+                    if (quad == 0) __stcg(reinterpret_cast<float2 *>(a.part_ml) + at_me, make_float2(mm, ll));
+                    continue;
+                }
+                const int r = (q0 + qi) / a.group, h = head * a.group + (q0 + qi) - r * a.group;
+                float sum = ll;
+                if (a.sinks) sum += sm100::ex2(fmaf(__ldg(a.sinks + h), PA_LOG2E, -mm));
+                const float inv = ll == 0.0f ? 0.0f : 1.0f / sum;
+                T *out = static_cast<T *>(a.out.data) + (s.first + r) * a.out.row_stride + h * a.out.head_stride + 4 * quad;
+                if (!a.out_vec) {
+                    store1(out, v.x * inv);
+                    store1(out + 1, v.y * inv);
+                    store1(out + 2, v.z * inv);
+                    store1(out + 3, v.w * inv);
+                } else if constexpr (F32) {
+                    *reinterpret_cast<float4 *>(out) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+                } else {
+                    *reinterpret_cast<uint2 *>(out) = make_uint2(bf16_pair(v.x * inv, v.y * inv), bf16_pair(v.z * inv, v.w * inv));
+                }
+                if (a.lse && quad == 0)
+                    a.lse[(s.first + r) * a.q.heads + h] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * PA_LN2;
+            }
+        };
+        join(false);
+        __syncwarp();
+        if (lane == 0) sm100::mbar_arrive(&sh.part_free);
+        if (!alone) {
+            // The last of the blocks to come (this warp's counter) joins the parts in
+            // their order.
+            unsigned *counter = a.counters + PA_EPILOGUES * c0 + me;
+            unsigned before = 0;
+            __threadfence();
+            __syncwarp();
+            if (lane == 0) before = atomicAdd(counter, 1u);
+            before = __shfl_sync(0xffffffffu, before, 0);
+            if (before == (unsigned)(c1 - c0)) {
+                if (lane == 0) *counter = 0;
+                __threadfence();
+                join(true);
+            }
+        }
+        i += n;
+        at.advance(a, n);
+    }
+}
+
+template <int D, int FORMAT, int NT, bool F32>
 __global__ void __launch_bounds__(PA_THREADS, 1)
     paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                            const __grid_constant__ fo_paged_attention_launch a) {
-    using Shape = PaShape<D>;
+    using Shape = PaShape<D, FORMAT, NT, F32>;
     constexpr int STAGES = PA_STAGES;
     constexpr int TILE = Shape::TILE, HALF = Shape::HALF;
-    constexpr int STEPS = HALF / 16;       // m16 steps of a consumer's half
-    constexpr int KW = D / 16;             // words of a K row per lane
-    constexpr int VW = D / 32;             // words of a V row per lane
-    constexpr int MT = D / 16;             // m16 tiles of the output's dimensions
-    constexpr int QN = 8 / TERMS;          // queries of an n8 tile
-    constexpr int WARP_QUERIES = NT * QN;  // queries of a consumer warp
-    using T = typename std::conditional<TERMS == 2, float, uint16_t>::type;
+    constexpr int STEPS = HALF / 16;   // m16 steps of a consumer's half
+    constexpr int KW = D / 16;         // words of a K row per lane
+    constexpr int KS = D / 32;         // k32 steps over a row's elements
+    constexpr int VS = HALF / 32;      // k32 steps over a half's keys
+    constexpr int MT = D / 16;         // m16 tiles of the output's dimensions
+    constexpr bool I8 = FORMAT == FO_PAGED_I8;
+    constexpr int QT = Shape::QT, PT = Shape::PT;
+    using T = typename std::conditional<F32, float, uint16_t>::type;
     extern __shared__ uint8_t pa_smem[];
     __shared__ PaShared sh;
     uint8_t *tiles = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(pa_smem) + 1023) & ~uintptr_t(1023));
-    float *comb = reinterpret_cast<float *>(tiles + STAGES * Shape::STAGE);
+    float *parts = reinterpret_cast<float *>(tiles + STAGES * Shape::STAGE);
+    uint2 *q_ops = reinterpret_cast<uint2 *>(tiles + STAGES * Shape::STAGE + Shape::PARTS);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int key_groups = PA_CONSUMERS / 2 / a.col_groups;
 
@@ -214,6 +465,10 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             sm100::mbar_init(&sh.full[i], 1);
             sm100::mbar_init(&sh.empty[i], 2 * a.col_groups);
         }
+        sm100::mbar_init(&sh.q_full, PA_EPILOGUES);
+        sm100::mbar_init(&sh.q_free, PA_CONSUMERS);
+        sm100::mbar_init(&sh.part_full, PA_CONSUMERS);
+        sm100::mbar_init(&sh.part_free, PA_EPILOGUES);
         sm100::mbar_fence_init();
         sh.abort = 0;
     }
@@ -229,7 +484,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         pa_scan(work_of(base + tid), sh, all);
         total += all;
     }
-    const long long per = max((total + gridDim.x - 1) / gridDim.x, (long long)key_groups);
+    const long long per = max(pa_share(total, gridDim.x), (long long)key_groups);
     const long long begin = per * blockIdx.x, end = min(begin + per, total);
     if (begin >= end) return;
     for (int64_t base = 0, sum = 0;;) {
@@ -260,7 +515,11 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
 
     if (warp >= PA_CONSUMERS) {
         // ------------------------------------------------------------ producer
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PA_PRODUCER_REGS));
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PA_OTHER_REGS));
+        if (warp >= PA_CONSUMERS + PA_PRODUCERS) {
+            pa_epilogue<D, FORMAT, NT, F32, TILE>(a, sh, at, count, begin, per, warp - PA_CONSUMERS - PA_PRODUCERS, parts, q_ops);
+            return;
+        }
         // Each producer warp issues every PA_PRODUCERS-th tile of the block's: one
         // warp's wait, expectation and two copies take about 500 cycles, more
         // than a tile's share of HBM's time.  Page numbers and scales are fetched
@@ -383,81 +642,49 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PA_CONSUMER_REGS));
     const int g = lane >> 2, t = lane & 3;
     const int col_group = warp % a.col_groups, half = warp / a.col_groups % 2, key_group = warp / a.col_groups / 2;
-    const int kg = pa_key<D>(g), kt0 = pa_key<D>(2 * t), kt1 = pa_key<D>(2 * t + 1);
-    // Byte offsets of this lane's pieces of a K row and of its V rows.
-    const int k_off = D == 128 ? kg * 128 + ((t ^ kg) << 4) : kg * 64 + ((t ^ (kg >> 1 & 3)) << 4);
-    const int v_off0 = D == 128 ? kt0 * 128 + ((g ^ kt0) << 4) : kt0 * 64 + (((g >> 1) ^ (kt0 >> 1 & 3)) << 4) + (g & 1) * 8;
-    const int v_off1 = D == 128 ? kt1 * 128 + ((g ^ kt1) << 4) : kt1 * 64 + (((g >> 1) ^ (kt1 >> 1 & 3)) << 4) + (g & 1) * 8;
+    // This lane's pieces of K rows g and g + 8 of a fragment, and its row of a V
+    // load: row 4 t' + i of a 16 x 16 matrix is the key of the fragment's row 2 t'
+    // + (i & 1) + 8 (i >> 1), as the probabilities' transposition leaves them.
+    const int k0 = pa_key<D>(g), k1 = pa_key<D>(g ^ 4);
+    const int k_off0 = k0 * D + ((D == 128 ? t ^ k0 : t ^ (k0 >> 1 & 3)) << 4);
+    const int k_off1 = (8 + k1) * D + ((D == 128 ? t ^ k1 : t ^ (k1 >> 1 & 3)) << 4);
+    const int v_pair = (lane >> 2 & 3) * 2 + (lane & 1), v_high = lane >> 1 & 1;
+    const int v_key = pa_key<D>(v_high ? v_pair ^ 4 : v_pair);
+    const int v_row = (lane >> 4) * 16 + v_high * 8 + v_key;
+    const uint32_t v_base = v_row * D;
+    const int v_swizzle = D == 128 ? v_key : v_key >> 1 & 3;
     const int page_shift = 31 - __clz(min(page, TILE) / 16);  // log2 of the m16 steps of a page's part of a tile
-    bool ok = true;
 
-    for (int i = 0; i < count;) {
+    for (int i = 0, segment = 0; i < count; segment++) {
         const int n = min(at.left(), count - i);
         const Sequence &s = at.w.s;
-        const int head = at.head(), q0 = at.group() * a.queries;
-        const int n_queries = min(s.n * a.group - q0, a.queries);  // of this unit
-        const int p_first = (int)(s.len - s.n);                    // position of the sequence's first row
-        // The queries as B operands: column g of tile nt, elements 16 t .. 16 t
-        // + 15 (and 64 more, of the second half).
-        uint32_t qf[NT][KW][2];
+        const int n_queries = min(s.n * a.group - at.group() * a.queries, a.queries);  // of this unit
+        const int p_first = (int)(s.len - s.n);  // positions of the sequence's first row and of its last
+        const int p_last = p_first + s.n - 1;
+        // The queries as B operands (a warp's n8 tiles are col_groups apart).
+        const int n_tiles = min(max((n_queries - col_group * 8 + a.col_groups * 8 - 1) / (a.col_groups * 8), 0), NT);
+        uint32_t qf[NT][QT][KS][2];
         float q_scale[NT][2];  // of this lane's columns 2 t, 2 t + 1
         int q_pos[NT][2];
-        auto query_of = [&](int nt, int col) { return col_group * WARP_QUERIES + nt * QN + (TERMS == 2 ? col >> 1 : col); };
+        if (!sm100::mbar_wait(&sh.q_full, segment & 1, &sh.abort, a.err)) return;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            const int qi = query_of(nt, g);
-            float x[KW / 4][16];
-            float top = 0.0f;
-            if (qi < n_queries) {
-                const int r = (q0 + qi) / a.group, hh = (q0 + qi) - r * a.group;
-                const T *q = static_cast<const T *>(a.q.data) + (s.first + r) * a.q.row_stride +
-                             (head * a.group + hh) * a.q.head_stride + 16 * t;
+            const int q_tile = nt * a.col_groups + col_group;
+            const uint2 *from = q_ops + q_tile * (Shape::Q_TILE / 8) + lane;
 #pragma unroll
-                for (int c = 0; c < KW / 4; c++) {
-                    if (a.q_vec) {
-                        load8(q + 64 * c, x[c]);
-                        load8(q + 64 * c + 8, x[c] + 8);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 16; e++) x[c][e] = load1(q + 64 * c + e);
-                    }
-#pragma unroll
-                    for (int e = 0; e < 16; e++) top = fmaxf(top, fabsf(x[c][e]));
-                }
-            } else {
-#pragma unroll
-                for (int c = 0; c < KW / 4; c++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) x[c][e] = 0.0f;
+            for (int x = 0; x < QT * KS; x++) {
+                const uint2 f = nt < n_tiles ? from[32 * x] : make_uint2(0, 0);
+                qf[nt][x / KS][x % KS][0] = f.x;
+                qf[nt][x / KS][x % KS][1] = f.y;
             }
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-            // A power of two near the largest element (1 for none, and within what
-            // both it and its inverse can be).
-            const int e = min(max((int)(__float_as_uint(top) >> 23), 1), 253);
-            const float unit = __uint_as_float((uint32_t)(254 - e) << 23);
-            const float back = __uint_as_float((uint32_t)e << 23) * a.scale * PA_LOG2E;
-#pragma unroll
-            for (int c = 0; c < KW / 4; c++)
-#pragma unroll
-                for (int w = 0; w < 4; w++)
-#pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        float y0 = x[c][4 * w + 2 * h] * unit, y1 = x[c][4 * w + 2 * h + 1] * unit;
-                        uint32_t f = pa_f16x2(y0, y1);
-                        if (TERMS == 2 && (g & 1)) {
-                            const float2 z = f16x2_f32x2(f);
-                            f = pa_f16x2(y0 - z.x, y1 - z.y);
-                        }
-                        qf[nt][4 * c + w][h] = f;
-                    }
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                q_scale[nt][h] = __shfl_sync(0xffffffffu, back, 4 * (2 * t + h));
-                const int qh = query_of(nt, 2 * t + h);
-                q_pos[nt][h] = qh < n_queries ? p_first + (q0 + qh) / a.group : -1;
+                q_scale[nt][h] = sh.q_scale[q_tile * 8 + 2 * t + h];
+                q_pos[nt][h] = sh.q_pos[q_tile * 8 + 2 * t + h];
             }
         }
+        __syncwarp();
+        if (lane == 0) sm100::mbar_arrive(&sh.q_free);
         float m[NT][2], l[NT][2], o[MT][NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
@@ -469,146 +696,97 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                 for (int e = 0; e < 4; e++) o[d][nt][e] = 0.0f;
         }
         // Tiles all of whose positions every row sees need no mask.
-        const int p_last = p_first + s.n - 1;
         const int low_last = a.window > 0 ? max(p_last + 1 - (int)min64(a.window, INT32_MAX / 2), 0) : 0;
+        bool any = false;
 
         int k = i + (key_group - i % key_groups + key_groups) % key_groups;
-        for (; ok && k < i + n; k += key_groups) {
+        for (; k < i + n; k += key_groups) {
             const int slot = k % STAGES;
             // The first position of this warp's half.
             const int pos0 = (at.w.t0 + at.tile + (k - i)) * TILE + half * HALF;
-            ok = sm100::mbar_wait(&sh.full[slot], (k / STAGES) & 1, &sh.abort, a.err);
-            if (!ok) break;
-            if (pos0 > p_last || pos0 + HALF <= at.w.low) {
-                // No row sees any of it.
+            if (!sm100::mbar_wait(&sh.full[slot], (k / STAGES) & 1, &sh.abort, a.err)) return;
+            if (n_tiles == 0 || pos0 > p_last || pos0 + HALF <= at.w.low) {
+                // No row of this warp's sees any of it.
                 __syncwarp();
                 if (lane == 0) sm100::mbar_arrive(&sh.empty[slot]);
                 continue;
             }
+            any = true;
             const uint8_t *kt = tiles + slot * Shape::STAGE + half * HALF * D;
             uint8_t *vt = tiles + slot * Shape::STAGE + Shape::TILE_BYTES + half * HALF * D;
-            // S^T: rows = keys, columns = queries.
-            float c[STEPS][NT][4];
+            // S^T: rows = keys, columns = queries; scores times log2 e.  All products
+            // of one kind are issued before the first is used.
+            float c[STEPS][NT][4], mx[NT][2];
+            const bool masked = pos0 + HALF - 1 > p_first || pos0 < low_last;
+            uint32_t kw[STEPS][2][KW];
 #pragma unroll
             for (int mt = 0; mt < STEPS; mt++) {
-                uint32_t kw[2][KW];
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    const uint8_t *row = kt + (16 * mt + 8 * h) * D;
-                    *reinterpret_cast<uint4 *>(kw[h]) = *reinterpret_cast<const uint4 *>(row + k_off);
-                    if constexpr (D == 128)
-                        *reinterpret_cast<uint4 *>(kw[h] + 4) = *reinterpret_cast<const uint4 *>(row + (k_off ^ 64));
-                }
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) c[mt][nt][e] = 0.0f;
-#pragma unroll
-                for (int w = 0; w < KW; w++) {
-                    uint32_t a0, a1, a2, a3;
-                    pa_codes<FORMAT>(kw[0][w], a0, a2);
-                    pa_codes<FORMAT>(kw[1][w], a1, a3);
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++) pa_mma(c[mt][nt], a0, a1, a2, a3, qf[nt][w][0], qf[nt][w][1]);
+                const uint8_t *row = kt + 16 * mt * D;
+                *reinterpret_cast<uint4 *>(kw[mt][0]) = *reinterpret_cast<const uint4 *>(row + k_off0);
+                *reinterpret_cast<uint4 *>(kw[mt][1]) = *reinterpret_cast<const uint4 *>(row + k_off1);
+                if constexpr (D == 128) {
+                    *reinterpret_cast<uint4 *>(kw[mt][0] + 4) = *reinterpret_cast<const uint4 *>(row + (k_off0 ^ 64));
+                    *reinterpret_cast<uint4 *>(kw[mt][1] + 4) = *reinterpret_cast<const uint4 *>(row + (k_off1 ^ 64));
                 }
             }
-            const bool masked = pos0 + HALF - 1 > p_first || pos0 < low_last;
-            // Scores, times log2 e; FP32 rows have a query's two terms in
-            // neighbouring columns.
-            float mx[NT][2];
+            float ks[STEPS];
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) mx[nt][0] = mx[nt][1] = -INFINITY;
+            for (int mt = 0; mt < STEPS; mt++) ks[mt] = sh.scales[slot][(half * STEPS + mt) >> page_shift];
 #pragma unroll
-            for (int mt = 0; mt < STEPS; mt++) {
-                const float ks = sh.scales[slot][(half * STEPS + mt) >> page_shift];
+            for (int nt = 0; nt < NT; nt++) {
+                if (nt >= n_tiles) break;
+                // int8: an accumulator for each term; e4m3: for each of two terms, or
+                // for each group of three.
+                constexpr int A = I8 ? 3 : 2;
+                typename std::conditional<I8, uint32_t, float>::type acc[STEPS][A][4];
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    if constexpr (TERMS == 2) {
-                        c[mt][nt][0] = c[mt][nt][1] = (c[mt][nt][0] + c[mt][nt][1]) * (ks * q_scale[nt][0]);
-                        c[mt][nt][2] = c[mt][nt][3] = (c[mt][nt][2] + c[mt][nt][3]) * (ks * q_scale[nt][0]);
-                    } else {
+                for (int mt = 0; mt < STEPS; mt++)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) c[mt][nt][e] *= ks * q_scale[nt][e & 1];
+                    for (int x = 0; x < A; x++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) acc[mt][x][e] = I8 ? PA_MAGIC : 0;
+#pragma unroll
+                for (int w = 0; w < KS; w++)
+#pragma unroll
+                    for (int x = 0; x < QT; x++)
+#pragma unroll
+                        for (int mt = 0; mt < STEPS; mt++) {
+                            const uint32_t a0 = kw[mt][0][2 * w], a1 = kw[mt][1][2 * w];
+                            const uint32_t a2 = kw[mt][0][2 * w + 1], a3 = kw[mt][1][2 * w + 1];
+                            const uint32_t b0 = qf[nt][x][w][0], b1 = qf[nt][x][w][1];
+                            if constexpr (!I8) pa_qmma(acc[mt][x / (QT / 2)], a0, a1, a2, a3, b0, b1);
+                            else if (x == 0) pa_imma<true>(acc[mt][0], a0, a1, a2, a3, b0, b1);
+                            else pa_imma<false>(acc[mt][x], a0, a1, a2, a3, b0, b1);
+                        }
+                mx[nt][0] = mx[nt][1] = -INFINITY;
+#pragma unroll
+                for (int mt = 0; mt < STEPS; mt++) {
+                    float (&sc)[4] = c[mt][nt];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        if constexpr (I8) {
+                            const float hi = __uint_as_float(acc[mt][0][e]) - PA_MAGIC_F;
+                            const float mid = __uint_as_float(acc[mt][1][e]) - PA_MAGIC_F;
+                            const float lo = __uint_as_float(acc[mt][A - 1][e]) - PA_MAGIC_F;
+                            sc[e] = fmaf(hi, 65536.0f, fmaf(mid, 256.0f, lo));
+                        } else {
+                            sc[e] = fmaf(acc[mt][1][e], F32 ? 1.0f / PA_GROUP : 1.0f, acc[mt][0][e]);
+                        }
+                        sc[e] *= ks[mt] * q_scale[nt][e & 1];
                     }
                     if (masked) {
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
-                            const int pos = pos0 + 16 * mt + kg + (e >> 1) * 8, p = q_pos[nt][e & 1];
+                            const int pos = pos0 + 16 * mt + (e < 2 ? k0 : 8 + k1), p = q_pos[nt][e & 1];
                             const bool seen = pos <= p && (a.window == 0 || pos > p - a.window);
-                            if (!seen) c[mt][nt][e] = -INFINITY;
+                            if (!seen) sc[e] = -INFINITY;
                         }
                     }
 #pragma unroll
-                    for (int e = 0; e < 4; e++) mx[nt][e & 1] = fmaxf(mx[nt][e & 1], c[mt][nt][e]);
+                    for (int e = 0; e < 4; e++) mx[nt][e & 1] = fmaxf(mx[nt][e & 1], sc[e]);
                 }
             }
-            float alpha[NT][2];
-            bool moved = false;
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    float x = mx[nt][h];
-                    if (TERMS == 2 && h == 1) {
-                        mx[nt][1] = mx[nt][0];
-                        m[nt][1] = m[nt][0];
-                        alpha[nt][1] = alpha[nt][0];
-                        continue;
-                    }
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                    x = fmaxf(x, m[nt][h]);
-                    moved |= x != m[nt][h];
-                    // While nothing has been seen the maximum stays -infinity and
-                    // every probability below is 0.
-                    alpha[nt][h] = x == -INFINITY ? 1.0f : sm100::ex2(m[nt][h] - x);
-                    m[nt][h] = x;
-                    mx[nt][h] = x == -INFINITY ? 0.0f : x - PA_P_BITS;
-                }
-            if (TERMS == 2) {
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    mx[nt][1] = mx[nt][0];
-                    m[nt][1] = m[nt][0];
-                    alpha[nt][1] = alpha[nt][0];
-                }
-            }
-            if (__any_sync(0xffffffffu, moved)) {
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-#pragma unroll
-                    for (int h = 0; h < 2; h++) l[nt][h] *= alpha[nt][h];
-#pragma unroll
-                    for (int d = 0; d < MT; d++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) o[d][nt][e] *= alpha[nt][e & 1];
-                }
-            }
-            // Probabilities, transposed into B operands: rows = keys of V.
-            uint32_t pf[STEPS][NT][2];
-#pragma unroll
-            for (int mt = 0; mt < STEPS; mt++)
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                    for (int r = 0; r < 2; r++) {
-                        uint32_t f;
-                        if constexpr (TERMS == 2) {
-                            const float p = sm100::ex2(c[mt][nt][2 * r] - mx[nt][0]);
-                            l[nt][0] += p;
-                            const uint32_t hi = pa_f16x2(p, 0.0f);
-                            f = pa_f16x2(p, p - f16x2_f32x2(hi).x);
-                        } else {
-                            const float p0 = sm100::ex2(c[mt][nt][2 * r] - mx[nt][0]);
-                            const float p1 = sm100::ex2(c[mt][nt][2 * r + 1] - mx[nt][1]);
-                            l[nt][0] += p0;
-                            l[nt][1] += p1;
-                            f = pa_f16x2(p0, p1);
-                        }
-                        pf[mt][nt][r] = pa_transpose(f);
-                    }
-            if constexpr (FORMAT == FO_PAGED_E4M3) {
+            if constexpr (!I8) {
                 // Rows beyond the sequence, or of pages that no row sees, may hold any
                 // bytes: an FP8 NaN times a probability of 0 would be NaN.
                 const int lo_row = max(at.w.low / page * page - pos0, 0), hi_row = (int)min64(s.len - pos0, HALF);
@@ -617,182 +795,192 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                         const int row = x / (D / 16);
                         if (row < lo_row || row >= hi_row) reinterpret_cast<uint4 *>(vt)[x] = make_uint4(0, 0, 0, 0);
                     }
+                    sm100::fence_proxy_async_smem();  // these before the next copy
                     __syncwarp();
                 }
             }
-            float acc[MT][NT][4];
+            // The values, while the maxima and probabilities are worked out.
+            const uint32_t v_at = sm100::smem_u32(vt) + v_base;
+            uint32_t va[MT][VS][4];
 #pragma unroll
             for (int d = 0; d < MT; d++)
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++)
+                for (int v = 0; v < VS; v++) pa_load_transposed(va[d][v], v_at + 32 * v * D + ((d ^ v_swizzle) << 4));
+            // The half's own maximum, which its probabilities are relative to, and
+            // the running one: alpha brings the sums so far to it, beta the half's.
+            float alpha[NT][2], beta[NT][2];
+            bool moved = false;
 #pragma unroll
-                    for (int e = 0; e < 4; e++) acc[d][nt][e] = 0.0f;
+            for (int nt = 0; nt < NT; nt++) {
+                if (nt >= n_tiles) break;
 #pragma unroll
-            for (int kk = 0; kk < STEPS; kk++) {
-                uint32_t va[VW], vb[VW], vc[VW], vd[VW];
-                const uint8_t *row = vt + 16 * kk * D;
-                if constexpr (D == 128) {
-                    *reinterpret_cast<uint4 *>(va) = *reinterpret_cast<const uint4 *>(row + v_off0);
-                    *reinterpret_cast<uint4 *>(vb) = *reinterpret_cast<const uint4 *>(row + v_off1);
-                    *reinterpret_cast<uint4 *>(vc) = *reinterpret_cast<const uint4 *>(row + 8 * D + v_off0);
-                    *reinterpret_cast<uint4 *>(vd) = *reinterpret_cast<const uint4 *>(row + 8 * D + v_off1);
-                } else {
-                    *reinterpret_cast<uint2 *>(va) = *reinterpret_cast<const uint2 *>(row + v_off0);
-                    *reinterpret_cast<uint2 *>(vb) = *reinterpret_cast<const uint2 *>(row + v_off1);
-                    *reinterpret_cast<uint2 *>(vc) = *reinterpret_cast<const uint2 *>(row + 8 * D + v_off0);
-                    *reinterpret_cast<uint2 *>(vd) = *reinterpret_cast<const uint2 *>(row + 8 * D + v_off1);
+                for (int h = 0; h < 2; h++) {
+                    float x = mx[nt][h];
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                    const float top = fmaxf(x, m[nt][h]);
+                    // While nothing has been seen the maximum stays -infinity and
+                    // every probability is 0.
+                    alpha[nt][h] = top == -INFINITY ? 1.0f : sm100::ex2(m[nt][h] - top);
+                    beta[nt][h] = x == -INFINITY ? 0.0f : sm100::ex2(x - top);
+                    moved |= top != m[nt][h];
+                    m[nt][h] = top;
+                    mx[nt][h] = x == -INFINITY ? 0.0f : x;
                 }
+            }
+            // Probabilities' terms, transposed into B operands.
+            uint32_t pf[NT][PT][VS][2];
 #pragma unroll
-                for (int w = 0; w < VW; w++)
+            for (int nt = 0; nt < NT; nt++) {
+                if (nt >= n_tiles) break;
+                float sum0 = 0.0f, sum1 = 0.0f;
 #pragma unroll
-                    for (int b = 0; b < 2; b++) {
-                        // Dimensions 4 w + 2 b, 4 w + 2 b + 1 of the lane's, two keys each.
-                        uint32_t a0, a1, a2, a3;
-                        pa_codes<FORMAT>(__byte_perm(va[w], vb[w], b ? 0x7362 : 0x5140), a0, a1);
-                        pa_codes<FORMAT>(__byte_perm(vc[w], vd[w], b ? 0x7362 : 0x5140), a2, a3);
+                for (int mt = 0; mt < STEPS; mt++) {
+                    constexpr int PAIRS = (PT + 1) / 2;
+                    uint32_t tr[PAIRS][2];  // two terms of the keys of rows 0 .. 7, and of 8 .. 15
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt++)
-                            pa_mma(acc[2 * w + b][nt], a0, a1, a2, a3, pf[kk][nt][0], pf[kk][nt][1]);
+                    for (int r = 0; r < 2; r++) {
+                        float p0 = sm100::ex2(c[mt][nt][2 * r] - mx[nt][0]);
+                        float p1 = sm100::ex2(c[mt][nt][2 * r + 1] - mx[nt][1]);
+                        sum0 += p0;
+                        sum1 += p1;
+                        if constexpr (I8) {
+                            // 2^23 + p times its largest integer: the bytes of that integer.
+                            constexpr float TOP = F32 ? 8388607.0f : 65535.0f;
+                            const uint32_t u0 = __float_as_uint(fmaf(p0, TOP, 8388608.0f));
+                            const uint32_t u1 = __float_as_uint(fmaf(p1, TOP, 8388608.0f));
+                            tr[0][r] = pa_transpose(__byte_perm(u0, u1, 0x5410));
+                            if constexpr (F32) tr[1][r] = pa_transpose(__byte_perm(u0, u1, 0x7632));
+                        } else {
+                            p0 *= 256.0f;
+                            p1 *= 256.0f;
+#pragma unroll
+                            for (int x = 0; x < PAIRS; x++) {
+                                const uint32_t x0 = pa_e4m3x2(p0, p1);
+                                if (2 * x + 1 == 3) p0 *= PA_GROUP, p1 *= PA_GROUP;
+                                const uint32_t x1 = 2 * x + 1 < PT ? pa_e4m3x2(p0, p1) : 0;
+                                tr[x][r] = pa_transpose(__byte_perm(x0, x1, 0x5140));
+                            }
+                        }
                     }
-                if (kk == STEPS - 1 || ((half * STEPS + kk + 1) & ((1 << page_shift) - 1)) == 0) {
-                    // The end of a page: its scale.
-                    const float vs = sh.scales[slot][8 + ((half * STEPS + kk) >> page_shift)];
+#pragma unroll
+                    for (int x = 0; x < PT; x++)
+                        pf[nt][x][mt / 2][mt % 2] = __byte_perm(tr[x / 2][0], tr[x / 2][1], x % 2 ? 0x7531 : 0x6420);
+                }
+                l[nt][0] = fmaf(sum0, beta[nt][0], l[nt][0] * alpha[nt][0]);
+                l[nt][1] = fmaf(sum1, beta[nt][1], l[nt][1] * alpha[nt][1]);
+            }
+            if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    if (nt >= n_tiles) break;
 #pragma unroll
                     for (int d = 0; d < MT; d++)
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                o[d][nt][e] = fmaf(acc[d][nt][e], vs, o[d][nt][e]);
-                                acc[d][nt][e] = 0.0f;
-                            }
+                        for (int e = 0; e < 4; e++) o[d][nt][e] *= alpha[nt][e & 1];
                 }
             }
-            if constexpr (FORMAT == FO_PAGED_E4M3) sm100::fence_proxy_async_smem();  // zeros before the next copy
+            // O^T: rows = dimensions, columns = queries; two m16 tiles of dimensions
+            // at a time, each page's sum times its scale.
+            constexpr float PART = I8 ? (F32 ? 1.0f / 8388607.0f : 1.0f / 65535.0f) : 1.0f / 256.0f;
+            // The products over one page's keys, the steps [from, to) of 16; WHOLE:
+            // all of the half's.
+            auto page_sum = [&](auto whole, int from, int to) {
+                constexpr bool WHOLE = decltype(whole)::value;
+                const float vs = sh.scales[slot][8 + ((half * STEPS + from) >> page_shift)] * PART;
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    if (nt >= n_tiles) break;
+                    const float f0 = vs * beta[nt][0], f1 = vs * beta[nt][1];
+                    // int8: an accumulator for each term; e4m3: for each of three
+                    // terms, or for each group of three.
+                    constexpr int A = I8 ? PT : F32 ? 2 : 3, PER = I8 ? 1 : PT / A;
+#pragma unroll
+                    for (int d2 = 0; d2 < MT; d2 += 2) {
+                        typename std::conditional<I8, uint32_t, float>::type acc[2][A][4];
+#pragma unroll
+                        for (int d = 0; d < 2; d++)
+#pragma unroll
+                            for (int x = 0; x < A; x++)
+#pragma unroll
+                                for (int e = 0; e < 4; e++) acc[d][x][e] = I8 ? PA_MAGIC : 0;
+#pragma unroll
+                        for (int v = 0; v < VS; v++) {
+                            const bool first = WHOLE || (2 * v >= from && 2 * v < to);
+                            const bool second = WHOLE || (2 * v + 1 >= from && 2 * v + 1 < to);
+                            if (!first && !second) continue;
+#pragma unroll
+                            for (int x = 0; x < PT; x++) {
+                                const uint32_t b0 = first ? pf[nt][x][v][0] : 0u, b1 = second ? pf[nt][x][v][1] : 0u;
+#pragma unroll
+                                for (int d = 0; d < 2; d++) {
+                                    const uint32_t (&r)[4] = va[d2 + d][v];
+                                    if constexpr (I8) pa_imma<false>(acc[d][x], r[0], r[1], r[2], r[3], b0, b1);
+                                    else pa_qmma(acc[d][x / PER], r[0], r[1], r[2], r[3], b0, b1);
+                                }
+                            }
+                        }
+#pragma unroll
+                        for (int d = 0; d < 2; d++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                float sum;
+                                if constexpr (I8) {
+                                    // Term 0 is the lowest byte.
+                                    sum = fmaf(__uint_as_float(acc[d][1][e]) - PA_MAGIC_F, 256.0f,
+                                               __uint_as_float(acc[d][0][e]) - PA_MAGIC_F);
+                                    if constexpr (F32)
+                                        sum = fmaf(__uint_as_float(acc[d][A - 1][e]) - PA_MAGIC_F, 65536.0f, sum);
+                                } else if constexpr (F32) {
+                                    sum = fmaf(acc[d][1][e], 1.0f / PA_GROUP, acc[d][0][e]);
+                                } else {
+                                    sum = acc[d][0][e] + (acc[d][1][e] + acc[d][A - 1][e]);
+                                }
+                                o[d2 + d][nt][e] = fmaf(sum, e & 1 ? f1 : f0, o[d2 + d][nt][e]);
+                            }
+                    }
+                }
+            };
+            if ((1 << page_shift) >= STEPS)
+                page_sum(std::true_type{}, 0, STEPS);
+            else
+                for (int from = 0; from < STEPS; from += 1 << page_shift)
+                    page_sum(std::false_type{}, from, from + (1 << page_shift));
             __syncwarp();
             if (lane == 0) sm100::mbar_arrive(&sh.empty[slot]);
         }
 
-        // Join the key groups' parts, an n8 tile at a time.
+        // This warp's part, for the epilogue warps to join.  A part that is not a
+        // number (a query that is not finite, a page number outside the pool)
+        // makes its queries' outputs NaN.
+        if (segment > 0 && !sm100::mbar_wait(&sh.part_free, (segment - 1) & 1, &sh.abort, a.err)) return;
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++)
+        for (int nt = 0; nt < NT; nt++) {
+            if (nt >= n_tiles) break;
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                float x = TERMS == 2 ? l[nt][0] : l[nt][h];
+                float x = l[nt][h];
                 x += __shfl_xor_sync(0xffffffffu, x, 4);
                 x += __shfl_xor_sync(0xffffffffu, x, 8);
                 x += __shfl_xor_sync(0xffffffffu, x, 16);
                 if (g == 0) {
-                    sh.ml[warp][8 * nt + 2 * t + h][0] = ok ? m[nt][h] : NAN;
+                    const bool good = x == x && q_scale[nt][h] == q_scale[nt][h];
+                    sh.ml[warp][8 * nt + 2 * t + h][0] = good ? m[nt][h] : NAN;
                     sh.ml[warp][8 * nt + 2 * t + h][1] = x;
                 }
-            }
-        // The unit's tiles in the line, and the blocks that share it.
-        const long long unit_begin = begin + i - at.tile, unit_end = unit_begin + at.w.tiles;
-        const int c0 = (int)(unit_begin / per), c1 = (int)((unit_end - 1) / per);
-        const int64_t part = 2 * (int64_t)blockIdx.x + ((int)blockIdx.x == c0 ? 1 : 0);
-        auto write_out = [&](int qi, int quad, float4 v, float mm, float ll) {
-            const int r = (q0 + qi) / a.group, h = head * a.group + (q0 + qi) - r * a.group;
-            float sum = ll;
-            if (a.sinks) sum += sm100::ex2(fmaf(__ldg(a.sinks + h), PA_LOG2E, PA_P_BITS - mm));
-            const float inv = ll == 0.0f ? 0.0f : 1.0f / sum;
-            T *out = static_cast<T *>(a.out.data) + (s.first + r) * a.out.row_stride + h * a.out.head_stride + 4 * quad;
-            if (a.out_vec) {
-                if constexpr (TERMS == 2)
-                    *reinterpret_cast<float4 *>(out) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-                else
-                    *reinterpret_cast<uint2 *>(out) = make_uint2(bf16_pair(v.x * inv, v.y * inv), bf16_pair(v.z * inv, v.w * inv));
-            } else {
-                store1(out, v.x * inv);
-                store1(out + 1, v.y * inv);
-                store1(out + 2, v.z * inv);
-                store1(out + 3, v.w * inv);
-            }
-            if (a.lse && quad == 0)
-                a.lse[(s.first + r) * a.q.heads + h] = ll == 0.0f ? -INFINITY : (mm + log2f(ll) - PA_P_BITS) * PA_LN2;
-        };
+                if (any) {
+                    float *col = parts + ((warp * NT + nt) * 8 + 2 * t + h) * Shape::PART_LD + g;
 #pragma unroll
-        for (int pass = 0; pass < NT * (D / 64); pass++) {
-            // An n8 tile's columns, 64 dimensions of them.
-            const int nt = pass / (D / 64), d64 = pass % (D / 64);
-            if (D == 64 || g / 4 == d64) {
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    float *col = comb + (warp * 8 + 2 * t + h) * Shape::COMB_LD + (D / 8) * g - 64 * d64;
-#pragma unroll
-                    for (int d = 0; d < MT; d += 2)
-                        *reinterpret_cast<float4 *>(col + 2 * d) =
-                            make_float4(o[d][nt][h], o[d][nt][2 + h], o[d + 1][nt][h], o[d + 1][nt][2 + h]);
-                }
-            }
-            pa_consumers_sync();
-            for (int x = tid; x < a.col_groups * QN * 16; x += 32 * PA_CONSUMERS) {
-                const int quad = x % 16, cq = x / 16;
-                const int cg = cq / QN, col = (cq - cg * QN) * TERMS;
-                const int qi = query_of(nt, 0) + (cg - col_group) * WARP_QUERIES + col / TERMS;
-                if (qi >= n_queries) continue;
-                float mm = -INFINITY, ll = 0.0f;
-                bool lost = false;
-                for (int w = cg; w < PA_CONSUMERS; w += a.col_groups) {
-                    const float mw = sh.ml[w][8 * nt + col][0];
-                    lost |= mw != mw;
-                    mm = fmaxf(mm, mw);
-                }
-                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                for (int w = cg; w < PA_CONSUMERS; w += a.col_groups) {
-                    const float mw = sh.ml[w][8 * nt + col][0];
-                    if (mw == -INFINITY) continue;
-                    const float f = sm100::ex2(mw - mm);
-                    ll = fmaf(sh.ml[w][8 * nt + col][1], f, ll);
-                    const float *from = comb + (w * 8 + col) * Shape::COMB_LD + 4 * quad;
-                    float4 u = *reinterpret_cast<const float4 *>(from);
-                    if constexpr (TERMS == 2) {
-                        const float4 u1 = *reinterpret_cast<const float4 *>(from + Shape::COMB_LD);
-                        u = make_float4(u.x + u1.x, u.y + u1.y, u.z + u1.z, u.w + u1.w);
+                    for (int d = 0; d < MT; d++) {
+                        col[16 * d] = o[d][nt][h];
+                        col[16 * d + 8] = o[d][nt][2 + h];
                     }
-                    v = make_float4(fmaf(u.x, f, v.x), fmaf(u.y, f, v.y), fmaf(u.z, f, v.z), fmaf(u.w, f, v.w));
-                }
-                if (lost) ll = NAN;
-                const int at_quad = 16 * d64 + quad;
-                if (c0 == c1) {
-                    write_out(qi, at_quad, v, mm, ll);
-                } else {
-                    *reinterpret_cast<float4 *>(a.part_o + (part * a.queries + qi) * D + 4 * at_quad) = v;
-                    if (at_quad == 0)
-                        *reinterpret_cast<float2 *>(a.part_ml + (part * a.queries + qi) * 2) = make_float2(mm, ll);
                 }
             }
-            pa_consumers_sync();
         }
-        if (c0 != c1) {
-            // The last block to come joins the parts in their order.
-            if (tid == 0) {
-                __threadfence();
-                sh.last = atomicAdd(a.counters + c0, 1u) == (unsigned)(c1 - c0);
-                if (sh.last) a.counters[c0] = 0;
-                __threadfence();
-            }
-            pa_consumers_sync();
-            if (sh.last) {
-                for (int x = tid; x < n_queries * (D / 4); x += 32 * PA_CONSUMERS) {
-                    const int quad = x % (D / 4), qi = x / (D / 4);
-                    auto at_part = [&](int cta) { return ((2 * (int64_t)cta + (cta == c0 ? 1 : 0)) * a.queries + qi); };
-                    float mm = -INFINITY, ll = 0.0f;
-                    for (int cta = c0; cta <= c1; cta++)
-                        mm = fmaxf(mm, __ldcg(reinterpret_cast<const float2 *>(a.part_ml) + at_part(cta)).x);
-                    float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    for (int cta = c0; cta <= c1; cta++) {
-                        const float2 ml = __ldcg(reinterpret_cast<const float2 *>(a.part_ml) + at_part(cta));
-                        const float4 u = __ldcg(reinterpret_cast<const float4 *>(a.part_o + at_part(cta) * D) + quad);
-                        const float f = ml.x == -INFINITY ? 0.0f : sm100::ex2(ml.x - mm);
-                        ll = fmaf(ml.y, f, ll);
-                        v = make_float4(fmaf(u.x, f, v.x), fmaf(u.y, f, v.y), fmaf(u.z, f, v.z), fmaf(u.w, f, v.w));
-                    }
-                    write_out(qi, quad, v, mm, ll);
-                }
-            }
-            pa_consumers_sync();
-        }
+        __syncwarp();
+        if (lane == 0) sm100::mbar_arrive(&sh.part_full);
         i += n;
         at.advance(a, n);
     }
@@ -825,16 +1013,18 @@ bool pa_map(CUtensorMap *map, const void *codes, const fo_paged_kv &kv) {
               CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int D, int FORMAT, int NT, int TERMS>
+template <int D, int FORMAT, int NT, bool F32>
 cudaError_t launch_attention(const fo_paged_attention_launch &a, unsigned grid, cudaStream_t stream) {
-    auto *kernel = paged_attention_kernel<D, FORMAT, NT, TERMS>;
+    auto *kernel = paged_attention_kernel<D, FORMAT, NT, F32>;
+    using Shape = PaShape<D, FORMAT, NT, F32>;
     // The attribute belongs to each device's context: set once per device.
     static std::atomic<unsigned long long> configured{0};
     int dev = 0;
     cudaGetDevice(&dev);
     const unsigned long long bit = 1ull << (dev & 63);
     if (!(configured.load() & bit)) {
-        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, PaShape<D>::SMEM);
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             Shape::smem(4 * NT));
         if (e != cudaSuccess) return e;
         // The kernel's register split is only sound at the launch count that it
         // was written for.
@@ -846,15 +1036,19 @@ cudaError_t launch_attention(const fo_paged_attention_launch &a, unsigned grid, 
     }
     CUtensorMap k_map, v_map;
     if (!pa_map(&k_map, a.kv.k_codes, a.kv) || !pa_map(&v_map, a.kv.v_codes, a.kv)) return cudaErrorNotSupported;
-    kernel<<<grid, PA_THREADS, PaShape<D>::SMEM, stream>>>(k_map, v_map, a);
+    kernel<<<grid, PA_THREADS, Shape::smem(a.queries / 8), stream>>>(k_map, v_map, a);
     return cudaGetLastError();
 }
 
 template <int D, int FORMAT>
 cudaError_t launch_attention(const fo_paged_attention_launch &a, int nt, unsigned grid, cudaStream_t stream) {
-    if (a.q.dtype == FO_DT_F32)
-        return nt == 1 ? launch_attention<D, FORMAT, 1, 2>(a, grid, stream) : launch_attention<D, FORMAT, 2, 2>(a, grid, stream);
-    return nt == 1 ? launch_attention<D, FORMAT, 1, 1>(a, grid, stream) : launch_attention<D, FORMAT, 2, 1>(a, grid, stream);
+    if (a.q.dtype == FO_DT_F32) {
+        if constexpr (FORMAT == FO_PAGED_I8)
+            if (nt == 2) return launch_attention<D, FORMAT, 2, true>(a, grid, stream);
+        return launch_attention<D, FORMAT, 1, true>(a, grid, stream);
+    }
+    return nt == 1 ? launch_attention<D, FORMAT, 1, false>(a, grid, stream)
+                   : launch_attention<D, FORMAT, 2, false>(a, grid, stream);
 }
 
 }  // namespace fo
@@ -863,24 +1057,25 @@ extern "C" cudaError_t fo_launch_paged_attention(const fo_paged_attention_launch
     fo_paged_attention_launch a = *args;
     if (a.batch.total_rows <= 0) return cudaSuccess;
     a.group = a.q.heads / a.kv.n_kv_heads;
-    // Columns of the products: a query's, times its terms.  A warp takes 8, or
-    // 16; beyond that 2 or 4 warps share each tile; beyond that a (sequence, KV
-    // head) is read once for each group of queries.
-    const int terms = a.q.dtype == FO_DT_F32 ? 2 : 1;
-    const int64_t columns = a.batch.max_rows * a.group * terms;
-    const int nt = columns <= 8 ? 1 : 2;
-    a.col_groups = columns <= 16 ? 1 : columns <= 32 ? 2 : 4;
-    a.queries = 8 * nt * a.col_groups / terms;
-    a.evict_first = columns <= 64;
+    // A warp takes the queries of one n8 tile, or two (six terms of an FP32 query
+    // leave registers for one); beyond that 2 or 4 warps share each half of a
+    // tile; beyond that a (sequence, KV head) is read once for each group of
+    // queries.
+    const int64_t queries = a.batch.max_rows * a.group;
+    const int most_nt = a.q.dtype == FO_DT_F32 && a.kv.format == FO_PAGED_E4M3 ? 1 : 2;
+    const int nt = queries <= 8 ? 1 : most_nt;
+    a.col_groups = queries <= 8 * nt ? 1 : queries <= 16 * nt ? 2 : 4;
+    a.queries = 8 * nt * a.col_groups;
+    a.evict_first = queries <= a.queries;
     auto aligned = [](const fo_rows &r, int64_t bytes) {
         const int64_t unit = bytes / (r.dtype == FO_DT_F32 ? 4 : 2);
         return reinterpret_cast<uintptr_t>(r.data) % bytes == 0 && r.row_stride % unit == 0 && r.head_stride % unit == 0;
     };
     a.q_vec = aligned(a.q, 16);
-    a.out_vec = aligned(a.out, terms == 2 ? 16 : 8);
+    a.out_vec = aligned(a.out, a.q.dtype == FO_DT_F32 ? 16 : 8);
     // No more blocks than the most tiles there can be for, one for each group
     // of consumer warps.
-    const int64_t most = a.batch.n_seqs * a.kv.n_kv_heads * ((columns / terms + a.queries - 1) / a.queries) *
+    const int64_t most = a.batch.n_seqs * a.kv.n_kv_heads * ((queries + a.queries - 1) / a.queries) *
                          ((a.batch.table_stride * a.kv.page_size * a.kv.head_dim + 8191) / 8192);
     const int64_t groups = fo::PA_CONSUMERS / 2 / a.col_groups;
     const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(sms, (most + groups - 1) / groups));
