@@ -26,21 +26,24 @@
 // or hand on the result, so that the consumers go from one to the next
 // without waiting for any of that.
 //
-// The codes themselves are the A operands of the tensor instructions: a
-// consumer computes S^T = K Q^T and O^T += V^T P^T on m16n8k32 products of
-// int8 (exact, 32-bit sums) or of e4m3 (exact products, FP32 sums), keys as
-// they lie, values through transposing shared-memory loads, so that nothing
-// of the cache is converted or rounded; a scale multiplies a finished sum.
-// Queries and probabilities are split into 8-bit terms, one product each.
-// int8: a query is a 23-bit integer relative to a power of two near its
-// largest element (three bytes), a probability one of 16 bits (BF16 rows, whose
-// output has 8) or 23 (FP32 rows) relative to its tile's largest.  e4m3: terms
-// of 4 bits, each what the ones before it leave: two for a BF16 query, which
-// hold it exactly, three for its probabilities (12 bits), twice three for
-// FP32 rows.  The 5th-generation MMA would want the few queries' side padded
-// and every score and output moved through TMEM; at a decode's few columns
-// these instructions take a small part of the time that HBM needs for a
-// tile.  Maxima, sums and outputs are FP32.
+// The codes are the A operands of tensor instructions, keys as they lie, values
+// through transposing shared-memory loads: a consumer computes S^T = K Q^T and
+// O^T += V^T P^T.  Nothing of the cache is rounded; a scale multiplies a
+// finished sum.
+//   int8: m16n8k32 products of bytes with exact 32-bit sums.  A query is a
+//   23-bit integer relative to a power of two near its largest element, three
+//   bytes; a probability one of 16 bits (BF16 rows, whose output has 8), or 23
+//   (FP32 rows), relative to its tile's largest; a product for each byte.
+//   e4m3: m16n8k16 products of FP16, which holds every e4m3 number (the 8-bit
+//   instruction is no faster than converting here).  A query is relative to a
+//   power of two near its largest element: BF16's 8 bits exactly, FP32 as the
+//   sum of two FP16 (22 bits); a probability, times 2^10 so that FP16 holds
+//   those down to 2^-24 of the largest at full precision, is one FP16 (11 bits)
+//   or two.
+// The 5th-generation MMA would want the few queries' side padded and every
+// score and output moved through TMEM; at a decode's few columns these
+// instructions take a small part of the time that HBM needs for a tile.
+// Maxima, sums and outputs are FP32.
 #include "paged.cuh"
 #include "sm100.cuh"
 
@@ -72,12 +75,16 @@ struct PaShape {
     static constexpr int TILE = TILE_BYTES / D;    // positions
     static constexpr int HALF = TILE / 2;          // a consumer warp's
     static constexpr int STAGE = 2 * TILE_BYTES;
-    static constexpr int QT = FORMAT == FO_PAGED_I8 ? 3 : F32 ? 6 : 2;                // a query's terms
-    static constexpr int PT = FORMAT == FO_PAGED_I8 ? (F32 ? 3 : 2) : F32 ? 6 : 3;    // a probability's
+    static constexpr bool I8 = FORMAT == FO_PAGED_I8;
+    static constexpr int QT = I8 ? 3 : F32 ? 2 : 1;          // a query's terms
+    static constexpr int PT = I8 ? (F32 ? 3 : 2) : QT;       // a probability's
+    static constexpr int KQ = I8 ? D / 32 : D / 16;          // k steps over a row's elements
     static constexpr int PART_LD = D + 4;          // a column of a consumer's part, in floats
     static constexpr int PARTS = PA_CONSUMERS * NT * 8 * PART_LD * 4;
-    static constexpr int Q_TILE = QT * (D / 32) * 32 * 8;  // an n8 tile of queries as operands
-    static int smem(int q_tiles) { return 1024 + PA_STAGES * STAGE + PARTS + q_tiles * Q_TILE; }
+    // Warps that can share a half of a tile: four, where their queries' operands fit.
+    static constexpr int MAX_GROUPS = !I8 && F32 && D == 128 ? 2 : 4;
+    static constexpr int Q_TILE = QT * KQ * 32 * 8;  // an n8 tile of queries as operands
+    static constexpr int smem(int q_tiles) { return 1024 + PA_STAGES * STAGE + PARTS + q_tiles * Q_TILE; }
 };
 
 // The key of eight that a fragment's row g stands for: such that a K
@@ -107,9 +114,10 @@ __device__ __forceinline__ void pa_imma(uint32_t (&c)[4], uint32_t a0, uint32_t 
             : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
             : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void pa_qmma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
+// The same with FP16, k16.
+__device__ __forceinline__ void pa_hmma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                         uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
@@ -127,18 +135,11 @@ __device__ __forceinline__ uint32_t pa_transpose(uint32_t x) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-// Two floats as e4m3 (nearest even), lo in the low byte, and what is left.
-__device__ __forceinline__ uint32_t pa_e4m3x2(float &lo, float &hi) {
+__device__ __forceinline__ uint32_t pa_f16x2(float lo, float hi) {
     uint32_t r;
-    asm("{\n\t.reg .b16 x;\n\tcvt.rn.satfinite.e4m3x2.f32 x, %2, %1;\n\tcvt.u32.u16 %0, x;\n\t}"
-        : "=r"(r)
-        : "f"(lo), "f"(hi));
-    const float2 back = f16x2_f32x2(e4m3x2_f16x2(r));
-    lo -= back.x;
-    hi -= back.y;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
-constexpr float PA_GROUP = 4096.0f;  // e4m3 terms 4 .. 6 stand for 2^-12 of their value
 
 // A sequence's share of the line of tiles.
 struct PaWork {
@@ -234,7 +235,7 @@ __device__ __forceinline__ void pa_epilogue(const fo_paged_attention_launch &a, 
     using Shape = PaShape<D, FORMAT, NT, F32>;
     using T = typename std::conditional<F32, float, uint16_t>::type;
     constexpr bool I8 = FORMAT == FO_PAGED_I8;
-    constexpr int KS = D / 32, QT = Shape::QT;
+    constexpr int QT = Shape::QT, KQ = Shape::KQ;
     const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 
     // A unit's queries as B operands: column g of an n8 tile, this lane's elements
@@ -251,10 +252,10 @@ __device__ __forceinline__ void pa_epilogue(const fo_paged_attention_launch &a, 
                 q = static_cast<const T *>(a.q.data) + (u.w.s.first + r) * a.q.row_stride +
                     (head * a.group + (q0 + qi) - r * a.group) * a.q.head_stride + 16 * t;
             }
-            float x[KS / 2][16], top = 0.0f;
+            float x[D / 64][16], top = 0.0f;
             bool finite = true;
 #pragma unroll
-            for (int c = 0; c < KS / 2; c++) {
+            for (int c = 0; c < D / 64; c++) {
                 if (!q) {
 #pragma unroll
                     for (int e = 0; e < 16; e++) x[c][e] = 0.0f;
@@ -267,7 +268,7 @@ __device__ __forceinline__ void pa_epilogue(const fo_paged_attention_launch &a, 
                 }
             }
 #pragma unroll
-            for (int c = 0; c < KS / 2; c++)
+            for (int c = 0; c < D / 64; c++)
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
                     top = fmaxf(top, fabsf(x[c][e]));
@@ -277,12 +278,12 @@ __device__ __forceinline__ void pa_epilogue(const fo_paged_attention_launch &a, 
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const unsigned all_finite = __ballot_sync(0xffffffffu, finite);
             // A power of two near the largest element brings it to [2^21, 2^22)
-            // (int8) or [2^7, 2^8) (e4m3); in two factors, so that FP32's whole
-            // range of exponents can be brought there.
+            // (int8) or [1, 2) (e4m3); in two factors, so that FP32's whole range
+            // of exponents can be brought there.
             const int e = max((int)(__float_as_uint(top) >> 23), 1);
-            const float up = I8 ? 2097152.0f : 128.0f;
+            const float up = I8 ? 2097152.0f : 1.0f;
             const float inv0 = __uint_as_float((uint32_t)(254 - (e + 1) / 2 - 63) << 23);
-            const float inv1 = __uint_as_float((uint32_t)(254 - (e - (e + 1) / 2) - 64) << 23);
+            const float inv1 = __uint_as_float((uint32_t)(254 - (e - (e + 1) / 2) - 64) << 23) * up;
             if (t == 0) {
                 const bool good = (all_finite >> (lane & 28) & 15) == 15;
                 sh.q_scale[qi] = good ? __uint_as_float((uint32_t)e << 23) / up * a.scale * PA_LOG2E : NAN;
@@ -290,38 +291,33 @@ __device__ __forceinline__ void pa_epilogue(const fo_paged_attention_launch &a, 
             }
             uint2 *to = q_ops + tile * (Shape::Q_TILE / 8) + lane;
 #pragma unroll
-            for (int c = 0; c < KS / 2; c++)
+            for (int c = 0; c < D / 64; c++)
 #pragma unroll
-                for (int w = 0; w < 2; w++) {
-                    // Elements 8 w .. 8 w + 7: step 2 c + w.
-                    float y[8];
+                for (int w = 0; w < 4; w++) {
+                    // Elements 4 w .. 4 w + 3.
+                    float y[4];
 #pragma unroll
-                    for (int i = 0; i < 8; i++) y[i] = x[c][8 * w + i] * inv0 * inv1 * up;
+                    for (int i = 0; i < 4; i++) y[i] = x[c][4 * w + i] * inv0 * inv1;
                     if constexpr (I8) {
-                        uint32_t f[3][2];
+                        // Step 2 c + w / 2, register w % 2.
+                        uint32_t z[4];
 #pragma unroll
-                        for (int h = 0; h < 2; h++) {
-                            uint32_t z[4];
+                        for (int i = 0; i < 4; i++) z[i] = (uint32_t)__float2int_rn(y[i]);
+                        const uint32_t lo01 = __byte_perm(z[0], z[1], 0x5140), lo23 = __byte_perm(z[2], z[3], 0x5140);
+                        const uint32_t f[3] = {
+                            __byte_perm(__byte_perm(z[0], z[1], 0x0062), __byte_perm(z[2], z[3], 0x0062), 0x5410),
+                            __byte_perm(lo01, lo23, 0x7632), __byte_perm(lo01, lo23, 0x5410)};
 #pragma unroll
-                            for (int i = 0; i < 4; i++) z[i] = (uint32_t)__float2int_rn(y[4 * h + i]);
-                            const uint32_t lo01 = __byte_perm(z[0], z[1], 0x5140), lo23 = __byte_perm(z[2], z[3], 0x5140);
-                            f[0][h] = __byte_perm(__byte_perm(z[0], z[1], 0x0062), __byte_perm(z[2], z[3], 0x0062), 0x5410);
-                            f[1][h] = __byte_perm(lo01, lo23, 0x7632);
-                            f[2][h] = __byte_perm(lo01, lo23, 0x5410);
-                        }
-#pragma unroll
-                        for (int i = 0; i < 3; i++) to[(i * KS + 2 * c + w) * 32] = make_uint2(f[i][0], f[i][1]);
+                        for (int i = 0; i < 3; i++)
+                            reinterpret_cast<uint32_t *>(to + (i * KQ + 2 * c + w / 2) * 32)[w % 2] = f[i];
                     } else {
+                        // Step 4 c + w.
 #pragma unroll
                         for (int i = 0; i < QT; i++) {
-                            if (i == 3) {
-#pragma unroll
-                                for (int j = 0; j < 8; j++) y[j] *= PA_GROUP;
-                            }
-                            uint32_t f[4];
-#pragma unroll
-                            for (int j = 0; j < 4; j++) f[j] = pa_e4m3x2(y[2 * j], y[2 * j + 1]);
-                            to[(i * KS + 2 * c + w) * 32] = make_uint2(f[0] | f[1] << 16, f[2] | f[3] << 16);
+                            const uint32_t f0 = pa_f16x2(y[0], y[1]), f1 = pa_f16x2(y[2], y[3]);
+                            to[(i * KQ + 4 * c + w) * 32] = make_uint2(f0, f1);
+                            const float2 b0 = f16x2_f32x2(f0), b1 = f16x2_f32x2(f1);
+                            y[0] -= b0.x, y[1] -= b0.y, y[2] -= b1.x, y[3] -= b1.y;
                         }
                     }
                 }
@@ -445,12 +441,13 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     constexpr int TILE = Shape::TILE, HALF = Shape::HALF;
     constexpr int STEPS = HALF / 16;   // m16 steps of a consumer's half
     constexpr int KW = D / 16;         // words of a K row per lane
-    constexpr int KS = D / 32;         // k32 steps over a row's elements
-    constexpr int VS = HALF / 32;      // k32 steps over a half's keys
+    constexpr int VS = HALF / 32;      // pairs of V loads over a half's keys, 32 keys each
     constexpr int MT = D / 16;         // m16 tiles of the output's dimensions
     constexpr bool I8 = FORMAT == FO_PAGED_I8;
-    constexpr int QT = Shape::QT, PT = Shape::PT;
-    using T = typename std::conditional<F32, float, uint16_t>::type;
+    constexpr int QT = Shape::QT, PT = Shape::PT, KQ = Shape::KQ;
+    // The queries' operands stay in registers where there is room, and are read
+    // for each tile otherwise.
+    constexpr bool Q_REGS = NT * QT * KQ <= 12;
     extern __shared__ uint8_t pa_smem[];
     __shared__ PaShared sh;
     uint8_t *tiles = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(pa_smem) + 1023) & ~uintptr_t(1023));
@@ -663,28 +660,29 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         const int p_last = p_first + s.n - 1;
         // The queries as B operands (a warp's n8 tiles are col_groups apart).
         const int n_tiles = min(max((n_queries - col_group * 8 + a.col_groups * 8 - 1) / (a.col_groups * 8), 0), NT);
-        uint32_t qf[NT][QT][KS][2];
+        uint2 qf[Q_REGS ? NT : 1][QT * KQ];
         float q_scale[NT][2];  // of this lane's columns 2 t, 2 t + 1
         int q_pos[NT][2];
         if (!sm100::mbar_wait(&sh.q_full, segment & 1, &sh.abort, a.err)) return;
+        const uint2 *q_from = q_ops + col_group * (Shape::Q_TILE / 8) + lane;
+        const int q_step = a.col_groups * (Shape::Q_TILE / 8);  // to the warp's next n8 tile
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            const int q_tile = nt * a.col_groups + col_group;
-            const uint2 *from = q_ops + q_tile * (Shape::Q_TILE / 8) + lane;
+            if constexpr (Q_REGS) {
 #pragma unroll
-            for (int x = 0; x < QT * KS; x++) {
-                const uint2 f = nt < n_tiles ? from[32 * x] : make_uint2(0, 0);
-                qf[nt][x / KS][x % KS][0] = f.x;
-                qf[nt][x / KS][x % KS][1] = f.y;
+                for (int x = 0; x < QT * KQ; x++) qf[nt][x] = nt < n_tiles ? q_from[nt * q_step + 32 * x] : make_uint2(0, 0);
             }
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                q_scale[nt][h] = sh.q_scale[q_tile * 8 + 2 * t + h];
-                q_pos[nt][h] = sh.q_pos[q_tile * 8 + 2 * t + h];
+                const int col = (nt * a.col_groups + col_group) * 8 + 2 * t + h;
+                q_scale[nt][h] = sh.q_scale[col];
+                q_pos[nt][h] = sh.q_pos[col];
             }
         }
-        __syncwarp();
-        if (lane == 0) sm100::mbar_arrive(&sh.q_free);
+        if constexpr (Q_REGS) {
+            __syncwarp();
+            if (lane == 0) sm100::mbar_arrive(&sh.q_free);
+        }
         float m[NT][2], l[NT][2], o[MT][NT][4];
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
@@ -718,72 +716,88 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             // of one kind are issued before the first is used.
             float c[STEPS][NT][4], mx[NT][2];
             const bool masked = pos0 + HALF - 1 > p_first || pos0 < low_last;
-            uint32_t kw[STEPS][2][KW];
 #pragma unroll
-            for (int mt = 0; mt < STEPS; mt++) {
-                const uint8_t *row = kt + 16 * mt * D;
-                *reinterpret_cast<uint4 *>(kw[mt][0]) = *reinterpret_cast<const uint4 *>(row + k_off0);
-                *reinterpret_cast<uint4 *>(kw[mt][1]) = *reinterpret_cast<const uint4 *>(row + k_off1);
-                if constexpr (D == 128) {
-                    *reinterpret_cast<uint4 *>(kw[mt][0] + 4) = *reinterpret_cast<const uint4 *>(row + (k_off0 ^ 64));
-                    *reinterpret_cast<uint4 *>(kw[mt][1] + 4) = *reinterpret_cast<const uint4 *>(row + (k_off1 ^ 64));
-                }
-            }
-            float ks[STEPS];
+            for (int nt = 0; nt < NT; nt++) mx[nt][0] = mx[nt][1] = -INFINITY;
+            // As many steps at a time as there are registers for.
+            constexpr int AHEAD = NT == 1 ? STEPS : D == 64 ? 2 : 1;
 #pragma unroll
-            for (int mt = 0; mt < STEPS; mt++) ks[mt] = sh.scales[slot][(half * STEPS + mt) >> page_shift];
+            for (int m0 = 0; m0 < STEPS; m0 += AHEAD) {
+                uint32_t kw[AHEAD][2][KW];
+                float ks[AHEAD];
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                if (nt >= n_tiles) break;
-                // int8: an accumulator for each term; e4m3: for each of two terms, or
-                // for each group of three.
-                constexpr int A = I8 ? 3 : 2;
-                typename std::conditional<I8, uint32_t, float>::type acc[STEPS][A][4];
-#pragma unroll
-                for (int mt = 0; mt < STEPS; mt++)
-#pragma unroll
-                    for (int x = 0; x < A; x++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) acc[mt][x][e] = I8 ? PA_MAGIC : 0;
-#pragma unroll
-                for (int w = 0; w < KS; w++)
-#pragma unroll
-                    for (int x = 0; x < QT; x++)
-#pragma unroll
-                        for (int mt = 0; mt < STEPS; mt++) {
-                            const uint32_t a0 = kw[mt][0][2 * w], a1 = kw[mt][1][2 * w];
-                            const uint32_t a2 = kw[mt][0][2 * w + 1], a3 = kw[mt][1][2 * w + 1];
-                            const uint32_t b0 = qf[nt][x][w][0], b1 = qf[nt][x][w][1];
-                            if constexpr (!I8) pa_qmma(acc[mt][x / (QT / 2)], a0, a1, a2, a3, b0, b1);
-                            else if (x == 0) pa_imma<true>(acc[mt][0], a0, a1, a2, a3, b0, b1);
-                            else pa_imma<false>(acc[mt][x], a0, a1, a2, a3, b0, b1);
-                        }
-                mx[nt][0] = mx[nt][1] = -INFINITY;
-#pragma unroll
-                for (int mt = 0; mt < STEPS; mt++) {
-                    float (&sc)[4] = c[mt][nt];
-#pragma unroll
-                    for (int e = 0; e < 4; e++) {
-                        if constexpr (I8) {
-                            const float hi = __uint_as_float(acc[mt][0][e]) - PA_MAGIC_F;
-                            const float mid = __uint_as_float(acc[mt][1][e]) - PA_MAGIC_F;
-                            const float lo = __uint_as_float(acc[mt][A - 1][e]) - PA_MAGIC_F;
-                            sc[e] = fmaf(hi, 65536.0f, fmaf(mid, 256.0f, lo));
-                        } else {
-                            sc[e] = fmaf(acc[mt][1][e], F32 ? 1.0f / PA_GROUP : 1.0f, acc[mt][0][e]);
-                        }
-                        sc[e] *= ks[mt] * q_scale[nt][e & 1];
+                for (int mt = 0; mt < AHEAD; mt++) {
+                    const uint8_t *row = kt + 16 * (m0 + mt) * D;
+                    *reinterpret_cast<uint4 *>(kw[mt][0]) = *reinterpret_cast<const uint4 *>(row + k_off0);
+                    *reinterpret_cast<uint4 *>(kw[mt][1]) = *reinterpret_cast<const uint4 *>(row + k_off1);
+                    if constexpr (D == 128) {
+                        *reinterpret_cast<uint4 *>(kw[mt][0] + 4) = *reinterpret_cast<const uint4 *>(row + (k_off0 ^ 64));
+                        *reinterpret_cast<uint4 *>(kw[mt][1] + 4) = *reinterpret_cast<const uint4 *>(row + (k_off1 ^ 64));
                     }
-                    if (masked) {
+                    ks[mt] = sh.scales[slot][(half * STEPS + m0 + mt) >> page_shift];
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+                    if (nt >= n_tiles) break;
+                    uint2 q_now[Q_REGS ? 1 : QT * KQ];
+                    if constexpr (!Q_REGS) {
+#pragma unroll
+                        for (int x = 0; x < QT * KQ; x++) q_now[x] = q_from[nt * q_step + 32 * x];
+                    }
+                    const uint2 *qs = Q_REGS ? qf[Q_REGS ? nt : 0] : q_now;
+                    constexpr int A = I8 ? 3 : 1;  // accumulators: int8's terms have their own
+                    typename std::conditional<I8, uint32_t, float>::type acc[AHEAD][A][4];
+#pragma unroll
+                    for (int mt = 0; mt < AHEAD; mt++)
+#pragma unroll
+                        for (int x = 0; x < A; x++)
+#pragma unroll
+                            for (int e = 0; e < 4; e++) acc[mt][x][e] = I8 ? PA_MAGIC : 0;
+#pragma unroll
+                    for (int w = 0; w < KQ; w++)
+#pragma unroll
+                        for (int mt = 0; mt < AHEAD; mt++) {
+                            uint32_t f[4];
+                            if constexpr (I8) {
+                                f[0] = kw[mt][0][2 * w], f[1] = kw[mt][1][2 * w];
+                                f[2] = kw[mt][0][2 * w + 1], f[3] = kw[mt][1][2 * w + 1];
+                            } else {
+                                f[0] = e4m3x2_f16x2(kw[mt][0][w] & 0xFFFFu), f[1] = e4m3x2_f16x2(kw[mt][1][w] & 0xFFFFu);
+                                f[2] = e4m3x2_f16x2(kw[mt][0][w] >> 16), f[3] = e4m3x2_f16x2(kw[mt][1][w] >> 16);
+                            }
+#pragma unroll
+                            for (int x = 0; x < QT; x++) {
+                                const uint2 b = qs[x * KQ + w];
+                                if constexpr (!I8) pa_hmma(acc[mt][0], f[0], f[1], f[2], f[3], b.x, b.y);
+                                else if (x == 0) pa_imma<true>(acc[mt][0], f[0], f[1], f[2], f[3], b.x, b.y);
+                                else pa_imma<false>(acc[mt][x], f[0], f[1], f[2], f[3], b.x, b.y);
+                            }
+                        }
+#pragma unroll
+                    for (int mt = 0; mt < AHEAD; mt++) {
+                        float (&sc)[4] = c[m0 + mt][nt];
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
-                            const int pos = pos0 + 16 * mt + (e < 2 ? k0 : 8 + k1), p = q_pos[nt][e & 1];
-                            const bool seen = pos <= p && (a.window == 0 || pos > p - a.window);
-                            if (!seen) sc[e] = -INFINITY;
+                            if constexpr (I8) {
+                                const float hi = __uint_as_float(acc[mt][0][e]) - PA_MAGIC_F;
+                                const float mid = __uint_as_float(acc[mt][1][e]) - PA_MAGIC_F;
+                                const float lo = __uint_as_float(acc[mt][A - 1][e]) - PA_MAGIC_F;
+                                sc[e] = fmaf(hi, 65536.0f, fmaf(mid, 256.0f, lo));
+                            } else {
+                                sc[e] = acc[mt][0][e];
+                            }
+                            sc[e] *= ks[mt] * q_scale[nt][e & 1];
                         }
-                    }
+                        if (masked) {
 #pragma unroll
-                    for (int e = 0; e < 4; e++) mx[nt][e & 1] = fmaxf(mx[nt][e & 1], sc[e]);
+                            for (int e = 0; e < 4; e++) {
+                                const int pos = pos0 + 16 * (m0 + mt) + (e < 2 ? k0 : 8 + k1), p = q_pos[nt][e & 1];
+                                const bool seen = pos <= p && (a.window == 0 || pos > p - a.window);
+                                if (!seen) sc[e] = -INFINITY;
+                            }
+                        }
+#pragma unroll
+                        for (int e = 0; e < 4; e++) mx[nt][e & 1] = fmaxf(mx[nt][e & 1], sc[e]);
+                    }
                 }
             }
             if constexpr (!I8) {
@@ -799,15 +813,21 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                     __syncwarp();
                 }
             }
-            // The values, while the maxima and probabilities are worked out.
+            // The values: where there is room, while the maxima and probabilities are
+            // worked out.
+            constexpr bool V_AHEAD = NT == 1;
             const uint32_t v_at = sm100::smem_u32(vt) + v_base;
-            uint32_t va[MT][VS][4];
+            uint32_t va[V_AHEAD ? MT : 2][VS][4];
+            if constexpr (V_AHEAD) {
 #pragma unroll
-            for (int d = 0; d < MT; d++)
+                for (int d = 0; d < MT; d++)
 #pragma unroll
-                for (int v = 0; v < VS; v++) pa_load_transposed(va[d][v], v_at + 32 * v * D + ((d ^ v_swizzle) << 4));
+                    for (int v = 0; v < VS; v++)
+                        pa_load_transposed(va[d][v], v_at + 32 * v * D + ((d ^ v_swizzle) << 4));
+            }
             // The half's own maximum, which its probabilities are relative to, and
             // the running one: alpha brings the sums so far to it, beta the half's.
+            constexpr float P_BITS = I8 ? 0.0f : 10.0f;  // e4m3: probabilities are held times 2^10
             float alpha[NT][2], beta[NT][2];
             bool moved = false;
 #pragma unroll
@@ -823,26 +843,26 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                     // While nothing has been seen the maximum stays -infinity and
                     // every probability is 0.
                     alpha[nt][h] = top == -INFINITY ? 1.0f : sm100::ex2(m[nt][h] - top);
-                    beta[nt][h] = x == -INFINITY ? 0.0f : sm100::ex2(x - top);
+                    beta[nt][h] = x == -INFINITY ? 0.0f : sm100::ex2(x - top - P_BITS);
                     moved |= top != m[nt][h];
                     m[nt][h] = top;
-                    mx[nt][h] = x == -INFINITY ? 0.0f : x;
+                    mx[nt][h] = x == -INFINITY ? 0.0f : x - P_BITS;
                 }
             }
             // Probabilities' terms, transposed into B operands.
-            uint32_t pf[NT][PT][VS][2];
+            // int8: [term][32 keys][16 of them], e4m3: [term][16 keys][8 of them].
+            uint32_t pf[NT][PT][STEPS * (I8 ? 1 : 2)];
 #pragma unroll
             for (int nt = 0; nt < NT; nt++) {
                 if (nt >= n_tiles) break;
                 float sum0 = 0.0f, sum1 = 0.0f;
 #pragma unroll
                 for (int mt = 0; mt < STEPS; mt++) {
-                    constexpr int PAIRS = (PT + 1) / 2;
-                    uint32_t tr[PAIRS][2];  // two terms of the keys of rows 0 .. 7, and of 8 .. 15
+                    uint32_t tr[2][2];  // int8: two terms each; of the keys of rows 0 .. 7, and of 8 .. 15
 #pragma unroll
                     for (int r = 0; r < 2; r++) {
-                        float p0 = sm100::ex2(c[mt][nt][2 * r] - mx[nt][0]);
-                        float p1 = sm100::ex2(c[mt][nt][2 * r + 1] - mx[nt][1]);
+                        const float p0 = sm100::ex2(c[mt][nt][2 * r] - mx[nt][0]);
+                        const float p1 = sm100::ex2(c[mt][nt][2 * r + 1] - mx[nt][1]);
                         sum0 += p0;
                         sum1 += p1;
                         if constexpr (I8) {
@@ -853,20 +873,19 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                             tr[0][r] = pa_transpose(__byte_perm(u0, u1, 0x5410));
                             if constexpr (F32) tr[1][r] = pa_transpose(__byte_perm(u0, u1, 0x7632));
                         } else {
-                            p0 *= 256.0f;
-                            p1 *= 256.0f;
-#pragma unroll
-                            for (int x = 0; x < PAIRS; x++) {
-                                const uint32_t x0 = pa_e4m3x2(p0, p1);
-                                if (2 * x + 1 == 3) p0 *= PA_GROUP, p1 *= PA_GROUP;
-                                const uint32_t x1 = 2 * x + 1 < PT ? pa_e4m3x2(p0, p1) : 0;
-                                tr[x][r] = pa_transpose(__byte_perm(x0, x1, 0x5140));
+                            const uint32_t f = pa_f16x2(p0, p1);
+                            pf[nt][0][2 * mt + r] = pa_transpose(f);
+                            if constexpr (F32) {
+                                const float2 b = f16x2_f32x2(f);
+                                pf[nt][PT - 1][2 * mt + r] = pa_transpose(pa_f16x2(p0 - b.x, p1 - b.y));
                             }
                         }
                     }
+                    if constexpr (I8) {
 #pragma unroll
-                    for (int x = 0; x < PT; x++)
-                        pf[nt][x][mt / 2][mt % 2] = __byte_perm(tr[x / 2][0], tr[x / 2][1], x % 2 ? 0x7531 : 0x6420);
+                        for (int x = 0; x < PT; x++)
+                            pf[nt][x][mt] = __byte_perm(tr[x / 2][0], tr[x / 2][1], x % 2 ? 0x7531 : 0x6420);
+                    }
                 }
                 l[nt][0] = fmaf(sum0, beta[nt][0], l[nt][0] * alpha[nt][0]);
                 l[nt][1] = fmaf(sum1, beta[nt][1], l[nt][1] * alpha[nt][1]);
@@ -883,21 +902,27 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             }
             // O^T: rows = dimensions, columns = queries; two m16 tiles of dimensions
             // at a time, each page's sum times its scale.
-            constexpr float PART = I8 ? (F32 ? 1.0f / 8388607.0f : 1.0f / 65535.0f) : 1.0f / 256.0f;
-            // The products over one page's keys, the steps [from, to) of 16; WHOLE:
-            // all of the half's.
-            auto page_sum = [&](auto whole, int from, int to) {
-                constexpr bool WHOLE = decltype(whole)::value;
-                const float vs = sh.scales[slot][8 + ((half * STEPS + from) >> page_shift)] * PART;
+            constexpr float PART = I8 ? (F32 ? 1.0f / 8388607.0f : 1.0f / 65535.0f) : 1.0f;
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    if (nt >= n_tiles) break;
-                    const float f0 = vs * beta[nt][0], f1 = vs * beta[nt][1];
-                    // int8: an accumulator for each term; e4m3: for each of three
-                    // terms, or for each group of three.
-                    constexpr int A = I8 ? PT : F32 ? 2 : 3, PER = I8 ? 1 : PT / A;
+            for (int d2 = 0; d2 < MT; d2 += 2) {
+                if constexpr (!V_AHEAD) {
 #pragma unroll
-                    for (int d2 = 0; d2 < MT; d2 += 2) {
+                    for (int d = 0; d < 2; d++)
+#pragma unroll
+                        for (int v = 0; v < VS; v++)
+                            pa_load_transposed(va[d][v], v_at + 32 * v * D + (((d2 + d) ^ v_swizzle) << 4));
+                }
+                const uint32_t (*vr)[VS][4] = va + (V_AHEAD ? d2 : 0);
+                // The products over one page's keys, the steps [from, to) of 16; WHOLE:
+                // all of the half's.
+                auto page_sum = [&](auto whole, int from, int to) {
+                    constexpr bool WHOLE = decltype(whole)::value;
+                    const float vs = sh.scales[slot][8 + ((half * STEPS + from) >> page_shift)] * PART;
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++) {
+                        if (nt >= n_tiles) break;
+                        const float f0 = vs * beta[nt][0], f1 = vs * beta[nt][1];
+                        constexpr int A = I8 ? PT : 1;
                         typename std::conditional<I8, uint32_t, float>::type acc[2][A][4];
 #pragma unroll
                         for (int d = 0; d < 2; d++)
@@ -909,15 +934,29 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                         for (int v = 0; v < VS; v++) {
                             const bool first = WHOLE || (2 * v >= from && 2 * v < to);
                             const bool second = WHOLE || (2 * v + 1 >= from && 2 * v + 1 < to);
-                            if (!first && !second) continue;
+                            if constexpr (I8) {
+                                if (!first && !second) continue;
 #pragma unroll
-                            for (int x = 0; x < PT; x++) {
-                                const uint32_t b0 = first ? pf[nt][x][v][0] : 0u, b1 = second ? pf[nt][x][v][1] : 0u;
+                                for (int x = 0; x < PT; x++) {
+                                    const uint32_t b0 = first ? pf[nt][x][2 * v] : 0u, b1 = second ? pf[nt][x][2 * v + 1] : 0u;
 #pragma unroll
-                                for (int d = 0; d < 2; d++) {
-                                    const uint32_t (&r)[4] = va[d2 + d][v];
-                                    if constexpr (I8) pa_imma<false>(acc[d][x], r[0], r[1], r[2], r[3], b0, b1);
-                                    else pa_qmma(acc[d][x / PER], r[0], r[1], r[2], r[3], b0, b1);
+                                    for (int d = 0; d < 2; d++)
+                                        pa_imma<false>(acc[d][x], vr[d][v][0], vr[d][v][1], vr[d][v][2], vr[d][v][3], b0, b1);
+                                }
+                            } else {
+#pragma unroll
+                                for (int y = 0; y < 2; y++) {
+                                    if (!(y ? second : first)) continue;
+#pragma unroll
+                                    for (int d = 0; d < 2; d++) {
+                                        const uint32_t u0 = vr[d][v][2 * y], u1 = vr[d][v][2 * y + 1];
+                                        const uint32_t a0 = e4m3x2_f16x2(u0 & 0xFFFFu), a1 = e4m3x2_f16x2(u1 & 0xFFFFu);
+                                        const uint32_t a2 = e4m3x2_f16x2(u0 >> 16), a3 = e4m3x2_f16x2(u1 >> 16);
+#pragma unroll
+                                        for (int x = 0; x < PT; x++)
+                                            pa_hmma(acc[d][0], a0, a1, a2, a3, pf[nt][x][4 * v + 2 * y],
+                                                    pf[nt][x][4 * v + 2 * y + 1]);
+                                    }
                                 }
                             }
                         }
@@ -928,29 +967,31 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                                 float sum;
                                 if constexpr (I8) {
                                     // Term 0 is the lowest byte.
-                                    sum = fmaf(__uint_as_float(acc[d][1][e]) - PA_MAGIC_F, 256.0f,
+                                    sum = fmaf(__uint_as_float(acc[d][A > 1][e]) - PA_MAGIC_F, 256.0f,
                                                __uint_as_float(acc[d][0][e]) - PA_MAGIC_F);
                                     if constexpr (F32)
                                         sum = fmaf(__uint_as_float(acc[d][A - 1][e]) - PA_MAGIC_F, 65536.0f, sum);
-                                } else if constexpr (F32) {
-                                    sum = fmaf(acc[d][1][e], 1.0f / PA_GROUP, acc[d][0][e]);
                                 } else {
-                                    sum = acc[d][0][e] + (acc[d][1][e] + acc[d][A - 1][e]);
+                                    sum = acc[d][0][e];
                                 }
                                 o[d2 + d][nt][e] = fmaf(sum, e & 1 ? f1 : f0, o[d2 + d][nt][e]);
                             }
                     }
-                }
-            };
-            if ((1 << page_shift) >= STEPS)
-                page_sum(std::true_type{}, 0, STEPS);
-            else
-                for (int from = 0; from < STEPS; from += 1 << page_shift)
-                    page_sum(std::false_type{}, from, from + (1 << page_shift));
+                };
+                if ((1 << page_shift) >= STEPS)
+                    page_sum(std::true_type{}, 0, STEPS);
+                else
+                    for (int from = 0; from < STEPS; from += 1 << page_shift)
+                        page_sum(std::false_type{}, from, from + (1 << page_shift));
+            }
             __syncwarp();
             if (lane == 0) sm100::mbar_arrive(&sh.empty[slot]);
         }
 
+        if constexpr (!Q_REGS) {
+            __syncwarp();
+            if (lane == 0) sm100::mbar_arrive(&sh.q_free);
+        }
         // This warp's part, for the epilogue warps to join.  A part that is not a
         // number (a query that is not finite, a page number outside the pool)
         // makes its queries' outputs NaN.
@@ -1017,6 +1058,7 @@ template <int D, int FORMAT, int NT, bool F32>
 cudaError_t launch_attention(const fo_paged_attention_launch &a, unsigned grid, cudaStream_t stream) {
     auto *kernel = paged_attention_kernel<D, FORMAT, NT, F32>;
     using Shape = PaShape<D, FORMAT, NT, F32>;
+    static_assert(Shape::smem(NT * Shape::MAX_GROUPS) + sizeof(PaShared) <= 227 * 1024, "shared memory");
     // The attribute belongs to each device's context: set once per device.
     static std::atomic<unsigned long long> configured{0};
     int dev = 0;
@@ -1024,7 +1066,7 @@ cudaError_t launch_attention(const fo_paged_attention_launch &a, unsigned grid, 
     const unsigned long long bit = 1ull << (dev & 63);
     if (!(configured.load() & bit)) {
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             Shape::smem(4 * NT));
+                                             Shape::smem(NT * Shape::MAX_GROUPS));
         if (e != cudaSuccess) return e;
         // The kernel's register split is only sound at the launch count that it
         // was written for.
@@ -1042,11 +1084,9 @@ cudaError_t launch_attention(const fo_paged_attention_launch &a, unsigned grid, 
 
 template <int D, int FORMAT>
 cudaError_t launch_attention(const fo_paged_attention_launch &a, int nt, unsigned grid, cudaStream_t stream) {
-    if (a.q.dtype == FO_DT_F32) {
-        if constexpr (FORMAT == FO_PAGED_I8)
-            if (nt == 2) return launch_attention<D, FORMAT, 2, true>(a, grid, stream);
-        return launch_attention<D, FORMAT, 1, true>(a, grid, stream);
-    }
+    if (a.q.dtype == FO_DT_F32)
+        return nt == 1 ? launch_attention<D, FORMAT, 1, true>(a, grid, stream)
+                       : launch_attention<D, FORMAT, 2, true>(a, grid, stream);
     return nt == 1 ? launch_attention<D, FORMAT, 1, false>(a, grid, stream)
                    : launch_attention<D, FORMAT, 2, false>(a, grid, stream);
 }
@@ -1057,14 +1097,17 @@ extern "C" cudaError_t fo_launch_paged_attention(const fo_paged_attention_launch
     fo_paged_attention_launch a = *args;
     if (a.batch.total_rows <= 0) return cudaSuccess;
     a.group = a.q.heads / a.kv.n_kv_heads;
-    // A warp takes the queries of one n8 tile, or two (six terms of an FP32 query
-    // leave registers for one); beyond that 2 or 4 warps share each half of a
-    // tile; beyond that a (sequence, KV head) is read once for each group of
-    // queries.
+    // A warp takes the queries of one n8 tile, or two; beyond that 2 or 4 warps
+    // share each half of a tile; beyond that a (sequence, KV head) is read once
+    // for each group of queries.
     const int64_t queries = a.batch.max_rows * a.group;
-    const int most_nt = a.q.dtype == FO_DT_F32 && a.kv.format == FO_PAGED_E4M3 ? 1 : 2;
-    const int nt = queries <= 8 ? 1 : most_nt;
-    a.col_groups = queries <= 8 * nt ? 1 : queries <= 16 * nt ? 2 : 4;
+    const int nt = queries <= 8 ? 1 : 2;
+    const bool f32 = a.q.dtype == FO_DT_F32, i8 = a.kv.format == FO_PAGED_I8;
+    const int most_groups = f32 ? (a.kv.head_dim == 64 ? fo::PaShape<64, FO_PAGED_E4M3, 2, true>::MAX_GROUPS
+                                   : i8 ? fo::PaShape<128, FO_PAGED_I8, 2, true>::MAX_GROUPS
+                                        : fo::PaShape<128, FO_PAGED_E4M3, 2, true>::MAX_GROUPS)
+                                : fo::PaShape<128, FO_PAGED_E4M3, 2, false>::MAX_GROUPS;
+    a.col_groups = queries <= 16 ? 1 : queries <= 32 || most_groups == 2 ? 2 : 4;
     a.queries = 8 * nt * a.col_groups;
     a.evict_first = queries <= a.queries;
     auto aligned = [](const fo_rows &r, int64_t bytes) {
