@@ -244,7 +244,7 @@ struct fo_paged_attention_launch {
     // holds, warps that share a tile, and what 16-byte accesses may be used for.
     int32_t group, queries, col_groups, q_vec, out_vec, evict_first;
 };
-#define FO_PAGED_QUERIES 64  // queries that a block holds at most
+#define FO_PAGED_QUERIES 48  // queries that a block holds at most
 cudaError_t fo_launch_paged_attention(const fo_paged_attention_launch *args, int sms, cudaStream_t stream);
 
 // The bounded-wait self-test kernel (selftest.cu).

@@ -19,7 +19,7 @@
 //
 // In a block two producer warps walk the page table a step ahead and copy
 // tiles into a ring in shared memory with TMA (swizzled, so that the reads
-// below meet no bank conflicts); eight consumer warps, two to a tile, a half
+// below meet no bank conflicts); twelve consumer warps, two to a tile, a half
 // each, take tiles in turn, each with its own running maximum and sum; and two
 // epilogue warps split the next (sequence, KV head)'s queries into operands
 // while the consumers are at this one's, join the consumers' parts, and write
@@ -53,23 +53,25 @@
 
 namespace fo {
 
-constexpr int PA_CONSUMERS = 8;  // consumer warps
-constexpr int PA_PRODUCERS = 2;  // producer warps
-constexpr int PA_EPILOGUES = 2;  // epilogue warps
-constexpr int PA_STAGES = 8;     // tiles in the ring
-// A parity wait cannot tell a barrier's phase from the one two before it.
-// Every slot of the ring is filled by one producer warp only and emptied by
-// one group of consumer warps only, each of which passes its phases one by one.
-static_assert(PA_STAGES % PA_PRODUCERS == 0 && PA_STAGES % (PA_CONSUMERS / 2) == 0, "owners of the ring's slots");
+constexpr int PA_CONSUMERS = 12;  // consumer warps
+constexpr int PA_PRODUCERS = 2;   // producer warps
+constexpr int PA_EPILOGUES = 2;   // epilogue warps
+constexpr int PA_STAGES = 8;      // tiles in the ring
+// A parity wait cannot tell a barrier's phase from the one two before it, so
+// every slot is filled by one producer warp only, which passes the phases of
+// its empty barrier one by one; a consumer, whose slots others use too, first
+// sees the slot's tile number, which is written once the phase before the
+// tile's own is over.
+static_assert(PA_STAGES % PA_PRODUCERS == 0, "owners of the ring's slots");
 constexpr int PA_THREADS = 32 * (PA_CONSUMERS + PA_PRODUCERS + PA_EPILOGUES);
-// Registers a thread: launched with 168 (65,536 over 384 threads), the
-// producers' and epilogues' warpgroup gives up what the consumers' two take:
-// 128 * 104 + 256 * 200 = 384 * 168.
-constexpr int PA_LAUNCH_REGS = 168, PA_OTHER_REGS = 104, PA_CONSUMER_REGS = 200;
-static_assert(128 * PA_OTHER_REGS + 256 * PA_CONSUMER_REGS == PA_THREADS * PA_LAUNCH_REGS, "register split");
+// Registers a thread: launched with 128 (65,536 over 512 threads), the
+// producers' and epilogues' warpgroup gives up what the consumers' three take:
+// 128 * 104 + 384 * 136 = 512 * 128.
+constexpr int PA_LAUNCH_REGS = 128, PA_OTHER_REGS = 104, PA_CONSUMER_REGS = 136;
+static_assert(128 * PA_OTHER_REGS + 384 * PA_CONSUMER_REGS == PA_THREADS * PA_LAUNCH_REGS, "register split");
 constexpr float PA_LOG2E = 1.4426950408889634f, PA_LN2 = 0.6931471805599453f;
 
-template <int D, int FORMAT, int NT, bool F32>
+template <int D, int FORMAT, bool F32>
 struct PaShape {
     static constexpr int TILE_BYTES = 8192;        // of keys, and of values
     static constexpr int TILE = TILE_BYTES / D;    // positions
@@ -80,9 +82,7 @@ struct PaShape {
     static constexpr int PT = I8 ? (F32 ? 3 : 2) : QT;       // a probability's
     static constexpr int KQ = I8 ? D / 32 : D / 16;          // k steps over a row's elements
     static constexpr int PART_LD = D + 4;          // a column of a consumer's part, in floats
-    static constexpr int PARTS = PA_CONSUMERS * NT * 8 * PART_LD * 4;
-    // Warps that can share a half of a tile: four, where their queries' operands fit.
-    static constexpr int MAX_GROUPS = !I8 && F32 && D == 128 ? 2 : 4;
+    static constexpr int PARTS = PA_CONSUMERS * 8 * PART_LD * 4;
     static constexpr int Q_TILE = QT * KQ * 32 * 8;  // an n8 tile of queries as operands
     static constexpr int smem(int q_tiles) { return 1024 + PA_STAGES * STAGE + PARTS + q_tiles * Q_TILE; }
 };
@@ -189,13 +189,30 @@ struct PaShared {
     uint64_t q_full, q_free;        // a segment's queries are there; have been taken
     uint64_t part_full, part_free;  // its parts
     float scales[PA_STAGES][16];    // keys' of a tile's pages, then values'
-    float ml[PA_CONSUMERS][16][2];
+    int tile[PA_STAGES];            // the block's number of the tile in a slot
+    float ml[PA_CONSUMERS][8][2];
     float q_scale[FO_PAGED_QUERIES];
     int q_pos[FO_PAGED_QUERIES];
     long long warp_sum[PA_THREADS / 32];
     long long begin_base;
     int begin_seq, abort;
 };
+
+// Waits for the block's tile k in its slot; false when the block gave up.
+__device__ __forceinline__ bool pa_wait_tile(PaShared &sh, int slot, int k, unsigned *err) {
+    uint64_t t0 = 0;
+    for (uint32_t it = 1; *(volatile int *)&sh.tile[slot] != k; ++it) {
+        if ((it & 63) != 0) continue;
+        if (*(volatile int *)&sh.abort) return false;
+        if (t0 == 0) t0 = sm100::globaltimer();
+        if (sm100::globaltimer() - t0 > FO_WAIT_NS) {
+            *(volatile int *)&sh.abort = 1;
+            atomicOr(err, FO_DEVERR_WAIT_TIMEOUT);
+            return false;
+        }
+    }
+    return sm100::mbar_wait(&sh.full[slot], (k / PA_STAGES) & 1, &sh.abort, err);
+}
 
 // Sum of x over the block's earlier threads; `all` the whole block's.
 __device__ __forceinline__ long long pa_scan(long long x, PaShared &sh, long long &all) {
@@ -229,10 +246,10 @@ __device__ __forceinline__ long long pa_share(long long total, int n) {
 
 // The epilogue warps: `me` of PA_EPILOGUES takes every PA_EPILOGUES-th n8 tile of
 // queries to split into operands, and every such query to join and write.
-template <int D, int FORMAT, int NT, bool F32, int TILE>
+template <int D, int FORMAT, bool F32, int TILE>
 __device__ __forceinline__ void pa_epilogue(const fo_paged_attention_launch &a, PaShared &sh, PaCursor<TILE> at, int count,
                                             long long begin, long long per, int me, float *parts, uint2 *q_ops) {
-    using Shape = PaShape<D, FORMAT, NT, F32>;
+    using Shape = PaShape<D, FORMAT, F32>;
     using T = typename std::conditional<F32, float, uint16_t>::type;
     constexpr bool I8 = FORMAT == FO_PAGED_I8;
     constexpr int QT = Shape::QT, KQ = Shape::KQ;
@@ -252,28 +269,31 @@ __device__ __forceinline__ void pa_epilogue(const fo_paged_attention_launch &a, 
                 q = static_cast<const T *>(a.q.data) + (u.w.s.first + r) * a.q.row_stride +
                     (head * a.group + (q0 + qi) - r * a.group) * a.q.head_stride + 16 * t;
             }
-            float x[D / 64][16], top = 0.0f;
+            // Read twice, 16 elements at a time: the largest first.
+            auto load = [&](int c, float (&x)[16]) {
+                if (!q) {
+#pragma unroll
+                    for (int e = 0; e < 16; e++) x[e] = 0.0f;
+                } else if (a.q_vec) {
+                    load8(q + 64 * c, x);
+                    load8(q + 64 * c + 8, x + 8);
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 16; e++) x[e] = load1(q + 64 * c + e);
+                }
+            };
+            float top = 0.0f;
             bool finite = true;
 #pragma unroll
             for (int c = 0; c < D / 64; c++) {
-                if (!q) {
-#pragma unroll
-                    for (int e = 0; e < 16; e++) x[c][e] = 0.0f;
-                } else if (a.q_vec) {
-                    load8(q + 64 * c, x[c]);
-                    load8(q + 64 * c + 8, x[c] + 8);
-                } else {
-#pragma unroll
-                    for (int e = 0; e < 16; e++) x[c][e] = load1(q + 64 * c + e);
-                }
-            }
-#pragma unroll
-            for (int c = 0; c < D / 64; c++)
+                float x[16];
+                load(c, x);
 #pragma unroll
                 for (int e = 0; e < 16; e++) {
-                    top = fmaxf(top, fabsf(x[c][e]));
-                    finite &= fabsf(x[c][e]) <= FLT_MAX;
+                    top = fmaxf(top, fabsf(x[e]));
+                    finite &= fabsf(x[e]) <= FLT_MAX;
                 }
+            }
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const unsigned all_finite = __ballot_sync(0xffffffffu, finite);
@@ -290,14 +310,16 @@ __device__ __forceinline__ void pa_epilogue(const fo_paged_attention_launch &a, 
                 sh.q_pos[qi] = q ? (int)(u.w.s.len - u.w.s.n) + r : -1;
             }
             uint2 *to = q_ops + tile * (Shape::Q_TILE / 8) + lane;
-#pragma unroll
-            for (int c = 0; c < D / 64; c++)
+#pragma unroll 1
+            for (int c = 0; c < D / 64; c++) {
+                float x[16];
+                load(c, x);
 #pragma unroll
                 for (int w = 0; w < 4; w++) {
                     // Elements 4 w .. 4 w + 3.
                     float y[4];
 #pragma unroll
-                    for (int i = 0; i < 4; i++) y[i] = x[c][4 * w + i] * inv0 * inv1;
+                    for (int i = 0; i < 4; i++) y[i] = x[4 * w + i] * inv0 * inv1;
                     if constexpr (I8) {
                         // Step 2 c + w / 2, register w % 2.
                         uint32_t z[4];
@@ -321,6 +343,7 @@ __device__ __forceinline__ void pa_epilogue(const fo_paged_attention_launch &a, 
                         }
                     }
                 }
+            }
         }
         __syncwarp();
         if (lane == 0) sm100::mbar_arrive(&sh.q_full);
@@ -357,7 +380,7 @@ __device__ __forceinline__ void pa_epilogue(const fo_paged_attention_launch &a, 
         auto join = [&](bool scratch) {
             for (int x = lane; x < (n_queries - me + PA_EPILOGUES - 1) / PA_EPILOGUES * (D / 4); x += 32) {
                 const int quad = x % (D / 4), qi = x / (D / 4) * PA_EPILOGUES + me;
-                const int tile = qi / 8, cg = tile % a.col_groups, nt = tile / a.col_groups, col = qi % 8;
+                const int cg = qi / 8, col = qi % 8;
                 const int parts_n = scratch ? c1 - c0 + 1 : PA_CONSUMERS / a.col_groups;
                 float mm = -INFINITY, ll = 0.0f;
                 float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -371,8 +394,8 @@ __device__ __forceinline__ void pa_epilogue(const fo_paged_attention_launch &a, 
                         ml = __ldcg(reinterpret_cast<const float2 *>(a.part_ml) + at_part(c0 + j, qi));
                         u = __ldcg(reinterpret_cast<const float4 *>(a.part_o + at_part(c0 + j, qi) * D) + quad);
                     } else {
-                        ml = *reinterpret_cast<const float2 *>(sh.ml[w][8 * nt + col]);
-                        u = *reinterpret_cast<const float4 *>(parts + ((w * NT + nt) * 8 + col) * Shape::PART_LD + 4 * quad);
+                        ml = *reinterpret_cast<const float2 *>(sh.ml[w][col]);
+                        u = *reinterpret_cast<const float4 *>(parts + (w * 8 + col) * Shape::PART_LD + 4 * quad);
                     }
                     lost |= ml.x != ml.x || ml.y != ml.y;
                     if (ml.x == -INFINITY) continue;  // it has seen nothing
@@ -432,11 +455,11 @@ __device__ __forceinline__ void pa_epilogue(const fo_paged_attention_launch &a, 
     }
 }
 
-template <int D, int FORMAT, int NT, bool F32>
+template <int D, int FORMAT, bool F32>
 __global__ void __launch_bounds__(PA_THREADS, 1)
     paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                            const __grid_constant__ fo_paged_attention_launch a) {
-    using Shape = PaShape<D, FORMAT, NT, F32>;
+    using Shape = PaShape<D, FORMAT, F32>;
     constexpr int STAGES = PA_STAGES;
     constexpr int TILE = Shape::TILE, HALF = Shape::HALF;
     constexpr int STEPS = HALF / 16;   // m16 steps of a consumer's half
@@ -447,7 +470,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     constexpr int QT = Shape::QT, PT = Shape::PT, KQ = Shape::KQ;
     // The queries' operands stay in registers where there is room, and are read
     // for each tile otherwise.
-    constexpr bool Q_REGS = NT * QT * KQ <= 12;
+    constexpr bool Q_REGS = QT * KQ <= 6;
     extern __shared__ uint8_t pa_smem[];
     __shared__ PaShared sh;
     uint8_t *tiles = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(pa_smem) + 1023) & ~uintptr_t(1023));
@@ -467,6 +490,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         sm100::mbar_init(&sh.part_full, PA_CONSUMERS);
         sm100::mbar_init(&sh.part_free, PA_EPILOGUES);
         sm100::mbar_fence_init();
+        for (int i = 0; i < STAGES; i++) sh.tile[i] = -1;
         sh.abort = 0;
     }
     auto work_of = [&](int64_t seq) -> long long {
@@ -514,7 +538,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         // ------------------------------------------------------------ producer
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PA_OTHER_REGS));
         if (warp >= PA_CONSUMERS + PA_PRODUCERS) {
-            pa_epilogue<D, FORMAT, NT, F32, TILE>(a, sh, at, count, begin, per, warp - PA_CONSUMERS - PA_PRODUCERS, parts, q_ops);
+            pa_epilogue<D, FORMAT, F32, TILE>(a, sh, at, count, begin, per, warp - PA_CONSUMERS - PA_PRODUCERS, parts, q_ops);
             return;
         }
         // Each producer warp issues every PA_PRODUCERS-th tile of the block's: one
@@ -592,6 +616,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                     ok = false;
                     break;
                 }
+                if (lane == 0) *(volatile int *)&sh.tile[slot] = tile;
                 const bool here = off == i;
                 const bool load = here && now.id != -1 && !now.bad;
                 const uint32_t n_loads = __popc(__ballot_sync(0xffffffffu, load));
@@ -652,47 +677,33 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     const int v_swizzle = D == 128 ? v_key : v_key >> 1 & 3;
     const int page_shift = 31 - __clz(min(page, TILE) / 16);  // log2 of the m16 steps of a page's part of a tile
 
+    const uint2 *q_from = q_ops + col_group * (Shape::Q_TILE / 8) + lane;
+
     for (int i = 0, segment = 0; i < count; segment++) {
         const int n = min(at.left(), count - i);
         const Sequence &s = at.w.s;
         const int n_queries = min(s.n * a.group - at.group() * a.queries, a.queries);  // of this unit
         const int p_first = (int)(s.len - s.n);  // positions of the sequence's first row and of its last
         const int p_last = p_first + s.n - 1;
-        // The queries as B operands (a warp's n8 tiles are col_groups apart).
-        const int n_tiles = min(max((n_queries - col_group * 8 + a.col_groups * 8 - 1) / (a.col_groups * 8), 0), NT);
-        uint2 qf[Q_REGS ? NT : 1][QT * KQ];
-        float q_scale[NT][2];  // of this lane's columns 2 t, 2 t + 1
-        int q_pos[NT][2];
+        // The queries as B operands.
+        uint2 qf[Q_REGS ? QT * KQ : 1];
+        float q_scale[2];  // of this lane's columns 2 t, 2 t + 1
+        int q_pos[2];
         if (!sm100::mbar_wait(&sh.q_full, segment & 1, &sh.abort, a.err)) return;
-        const uint2 *q_from = q_ops + col_group * (Shape::Q_TILE / 8) + lane;
-        const int q_step = a.col_groups * (Shape::Q_TILE / 8);  // to the warp's next n8 tile
+        if constexpr (Q_REGS) {
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-            if constexpr (Q_REGS) {
+            for (int x = 0; x < QT * KQ; x++) qf[x] = q_from[32 * x];
+        }
 #pragma unroll
-                for (int x = 0; x < QT * KQ; x++) qf[nt][x] = nt < n_tiles ? q_from[nt * q_step + 32 * x] : make_uint2(0, 0);
-            }
-#pragma unroll
-            for (int h = 0; h < 2; h++) {
-                const int col = (nt * a.col_groups + col_group) * 8 + 2 * t + h;
-                q_scale[nt][h] = sh.q_scale[col];
-                q_pos[nt][h] = sh.q_pos[col];
-            }
+        for (int h = 0; h < 2; h++) {
+            q_scale[h] = sh.q_scale[col_group * 8 + 2 * t + h];
+            q_pos[h] = sh.q_pos[col_group * 8 + 2 * t + h];
         }
         if constexpr (Q_REGS) {
             __syncwarp();
             if (lane == 0) sm100::mbar_arrive(&sh.q_free);
         }
-        float m[NT][2], l[NT][2], o[MT][NT][4];
-#pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-            m[nt][0] = m[nt][1] = -INFINITY;
-            l[nt][0] = l[nt][1] = 0.0f;
-#pragma unroll
-            for (int d = 0; d < MT; d++)
-#pragma unroll
-                for (int e = 0; e < 4; e++) o[d][nt][e] = 0.0f;
-        }
+        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[MT][4] = {};
         // Tiles all of whose positions every row sees need no mask.
         const int low_last = a.window > 0 ? max(p_last + 1 - (int)min64(a.window, INT32_MAX / 2), 0) : 0;
         bool any = false;
@@ -702,8 +713,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             const int slot = k % STAGES;
             // The first position of this warp's half.
             const int pos0 = (at.w.t0 + at.tile + (k - i)) * TILE + half * HALF;
-            if (!sm100::mbar_wait(&sh.full[slot], (k / STAGES) & 1, &sh.abort, a.err)) return;
-            if (n_tiles == 0 || pos0 > p_last || pos0 + HALF <= at.w.low) {
+            if (!pa_wait_tile(sh, slot, k, a.err)) return;
+            if (col_group * 8 >= n_queries || pos0 > p_last || pos0 + HALF <= at.w.low) {
                 // No row of this warp's sees any of it.
                 __syncwarp();
                 if (lane == 0) sm100::mbar_arrive(&sh.empty[slot]);
@@ -712,94 +723,6 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             any = true;
             const uint8_t *kt = tiles + slot * Shape::STAGE + half * HALF * D;
             uint8_t *vt = tiles + slot * Shape::STAGE + Shape::TILE_BYTES + half * HALF * D;
-            // S^T: rows = keys, columns = queries; scores times log2 e.  All products
-            // of one kind are issued before the first is used.
-            float c[STEPS][NT][4], mx[NT][2];
-            const bool masked = pos0 + HALF - 1 > p_first || pos0 < low_last;
-#pragma unroll
-            for (int nt = 0; nt < NT; nt++) mx[nt][0] = mx[nt][1] = -INFINITY;
-            // As many steps at a time as there are registers for.
-            constexpr int AHEAD = NT == 1 ? STEPS : D == 64 ? 2 : 1;
-#pragma unroll
-            for (int m0 = 0; m0 < STEPS; m0 += AHEAD) {
-                uint32_t kw[AHEAD][2][KW];
-                float ks[AHEAD];
-#pragma unroll
-                for (int mt = 0; mt < AHEAD; mt++) {
-                    const uint8_t *row = kt + 16 * (m0 + mt) * D;
-                    *reinterpret_cast<uint4 *>(kw[mt][0]) = *reinterpret_cast<const uint4 *>(row + k_off0);
-                    *reinterpret_cast<uint4 *>(kw[mt][1]) = *reinterpret_cast<const uint4 *>(row + k_off1);
-                    if constexpr (D == 128) {
-                        *reinterpret_cast<uint4 *>(kw[mt][0] + 4) = *reinterpret_cast<const uint4 *>(row + (k_off0 ^ 64));
-                        *reinterpret_cast<uint4 *>(kw[mt][1] + 4) = *reinterpret_cast<const uint4 *>(row + (k_off1 ^ 64));
-                    }
-                    ks[mt] = sh.scales[slot][(half * STEPS + m0 + mt) >> page_shift];
-                }
-#pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    if (nt >= n_tiles) break;
-                    uint2 q_now[Q_REGS ? 1 : QT * KQ];
-                    if constexpr (!Q_REGS) {
-#pragma unroll
-                        for (int x = 0; x < QT * KQ; x++) q_now[x] = q_from[nt * q_step + 32 * x];
-                    }
-                    const uint2 *qs = Q_REGS ? qf[Q_REGS ? nt : 0] : q_now;
-                    constexpr int A = I8 ? 3 : 1;  // accumulators: int8's terms have their own
-                    typename std::conditional<I8, uint32_t, float>::type acc[AHEAD][A][4];
-#pragma unroll
-                    for (int mt = 0; mt < AHEAD; mt++)
-#pragma unroll
-                        for (int x = 0; x < A; x++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) acc[mt][x][e] = I8 ? PA_MAGIC : 0;
-#pragma unroll
-                    for (int w = 0; w < KQ; w++)
-#pragma unroll
-                        for (int mt = 0; mt < AHEAD; mt++) {
-                            uint32_t f[4];
-                            if constexpr (I8) {
-                                f[0] = kw[mt][0][2 * w], f[1] = kw[mt][1][2 * w];
-                                f[2] = kw[mt][0][2 * w + 1], f[3] = kw[mt][1][2 * w + 1];
-                            } else {
-                                f[0] = e4m3x2_f16x2(kw[mt][0][w] & 0xFFFFu), f[1] = e4m3x2_f16x2(kw[mt][1][w] & 0xFFFFu);
-                                f[2] = e4m3x2_f16x2(kw[mt][0][w] >> 16), f[3] = e4m3x2_f16x2(kw[mt][1][w] >> 16);
-                            }
-#pragma unroll
-                            for (int x = 0; x < QT; x++) {
-                                const uint2 b = qs[x * KQ + w];
-                                if constexpr (!I8) pa_hmma(acc[mt][0], f[0], f[1], f[2], f[3], b.x, b.y);
-                                else if (x == 0) pa_imma<true>(acc[mt][0], f[0], f[1], f[2], f[3], b.x, b.y);
-                                else pa_imma<false>(acc[mt][x], f[0], f[1], f[2], f[3], b.x, b.y);
-                            }
-                        }
-#pragma unroll
-                    for (int mt = 0; mt < AHEAD; mt++) {
-                        float (&sc)[4] = c[m0 + mt][nt];
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            if constexpr (I8) {
-                                const float hi = __uint_as_float(acc[mt][0][e]) - PA_MAGIC_F;
-                                const float mid = __uint_as_float(acc[mt][1][e]) - PA_MAGIC_F;
-                                const float lo = __uint_as_float(acc[mt][A - 1][e]) - PA_MAGIC_F;
-                                sc[e] = fmaf(hi, 65536.0f, fmaf(mid, 256.0f, lo));
-                            } else {
-                                sc[e] = acc[mt][0][e];
-                            }
-                            sc[e] *= ks[mt] * q_scale[nt][e & 1];
-                        }
-                        if (masked) {
-#pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                const int pos = pos0 + 16 * (m0 + mt) + (e < 2 ? k0 : 8 + k1), p = q_pos[nt][e & 1];
-                                const bool seen = pos <= p && (a.window == 0 || pos > p - a.window);
-                                if (!seen) sc[e] = -INFINITY;
-                            }
-                        }
-#pragma unroll
-                        for (int e = 0; e < 4; e++) mx[nt][e & 1] = fmaxf(mx[nt][e & 1], sc[e]);
-                    }
-                }
-            }
             if constexpr (!I8) {
                 // Rows beyond the sequence, or of pages that no row sees, may hold any
                 // bytes: an FP8 NaN times a probability of 0 would be NaN.
@@ -813,179 +736,231 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                     __syncwarp();
                 }
             }
-            // The values: where there is room, while the maxima and probabilities are
-            // worked out.
-            constexpr bool V_AHEAD = NT == 1;
-            const uint32_t v_at = sm100::smem_u32(vt) + v_base;
-            uint32_t va[V_AHEAD ? MT : 2][VS][4];
-            if constexpr (V_AHEAD) {
+            // S^T: rows = keys, columns = queries; scores times log2 e.
+            float c[STEPS][4], mx[2] = {-INFINITY, -INFINITY};
+            const bool masked = pos0 + HALF - 1 > p_first || pos0 < low_last;
+            constexpr int AHEAD = D == 64 ? 2 : 1;  // as many steps at a time as there are registers for
 #pragma unroll
-                for (int d = 0; d < MT; d++)
+            for (int m0 = 0; m0 < STEPS; m0 += AHEAD) {
+                uint32_t kw[AHEAD][2][KW];
 #pragma unroll
-                    for (int v = 0; v < VS; v++)
-                        pa_load_transposed(va[d][v], v_at + 32 * v * D + ((d ^ v_swizzle) << 4));
+                for (int mt = 0; mt < AHEAD; mt++) {
+                    const uint8_t *row = kt + 16 * (m0 + mt) * D;
+                    *reinterpret_cast<uint4 *>(kw[mt][0]) = *reinterpret_cast<const uint4 *>(row + k_off0);
+                    *reinterpret_cast<uint4 *>(kw[mt][1]) = *reinterpret_cast<const uint4 *>(row + k_off1);
+                    if constexpr (D == 128) {
+                        *reinterpret_cast<uint4 *>(kw[mt][0] + 4) = *reinterpret_cast<const uint4 *>(row + (k_off0 ^ 64));
+                        *reinterpret_cast<uint4 *>(kw[mt][1] + 4) = *reinterpret_cast<const uint4 *>(row + (k_off1 ^ 64));
+                    }
+                }
+                constexpr int A = I8 ? 3 : 1;  // accumulators: int8's terms have their own
+                typename std::conditional<I8, uint32_t, float>::type acc[AHEAD][A][4];
+#pragma unroll
+                for (int mt = 0; mt < AHEAD; mt++)
+#pragma unroll
+                    for (int x = 0; x < A; x++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) acc[mt][x][e] = I8 ? PA_MAGIC : 0;
+#pragma unroll
+                for (int w = 0; w < KQ; w++) {
+                    uint2 b[QT];
+#pragma unroll
+                    for (int x = 0; x < QT; x++) b[x] = Q_REGS ? qf[Q_REGS ? x * KQ + w : 0] : q_from[32 * (x * KQ + w)];
+#pragma unroll
+                    for (int mt = 0; mt < AHEAD; mt++) {
+                        uint32_t f[4];
+                        if constexpr (I8) {
+                            f[0] = kw[mt][0][2 * w], f[1] = kw[mt][1][2 * w];
+                            f[2] = kw[mt][0][2 * w + 1], f[3] = kw[mt][1][2 * w + 1];
+                        } else {
+                            f[0] = e4m3x2_f16x2(kw[mt][0][w] & 0xFFFFu), f[1] = e4m3x2_f16x2(kw[mt][1][w] & 0xFFFFu);
+                            f[2] = e4m3x2_f16x2(kw[mt][0][w] >> 16), f[3] = e4m3x2_f16x2(kw[mt][1][w] >> 16);
+                        }
+#pragma unroll
+                        for (int x = 0; x < QT; x++) {
+                            if constexpr (!I8) pa_hmma(acc[mt][0], f[0], f[1], f[2], f[3], b[x].x, b[x].y);
+                            else if (x == 0) pa_imma<true>(acc[mt][0], f[0], f[1], f[2], f[3], b[x].x, b[x].y);
+                            else pa_imma<false>(acc[mt][x], f[0], f[1], f[2], f[3], b[x].x, b[x].y);
+                        }
+                    }
+                }
+#pragma unroll
+                for (int mt = 0; mt < AHEAD; mt++) {
+                    float (&sc)[4] = c[m0 + mt];
+                    const float ks = sh.scales[slot][(half * STEPS + m0 + mt) >> page_shift];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        if constexpr (I8) {
+                            const float hi = __uint_as_float(acc[mt][0][e]) - PA_MAGIC_F;
+                            const float mid = __uint_as_float(acc[mt][1][e]) - PA_MAGIC_F;
+                            const float lo = __uint_as_float(acc[mt][A - 1][e]) - PA_MAGIC_F;
+                            sc[e] = fmaf(hi, 65536.0f, fmaf(mid, 256.0f, lo));
+                        } else {
+                            sc[e] = acc[mt][0][e];
+                        }
+                        sc[e] *= ks * q_scale[e & 1];
+                    }
+                    if (masked) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const int pos = pos0 + 16 * (m0 + mt) + (e < 2 ? k0 : 8 + k1), p = q_pos[e & 1];
+                            const bool seen = pos <= p && (a.window == 0 || pos > p - a.window);
+                            if (!seen) sc[e] = -INFINITY;
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 4; e++) mx[e & 1] = fmaxf(mx[e & 1], sc[e]);
+                }
             }
+            // The values and their scales, and the slot is free.
+            const uint32_t v_at = sm100::smem_u32(vt) + v_base;
+            uint32_t va[MT][VS][4];
+#pragma unroll
+            for (int d = 0; d < MT; d++)
+#pragma unroll
+                for (int v = 0; v < VS; v++) pa_load_transposed(va[d][v], v_at + 32 * v * D + ((d ^ v_swizzle) << 4));
+            float vs[STEPS];
+#pragma unroll
+            for (int x = 0; x < STEPS; x++) vs[x] = sh.scales[slot][8 + ((half * STEPS + x) >> page_shift)];
+            __syncwarp();
+            if (lane == 0) sm100::mbar_arrive(&sh.empty[slot]);
             // The half's own maximum, which its probabilities are relative to, and
             // the running one: alpha brings the sums so far to it, beta the half's.
             constexpr float P_BITS = I8 ? 0.0f : 10.0f;  // e4m3: probabilities are held times 2^10
-            float alpha[NT][2], beta[NT][2];
+            float alpha[2], beta[2];
             bool moved = false;
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                if (nt >= n_tiles) break;
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    float x = mx[nt][h];
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
-                    x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
-                    const float top = fmaxf(x, m[nt][h]);
-                    // While nothing has been seen the maximum stays -infinity and
-                    // every probability is 0.
-                    alpha[nt][h] = top == -INFINITY ? 1.0f : sm100::ex2(m[nt][h] - top);
-                    beta[nt][h] = x == -INFINITY ? 0.0f : sm100::ex2(x - top - P_BITS);
-                    moved |= top != m[nt][h];
-                    m[nt][h] = top;
-                    mx[nt][h] = x == -INFINITY ? 0.0f : x - P_BITS;
-                }
+            for (int h = 0; h < 2; h++) {
+                float x = mx[h];
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+                x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+                const float top = fmaxf(x, m[h]);
+                // While nothing has been seen the maximum stays -infinity and every
+                // probability is 0.
+                alpha[h] = top == -INFINITY ? 1.0f : sm100::ex2(m[h] - top);
+                beta[h] = x == -INFINITY ? 0.0f : sm100::ex2(x - top - P_BITS);
+                moved |= top != m[h];
+                m[h] = top;
+                mx[h] = x == -INFINITY ? 0.0f : x - P_BITS;
             }
             // Probabilities' terms, transposed into B operands.
             // int8: [term][32 keys][16 of them], e4m3: [term][16 keys][8 of them].
-            uint32_t pf[NT][PT][STEPS * (I8 ? 1 : 2)];
+            uint32_t pf[PT][STEPS * (I8 ? 1 : 2)];
+            float sum0 = 0.0f, sum1 = 0.0f;
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++) {
-                if (nt >= n_tiles) break;
-                float sum0 = 0.0f, sum1 = 0.0f;
+            for (int mt = 0; mt < STEPS; mt++) {
+                uint32_t tr[2][2];  // int8: two terms each; of the keys of rows 0 .. 7, and of 8 .. 15
 #pragma unroll
-                for (int mt = 0; mt < STEPS; mt++) {
-                    uint32_t tr[2][2];  // int8: two terms each; of the keys of rows 0 .. 7, and of 8 .. 15
-#pragma unroll
-                    for (int r = 0; r < 2; r++) {
-                        const float p0 = sm100::ex2(c[mt][nt][2 * r] - mx[nt][0]);
-                        const float p1 = sm100::ex2(c[mt][nt][2 * r + 1] - mx[nt][1]);
-                        sum0 += p0;
-                        sum1 += p1;
-                        if constexpr (I8) {
-                            // 2^23 + p times its largest integer: the bytes of that integer.
-                            constexpr float TOP = F32 ? 8388607.0f : 65535.0f;
-                            const uint32_t u0 = __float_as_uint(fmaf(p0, TOP, 8388608.0f));
-                            const uint32_t u1 = __float_as_uint(fmaf(p1, TOP, 8388608.0f));
-                            tr[0][r] = pa_transpose(__byte_perm(u0, u1, 0x5410));
-                            if constexpr (F32) tr[1][r] = pa_transpose(__byte_perm(u0, u1, 0x7632));
-                        } else {
-                            const uint32_t f = pa_f16x2(p0, p1);
-                            pf[nt][0][2 * mt + r] = pa_transpose(f);
-                            if constexpr (F32) {
-                                const float2 b = f16x2_f32x2(f);
-                                pf[nt][PT - 1][2 * mt + r] = pa_transpose(pa_f16x2(p0 - b.x, p1 - b.y));
-                            }
+                for (int r = 0; r < 2; r++) {
+                    const float p0 = sm100::ex2(c[mt][2 * r] - mx[0]), p1 = sm100::ex2(c[mt][2 * r + 1] - mx[1]);
+                    sum0 += p0;
+                    sum1 += p1;
+                    if constexpr (I8) {
+                        // 2^23 + p times its largest integer: the bytes of that integer.
+                        constexpr float TOP = F32 ? 8388607.0f : 65535.0f;
+                        const uint32_t u0 = __float_as_uint(fmaf(p0, TOP, 8388608.0f));
+                        const uint32_t u1 = __float_as_uint(fmaf(p1, TOP, 8388608.0f));
+                        tr[0][r] = pa_transpose(__byte_perm(u0, u1, 0x5410));
+                        if constexpr (F32) tr[1][r] = pa_transpose(__byte_perm(u0, u1, 0x7632));
+                    } else {
+                        const uint32_t f = pa_f16x2(p0, p1);
+                        pf[0][2 * mt + r] = pa_transpose(f);
+                        if constexpr (F32) {
+                            const float2 b = f16x2_f32x2(f);
+                            pf[PT - 1][2 * mt + r] = pa_transpose(pa_f16x2(p0 - b.x, p1 - b.y));
                         }
                     }
-                    if constexpr (I8) {
-#pragma unroll
-                        for (int x = 0; x < PT; x++)
-                            pf[nt][x][mt] = __byte_perm(tr[x / 2][0], tr[x / 2][1], x % 2 ? 0x7531 : 0x6420);
-                    }
                 }
-                l[nt][0] = fmaf(sum0, beta[nt][0], l[nt][0] * alpha[nt][0]);
-                l[nt][1] = fmaf(sum1, beta[nt][1], l[nt][1] * alpha[nt][1]);
+                if constexpr (I8) {
+#pragma unroll
+                    for (int x = 0; x < PT; x++)
+                        pf[x][mt] = __byte_perm(tr[x / 2][0], tr[x / 2][1], x % 2 ? 0x7531 : 0x6420);
+                }
             }
+            l[0] = fmaf(sum0, beta[0], l[0] * alpha[0]);
+            l[1] = fmaf(sum1, beta[1], l[1] * alpha[1]);
             if (__any_sync(0xffffffffu, moved)) {
 #pragma unroll
-                for (int nt = 0; nt < NT; nt++) {
-                    if (nt >= n_tiles) break;
+                for (int d = 0; d < MT; d++)
 #pragma unroll
-                    for (int d = 0; d < MT; d++)
-#pragma unroll
-                        for (int e = 0; e < 4; e++) o[d][nt][e] *= alpha[nt][e & 1];
-                }
+                    for (int e = 0; e < 4; e++) o[d][e] *= alpha[e & 1];
             }
             // O^T: rows = dimensions, columns = queries; two m16 tiles of dimensions
-            // at a time, each page's sum times its scale.
+            // at a time, each page's sum times its scale: the products over one
+            // page's keys, the steps [from, to) of 16; WHOLE: all of the half's.
             constexpr float PART = I8 ? (F32 ? 1.0f / 8388607.0f : 1.0f / 65535.0f) : 1.0f;
+            auto page_sum = [&](auto whole, int from, int to, float scale) {
+                constexpr bool WHOLE = decltype(whole)::value;
+                const float f0 = scale * PART * beta[0], f1 = scale * PART * beta[1];
+                constexpr int A = I8 ? PT : 1;
 #pragma unroll
-            for (int d2 = 0; d2 < MT; d2 += 2) {
-                if constexpr (!V_AHEAD) {
+                for (int d2 = 0; d2 < MT; d2 += 2) {
+                    typename std::conditional<I8, uint32_t, float>::type acc[2][A][4];
 #pragma unroll
                     for (int d = 0; d < 2; d++)
 #pragma unroll
-                        for (int v = 0; v < VS; v++)
-                            pa_load_transposed(va[d][v], v_at + 32 * v * D + (((d2 + d) ^ v_swizzle) << 4));
-                }
-                const uint32_t (*vr)[VS][4] = va + (V_AHEAD ? d2 : 0);
-                // The products over one page's keys, the steps [from, to) of 16; WHOLE:
-                // all of the half's.
-                auto page_sum = [&](auto whole, int from, int to) {
-                    constexpr bool WHOLE = decltype(whole)::value;
-                    const float vs = sh.scales[slot][8 + ((half * STEPS + from) >> page_shift)] * PART;
+                        for (int x = 0; x < A; x++)
 #pragma unroll
-                    for (int nt = 0; nt < NT; nt++) {
-                        if (nt >= n_tiles) break;
-                        const float f0 = vs * beta[nt][0], f1 = vs * beta[nt][1];
-                        constexpr int A = I8 ? PT : 1;
-                        typename std::conditional<I8, uint32_t, float>::type acc[2][A][4];
+                            for (int e = 0; e < 4; e++) acc[d][x][e] = I8 ? PA_MAGIC : 0;
 #pragma unroll
-                        for (int d = 0; d < 2; d++)
+                    for (int v = 0; v < VS; v++) {
+                        const bool first = WHOLE || (2 * v >= from && 2 * v < to);
+                        const bool second = WHOLE || (2 * v + 1 >= from && 2 * v + 1 < to);
+                        if constexpr (I8) {
+                            if (!first && !second) continue;
 #pragma unroll
-                            for (int x = 0; x < A; x++)
+                            for (int x = 0; x < PT; x++) {
+                                const uint32_t b0 = first ? pf[x][2 * v] : 0u, b1 = second ? pf[x][2 * v + 1] : 0u;
 #pragma unroll
-                                for (int e = 0; e < 4; e++) acc[d][x][e] = I8 ? PA_MAGIC : 0;
-#pragma unroll
-                        for (int v = 0; v < VS; v++) {
-                            const bool first = WHOLE || (2 * v >= from && 2 * v < to);
-                            const bool second = WHOLE || (2 * v + 1 >= from && 2 * v + 1 < to);
-                            if constexpr (I8) {
-                                if (!first && !second) continue;
-#pragma unroll
-                                for (int x = 0; x < PT; x++) {
-                                    const uint32_t b0 = first ? pf[nt][x][2 * v] : 0u, b1 = second ? pf[nt][x][2 * v + 1] : 0u;
-#pragma unroll
-                                    for (int d = 0; d < 2; d++)
-                                        pa_imma<false>(acc[d][x], vr[d][v][0], vr[d][v][1], vr[d][v][2], vr[d][v][3], b0, b1);
+                                for (int d = 0; d < 2; d++) {
+                                    const uint32_t (&r)[4] = va[d2 + d][v];
+                                    pa_imma<false>(acc[d][x], r[0], r[1], r[2], r[3], b0, b1);
                                 }
-                            } else {
+                            }
+                        } else {
 #pragma unroll
-                                for (int y = 0; y < 2; y++) {
-                                    if (!(y ? second : first)) continue;
+                            for (int y = 0; y < 2; y++) {
+                                if (!(y ? second : first)) continue;
 #pragma unroll
-                                    for (int d = 0; d < 2; d++) {
-                                        const uint32_t u0 = vr[d][v][2 * y], u1 = vr[d][v][2 * y + 1];
-                                        const uint32_t a0 = e4m3x2_f16x2(u0 & 0xFFFFu), a1 = e4m3x2_f16x2(u1 & 0xFFFFu);
-                                        const uint32_t a2 = e4m3x2_f16x2(u0 >> 16), a3 = e4m3x2_f16x2(u1 >> 16);
+                                for (int d = 0; d < 2; d++) {
+                                    const uint32_t u0 = va[d2 + d][v][2 * y], u1 = va[d2 + d][v][2 * y + 1];
+                                    const uint32_t a0 = e4m3x2_f16x2(u0 & 0xFFFFu), a1 = e4m3x2_f16x2(u1 & 0xFFFFu);
+                                    const uint32_t a2 = e4m3x2_f16x2(u0 >> 16), a3 = e4m3x2_f16x2(u1 >> 16);
 #pragma unroll
-                                        for (int x = 0; x < PT; x++)
-                                            pa_hmma(acc[d][0], a0, a1, a2, a3, pf[nt][x][4 * v + 2 * y],
-                                                    pf[nt][x][4 * v + 2 * y + 1]);
-                                    }
+                                    for (int x = 0; x < PT; x++)
+                                        pa_hmma(acc[d][0], a0, a1, a2, a3, pf[x][4 * v + 2 * y], pf[x][4 * v + 2 * y + 1]);
                                 }
                             }
                         }
-#pragma unroll
-                        for (int d = 0; d < 2; d++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                float sum;
-                                if constexpr (I8) {
-                                    // Term 0 is the lowest byte.
-                                    sum = fmaf(__uint_as_float(acc[d][A > 1][e]) - PA_MAGIC_F, 256.0f,
-                                               __uint_as_float(acc[d][0][e]) - PA_MAGIC_F);
-                                    if constexpr (F32)
-                                        sum = fmaf(__uint_as_float(acc[d][A - 1][e]) - PA_MAGIC_F, 65536.0f, sum);
-                                } else {
-                                    sum = acc[d][0][e];
-                                }
-                                o[d2 + d][nt][e] = fmaf(sum, e & 1 ? f1 : f0, o[d2 + d][nt][e]);
-                            }
                     }
-                };
-                if ((1 << page_shift) >= STEPS)
-                    page_sum(std::true_type{}, 0, STEPS);
-                else
-                    for (int from = 0; from < STEPS; from += 1 << page_shift)
-                        page_sum(std::false_type{}, from, from + (1 << page_shift));
+#pragma unroll
+                    for (int d = 0; d < 2; d++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            float sum;
+                            if constexpr (I8) {
+                                // Term 0 is the lowest byte.
+                                sum = fmaf(__uint_as_float(acc[d][A > 1][e]) - PA_MAGIC_F, 256.0f,
+                                           __uint_as_float(acc[d][0][e]) - PA_MAGIC_F);
+                                if constexpr (F32)
+                                    sum = fmaf(__uint_as_float(acc[d][A - 1][e]) - PA_MAGIC_F, 65536.0f, sum);
+                            } else {
+                                sum = acc[d][0][e];
+                            }
+                            o[d2 + d][e] = fmaf(sum, e & 1 ? f1 : f0, o[d2 + d][e]);
+                        }
+                }
+            };
+            if ((1 << page_shift) >= STEPS) {
+                page_sum(std::true_type{}, 0, STEPS, vs[0]);
+            } else if (page_shift == 1) {
+#pragma unroll
+                for (int from = 0; from < STEPS; from += 2) page_sum(std::false_type{}, from, from + 2, vs[from]);
+            } else {
+#pragma unroll
+                for (int from = 0; from < STEPS; from++) page_sum(std::false_type{}, from, from + 1, vs[from]);
             }
-            __syncwarp();
-            if (lane == 0) sm100::mbar_arrive(&sh.empty[slot]);
         }
 
         if constexpr (!Q_REGS) {
@@ -997,26 +972,22 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         // makes its queries' outputs NaN.
         if (segment > 0 && !sm100::mbar_wait(&sh.part_free, (segment - 1) & 1, &sh.abort, a.err)) return;
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++) {
-            if (nt >= n_tiles) break;
+        for (int h = 0; h < 2; h++) {
+            float x = l[h];
+            x += __shfl_xor_sync(0xffffffffu, x, 4);
+            x += __shfl_xor_sync(0xffffffffu, x, 8);
+            x += __shfl_xor_sync(0xffffffffu, x, 16);
+            if (g == 0) {
+                const bool good = x == x && q_scale[h] == q_scale[h];
+                sh.ml[warp][2 * t + h][0] = good ? m[h] : NAN;
+                sh.ml[warp][2 * t + h][1] = x;
+            }
+            if (any) {
+                float *col = parts + (warp * 8 + 2 * t + h) * Shape::PART_LD + g;
 #pragma unroll
-            for (int h = 0; h < 2; h++) {
-                float x = l[nt][h];
-                x += __shfl_xor_sync(0xffffffffu, x, 4);
-                x += __shfl_xor_sync(0xffffffffu, x, 8);
-                x += __shfl_xor_sync(0xffffffffu, x, 16);
-                if (g == 0) {
-                    const bool good = x == x && q_scale[nt][h] == q_scale[nt][h];
-                    sh.ml[warp][8 * nt + 2 * t + h][0] = good ? m[nt][h] : NAN;
-                    sh.ml[warp][8 * nt + 2 * t + h][1] = x;
-                }
-                if (any) {
-                    float *col = parts + ((warp * NT + nt) * 8 + 2 * t + h) * Shape::PART_LD + g;
-#pragma unroll
-                    for (int d = 0; d < MT; d++) {
-                        col[16 * d] = o[d][nt][h];
-                        col[16 * d + 8] = o[d][nt][2 + h];
-                    }
+                for (int d = 0; d < MT; d++) {
+                    col[16 * d] = o[d][h];
+                    col[16 * d + 8] = o[d][2 + h];
                 }
             }
         }
@@ -1054,11 +1025,11 @@ bool pa_map(CUtensorMap *map, const void *codes, const fo_paged_kv &kv) {
               CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int D, int FORMAT, int NT, bool F32>
+template <int D, int FORMAT, bool F32>
 cudaError_t launch_attention(const fo_paged_attention_launch &a, unsigned grid, cudaStream_t stream) {
-    auto *kernel = paged_attention_kernel<D, FORMAT, NT, F32>;
-    using Shape = PaShape<D, FORMAT, NT, F32>;
-    static_assert(Shape::smem(NT * Shape::MAX_GROUPS) + sizeof(PaShared) <= 227 * 1024, "shared memory");
+    auto *kernel = paged_attention_kernel<D, FORMAT, F32>;
+    using Shape = PaShape<D, FORMAT, F32>;
+    static_assert(Shape::smem(PA_CONSUMERS / 2) + sizeof(PaShared) <= 227 * 1024, "shared memory");
     // The attribute belongs to each device's context: set once per device.
     static std::atomic<unsigned long long> configured{0};
     int dev = 0;
@@ -1066,7 +1037,7 @@ cudaError_t launch_attention(const fo_paged_attention_launch &a, unsigned grid, 
     const unsigned long long bit = 1ull << (dev & 63);
     if (!(configured.load() & bit)) {
         cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                             Shape::smem(NT * Shape::MAX_GROUPS));
+                                             Shape::smem(PA_CONSUMERS / 2));
         if (e != cudaSuccess) return e;
         // The kernel's register split is only sound at the launch count that it
         // was written for.
@@ -1082,13 +1053,13 @@ cudaError_t launch_attention(const fo_paged_attention_launch &a, unsigned grid, 
     return cudaGetLastError();
 }
 
-template <int D, int FORMAT>
-cudaError_t launch_attention(const fo_paged_attention_launch &a, int nt, unsigned grid, cudaStream_t stream) {
+template <int D>
+cudaError_t launch_attention(const fo_paged_attention_launch &a, unsigned grid, cudaStream_t stream) {
     if (a.q.dtype == FO_DT_F32)
-        return nt == 1 ? launch_attention<D, FORMAT, 1, true>(a, grid, stream)
-                       : launch_attention<D, FORMAT, 2, true>(a, grid, stream);
-    return nt == 1 ? launch_attention<D, FORMAT, 1, false>(a, grid, stream)
-                   : launch_attention<D, FORMAT, 2, false>(a, grid, stream);
+        return a.kv.format == FO_PAGED_I8 ? launch_attention<D, FO_PAGED_I8, true>(a, grid, stream)
+                                          : launch_attention<D, FO_PAGED_E4M3, true>(a, grid, stream);
+    return a.kv.format == FO_PAGED_I8 ? launch_attention<D, FO_PAGED_I8, false>(a, grid, stream)
+                                      : launch_attention<D, FO_PAGED_E4M3, false>(a, grid, stream);
 }
 
 }  // namespace fo
@@ -1097,18 +1068,12 @@ extern "C" cudaError_t fo_launch_paged_attention(const fo_paged_attention_launch
     fo_paged_attention_launch a = *args;
     if (a.batch.total_rows <= 0) return cudaSuccess;
     a.group = a.q.heads / a.kv.n_kv_heads;
-    // A warp takes the queries of one n8 tile, or two; beyond that 2 or 4 warps
-    // share each half of a tile; beyond that a (sequence, KV head) is read once
-    // for each group of queries.
+    // A warp takes the queries of one n8 tile; beyond that 2, 3 or 6 warps share
+    // each half of a tile; beyond that a (sequence, KV head) is read once for
+    // each group of queries.
     const int64_t queries = a.batch.max_rows * a.group;
-    const int nt = queries <= 8 ? 1 : 2;
-    const bool f32 = a.q.dtype == FO_DT_F32, i8 = a.kv.format == FO_PAGED_I8;
-    const int most_groups = f32 ? (a.kv.head_dim == 64 ? fo::PaShape<64, FO_PAGED_E4M3, 2, true>::MAX_GROUPS
-                                   : i8 ? fo::PaShape<128, FO_PAGED_I8, 2, true>::MAX_GROUPS
-                                        : fo::PaShape<128, FO_PAGED_E4M3, 2, true>::MAX_GROUPS)
-                                : fo::PaShape<128, FO_PAGED_E4M3, 2, false>::MAX_GROUPS;
-    a.col_groups = queries <= 16 ? 1 : queries <= 32 || most_groups == 2 ? 2 : 4;
-    a.queries = 8 * nt * a.col_groups;
+    a.col_groups = queries <= 8 ? 1 : queries <= 16 ? 2 : queries <= 24 ? 3 : 6;
+    a.queries = 8 * a.col_groups;
     a.evict_first = queries <= a.queries;
     auto aligned = [](const fo_rows &r, int64_t bytes) {
         const int64_t unit = bytes / (r.dtype == FO_DT_F32 ? 4 : 2);
@@ -1122,9 +1087,5 @@ extern "C" cudaError_t fo_launch_paged_attention(const fo_paged_attention_launch
                          ((a.batch.table_stride * a.kv.page_size * a.kv.head_dim + 8191) / 8192);
     const int64_t groups = fo::PA_CONSUMERS / 2 / a.col_groups;
     const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(sms, (most + groups - 1) / groups));
-    if (a.kv.head_dim == 64)
-        return a.kv.format == FO_PAGED_I8 ? fo::launch_attention<64, FO_PAGED_I8>(a, nt, grid, stream)
-                                          : fo::launch_attention<64, FO_PAGED_E4M3>(a, nt, grid, stream);
-    return a.kv.format == FO_PAGED_I8 ? fo::launch_attention<128, FO_PAGED_I8>(a, nt, grid, stream)
-                                      : fo::launch_attention<128, FO_PAGED_E4M3>(a, nt, grid, stream);
+    return a.kv.head_dim == 64 ? fo::launch_attention<64>(a, grid, stream) : fo::launch_attention<128>(a, grid, stream);
 }
