@@ -19,23 +19,35 @@ __device__ __forceinline__ float load1<float>(const float *p) { return *p; }
 template <>
 __device__ __forceinline__ float load1<uint16_t>(const uint16_t *p) { return bf16_f32(*p); }
 
-// Eight adjacent elements; p 16-byte aligned.
+// Eight adjacent elements as they lie in memory (16 bytes of BF16, 32 of
+// FP32), 16-byte aligned, and as floats.
 template <typename T>
-__device__ __forceinline__ void load8(const T *p, float *x);
-template <>
-__device__ __forceinline__ void load8<float>(const float *p, float *x) {
-    const float4 a = reinterpret_cast<const float4 *>(p)[0], b = reinterpret_cast<const float4 *>(p)[1];
-    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w, x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+struct Raw8 {
+    uint4 w[sizeof(T) / 2];
+};
+template <typename T>
+__device__ __forceinline__ Raw8<T> load_raw8(const T *p) {
+    Raw8<T> r;
+#pragma unroll
+    for (int i = 0; i < (int)sizeof(T) / 2; i++) r.w[i] = reinterpret_cast<const uint4 *>(p)[i];
+    return r;
 }
-template <>
-__device__ __forceinline__ void load8<uint16_t>(const uint16_t *p, float *x) {
-    const uint4 a = *reinterpret_cast<const uint4 *>(p);
-    const uint32_t w[4] = {a.x, a.y, a.z, a.w};
+__device__ __forceinline__ void unpack8(const Raw8<float> &r, float *x) {
+    const uint32_t w[8] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w, r.w[1].x, r.w[1].y, r.w[1].z, r.w[1].w};
+#pragma unroll
+    for (int i = 0; i < 8; i++) x[i] = __uint_as_float(w[i]);
+}
+__device__ __forceinline__ void unpack8(const Raw8<uint16_t> &r, float *x) {
+    const uint32_t w[4] = {r.w[0].x, r.w[0].y, r.w[0].z, r.w[0].w};
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         x[2 * i] = __uint_as_float(w[i] << 16);
         x[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
     }
+}
+template <typename T>
+__device__ __forceinline__ void load8(const T *p, float *x) {
+    unpack8(load_raw8(p), x);
 }
 
 // Two floats as a BF16 pair, each rounded to nearest even (NaN stays NaN).
@@ -120,13 +132,13 @@ __device__ __forceinline__ float scaled(float x, float scale, float top) {
 }
 
 // Four codes from four values within the codes' range, rounded to nearest
-// even.
+// even.  1.5 * 2^23 + x has the integer nearest x in its low bits.
 template <int FORMAT>
 __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
     if constexpr (FORMAT == FO_PAGED_I8) {
-        const uint32_t x = (uint32_t)__float2int_rn(a) & 255u, y = (uint32_t)__float2int_rn(b) & 255u;
-        const uint32_t z = (uint32_t)__float2int_rn(c) & 255u, w = (uint32_t)__float2int_rn(d);
-        return x | y << 8 | z << 16 | w << 24;
+        const uint32_t x = __float_as_uint(a + 12582912.0f), y = __float_as_uint(b + 12582912.0f);
+        const uint32_t z = __float_as_uint(c + 12582912.0f), w = __float_as_uint(d + 12582912.0f);
+        return __byte_perm(__byte_perm(x, y, 0x0040), __byte_perm(z, w, 0x0040), 0x5410);
     } else {
         uint32_t r;
         asm("{\n\t.reg .b16 lo, hi;\n\t"
@@ -136,6 +148,52 @@ __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) 
             : "=r"(r)
             : "f"(a), "f"(b), "f"(c), "f"(d));
         return r;
+    }
+}
+
+// Eight values x as codes of x / scale (scaled(), then encode4()).  Nearly always
+// x times the scale's reciprocal, off from the quotient by 2^-23 of it at most,
+// rounds to the same code, and only where one of the eight comes near a tie
+// between two codes (or is one of FP8's subnormal codes, or the reciprocal is no
+// normal number, or a value is not finite) are the divisions done: a third of
+// their instructions.
+template <int FORMAT>
+__device__ __forceinline__ uint2 encode8(const float *x, float scale, float inverse, bool exact) {
+    if constexpr (FORMAT == FO_PAGED_I8) {
+        // 1.5 * 2^23 + y has the integer nearest y in its low bits.
+        uint32_t z[8];
+        float most = 0.0f;  // distance from an integer
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float y = x[e] * inverse, m = y + 12582912.0f;
+            z[e] = __float_as_uint(m);
+            most = fmaxf(most, fabsf(y - (m - 12582912.0f)));
+        }
+        if (!(most < 0.4999f) || exact) {
+            float y[8];
+#pragma unroll
+            for (int e = 0; e < 8; e++) y[e] = scaled(x[e], scale, code_max(FORMAT));
+            return make_uint2(encode4<FORMAT>(y[0], y[1], y[2], y[3]), encode4<FORMAT>(y[4], y[5], y[6], y[7]));
+        }
+        return make_uint2(
+            __byte_perm(__byte_perm(z[0], z[1], 0x0040), __byte_perm(z[2], z[3], 0x0040), 0x5410),
+            __byte_perm(__byte_perm(z[4], z[5], 0x0040), __byte_perm(z[6], z[7], 0x0040), 0x5410));
+    } else {
+        // A normal code has 20 bits fewer than FP32; a tie is a half of their range.
+        float y[8];
+        uint32_t near = 0xFFFFFu;
+        float least = 1.0f;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            y[e] = x[e] * inverse;
+            near = min(near, (__float_as_uint(y[e]) + 0x80010u) & 0xFFFFFu);
+            least = fminf(least, fabsf(y[e]));
+        }
+        if (near < 0x20u || least < 0.015625f || exact) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) y[e] = scaled(x[e], scale, code_max(FORMAT));
+        }
+        return make_uint2(encode4<FORMAT>(y[0], y[1], y[2], y[3]), encode4<FORMAT>(y[4], y[5], y[6], y[7]));
     }
 }
 

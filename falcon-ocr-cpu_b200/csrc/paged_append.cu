@@ -10,31 +10,22 @@
 // segment's rows are read once and kept in registers between the maximum and
 // the codes.
 //
-// One task is (segment, KV head, keys | values).  A task of few rows is one
-// warp's; of many rows (a prompt's), a whole block's.  Blocks behind the
-// tasks rotate the queries.
+// A segment's rows of one head's keys or values are a task.  With few rows a
+// call (a decode step, drafts to verify) a task is a warp's, blocks behind
+// the tasks' rotate the queries, and one launch does it all.  With many rows
+// (prompts) a team of threads takes a task, 16 elements a thread, and goes
+// through several heads of the segment with one read of its rotation table's
+// entries, which are twice the size of a head's BF16 values; the next
+// head's rows are on their way while this one's are encoded.  The queries'
+// rotation is a launch of its own then.
 #include "paged_rope.cuh"
 
 #include <algorithm>
 
 namespace fo {
 
-constexpr int APPEND_THREADS = 256;
+constexpr int APPEND_FEW_THREADS = 256;
 constexpr int APPEND_FEW_ROWS = 8;  // rows that a warp's task holds in registers
-
-// Maximum over a task's threads, a warp or the block.
-template <int THREADS>
-__device__ __forceinline__ float task_max(float m, float *red) {
-    m = warp_max(m);
-    if constexpr (THREADS > 32) {
-        if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
-        __syncthreads();
-        m = red[0];
-#pragma unroll
-        for (int w = 1; w < THREADS / 32; w++) m = fmaxf(m, red[w]);
-    }
-    return m;
-}
 
 // Eight elements d .. d + 7 of a row, rotated when `rotate` is set.
 template <typename T, bool VEC>
@@ -86,30 +77,95 @@ __device__ __forceinline__ void append_load(const fo_append_launch &a, const T *
     }
 }
 
-// The segment of sequence `seq` in its j-th touched page, for KV head `head`
-// of the keys or the values, by THREADS threads (t of them): MAXIT groups of
-// eight elements each.
-template <int D, typename T, int FORMAT, bool VEC, int THREADS, int MAXIT>
-__device__ __forceinline__ void append_segment(const fo_append_launch &a, int64_t seq, int64_t j, int head, bool value,
-                                               int t, float *red) {
-    constexpr int GROUPS = D / 8;               // groups of eight in a row
-    constexpr int ROWS_STEP = THREADS / GROUPS;  // rows a step covers
-    const int page = a.kv.page_size;
+// A segment: sequence `seq`'s rows in its j-th touched page.  (Positions and rows
+// are below 2^31, pages a power of two: 64-bit divisions are kept out.)
+struct Segment {
+    int seq, page, row0, p0;  // the sequence's page number, its first row here and that one's position
+    int rows, begin;          // rows (none: nothing to do) and where in the page they begin
+};
+__device__ __forceinline__ Segment segment_at(const fo_append_launch &a, int seq, int j) {
+    const int page = a.kv.page_size, shift = 31 - __clz(page);
     const Sequence s = load_sequence(a.batch, page, seq, a.err);
-    const int64_t from = max64(s.len - s.n, 0);  // first position that is stored
-    const int64_t pg = from / page + j;
-    const int64_t p0 = max64(from, pg * page), p1 = min64(s.len, (pg + 1) * page);
-    if (s.n == 0 || p0 >= p1) return;
+    const int len = (int)s.len, from = max(len - s.n, 0);  // first position that is stored
+    Segment g;
+    g.seq = seq;
+    g.page = (from >> shift) + j;
+    g.p0 = max(from, g.page << shift);
+    const int p1 = (int)min64(len, (int64_t)(g.page + 1) << shift);
+    g.rows = s.n > 0 && p1 > g.p0 ? p1 - g.p0 : 0;
+    g.begin = g.p0 & (page - 1);
+    g.row0 = (int)s.first + (g.p0 - (len - s.n));
+    return g;
+}
+
+// A task's part of the pool.
+struct Tile {
+    uint8_t *codes;
+    float *scale;
     bool valid;
-    const int64_t id = page_of(a.batch, a.kv.n_pages, seq, pg, a.err, valid);
-    if (!valid) return;
-    const int rows = (int)(p1 - p0), begin = (int)(p0 - pg * page);
-    const int64_t row0 = s.first + (p0 - (s.len - s.n));
+};
+template <int D>
+__device__ __forceinline__ Tile tile_of(const fo_append_launch &a, const Segment &s, int head, bool value) {
+    Tile t;
+    const int64_t id = page_of(a.batch, a.kv.n_pages, s.seq, s.page, a.err, t.valid) * a.kv.n_kv_heads + head;
+    t.scale = (value ? a.kv.v_scales : a.kv.k_scales) + id;
+    t.codes = static_cast<uint8_t *>(value ? a.kv.v_codes : a.kv.k_codes) + id * a.kv.page_size * D;
+    return t;
+}
+
+// A row's entries of the rotation table (valid is false outside it).
+__device__ __forceinline__ const float2 *entries_of(const fo_append_launch &a, int64_t row, int64_t position, bool first,
+                                                    bool &inside) {
+    const int64_t p = a.rope.row_positions ? (int64_t)__ldg(a.rope.row_positions + row) : position;
+    inside = p >= 0 && p < a.rope.positions;
+    if (!inside && first) atomicOr(a.err, FO_DEVERR_POSITION);
+    return reinterpret_cast<const float2 *>(a.rope.table) + (inside ? p : 0) * (a.rope.rot_dim / 2);
+}
+
+// The page's earlier codes, `begin` positions of them, against a larger scale.
+template <int D, int FORMAT>
+__device__ __forceinline__ void encode_again(uint8_t *codes, int begin, float ratio, int t, int threads) {
+    uint4 *held = reinterpret_cast<uint4 *>(codes);
+    for (int i = t; i < begin * (D / 16); i += threads) {
+        uint4 w = held[i];
+        uint32_t *ws = reinterpret_cast<uint32_t *>(&w);
+#pragma unroll
+        for (int q = 0; q < 4; q++) {
+            float f[4];
+            decode4<FORMAT>(ws[q], f);
+            ws[q] = encode4<FORMAT>(__fmul_rn(f[0], ratio), __fmul_rn(f[1], ratio), __fmul_rn(f[2], ratio),
+                                    __fmul_rn(f[3], ratio));
+        }
+        held[i] = w;
+    }
+}
+
+// The largest finite magnitude of N values and `m`; `odd` if one is not finite.
+template <int N>
+__device__ __forceinline__ void note(const float *x, float &m, bool &odd) {
+    float top = m, zero = 0.0f;
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+        top = fmaxf(top, fabsf(x[e]));
+        zero = fmaf(x[e], 0.0f, zero);  // NaN from a value that is not finite
+    }
+    if (zero != zero) {
+        odd = true;
+        top = m;
+#pragma unroll
+        for (int e = 0; e < N; e++)
+            if (fabsf(x[e]) <= FLT_MAX) top = fmaxf(top, fabsf(x[e]));
+    }
+    m = top;
+}
+
+// A task of few rows by a warp.
+template <int D, typename T, int FORMAT, bool VEC>
+__device__ __forceinline__ void append_few(const fo_append_launch &a, const Segment &s, int head, bool value, int t) {
+    constexpr int GROUPS = D / 8;            // groups of eight in a row
+    constexpr int ROWS_STEP = 32 / GROUPS;   // rows a step covers
+    constexpr int MAXIT = APPEND_FEW_ROWS / ROWS_STEP;
     const fo_rows &src = value ? a.v : a.k;
-    const int64_t tile = id * a.kv.n_kv_heads + head;
-    float *scale_at = (value ? a.kv.v_scales : a.kv.k_scales) + tile;
-    uint8_t *codes = static_cast<uint8_t *>(value ? a.kv.v_codes : a.kv.k_codes) + tile * page * D;
-    const float old = begin > 0 ? *scale_at : 0.0f;
     const int d = (t % GROUPS) * 8, r0 = t / GROUPS;
     const bool rotate = a.rotate && !value;
     float x[MAXIT][8];
@@ -118,64 +174,40 @@ __device__ __forceinline__ void append_segment(const fo_append_launch &a, int64_
 #pragma unroll
     for (int it = 0; it < MAXIT; it++) {
         const int r = r0 + it * ROWS_STEP;
-        if (r >= rows) continue;
-        const T *xr = static_cast<const T *>(src.data) + (row0 + r) * src.row_stride + head * src.head_stride;
+        if (r >= s.rows) continue;
+        const T *xr = static_cast<const T *>(src.data) + (s.row0 + r) * src.row_stride + head * src.head_stride;
         const float2 *entries = nullptr;
         bool inside = true;
-        if (rotate) {
-            const int64_t p = a.rope.row_positions ? (int64_t)__ldg(a.rope.row_positions + row0 + r) : p0 + r;
-            inside = p >= 0 && p < a.rope.positions;
-            if (!inside && d == 0) atomicOr(a.err, FO_DEVERR_POSITION);
-            entries = reinterpret_cast<const float2 *>(a.rope.table) + (inside ? p : 0) * (a.rope.rot_dim / 2);
-        }
+        if (rotate) entries = entries_of(a, s.row0 + r, s.p0 + r, d == 0, inside);
         append_load<T, VEC>(a, xr, d, entries, inside, rotate, x[it]);
-#pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const float y = fabsf(x[it][e]);
-            if (y <= FLT_MAX) m = fmaxf(m, y);
-            else odd = true;
-        }
+        note<8>(x[it], m, odd);
     }
-    m = task_max<THREADS>(m, red);
+    // The page, looked up while the rows are on their way.
+    const Tile tile = tile_of<D>(a, s, head, value);
+    const float old = s.begin > 0 ? *tile.scale : 0.0f;
+    m = warp_max(m);
     if (odd) atomicOr(a.err, FO_DEVERR_VALUE);
-    const float top = code_max(FORMAT);
-    const float scale = fmaxf(old, __fdiv_rn(m, top));
-    if (scale > old && begin > 0) {
-        // The page's earlier codes against the larger scale.
-        const float ratio = __fdiv_rn(old, scale);
-        uint4 *held = reinterpret_cast<uint4 *>(codes);
-        for (int i = t; i < begin * (D / 16); i += THREADS) {
-            uint4 w = held[i];
-            uint32_t *ws = reinterpret_cast<uint32_t *>(&w);
-#pragma unroll
-            for (int q = 0; q < 4; q++) {
-                float f[4];
-                decode4<FORMAT>(ws[q], f);
-                ws[q] = encode4<FORMAT>(__fmul_rn(f[0], ratio), __fmul_rn(f[1], ratio), __fmul_rn(f[2], ratio),
-                                        __fmul_rn(f[3], ratio));
-            }
-            held[i] = w;
-        }
-    }
-    if (t == 0) *scale_at = scale;
+    if (!tile.valid) return;
+    const float scale = fmaxf(old, __fdiv_rn(m, code_max(FORMAT)));
+    if (scale > old && s.begin > 0) encode_again<D, FORMAT>(tile.codes, s.begin, __fdiv_rn(old, scale), t, 32);
+    if (t == 0) *tile.scale = scale;
+    const bool normal = scale >= 1e-30f;
+    const float inverse = normal ? __frcp_rn(scale) : 0.0f;
 #pragma unroll
     for (int it = 0; it < MAXIT; it++) {
         const int r = r0 + it * ROWS_STEP;
-        if (r >= rows) continue;
-        float y[8];
-#pragma unroll
-        for (int e = 0; e < 8; e++) y[e] = scaled(x[it][e], scale, top);
-        const uint2 w = make_uint2(encode4<FORMAT>(y[0], y[1], y[2], y[3]), encode4<FORMAT>(y[4], y[5], y[6], y[7]));
-        *reinterpret_cast<uint2 *>(codes + (begin + r) * D + d) = w;
+        if (r >= s.rows) continue;
+        *reinterpret_cast<uint2 *>(tile.codes + (s.begin + r) * D + d) =
+            encode8<FORMAT>(x[it], scale, inverse, odd || !normal);
     }
 }
 
 // Sequence of a row when the sequences' row counts differ: the last one that
 // starts at or before it.
-__device__ __forceinline__ int64_t sequence_of_row(const fo_paged_batch &b, int64_t row) {
-    int64_t lo = 0, hi = b.n_seqs - 1;
+__device__ __forceinline__ int sequence_of_row(const fo_paged_batch &b, int row) {
+    int lo = 0, hi = (int)b.n_seqs - 1;
     while (lo < hi) {
-        const int64_t mid = (lo + hi + 1) >> 1;
+        const int mid = (lo + hi + 1) >> 1;
         if (__ldg(b.row_start + mid) <= row) lo = mid;
         else hi = mid - 1;
     }
@@ -187,90 +219,240 @@ __host__ __device__ inline int64_t segments_of(int64_t rows, int64_t page) {
     return rows <= 0 ? 0 : (rows + page - 2) / page + 1;
 }
 
-// Segments are numbered per sequence; when row counts differ and are large,
-// sequence b's start at row_start[b] / page + 2 b, which leaves each at least
-// rows / page + 2 numbers, enough for what it can touch, in total_rows / page
-// + 2 n_seqs of them.
-template <int D, typename T, int FORMAT, bool VEC, bool FEW>
-__global__ void __launch_bounds__(APPEND_THREADS) paged_append_kernel(const __grid_constant__ fo_append_launch a,
-                                                                      int64_t task_blocks, int64_t segments,
-                                                                      int64_t per_seq, bool q_half, bool q_vec) {
-    __shared__ float red[APPEND_THREADS / 32];
-    const int64_t page = a.kv.page_size;
+// The rotation of the queries: a row's position is its place in the cache
+// unless positions are given.
+__device__ __forceinline__ int64_t position_of_row(const fo_append_launch &a, int64_t row, bool &padded) {
+    padded = false;
+    if (a.rope.row_positions) return (int64_t)__ldg(a.rope.row_positions + row);
+    const int seq = a.batch.row_start ? sequence_of_row(a.batch, (int)row) : (int)((unsigned)row / (unsigned)a.batch.max_rows);
+    const Sequence s = load_sequence(a.batch, a.kv.page_size, seq, a.err);
+    const int64_t p = s.len - s.n + (row - s.first);
+    padded = p < 0;
+    return p;
+}
+template <typename T>
+__device__ __forceinline__ void rotate_queries(const fo_append_launch &a, int64_t block, bool half, bool vec) {
+    auto position = [&](int64_t row, bool &padded) { return position_of_row(a, row, padded); };
+    if (half) vec ? rope_block<T, true, true>(a.q, block, position) : rope_block<T, true, false>(a.q, block, position);
+    else vec ? rope_block<T, false, true>(a.q, block, position) : rope_block<T, false, false>(a.q, block, position);
+}
+template <typename T>
+__global__ void __launch_bounds__(ROPE_THREADS, 3) paged_rope_kernel(const __grid_constant__ fo_append_launch a, bool half,
+                                                                     bool vec) {
+    rotate_queries<T>(a, blockIdx.x, half, vec);
+}
+
+// Few rows a sequence: as many segments for each sequence as it can touch.
+template <int D, typename T, int FORMAT, bool VEC>
+__global__ void __launch_bounds__(APPEND_FEW_THREADS, 3)
+    append_few_kernel(const __grid_constant__ fo_append_launch a, unsigned task_blocks, unsigned per_seq, bool q_half,
+                      bool q_vec) {
     if (blockIdx.x >= task_blocks) {
-        auto position = [&](int64_t row, bool &padded) {
-            padded = false;
-            if (a.rope.row_positions) return (int64_t)__ldg(a.rope.row_positions + row);
-            const int64_t seq = a.batch.row_start ? sequence_of_row(a.batch, row) : row / a.batch.max_rows;
-            const Sequence s = load_sequence(a.batch, (int)page, seq, a.err);
-            const int64_t p = s.len - s.n + (row - s.first);
-            padded = p < 0;
-            return p;
-        };
-        const int64_t block = blockIdx.x - task_blocks;
-        if (q_half) q_vec ? rope_block<T, true, true>(a.q, block, position) : rope_block<T, true, false>(a.q, block, position);
-        else q_vec ? rope_block<T, false, true>(a.q, block, position) : rope_block<T, false, false>(a.q, block, position);
+        rotate_queries<T>(a, blockIdx.x - task_blocks, q_half, q_vec);
         return;
     }
-    const int64_t heads2 = 2 * (int64_t)a.kv.n_kv_heads;
-    const int64_t task = FEW ? blockIdx.x * (APPEND_THREADS / 32) + (threadIdx.x >> 5) : blockIdx.x;
-    const int64_t segment = task / heads2;
-    const int part = (int)(task - segment * heads2);
-    if (segment >= segments) return;
-    int64_t seq, j;
+    const unsigned heads2 = 2 * a.kv.n_kv_heads;
+    const unsigned task = blockIdx.x * (APPEND_FEW_THREADS / 32) + (threadIdx.x >> 5), segment = task / heads2;
+    const unsigned part = task - segment * heads2, seq = segment / per_seq;
+    if (seq >= a.batch.n_seqs) return;
+    const Segment s = segment_at(a, (int)seq, (int)(segment - seq * per_seq));
+    if (s.rows > 0) append_few<D, T, FORMAT, VEC>(a, s, part >> 1, part & 1, threadIdx.x & 31);
+}
+
+// Many rows.  A block takes `heads` heads of a segment's keys or values, a team
+// of page_size * D / 16 threads a head at a time.  A thread's 16 elements are
+// two groups of eight: neighbours, or in the half layout the two elements of
+// eight pairs (when rot_dim / 2 is a multiple of eight; LINED_UP is false for
+// other half layouts).
+// Segments are numbered per sequence; when row counts differ, sequence b's
+// start at row_start[b] / page + 2 b, which leaves each at least rows / page +
+// 2 numbers, enough for what it can touch, in total_rows / page + 2 n_seqs.
+template <int D, typename T, int FORMAT, bool VEC, bool LINED_UP>
+__global__ void __launch_bounds__(D == 64 ? 512 : 1024, D == 64 ? 2 : 1) append_many_kernel(const __grid_constant__ fo_append_launch a, unsigned per_seq,
+                                                           int heads) {
+    __shared__ float red[2][32];
+    const int page = a.kv.page_size, n_heads = a.kv.n_kv_heads;
+    const int chunks = (n_heads + heads - 1) / heads;
+    const unsigned segment = blockIdx.x / (2 * chunks);
+    const int part = (int)(blockIdx.x - segment * 2 * chunks);
+    const bool value = part >= chunks;
+    const int head0 = (part - (value ? chunks : 0)) * heads, head1 = min(head0 + heads, n_heads);
+    int seq, j;
     if (per_seq > 0) {
-        seq = segment / per_seq;
-        j = segment - seq * per_seq;
+        seq = (int)(segment / per_seq);
+        j = (int)(segment - seq * per_seq);
     } else {
-        int64_t lo = 0, hi = a.batch.n_seqs - 1;
+        const int shift = 31 - __clz(page);
+        int lo = 0, hi = (int)a.batch.n_seqs - 1;
         while (lo < hi) {
-            const int64_t mid = (lo + hi + 1) >> 1;
-            if (__ldg(a.batch.row_start + mid) / page + 2 * mid <= segment) lo = mid;
+            const int mid = (lo + hi + 1) >> 1;
+            if ((__ldg(a.batch.row_start + mid) >> shift) + 2 * mid <= (int)segment) lo = mid;
             else hi = mid - 1;
         }
         seq = lo;
-        j = segment - (__ldg(a.batch.row_start + seq) / page + 2 * seq);
+        j = (int)segment - ((__ldg(a.batch.row_start + seq) >> shift) + 2 * seq);
         if (j < 0) return;  // row_start out of order (the sequence's own check reports it)
     }
-    const int head = part >> 1;
-    const bool value = part & 1;
-    if constexpr (FEW)
-        append_segment<D, T, FORMAT, VEC, 32, APPEND_FEW_ROWS * (D / 8) / 32>(a, seq, j, head, value, threadIdx.x & 31,
-                                                                             red);
-    else
-        append_segment<D, T, FORMAT, VEC, APPEND_THREADS, 128 * (D / 8) / APPEND_THREADS>(a, seq, j, head, value,
-                                                                                         threadIdx.x, red);
+    const Segment s = segment_at(a, seq, j);
+    if (s.rows == 0) return;
+    const int team_shift = 31 - __clz(page * (D / 16)), team_size = 1 << team_shift, teams = blockDim.x >> team_shift;
+    const int team = threadIdx.x >> team_shift, t = threadIdx.x & (team_size - 1);
+    const int r = t / (D / 16), slot = t % (D / 16);
+    const bool mine = r < s.rows;
+    const fo_rows &src = value ? a.v : a.k;
+    const bool rotate = a.rotate && !value;
+    const int rot = a.rope.rot_dim, h2 = rot / 2;
+    const bool half = rotate && a.rope.layout == FO_ROPE_HALF;
+    const bool pair = LINED_UP && half && slot < rot / 16;
+    const int d0 = pair ? 8 * slot : 16 * slot, d1 = pair ? d0 + h2 : d0 + 8;
+    const T *row = static_cast<const T *>(src.data) + (s.row0 + (mine ? r : 0)) * src.row_stride;
+    auto load = [&](int head, Raw8<T> (&to)[2]) {
+        const T *x = row + head * src.head_stride;
+        if constexpr (VEC) {
+            to[0] = load_raw8(x + d0);
+            to[1] = load_raw8(x + d1);
+        } else {
+#pragma unroll
+            for (int g = 0; g < 2; g++)
+#pragma unroll
+                for (int e = 0; e < 8; e++) reinterpret_cast<T *>(to[g].w)[e] = x[(g ? d1 : d0) + e];
+        }
+    };
+    // The next head's rows are asked for while there are registers for them.
+    constexpr bool AHEAD = sizeof(T) == 2;
+    Raw8<T> now[2], next[2];
+    const int rounds = (heads + teams - 1) >> (31 - __clz(teams));
+    if (AHEAD && mine && head0 + team < head1) load(head0 + team, now);
+    bool inside = true;
+    const float2 *entries = nullptr;
+    if (rotate && mine) entries = entries_of(a, s.row0 + r, s.p0 + r, slot == 0, inside);
+    // Entries of the eight pairs, the same for every head: of (d0 + e, d1 + e), or
+    // of (d0 + 2 e, d0 + 2 e + 1).
+    float2 cs[8];
+    const bool turned = rotate && mine && (!half || pair) && d0 < rot;
+    if (turned) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const bool turn = pair || d0 + 2 * e < rot;
+            cs[e] = !turn ? make_float2(1.0f, 0.0f)
+                          : inside ? __ldg(entries + (pair ? d0 + e : d0 / 2 + e)) : make_float2(NAN, NAN);
+        }
+    }
+    bool valid;
+    const int64_t id = page_of(a.batch, a.kv.n_pages, s.seq, s.page, a.err, valid) * n_heads;
+    float *scales = (value ? a.kv.v_scales : a.kv.k_scales) + id;
+    uint8_t *codes = static_cast<uint8_t *>(value ? a.kv.v_codes : a.kv.k_codes) + id * page * D;
+    for (int round = 0; round < rounds; round++) {
+        const int head = head0 + round * teams + team;
+        const bool live = mine && head < head1;
+        if (!AHEAD && live) load(head, now);
+        const float old = s.begin > 0 && valid && head < head1 ? scales[head] : 0.0f;
+        if (AHEAD && mine && head + teams < head1) load(head + teams, next);
+        float y[16];
+        float m = 0.0f;
+        bool odd = false;
+        if (live) {
+            unpack8(now[0], y);
+            unpack8(now[1], y + 8);
+            if (pair) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float u = y[e], v = y[8 + e];
+                    y[e] = rot_first(u, v, cs[e]);
+                    y[8 + e] = rot_second(u, v, cs[e]);
+                }
+            } else if (turned) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    const float u = y[2 * e], v = y[2 * e + 1];
+                    const bool turn = d0 + 2 * e < rot;
+                    y[2 * e] = turn ? rot_first(u, v, cs[e]) : u;
+                    y[2 * e + 1] = turn ? rot_second(u, v, cs[e]) : v;
+                }
+            }
+            if constexpr (!LINED_UP) {
+                const T *x = row + head * src.head_stride;
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    const int i = d0 + e, p = i < h2 ? i : i - h2;
+                    if (!rotate || i >= rot) continue;
+                    const float2 c = inside ? __ldg(entries + p) : make_float2(NAN, NAN);
+                    y[e] = i < h2 ? rot_first(y[e], load1(x + i + h2), c) : rot_second(load1(x + i - h2), y[e], c);
+                }
+            }
+            note<16>(y, m, odd);
+        }
+        m = warp_max(m);
+        float *box = red[round & 1];
+        if ((threadIdx.x & 31) == 0) box[threadIdx.x >> 5] = m;
+        __syncthreads();
+        const int warps = team_size / 32, lane = threadIdx.x & 31;
+        m = warp_max(lane < warps ? box[team * warps + lane] : 0.0f);
+        if (odd) atomicOr(a.err, FO_DEVERR_VALUE);
+        if (valid && head < head1) {
+            const float scale = fmaxf(old, __fdiv_rn(m, code_max(FORMAT)));
+            uint8_t *at = codes + (int64_t)head * page * D;
+            if (scale > old && s.begin > 0) encode_again<D, FORMAT>(at, s.begin, __fdiv_rn(old, scale), t, team_size);
+            if (t == 0) scales[head] = scale;
+            if (live) {
+                const bool normal = scale >= 1e-30f;
+                const float inverse = normal ? __frcp_rn(scale) : 0.0f;
+                uint8_t *to = at + (s.begin + r) * D;
+                const uint2 c0 = encode8<FORMAT>(y, scale, inverse, odd || !normal);
+                const uint2 c1 = encode8<FORMAT>(y + 8, scale, inverse, odd || !normal);
+                if (pair) {
+                    *reinterpret_cast<uint2 *>(to + d0) = c0;
+                    *reinterpret_cast<uint2 *>(to + d1) = c1;
+                } else {
+                    *reinterpret_cast<uint4 *>(to + d0) = make_uint4(c0.x, c0.y, c1.x, c1.y);
+                }
+            }
+        }
+        if constexpr (AHEAD) {
+            now[0] = next[0];
+            now[1] = next[1];
+        }
+    }
 }
 
 template <int D, typename T, int FORMAT, bool VEC>
 cudaError_t launch_append(const fo_append_launch &in, cudaStream_t stream) {
     fo_append_launch a = in;
     const int64_t page = a.kv.page_size, heads2 = 2 * (int64_t)a.kv.n_kv_heads;
-    const bool few = a.batch.max_rows <= APPEND_FEW_ROWS;
-    // Few rows: every sequence has as many segments as it can touch.  Many
-    // rows of one number: likewise.  Many of different numbers: numbered by
-    // row_start.
-    const bool numbered = !few && a.batch.row_start;
-    const int64_t per_seq = numbered ? 0 : segments_of(a.batch.max_rows, page);
-    const int64_t segments = numbered ? a.batch.total_rows / page + 2 * a.batch.n_seqs : per_seq * a.batch.n_seqs;
-    const int64_t per_block = few ? APPEND_THREADS / 32 : 1;
-    const int64_t task_blocks = (segments * heads2 + per_block - 1) / per_block;
     bool q_vec = false;
-    int64_t q_blocks = 0;
+    int64_t q_blocks = 0;  // each of ROPE_THREADS threads
     if (a.q.rows > 0) {
         q_vec = rope_shape(&a.q);
         const int64_t rows = ROPE_THREADS / a.q.block_x;
         q_blocks = (a.q.rows + rows - 1) / rows;
     }
-    const int64_t grid = task_blocks + q_blocks;
-    if (grid > 0x7FFFFFFF) return cudaErrorInvalidValue;
     const bool q_half = a.rope.layout == FO_ROPE_HALF;
-    if (few)
-        paged_append_kernel<D, T, FORMAT, VEC, true><<<(unsigned)grid, APPEND_THREADS, 0, stream>>>(
-            a, task_blocks, segments, per_seq, q_half, q_vec);
+    if (a.batch.max_rows <= APPEND_FEW_ROWS) {
+        const int64_t per_seq = segments_of(a.batch.max_rows, page), per_block = APPEND_FEW_THREADS / 32;
+        const int64_t task_blocks = (per_seq * a.batch.n_seqs * heads2 + per_block - 1) / per_block;
+        if (task_blocks + q_blocks > 0x7FFFFFFF) return cudaErrorInvalidValue;
+        append_few_kernel<D, T, FORMAT, VEC><<<(unsigned)(task_blocks + q_blocks), APPEND_FEW_THREADS, 0, stream>>>(
+            a, (unsigned)task_blocks, (unsigned)per_seq, q_half, q_vec);
+        return cudaGetLastError();
+    }
+    const int64_t per_seq = a.batch.row_start ? 0 : segments_of(a.batch.max_rows, page);
+    const int64_t segments =
+        a.batch.row_start ? a.batch.total_rows / page + 2 * a.batch.n_seqs : per_seq * a.batch.n_seqs;
+    // Heads a block goes through: the more, the fewer reads of the rotation
+    // table; but blocks enough for every SM.
+    const int team = (int)page * (D / 16), threads = std::max(team, 256);
+    int heads = a.kv.n_kv_heads;
+    auto blocks = [&](int64_t h) { return segments * 2 * ((a.kv.n_kv_heads + h - 1) / h); };
+    while (heads > threads / team && blocks(heads) < 1184) heads = (heads + 1) / 2;
+    if (blocks(heads) > 0x7FFFFFFF) return cudaErrorInvalidValue;
+    const unsigned grid = (unsigned)blocks(heads);
+    if (!a.rotate || !q_half || a.rope.rot_dim % 16 == 0)
+        append_many_kernel<D, T, FORMAT, VEC, true><<<grid, threads, 0, stream>>>(a, (unsigned)per_seq, heads);
     else
-        paged_append_kernel<D, T, FORMAT, VEC, false><<<(unsigned)grid, APPEND_THREADS, 0, stream>>>(
-            a, task_blocks, segments, per_seq, q_half, q_vec);
+        append_many_kernel<D, T, FORMAT, VEC, false><<<grid, threads, 0, stream>>>(a, (unsigned)per_seq, heads);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess || q_blocks == 0) return e;
+    paged_rope_kernel<T><<<(unsigned)q_blocks, ROPE_THREADS, 0, stream>>>(a, q_half, q_vec);
     return cudaGetLastError();
 }
 
@@ -293,7 +475,6 @@ cudaError_t launch_append(const fo_append_launch &a, cudaStream_t stream) {
 }  // namespace fo
 
 extern "C" cudaError_t fo_launch_paged_append(const fo_append_launch *a, cudaStream_t stream) {
-    static_assert(fo::APPEND_THREADS == fo::ROPE_THREADS, "the queries' blocks have the tasks' width");
     if (a->batch.total_rows <= 0) return cudaSuccess;
     const bool f32 = a->k.dtype == FO_DT_F32;
     if (a->kv.head_dim == 64) return f32 ? fo::launch_append<64, float>(*a, stream) : fo::launch_append<64, uint16_t>(*a, stream);

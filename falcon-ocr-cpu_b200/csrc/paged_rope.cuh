@@ -8,7 +8,12 @@
 namespace fo {
 
 constexpr int ROPE_THREADS = 256;
-constexpr int ROPE_HEADS = 4;  // heads a thread takes, with one read of its table entries
+// Heads a thread takes with one read of its table entries: 64 or 128 bytes of
+// loads in flight for each thread.
+template <typename T, bool HALF>
+__host__ __device__ constexpr int rope_heads() {
+    return sizeof(T) == 4 && HALF ? 2 : 4;
+}
 
 // Work of one row: a slot is eight adjacent elements of a head (interleaved
 // layout, and elements that pass unrotated), or eight pairs (half layout:
@@ -30,7 +35,8 @@ inline bool rope_shape(fo_rope_launch *a) {
     const bool half = a->rope.layout == FO_ROPE_HALF;
     const bool vec = ok(a->x) && ok(a->out) && a->head_dim % 8 == 0 && (!half || a->rope.rot_dim % 16 == 0);
     a->slots = rope_slots(*a, vec, half);
-    a->head_blocks = (a->x.heads + ROPE_HEADS - 1) / ROPE_HEADS;
+    const int heads = a->x.dtype == FO_DT_F32 && half ? rope_heads<float, true>() : rope_heads<uint16_t, false>();
+    a->head_blocks = (a->x.heads + heads - 1) / heads;
     const int64_t width = (int64_t)a->slots * a->head_blocks;
     a->block_x = (int)(width < ROPE_THREADS ? (width < 1 ? 1 : width) : ROPE_THREADS);
     return vec;
@@ -47,93 +53,82 @@ __device__ __forceinline__ void rope_block(const fo_rope_launch &a, int64_t bloc
     const int ty = t / a.block_x, tx = t - ty * a.block_x;
     const int64_t row = block * rows_per_block + ty;
     if (ty >= rows_per_block || row >= a.rows) return;
-    bool padded;
-    const int64_t p = position(row, padded);
-    const bool inside = p >= 0 && p < a.rope.positions;
-    if (!inside && !padded && tx == 0) atomicOr(a.err, FO_DEVERR_POSITION);
+    constexpr int HEADS = rope_heads<T, HALF>();
     const int rot = a.rope.rot_dim, h2 = rot / 2;
-    const float2 *entries = reinterpret_cast<const float2 *>(a.rope.table) + (inside ? p : 0) * h2;
+    const T *xr = static_cast<const T *>(a.x.data) + row * a.x.row_stride;
+    T *yr = static_cast<T *>(a.out.data) + row * a.out.row_stride;
+    // A row's table entries: looked up behind the first loads of its elements,
+    // which do not wait for its position.
+    const float2 *entries = nullptr;
+    bool inside = false, padded = false;
+    auto look_up = [&]() {
+        if (entries) return;
+        const int64_t p = position(row, padded);
+        inside = p >= 0 && p < a.rope.positions;
+        if (!inside && !padded && tx == 0) atomicOr(a.err, FO_DEVERR_POSITION);
+        entries = reinterpret_cast<const float2 *>(a.rope.table) + (inside ? p : 0) * h2;
+    };
     auto entry = [&](int pair) {
         float2 cs = __ldg(entries + pair);
         if (!inside) cs = padded ? make_float2(1.0f, 0.0f) : make_float2(NAN, NAN);
         if (a.transpose) cs.y = -cs.y;
         return cs;
     };
-    const T *xr = static_cast<const T *>(a.x.data) + row * a.x.row_stride;
-    T *yr = static_cast<T *>(a.out.data) + row * a.out.row_stride;
     const int width = a.slots * a.head_blocks;
     for (int w = tx; w < width; w += a.block_x) {
+        // Heads hb, hb + head_blocks, ..: neighbouring threads take neighbouring
+        // heads.
         const int hb = w / a.slots, slot = w - hb * a.slots;
-        // Heads hb, hb + head_blocks, ..: neighbouring threads take
-        // neighbouring heads.
-        if constexpr (VEC && HALF) {
-            const int pairs8 = rot / 16;
-            if (slot < pairs8) {
-                const int d = slot * 8;
-                float x0[ROPE_HEADS][8], x1[ROPE_HEADS][8];
+        if constexpr (VEC) {
+            const bool pairs = HALF && slot < rot / 16;  // eight pairs: two groups of eight elements
+            const int d = !HALF || pairs ? slot * 8 : rot + (slot - rot / 16) * 8;
+            Raw8<T> r0[HEADS], r1[HEADS];
 #pragma unroll
-                for (int k = 0; k < ROPE_HEADS; k++) {
-                    const int h = hb + k * a.head_blocks;
-                    if (h < a.x.heads) {
-                        load8(xr + h * a.x.head_stride + d, x0[k]);
-                        load8(xr + h * a.x.head_stride + d + h2, x1[k]);
-                    }
-                }
-                float2 cs[8];
-#pragma unroll
-                for (int e = 0; e < 8; e++) cs[e] = entry(d + e);
-#pragma unroll
-                for (int k = 0; k < ROPE_HEADS; k++) {
-                    const int h = hb + k * a.head_blocks;
-                    if (h < a.x.heads) {
-                        float y0[8], y1[8];
-#pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            y0[e] = rot_first(x0[k][e], x1[k][e], cs[e]);
-                            y1[e] = rot_second(x0[k][e], x1[k][e], cs[e]);
-                        }
-                        store8(yr + h * a.out.head_stride + d, y0);
-                        store8(yr + h * a.out.head_stride + d + h2, y1);
-                    }
-                }
-            } else {
-                const int d = rot + (slot - pairs8) * 8;
-#pragma unroll
-                for (int k = 0; k < ROPE_HEADS; k++) {
-                    const int h = hb + k * a.head_blocks;
-                    float x[8];
-                    if (h < a.x.heads) {
-                        load8(xr + h * a.x.head_stride + d, x);
-                        store8(yr + h * a.out.head_stride + d, x);
-                    }
-                }
-            }
-        } else if constexpr (VEC) {
-            const int d = slot * 8;
-            float x[ROPE_HEADS][8];
-#pragma unroll
-            for (int k = 0; k < ROPE_HEADS; k++) {
-                const int h = hb + k * a.head_blocks;
-                if (h < a.x.heads) load8(xr + h * a.x.head_stride + d, x[k]);
-            }
-            float2 cs[4];
-#pragma unroll
-            for (int e = 0; e < 4; e++) cs[e] = d + 2 * e < rot ? entry(d / 2 + e) : make_float2(1.0f, 0.0f);
-#pragma unroll
-            for (int k = 0; k < ROPE_HEADS; k++) {
+            for (int k = 0; k < HEADS; k++) {
                 const int h = hb + k * a.head_blocks;
                 if (h < a.x.heads) {
-                    float y[8];
+                    r0[k] = load_raw8(xr + h * a.x.head_stride + d);
+                    if (HALF && pairs) r1[k] = load_raw8(xr + h * a.x.head_stride + d + h2);
+                }
+            }
+            float2 cs[HALF ? 8 : 4];
+            if (d < rot) {
+                look_up();
+#pragma unroll
+                for (int e = 0; e < (HALF ? 8 : 4); e++)
+                    cs[e] = HALF || d + 2 * e < rot ? entry(HALF ? d + e : d / 2 + e) : make_float2(1.0f, 0.0f);
+            }
+#pragma unroll
+            for (int k = 0; k < HEADS; k++) {
+                const int h = hb + k * a.head_blocks;
+                if (h >= a.x.heads) break;
+                T *to = yr + h * a.out.head_stride + d;
+                float x[8], y[8];
+                unpack8(r0[k], x);
+                if (d >= rot) {
+                    store8(to, x);
+                } else if constexpr (HALF) {
+                    float z[8];
+                    unpack8(r1[k], z);
+#pragma unroll
+                    for (int e = 0; e < 8; e++) {
+                        y[e] = rot_first(x[e], z[e], cs[e]);
+                        z[e] = rot_second(x[e], z[e], cs[e]);
+                    }
+                    store8(to, y);
+                    store8(to + h2, z);
+                } else {
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
-                        const bool turn = d + 2 * e < rot;  // a passing element keeps its bits
-                        y[2 * e] = turn ? rot_first(x[k][2 * e], x[k][2 * e + 1], cs[e]) : x[k][2 * e];
-                        y[2 * e + 1] = turn ? rot_second(x[k][2 * e], x[k][2 * e + 1], cs[e]) : x[k][2 * e + 1];
+                        const bool turn = d + 2 * e < rot;  // a passing element keeps its value
+                        y[2 * e] = turn ? rot_first(x[2 * e], x[2 * e + 1], cs[e]) : x[2 * e];
+                        y[2 * e + 1] = turn ? rot_second(x[2 * e], x[2 * e + 1], cs[e]) : x[2 * e + 1];
                     }
-                    store8(yr + h * a.out.head_stride + d, y);
+                    store8(to, y);
                 }
             }
         } else {
+            look_up();
             const bool pair = slot < h2;
             const int d0 = !pair ? rot + slot - h2 : HALF ? slot : 2 * slot;
             const int d1 = HALF ? slot + h2 : 2 * slot + 1;

@@ -5,7 +5,7 @@
 // {c, s} = table[p][pair].  Every value is read once and written once and a
 // table row serves all heads of a token, so the kernel is bound by HBM: a
 // thread takes the same eight elements (or the same eight pairs, in the half
-// layout) of up to ROPE_HEADS heads of one row, so its table entries are read
+// layout) of two or four heads of one row, so its table entries are read
 // once and all its loads are in flight together.
 #include "paged_rope.cuh"
 
@@ -40,7 +40,7 @@ __global__ void __launch_bounds__(256) rope_table_kernel(float2 *table, int64_t 
 }
 
 template <typename T, bool HALF, bool VEC>
-__global__ void __launch_bounds__(ROPE_THREADS) rope_kernel(const __grid_constant__ fo_rope_launch a) {
+__global__ void __launch_bounds__(ROPE_THREADS, 3) rope_kernel(const __grid_constant__ fo_rope_launch a) {
     rope_block<T, HALF, VEC>(a, blockIdx.x, [&](int64_t row, bool &padded) {
         padded = false;
         return a.rope.row_positions ? (int64_t)__ldg(a.rope.row_positions + row) : row;
