@@ -1908,7 +1908,7 @@ int fo_paged_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch 
         int sms = 0;
         FO_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, ctx->device), "cudaDeviceGetAttribute");
         const size_t parts = (size_t)2 * sms * FO_PAGED_QUERIES;
-        FO_CUDA(ctx->paged_parts.ensure(parts * (128 + 2) * 4 + (size_t)2 * sms * 4), "cudaMalloc(paged attention parts)");
+        FO_CUDA(ctx->paged_parts.ensure(parts * (128 + 2) * 4 + (size_t)sms * 4), "cudaMalloc(paged attention parts)");
         FO_CUDA(cudaMemsetAsync(ctx->paged_parts.ptr, 0, ctx->paged_parts.bytes, ctx->stream), "cudaMemset(parts)");
         ctx->sms = sms;
     }

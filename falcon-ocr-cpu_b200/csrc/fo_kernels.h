@@ -239,10 +239,11 @@ struct fo_paged_attention_launch {
     // Scratch of the context: a block's two unfinished parts and a counter.
     float *part_o;       // [2 sms][FO_PAGED_QUERIES][head_dim]
     float *part_ml;      // [2 sms][FO_PAGED_QUERIES][2]
-    unsigned *counters;  // [2 sms], zero between calls
+    unsigned *counters;  // [sms], zero between calls
     // Filled in by the launcher: query heads per KV head, queries that a block
-    // holds, warps that share a tile, and what 16-byte accesses may be used for.
-    int32_t group, queries, col_groups, q_vec, out_vec, evict_first;
+    // holds, warps that share a tile, what 16-byte accesses may be used for, and
+    // whether there are at most as many (sequence, KV head)s as blocks.
+    int32_t group, queries, col_groups, q_vec, out_vec, evict_first, whole_units;
 };
 #define FO_PAGED_QUERIES 48  // queries that a block holds at most
 cudaError_t fo_launch_paged_attention(const fo_paged_attention_launch *args, int sms, cudaStream_t stream);

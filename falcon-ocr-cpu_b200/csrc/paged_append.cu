@@ -443,7 +443,7 @@ cudaError_t launch_append(const fo_append_launch &in, cudaStream_t stream) {
     const int team = (int)page * (D / 16), threads = std::max(team, 256);
     int heads = a.kv.n_kv_heads;
     auto blocks = [&](int64_t h) { return segments * 2 * ((a.kv.n_kv_heads + h - 1) / h); };
-    while (heads > threads / team && blocks(heads) < 1184) heads = (heads + 1) / 2;
+    while (heads > threads / team && blocks(heads) < 592) heads = (heads + 1) / 2;
     if (blocks(heads) > 0x7FFFFFFF) return cudaErrorInvalidValue;
     const unsigned grid = (unsigned)blocks(heads);
     if (!a.rotate || !q_half || a.rope.rot_dim % 16 == 0)

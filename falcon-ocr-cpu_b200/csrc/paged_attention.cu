@@ -157,7 +157,8 @@ __device__ __forceinline__ PaWork pa_work(const fo_paged_attention_launch &a, in
     w.low = a.window > 0 ? (int)max64(p0 + 1 - a.window, 0) : 0;
     w.t0 = w.low / TILE;
     w.tiles = max((int)((w.s.len + TILE - 1) / TILE) - w.t0, 1);
-    w.groups = (w.s.n * a.group + a.queries - 1) / a.queries;
+    const int queries = w.s.n * a.group;
+    w.groups = queries <= a.queries ? queries > 0 : (queries + a.queries - 1) / a.queries;
     return w;
 }
 
@@ -167,8 +168,8 @@ template <int TILE>
 struct PaCursor {
     PaWork w;
     int seq, unit, tile;
-    __device__ __forceinline__ int head() const { return unit / w.groups; }
-    __device__ __forceinline__ int group() const { return unit % w.groups; }
+    __device__ __forceinline__ int head() const { return w.groups == 1 ? unit : unit / w.groups; }
+    __device__ __forceinline__ int group() const { return w.groups == 1 ? 0 : unit % w.groups; }
     __device__ __forceinline__ int left() const { return w.tiles - tile; }
     // Moves on by n tiles, at most to the unit's end.
     __device__ __forceinline__ void advance(const fo_paged_attention_launch &a, int n) {
@@ -188,6 +189,10 @@ struct PaShared {
     uint64_t full[PA_STAGES], empty[PA_STAGES];
     uint64_t q_full, q_free;        // a segment's queries are there; have been taken
     uint64_t part_full, part_free;  // its parts
+    // Of a unit that other blocks share, at the block's last segment (1) or its
+    // first one: its part is in scratch; whether this block joins them is known.
+    uint64_t shared_ready[2], shared_go[2];
+    int joins[2];
     float scales[PA_STAGES][16];    // keys' of a tile's pages, then values'
     int tile[PA_STAGES];            // the block's number of the tile in a slot
     float ml[PA_CONSUMERS][8][2];
@@ -242,6 +247,110 @@ __device__ __forceinline__ long long pa_share(long long total, int n) {
     long long x = (long long)((double)total / n);
     while (x * n < total) x++;
     return x;
+}
+
+// A unit's queries and the blocks [c0, c1] that share its tiles in the line.
+struct PaUnit {
+    int64_t first;  // the sequence's first row
+    int head, q0, n_queries, c0, c1;
+    bool alone;
+    // Scratch of block `cta`'s part (a block shares two units at most: the one it
+    // begins in, and the one that begins in it).
+    __device__ __forceinline__ int64_t part(const fo_paged_attention_launch &a, int cta, int qi) const {
+        return (2 * (int64_t)cta + (cta == c0 ? 1 : 0)) * a.queries + qi;
+    }
+};
+template <int TILE>
+__device__ __forceinline__ PaUnit pa_unit(const fo_paged_attention_launch &a, const PaCursor<TILE> &at, long long at_line,
+                                          int n, long long per) {
+    PaUnit u;
+    u.first = at.w.s.first;
+    u.head = at.head();
+    u.q0 = at.group() * a.queries;
+    u.n_queries = min(at.w.s.n * a.group - u.q0, a.queries);
+    u.alone = at.tile == 0 && n == at.w.tiles;
+    u.c0 = u.c1 = blockIdx.x;
+    if (!u.alone) {
+        const long long begin = at_line - at.tile, end = begin + at.w.tiles;
+        u.c0 = (int)((double)begin / (double)per);
+        u.c1 = (int)((double)(end - 1) / (double)per);
+    }
+    return u;
+}
+
+// Four dimensions of a query's output from their sum v, the sum ll of the
+// probabilities and the maximum mm that both are relative to.
+template <int D, bool F32>
+__device__ __forceinline__ void pa_write(const fo_paged_attention_launch &a, const PaUnit &u, int qi, int quad, float4 v,
+                                         float mm, float ll) {
+    using T = typename std::conditional<F32, float, uint16_t>::type;
+    const int q = u.q0 + qi, r = q / a.group, h = u.head * a.group + q - r * a.group;
+    float sum = ll;
+    if (a.sinks) sum += sm100::ex2(fmaf(__ldg(a.sinks + h), PA_LOG2E, -mm));
+    const float inv = ll == 0.0f ? 0.0f : 1.0f / sum;
+    v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
+    T *out = static_cast<T *>(a.out.data) + (u.first + r) * a.out.row_stride + h * a.out.head_stride + 4 * quad;
+    if (!a.out_vec) {
+        store1(out, v.x);
+        store1(out + 1, v.y);
+        store1(out + 2, v.z);
+        store1(out + 3, v.w);
+    } else if constexpr (F32) {
+        *reinterpret_cast<float4 *>(out) = v;
+    } else {
+        *reinterpret_cast<uint2 *>(out) = make_uint2(bf16_pair(v.x, v.y), bf16_pair(v.z, v.w));
+    }
+    if (a.lse && quad == 0) a.lse[(u.first + r) * a.q.heads + h] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * PA_LN2;
+}
+
+// The blocks' parts of a unit joined in their order, by warp `rank` of `warps`
+// (all of them in the last block to come), a query at a time: the maxima and
+// sums a block to a lane, then four dimensions to a lane.
+template <int D, bool F32>
+__device__ __forceinline__ void pa_join_blocks(const fo_paged_attention_launch &a, const PaUnit &u, int rank, int warps) {
+    constexpr int QUADS = D / 4, SETS = 32 / QUADS;  // lanes that share a quad take every SETS-th block
+    const int lane = threadIdx.x & 31, quad = lane % QUADS, set = lane / QUADS;
+    const int n = u.c1 - u.c0 + 1;
+    const float2 *mls = reinterpret_cast<const float2 *>(a.part_ml);
+    for (int qi = rank; qi < u.n_queries; qi += warps) {
+        float mm = -INFINITY;
+        bool lost = false;
+        for (int j = lane; j < n; j += 32) {
+            const float2 ml = __ldcg(mls + u.part(a, u.c0 + j, qi));
+            lost |= ml.x != ml.x || ml.y != ml.y;
+            mm = fmaxf(mm, ml.x);
+        }
+        mm = warp_max(mm);
+        lost = __any_sync(0xffffffffu, lost);
+        float ll = 0.0f;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int j0 = 0; j0 < n; j0 += 32) {
+            float f = 0.0f;
+            if (j0 + lane < n) {
+                const float2 ml = __ldcg(mls + u.part(a, u.c0 + j0 + lane, qi));
+                if (ml.x != -INFINITY) f = sm100::ex2(ml.x - mm);
+                ll = fmaf(ml.y, f, ll);
+            }
+            const int most = min(32, n - j0);
+#pragma unroll 8
+            for (int j = 0; j < most; j += SETS) {
+                const float fj = __shfl_sync(0xffffffffu, f, j + set);
+                if (j + set < most && fj != 0.0f) {
+                    const float4 x =
+                        __ldcg(reinterpret_cast<const float4 *>(a.part_o + u.part(a, u.c0 + j0 + j + set, qi) * D) + quad);
+                    v = make_float4(fmaf(x.x, fj, v.x), fmaf(x.y, fj, v.y), fmaf(x.z, fj, v.z), fmaf(x.w, fj, v.w));
+                }
+            }
+        }
+        ll = warp_sum(ll);
+        if constexpr (SETS == 2) {
+            v.x += __shfl_xor_sync(0xffffffffu, v.x, 16);
+            v.y += __shfl_xor_sync(0xffffffffu, v.y, 16);
+            v.z += __shfl_xor_sync(0xffffffffu, v.z, 16);
+            v.w += __shfl_xor_sync(0xffffffffu, v.w, 16);
+        }
+        if (set == 0) pa_write<D, F32>(a, u, qi, quad, v, mm, lost ? NAN : ll);
+    }
 }
 
 // The epilogue warps: `me` of PA_EPILOGUES takes every PA_EPILOGUES-th n8 tile of
@@ -361,94 +470,63 @@ __device__ __forceinline__ void pa_epilogue(const fo_paged_attention_launch &a, 
             if (!sm100::mbar_wait(&sh.q_free, segment & 1, &sh.abort, a.err)) return;
             split(next);
         }
-        const Sequence &s = at.w.s;
-        const int head = at.head(), q0 = at.group() * a.queries;
-        const int n_queries = min(s.n * a.group - q0, a.queries);
-        // The unit's tiles in the line, and the blocks that share it.
-        const long long unit_begin = begin + i - at.tile, unit_end = unit_begin + at.w.tiles;
-        const bool alone = unit_begin >= begin && unit_end <= begin + count;
-        int c0 = blockIdx.x, c1 = blockIdx.x;
-        if (!alone) {
-            c0 = (int)((double)unit_begin / (double)per);
-            c1 = (int)((double)(unit_end - 1) / (double)per);
-        }
+        const PaUnit u = pa_unit(a, at, begin + i, n, per);
         if (!sm100::mbar_wait(&sh.part_full, segment & 1, &sh.abort, a.err)) return;
-
-        // One query's four dimensions at a time, from parts in shared memory or, at
-        // the last block to come, in scratch.
-        auto at_part = [&](int cta, int qi) { return (2 * (int64_t)cta + (cta == c0 ? 1 : 0)) * a.queries + qi; };
-        auto join = [&](bool scratch) {
-            for (int x = lane; x < (n_queries - me + PA_EPILOGUES - 1) / PA_EPILOGUES * (D / 4); x += 32) {
-                const int quad = x % (D / 4), qi = x / (D / 4) * PA_EPILOGUES + me;
-                const int cg = qi / 8, col = qi % 8;
-                const int parts_n = scratch ? c1 - c0 + 1 : PA_CONSUMERS / a.col_groups;
-                float mm = -INFINITY, ll = 0.0f;
-                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                bool lost = false;
+        // The consumers' parts of one query, four dimensions at a time.
+        for (int x = lane; x < (u.n_queries - me + PA_EPILOGUES - 1) / PA_EPILOGUES * (D / 4); x += 32) {
+            const int quad = x % (D / 4), qi = x / (D / 4) * PA_EPILOGUES + me;
+            const int cg = qi / 8, col = qi % 8;
+            float mm = -INFINITY, ll = 0.0f;
+            float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            bool lost = false;
 #pragma unroll 4
-                for (int j = 0; j < parts_n; j++) {
-                    const int w = j * a.col_groups + cg;
-                    float2 ml;
-                    float4 u;
-                    if (scratch) {
-                        ml = __ldcg(reinterpret_cast<const float2 *>(a.part_ml) + at_part(c0 + j, qi));
-                        u = __ldcg(reinterpret_cast<const float4 *>(a.part_o + at_part(c0 + j, qi) * D) + quad);
-                    } else {
-                        ml = *reinterpret_cast<const float2 *>(sh.ml[w][col]);
-                        u = *reinterpret_cast<const float4 *>(parts + (w * 8 + col) * Shape::PART_LD + 4 * quad);
-                    }
-                    lost |= ml.x != ml.x || ml.y != ml.y;
-                    if (ml.x == -INFINITY) continue;  // it has seen nothing
-                    const float top = fmaxf(mm, ml.x);
-                    const float f0 = sm100::ex2(mm - top), f1 = sm100::ex2(ml.x - top);
-                    mm = top;
-                    ll = fmaf(ml.y, f1, ll * f0);
-                    v = make_float4(fmaf(u.x, f1, v.x * f0), fmaf(u.y, f1, v.y * f0), fmaf(u.z, f1, v.z * f0),
-                                    fmaf(u.w, f1, v.w * f0));
-                }
-                if (lost) ll = NAN;
-                if (!scratch && !alone) {
-                    const int64_t at_me = at_part(blockIdx.x, qi);
-                    __stcg(reinterpret_cast<float4 *>(a.part_o + at_me * D) + quad, v);
-                    if (quad == 0) __stcg(reinterpret_cast<float2 *>(a.part_ml) + at_me, make_float2(mm, ll));
-                    continue;
-                }
-                const int r = (q0 + qi) / a.group, h = head * a.group + (q0 + qi) - r * a.group;
-                float sum = ll;
-                if (a.sinks) sum += sm100::ex2(fmaf(__ldg(a.sinks + h), PA_LOG2E, -mm));
-                const float inv = ll == 0.0f ? 0.0f : 1.0f / sum;
-                T *out = static_cast<T *>(a.out.data) + (s.first + r) * a.out.row_stride + h * a.out.head_stride + 4 * quad;
-                if (!a.out_vec) {
-                    store1(out, v.x * inv);
-                    store1(out + 1, v.y * inv);
-                    store1(out + 2, v.z * inv);
-                    store1(out + 3, v.w * inv);
-                } else if constexpr (F32) {
-                    *reinterpret_cast<float4 *>(out) = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-                } else {
-                    *reinterpret_cast<uint2 *>(out) = make_uint2(bf16_pair(v.x * inv, v.y * inv), bf16_pair(v.z * inv, v.w * inv));
-                }
-                if (a.lse && quad == 0)
-                    a.lse[(s.first + r) * a.q.heads + h] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * PA_LN2;
+            for (int w = cg; w < PA_CONSUMERS; w += a.col_groups) {
+                const float2 ml = *reinterpret_cast<const float2 *>(sh.ml[w][col]);
+                lost |= ml.x != ml.x || ml.y != ml.y;
+                mm = fmaxf(mm, ml.x);
             }
-        };
-        join(false);
+#pragma unroll 4
+            for (int w = cg; w < PA_CONSUMERS; w += a.col_groups) {
+                const float2 ml = *reinterpret_cast<const float2 *>(sh.ml[w][col]);
+                if (ml.x == -INFINITY) continue;  // it has seen nothing, and left no output
+                const float4 z = *reinterpret_cast<const float4 *>(parts + (w * 8 + col) * Shape::PART_LD + 4 * quad);
+                const float f = sm100::ex2(ml.x - mm);
+                ll = fmaf(ml.y, f, ll);
+                v = make_float4(fmaf(z.x, f, v.x), fmaf(z.y, f, v.y), fmaf(z.z, f, v.z), fmaf(z.w, f, v.w));
+            }
+            if (lost) ll = NAN;
+            if (u.alone) {
+                pa_write<D, F32>(a, u, qi, quad, v, mm, ll);
+            } else {
+                const int64_t at_me = u.part(a, blockIdx.x, qi);
+                __stcg(reinterpret_cast<float4 *>(a.part_o + at_me * D) + quad, v);
+                if (quad == 0) __stcg(reinterpret_cast<float2 *>(a.part_ml) + at_me, make_float2(mm, ll));
+            }
+        }
         __syncwarp();
         if (lane == 0) sm100::mbar_arrive(&sh.part_free);
-        if (!alone) {
-            // The last of the blocks to come (this warp's counter) joins the parts in
-            // their order.
-            unsigned *counter = a.counters + PA_EPILOGUES * c0 + me;
-            unsigned before = 0;
+        if (!u.alone) {
+            // The last block to come (the unit's counter says so) joins the parts: with
+            // all its warps when this was its last segment, else with these two.
+            const int last = i + n == count;
             __threadfence();
             __syncwarp();
-            if (lane == 0) before = atomicAdd(counter, 1u);
-            before = __shfl_sync(0xffffffffu, before, 0);
-            if (before == (unsigned)(c1 - c0)) {
-                if (lane == 0) *counter = 0;
-                __threadfence();
-                join(true);
+            if (lane == 0) sm100::mbar_arrive(&sh.shared_ready[last]);
+            if (me == 0) {
+                if (!sm100::mbar_wait(&sh.shared_ready[last], 0, &sh.abort, a.err)) return;
+                if (lane == 0) {
+                    __threadfence();
+                    const bool joins = atomicAdd(a.counters + u.c0, 1u) == (unsigned)(u.c1 - u.c0);
+                    if (joins) a.counters[u.c0] = 0;
+                    __threadfence();
+                    sh.joins[last] = joins;
+                    sm100::mbar_arrive(&sh.shared_go[last]);
+                }
+                __syncwarp();
             }
+            if (!sm100::mbar_wait(&sh.shared_go[last], 0, &sh.abort, a.err)) return;
+            if (sh.joins[last])
+                pa_join_blocks<D, F32>(a, u, me, last ? PA_EPILOGUES + PA_CONSUMERS : PA_EPILOGUES);
         }
         i += n;
         at.advance(a, n);
@@ -489,50 +567,75 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         sm100::mbar_init(&sh.q_free, PA_CONSUMERS);
         sm100::mbar_init(&sh.part_full, PA_CONSUMERS);
         sm100::mbar_init(&sh.part_free, PA_EPILOGUES);
+        for (int i = 0; i < 2; i++) {
+            sm100::mbar_init(&sh.shared_ready[i], PA_EPILOGUES);
+            sm100::mbar_init(&sh.shared_go[i], 1);
+        }
         sm100::mbar_fence_init();
         for (int i = 0; i < STAGES; i++) sh.tile[i] = -1;
         sh.abort = 0;
     }
+    // A sequence's tiles, in the low 40 bits, and units.
     auto work_of = [&](int64_t seq) -> long long {
         if (seq >= a.batch.n_seqs) return 0;
         const PaWork w = pa_work<TILE>(a, seq);
-        return (long long)w.tiles * w.groups * a.kv.n_kv_heads;
+        const long long units = (long long)w.groups * a.kv.n_kv_heads;
+        return w.tiles * units | (a.whole_units ? units << 40 : 0);
     };
     long long all, mine = work_of(tid);
     long long before = pa_scan(mine, sh, all);
-    long long total = all, chunk = all;
-    for (int64_t base = PA_THREADS; base < a.batch.n_seqs; base += PA_THREADS) {
-        pa_scan(work_of(base + tid), sh, all);
-        total += all;
-    }
-    const long long per = max(pa_share(total, gridDim.x), (long long)key_groups);
-    const long long begin = per * blockIdx.x, end = min(begin + per, total);
-    if (begin >= end) return;
-    for (int64_t base = 0, sum = 0;;) {
-        if (begin >= sum + before && begin < sum + before + mine) {
-            sh.begin_seq = (int)base + tid;
-            sh.begin_base = sum + before;
-        }
-        base += PA_THREADS;
-        if (base >= a.batch.n_seqs) break;
-        // Only batches wider than a block come here.
-        sum += chunk;
-        mine = work_of(base + tid);
-        before = pa_scan(mine, sh, chunk);
-    }
-    __syncthreads();
     PaCursor<TILE> at;
-    at.seq = sh.begin_seq;
-    at.w = pa_work<TILE>(a, at.seq);
-    long long base = sh.begin_base;  // the line's number of at's sequence's first tile
-    {
-        const int in = (int)(begin - base);
+    long long per, begin, end;
+    // No more units than blocks, and short ones: a block for each, since handing a
+    // part on to another block takes longer (about 4 us) than these tiles.
+    const long long low40 = (1ll << 40) - 1;
+    if (a.whole_units && __syncthreads_and(mine >> 40 == 0 || (mine & low40) <= (mine >> 40) * 4 * key_groups)) {
+        const long long unit = blockIdx.x;
+        if (unit >= all >> 40) return;
+        if (unit >= before >> 40 && unit < (before >> 40) + (mine >> 40)) {
+            sh.begin_seq = tid;
+            sh.begin_base = before >> 40;
+        }
+        __syncthreads();
+        at.seq = sh.begin_seq;
+        at.w = pa_work<TILE>(a, at.seq);
+        at.unit = (int)(unit - sh.begin_base);
+        at.tile = 0;
+        per = begin = 0;
+        end = at.w.tiles;
+    } else {
+        if (a.whole_units) mine &= low40, before &= low40, all &= low40;
+        long long total = all, chunk = all;
+        for (int64_t base = PA_THREADS; base < a.batch.n_seqs; base += PA_THREADS) {
+            pa_scan(work_of(base + tid), sh, all);
+            total += all;
+        }
+        per = max(pa_share(total, gridDim.x), (long long)key_groups);
+        begin = per * blockIdx.x;
+        end = min(begin + per, total);
+        if (begin >= end) return;
+        for (int64_t base = 0, sum = 0;;) {
+            if (begin >= sum + before && begin < sum + before + mine) {
+                sh.begin_seq = (int)base + tid;
+                sh.begin_base = sum + before;
+            }
+            base += PA_THREADS;
+            if (base >= a.batch.n_seqs) break;
+            // Only batches wider than a block come here.
+            sum += chunk;
+            mine = work_of(base + tid);
+            before = pa_scan(mine, sh, chunk);
+        }
+        __syncthreads();
+        at.seq = sh.begin_seq;
+        at.w = pa_work<TILE>(a, at.seq);
+        const int in = (int)(begin - sh.begin_base);  // tiles of the sequence before
         at.unit = in / at.w.tiles;
         at.tile = in - at.unit * at.w.tiles;
     }
     const int count = (int)(end - begin);
-    const int page = a.kv.page_size;
-    const int pages = page >= TILE ? 1 : TILE / page;  // of a tile
+    const int page = a.kv.page_size, log_page = 31 - __clz(page);
+    const int pages = max(TILE >> log_page, 1);  // of a tile
 
     if (warp >= PA_CONSUMERS) {
         // ------------------------------------------------------------ producer
@@ -547,8 +650,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         // a batch of 32 pages at a time, the numbers two batches ahead of the
         // copies and the scales one.
         const int producer = warp - PA_CONSUMERS;
-        const int per_batch = 32 / pages;
-        const int j = lane % pages, off = lane / pages;
+        const int log_pages = 31 - __clz(pages), per_batch = 32 >> log_pages;
+        const int j = lane & (pages - 1), off = lane >> log_pages;
         struct Batch {
             int first, n;   // the block's tiles first, first + PA_PRODUCERS, ..: n of them
             int head, row;  // KV head, and this lane's page: its first row, its number (-1: none)
@@ -575,10 +678,10 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             b.n = (span - skip + PA_PRODUCERS - 1) / PA_PRODUCERS;
             b.head = at.head();
             // The first position that the page's copy holds.
-            const int64_t pos = (int64_t)(at.w.t0 + at.tile + skip + PA_PRODUCERS * off) * TILE + j * page;
-            const int64_t begins = pos / page * page;
+            const int64_t pos = (int64_t)(at.w.t0 + at.tile + skip + PA_PRODUCERS * off) * TILE + (j << log_page);
+            const int64_t begins = pos >> log_page << log_page;
             if (off < b.n && pos < at.w.s.len && begins + page > at.w.low) {
-                b.id = __ldg(a.batch.page_table + at.seq * a.batch.table_stride + pos / page);
+                b.id = __ldg(a.batch.page_table + at.seq * a.batch.table_stride + (pos >> log_page));
                 b.row = (int)(pos - begins);
             }
             ahead += span;
@@ -726,7 +829,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             if constexpr (!I8) {
                 // Rows beyond the sequence, or of pages that no row sees, may hold any
                 // bytes: an FP8 NaN times a probability of 0 would be NaN.
-                const int lo_row = max(at.w.low / page * page - pos0, 0), hi_row = (int)min64(s.len - pos0, HALF);
+                const int lo_row = max((at.w.low >> log_page << log_page) - pos0, 0), hi_row = (int)min64(s.len - pos0, HALF);
                 if (lo_row > 0 || hi_row < HALF) {
                     for (int x = lane; x < HALF * D / 16; x += 32) {
                         const int row = x / (D / 16);
@@ -993,6 +1096,12 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         }
         __syncwarp();
         if (lane == 0) sm100::mbar_arrive(&sh.part_full);
+        if (i + n == count && !(at.tile == 0 && n == at.w.tiles)) {
+            if (!sm100::mbar_wait(&sh.shared_go[1], 0, &sh.abort, a.err)) return;
+            if (sh.joins[1])
+                pa_join_blocks<D, F32>(a, pa_unit(a, at, begin + i, n, per), PA_EPILOGUES + warp,
+                                       PA_EPILOGUES + PA_CONSUMERS);
+        }
         i += n;
         at.advance(a, n);
     }
@@ -1086,6 +1195,10 @@ extern "C" cudaError_t fo_launch_paged_attention(const fo_paged_attention_launch
     const int64_t most = a.batch.n_seqs * a.kv.n_kv_heads * ((queries + a.queries - 1) / a.queries) *
                          ((a.batch.table_stride * a.kv.page_size * a.kv.head_dim + 8191) / 8192);
     const int64_t groups = fo::PA_CONSUMERS / 2 / a.col_groups;
-    const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(sms, (most + groups - 1) / groups));
+    const int64_t units = a.batch.n_seqs * a.kv.n_kv_heads * ((queries + a.queries - 1) / a.queries);
+    a.whole_units = units <= sms && a.batch.n_seqs <= fo::PA_THREADS;
+    int64_t blocks = std::min<int64_t>(sms, (most + groups - 1) / groups);
+    if (a.whole_units) blocks = std::max(blocks, units);
+    const unsigned grid = (unsigned)std::max<int64_t>(1, blocks);
     return a.kv.head_dim == 64 ? fo::launch_attention<64>(a, grid, stream) : fo::launch_attention<128>(a, grid, stream);
 }
