@@ -1889,6 +1889,13 @@ int fo_paged_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch 
     if (batch->max_rows > FO_PAGED_MAX_ROWS)
         return fail(FO_ERR_INVALID, "fo_paged_attention: at most %d rows a sequence", FO_PAGED_MAX_ROWS);
     if (!std::isfinite(scale)) return fail(FO_ERR_INVALID, "fo_paged_attention: scale must be finite");
+    // The kernel numbers the tables' 8 KB tiles of keys, for every 48 queries of
+    // a KV head, in 32 bits.
+    const double tiles = (double)batch->n_seqs * kv->n_kv_heads *
+                         ((double)batch->max_rows * (q->heads / kv->n_kv_heads) / FO_PAGED_QUERIES + 1) *
+                         ((double)batch->table_stride * kv->page_size * kv->head_dim / 8192 + 1);
+    if (tiles > INT32_MAX)
+        return fail(FO_ERR_CAPACITY, "fo_paged_attention: the batch's page tables have room for more than 2^31 tiles");
     if (window < 0) return fail(FO_ERR_INVALID, "fo_paged_attention: negative window");
     if (!aligned4(sinks) || !aligned4(lse)) return fail(FO_ERR_INVALID, "fo_paged_attention: misaligned sinks or lse");
     if (!ctx) return fail(FO_ERR_INVALID, "null context");
@@ -1902,7 +1909,7 @@ int fo_paged_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch 
     a.sinks = sinks;
     a.lse = lse;
     a.scale = scale;
-    a.window = window;
+    a.window = window < INT32_MAX ? (int32_t)window : 0;  // as many positions as there can be
     a.err = ctx->dev_err;
     if (!ctx->sms) {
         int sms = 0;

@@ -234,7 +234,7 @@ struct fo_paged_attention_launch {
     const float *sinks;
     float *lse;
     float scale;
-    int64_t window;
+    int32_t window;  // 0: none
     unsigned *err;
     // Scratch of the context: a block's two unfinished parts and a counter.
     float *part_o;       // [2 sms][FO_PAGED_QUERIES][head_dim]

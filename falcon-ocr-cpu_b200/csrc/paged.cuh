@@ -83,30 +83,30 @@ __device__ __forceinline__ float rot_second(float a, float b, float2 cs) {
 // max_rows; a length beyond the page table) raises FO_DEVERR_PAGED and leaves
 // the sequence without rows, or without positions.
 struct Sequence {
-    int64_t first, len;
-    int n;
+    int first, len, n;
 };
-__device__ __forceinline__ Sequence load_sequence(const fo_paged_batch &b, int page_size, int64_t seq, unsigned *err) {
+__device__ __forceinline__ Sequence load_sequence(const fo_paged_batch &b, int page_size, int seq, unsigned *err) {
+    // Rows and a table's positions are below 2^31 (checked on the host).
     Sequence s;
     s.len = __ldg(b.lens + seq);
     if (b.row_start) {
-        const int64_t r0 = __ldg(b.row_start + seq), r1 = __ldg(b.row_start + seq + 1);
+        const int r0 = __ldg(b.row_start + seq), r1 = __ldg(b.row_start + seq + 1);
         s.first = r0;
-        s.n = (int)(r1 - r0);
-        if (r0 < 0 || r1 < r0 || r1 > b.total_rows || r1 - r0 > b.max_rows) {
+        s.n = r1 - r0;
+        if (r0 < 0 || r1 < r0 || r1 > (int)b.total_rows || s.n > (int)b.max_rows) {
             atomicOr(err, FO_DEVERR_PAGED);
             s.first = 0;
             s.n = 0;
         }
     } else {
-        s.first = seq * b.max_rows;
+        s.first = seq * (int)b.max_rows;
         s.n = (int)b.max_rows;
     }
-    if (s.len > b.table_stride * page_size) {
+    if (s.len > (int)b.table_stride * page_size) {
         atomicOr(err, FO_DEVERR_PAGED);
         s.len = 0;
     }
-    if (s.len < 0) s.len = 0;
+    s.len = max(s.len, 0);
     return s;
 }
 

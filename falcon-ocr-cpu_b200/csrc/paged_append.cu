@@ -86,7 +86,7 @@ struct Segment {
 __device__ __forceinline__ Segment segment_at(const fo_append_launch &a, int seq, int j) {
     const int page = a.kv.page_size, shift = 31 - __clz(page);
     const Sequence s = load_sequence(a.batch, page, seq, a.err);
-    const int len = (int)s.len, from = max(len - s.n, 0);  // first position that is stored
+    const int len = s.len, from = max(len - s.n, 0);  // first position that is stored
     Segment g;
     g.seq = seq;
     g.page = (from >> shift) + j;
@@ -94,7 +94,7 @@ __device__ __forceinline__ Segment segment_at(const fo_append_launch &a, int seq
     const int p1 = (int)min64(len, (int64_t)(g.page + 1) << shift);
     g.rows = s.n > 0 && p1 > g.p0 ? p1 - g.p0 : 0;
     g.begin = g.p0 & (page - 1);
-    g.row0 = (int)s.first + (g.p0 - (len - s.n));
+    g.row0 = s.first + (g.p0 - (len - s.n));
     return g;
 }
 
@@ -226,7 +226,7 @@ __device__ __forceinline__ int64_t position_of_row(const fo_append_launch &a, in
     if (a.rope.row_positions) return (int64_t)__ldg(a.rope.row_positions + row);
     const int seq = a.batch.row_start ? sequence_of_row(a.batch, (int)row) : (int)((unsigned)row / (unsigned)a.batch.max_rows);
     const Sequence s = load_sequence(a.batch, a.kv.page_size, seq, a.err);
-    const int64_t p = s.len - s.n + (row - s.first);
+    const int p = s.len - s.n + ((int)row - s.first);
     padded = p < 0;
     return p;
 }

@@ -150,13 +150,13 @@ struct PaWork {
     int groups;  // groups of `queries` queries
 };
 template <int TILE>
-__device__ __forceinline__ PaWork pa_work(const fo_paged_attention_launch &a, int64_t seq) {
+__device__ __forceinline__ PaWork pa_work(const fo_paged_attention_launch &a, int seq) {
     PaWork w;
     w.s = load_sequence(a.batch, a.kv.page_size, seq, a.err);
-    const int64_t p0 = max64(w.s.len - w.s.n, 0);
-    w.low = a.window > 0 ? (int)max64(p0 + 1 - a.window, 0) : 0;
+    const int p0 = max(w.s.len - w.s.n, 0);
+    w.low = a.window > 0 ? max(p0 + 1 - a.window, 0) : 0;
     w.t0 = w.low / TILE;
-    w.tiles = max((int)((w.s.len + TILE - 1) / TILE) - w.t0, 1);
+    w.tiles = max((int)(((unsigned)w.s.len + TILE - 1) / TILE) - w.t0, 1);
     const int queries = w.s.n * a.group;
     w.groups = queries <= a.queries ? queries > 0 : (queries + a.queries - 1) / a.queries;
     return w;
@@ -198,9 +198,8 @@ struct PaShared {
     float ml[PA_CONSUMERS][8][2];
     float q_scale[FO_PAGED_QUERIES];
     int q_pos[FO_PAGED_QUERIES];
-    long long warp_sum[PA_THREADS / 32];
-    long long begin_base;
-    int begin_seq, abort;
+    int2 warp_sum[PA_THREADS / 32];
+    int begin_base, begin_seq, abort;
 };
 
 // Waits for the block's tile k in its slot; false when the block gave up.
@@ -220,38 +219,31 @@ __device__ __forceinline__ bool pa_wait_tile(PaShared &sh, int slot, int k, unsi
 }
 
 // Sum of x over the block's earlier threads; `all` the whole block's.
-__device__ __forceinline__ long long pa_scan(long long x, PaShared &sh, long long &all) {
+__device__ __forceinline__ int2 pa_scan(int2 x, PaShared &sh, int2 &all) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    long long incl = x;
+    int2 sum = x;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const long long y = __shfl_up_sync(0xffffffffu, incl, o);
-        if (lane >= o) incl += y;
+        const int u = __shfl_up_sync(0xffffffffu, sum.x, o), v = __shfl_up_sync(0xffffffffu, sum.y, o);
+        if (lane >= o) sum.x += u, sum.y += v;
     }
     __syncthreads();  // the last scan's sums have been read
-    if (lane == 31) sh.warp_sum[warp] = incl;
+    if (lane == 31) sh.warp_sum[warp] = sum;
     __syncthreads();
-    long long before = 0;
-    all = 0;
-#pragma unroll
+    int2 before = make_int2(sum.x - x.x, sum.y - x.y);
+    all = make_int2(0, 0);
+#pragma unroll 4
     for (int w = 0; w < PA_THREADS / 32; w++) {
-        if (w < warp) before += sh.warp_sum[w];
-        all += sh.warp_sum[w];
+        const int2 y = sh.warp_sum[w];
+        if (w < warp) before.x += y.x, before.y += y.y;
+        all.x += y.x, all.y += y.y;
     }
-    return before + incl - x;
-}
-
-// The smallest whole number of at least total / n (FP64 holds what there can be
-// of tiles exactly; its quotient is off by one at most).
-__device__ __forceinline__ long long pa_share(long long total, int n) {
-    long long x = (long long)((double)total / n);
-    while (x * n < total) x++;
-    return x;
+    return before;
 }
 
 // A unit's queries and the blocks [c0, c1] that share its tiles in the line.
 struct PaUnit {
-    int64_t first;  // the sequence's first row
+    int first;  // the sequence's first row
     int head, q0, n_queries, c0, c1;
     bool alone;
     // Scratch of block `cta`'s part (a block shares two units at most: the one it
@@ -261,8 +253,8 @@ struct PaUnit {
     }
 };
 template <int TILE>
-__device__ __forceinline__ PaUnit pa_unit(const fo_paged_attention_launch &a, const PaCursor<TILE> &at, long long at_line,
-                                          int n, long long per) {
+__device__ __forceinline__ PaUnit pa_unit(const fo_paged_attention_launch &a, const PaCursor<TILE> &at, int at_line,
+                                          int n, int per) {
     PaUnit u;
     u.first = at.w.s.first;
     u.head = at.head();
@@ -271,9 +263,9 @@ __device__ __forceinline__ PaUnit pa_unit(const fo_paged_attention_launch &a, co
     u.alone = at.tile == 0 && n == at.w.tiles;
     u.c0 = u.c1 = blockIdx.x;
     if (!u.alone) {
-        const long long begin = at_line - at.tile, end = begin + at.w.tiles;
-        u.c0 = (int)((double)begin / (double)per);
-        u.c1 = (int)((double)(end - 1) / (double)per);
+        const int begin = at_line - at.tile;
+        u.c0 = begin / per;
+        u.c1 = (begin + at.w.tiles - 1) / per;
     }
     return u;
 }
@@ -289,7 +281,7 @@ __device__ __forceinline__ void pa_write(const fo_paged_attention_launch &a, con
     if (a.sinks) sum += sm100::ex2(fmaf(__ldg(a.sinks + h), PA_LOG2E, -mm));
     const float inv = ll == 0.0f ? 0.0f : 1.0f / sum;
     v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
-    T *out = static_cast<T *>(a.out.data) + (u.first + r) * a.out.row_stride + h * a.out.head_stride + 4 * quad;
+    T *out = static_cast<T *>(a.out.data) + (int64_t)(u.first + r) * a.out.row_stride + h * a.out.head_stride + 4 * quad;
     if (!a.out_vec) {
         store1(out, v.x);
         store1(out + 1, v.y);
@@ -300,7 +292,7 @@ __device__ __forceinline__ void pa_write(const fo_paged_attention_launch &a, con
     } else {
         *reinterpret_cast<uint2 *>(out) = make_uint2(bf16_pair(v.x, v.y), bf16_pair(v.z, v.w));
     }
-    if (a.lse && quad == 0) a.lse[(u.first + r) * a.q.heads + h] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * PA_LN2;
+    if (a.lse && quad == 0) a.lse[(int64_t)(u.first + r) * a.q.heads + h] = ll == 0.0f ? -INFINITY : (mm + log2f(ll)) * PA_LN2;
 }
 
 // The blocks' parts of a unit joined in their order, by warp `rank` of `warps`
@@ -357,7 +349,7 @@ __device__ __forceinline__ void pa_join_blocks(const fo_paged_attention_launch &
 // queries to split into operands, and every such query to join and write.
 template <int D, int FORMAT, bool F32, int TILE>
 __device__ __forceinline__ void pa_epilogue(const fo_paged_attention_launch &a, PaShared &sh, PaCursor<TILE> at, int count,
-                                            long long begin, long long per, int me, float *parts, uint2 *q_ops) {
+                                            int begin, int per, int me, float *parts, uint2 *q_ops) {
     using Shape = PaShape<D, FORMAT, F32>;
     using T = typename std::conditional<F32, float, uint16_t>::type;
     constexpr bool I8 = FORMAT == FO_PAGED_I8;
@@ -375,7 +367,7 @@ __device__ __forceinline__ void pa_epilogue(const fo_paged_attention_launch &a, 
             int r = 0;
             if (qi < n_queries) {
                 r = (q0 + qi) / a.group;
-                q = static_cast<const T *>(a.q.data) + (u.w.s.first + r) * a.q.row_stride +
+                q = static_cast<const T *>(a.q.data) + (int64_t)(u.w.s.first + r) * a.q.row_stride +
                     (head * a.group + (q0 + qi) - r * a.group) * a.q.head_stride + 16 * t;
             }
             // Read twice, 16 elements at a time: the largest first.
@@ -416,7 +408,7 @@ __device__ __forceinline__ void pa_epilogue(const fo_paged_attention_launch &a, 
             if (t == 0) {
                 const bool good = (all_finite >> (lane & 28) & 15) == 15;
                 sh.q_scale[qi] = good ? __uint_as_float((uint32_t)e << 23) / up * a.scale * PA_LOG2E : NAN;
-                sh.q_pos[qi] = q ? (int)(u.w.s.len - u.w.s.n) + r : -1;
+                sh.q_pos[qi] = q ? u.w.s.len - u.w.s.n + r : -1;
             }
             uint2 *to = q_ops + tile * (Shape::Q_TILE / 8) + lane;
 #pragma unroll 1
@@ -557,83 +549,108 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int key_groups = PA_CONSUMERS / 2 / a.col_groups;
 
-    // This block's piece [begin, end) of the line, and where it begins.
-    if (tid == 0) {
-        for (int i = 0; i < STAGES; i++) {
-            sm100::mbar_init(&sh.full[i], 1);
-            sm100::mbar_init(&sh.empty[i], 2 * a.col_groups);
+    if (warp == PA_THREADS / 32 - 1) {
+        if (lane < STAGES) {
+            sm100::mbar_init(&sh.full[lane], 1);
+            sm100::mbar_init(&sh.empty[lane], 2 * a.col_groups);
+            sh.tile[lane] = -1;
         }
-        sm100::mbar_init(&sh.q_full, PA_EPILOGUES);
-        sm100::mbar_init(&sh.q_free, PA_CONSUMERS);
-        sm100::mbar_init(&sh.part_full, PA_CONSUMERS);
-        sm100::mbar_init(&sh.part_free, PA_EPILOGUES);
-        for (int i = 0; i < 2; i++) {
-            sm100::mbar_init(&sh.shared_ready[i], PA_EPILOGUES);
-            sm100::mbar_init(&sh.shared_go[i], 1);
+        if (lane == 8) sm100::mbar_init(&sh.q_full, PA_EPILOGUES), sm100::mbar_init(&sh.part_free, PA_EPILOGUES);
+        if (lane == 9) sm100::mbar_init(&sh.q_free, PA_CONSUMERS), sm100::mbar_init(&sh.part_full, PA_CONSUMERS);
+        if (lane == 10 || lane == 11) {
+            sm100::mbar_init(&sh.shared_ready[lane - 10], PA_EPILOGUES);
+            sm100::mbar_init(&sh.shared_go[lane - 10], 1);
         }
         sm100::mbar_fence_init();
-        for (int i = 0; i < STAGES; i++) sh.tile[i] = -1;
-        sh.abort = 0;
+        if (lane == 12) sh.abort = 0;
     }
-    // A sequence's tiles, in the low 40 bits, and units.
-    auto work_of = [&](int64_t seq) -> long long {
-        if (seq >= a.batch.n_seqs) return 0;
-        const PaWork w = pa_work<TILE>(a, seq);
-        const long long units = (long long)w.groups * a.kv.n_kv_heads;
-        return w.tiles * units | (a.whole_units ? units << 40 : 0);
-    };
-    long long all, mine = work_of(tid);
-    long long before = pa_scan(mine, sh, all);
-    PaCursor<TILE> at;
-    long long per, begin, end;
+    // This block's piece [begin, end) of the line, and where it begins.  (The
+    // line's tiles are below 2^31, checked on the host.)
     // No more units than blocks, and short ones: a block for each, since handing a
     // part on to another block takes longer (about 4 us) than these tiles.
-    const long long low40 = (1ll << 40) - 1;
-    if (a.whole_units && __syncthreads_and(mine >> 40 == 0 || (mine & low40) <= (mine >> 40) * 4 * key_groups)) {
-        const long long unit = blockIdx.x;
-        if (unit >= all >> 40) return;
-        if (unit >= before >> 40 && unit < (before >> 40) + (mine >> 40)) {
-            sh.begin_seq = tid;
-            sh.begin_base = before >> 40;
+    const int n_seqs = (int)a.batch.n_seqs, few = 4 * key_groups;
+    PaCursor<TILE> at;
+    int per = 0, begin = 0, end, base;
+    bool whole = false;
+    auto work_of = [&](int seq, PaWork &w) {  // its tiles and units
+        if (seq >= n_seqs) return make_int2(0, 0);
+        w = pa_work<TILE>(a, seq);
+        const int units = w.groups * a.kv.n_kv_heads;
+        return make_int2(w.tiles * units, units);
+    };
+    if (n_seqs <= 32) {
+        // Every warp for itself, a sequence to a lane.
+        PaWork w = {};
+        const int2 mine = work_of(lane, w);
+        int2 sum = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int u = __shfl_up_sync(0xffffffffu, sum.x, o), v = __shfl_up_sync(0xffffffffu, sum.y, o);
+            if (lane >= o) sum.x += u, sum.y += v;
         }
-        __syncthreads();
-        at.seq = sh.begin_seq;
-        at.w = pa_work<TILE>(a, at.seq);
-        at.unit = (int)(unit - sh.begin_base);
-        at.tile = 0;
-        per = begin = 0;
-        end = at.w.tiles;
+        const int2 all = make_int2(__shfl_sync(0xffffffffu, sum.x, 31), __shfl_sync(0xffffffffu, sum.y, 31));
+        whole = a.whole_units && __all_sync(0xffffffffu, mine.y == 0 || w.tiles <= few);
+        if (!whole) {
+            per = max((int)((unsigned)(all.x + gridDim.x - 1) / gridDim.x), key_groups);
+            begin = (int)min((long long)per * blockIdx.x, (long long)all.x);
+        }
+        end = whole ? all.y : (int)min((long long)begin + per, (long long)all.x);
+        if (whole ? (int)blockIdx.x >= end : begin >= end) return;
+        const int at_line = whole ? (int)blockIdx.x : begin, before = whole ? sum.y - mine.y : sum.x - mine.x;
+        const int own = __ffs(__ballot_sync(0xffffffffu, at_line >= before && at_line < before + (whole ? mine.y : mine.x))) - 1;
+        at.seq = own;
+        base = __shfl_sync(0xffffffffu, before, own);
+        at.w.s.first = __shfl_sync(0xffffffffu, w.s.first, own);
+        at.w.s.len = __shfl_sync(0xffffffffu, w.s.len, own);
+        at.w.s.n = __shfl_sync(0xffffffffu, w.s.n, own);
+        at.w.low = __shfl_sync(0xffffffffu, w.low, own);
+        at.w.t0 = __shfl_sync(0xffffffffu, w.t0, own);
+        at.w.tiles = __shfl_sync(0xffffffffu, w.tiles, own);
+        at.w.groups = __shfl_sync(0xffffffffu, w.groups, own);
+        __syncthreads();  // the barriers are there
     } else {
-        if (a.whole_units) mine &= low40, before &= low40, all &= low40;
-        long long total = all, chunk = all;
-        for (int64_t base = PA_THREADS; base < a.batch.n_seqs; base += PA_THREADS) {
-            pa_scan(work_of(base + tid), sh, all);
-            total += all;
+        PaWork w = {};
+        int2 all, mine = work_of(tid, w), before = pa_scan(mine, sh, all), chunk = all;
+        whole = a.whole_units && __syncthreads_and(mine.y == 0 || w.tiles <= few);
+        for (int first = PA_THREADS; first < n_seqs; first += PA_THREADS) {
+            int2 more;
+            pa_scan(work_of(first + tid, w), sh, more);
+            all.x += more.x;
         }
-        per = max(pa_share(total, gridDim.x), (long long)key_groups);
-        begin = per * blockIdx.x;
-        end = min(begin + per, total);
-        if (begin >= end) return;
-        for (int64_t base = 0, sum = 0;;) {
-            if (begin >= sum + before && begin < sum + before + mine) {
-                sh.begin_seq = (int)base + tid;
-                sh.begin_base = sum + before;
+        if (!whole) {
+            per = max((int)((unsigned)(all.x + gridDim.x - 1) / gridDim.x), key_groups);
+            begin = (int)min((long long)per * blockIdx.x, (long long)all.x);
+        }
+        end = whole ? all.y : (int)min((long long)begin + per, (long long)all.x);
+        if (whole ? (int)blockIdx.x >= end : begin >= end) return;
+        const int at_line = whole ? (int)blockIdx.x : begin;
+        for (int first = 0, sum = 0;;) {
+            const int from = sum + (whole ? before.y : before.x);
+            if (at_line >= from && at_line < from + (whole ? mine.y : mine.x)) {
+                sh.begin_seq = first + tid;
+                sh.begin_base = from;
             }
-            base += PA_THREADS;
-            if (base >= a.batch.n_seqs) break;
+            first += PA_THREADS;
+            if (first >= n_seqs) break;
             // Only batches wider than a block come here.
-            sum += chunk;
-            mine = work_of(base + tid);
+            sum += chunk.x;
+            mine = work_of(first + tid, w);
             before = pa_scan(mine, sh, chunk);
         }
         __syncthreads();
         at.seq = sh.begin_seq;
+        base = sh.begin_base;
         at.w = pa_work<TILE>(a, at.seq);
-        const int in = (int)(begin - sh.begin_base);  // tiles of the sequence before
-        at.unit = in / at.w.tiles;
-        at.tile = in - at.unit * at.w.tiles;
     }
-    const int count = (int)(end - begin);
+    if (whole) {
+        at.unit = blockIdx.x - base;
+        at.tile = 0;
+        end = at.w.tiles;
+    } else {
+        at.unit = (begin - base) / at.w.tiles;
+        at.tile = (begin - base) - at.unit * at.w.tiles;
+    }
+    const int count = end - begin;
     const int page = a.kv.page_size, log_page = 31 - __clz(page);
     const int pages = max(TILE >> log_page, 1);  // of a tile
 
@@ -786,7 +803,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         const int n = min(at.left(), count - i);
         const Sequence &s = at.w.s;
         const int n_queries = min(s.n * a.group - at.group() * a.queries, a.queries);  // of this unit
-        const int p_first = (int)(s.len - s.n);  // positions of the sequence's first row and of its last
+        const int p_first = s.len - s.n;  // positions of the sequence's first row and of its last
         const int p_last = p_first + s.n - 1;
         // The queries as B operands.
         uint2 qf[Q_REGS ? QT * KQ : 1];
@@ -808,7 +825,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         }
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[MT][4] = {};
         // Tiles all of whose positions every row sees need no mask.
-        const int low_last = a.window > 0 ? max(p_last + 1 - (int)min64(a.window, INT32_MAX / 2), 0) : 0;
+        const int low_last = a.window > 0 ? max(p_last + 1 - a.window, 0) : 0;
         bool any = false;
 
         int k = i + (key_group - i % key_groups + key_groups) % key_groups;
@@ -829,7 +846,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             if constexpr (!I8) {
                 // Rows beyond the sequence, or of pages that no row sees, may hold any
                 // bytes: an FP8 NaN times a probability of 0 would be NaN.
-                const int lo_row = max((at.w.low >> log_page << log_page) - pos0, 0), hi_row = (int)min64(s.len - pos0, HALF);
+                const int lo_row = max((at.w.low >> log_page << log_page) - pos0, 0), hi_row = min(s.len - pos0, HALF);
                 if (lo_row > 0 || hi_row < HALF) {
                     for (int x = lane; x < HALF * D / 16; x += 32) {
                         const int row = x / (D / 16);
@@ -1200,5 +1217,6 @@ extern "C" cudaError_t fo_launch_paged_attention(const fo_paged_attention_launch
     int64_t blocks = std::min<int64_t>(sms, (most + groups - 1) / groups);
     if (a.whole_units) blocks = std::max(blocks, units);
     const unsigned grid = (unsigned)std::max<int64_t>(1, blocks);
+    if (most > INT32_MAX) return cudaErrorInvalidValue;
     return a.kv.head_dim == 64 ? fo::launch_attention<64>(a, grid, stream) : fo::launch_attention<128>(a, grid, stream);
 }

@@ -568,7 +568,9 @@ int fo_paged_append(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch *ba
  * s_j = scale * q . k_j: out = sum_j exp(s_j) v_j / (sum_j exp(s_j) +
  * exp(sinks[head])), sinks NULL: without that term; lse (NULL: not wanted)
  * [total_rows][n_heads] = ln sum_j exp(s_j).  A row that sees nothing gives 0
- * and -infinity.  max_rows is at most 64. */
+ * and -infinity.  max_rows is at most 64, and the page tables' 8 KB tiles of
+ * keys, of all KV heads and for every 48 query rows of one, are at most 2^31
+ * (FO_ERR_CAPACITY). */
 int fo_paged_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch *batch, const fo_rows *q,
                        const float *sinks, float scale, int64_t window, const fo_rows *out, float *lse);
 
