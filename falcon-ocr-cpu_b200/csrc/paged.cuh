@@ -10,6 +10,30 @@
 
 namespace fo {
 
+// ------------------------------------------------------------------ launches
+// The kernels here follow one another closely (a decode step is an append and
+// an attention, of some microseconds each): each lets the next one be set up as
+// soon as all its own blocks run, and waits for the one before it to be over
+// before it touches memory.
+__device__ __forceinline__ void wait_for_prior_kernel() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+template <typename... Params, typename... Args>
+cudaError_t launch(void (*kernel)(Params...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream, Args... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 // ------------------------------------------------------------- row elements
 // Ordinary loads: fo_rope may write the rows that it reads.
 template <typename T>

@@ -564,6 +564,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         sm100::mbar_fence_init();
         if (lane == 12) sh.abort = 0;
     }
+    wait_for_prior_kernel();
     // This block's piece [begin, end) of the line, and where it begins.  (The
     // line's tiles are below 2^31, checked on the host.)
     // No more units than blocks, and short ones: a block for each, since handing a
@@ -1175,8 +1176,7 @@ cudaError_t launch_attention(const fo_paged_attention_launch &a, unsigned grid, 
     }
     CUtensorMap k_map, v_map;
     if (!pa_map(&k_map, a.kv.k_codes, a.kv) || !pa_map(&v_map, a.kv.v_codes, a.kv)) return cudaErrorNotSupported;
-    kernel<<<grid, PA_THREADS, Shape::smem(a.queries / 8), stream>>>(k_map, v_map, a);
-    return cudaGetLastError();
+    return launch(kernel, dim3(grid), dim3(PA_THREADS), Shape::smem(a.queries / 8), stream, k_map, v_map, a);
 }
 
 template <int D>

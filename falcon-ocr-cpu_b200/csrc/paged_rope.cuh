@@ -42,13 +42,11 @@ inline bool rope_shape(fo_rope_launch *a) {
     return vec;
 }
 
-// Block `block` of the rotation; `position(row, padded)` gives a row's
+// Block `block` of the rotation, thread t of ROPE_THREADS; `position(row, padded)` gives a row's
 // position, or sets padded (the row is copied as it is).
 template <typename T, bool HALF, bool VEC, typename Position>
-__device__ __forceinline__ void rope_block(const fo_rope_launch &a, int64_t block, Position position) {
-    // Threads x over (head block, slot), y over rows; the block's shape is
-    // recomputed from block_x so that it also runs inside a 1-D block.
-    const int t = threadIdx.y * blockDim.x + threadIdx.x;
+__device__ __forceinline__ void rope_block(const fo_rope_launch &a, int64_t block, int t, Position position) {
+    // block_x threads over (head block, slot), the others over rows.
     const int rows_per_block = ROPE_THREADS / a.block_x;
     const int ty = t / a.block_x, tx = t - ty * a.block_x;
     const int64_t row = block * rows_per_block + ty;

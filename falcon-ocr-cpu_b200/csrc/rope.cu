@@ -41,7 +41,8 @@ __global__ void __launch_bounds__(256) rope_table_kernel(float2 *table, int64_t 
 
 template <typename T, bool HALF, bool VEC>
 __global__ void __launch_bounds__(ROPE_THREADS, 3) rope_kernel(const __grid_constant__ fo_rope_launch a) {
-    rope_block<T, HALF, VEC>(a, blockIdx.x, [&](int64_t row, bool &padded) {
+    wait_for_prior_kernel();
+    rope_block<T, HALF, VEC>(a, blockIdx.x, threadIdx.x, [&](int64_t row, bool &padded) {
         padded = false;
         return a.rope.row_positions ? (int64_t)__ldg(a.rope.row_positions + row) : row;
     });
@@ -63,10 +64,11 @@ extern "C" cudaError_t fo_launch_rope(const fo_rope_launch *args, cudaStream_t s
     if (args->rows <= 0 || args->x.heads <= 0) return cudaSuccess;
     fo_rope_launch a = *args;
     const bool vec = fo::rope_shape(&a);
-    const dim3 block(a.block_x, fo::ROPE_THREADS / a.block_x);
-    const unsigned grid = (unsigned)((a.rows + block.y - 1) / block.y);
+    const int rows = fo::ROPE_THREADS / a.block_x;
+    const unsigned grid = (unsigned)((a.rows + rows - 1) / rows), block = fo::ROPE_THREADS;
     const bool half = a.rope.layout == FO_ROPE_HALF;
-    auto go = [&](auto *kernel) { kernel<<<grid, block, 0, stream>>>(a); };
+    cudaError_t e = cudaSuccess;
+    auto go = [&](auto *kernel) { e = fo::launch(kernel, grid, block, 0, stream, a); };
     if (a.x.dtype == FO_DT_F32) {
         if (half) vec ? go(fo::rope_kernel<float, true, true>) : go(fo::rope_kernel<float, true, false>);
         else vec ? go(fo::rope_kernel<float, false, true>) : go(fo::rope_kernel<float, false, false>);
@@ -74,5 +76,5 @@ extern "C" cudaError_t fo_launch_rope(const fo_rope_launch *args, cudaStream_t s
         if (half) vec ? go(fo::rope_kernel<uint16_t, true, true>) : go(fo::rope_kernel<uint16_t, true, false>);
         else vec ? go(fo::rope_kernel<uint16_t, false, true>) : go(fo::rope_kernel<uint16_t, false, false>);
     }
-    return cudaGetLastError();
+    return e;
 }

@@ -18,6 +18,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 from typing import Optional, Sequence
 
 import numpy as np
@@ -94,6 +95,10 @@ class Rows(ctypes.Structure):
     """fo_rows: rows of heads in device memory."""
     _fields_ = [("data", ctypes.c_void_p), ("row_stride", ctypes.c_int64), ("head_stride", ctypes.c_int64),
                 ("heads", ctypes.c_int32), ("dtype", ctypes.c_int32)]
+
+
+_PACK_ROWS = struct.Struct("=QqqiI").pack  # Rows and RopeSpec as bytes: a third of a Structure's time
+_PACK_ROPE = struct.Struct("=QqQii").pack
 
 
 class RopeScaling(ctypes.Structure):
@@ -735,7 +740,7 @@ def stream_context(device: int) -> Context:
     return ctx
 
 
-def _rows(t, name: str) -> Rows:
+def _rows(t, name: str) -> bytes:
     """A CUDA tensor [rows][heads][head_dim] as fo_rows; rows and heads in any
     strides."""
     if _ROW_TYPES is None:
@@ -743,15 +748,21 @@ def _rows(t, name: str) -> Rows:
     kind = _ROW_TYPES.get(t.dtype)
     if kind is None or not t.is_cuda or t.dim() != 3:
         raise FoError(f"{name} must be a CUDA tensor [rows][heads][head_dim] of float32 or bfloat16")
-    shape, stride = t.shape, t.stride()
-    if stride[2] != 1:
+    row, head, one = t.stride()
+    if one != 1:
         raise FoError(f"{name}: a head's values must be adjacent")
-    return Rows(t.data_ptr(), stride[0], stride[1], shape[1], kind)
+    return _PACK_ROWS(t.data_ptr(), row, head, t.size(1), kind)
 
 
 def _device_ints(t, name: str):
-    if not _on_device(t) or not t.is_contiguous() or str(t.dtype) != "torch.int32":
+    if not t.is_cuda or not t.is_contiguous() or t.dtype != _torch().int32:
         raise FoError(f"{name} must be a contiguous CUDA tensor of int32")
+    return t.data_ptr()
+
+
+def _floats(t, n: int, name: str):
+    if not t.is_cuda or not t.is_contiguous() or t.numel() != n or t.dtype != _torch().float32:
+        raise FoError(f"{name} must be a contiguous CUDA tensor of {n} float32")
     return t.data_ptr()
 
 
@@ -779,13 +790,15 @@ class Rope:
         self.table = table
         self.spec = (table.data_ptr(), table.shape[0], 2 * table.shape[1], ROPE_LAYOUTS[layout])
 
-    def at(self, positions, rows: int) -> RopeSpec:
-        table, n, rot_dim, layout = self.spec
+        self.plain = _PACK_ROPE(self.spec[0], self.spec[1], 0, self.spec[2], self.spec[3])
+
+    def at(self, positions, rows: int) -> bytes:
         if positions is None:
-            return RopeSpec(table, n, None, rot_dim, layout)
+            return self.plain
         if positions.numel() != rows:
             raise FoError("one position for each row")
-        return RopeSpec(table, n, _device_ints(positions, "positions"), rot_dim, layout)
+        table, n, rot_dim, layout = self.spec
+        return _PACK_ROPE(table, n, _device_ints(positions, "positions"), rot_dim, layout)
 
 
 def rope(x, out, rope: Rope, positions=None, inverse=False, ctx=None):
@@ -793,12 +806,12 @@ def rope(x, out, rope: Rope, positions=None, inverse=False, ctx=None):
     allowed) at `positions` [rows] int32 (None: the row's number).  inverse:
     the transposed rotation, which takes a gradient back."""
     a, b = _rows(x, "x"), _rows(out, "out")
-    if x.shape != out.shape:
+    shape = x.shape
+    if shape != out.shape:
         raise FoError("rope: x and out must have one shape")
-    spec = rope.at(positions, x.shape[0])
-    ctx = ctx or stream_context(x.device.index)
-    check(lib().fo_rope(ctx.handle, ctypes.byref(a), ctypes.byref(b), x.shape[0], x.shape[2], ctypes.byref(spec),
-                        1 if inverse else 0))
+    rows, _, dim = shape
+    ctx = ctx or stream_context(x.get_device())
+    check(lib().fo_rope(ctx.handle, a, b, rows, dim, rope.at(positions, rows), 1 if inverse else 0))
     return out
 
 
@@ -825,6 +838,7 @@ class PagedKv:
         self.device = k_codes.device.index
         self.pool = PagedPool(k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
                               n_pages, page_size, kv_heads, self.head_dim, formats[k_codes.dtype])
+        self.ref, self.scale = ctypes.byref(self.pool), self.head_dim ** -0.5
 
 
 class PagedBatch:
@@ -844,9 +858,13 @@ class PagedBatch:
                                         None if row_start is None else _device_ints(row_start, "row_start"),
                                         page_table.shape[1], n, rows, n * rows)
 
-    def of(self, rows: int) -> PagedSequences:
-        self.sequences.total_rows = rows
-        return self.sequences
+        self.ref = ctypes.byref(self.sequences)
+
+    def of(self, rows: int):
+        """The batch for a call with so many rows in all."""
+        if self.sequences.total_rows != rows:
+            self.sequences.total_rows = rows
+        return self.ref
 
 
 def paged_append(kv: PagedKv, batch: PagedBatch, k, v, rope: Optional[Rope] = None, positions=None, q=None,
@@ -855,35 +873,32 @@ def paged_append(kv: PagedKv, batch: PagedBatch, k, v, rope: Optional[Rope] = No
     pages, keys rotated on the way when `rope` is given (at `positions`, else
     at their place in the cache), and queries q rotated into q_out."""
     rk, rv = _rows(k, "k"), _rows(v, "v")
-    if k.shape[2] != kv.head_dim or v.shape != k.shape:
+    rows, _, dim = shape = k.shape
+    if dim != kv.head_dim or v.shape != shape:
         raise FoError("paged_append: k and v must be [rows][kv heads][head dim] of the cache")
-    rows = k.shape[0]
-    rq = ro = spec = None
-    if rope is not None:
-        spec = ctypes.byref(rope.at(positions, rows))
+    rq = ro = None
     if q is not None:
-        if q_out is None or q.shape != q_out.shape or q.shape[0] != rows or q.shape[2] != kv.head_dim:
+        shape = q.shape
+        if q_out is None or shape != q_out.shape or shape[0] != rows or shape[2] != dim:
             raise FoError("paged_append: q and q_out must be [rows][heads][head dim]")
-        rq, ro = ctypes.byref(_rows(q, "q")), ctypes.byref(_rows(q_out, "q_out"))
+        rq, ro = _rows(q, "q"), _rows(q_out, "q_out")
     ctx = ctx or stream_context(kv.device)
-    check(lib().fo_paged_append(ctx.handle, ctypes.byref(kv.pool), ctypes.byref(batch.of(rows)), ctypes.byref(rk),
-                                ctypes.byref(rv), rq, ro, spec))
+    check(lib().fo_paged_append(ctx.handle, kv.ref, batch.of(rows), rk, rv, rq, ro,
+                                None if rope is None else rope.at(positions, rows)))
 
 
 def paged_attention(kv: PagedKv, batch: PagedBatch, q, out, sinks=None, scale=None, window=0, lse=None, ctx=None):
     """fo_paged_attention: q [rows][heads][head dim] over the batch's cached
     positions into `out`; scale None: 1 / sqrt(head dim)."""
     rq, ro = _rows(q, "q"), _rows(out, "out")
-    if q.shape[2] != kv.head_dim or out.shape != q.shape:
+    rows, heads, dim = shape = q.shape
+    if dim != kv.head_dim or out.shape != shape:
         raise FoError("paged_attention: q and out must be [rows][heads][head dim] of the cache's width")
-    for t, n, name in ((sinks, q.shape[1], "sinks"), (lse, q.shape[0] * q.shape[1], "lse")):
-        if t is not None and (not t.is_cuda or not t.is_contiguous() or t.numel() != n or t.element_size() != 4):
-            raise FoError(f"paged_attention: {name} must be a contiguous float32 CUDA tensor of {n}")
     ctx = ctx or stream_context(kv.device)
-    check(lib().fo_paged_attention(ctx.handle, ctypes.byref(kv.pool), ctypes.byref(batch.of(q.shape[0])),
-                                   ctypes.byref(rq), None if sinks is None else sinks.data_ptr(),
-                                   kv.head_dim ** -0.5 if scale is None else scale, window, ctypes.byref(ro),
-                                   None if lse is None else lse.data_ptr()))
+    check(lib().fo_paged_attention(ctx.handle, kv.ref, batch.of(rows), rq,
+                                   None if sinks is None else _floats(sinks, heads, "sinks"),
+                                   kv.scale if scale is None else scale, window, ro,
+                                   None if lse is None else _floats(lse, rows * heads, "lse")))
     return out
 
 
