@@ -578,3 +578,60 @@ def test_offsets_beyond_32_bits():
     step = max(np.abs(kx).max(), np.abs(vx).max()) / 254
     assert np.abs(out.double().cpu().numpy()[0] - o).max() <= step * (1 + 4 * np.abs(qv).sum(-1).max() * dim ** -0.5)
     assert int(sum((c != 0).any(dim=(1, 2, 3)).sum() for c in codes)) == 6  # three pages each, nothing else
+
+
+def test_example_decodes():
+    """The example's loop runs, and picks the same tokens for the same seed."""
+    import importlib.util
+    import os
+    path = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "examples", "paged_decode.py")
+    spec = importlib.util.spec_from_file_location("paged_decode", path)
+    example = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(example)
+    for fmt in ("e4m3", "i8"):
+        a, _ = example.decode(seqs=3, prompt=300, steps=20, fmt=fmt)
+        b, _ = example.decode(seqs=3, prompt=300, steps=20, fmt=fmt)
+        assert a.shape == (20, 3) and torch.equal(a, b)
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+def test_attention_query_that_is_not_finite(bad):
+    """Its own row's head becomes NaN; the others are as without it."""
+    rng = np.random.default_rng(34)
+    for fmt, dtype in (("i8", "bf16"), ("e4m3", "f32")):
+        cache = Cache(rng, fmt, 64, 16, 2, [40, 300])
+        kv, batch = cache.on_device(), cache.batch([2, 2], False)
+        q, _ = rows_of(rng, 4, 4, 64, dtype)
+        good, out = (torch.empty_like(q) for _ in range(2))
+        F.paged_attention(kv, batch, q, good)
+        q[2, 1, 7] = bad
+        F.paged_attention(kv, batch, q, out)
+        assert out[2, 1].isnan().all()
+        out[2, 1] = good[2, 1]
+        assert torch.equal(out, good)
+
+
+def test_attention_windows_whose_older_pages_are_gone():
+    """Pages that no row of a window sees may be handed back: their table entries are not read."""
+    rng = np.random.default_rng(35)
+    for fmt in ("i8", "e4m3"):
+        cache = Cache(rng, fmt, 64, 16, 1, [700])
+        q, qv = rows_of(rng, 2, 2, 64, "f32")
+        out = torch.empty_like(q)
+        k, v = cache.values(0, 0), cache.values(1, 0)
+        cache.table[0, :(700 - 2 - 100) // 16] = -1
+        ctx = F.Context(0)
+        F.paged_attention(cache.on_device(), cache.batch([2], False), q, out, window=100, ctx=ctx)
+        ctx.synchronize()
+        for r in range(2):
+            o, _, size = R.attend(qv[r], k, v, 698 + r, 100, None, 0.125)
+            top = np.abs(v).max()
+            assert within(out[r].double().cpu().numpy(), o, (4 * 2.0 ** -17 * size + 2.0 ** -18) * top, "f32")
+        ctx.close()
+
+
+def test_attention_more_sequences_than_a_block_has_threads():
+    """The schedule in pieces: 1,100 sequences of up to a few pages, some without a position."""
+    lens = [int(n) for n in np.random.default_rng(1).integers(0, 40, 1100)]
+    attention_case(36, "i8", 64, 16, 1, 2, "bf16", lens, [1] * 1100)
+    attention_case(37, "e4m3", 64, 16, 2, 1, "f32", lens[:33], [1] * 33)

@@ -116,6 +116,11 @@ def test_refusals(call, message):
     assert message in last_error()
 
 
+def test_tables_with_room_for_too_many_tiles():
+    many = batch(n_seqs=60000, total_rows=60000, table_stride=(1 << 31) // 128 - 1)
+    assert attend(b=many) == F.ERR_CAPACITY and "2^31 tiles" in last_error()
+
+
 @pytest.mark.parametrize("change", [
     dict(theta=1.0), dict(theta=float("nan")), dict(scaling=4), dict(scaling=1, factor=0.0),
     dict(scaling=3, original_positions=0.0), dict(scaling=3, beta_slow=0.0), dict(scaling=3, beta_fast=0.5),
