@@ -450,7 +450,7 @@ cudaError_t launch_append(const fo_append_launch &in, cudaStream_t stream) {
     const int team = (int)page * (D / 16), threads = std::max(team, ROPE_THREADS);
     int heads = a.kv.n_kv_heads;
     auto blocks = [&](int64_t h) { return segments * 2 * ((a.kv.n_kv_heads + h - 1) / h); };
-    while (heads > threads / team && blocks(heads) < 592) heads = (heads + 1) / 2;
+    while (heads > threads / team && blocks(heads) < 296) heads = (heads + 1) / 2;
     // The queries' blocks go along with tasks' blocks of their own size (a 6,544-row
     // FP32 page in 64-position pages: 28.5 us apart, 23.3 together); next to wider
     // ones they would run at half their occupancy (24 ragged prompts: 281 us apart,

@@ -30,10 +30,12 @@
 // through transposing shared-memory loads: a consumer computes S^T = K Q^T and
 // O^T += V^T P^T.  Nothing of the cache is rounded; a scale multiplies a
 // finished sum.
-//   int8: m16n8k32 products of bytes with exact 32-bit sums.  A query is a
-//   23-bit integer relative to a power of two near its largest element, three
-//   bytes; a probability one of 16 bits (BF16 rows, whose output has 8), or 23
-//   (FP32 rows), relative to its tile's largest; a product for each byte.
+//   int8: m16n8k32 products of bytes with exact 32-bit sums, one for each byte
+//   of a query and of a probability.  A query is an integer relative to a power
+//   of two near its largest element: of 16 bits for BF16 rows (exactly the
+//   query, where an element is at least 2^-8 of the largest; 2^-16 of that
+//   one otherwise), of 23 for FP32 rows.  A probability is one of 16 bits
+//   (BF16 rows, whose output has 8), or 23, relative to its tile's largest.
 //   e4m3: m16n8k16 products of FP16, which holds every e4m3 number (the 8-bit
 //   instruction is no faster than converting here).  A query is relative to a
 //   power of two near its largest element: BF16's 8 bits exactly, FP32 as the
@@ -78,8 +80,8 @@ struct PaShape {
     static constexpr int HALF = TILE / 2;          // a consumer warp's
     static constexpr int STAGE = 2 * TILE_BYTES;
     static constexpr bool I8 = FORMAT == FO_PAGED_I8;
-    static constexpr int QT = I8 ? 3 : F32 ? 2 : 1;          // a query's terms
-    static constexpr int PT = I8 ? (F32 ? 3 : 2) : QT;       // a probability's
+    static constexpr int QT = (I8 ? 2 : 1) + F32;  // a query's terms, and a probability's
+    static constexpr int PT = QT;
     static constexpr int KQ = I8 ? D / 32 : D / 16;          // k steps over a row's elements
     static constexpr int PART_LD = D + 4;          // a column of a consumer's part, in floats
     static constexpr int PARTS = PA_CONSUMERS * 8 * PART_LD * 4;
@@ -202,10 +204,15 @@ struct PaShared {
     int begin_base, begin_seq, abort;
 };
 
-// Waits for the block's tile k in its slot; false when the block gave up.
+// Waits for the block's tile k in its slot; false when the block gave up.  The
+// first wait may have been for the phase two before; the tile's number says
+// that the one before is over, and the second wait is for the tile's own.
 __device__ __forceinline__ bool pa_wait_tile(PaShared &sh, int slot, int k, unsigned *err) {
+    const uint32_t phase = (k / PA_STAGES) & 1;
     uint64_t t0 = 0;
-    for (uint32_t it = 1; *(volatile int *)&sh.tile[slot] != k; ++it) {
+    for (uint32_t it = 1;; ++it) {
+        if (!sm100::mbar_wait(&sh.full[slot], phase, &sh.abort, err)) return false;
+        if (*(volatile int *)&sh.tile[slot] == k) return sm100::mbar_wait(&sh.full[slot], phase, &sh.abort, err);
         if ((it & 63) != 0) continue;
         if (*(volatile int *)&sh.abort) return false;
         if (t0 == 0) t0 = sm100::globaltimer();
@@ -215,7 +222,6 @@ __device__ __forceinline__ bool pa_wait_tile(PaShared &sh, int slot, int k, unsi
             return false;
         }
     }
-    return sm100::mbar_wait(&sh.full[slot], (k / PA_STAGES) & 1, &sh.abort, err);
 }
 
 // Sum of x over the block's earlier threads; `all` the whole block's.
@@ -398,11 +404,11 @@ __device__ __forceinline__ void pa_epilogue(const fo_paged_attention_launch &a, 
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const unsigned all_finite = __ballot_sync(0xffffffffu, finite);
-            // A power of two near the largest element brings it to [2^21, 2^22)
-            // (int8) or [1, 2) (e4m3); in two factors, so that FP32's whole range
+            // A power of two near the largest element brings it to [2^14, 2^15) or
+            // [2^21, 2^22) (int8) or [1, 2) (e4m3); in two factors, so that FP32's whole range
             // of exponents can be brought there.
             const int e = max((int)(__float_as_uint(top) >> 23), 1);
-            const float up = I8 ? 2097152.0f : 1.0f;
+            const float up = I8 ? (F32 ? 2097152.0f : 16384.0f) : 1.0f;
             const float inv0 = __uint_as_float((uint32_t)(254 - (e + 1) / 2 - 63) << 23);
             const float inv1 = __uint_as_float((uint32_t)(254 - (e - (e + 1) / 2) - 64) << 23) * up;
             if (t == 0) {
@@ -427,12 +433,13 @@ __device__ __forceinline__ void pa_epilogue(const fo_paged_attention_launch &a, 
 #pragma unroll
                         for (int i = 0; i < 4; i++) z[i] = (uint32_t)__float2int_rn(y[i]);
                         const uint32_t lo01 = __byte_perm(z[0], z[1], 0x5140), lo23 = __byte_perm(z[2], z[3], 0x5140);
-                        const uint32_t f[3] = {
-                            __byte_perm(__byte_perm(z[0], z[1], 0x0062), __byte_perm(z[2], z[3], 0x0062), 0x5410),
-                            __byte_perm(lo01, lo23, 0x7632), __byte_perm(lo01, lo23, 0x5410)};
+                        const uint32_t hi01 = __byte_perm(z[0], z[1], 0x0062), hi23 = __byte_perm(z[2], z[3], 0x0062);
+                        // The highest byte, which is signed, first.
+                        const uint32_t f[3] = {__byte_perm(hi01, hi23, 0x5410), __byte_perm(lo01, lo23, 0x7632),
+                                               __byte_perm(lo01, lo23, 0x5410)};
 #pragma unroll
-                        for (int i = 0; i < 3; i++)
-                            reinterpret_cast<uint32_t *>(to + (i * KQ + 2 * c + w / 2) * 32)[w % 2] = f[i];
+                        for (int i = 0; i < QT; i++)
+                            reinterpret_cast<uint32_t *>(to + (i * KQ + 2 * c + w / 2) * 32)[w % 2] = f[3 - QT + i];
                     } else {
                         // Step 4 c + w.
 #pragma unroll
@@ -540,7 +547,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     constexpr int QT = Shape::QT, PT = Shape::PT, KQ = Shape::KQ;
     // The queries' operands stay in registers where there is room, and are read
     // for each tile otherwise.
-    constexpr bool Q_REGS = QT * KQ <= 6;
+    constexpr bool Q_REGS = QT * KQ <= (I8 ? 6 : 8);
     extern __shared__ uint8_t pa_smem[];
     __shared__ PaShared sh;
     uint8_t *tiles = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(pa_smem) + 1023) & ~uintptr_t(1023));
@@ -874,7 +881,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                         *reinterpret_cast<uint4 *>(kw[mt][1] + 4) = *reinterpret_cast<const uint4 *>(row + (k_off1 ^ 64));
                     }
                 }
-                constexpr int A = I8 ? 3 : 1;  // accumulators: int8's terms have their own
+                constexpr int A = I8 ? QT : 1;  // accumulators: int8's terms have their own
                 typename std::conditional<I8, uint32_t, float>::type acc[AHEAD][A][4];
 #pragma unroll
                 for (int mt = 0; mt < AHEAD; mt++)
@@ -912,10 +919,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         if constexpr (I8) {
-                            const float hi = __uint_as_float(acc[mt][0][e]) - PA_MAGIC_F;
-                            const float mid = __uint_as_float(acc[mt][1][e]) - PA_MAGIC_F;
-                            const float lo = __uint_as_float(acc[mt][A - 1][e]) - PA_MAGIC_F;
-                            sc[e] = fmaf(hi, 65536.0f, fmaf(mid, 256.0f, lo));
+                            sc[e] = __uint_as_float(acc[mt][A - 1][e]) - PA_MAGIC_F;
+                            sc[e] = fmaf(__uint_as_float(acc[mt][A > 1 ? A - 2 : 0][e]) - PA_MAGIC_F, 256.0f, sc[e]);
+                            if constexpr (F32) sc[e] = fmaf(__uint_as_float(acc[mt][0][e]) - PA_MAGIC_F, 65536.0f, sc[e]);
                         } else {
                             sc[e] = acc[mt][0][e];
                         }
