@@ -326,6 +326,8 @@ int check_device_errors(fo_ctx *ctx) {
             if (bits & FO_DEVERR_POSITION) return fail(FO_ERR_INVALID, "a rotary position lies outside its table");
             return fail(FO_ERR_NONFINITE, "a value appended to a paged cache is not finite");
         }
+        // A paged attention that unwound may have left its blocks' counters short.
+        if (ctx->paged_parts.ptr) cudaMemset(ctx->paged_parts.ptr, 0, ctx->paged_parts.bytes);
         return fail(FO_ERR_CUDA, "a kernel wait exceeded its time limit and the kernel unwound (bits 0x%x)", bits);
     }
     return FO_OK;
