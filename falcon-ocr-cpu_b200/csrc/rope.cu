@@ -6,7 +6,10 @@
 // table row serves all heads of a token, so the kernel is bound by HBM: a
 // thread takes the same eight elements (or the same eight pairs, in the half
 // layout) of two or four heads of one row, so its table entries are read
-// once and all its loads are in flight together.
+// once and all its loads are in flight together, asked for before the row's
+// position is known.  Measured: 32,771 rows x 40 heads x 128 BF16 119 us (5.8
+// TB/s, 0.90 of the measured copy bandwidth), 6,544 rows x 24 x 64 FP32 16.6 us
+// (4.9 TB/s; a launch that does next to nothing takes 2.4 us), 8 rows 2.4 us.
 #include "paged_rope.cuh"
 
 namespace fo {

@@ -3,6 +3,9 @@ reference's attention operator interface for tests and benchmarks:
 
 * ``attention_with``          kernels::attention_with (src/kernels/attention/mod.rs:256-311)
 * ``attention_prefill_bf16``  kernels::attention_prefill_bf16 (mod.rs:321-349)
+* ``rope``, ``PagedKv``, ``paged_append``, ``paged_attention``  rotary positions
+  and a paged 8-bit cache for many sequences (no counterpart); without ``ctx``
+  these run on torch's current stream
 * ``SplitPrefix``             quant::kv::SplitPrefix (src/quant/kv.rs:155-972):
   ``from_compact``, ``append``, ``truncate_tail``, ``tail_len``, ``bytes``,
   ``attention_decode``, ``attention_decode_rows``; ``decode_batch`` for pages.
