@@ -1764,6 +1764,8 @@ int check_paged(const fo_paged_kv *kv, const fo_paged_batch *b) {
         return fail(FO_ERR_INVALID, "paged batch: at most 65,535 sequences and 2^31 - 1 rows");
     if (!b->row_start && b->total_rows != b->n_seqs * b->max_rows)
         return fail(FO_ERR_INVALID, "paged batch: total_rows must be n_seqs * max_rows");
+    if (b->total_rows > 0 && (b->n_seqs == 0 || b->max_rows == 0))
+        return fail(FO_ERR_INVALID, "paged batch: rows without a sequence that could have them");
     if (b->n_seqs > 0) {
         if (!b->page_table || !b->lens) return fail(FO_ERR_INVALID, "paged batch: null page table or lengths");
         if (b->table_stride < 1 || b->table_stride > INT32_MAX / kv->page_size)

@@ -182,3 +182,15 @@ def test_plain_append_against_the_definition():
     whole, ws = np.zeros_like(codes), np.zeros_like(scales)
     R.append(whole, ws, x, [40], [40], table, "i8")
     assert np.array_equal(ws, scales)
+
+
+@pytest.mark.parametrize("change", [
+    dict(n_seqs=0, row_start=BASE, total_rows=5, max_rows=5), dict(n_seqs=0, row_start=BASE, total_rows=200, max_rows=64),
+    dict(n_seqs=0, row_start=BASE, total_rows=5, max_rows=5, page_table=None, lens=None),
+    dict(n_seqs=2, row_start=BASE, total_rows=5, max_rows=0),
+])
+def test_rows_without_sequences_are_refused(change):
+    """Rows that no sequence could have (the kernels would look for lengths that are not there, or launch no block)."""
+    b = batch(**change)
+    for status in (append(b=b), append(b=b, q=rows(), q_out=rows(), s=spec()), attend(b=b)):
+        assert status == F.ERR_INVALID and "rows without a sequence" in last_error()
