@@ -87,7 +87,8 @@ __device__ __forceinline__ void append_load(const fo_append_launch &a, const T *
 }
 
 // A segment: sequence `seq`'s rows in its j-th touched page.  (Positions and rows
-// are below 2^31, pages a power of two: 64-bit divisions are kept out.)
+// are below 2^31, pages a power of two: 64-bit divisions are kept out.  Segments
+// are numbered with some to spare, whose pages may begin beyond 2^31.)
 struct Segment {
     int seq, page, row0, p0;  // the sequence's page number, its first row here and that one's position
     int rows, begin;          // rows (none: nothing to do) and where in the page they begin
@@ -99,8 +100,9 @@ __device__ __forceinline__ Segment segment_at(const fo_append_launch &a, int seq
     Segment g;
     g.seq = seq;
     g.page = (from >> shift) + j;
-    g.p0 = max(from, g.page << shift);
-    const int p1 = (int)min64(len, (int64_t)(g.page + 1) << shift);
+    const int64_t begins = (int64_t)g.page << shift;
+    g.p0 = max(from, (int)min64(len, begins));
+    const int p1 = (int)min64(len, begins + page);
     g.rows = s.n > 0 && p1 > g.p0 ? p1 - g.p0 : 0;
     g.begin = g.p0 & (page - 1);
     g.row0 = s.first + (g.p0 - (len - s.n));

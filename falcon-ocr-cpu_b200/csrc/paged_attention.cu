@@ -856,7 +856,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             // The first position of this warp's half.
             const int pos0 = (at.w.t0 + at.tile + (k - i)) * TILE + half * HALF;
             if (!pa_wait_tile(sh, slot, k, a.err)) return;
-            if (col_group * 8 >= n_queries || pos0 > p_last || pos0 + HALF <= at.w.low) {
+            // (Differences, since pos0 + HALF may be 2^31.)
+            if (col_group * 8 >= n_queries || pos0 > p_last || at.w.low - pos0 >= HALF) {
                 // No row of this warp's sees any of it.
                 __syncwarp();
                 if (lane == 0) sm100::mbar_arrive(&sh.empty[slot]);
@@ -880,7 +881,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             }
             // S^T: rows = keys, columns = queries; scores times log2 e.
             float c[STEPS][4], mx[2] = {-INFINITY, -INFINITY};
-            const bool masked = pos0 + HALF - 1 > p_first || pos0 < low_last;
+            const bool masked = p_first - pos0 < HALF - 1 || pos0 < low_last;
             constexpr int AHEAD = D == 64 ? 2 : 1;  // as many steps at a time as there are registers for
 #pragma unroll
             for (int m0 = 0; m0 < STEPS; m0 += AHEAD) {
@@ -945,7 +946,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
 #pragma unroll
                         for (int e = 0; e < 4; e++) {
                             const int pos = pos0 + 16 * (m0 + mt) + (e < 2 ? k0 : 8 + k1), p = q_pos[e & 1];
-                            const bool seen = pos <= p && (a.window == 0 || pos > p - a.window);
+                            const bool seen = pos <= p && (a.window == 0 || p - pos < a.window);
                             if (!seen) sc[e] = -INFINITY;
                         }
                     }

@@ -635,3 +635,47 @@ def test_attention_more_sequences_than_a_block_has_threads():
     lens = [int(n) for n in np.random.default_rng(1).integers(0, 40, 1100)]
     attention_case(36, "i8", 64, 16, 1, 2, "bf16", lens, [1] * 1100)
     attention_case(37, "e4m3", 64, 16, 2, 1, "f32", lens[:33], [1] * 33)
+
+
+def test_positions_near_two_to_the_31():
+    """A table with room for nearly 2^31 positions (one sequence whose older pages are gone): rows are appended to its
+    last pages and a window over the last tile is read, without an index that wraps."""
+    page, room = 16, (2 ** 31 - 1) // 16
+    last, rows, kv_heads, dim = room * page, 32, 2, 64
+    table = torch.full((1, room), -1, dtype=torch.int32, device="cuda")
+    table[0, -6:] = torch.arange(6, dtype=torch.int32, device="cuda")
+    for fmt, kind in (("i8", torch.int8), ("e4m3", torch.float8_e4m3fn)):
+        rng = np.random.default_rng(50)
+        # One page more than the table names, which stays as it is.
+        codes = [np.zeros((7, kv_heads, page, dim), np.uint8) for _ in range(2)]
+        scales = [np.zeros((7, kv_heads), np.float32) for _ in range(2)]
+        on_device = [dev(c).view(kind) for c in codes] + [dev(s) for s in scales]
+        kv = F.PagedKv(*on_device)
+        x = [rows_of(rng, 6 * page, kv_heads, dim, "f32") for _ in range(2)]
+        ctx = F.Context(0)
+        for to in (last - 2 * rows, last - rows, last):
+            at = 6 * page - (last - to) - rows
+            part = slice(at, at + rows)
+            F.paged_append(kv, F.PagedBatch(table, dev(np.array([to], np.int32)), rows=rows,
+                                            row_start=dev(np.array([0, rows], np.int32))), x[0][0][part], x[1][0][part],
+                           ctx=ctx)
+            for i in range(2):
+                R.append(codes[i], scales[i], x[i][1][part].astype(np.float32), [rows], [at + rows], np.arange(6)[None],
+                         fmt)
+        ctx.synchronize()
+        for i in range(2):
+            assert np.array_equal(on_device[i].view(torch.uint8).cpu().numpy(), codes[i])
+            assert np.array_equal(on_device[2 + i].cpu().numpy(), scales[i])
+        k, v = ((R.decode(c[:6], fmt) * s[:6, :, None, None].astype(np.float64)).transpose(1, 0, 2, 3).reshape(
+            kv_heads, -1, dim) for c, s in zip(codes, scales))
+        for n in (1, 3):
+            q, qv = rows_of(rng, n, 4, dim, "f32")
+            out = torch.empty_like(q)
+            F.paged_attention(kv, F.PagedBatch(table, dev(np.array([last], np.int32)), rows=n), q, out, window=50,
+                              ctx=ctx)
+            ctx.synchronize()
+            for r in range(n):
+                o, _, size = R.attend(qv[r], k, v, 6 * page - n + r, 50, None, dim ** -0.5)
+                bound = (4 * 2.0 ** -17 * size + 2.0 ** -18) * np.abs(v).max()
+                assert within(out[r].double().cpu().numpy(), o, bound, "f32")
+        ctx.close()
