@@ -56,7 +56,7 @@ __device__ __forceinline__ void append_load(const fo_append_launch &a, const T *
         for (int e = 0; e < 8; e++) y[e] = u[e];
         return;
     }
-    auto entry = [&](int pair) { return inside ? __ldg(entries + pair) : make_float2(NAN, NAN); };
+    auto entry = [&](int pair) { return inside ? load_entry(entries + pair) : make_float2(NAN, NAN); };
     if (a.rope.layout == FO_ROPE_INTERLEAVED) {
 #pragma unroll
         for (int e = 0; e < 8; e += 2) {
@@ -127,7 +127,7 @@ __device__ __forceinline__ Tile tile_of(const fo_append_launch &a, const Segment
 // A row's entries of the rotation table (valid is false outside it).
 __device__ __forceinline__ const float2 *entries_of(const fo_append_launch &a, int64_t row, int64_t position, bool first,
                                                     bool &inside) {
-    const int64_t p = a.rope.row_positions ? (int64_t)__ldg(a.rope.row_positions + row) : position;
+    const int64_t p = a.rope.row_positions ? (int64_t)a.rope.row_positions[row] : position;
     inside = p >= 0 && p < a.rope.positions;
     if (!inside && first) atomicOr(a.err, FO_DEVERR_POSITION);
     return reinterpret_cast<const float2 *>(a.rope.table) + (inside ? p : 0) * (a.rope.rot_dim / 2);
@@ -219,7 +219,7 @@ __device__ __forceinline__ int sequence_of_row(const fo_paged_batch &b, int row)
     int lo = 0, hi = (int)b.n_seqs - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
-        if (__ldg(b.row_start + mid) <= row) lo = mid;
+        if (b.row_start[mid] <= row) lo = mid;
         else hi = mid - 1;
     }
     return lo;
@@ -234,7 +234,7 @@ __host__ __device__ inline int64_t segments_of(int64_t rows, int64_t page) {
 // unless positions are given.
 __device__ __forceinline__ int64_t position_of_row(const fo_append_launch &a, int64_t row, bool &padded) {
     padded = false;
-    if (a.rope.row_positions) return (int64_t)__ldg(a.rope.row_positions + row);
+    if (a.rope.row_positions) return (int64_t)a.rope.row_positions[row];
     const int seq = a.batch.row_start ? sequence_of_row(a.batch, (int)row) : (int)((unsigned)row / (unsigned)a.batch.max_rows);
     const Sequence s = load_sequence(a.batch, a.kv.page_size, seq, a.err);
     const int p = s.len - s.n + ((int)row - s.first);
@@ -306,11 +306,11 @@ __global__ void __launch_bounds__(D == 64 ? 512 : 1024, D == 64 ? 2 : 1) append_
         int lo = 0, hi = (int)a.batch.n_seqs - 1;
         while (lo < hi) {
             const int mid = (lo + hi + 1) >> 1;
-            if ((__ldg(a.batch.row_start + mid) >> shift) + 2 * mid <= (int)segment) lo = mid;
+            if ((a.batch.row_start[mid] >> shift) + 2 * mid <= (int)segment) lo = mid;
             else hi = mid - 1;
         }
         seq = lo;
-        j = (int)segment - ((__ldg(a.batch.row_start + seq) >> shift) + 2 * seq);
+        j = (int)segment - ((a.batch.row_start[seq] >> shift) + 2 * seq);
         if (j < 0) return;  // row_start out of order (the sequence's own check reports it)
     }
     const Segment s = segment_at(a, seq, j);
@@ -355,7 +355,7 @@ __global__ void __launch_bounds__(D == 64 ? 512 : 1024, D == 64 ? 2 : 1) append_
         for (int e = 0; e < 8; e++) {
             const bool turn = pair || d0 + 2 * e < rot;
             cs[e] = !turn ? make_float2(1.0f, 0.0f)
-                          : inside ? __ldg(entries + (pair ? d0 + e : d0 / 2 + e)) : make_float2(NAN, NAN);
+                          : inside ? load_entry(entries + (pair ? d0 + e : d0 / 2 + e)) : make_float2(NAN, NAN);
         }
     }
     bool valid;
@@ -396,7 +396,7 @@ __global__ void __launch_bounds__(D == 64 ? 512 : 1024, D == 64 ? 2 : 1) append_
                 for (int e = 0; e < 16; e++) {
                     const int i = d0 + e, p = i < h2 ? i : i - h2;
                     if (!rotate || i >= rot) continue;
-                    const float2 c = inside ? __ldg(entries + p) : make_float2(NAN, NAN);
+                    const float2 c = inside ? load_entry(entries + p) : make_float2(NAN, NAN);
                     y[e] = i < h2 ? rot_first(y[e], load1(x + i + h2), c) : rot_second(load1(x + i - h2), y[e], c);
                 }
             }

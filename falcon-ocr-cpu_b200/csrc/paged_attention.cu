@@ -298,7 +298,7 @@ __device__ __forceinline__ void pa_write(const fo_paged_attention_launch &a, con
     using T = typename std::conditional<F32, float, uint16_t>::type;
     const int q = u.q0 + qi, r = q / a.group, h = u.head * a.group + q - r * a.group;
     float sum = ll;
-    if (a.sinks) sum += sm100::ex2(fmaf(__ldg(a.sinks + h), PA_LOG2E, -mm));
+    if (a.sinks) sum += sm100::ex2(fmaf(a.sinks[h], PA_LOG2E, -mm));
     const float inv = ll == 0.0f ? 0.0f : 1.0f / sum;
     v = make_float4(v.x * inv, v.y * inv, v.z * inv, v.w * inv);
     T *out = static_cast<T *>(a.out.data) + (int64_t)(u.first + r) * a.out.row_stride + h * a.out.head_stride + 4 * quad;
@@ -720,7 +720,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             const int64_t pos = (int64_t)(at.w.t0 + at.tile + skip + PA_PRODUCERS * off) * TILE + (j << log_page);
             const int64_t begins = pos >> log_page << log_page;
             if (off < b.n && pos < at.w.s.len && begins + page > at.w.low) {
-                b.id = __ldg(a.batch.page_table + at.seq * a.batch.table_stride + (pos >> log_page));
+                b.id = a.batch.page_table[at.seq * a.batch.table_stride + (pos >> log_page)];
                 b.row = (int)(pos - begins);
             }
             ahead += span;
@@ -732,8 +732,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             b.bad = b.id < 0 || b.id >= a.kv.n_pages;
             if (b.bad) return;
             const int64_t tile = (int64_t)b.id * a.kv.n_kv_heads + b.head;
-            b.ks = __ldg(a.kv.k_scales + tile);
-            b.vs = __ldg(a.kv.v_scales + tile);
+            b.ks = a.kv.k_scales[tile];
+            b.vs = a.kv.v_scales[tile];
         };
         if (lane == 0) {
             sm100::tma_prefetch(&k_map);

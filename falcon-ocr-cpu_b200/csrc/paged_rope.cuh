@@ -67,7 +67,7 @@ __device__ __forceinline__ void rope_block(const fo_rope_launch &a, int64_t bloc
         entries = reinterpret_cast<const float2 *>(a.rope.table) + (inside ? p : 0) * h2;
     };
     auto entry = [&](int pair) {
-        float2 cs = __ldg(entries + pair);
+        float2 cs = load_entry(entries + pair);
         if (!inside) cs = padded ? make_float2(1.0f, 0.0f) : make_float2(NAN, NAN);
         if (a.transpose) cs.y = -cs.y;
         return cs;

@@ -47,7 +47,7 @@ __global__ void __launch_bounds__(ROPE_THREADS, 3) rope_kernel(const __grid_cons
     wait_for_prior_kernel();
     rope_block<T, HALF, VEC>(a, blockIdx.x, threadIdx.x, [&](int64_t row, bool &padded) {
         padded = false;
-        return a.rope.row_positions ? (int64_t)__ldg(a.rope.row_positions + row) : row;
+        return a.rope.row_positions ? (int64_t)a.rope.row_positions[row] : row;
     });
 }
 

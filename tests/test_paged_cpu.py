@@ -194,3 +194,22 @@ def test_rows_without_sequences_are_refused(change):
     b = batch(**change)
     for status in (append(b=b), append(b=b, q=rows(), q_out=rows(), s=spec()), attend(b=b)):
         assert status == F.ERR_INVALID and "rows without a sequence" in last_error()
+
+
+def test_overlapped_kernels_make_no_read_only_loads():
+    """A kernel that starts while the one before it ends may not load through the read-only path: it asks for memory
+    that nothing writes while the kernel lives, and its life begins before the other's stores."""
+    import os
+    csrc = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "falcon-ocr-cpu_b200", "csrc")
+    files = {name: open(os.path.join(csrc, name)).read() for name in sorted(os.listdir(csrc))
+             if name.endswith((".cu", ".cuh"))}
+    overlapped = {name for name, text in files.items() if "wait_for_prior_kernel" in text}
+    grown = True
+    while grown:  # and what they include
+        more = {name for name in files for user in overlapped if '#include "%s"' % name in files[user]}
+        grown = not more <= overlapped
+        overlapped |= more
+    assert {"paged.cuh", "paged_rope.cuh", "rope.cu", "paged_append.cu", "paged_attention.cu"} <= overlapped
+    for name in overlapped:
+        for word in ("__ldg(", "ld.global.nc", "__restrict__"):
+            assert word not in files[name], (name, word)
