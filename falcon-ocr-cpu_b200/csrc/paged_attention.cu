@@ -693,17 +693,17 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         const int j = lane & (pages - 1), off = lane >> log_pages;
         struct Batch {
             int first, n;   // the block's tiles first, first + PA_PRODUCERS, ..: n of them
-            int head, row;  // KV head, and this lane's page: its first row, its number (-1: none)
+            int head, row;  // KV head, and this lane's page: its first row, its number
             int id;
-            bool bad;
+            bool wanted, bad;  // rows see it; they do and its number is outside the pool
             float ks, vs;
         };
         int ahead = 0;  // tiles handed to batches
         bool more = true;
         auto fetch_id = [&]() {
             Batch b;
-            b.id = -1;
-            b.bad = false;
+            b.id = 0;
+            b.wanted = b.bad = false;
             b.row = 0;
             b.ks = b.vs = 0.0f;
             b.first = b.n = b.head = 0;
@@ -722,13 +722,14 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             if (off < b.n && pos < at.w.s.len && begins + page > at.w.low) {
                 b.id = a.batch.page_table[at.seq * a.batch.table_stride + (pos >> log_page)];
                 b.row = (int)(pos - begins);
+                b.wanted = true;
             }
             ahead += span;
             at.advance(a, span);
             return b;
         };
         auto fetch_scales = [&](Batch &b) {
-            if (b.id == -1) return;
+            if (!b.wanted) return;
             b.bad = b.id < 0 || b.id >= a.kv.n_pages;
             if (b.bad) return;
             const int64_t tile = (int64_t)b.id * a.kv.n_kv_heads + b.head;
@@ -760,7 +761,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                 }
                 if (lane == 0) *(volatile int *)&sh.tile[slot] = tile;
                 const bool here = off == i;
-                const bool load = here && now.id != -1 && !now.bad;
+                const bool load = here && now.wanted && !now.bad;
                 const uint32_t n_loads = __popc(__ballot_sync(0xffffffffu, load));
                 if (lane == 0) {
                     asm volatile("mbarrier.expect_tx.relaxed.cta.shared::cta.b64 [%0], %1;" ::"r"(

@@ -679,3 +679,30 @@ def test_positions_near_two_to_the_31():
                 bound = (4 * 2.0 ** -17 * size + 2.0 ** -18) * np.abs(v).max()
                 assert within(out[r].double().cpu().numpy(), o, bound, "f32")
         ctx.close()
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("number", [-1, -7, -(1 << 31), "pages", 1 << 30])
+def test_attention_reports_every_page_number_outside_the_pool(fmt, number):
+    """-1, the usual mark of a place that has no page, among them: where rows see it the error word says so and they
+    are NaN; the other sequences are whole."""
+    rng = np.random.default_rng(40)
+    for dim, lens, bad in ((64, [40, 200, 9], 3), (128, [500, 333], 0)):
+        cache = Cache(rng, fmt, dim, 16, 2, lens)
+        q, qv = rows_of(rng, len(lens), 4, dim, "bf16")
+        out, lse = torch.full_like(q, 9.0), torch.full((len(lens), 4), 9.0, device="cuda")
+        cache.table[1, bad] = cache.codes[0].shape[0] if number == "pages" else number
+        ctx = F.Context(0)
+        F.paged_attention(cache.on_device(), cache.batch([1] * len(lens), False), q, out, lse=lse, ctx=ctx)
+        with pytest.raises(F.FoError, match="page table"):
+            ctx.synchronize()
+        ctx.synchronize()  # reported once
+        assert out[1].isnan().all() and lse[1].isnan().all()
+        for b in range(len(lens)):
+            if b == 1:
+                continue
+            o, _, size = R.attend(qv[b], cache.values(0, b), cache.values(1, b), lens[b] - 1, 0, None, dim ** -0.5)
+            top = np.abs(cache.values(1, b)).max()
+            bound = (4 * 2.0 ** -17 * size + 2.0 ** -18 + 2.0 ** -11) * top
+            assert within(out[b].double().cpu().numpy(), o, bound, "bf16")
+        ctx.close()
