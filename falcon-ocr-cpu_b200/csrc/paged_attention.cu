@@ -329,7 +329,7 @@ __device__ __forceinline__ void pa_join_blocks(const fo_paged_attention_launch &
         bool lost = false;
         for (int j = lane; j < n; j += 32) {
             const float2 ml = __ldcg(mls + u.part(a, u.c0 + j, qi));
-            lost |= ml.x != ml.x || ml.y != ml.y;
+            lost |= ml.y != ml.y;
             mm = fmaxf(mm, ml.x);
         }
         mm = warp_max(mm);
@@ -495,7 +495,7 @@ __device__ __forceinline__ void pa_epilogue(const fo_paged_attention_launch &a, 
 #pragma unroll 4
             for (int w = cg; w < PA_CONSUMERS; w += a.col_groups) {
                 const float2 ml = *reinterpret_cast<const float2 *>(sh.ml[w][col]);
-                lost |= ml.x != ml.x || ml.y != ml.y;
+                lost |= ml.y != ml.y;
                 mm = fmaxf(mm, ml.x);
             }
 #pragma unroll 4
@@ -1110,9 +1110,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             __syncwarp();
             if (lane == 0) sm100::mbar_arrive(&sh.q_free);
         }
-        // This warp's part, for the epilogue warps to join.  A part that is not a
-        // number (a query that is not finite, a page number outside the pool)
-        // makes its queries' outputs NaN.
+        // This warp's part, for the epilogue warps to join.  A sum that is not a
+        // number (a query that is not finite and saw a position, a page number
+        // outside the pool) makes its query's output NaN.
         if (segment > 0 && !sm100::mbar_wait(&sh.part_free, (segment - 1) & 1, &sh.abort, a.err)) return;
 #pragma unroll
         for (int h = 0; h < 2; h++) {
@@ -1121,8 +1121,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             x += __shfl_xor_sync(0xffffffffu, x, 8);
             x += __shfl_xor_sync(0xffffffffu, x, 16);
             if (g == 0) {
-                const bool good = x == x && q_scale[h] == q_scale[h];
-                sh.ml[warp][2 * t + h][0] = good ? m[h] : NAN;
+                sh.ml[warp][2 * t + h][0] = m[h];
                 sh.ml[warp][2 * t + h][1] = x;
             }
             if (any) {

@@ -706,3 +706,47 @@ def test_attention_reports_every_page_number_outside_the_pool(fmt, number):
             bound = (4 * 2.0 ** -17 * size + 2.0 ** -18 + 2.0 ** -11) * top
             assert within(out[b].double().cpu().numpy(), o, bound, "bf16")
         ctx.close()
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_attention_rows_that_see_nothing_whatever_they_hold(bad, fmt, dtype):
+    """A padded slot's queries are whatever its buffer was left with: 0 and -infinity all the same, and nothing of
+    them reaches the other rows."""
+    rng = np.random.default_rng(41)
+    for dim, group, rows, lens, window in ((64, 2, 1, [0, 300, 0], 0), (128, 1, 5, [3, 0, 700], 0),
+                                           (64, 5, 5, [2, 0, 90], 16), (128, 8, 7, [2500, 6], 0)):
+        cache = Cache(rng, fmt, dim, 16, 2, lens)
+        kv, batch = cache.on_device(), cache.batch([rows] * len(lens), False)
+        q, _ = rows_of(rng, rows * len(lens), 2 * group, dim, dtype)
+        sinks = dev(rng.standard_normal(2 * group).astype(np.float32))
+        empty = [b * rows + r for b, n in enumerate(lens) for r in range(rows) if n - rows + r < 0]
+        good, out = (torch.full_like(q, 9.0) for _ in range(2))
+        lses = [torch.full((q.shape[0], 2 * group), 9.0, device="cuda") for _ in range(2)]
+        F.paged_attention(kv, batch, q, good, sinks=sinks, window=window, lse=lses[0])
+        q[empty] = bad
+        F.paged_attention(kv, batch, q, out, sinks=sinks, window=window, lse=lses[1])
+        assert torch.equal(out, good) and torch.equal(lses[1], lses[0])
+        assert (out[empty] == 0).all() and (lses[1][empty] == -math.inf).all()
+
+
+def test_padded_slots_from_append_to_attention():
+    """A captured graph's padded slot (length 0) with NaN left in its rows, through a whole step."""
+    rng = np.random.default_rng(42)
+    for fmt in ("i8", "e4m3"):
+        cache = Cache(rng, fmt, 64, 16, 2, [0, 20], extra_positions=1)
+        kv = cache.on_device()
+        cache.lens = [0, 21]
+        batch = cache.batch([1, 1], False)
+        k, v = (rows_of(rng, 2, 2, 64, "bf16")[0] for _ in range(2))
+        q, _ = rows_of(rng, 2, 4, 64, "bf16")
+        for t in (k, v, q):
+            t[0] = math.nan
+        q_out, out = (torch.full_like(q, 9.0) for _ in range(2))
+        ctx = F.Context(0)
+        F.paged_append(kv, batch, k, v, rope=F.Rope(dev(plain_table(40, 64))), q=q, q_out=q_out, ctx=ctx)
+        F.paged_attention(kv, batch, q_out, out, ctx=ctx)
+        ctx.synchronize()
+        assert (out[0] == 0).all() and out[1].isfinite().all() and (out[1] != 0).any()
+        ctx.close()
