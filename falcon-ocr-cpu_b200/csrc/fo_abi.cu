@@ -162,6 +162,9 @@ struct fo_ctx {
     // size for all calls, made by the first.
     DevBuf paged_parts;
     int sms = 0;
+    size_t paged_part_rows() const { return (size_t)2 * sms * FO_PAGED_QUERIES; }
+    float *paged_part_ml() const { return (float *)paged_parts.ptr + paged_part_rows() * 128; }
+    unsigned *paged_counters() const { return (unsigned *)(paged_part_ml() + paged_part_rows() * 2); }
 };
 
 struct fo_kv_cache {
@@ -314,12 +317,16 @@ int stage_compact(fo_ctx *ctx, const float *q, const fo_compact_kv *kv, int64_t 
     return FO_OK;
 }
 
-// Reads and clears the context's device error word (after a synchronize).
+// Reads and clears the context's device error word (after a synchronize).  All
+// of it goes through the context's own stream, so that it neither waits for
+// other streams nor is overtaken by the context's next calls.
 int check_device_errors(fo_ctx *ctx) {
     unsigned bits = 0;
-    FO_CUDA(cudaMemcpy(&bits, ctx->dev_err, sizeof bits, cudaMemcpyDeviceToHost), "cudaMemcpy(error word)");
+    FO_CUDA(cudaMemcpyAsync(&bits, ctx->dev_err, sizeof bits, cudaMemcpyDeviceToHost, ctx->stream),
+            "cudaMemcpyAsync(error word)");
+    FO_CUDA(cudaStreamSynchronize(ctx->stream), "cudaStreamSynchronize");
     if (bits) {
-        cudaMemset(ctx->dev_err, 0, sizeof bits);
+        FO_CUDA(cudaMemsetAsync(ctx->dev_err, 0, sizeof bits, ctx->stream), "cudaMemsetAsync(error word)");
         if (!(bits & ~(FO_DEVERR_PAGED | FO_DEVERR_POSITION | FO_DEVERR_VALUE))) {
             if (bits & FO_DEVERR_PAGED)
                 return fail(FO_ERR_INVALID, "a paged call's page table, lengths or row ranges do not fit its buffers");
@@ -327,7 +334,9 @@ int check_device_errors(fo_ctx *ctx) {
             return fail(FO_ERR_NONFINITE, "a value appended to a paged cache is not finite");
         }
         // A paged attention that unwound may have left its blocks' counters short.
-        if (ctx->paged_parts.ptr) cudaMemset(ctx->paged_parts.ptr, 0, ctx->paged_parts.bytes);
+        if (ctx->sms)
+            FO_CUDA(cudaMemsetAsync(ctx->paged_counters(), 0, (size_t)ctx->sms * 4, ctx->stream),
+                    "cudaMemsetAsync(paged attention counters)");
         return fail(FO_ERR_CUDA, "a kernel wait exceeded its time limit and the kernel unwound (bits 0x%x)", bits);
     }
     return FO_OK;
@@ -473,7 +482,7 @@ int fo_ctx_create(int device, void *stream, fo_ctx **out) {
     ctx->stream = (cudaStream_t)stream;
     cudaError_t e = cudaMalloc(&ctx->flags, sizeof(unsigned));
     if (e == cudaSuccess) e = cudaMalloc(&ctx->dev_err, sizeof(unsigned));
-    if (e == cudaSuccess) e = cudaMemset(ctx->dev_err, 0, sizeof(unsigned));
+    if (e == cudaSuccess) e = cudaMemsetAsync(ctx->dev_err, 0, sizeof(unsigned), ctx->stream);
     if (e == cudaSuccess) e = cudaEventCreate(&ctx->ev0);
     if (e == cudaSuccess) e = cudaEventCreate(&ctx->ev1);
     if (e == cudaSuccess) e = ctx->pages.ensure(sizeof(fo_decode_page) * FO_BATCH_PAGES);
@@ -1233,9 +1242,10 @@ int fo_kv_plan_finish(fo_kv_plan *p) {
     std::vector<fo_append_page> ha((size_t)n);
     cudaError_t e = cudaMemcpyAsync(ha.data(), p->ap, sizeof(fo_append_page) * n, cudaMemcpyDeviceToHost,
                                     p->ctx->stream);
-    if (e == cudaSuccess) e = cudaStreamSynchronize(p->ctx->stream);
     unsigned bits = 0;
-    if (e == cudaSuccess) e = cudaMemcpy(&bits, p->ctx->dev_err, sizeof bits, cudaMemcpyDeviceToHost);
+    if (e == cudaSuccess) e = cudaMemcpyAsync(&bits, ctx->dev_err, sizeof bits, cudaMemcpyDeviceToHost, ctx->stream);
+    if (e == cudaSuccess) e = cudaStreamSynchronize(ctx->stream);
+    if (e == cudaSuccess && bits) e = cudaMemsetAsync(ctx->dev_err, 0, sizeof bits, ctx->stream);
     if (e != cudaSuccess) {
         plan_free(p);
         return cuda_fail(e, "fo_kv_plan_finish");
@@ -1246,7 +1256,6 @@ int fo_kv_plan_finish(fo_kv_plan *p) {
         p->caches[i]->tail_len = std::min<int64_t>(ha[i].first, p->caches[i]->tail_capacity);
     plan_free(p);
     if (bits) {
-        cudaMemset(ctx->dev_err, 0, sizeof bits);
         if (bits & FO_DEVERR_CAPACITY)
             return fail(FO_ERR_CAPACITY, "a batch plan step found a cache's tail full (later steps repeated its last position)");
         return fail(FO_ERR_CUDA, "a kernel wait exceeded its time limit and the kernel unwound (bits 0x%x)", bits);
@@ -1923,10 +1932,9 @@ int fo_paged_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch 
         FO_CUDA(cudaMemsetAsync(ctx->paged_parts.ptr, 0, ctx->paged_parts.bytes, ctx->stream), "cudaMemset(parts)");
         ctx->sms = sms;
     }
-    const size_t parts = (size_t)2 * ctx->sms * FO_PAGED_QUERIES;
     a.part_o = (float *)ctx->paged_parts.ptr;
-    a.part_ml = a.part_o + parts * 128;
-    a.counters = (unsigned *)(a.part_ml + parts * 2);
+    a.part_ml = ctx->paged_part_ml();
+    a.counters = ctx->paged_counters();
     cudaError_t e = fo_launch_paged_attention(&a, ctx->sms, ctx->stream);
     return e == cudaSuccess ? FO_OK : cuda_fail(e, "paged attention launch");
 }

@@ -750,3 +750,29 @@ def test_padded_slots_from_append_to_attention():
         ctx.synchronize()
         assert (out[0] == 0).all() and out[1].isfinite().all() and (out[1] != 0).any()
         ctx.close()
+
+
+def test_reports_touch_their_own_stream_alone():
+    """A report reads and clears the error word, and after a bounded wait the attention's counters, in the order of the
+    context's stream: work on the default stream neither delays it nor can be overtaken by it."""
+    side = torch.cuda.Stream()
+    rng = np.random.default_rng(43)
+    cache = Cache(rng, "i8", 64, 16, 1, [9000])
+    q, _ = rows_of(rng, 1, 1, 64, "f32")
+    outs = [torch.empty_like(q) for _ in range(2)]
+    kv, batch = cache.on_device(), cache.batch([1], False)
+    ctx = F.Context(0, side.cuda_stream)
+    torch.cuda.synchronize()
+    F.paged_attention(kv, batch, q, outs[0], ctx=ctx)
+    assert ctx.selftest_bounded_wait(1000) == F.ERR_CUDA
+    torch.cuda.synchronize()
+    torch.cuda._sleep(int(1e9))  # half a second on the default stream
+    busy = torch.cuda.Event()
+    busy.record()
+    assert ctx.selftest_bounded_wait(1000) == F.ERR_CUDA
+    F.paged_attention(kv, batch, q, outs[1], ctx=ctx)
+    ctx.synchronize()
+    assert not busy.query()
+    assert torch.equal(*outs)
+    torch.cuda.synchronize()
+    ctx.close()
