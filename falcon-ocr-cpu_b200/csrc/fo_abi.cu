@@ -317,6 +317,22 @@ int stage_compact(fo_ctx *ctx, const float *q, const fo_compact_kv *kv, int64_t 
     return FO_OK;
 }
 
+// The status that the (already cleared) bits of a context's error word stand for.
+int report_device_errors(fo_ctx *ctx, unsigned bits) {
+    if (!bits) return FO_OK;
+    if (!(bits & ~(FO_DEVERR_PAGED | FO_DEVERR_POSITION | FO_DEVERR_VALUE))) {
+        if (bits & FO_DEVERR_PAGED)
+            return fail(FO_ERR_INVALID, "a paged call's page table, lengths or row ranges do not fit its buffers");
+        if (bits & FO_DEVERR_POSITION) return fail(FO_ERR_INVALID, "a rotary position lies outside its table");
+        return fail(FO_ERR_NONFINITE, "a value appended to a paged cache is not finite");
+    }
+    // A paged attention that unwound may have left its blocks' counters short.
+    if (ctx->sms)
+        FO_CUDA(cudaMemsetAsync(ctx->paged_counters(), 0, (size_t)ctx->sms * 4, ctx->stream),
+                "cudaMemsetAsync(paged attention counters)");
+    return fail(FO_ERR_CUDA, "a kernel wait exceeded its time limit and the kernel unwound (bits 0x%x)", bits);
+}
+
 // Reads and clears the context's device error word (after a synchronize).  All
 // of it goes through the context's own stream, so that it neither waits for
 // other streams nor is overtaken by the context's next calls.
@@ -325,21 +341,8 @@ int check_device_errors(fo_ctx *ctx) {
     FO_CUDA(cudaMemcpyAsync(&bits, ctx->dev_err, sizeof bits, cudaMemcpyDeviceToHost, ctx->stream),
             "cudaMemcpyAsync(error word)");
     FO_CUDA(cudaStreamSynchronize(ctx->stream), "cudaStreamSynchronize");
-    if (bits) {
-        FO_CUDA(cudaMemsetAsync(ctx->dev_err, 0, sizeof bits, ctx->stream), "cudaMemsetAsync(error word)");
-        if (!(bits & ~(FO_DEVERR_PAGED | FO_DEVERR_POSITION | FO_DEVERR_VALUE))) {
-            if (bits & FO_DEVERR_PAGED)
-                return fail(FO_ERR_INVALID, "a paged call's page table, lengths or row ranges do not fit its buffers");
-            if (bits & FO_DEVERR_POSITION) return fail(FO_ERR_INVALID, "a rotary position lies outside its table");
-            return fail(FO_ERR_NONFINITE, "a value appended to a paged cache is not finite");
-        }
-        // A paged attention that unwound may have left its blocks' counters short.
-        if (ctx->sms)
-            FO_CUDA(cudaMemsetAsync(ctx->paged_counters(), 0, (size_t)ctx->sms * 4, ctx->stream),
-                    "cudaMemsetAsync(paged attention counters)");
-        return fail(FO_ERR_CUDA, "a kernel wait exceeded its time limit and the kernel unwound (bits 0x%x)", bits);
-    }
-    return FO_OK;
+    if (bits) FO_CUDA(cudaMemsetAsync(ctx->dev_err, 0, sizeof bits, ctx->stream), "cudaMemsetAsync(error word)");
+    return report_device_errors(ctx, bits);
 }
 
 int finish_host(fo_ctx *ctx, float *host_out, const float *dev_out, int64_t n, int mem) {
@@ -1255,12 +1258,10 @@ int fo_kv_plan_finish(fo_kv_plan *p) {
     for (int64_t i = 0; i < n; i++)
         p->caches[i]->tail_len = std::min<int64_t>(ha[i].first, p->caches[i]->tail_capacity);
     plan_free(p);
-    if (bits) {
-        if (bits & FO_DEVERR_CAPACITY)
-            return fail(FO_ERR_CAPACITY, "a batch plan step found a cache's tail full (later steps repeated its last position)");
-        return fail(FO_ERR_CUDA, "a kernel wait exceeded its time limit and the kernel unwound (bits 0x%x)", bits);
-    }
-    return FO_OK;
+    const int status = report_device_errors(ctx, bits);
+    if (bits & FO_DEVERR_CAPACITY)
+        return fail(FO_ERR_CAPACITY, "a batch plan step found a cache's tail full (later steps repeated its last position)");
+    return status;
 }
 
 static bool aligned8(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 7) == 0; }

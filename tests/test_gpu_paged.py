@@ -776,3 +776,22 @@ def test_reports_touch_their_own_stream_alone():
     assert torch.equal(*outs)
     torch.cuda.synchronize()
     ctx.close()
+
+
+def test_a_batch_plan_tells_other_calls_errors_apart():
+    """A paged call's error that is still unread when a plan on the same context finishes is reported as what it is."""
+    import generators as G
+    ctx = F.Context(0)
+    k, v, _ = G.kv_fixture(300, 21)
+    cache = F.SplitPrefix.from_compact(dev(k), dev(v), 300, 308, fmt=F.KV_Q8, ctx=ctx)
+    rows = [[torch.zeros(1024, device="cuda")] for _ in range(4)]
+    plan = F.BatchPlan([cache], *rows[:3], [torch.zeros(16, device="cuda")], rows[3])
+    plan.step()
+    x = torch.ones(1, 2, 64, device="cuda")
+    F.rope(x, torch.empty_like(x), F.Rope(dev(plain_table(4, 64))), dev(np.array([4], np.int32)), ctx=ctx)
+    with pytest.raises(F.FoError, match="outside its table"):
+        plan.finish()
+    ctx.synchronize()  # reported once
+    assert cache.tail_len == 1
+    cache.close()
+    ctx.close()
