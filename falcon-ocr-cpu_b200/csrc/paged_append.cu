@@ -231,15 +231,16 @@ __host__ __device__ inline int64_t segments_of(int64_t rows, int64_t page) {
 }
 
 // The rotation of the queries: a row's position is its place in the cache
-// unless positions are given.
+// unless positions are given; a row without such a place (a padded slot's, or of
+// no sequence) is copied.
 __device__ __forceinline__ int64_t position_of_row(const fo_append_launch &a, int64_t row, bool &padded) {
     padded = false;
     if (a.rope.row_positions) return (int64_t)a.rope.row_positions[row];
     const int seq = a.batch.row_start ? sequence_of_row(a.batch, (int)row) : (int)((unsigned)row / (unsigned)a.batch.max_rows);
     const Sequence s = load_sequence(a.batch, a.kv.page_size, seq, a.err);
-    const int p = s.len - s.n + ((int)row - s.first);
-    padded = p < 0;
-    return p;
+    const int r = (int)row - s.first, p = s.len - s.n + r;
+    padded = r < 0 || r >= s.n || p < 0;
+    return padded ? -1 : p;
 }
 template <typename T>
 __device__ __forceinline__ void rotate_queries(const fo_append_launch &a, int64_t block, bool half, bool vec) {

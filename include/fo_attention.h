@@ -537,6 +537,8 @@ typedef struct {
  * lens[b] - 1.  row_start NULL: every sequence has max_rows rows, sequence
  * b's from row b * max_rows; otherwise sequence b's rows are row_start[b] ..
  * row_start[b + 1] - 1, at most max_rows of them and none beyond total_rows.
+ * Rows before row_start[0] and from row_start[n_seqs] on are no sequence's:
+ * nothing of them is stored, and the attention leaves their out and lse alone.
  * A row whose position is negative (a padded slot of a captured graph has
  * lens 0) stores nothing and attends to nothing.  Position p of sequence b
  * is in page page_table[b * table_stride + p / page_size], p % page_size. */
@@ -550,11 +552,14 @@ typedef struct {
 /* Appends the rows of k and v [total_rows][n_kv_heads][head_dim] to the
  * sequences' pages, and rotates rows: k on its way into the cache and q into
  * q_out (q and q_out NULL: no queries; rope NULL: nothing is rotated, and q
- * must be NULL).  The rows that fall into one page share the page's scale: a
- * page whose first position is among them takes max |x| / 127 (int8) or
- * / 448 (e4m3) of its new rows; a page that holds earlier positions keeps
- * its scale unless the new rows need a larger one, and then its earlier codes
- * are rounded again against that.  code = x / scale, rounded to nearest even.
+ * must be NULL).  Without row_positions a query row that has no place in the
+ * cache (of a negative position, or no sequence's) is copied as it is.
+ *
+ * The rows that fall into one page share the page's scale: a page whose first
+ * position is among them takes max |x| / 127 (int8) or / 448 (e4m3) of its
+ * new rows; a page that holds earlier positions keeps its scale unless the
+ * new rows need a larger one, and then its earlier codes are rounded again
+ * against that.  code = x / scale, rounded to nearest even.
  * Pages that sequences share must not be appended to.  A value that is not
  * finite takes no part in the scale; infinities are stored as the largest
  * code, NaN as zero, and the error word says so. */

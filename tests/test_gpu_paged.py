@@ -795,3 +795,47 @@ def test_a_batch_plan_tells_other_calls_errors_apart():
     assert cache.tail_len == 1
     cache.close()
     ctx.close()
+
+
+@pytest.mark.parametrize("per", [2, 30])
+def test_rows_of_no_sequence(per):
+    """Rows before the first sequence's and behind the last one's: their queries are copied as they are, nothing of
+    them is stored or reported, and the attention leaves their outputs alone."""
+    rng = np.random.default_rng(44)
+    start = [3, 3 + per, 3 + per, 3 + 2 * per]
+    total, held, rows = start[-1] + 40, [10, 5, 0], [per, 0, per]
+    cache = Cache(rng, "i8", 64, 16, 2, held, extra_positions=per)
+    kv = cache.on_device()
+    cache.lens = [n + m for n, m in zip(held, rows)]
+    batch = F.PagedBatch(dev(cache.table), dev(np.array(cache.lens, np.int32)), rows=per,
+                         row_start=dev(np.array(start, np.int32)))
+    table = plain_table(10 + per, 64)  # no position beyond the longest sequence's
+    k, kx = rows_of(rng, total, 2, 64, "f32")
+    v, vx = rows_of(rng, total, 2, 64, "f32")
+    q, qx = rows_of(rng, total, 4, 64, "f32")
+    q_out, out = (torch.full_like(q, 5.0) for _ in range(2))
+    lse = torch.full((total, 4), 5.0, device="cuda")
+    own = np.array(list(range(start[0], start[1])) + list(range(start[2], start[3])))
+    others = np.setdiff1d(np.arange(total), own)
+    k[others], v[others] = math.nan, math.inf
+    ctx = F.Context(0)
+    F.paged_append(kv, batch, k, v, rope=F.Rope(dev(table)), q=q, q_out=q_out, ctx=ctx)
+    F.paged_attention(kv, batch, q_out, out, lse=lse, ctx=ctx)
+    ctx.synchronize()
+    at = np.concatenate([np.arange(n, n + m) for n, m in zip(held, rows)])
+    kr = R.rotate(kx[own], table, at, "interleaved", dtype=np.float32)
+    R.append(cache.codes[0], cache.scales[0], kr.astype(np.float32), rows, cache.lens, cache.table, "i8")
+    R.append(cache.codes[1], cache.scales[1], vx[own].astype(np.float32), rows, cache.lens, cache.table, "i8")
+    cache.check()
+    expected = qx.astype(np.float32)
+    expected[own] = R.rotate(qx[own], table, at, "interleaved", dtype=np.float32)
+    assert np.array_equal(q_out.cpu().numpy(), expected)
+    assert (out[others] == 5).all() and (lse[others] == 5).all()
+    assert (out[own] != 5).all() and lse[own].isfinite().all()
+    # Positions that are given hold for every row.
+    where = dev((np.arange(total) % (10 + per)).astype(np.int32))
+    F.paged_append(kv, batch, k, v, rope=F.Rope(dev(table)), positions=where, q=q, q_out=q_out, ctx=ctx)
+    ctx.synchronize()
+    expected = R.rotate(qx, table, np.arange(total) % (10 + per), "interleaved", dtype=np.float32)
+    assert np.array_equal(q_out.cpu().numpy(), expected)
+    ctx.close()
