@@ -120,8 +120,12 @@ struct HostDesc {
 struct DeviceGuard {
     int prev = -1;
     explicit DeviceGuard(int dev) {
+        // A thread that has made no CUDA call yet has device 0, but not its context,
+        // which encoding a tensor map needs: set once by each thread at least.
+        static thread_local int bound = -1;
         cudaGetDevice(&prev);
-        if (prev != dev) cudaSetDevice(dev);
+        if (prev != dev || bound != dev) cudaSetDevice(dev);
+        bound = dev;
     }
     ~DeviceGuard() {
         int cur = -1;

@@ -839,3 +839,29 @@ def test_rows_of_no_sequence(per):
     expected = R.rotate(qx, table, np.arange(total) % (10 + per), "interleaved", dtype=np.float32)
     assert np.array_equal(q_out.cpu().numpy(), expected)
     ctx.close()
+
+
+def test_attention_from_a_thread_without_cuda_calls_before_it():
+    """A server's worker thread, whose first CUDA call of any kind is an attention on a context that others made."""
+    import threading
+    rng = np.random.default_rng(51)
+    cache = Cache(rng, "e4m3", 64, 16, 2, [300])
+    kv, batch = cache.on_device(), cache.batch([1], False)
+    q, _ = rows_of(rng, 1, 4, 64, "bf16")
+    expected, out = (torch.zeros_like(q) for _ in range(2))
+    ctx = F.Context(0)
+    F.paged_attention(kv, batch, q, expected, ctx=ctx)
+    failures = []
+
+    def call():
+        try:
+            F.paged_attention(kv, batch, q, out, ctx=ctx)
+        except Exception as e:  # noqa: BLE001
+            failures.append(e)
+
+    worker = threading.Thread(target=call)
+    worker.start()
+    worker.join()
+    ctx.synchronize()
+    assert not failures and torch.equal(out, expected)
+    ctx.close()
