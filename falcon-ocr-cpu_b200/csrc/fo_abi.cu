@@ -10,6 +10,7 @@
 #include <cstdio>
 #include <algorithm>
 #include <cstring>
+#include <mutex>
 #include <string>
 #include <vector>
 
@@ -55,6 +56,20 @@ int cuda_fail(cudaError_t e, const char *what) {
         cudaError_t e_ = (call);                    \
         if (e_ != cudaSuccess) return cuda_fail(e_, what); \
     } while (0)
+
+#define FO_TRY(call)                  \
+    do {                              \
+        const int st_ = (call);       \
+        if (st_ != FO_OK) return st_; \
+    } while (0)
+
+// What allocates cannot be part of a graph, and trying would end the capture.
+int refuse_capture(cudaStream_t stream, const char *what) {
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    FO_CUDA(cudaStreamIsCapturing(stream, &capture), "cudaStreamIsCapturing");
+    if (capture == cudaStreamCaptureStatusNone) return FO_OK;
+    return fail(FO_ERR_INVALID, "%s cannot be captured in a CUDA graph: do it on this stream once before", what);
+}
 
 // A device buffer that grows on demand (prefill staging and scratch only;
 // decode paths use buffers reserved at seal time).
@@ -163,7 +178,8 @@ struct fo_ctx {
     cudaStream_t comm = nullptr;
     std::vector<cudaEvent_t> comm_ev;
     // Paged attention: the blocks' unfinished parts and their counters, of one
-    // size for all calls, made by the first.
+    // size for all calls, made by the first (of several threads' too).
+    std::mutex paged_mutex;
     DevBuf paged_parts;
     int sms = 0;
     size_t paged_part_rows() const { return (size_t)2 * sms * FO_PAGED_QUERIES; }
@@ -331,6 +347,7 @@ int report_device_errors(fo_ctx *ctx, unsigned bits) {
         return fail(FO_ERR_NONFINITE, "a value appended to a paged cache is not finite");
     }
     // A paged attention that unwound may have left its blocks' counters short.
+    std::lock_guard<std::mutex> lock(ctx->paged_mutex);
     if (ctx->sms)
         FO_CUDA(cudaMemsetAsync(ctx->paged_counters(), 0, (size_t)ctx->sms * 4, ctx->stream),
                 "cudaMemsetAsync(paged attention counters)");
@@ -483,6 +500,7 @@ int fo_ctx_create(int device, void *stream, fo_ctx **out) {
     FO_CUDA(cudaGetDeviceCount(&count), "cudaGetDeviceCount");
     if (device < 0 || device >= count) return fail(FO_ERR_INVALID, "fo_ctx_create: no CUDA device %d", device);
     DeviceGuard guard(device);
+    FO_TRY(refuse_capture((cudaStream_t)stream, "a context allocates and"));
     fo_ctx *ctx = new fo_ctx();
     ctx->device = device;
     // NULL is CUDA's default stream, as in the runtime API.
@@ -1790,11 +1808,19 @@ int check_paged(const fo_paged_kv *kv, const fo_paged_batch *b) {
     return FO_OK;
 }
 
-#define FO_TRY(call)                  \
-    do {                              \
-        const int st_ = (call);       \
-        if (st_ != FO_OK) return st_; \
-    } while (0)
+// The scratch of a context's paged attentions, at the first of them.
+int make_paged_parts(fo_ctx *ctx) {
+    std::lock_guard<std::mutex> lock(ctx->paged_mutex);
+    if (ctx->sms) return FO_OK;
+    FO_TRY(refuse_capture(ctx->stream, "a context's first paged attention makes its scratch and"));
+    int sms = 0;
+    FO_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, ctx->device), "cudaDeviceGetAttribute");
+    const size_t parts = (size_t)2 * sms * FO_PAGED_QUERIES;
+    FO_CUDA(ctx->paged_parts.ensure(parts * (128 + 2) * 4 + (size_t)sms * 4), "cudaMalloc(paged attention parts)");
+    FO_CUDA(cudaMemsetAsync(ctx->paged_parts.ptr, 0, ctx->paged_parts.bytes, ctx->stream), "cudaMemset(parts)");
+    ctx->sms = sms;
+    return FO_OK;
+}
 
 }  // namespace
 
@@ -1929,14 +1955,7 @@ int fo_paged_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch 
     a.scale = scale;
     a.window = window < INT32_MAX ? (int32_t)window : 0;  // as many positions as there can be
     a.err = ctx->dev_err;
-    if (!ctx->sms) {
-        int sms = 0;
-        FO_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, ctx->device), "cudaDeviceGetAttribute");
-        const size_t parts = (size_t)2 * sms * FO_PAGED_QUERIES;
-        FO_CUDA(ctx->paged_parts.ensure(parts * (128 + 2) * 4 + (size_t)sms * 4), "cudaMalloc(paged attention parts)");
-        FO_CUDA(cudaMemsetAsync(ctx->paged_parts.ptr, 0, ctx->paged_parts.bytes, ctx->stream), "cudaMemset(parts)");
-        ctx->sms = sms;
-    }
+    FO_TRY(make_paged_parts(ctx));
     a.part_o = (float *)ctx->paged_parts.ptr;
     a.part_ml = ctx->paged_part_ml();
     a.counters = ctx->paged_counters();

@@ -22,6 +22,7 @@ from __future__ import annotations
 import ctypes
 import os
 import struct
+import threading
 from typing import Optional, Sequence
 
 import numpy as np
@@ -723,6 +724,7 @@ def static_scratch_status(stream=None):
 # ------------------------------------------------ rotary positions, paged cache
 _ROW_TYPES = None  # torch dtype -> FO_DT_*
 _stream_contexts = {}
+_stream_contexts_lock = threading.Lock()
 
 
 def _torch():
@@ -734,12 +736,18 @@ def _torch():
 
 
 def stream_context(device: int) -> Context:
-    """The context of torch's current stream on `device` (made at its first
-    use, so a stream that is to be captured runs once before)."""
+    """The context of torch's current stream on `device`, made at its first
+    use.  That and the first attention on it allocate, which a capture refuses:
+    a graph is captured on a stream that its calls have run on before
+    (``torch.cuda.graph(g, stream=side)``; without ``stream`` torch captures on
+    one of its own)."""
     stream = _torch()._C._cuda_getCurrentRawStream(device)
     ctx = _stream_contexts.get((device, stream))
     if ctx is None:
-        ctx = _stream_contexts[(device, stream)] = Context(device, stream or None)
+        with _stream_contexts_lock:  # one for all threads on the stream
+            ctx = _stream_contexts.get((device, stream))
+            if ctx is None:
+                ctx = _stream_contexts[(device, stream)] = Context(device, stream or None)
     return ctx
 
 

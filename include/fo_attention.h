@@ -450,12 +450,14 @@ int fo_draft_attend(fo_draft_kv *kv, const float *q, int64_t bases, int64_t wind
  * reference, whose caches are one contiguous allocation per page of text).
  *
  * These calls take DEVICE pointers only, launch on the context's stream and
- * return; none synchronizes, and after its first call on a context none
- * allocates, so they can be captured in CUDA graphs.  What the device alone
- * can see (a page number outside the pool, a rotary position outside the
- * table, a value that is not finite) goes to the context's error word, which
- * fo_ctx_synchronize reports and clears; no such input reads or writes out
- * of bounds. */
+ * return; none synchronizes, and only a context's first fo_paged_attention
+ * allocates (its scratch), so they can be captured in CUDA graphs; that first
+ * one, and fo_ctx_create, on a stream that is being captured are refused.
+ *
+ * What the device alone can see (a page number outside the pool, a rotary
+ * position outside the table, a value that is not finite) goes to the
+ * context's error word, which fo_ctx_synchronize reports and clears; no such
+ * input reads or writes out of bounds. */
 
 #define FO_DT_F32 0
 #define FO_DT_BF16 1

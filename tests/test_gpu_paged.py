@@ -841,6 +841,79 @@ def test_rows_of_no_sequence(per):
     ctx.close()
 
 
+def test_first_use_while_a_graph_is_captured(monkeypatch):
+    """A stream's context and its attention's scratch cannot be made inside a capture: the call says so, before it
+    launches or allocates anything, and works once they are there."""
+    rng = np.random.default_rng(45)
+    cache = Cache(rng, "i8", 64, 16, 1, [40])
+    kv, batch = cache.on_device(), cache.batch([1], False)
+    q, _ = rows_of(rng, 1, 2, 64, "f32")
+    expected, out = torch.empty_like(q), torch.zeros_like(q)
+    F.paged_attention(kv, batch, q, expected)
+    monkeypatch.setattr(F, "_stream_contexts", {})
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+
+    def refused():
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=side):
+            with pytest.raises(F.FoError, match="captur"):
+                F.paged_attention(kv, batch, q, out)
+            out.add_(0.0)  # the capture itself goes on
+        graph.replay()
+        torch.cuda.synchronize()
+
+    refused()  # no context
+    with torch.cuda.stream(side):
+        F.rope(q, torch.empty_like(q), F.Rope(dev(plain_table(4, 64))))
+    refused()  # a context that no attention has run on
+    with torch.cuda.stream(side):
+        F.paged_attention(kv, batch, q, out)
+    torch.cuda.synchronize()
+    out.zero_()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        F.paged_attention(kv, batch, q, out)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, expected)
+
+
+def test_first_attentions_of_a_context_from_several_threads():
+    """They make its scratch once."""
+    import threading
+    rng = np.random.default_rng(46)
+    cache = Cache(rng, "i8", 64, 16, 2, [5000, 40])
+    kv = cache.on_device()
+    batches = [cache.batch([1, 1], False) for _ in range(8)]
+    q, _ = rows_of(rng, 2, 4, 64, "f32")
+    expected = torch.empty_like(q)
+    F.paged_attention(kv, cache.batch([1, 1], False), q, expected)
+    torch.cuda.synchronize()
+    for _ in range(5):
+        ctx = F.Context(0)
+        outs = [torch.zeros_like(q) for _ in batches]
+        gate = threading.Barrier(len(batches))
+        failures = []
+
+        def call(batch, out):
+            gate.wait()
+            try:
+                F.paged_attention(kv, batch, q, out, ctx=ctx)
+            except Exception as e:  # noqa: BLE001
+                failures.append(e)
+
+        threads = [threading.Thread(target=call, args=a) for a in zip(batches, outs)]
+        for t in threads:
+            t.start()
+        for t in threads:
+            t.join()
+        ctx.synchronize()
+        assert not failures
+        assert all(torch.equal(o, expected) for o in outs)
+        ctx.close()
+
+
 def test_attention_from_a_thread_without_cuda_calls_before_it():
     """A server's worker thread, whose first CUDA call of any kind is an attention on a context that others made."""
     import threading
