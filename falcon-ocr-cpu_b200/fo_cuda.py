@@ -740,7 +740,8 @@ def stream_context(device: int) -> Context:
     use.  That and the first attention on it allocate, which a capture refuses:
     a graph is captured on a stream that its calls have run on before
     (``torch.cuda.graph(g, stream=side)``; without ``stream`` torch captures on
-    one of its own)."""
+    one of its own).  Attentions of one context share its scratch: graphs that
+    were captured on one stream must not be replayed at the same time."""
     stream = _torch()._C._cuda_getCurrentRawStream(device)
     ctx = _stream_contexts.get((device, stream))
     if ctx is None:

@@ -453,11 +453,17 @@ int fo_draft_attend(fo_draft_kv *kv, const float *q, int64_t bases, int64_t wind
  * return; none synchronizes, and only a context's first fo_paged_attention
  * allocates (its scratch), so they can be captured in CUDA graphs; that first
  * one, and fo_ctx_create, on a stream that is being captured are refused.
+ * A context's attentions share its scratch, so they, and the graphs that hold
+ * them, must not run at the same time: graphs captured on one stream are not
+ * to be replayed on two streams at once, nor beside the context's own calls on
+ * another (outputs would be wrong without an error).
  *
  * What the device alone can see (a page number outside the pool, a rotary
  * position outside the table, a value that is not finite) goes to the
  * context's error word, which fo_ctx_synchronize reports and clears; no such
- * input reads or writes out of bounds. */
+ * input reads or writes out of bounds.  When it reports a wait that ran out
+ * (FO_ERR_CUDA), what the context's calls gave since the last report is not to
+ * be used; the calls after it start clean. */
 
 #define FO_DT_F32 0
 #define FO_DT_BF16 1
