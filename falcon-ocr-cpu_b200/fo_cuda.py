@@ -752,30 +752,44 @@ def stream_context(device: int) -> Context:
     return ctx
 
 
-def _rows(t, name: str) -> bytes:
-    """A CUDA tensor [rows][heads][head_dim] as fo_rows; rows and heads in any
-    strides."""
+def _rows(t, name: str, device: int) -> bytes:
+    """A tensor [rows][heads][head_dim] on GPU `device` as fo_rows; rows and
+    heads in any strides."""
     if _ROW_TYPES is None:
         _torch()
-    kind = _ROW_TYPES.get(t.dtype)
-    if kind is None or not t.is_cuda or t.dim() != 3:
+    kind, at = _ROW_TYPES.get(t.dtype), t.get_device()
+    if kind is None or at < 0 or t.dim() != 3:
         raise FoError(f"{name} must be a CUDA tensor [rows][heads][head_dim] of float32 or bfloat16")
+    if at != device:
+        raise FoError(f"{name} is on GPU {at}, the call on GPU {device}")
     row, head, one = t.stride()
     if one != 1:
         raise FoError(f"{name}: a head's values must be adjacent")
     return _PACK_ROWS(t.data_ptr(), row, head, t.size(1), kind)
 
 
-def _device_ints(t, name: str):
+def _device_ints(t, name: str, device: int):
     if not t.is_cuda or not t.is_contiguous() or t.dtype != _torch().int32:
         raise FoError(f"{name} must be a contiguous CUDA tensor of int32")
+    if t.get_device() != device:
+        raise FoError(f"{name} is on GPU {t.get_device()}, the call on GPU {device}")
     return t.data_ptr()
 
 
-def _floats(t, n: int, name: str):
+def _floats(t, n: int, name: str, device: int):
     if not t.is_cuda or not t.is_contiguous() or t.numel() != n or t.dtype != _torch().float32:
         raise FoError(f"{name} must be a contiguous CUDA tensor of {n} float32")
+    if t.get_device() != device:
+        raise FoError(f"{name} is on GPU {t.get_device()}, the call on GPU {device}")
     return t.data_ptr()
+
+
+def _context(ctx, device: int):
+    if ctx is None:
+        return stream_context(device)
+    if ctx.device != device:
+        raise FoError(f"the context is on GPU {ctx.device}, the call's tensors on GPU {device}")
+    return ctx
 
 
 def rope_table(table, theta=10000.0, scaling="none", factor=1.0, original_positions=0, beta_fast=32.0, beta_slow=1.0,
@@ -785,7 +799,7 @@ def rope_table(table, theta=10000.0, scaling="none", factor=1.0, original_positi
     if not _on_device(table) or not table.is_contiguous() or table.dim() != 3 or table.shape[2] != 2 or \
             str(table.dtype) != "torch.float32":
         raise FoError("a rope table is a contiguous float32 CUDA tensor [positions][rot_dim / 2][2]")
-    ctx = ctx or stream_context(table.device.index)
+    ctx = _context(ctx, table.get_device())
     check(lib().fo_rope_table(ctx.handle, table.data_ptr(), table.shape[0], 2 * table.shape[1],
                               RopeScaling(theta, ROPE_SCALINGS[scaling], factor, original_positions, beta_fast,
                                           beta_slow, attention_factor)))
@@ -799,31 +813,33 @@ class Rope:
         if not _on_device(table) or not table.is_contiguous() or table.dim() != 3 or table.shape[2] != 2 or \
                 str(table.dtype) != "torch.float32":
             raise FoError("a rope table is a contiguous float32 CUDA tensor [positions][rot_dim / 2][2]")
-        self.table = table
+        self.table, self.device = table, table.get_device()
         self.spec = (table.data_ptr(), table.shape[0], 2 * table.shape[1], ROPE_LAYOUTS[layout])
-
         self.plain = _PACK_ROPE(self.spec[0], self.spec[1], 0, self.spec[2], self.spec[3])
 
-    def at(self, positions, rows: int) -> bytes:
+    def at(self, positions, rows: int, device: int) -> bytes:
+        if self.device != device:
+            raise FoError(f"the rope table is on GPU {self.device}, the call on GPU {device}")
         if positions is None:
             return self.plain
         if positions.numel() != rows:
             raise FoError("one position for each row")
         table, n, rot_dim, layout = self.spec
-        return _PACK_ROPE(table, n, _device_ints(positions, "positions"), rot_dim, layout)
+        return _PACK_ROPE(table, n, _device_ints(positions, "positions", device), rot_dim, layout)
 
 
 def rope(x, out, rope: Rope, positions=None, inverse=False, ctx=None):
     """fo_rope: rows x [rows][heads][head_dim] rotated into `out` (x itself is
     allowed) at `positions` [rows] int32 (None: the row's number).  inverse:
     the transposed rotation, which takes a gradient back."""
-    a, b = _rows(x, "x"), _rows(out, "out")
+    device = x.get_device()
+    a, b = _rows(x, "x", device), _rows(out, "out", device)
     shape = x.shape
     if shape != out.shape:
         raise FoError("rope: x and out must have one shape")
     rows, _, dim = shape
-    ctx = ctx or stream_context(x.get_device())
-    check(lib().fo_rope(ctx.handle, a, b, rows, dim, rope.at(positions, rows), 1 if inverse else 0))
+    ctx = _context(ctx, device)
+    check(lib().fo_rope(ctx.handle, a, b, rows, dim, rope.at(positions, rows, device), 1 if inverse else 0))
     return out
 
 
@@ -845,9 +861,11 @@ class PagedKv:
         for t in (k_codes, v_codes, k_scales, v_scales):
             if not t.is_cuda or not t.is_contiguous():
                 raise FoError("paged codes and scales must be contiguous CUDA tensors")
+            if t.get_device() != k_codes.get_device():
+                raise FoError("paged codes and scales must be on one GPU")
         self.keep = (k_codes, v_codes, k_scales, v_scales)
         n_pages, kv_heads, page_size, self.head_dim = k_codes.shape
-        self.device = k_codes.device.index
+        self.device = k_codes.get_device()
         self.pool = PagedPool(k_codes.data_ptr(), v_codes.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr(),
                               n_pages, page_size, kv_heads, self.head_dim, formats[k_codes.dtype])
         self.ref, self.scale = ctypes.byref(self.pool), self.head_dim ** -0.5
@@ -866,17 +884,28 @@ class PagedBatch:
             raise FoError("row_start must have one entry more than there are sequences")
         self.keep = (page_table, lens, row_start)
         n = lens.numel()
-        self.sequences = PagedSequences(_device_ints(page_table, "page_table"), _device_ints(lens, "lens"),
-                                        None if row_start is None else _device_ints(row_start, "row_start"),
-                                        page_table.shape[1], n, rows, n * rows)
-
-        self.ref = ctypes.byref(self.sequences)
+        self.device = device = page_table.get_device()
+        self.sequences = PagedSequences(
+            _device_ints(page_table, "page_table", device), _device_ints(lens, "lens", device),
+            None if row_start is None else _device_ints(row_start, "row_start", device), page_table.shape[1], n, rows,
+            n * rows)
+        self._made = (n * rows, ctypes.byref(self.sequences))
 
     def of(self, rows: int):
-        """The batch for a call with so many rows in all."""
-        if self.sequences.total_rows != rows:
-            self.sequences.total_rows = rows
-        return self.ref
+        """The batch for a call with so many rows in all (never changed after: another thread's call may be reading
+        it)."""
+        made = self._made
+        if made[0] != rows:
+            sequences = PagedSequences.from_buffer_copy(self.sequences)
+            sequences.total_rows = rows
+            made = self._made = (rows, ctypes.byref(sequences))
+        return made[1]
+
+
+def _paged_device(kv: PagedKv, batch: PagedBatch) -> int:
+    if batch.device != kv.device:
+        raise FoError(f"the page table is on GPU {batch.device}, the pool on GPU {kv.device}")
+    return kv.device
 
 
 def paged_append(kv: PagedKv, batch: PagedBatch, k, v, rope: Optional[Rope] = None, positions=None, q=None,
@@ -884,7 +913,8 @@ def paged_append(kv: PagedKv, batch: PagedBatch, k, v, rope: Optional[Rope] = No
     """fo_paged_append: rows k, v [rows][kv heads][head dim] into the batch's
     pages, keys rotated on the way when `rope` is given (at `positions`, else
     at their place in the cache), and queries q rotated into q_out."""
-    rk, rv = _rows(k, "k"), _rows(v, "v")
+    device = _paged_device(kv, batch)
+    rk, rv = _rows(k, "k", device), _rows(v, "v", device)
     rows, _, dim = shape = k.shape
     if dim != kv.head_dim or v.shape != shape:
         raise FoError("paged_append: k and v must be [rows][kv heads][head dim] of the cache")
@@ -893,24 +923,27 @@ def paged_append(kv: PagedKv, batch: PagedBatch, k, v, rope: Optional[Rope] = No
         shape = q.shape
         if q_out is None or shape != q_out.shape or shape[0] != rows or shape[2] != dim:
             raise FoError("paged_append: q and q_out must be [rows][heads][head dim]")
-        rq, ro = _rows(q, "q"), _rows(q_out, "q_out")
-    ctx = ctx or stream_context(kv.device)
+        rq, ro = _rows(q, "q", device), _rows(q_out, "q_out", device)
+    if rope is None and positions is not None:
+        raise FoError("paged_append: positions are the rotation's, without rope there is nothing to do with them")
+    ctx = _context(ctx, device)
     check(lib().fo_paged_append(ctx.handle, kv.ref, batch.of(rows), rk, rv, rq, ro,
-                                None if rope is None else rope.at(positions, rows)))
+                                None if rope is None else rope.at(positions, rows, device)))
 
 
 def paged_attention(kv: PagedKv, batch: PagedBatch, q, out, sinks=None, scale=None, window=0, lse=None, ctx=None):
     """fo_paged_attention: q [rows][heads][head dim] over the batch's cached
     positions into `out`; scale None: 1 / sqrt(head dim)."""
-    rq, ro = _rows(q, "q"), _rows(out, "out")
+    device = _paged_device(kv, batch)
+    rq, ro = _rows(q, "q", device), _rows(out, "out", device)
     rows, heads, dim = shape = q.shape
     if dim != kv.head_dim or out.shape != shape:
         raise FoError("paged_attention: q and out must be [rows][heads][head dim] of the cache's width")
-    ctx = ctx or stream_context(kv.device)
+    ctx = _context(ctx, device)
     check(lib().fo_paged_attention(ctx.handle, kv.ref, batch.of(rows), rq,
-                                   None if sinks is None else _floats(sinks, heads, "sinks"),
+                                   None if sinks is None else _floats(sinks, heads, "sinks", device),
                                    kv.scale if scale is None else scale, window, ro,
-                                   None if lse is None else _floats(lse, rows * heads, "lse")))
+                                   None if lse is None else _floats(lse, rows * heads, "lse", device)))
     return out
 
 

@@ -213,3 +213,97 @@ def test_overlapped_kernels_make_no_read_only_loads():
     for name in overlapped:
         for word in ("__ldg(", "ld.global.nc", "__restrict__"):
             assert word not in files[name], (name, word)
+
+
+class DeviceTensor:
+    """What the bindings ask of a CUDA tensor, on whichever GPU."""
+    is_cuda = True
+    __module__ = "torch"  # by which the bindings tell torch's tensors
+
+    def __init__(self, shape, dtype, device=0):
+        self.shape, self.dtype, self.index = tuple(shape), dtype, device
+        self.device = self
+        self.__cuda_array_interface__ = {}
+
+    def dim(self):
+        return len(self.shape)
+
+    def numel(self):
+        return int(np.prod(self.shape))
+
+    def size(self, i):
+        return self.shape[i]
+
+    def stride(self, i=None):
+        s = tuple(int(np.prod(self.shape[j + 1:])) for j in range(len(self.shape)))
+        return s if i is None else s[i]
+
+    def get_device(self):
+        return self.index
+
+    def is_contiguous(self):
+        return True
+
+    def data_ptr(self):
+        return BASE
+
+
+class NoContext:
+    handle, device = None, 0
+
+
+def device_call(call, **other):
+    """One of the paged calls, all its tensors on GPU 0 but those named."""
+    torch = pytest.importorskip("torch")
+
+    def t(name, shape, dtype=torch.float32):
+        return DeviceTensor(shape, dtype, other.get(name, 0))
+
+    ints = torch.int32
+    rope = F.Rope(t("table", (16, 32, 2)))
+    kv = F.PagedKv(t("k_codes", (4, 8, 16, 64), torch.int8), t("v_codes", (4, 8, 16, 64), torch.int8),
+                   t("k_scales", (4, 8)), t("v_scales", (4, 8)))
+    batch = F.PagedBatch(t("page_table", (2, 2), ints), t("lens", (2,), ints), row_start=t("row_start", (3,), ints))
+    if call == "rope":
+        F.rope(t("q", (2, 16, 64)), t("out", (2, 16, 64)), rope, t("positions", (2,), ints), ctx=NoContext)
+    elif call == "append":
+        F.paged_append(kv, batch, t("k", (2, 8, 64)), t("v", (2, 8, 64)), rope, t("positions", (2,), ints),
+                       t("q", (2, 16, 64)), t("q_out", (2, 16, 64)), ctx=NoContext)
+    else:
+        F.paged_attention(kv, batch, t("q", (2, 16, 64)), t("out", (2, 16, 64)), t("sinks", (16,)), lse=t("lse", (2, 16)),
+                          ctx=NoContext)
+
+
+@pytest.mark.parametrize("call,names", [
+    ("rope", ["table", "out", "positions"]),
+    ("append", ["k_codes", "v_codes", "k_scales", "v_scales", "page_table", "lens", "row_start", "k", "v", "table",
+                "positions", "q", "q_out"]),
+    ("attend", ["k_codes", "v_codes", "k_scales", "v_scales", "page_table", "lens", "row_start", "q", "out", "sinks",
+                "lse"]),
+])
+def test_bindings_refuse_tensors_of_another_gpu(call, names):
+    with pytest.raises(F.FoError, match="null context"):  # all on one: taken
+        device_call(call)
+    for name in names:
+        with pytest.raises(F.FoError, match="GPU"):
+            device_call(call, **{name: 1})
+
+
+def test_append_refuses_positions_without_a_rotation():
+    torch = pytest.importorskip("torch")
+    kv = F.PagedKv(DeviceTensor((4, 8, 16, 64), torch.int8), DeviceTensor((4, 8, 16, 64), torch.int8),
+                   DeviceTensor((4, 8), torch.float32), DeviceTensor((4, 8), torch.float32))
+    batch = F.PagedBatch(DeviceTensor((2, 2), torch.int32), DeviceTensor((2,), torch.int32))
+    k = DeviceTensor((2, 8, 64), torch.float32)
+    with pytest.raises(F.FoError, match="positions"):
+        F.paged_append(kv, batch, k, k, positions=DeviceTensor((2,), torch.int32), ctx=NoContext)
+
+
+def test_a_batch_that_another_call_uses_does_not_change_under_it():
+    torch = pytest.importorskip("torch")
+    batch = F.PagedBatch(DeviceTensor((2, 2), torch.int32), DeviceTensor((2,), torch.int32), rows=9,
+                         row_start=DeviceTensor((3,), torch.int32))
+    first = batch.of(5)
+    second = batch.of(7)
+    assert first._obj.total_rows == 5 and second._obj.total_rows == 7
+    assert batch.of(7)._obj.total_rows == 7 and batch.of(5)._obj.max_rows == 9
