@@ -1746,9 +1746,10 @@ int fo_draft_attend(fo_draft_kv *kv, const float *q, int64_t bases, int64_t wind
 // ------------------------------------------- rotary positions, paged cache
 namespace {
 
-// Rows of heads that a call reads, or writes (every element apart).
+// Rows of heads that a call reads, or writes (every element apart); no rows
+// need no memory.
 int check_rows(const fo_rows *r, const char *name, int64_t rows, int64_t dim, bool written) {
-    if (!r || !r->data) return fail(FO_ERR_INVALID, "%s: null pointer", name);
+    if (!r || (!r->data && rows > 0)) return fail(FO_ERR_INVALID, "%s: null pointer", name);
     if (r->dtype != FO_DT_F32 && r->dtype != FO_DT_BF16) return fail(FO_ERR_INVALID, "%s: unknown type %d", name, r->dtype);
     if (r->heads < 1) return fail(FO_ERR_INVALID, "%s: head count must be positive", name);
     if (r->row_stride < 0 || r->head_stride < 0) return fail(FO_ERR_INVALID, "%s: negative stride", name);

@@ -914,6 +914,27 @@ def test_first_attentions_of_a_context_from_several_threads():
         ctx.close()
 
 
+def test_calls_without_rows():
+    """Empty batches (torch gives their tensors no memory) do nothing."""
+    kv = F.PagedKv(*(torch.ones(3, 2, 16, 64, dtype=torch.int8, device="cuda") for _ in range(2)),
+                   *(torch.ones(3, 2, device="cuda") for _ in range(2)))
+    rope = F.Rope(dev(plain_table(4, 64)))
+    ints = dict(dtype=torch.int32, device="cuda")
+    ctx = F.Context(0)
+    for batch in (F.PagedBatch(torch.zeros(0, 2, **ints), torch.zeros(0, **ints)),
+                  F.PagedBatch(torch.zeros(0, 2, **ints), torch.zeros(0, **ints), row_start=torch.zeros(1, **ints)),
+                  F.PagedBatch(torch.zeros(2, 2, **ints), torch.zeros(2, **ints), row_start=torch.zeros(3, **ints)),
+                  F.PagedBatch(torch.zeros(2, 2, **ints), torch.zeros(2, **ints), rows=0)):
+        for dtype in DTYPES.values():
+            q, k = torch.empty(0, 4, 64, dtype=dtype, device="cuda"), torch.empty(0, 2, 64, dtype=dtype, device="cuda")
+            F.rope(q, q, rope, ctx=ctx)
+            F.paged_append(kv, batch, k, k, rope=rope, q=q, q_out=torch.empty_like(q), ctx=ctx)
+            F.paged_attention(kv, batch, q, torch.empty_like(q), lse=torch.empty(0, 4, device="cuda"), ctx=ctx)
+    ctx.synchronize()
+    assert all((t.float() == 1).all() for t in kv.keep)
+    ctx.close()
+
+
 def test_attention_from_a_thread_without_cuda_calls_before_it():
     """A server's worker thread, whose first CUDA call of any kind is an attention on a context that others made."""
     import threading

@@ -307,3 +307,18 @@ def test_a_batch_that_another_call_uses_does_not_change_under_it():
     second = batch.of(7)
     assert first._obj.total_rows == 5 and second._obj.total_rows == 7
     assert batch.of(7)._obj.total_rows == 7 and batch.of(5)._obj.max_rows == 9
+
+
+def test_calls_without_rows_need_no_memory():
+    """No rows: the rows' pointers may be null (torch gives an empty tensor none); everything else is checked."""
+    none, none16, s = rows(data=None), rows(16, data=None, row_stride=1024), spec()
+    empty = batch(n_seqs=0, total_rows=0, page_table=None, lens=None)
+    calls = [lambda: rope(x=none, out=none, n=0), lambda: append(b=empty, k=none, v=none),
+             lambda: append(b=empty, k=none, v=none, q=none16, q_out=none16, s=s),
+             lambda: append(b=batch(total_rows=0, max_rows=0), k=none, v=none),
+             lambda: attend(b=empty, q=none16, out=none16),
+             lambda: attend(b=batch(row_start=BASE, total_rows=0), q=none16, out=none16)]
+    for call in calls:
+        assert call() == F.ERR_INVALID and last_error() == "null context"
+    assert rope(x=none, out=none, n=1) == F.ERR_INVALID and "null pointer" in last_error()
+    assert append(b=empty, k=rows(4, data=None), v=none) == F.ERR_INVALID and "cache's heads" in last_error()
