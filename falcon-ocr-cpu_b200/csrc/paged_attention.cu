@@ -31,11 +31,14 @@
 // O^T += V^T P^T.  Nothing of the cache is rounded; a scale multiplies a
 // finished sum.
 //   int8: m16n8k32 products of bytes with exact 32-bit sums, one for each byte
-//   of a query and of a probability.  A query is an integer relative to a power
-//   of two near its largest element: of 16 bits for BF16 rows (exactly the
-//   query, where an element is at least 2^-8 of the largest; 2^-16 of that
-//   one otherwise), of 23 for FP32 rows.  A probability is one of 16 bits
-//   (BF16 rows, whose output has 8), or 23, relative to its tile's largest.
+//   of a query and of a probability.  A query is a 23-bit integer relative to a
+//   power of two near its largest element: within 2^-22 of that one, and exactly a
+//   BF16 query's element where it is at least 2^-14 of the largest.  (16 bits for BF16
+//   rows, one product of three fewer, take 282 us instead of 303 at 40 queries to a
+//   KV head and 89 instead of 91 at two, but next to one large element the scores
+//   lose what BF16 holds.)
+//   A probability is an integer of 16 bits (BF16 rows, whose output has 8), or
+//   23, relative to its tile's largest.
 //   e4m3: m16n8k16 products of FP16, which holds every e4m3 number.  (With
 //   m16n8k32 products of e4m3, two terms to a query and three to a probability,
 //   an earlier form took 124 us for 64 sequences of 7,500, and 97 with FP16,
@@ -94,8 +97,8 @@ struct PaShape {
     static constexpr int HALF = TILE / 2;          // a consumer warp's
     static constexpr int STAGE = 2 * TILE_BYTES;
     static constexpr bool I8 = FORMAT == FO_PAGED_I8;
-    static constexpr int QT = (I8 ? 2 : 1) + F32;  // a query's terms, and a probability's
-    static constexpr int PT = QT;
+    static constexpr int QT = I8 ? 3 : 1 + F32;    // a query's terms
+    static constexpr int PT = (I8 ? 2 : 1) + F32;  // a probability's
     static constexpr int KQ = I8 ? D / 32 : D / 16;          // k steps over a row's elements
     static constexpr int PART_LD = D + 4;          // a column of a consumer's part, in floats
     static constexpr int PARTS = PA_CONSUMERS * 8 * PART_LD * 4;
@@ -418,11 +421,11 @@ __device__ __forceinline__ void pa_epilogue(const fo_paged_attention_launch &a, 
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
             top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
             const unsigned all_finite = __ballot_sync(0xffffffffu, finite);
-            // A power of two near the largest element brings it to [2^14, 2^15) or
-            // [2^21, 2^22) (int8) or [1, 2) (e4m3); in two factors, so that FP32's whole range
+            // A power of two near the largest element brings it to [2^21, 2^22)
+            // (int8) or [1, 2) (e4m3); in two factors, so that FP32's whole range
             // of exponents can be brought there.
             const int e = max((int)(__float_as_uint(top) >> 23), 1);
-            const float up = I8 ? (F32 ? 2097152.0f : 16384.0f) : 1.0f;
+            const float up = I8 ? 2097152.0f : 1.0f;
             const float inv0 = __uint_as_float((uint32_t)(254 - (e + 1) / 2 - 63) << 23);
             const float inv1 = __uint_as_float((uint32_t)(254 - (e - (e + 1) / 2) - 64) << 23) * up;
             if (t == 0) {
@@ -453,7 +456,7 @@ __device__ __forceinline__ void pa_epilogue(const fo_paged_attention_launch &a, 
                                                __byte_perm(lo01, lo23, 0x5410)};
 #pragma unroll
                         for (int i = 0; i < QT; i++)
-                            reinterpret_cast<uint32_t *>(to + (i * KQ + 2 * c + w / 2) * 32)[w % 2] = f[3 - QT + i];
+                            reinterpret_cast<uint32_t *>(to + (i * KQ + 2 * c + w / 2) * 32)[w % 2] = f[i];
                     } else {
                         // Step 4 c + w.
 #pragma unroll
@@ -937,7 +940,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                         if constexpr (I8) {
                             sc[e] = __uint_as_float(acc[mt][A - 1][e]) - PA_MAGIC_F;
                             sc[e] = fmaf(__uint_as_float(acc[mt][A > 1 ? A - 2 : 0][e]) - PA_MAGIC_F, 256.0f, sc[e]);
-                            if constexpr (F32) sc[e] = fmaf(__uint_as_float(acc[mt][0][e]) - PA_MAGIC_F, 65536.0f, sc[e]);
+                            sc[e] = fmaf(__uint_as_float(acc[mt][0][e]) - PA_MAGIC_F, 65536.0f, sc[e]);
                         } else {
                             sc[e] = acc[mt][0][e];
                         }

@@ -935,6 +935,32 @@ def test_calls_without_rows():
     ctx.close()
 
 
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_attention_queries_with_one_large_element(dim, dtype):
+    """One element 2^7 times the others, in a dimension where all keys are 0: the scores come from the others, and are
+    as exact as without it (the bound on a score, 2^-17 of its sum of magnitudes).  FP32 rows hold an element to 2^-22 of
+    their largest one, which adds that to each product."""
+    rng = np.random.default_rng(47)
+    for n in (8, 500):
+        cache = Cache(rng, "i8", dim, 16, 2, [n])
+        cache.codes[0][..., 5] = 0
+        kv, batch = cache.on_device(), cache.batch([1], False)
+        q, _ = rows_of(rng, 1, 6, dim, dtype)
+        q[..., 5] = 128.0 * q.abs().amax(-1)
+        qv = q.double().cpu().numpy()
+        out, lse = torch.empty_like(q), torch.empty(1, 6, device="cuda")
+        F.paged_attention(kv, batch, q, out, lse=lse)
+        k, v = cache.values(0, 0), cache.values(1, 0)
+        o, z, size = R.attend(qv[0], k, v, n - 1, 0, None, dim ** -0.5)
+        d, top = 2.0 ** -17 * size, np.abs(v).max()
+        if dtype == "f32":
+            d += 2.0 ** -22 * np.abs(qv).max() * np.abs(k).sum(-1).max() * dim ** -0.5
+        assert (np.abs(lse[0].double().cpu().numpy() - z) <= d + 2.0 ** -20 * (1 + np.abs(z))).all()
+        bound = (4 * d + 2.0 ** -18 + (2.0 ** -11 if dtype == "bf16" else 0)) * top
+        assert within(out[0].double().cpu().numpy(), o, bound, dtype)
+
+
 def test_attention_from_a_thread_without_cuda_calls_before_it():
     """A server's worker thread, whose first CUDA call of any kind is an attention on a context that others made."""
     import threading
