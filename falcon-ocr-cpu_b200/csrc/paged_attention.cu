@@ -38,7 +38,12 @@
 //   KV head and 89 instead of 91 at two, but next to one large element the scores
 //   lose what BF16 holds.)
 //   A probability is an integer of 16 bits (BF16 rows, whose output has 8), or
-//   23, relative to its tile's largest.
+//   23, relative to its half tile's largest.  Where a few keys are so large that
+//   half or more of a query's lanes have none of 2^-8 of the largest (a text's
+//   first tokens often take most of the softmax, with values near zero),
+//   what the integers leave is multiplied too, in a second set of products: each
+//   probability then keeps 8 bits, or 15, of its own down to 2^-24 of the largest.
+//   (Looking for that takes 2 us of 93 where HBM bounds the call.)
 //   e4m3: m16n8k16 products of FP16, which holds every e4m3 number.  (With
 //   m16n8k32 products of e4m3, two terms to a query and three to a probability,
 //   an earlier form took 124 us for 64 sequences of 7,500, and 97 with FP16,
@@ -53,15 +58,15 @@
 // Maxima, sums and outputs are FP32.
 //
 // Measured (CUDA graph): 64 sequences of 6,545 to 8,592 positions, 2 queries to
-// each of 8 KV heads of 64, int8: 85 us, 5.8 TB/s, 0.90 of the measured copy
-// bandwidth; 16 of 1,000 to 32,768, 4 queries, heads of 128, e4m3: 113 us, 6.0
+// each of 8 KV heads of 64, int8: 87 us, 5.7 TB/s, 0.88 of the measured copy
+// bandwidth; 16 of 1,000 to 32,768, 4 queries, heads of 128, e4m3: 112 us, 6.0
 // TB/s.  Earlier forms, 64 sequences of 7,500 in a stream of calls: one
 // producer warp 165 us; four, with int8 converted to FP16 for m16n8k16 products,
 // 110; products of the codes themselves, parts joined by the consumers, 103; by
 // epilogue warps, 95.  With 40 queries to a KV head (10 of the 12 consumer warps
-// at one tile) a tile takes some 6,600 warp instructions, at 36 % of the issue
-// slots with the integer tensor pipe at 14 %: 283 us for 48 sequences in a
-// window of 4,096, 1.3 TB/s.  A call of one short sequence takes 9.2 us, a
+// at one tile): 304 us for 48 sequences in a window of 4,096, 1.2 TB/s; a tile took
+// some 6,600 warp instructions with 16-bit queries, at 36 % of the issue slots with
+// the integer tensor pipe at 14 %.  A call of one short sequence takes 9.6 us, a
 // chain of launch, length, page number, tile and join.
 #include "paged.cuh"
 #include "sm100.cuh"
@@ -102,8 +107,11 @@ struct PaShape {
     static constexpr int KQ = I8 ? D / 32 : D / 16;          // k steps over a row's elements
     static constexpr int PART_LD = D + 4;          // a column of a consumer's part, in floats
     static constexpr int PARTS = PA_CONSUMERS * 8 * PART_LD * 4;
+    static constexpr int REST = I8 ? PT * (HALF / 16) * 128 : 0;  // a warp's second set of probabilities
     static constexpr int Q_TILE = QT * KQ * 32 * 8;  // an n8 tile of queries as operands
-    static constexpr int smem(int q_tiles) { return 1024 + PA_STAGES * STAGE + PARTS + q_tiles * Q_TILE; }
+    static constexpr int smem(int q_tiles) {
+        return 1024 + PA_STAGES * STAGE + PARTS + PA_CONSUMERS * REST + q_tiles * Q_TILE;
+    }
 };
 
 // The key of eight that a fragment's row g stands for: such that a K
@@ -177,7 +185,7 @@ __device__ __forceinline__ PaWork pa_work(const fo_paged_attention_launch &a, in
     w.t0 = w.low / TILE;
     w.tiles = max((int)(((unsigned)w.s.len + TILE - 1) / TILE) - w.t0, 1);
     const int queries = w.s.n * a.group;
-    w.groups = queries <= a.queries ? queries > 0 : (queries + a.queries - 1) / a.queries;
+    w.groups = queries <= a.queries ? queries > 0 : (queries + FO_PAGED_QUERIES - 1) / FO_PAGED_QUERIES;
     return w;
 }
 
@@ -204,6 +212,14 @@ struct PaCursor {
     }
 };
 
+// Where a consumer warp is.  It waits in shared memory while the warp goes
+// through a segment's tiles, which want its registers.
+template <int TILE>
+struct PaPlace {
+    PaCursor<TILE> at;
+    int begin, per;
+};
+
 struct PaShared {
     uint64_t full[PA_STAGES], empty[PA_STAGES];
     uint64_t q_full, q_free;        // a segment's queries are there; have been taken
@@ -219,6 +235,7 @@ struct PaShared {
     int q_pos[FO_PAGED_QUERIES];
     int2 warp_sum[PA_THREADS / 32];
     int begin_base, begin_seq, abort;
+    int places[PA_CONSUMERS][12];  // a consumer warp's PaPlace
 };
 
 // Waits for the block's tile k in its slot; false when the block gave up.  The
@@ -569,7 +586,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     __shared__ PaShared sh;
     uint8_t *tiles = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(pa_smem) + 1023) & ~uintptr_t(1023));
     float *parts = reinterpret_cast<float *>(tiles + STAGES * Shape::STAGE);
-    uint2 *q_ops = reinterpret_cast<uint2 *>(tiles + STAGES * Shape::STAGE + Shape::PARTS);
+    uint32_t *rests = reinterpret_cast<uint32_t *>(tiles + STAGES * Shape::STAGE + Shape::PARTS);
+    uint2 *q_ops = reinterpret_cast<uint2 *>(tiles + STAGES * Shape::STAGE + Shape::PARTS + PA_CONSUMERS * Shape::REST);
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const int key_groups = PA_CONSUMERS / 2 / a.col_groups;
 
@@ -824,13 +842,21 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     const int page_shift = 31 - __clz(min(page, TILE) / 16);  // log2 of the m16 steps of a page's part of a tile
 
     const uint2 *q_from = q_ops + col_group * (Shape::Q_TILE / 8) + lane;
+    uint32_t *rest = rests + warp * (Shape::REST / 4) + lane;
+
+    PaPlace<TILE> *place = reinterpret_cast<PaPlace<TILE> *>(sh.places[warp]);
+    static_assert(sizeof(PaPlace<TILE>) == sizeof(sh.places[0]), "a place");
+    if (lane == 0) *place = {at, begin, per};
+    __syncwarp();
 
     for (int i = 0, segment = 0; i < count; segment++) {
-        const int n = min(at.left(), count - i);
-        const Sequence &s = at.w.s;
-        const int n_queries = min(s.n * a.group - at.group() * a.queries, a.queries);  // of this unit
-        const int p_first = s.len - s.n;  // positions of the sequence's first row and of its last
-        const int p_last = p_first + s.n - 1;
+        const PaCursor<TILE> here = place->at;
+        const int n = min(here.left(), count - i);
+        const int n_queries = min(here.w.s.n * a.group - here.group() * a.queries, a.queries);  // of this unit
+        const int len = here.w.s.len, low = here.w.low;
+        const int p_first = len - here.w.s.n;  // positions of the sequence's first row and of its last
+        const int p_last = p_first + here.w.s.n - 1;
+        const int tile0 = here.w.t0 + here.tile - i;
         // The queries as B operands.
         uint2 qf[Q_REGS ? QT * KQ : 1];
         float q_scale[2];  // of this lane's columns 2 t, 2 t + 1
@@ -858,10 +884,10 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         for (; k < i + n; k += key_groups) {
             const int slot = k % STAGES;
             // The first position of this warp's half.
-            const int pos0 = (at.w.t0 + at.tile + (k - i)) * TILE + half * HALF;
+            const int pos0 = (tile0 + k) * TILE + half * HALF;
             if (!pa_wait_tile(sh, slot, k, a.err)) return;
             // (Differences, since pos0 + HALF may be 2^31.)
-            if (col_group * 8 >= n_queries || pos0 > p_last || at.w.low - pos0 >= HALF) {
+            if (col_group * 8 >= n_queries || pos0 > p_last || low - pos0 >= HALF) {
                 // No row of this warp's sees any of it.
                 __syncwarp();
                 if (lane == 0) sm100::mbar_arrive(&sh.empty[slot]);
@@ -873,7 +899,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             if constexpr (!I8) {
                 // Rows beyond the sequence, or of pages that no row sees, may hold any
                 // bytes: an FP8 NaN times a probability of 0 would be NaN.
-                const int lo_row = max((at.w.low >> log_page << log_page) - pos0, 0), hi_row = min(s.len - pos0, HALF);
+                const int lo_row = max((low >> log_page << log_page) - pos0, 0), hi_row = min(len - pos0, HALF);
                 if (lo_row > 0 || hi_row < HALF) {
                     for (int x = lane; x < HALF * D / 16; x += 32) {
                         const int row = x / (D / 16);
@@ -994,34 +1020,83 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             // int8: [term][32 keys][16 of them], e4m3: [term][16 keys][8 of them].
             uint32_t pf[PT][STEPS * (I8 ? 1 : 2)];
             float sum0 = 0.0f, sum1 = 0.0f;
+            // int8: 2^23 + p times its largest integer holds that integer's bytes.
+            constexpr float TOP = F32 ? 8388607.0f : 65535.0f, BASE = 8388608.0f;
+            auto bytes = [&](int mt, const uint2 &lower, const uint2 &upper) {  // rows 0 .. 7 of the m16 step, 8 .. 15
+                const uint32_t lo0 = pa_transpose(__byte_perm(lower.x, lower.y, 0x5410));
+                const uint32_t lo1 = pa_transpose(__byte_perm(upper.x, upper.y, 0x5410));
+                pf[0][mt] = __byte_perm(lo0, lo1, 0x6420);
+                pf[1 % PT][mt] = __byte_perm(lo0, lo1, 0x7531);
+                if constexpr (F32)
+                    pf[PT - 1][mt] = __byte_perm(pa_transpose(__byte_perm(lower.x, lower.y, 0x7632)),
+                                                 pa_transpose(__byte_perm(upper.x, upper.y, 0x7632)), 0x6420);
+            };
+            auto probabilities = [&](int mt, int r) {
+                const float2 p = make_float2(sm100::ex2(c[mt][2 * r] - mx[0]), sm100::ex2(c[mt][2 * r + 1] - mx[1]));
+                sum0 += p.x;
+                sum1 += p.y;
+                return p;
+            };
+            if constexpr (!I8) {
 #pragma unroll
-            for (int mt = 0; mt < STEPS; mt++) {
-                uint32_t tr[2][2];  // int8: two terms each; of the keys of rows 0 .. 7, and of 8 .. 15
+                for (int mt = 0; mt < STEPS; mt++)
 #pragma unroll
-                for (int r = 0; r < 2; r++) {
-                    const float p0 = sm100::ex2(c[mt][2 * r] - mx[0]), p1 = sm100::ex2(c[mt][2 * r + 1] - mx[1]);
-                    sum0 += p0;
-                    sum1 += p1;
-                    if constexpr (I8) {
-                        // 2^23 + p times its largest integer: the bytes of that integer.
-                        constexpr float TOP = F32 ? 8388607.0f : 65535.0f;
-                        const uint32_t u0 = __float_as_uint(fmaf(p0, TOP, 8388608.0f));
-                        const uint32_t u1 = __float_as_uint(fmaf(p1, TOP, 8388608.0f));
-                        tr[0][r] = pa_transpose(__byte_perm(u0, u1, 0x5410));
-                        if constexpr (F32) tr[1][r] = pa_transpose(__byte_perm(u0, u1, 0x7632));
-                    } else {
-                        const uint32_t f = pa_f16x2(p0, p1);
+                    for (int r = 0; r < 2; r++) {
+                        const float2 p = probabilities(mt, r);
+                        const uint32_t f = pa_f16x2(p.x, p.y);
                         pf[0][2 * mt + r] = pa_transpose(f);
                         if constexpr (F32) {
                             const float2 b = f16x2_f32x2(f);
-                            pf[PT - 1][2 * mt + r] = pa_transpose(pa_f16x2(p0 - b.x, p1 - b.y));
+                            pf[PT - 1][2 * mt + r] = pa_transpose(pa_f16x2(p.x - b.x, p.y - b.y));
                         }
                     }
-                }
-                if constexpr (I8) {
+            } else {
 #pragma unroll
-                    for (int x = 0; x < PT; x++)
-                        pf[x][mt] = __byte_perm(tr[x / 2][0], tr[x / 2][1], x % 2 ? 0x7531 : 0x6420);
+                for (int mt = 0; mt < STEPS; mt++) {
+                    const float2 lower = probabilities(mt, 0), upper = probabilities(mt, 1);
+                    bytes(mt, make_uint2(__float_as_uint(fmaf(lower.x, TOP, BASE)), __float_as_uint(fmaf(lower.y, TOP, BASE))),
+                          make_uint2(__float_as_uint(fmaf(upper.x, TOP, BASE)), __float_as_uint(fmaf(upper.y, TOP, BASE))));
+                }
+            }
+            // A lane whose probabilities sum to less than 2^-8 has none of that size.
+            bool twice = false;
+            if constexpr (I8) {
+                constexpr float SMALL = 1.0f / 256.0f;
+                if (__any_sync(0xffffffffu, fminf(sum0, sum1) < SMALL)) {
+                    // Such lanes, among the eight of a query's that see any key.
+                    const uint32_t mine = 0x11111111u << t;
+                    auto few = [&](float sum) {
+                        const int see = __popc(__ballot_sync(0xffffffffu, sum > 0.0f) & mine);
+                        const int small = __popc(__ballot_sync(0xffffffffu, sum > 0.0f && sum < SMALL) & mine);
+                        return small > 0 && 2 * small >= see;
+                    };
+                    const bool few0 = few(sum0), few1 = few(sum1);
+                    twice = __any_sync(0xffffffffu, few0 || few1);
+                    if (twice) {
+                        // Again, rounded down; what that leaves, as another integer of as
+                        // many bits, waits in shared memory for the products of the first.
+                        auto whole = [&](const float2 &p) {
+                            return make_uint2(__float_as_uint(__fmaf_rd(p.x, TOP, BASE)),
+                                              __float_as_uint(__fmaf_rd(p.y, TOP, BASE)));
+                        };
+                        auto left = [&](const float2 &p, const uint2 &u) {
+                            const float x = fmaf(p.x, TOP, BASE - __uint_as_float(u.x));
+                            const float y = fmaf(p.y, TOP, BASE - __uint_as_float(u.y));
+                            return make_uint2(__float_as_uint(fmaf(x, TOP, BASE)), __float_as_uint(fmaf(y, TOP, BASE)));
+                        };
+                        const float keep0 = sum0, keep1 = sum1;
+#pragma unroll
+                        for (int mt = 0; mt < STEPS; mt++) {
+                            const float2 lower = probabilities(mt, 0), upper = probabilities(mt, 1);
+                            const uint2 u0 = whole(lower), u1 = whole(upper);
+                            bytes(mt, left(lower, u0), left(upper, u1));
+#pragma unroll
+                            for (int x = 0; x < PT; x++) rest[32 * (x * STEPS + mt)] = pf[x][mt];
+                            bytes(mt, u0, u1);
+                        }
+                        sum0 = keep0;
+                        sum1 = keep1;
+                    }
                 }
             }
             l[0] = fmaf(sum0, beta[0], l[0] * alpha[0]);
@@ -1035,10 +1110,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             // O^T: rows = dimensions, columns = queries; two m16 tiles of dimensions
             // at a time, each page's sum times its scale: the products over one
             // page's keys, the steps [from, to) of 16; WHOLE: all of the half's.
-            constexpr float PART = I8 ? (F32 ? 1.0f / 8388607.0f : 1.0f / 65535.0f) : 1.0f;
             auto page_sum = [&](auto whole, int from, int to, float scale) {
                 constexpr bool WHOLE = decltype(whole)::value;
-                const float f0 = scale * PART * beta[0], f1 = scale * PART * beta[1];
+                const float f0 = scale * beta[0], f1 = scale * beta[1];
                 constexpr int A = I8 ? PT : 1;
 #pragma unroll
                 for (int d2 = 0; d2 < MT; d2 += 2) {
@@ -1098,14 +1172,22 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                         }
                 }
             };
-            if ((1 << page_shift) >= STEPS) {
-                page_sum(std::true_type{}, 0, STEPS, vs[0]);
-            } else if (page_shift == 1) {
+            for (bool again = twice;; again = false) {
+                if constexpr (I8) beta[0] *= 1.0f / TOP, beta[1] *= 1.0f / TOP;
+                if ((1 << page_shift) >= STEPS) {
+                    page_sum(std::true_type{}, 0, STEPS, vs[0]);
+                } else if (page_shift == 1) {
 #pragma unroll
-                for (int from = 0; from < STEPS; from += 2) page_sum(std::false_type{}, from, from + 2, vs[from]);
-            } else {
+                    for (int from = 0; from < STEPS; from += 2) page_sum(std::false_type{}, from, from + 2, vs[from]);
+                } else {
 #pragma unroll
-                for (int from = 0; from < STEPS; from++) page_sum(std::false_type{}, from, from + 1, vs[from]);
+                    for (int from = 0; from < STEPS; from++) page_sum(std::false_type{}, from, from + 1, vs[from]);
+                }
+                if (!I8 || !again) break;
+#pragma unroll
+                for (int x = 0; x < PT; x++)
+#pragma unroll
+                    for (int mt = 0; mt < STEPS; mt++) pf[x][mt] = rest[32 * (x * STEPS + mt)];
             }
         }
 
@@ -1138,14 +1220,19 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         }
         __syncwarp();
         if (lane == 0) sm100::mbar_arrive(&sh.part_full);
-        if (i + n == count && !(at.tile == 0 && n == at.w.tiles)) {
+        PaPlace<TILE> was = *place;
+        if (i + n == count && !(was.at.tile == 0 && n == was.at.w.tiles)) {
             if (!sm100::mbar_wait(&sh.shared_go[1], 0, &sh.abort, a.err)) return;
             if (sh.joins[1])
-                pa_join_blocks<D, F32>(a, pa_unit(a, at, begin + i, n, per), PA_EPILOGUES + warp,
+                pa_join_blocks<D, F32>(a, pa_unit(a, was.at, was.begin + i, n, was.per), PA_EPILOGUES + warp,
                                        PA_EPILOGUES + PA_CONSUMERS);
         }
         i += n;
-        at.advance(a, n);
+        if (i >= count) break;
+        was.at.advance(a, n);
+        __syncwarp();
+        if (lane == 0) place->at = was.at;
+        __syncwarp();
     }
 }
 

@@ -961,6 +961,42 @@ def test_attention_queries_with_one_large_element(dim, dtype):
         assert within(out[0].double().cpu().numpy(), o, bound, dtype)
 
 
+@pytest.mark.parametrize("nats", [2.0, 5.0, 8.0, 12.0, 15.0])
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+def test_attention_large_weights_with_small_values(nats, dtype, fmt):
+    """Keys that take nearly all of the softmax and whose values are zero (as a text's first tokens often do): what is
+    left of the output is the other keys', and their probabilities have to be exact to their own size.  Each
+    probability keeps 8 bits with BF16 rows (a relative 2^-9 and, where all keys of a group are like one another, at
+    most twice that) and 15 with FP32 rows; a score is off by d at most, which moves a probability and the sum by e^d
+    each; FP32 sums add 2^-18."""
+    rng = np.random.default_rng(48)
+    kept = 2.0 ** (-8 if dtype == "bf16" else -15 if fmt == "i8" else -13)
+    for dim, n, large in ((64, 2, 1), (128, 3, 1), (64, 7, 2), (64, 60, 1), (64, 64, 4), (64, 2000, 1), (128, 30, 1),
+                          (128, 777, 4)):
+        cache = Cache(rng, fmt, dim, 64, 1, [n])
+        pages = cache.table[0, :-(-n // 64)]
+        sign = np.where(rng.standard_normal(dim) < 0, -1.0, 1.0)
+        q = torch.from_numpy((sign * rng.uniform(0.5, 1.5, (1, 2, dim))).astype(np.float32)).to(DTYPES[dtype]).cuda()
+        qv = q.double().cpu().numpy()
+        # Keys near zero, but for the first ones, whose scores are `nats` above with the first query.
+        unit = nats / (127.0 * dim ** -0.5 * np.abs(qv[0, 0]).sum())
+        small = R.encode(rng.integers(-12, 13, cache.codes[0].shape).astype(np.float32), fmt)
+        cache.codes[0][:] = small
+        cache.codes[0][pages[0], :, :large] = R.encode((127.0 if fmt == "i8" else 128.0) * sign.astype(np.float32), fmt)
+        cache.codes[1][pages[0], :, :large] = 0
+        cache.scales[0][pages] = np.float32(unit)
+        out, lse = torch.empty_like(q), torch.empty(1, 2, device="cuda")
+        F.paged_attention(cache.on_device(), cache.batch([1], False), q, out, lse=lse)
+        k, v = cache.values(0, 0), cache.values(1, 0)
+        o, z, size = R.attend(qv[0], k, v, n - 1, 0, None, dim ** -0.5)
+        sizes, _, _ = R.attend(qv[0], k, np.abs(v), n - 1, 0, None, dim ** -0.5)
+        d = 2.0 ** -17 * size
+        bound = (2 * (math.exp(d) - 1) + kept + 2.0 ** -18) * sizes
+        assert within(out[0].double().cpu().numpy(), o, bound, dtype)
+        assert (np.abs(lse[0].double().cpu().numpy() - z) <= d + 2.0 ** -20 * (1 + np.abs(z))).all()
+
+
 def test_attention_from_a_thread_without_cuda_calls_before_it():
     """A server's worker thread, whose first CUDA call of any kind is an attention on a context that others made."""
     import threading
