@@ -1021,3 +1021,37 @@ def test_attention_from_a_thread_without_cuda_calls_before_it():
     ctx.synchronize()
     assert not failures and torch.equal(out, expected)
     ctx.close()
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+def test_offsets_beyond_32_bits_bit_for_bit(fmt):
+    """A pool of more than 2^32 bytes: rows appended to its last pages are there, code for code, nothing is anywhere
+    else, and the attention over them is as exact as over any."""
+    page, kv_heads, dim, held = 128, 8, 128, 300
+    pages = (1 << 32) // (page * kv_heads * dim) + 40
+    kind = torch.int8 if fmt == "i8" else torch.float8_e4m3fn
+    codes = [torch.zeros(pages, kv_heads, page, dim, dtype=torch.int8, device="cuda") for _ in range(2)]
+    scales = [torch.zeros(pages, kv_heads, device="cuda") for _ in range(2)]
+    kv = F.PagedKv(*(c.view(kind) for c in codes), *scales)
+    ids = np.arange(pages - 1, pages - 4, -1, dtype=np.int32)
+    rng = np.random.default_rng(49)
+    k, kx = rows_of(rng, held, kv_heads, dim, "f32")
+    v, vx = rows_of(rng, held, kv_heads, dim, "f32")
+    F.paged_append(kv, F.PagedBatch(dev(ids[None]), dev(np.array([held], np.int32)), rows=held), k, v)
+    F.paged_append(kv, F.PagedBatch(dev(ids[None]), dev(np.array([held + 1], np.int32))), k[:1], v[:1])  # one row more
+    values = []
+    for i, x in enumerate((kx, vx)):
+        c, s = np.zeros((3, kv_heads, page, dim), np.uint8), np.zeros((3, kv_heads), np.float32)
+        R.append(c, s, x.astype(np.float32), [held], [held], np.array([[0, 1, 2]]), fmt)
+        R.append(c, s, x[:1].astype(np.float32), [1], [held + 1], np.array([[0, 1, 2]]), fmt)
+        assert np.array_equal(codes[i][ids.astype(np.int64)].view(torch.uint8).cpu().numpy(), c)
+        assert np.array_equal(scales[i][ids.astype(np.int64)].cpu().numpy(), s)
+        assert not codes[i][:pages - 3].any() and not scales[i][:pages - 3].any()
+        values.append((R.decode(c, fmt) * s[..., None, None].astype(np.float64)).transpose(1, 0, 2, 3).reshape(
+            kv_heads, -1, dim)[:, :held + 1])
+    q, qv = rows_of(rng, 1, kv_heads, dim, "f32")
+    out = torch.empty(1, kv_heads, dim, device="cuda")
+    F.paged_attention(kv, F.PagedBatch(dev(ids[None]), dev(np.array([held + 1], np.int32))), q, out)
+    o, _, size = R.attend(qv[0], *values, held, 0, None, dim ** -0.5)
+    bound = (4 * 2.0 ** -17 * size + 2.0 ** -18) * np.abs(values[1]).max()
+    assert within(out[0].double().cpu().numpy(), o, bound, "f32")
