@@ -25,7 +25,9 @@
 // with the queries in a launch of their own); 24 ragged prompts of 49,000 rows,
 // 8 heads of 128 and 32 of queries, BF16, 270 us (4.3 TB/s; the queries' launch
 // alone, profiled, 134 us at 6.0).  A thread for each 16 values keeps them
-// between the maximum and the codes.  Before heads shared a read of the
+// between the maximum and the codes; at the 64 registers that this leaves, every
+// variant spills some (172 to 322 bytes of stores), which is part of those
+// instructions.  Before heads shared a read of the
 // rotation's table, and with a division for each code, the prompts took 505 us.
 #include "paged_rope.cuh"
 
@@ -465,9 +467,9 @@ cudaError_t launch_append(const fo_append_launch &in, cudaStream_t stream) {
     auto blocks = [&](int64_t h) { return segments * 2 * ((a.kv.n_kv_heads + h - 1) / h); };
     while (heads > threads / team && blocks(heads) < 296) heads = (heads + 1) / 2;
     // The queries' blocks go along with tasks' blocks of their own size (a 6,544-row
-    // FP32 page in 64-position pages: 28.5 us apart, 23.3 together); next to wider
-    // ones they would run at half their occupancy (24 ragged prompts: 281 us apart,
-    // 334 together).
+    // FP32 page in 64-position pages: 28.5 us apart, 23.3 together, 21.4 now); next
+    // to wider ones they would run at half their occupancy (24 ragged prompts: 281 us
+    // apart, 334 together, 270 apart now).
     const bool together = threads == ROPE_THREADS;
     const int64_t grid = blocks(heads) + (together ? q_blocks : 0);
     if (grid > 0x7FFFFFFF) return cudaErrorInvalidValue;

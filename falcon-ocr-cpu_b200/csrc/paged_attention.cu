@@ -58,16 +58,16 @@
 // Maxima, sums and outputs are FP32.
 //
 // Measured (CUDA graph): 64 sequences of 6,545 to 8,592 positions, 2 queries to
-// each of 8 KV heads of 64, int8: 87 us, 5.7 TB/s, 0.88 of the measured copy
+// each of 8 KV heads of 64, int8: 86 us, 5.7 TB/s, 0.89 of the measured copy
 // bandwidth; 16 of 1,000 to 32,768, 4 queries, heads of 128, e4m3: 112 us, 6.0
 // TB/s.  Earlier forms, 64 sequences of 7,500 in a stream of calls: one
 // producer warp 165 us; four, with int8 converted to FP16 for m16n8k16 products,
 // 110; products of the codes themselves, parts joined by the consumers, 103; by
 // epilogue warps, 95.  With 40 queries to a KV head (10 of the 12 consumer warps
-// at one tile): 304 us for 48 sequences in a window of 4,096, 1.2 TB/s; a tile took
-// some 6,600 warp instructions with 16-bit queries, at 36 % of the issue slots with
-// the integer tensor pipe at 14 %.  A call of one short sequence takes 9.6 us, a
-// chain of launch, length, page number, tile and join.
+// at one tile) a tile takes some 7,200 warp instructions, at 36 % of the issue slots
+// with the tensor pipe at 13 %: 304 us for 48 sequences in a window of 4,096, 1.2
+// TB/s.  A call of one short sequence takes 9.7 us, a chain of launch, length, page
+// number, tile and join.  Spills: 0 to 88 bytes of stores in a variant.
 #include "paged.cuh"
 #include "sm100.cuh"
 

@@ -581,8 +581,19 @@ int fo_paged_append(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch *ba
  * s_j = scale * q . k_j: out = sum_j exp(s_j) v_j / (sum_j exp(s_j) +
  * exp(sinks[head])), sinks NULL: without that term; lse (NULL: not wanted)
  * [total_rows][n_heads] = ln sum_j exp(s_j).  A row that sees nothing gives 0
- * and -infinity.  max_rows is at most 64, and the page tables' 8 KB tiles of
- * keys, of all KV heads and for every 48 query rows of one, are at most 2^31
+ * and -infinity, whatever q holds there; a row that sees something and whose
+ * q is not finite gives NaN.
+ *
+ * Codes are exact; scores, maxima, sums and outputs are FP32.  An element of
+ * q is held to 2^-22 of the largest of its row and head.  A probability is
+ * held, over int8 codes, to 2^-17 (BF16 rows) or 2^-24 (FP32 rows) of the
+ * largest among the 64 (head_dim 64) or 32 positions that it is computed
+ * with, and where few of those dominate to 8 or 15 bits of its own; over e4m3
+ * codes to 11 (BF16) or 22 (FP32) bits of its own, no finer than 2^-35 of that
+ * largest.  The sum of probabilities has no such rounding.
+ *
+ * max_rows is at most 64, and the page tables' 8 KB tiles of keys, of all KV
+ * heads and for every 48 query rows of one, are at most 2^31
  * (FO_ERR_CAPACITY). */
 int fo_paged_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch *batch, const fo_rows *q,
                        const float *sinks, float scale, int64_t window, const fo_rows *out, float *lse);
