@@ -182,6 +182,13 @@ struct fo_ctx {
     std::mutex paged_mutex;
     DevBuf paged_parts;
     int sms = 0;
+    // Attention of many query rows: parts and joins, of one size, made by the first
+    // such call; and rows that wait to be joined, which grow (what captured graphs
+    // use is kept).
+    DevBuf tile_parts;
+    std::vector<DevBuf> waiting;
+    float *tile_part_ml() const { return (float *)tile_parts.ptr + (size_t)2 * sms * FO_TILES_QUERIES * 128; }
+    int32_t *tile_joins() const { return (int32_t *)(tile_part_ml() + (size_t)2 * sms * FO_TILES_QUERIES * 2); }
     size_t paged_part_rows() const { return (size_t)2 * sms * FO_PAGED_QUERIES; }
     float *paged_part_ml() const { return (float *)paged_parts.ptr + paged_part_rows() * 128; }
     unsigned *paged_counters() const { return (unsigned *)(paged_part_ml() + paged_part_rows() * 2); }
@@ -540,6 +547,8 @@ int fo_ctx_destroy(fo_ctx *ctx) {
     ctx->i8_pages.release();
     ctx->host_i8_pages.release();
     ctx->paged_parts.release();
+    ctx->tile_parts.release();
+    for (auto &b : ctx->waiting) b.release();
     if (ctx->flags) cudaFree(ctx->flags);
     if (ctx->dev_err) cudaFree(ctx->dev_err);
     if (ctx->ev0) cudaEventDestroy(ctx->ev0);
@@ -1823,6 +1832,215 @@ int make_paged_parts(fo_ctx *ctx) {
     return FO_OK;
 }
 
+// The scratch of a context's attentions of many query rows, at the first of
+// them (after make_paged_parts).
+int make_tile_parts(fo_ctx *ctx) {
+    std::lock_guard<std::mutex> lock(ctx->paged_mutex);
+    if (ctx->tile_parts.ptr) return FO_OK;
+    FO_TRY(refuse_capture(ctx->stream, "a context's first attention of many query rows makes its scratch and"));
+    const size_t rows = (size_t)2 * ctx->sms * FO_TILES_QUERIES;
+    FO_CUDA(ctx->tile_parts.ensure(rows * (128 + 2) * 4 + (size_t)ctx->sms * 32), "cudaMalloc(attention parts)");
+    return FO_OK;
+}
+
+// Room for `rows` rows of `dim` that wait to be joined: sums, then {maximum, sum}.
+int make_waiting(fo_ctx *ctx, int64_t rows, int64_t dim, float **o, float **ml) {
+    std::lock_guard<std::mutex> lock(ctx->paged_mutex);
+    const size_t need = (size_t)rows * (size_t)(dim + 2) * 4;
+    if (ctx->waiting.empty() || ctx->waiting.back().bytes < need) {
+        FO_TRY(refuse_capture(ctx->stream, "an attention of shared beginnings that needs more scratch than any before"));
+        // Twice the last one at least, so that all of them are at most twice the largest.
+        DevBuf b;
+        const size_t twice = ctx->waiting.empty() ? (size_t)1 << 20 : 2 * ctx->waiting.back().bytes;
+        FO_CUDA(b.ensure(std::max(need, twice)), "cudaMalloc(rows that wait to be joined)");
+        ctx->waiting.push_back(b);
+    }
+    *o = (float *)ctx->waiting.back().ptr;
+    *ml = *o + rows * dim;
+    return FO_OK;
+}
+
+// The axes of a rotation as the kernels take them.
+int check_axes(const fo_rope_axes *r, int64_t head_dim, int64_t rows, fo_rope_spec *spec, fo_axes_launch *axes) {
+    if (!r) return fail(FO_ERR_INVALID, "rope: null axes");
+    *spec = {r->table, r->positions, r->row_positions, r->rot_dim, r->layout};
+    FO_TRY(check_rope(spec, head_dim));
+    if (r->rot_dim > 256) return fail(FO_ERR_INVALID, "rope: rot_dim must be at most 256");
+    if (r->n_axes < 1 || r->n_axes > FO_ROPE_MAX_AXES)
+        return fail(FO_ERR_INVALID, "rope: 1 to %d axes", FO_ROPE_MAX_AXES);
+    if (!r->row_positions && rows > 0) return fail(FO_ERR_INVALID, "rope: positions on several axes must be given");
+    *axes = {};
+    axes->positions = r->row_positions;
+    axes->row_stride = r->row_stride;
+    axes->axis_stride = r->axis_stride;
+    for (int i = 0; i < r->rot_dim / 2; i++) {
+        if (r->pair_axis[i] >= r->n_axes) return fail(FO_ERR_INVALID, "rope: pair %d has axis %d of %d", i, r->pair_axis[i], r->n_axes);
+        axes->used |= 1u << r->pair_axis[i];
+        axes->pair_axis[i >> 4] |= (uint32_t)r->pair_axis[i] << (2 * (i & 15));
+    }
+    return FO_OK;
+}
+
+// fo_rope, by one position a row or on axes.
+int rope_rows(fo_ctx *ctx, const fo_rows *x, const fo_rows *out, int64_t rows, int32_t head_dim, const fo_rope_spec *rope,
+              const fo_rope_axes *by_axes, int32_t transpose) {
+    if (rows < 0 || rows > INT32_MAX) return fail(FO_ERR_INVALID, "fo_rope: rows must be 0..2^31 - 1");
+    if (head_dim < 2 || head_dim > 256) return fail(FO_ERR_INVALID, "fo_rope: head_dim must be 2..256");
+    FO_TRY(check_rows(x, "fo_rope x", rows, head_dim, false));
+    FO_TRY(check_rows(out, "fo_rope out", rows, head_dim, true));
+    if (x->heads != out->heads || x->dtype != out->dtype)
+        return fail(FO_ERR_INVALID, "fo_rope: x and out must have one type and as many heads");
+    fo_rope_launch a = {};
+    if (by_axes) {
+        FO_TRY(check_axes(by_axes, head_dim, rows, &a.rope, &a.axes));
+    } else {
+        FO_TRY(check_rope(rope, head_dim));
+        a.rope = *rope;
+    }
+    const bool in_place = x->data == out->data;
+    if (in_place && (x->row_stride != out->row_stride || x->head_stride != out->head_stride))
+        return fail(FO_ERR_INVALID, "fo_rope: in place, x and out must be laid out alike");
+    if (!ctx) return fail(FO_ERR_INVALID, "null context");
+    DeviceGuard guard(ctx->device);
+    a.x = *x;
+    a.out = *out;
+    a.rows = rows;
+    a.err = ctx->dev_err;
+    a.head_dim = head_dim;
+    a.transpose = transpose != 0;
+    a.in_place = in_place;
+    cudaError_t e = fo_launch_rope(&a, ctx->stream);
+    return e == cudaSuccess ? FO_OK : cuda_fail(e, "rope launch");
+}
+
+// fo_paged_append, by one position a row or on axes.
+int append_rows(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch *batch, const fo_rows *k, const fo_rows *v,
+                const fo_rows *q, const fo_rows *q_out, const fo_rope_spec *rope, const fo_rope_axes *by_axes) {
+    FO_TRY(check_paged(kv, batch));
+    const int64_t rows = batch->total_rows;
+    FO_TRY(check_rows(k, "fo_paged_append k", rows, kv->head_dim, false));
+    FO_TRY(check_rows(v, "fo_paged_append v", rows, kv->head_dim, false));
+    if (k->heads != kv->n_kv_heads || v->heads != kv->n_kv_heads)
+        return fail(FO_ERR_INVALID, "fo_paged_append: k and v must have the cache's heads");
+    if (k->dtype != v->dtype) return fail(FO_ERR_INVALID, "fo_paged_append: k and v must have one type");
+    fo_append_launch a = {};
+    if (by_axes) {
+        FO_TRY(check_axes(by_axes, kv->head_dim, rows, &a.rope, &a.axes));
+        a.rotate = 1;
+    } else if (rope) {
+        FO_TRY(check_rope(rope, kv->head_dim));
+        a.rope = *rope;
+        a.rotate = 1;
+    }
+    if ((q != nullptr) != (q_out != nullptr)) return fail(FO_ERR_INVALID, "fo_paged_append: q needs q_out");
+    bool in_place = false;
+    if (q) {
+        if (!a.rotate) return fail(FO_ERR_INVALID, "fo_paged_append: queries are taken to be rotated, without rope there is nothing to do");
+        FO_TRY(check_rows(q, "fo_paged_append q", rows, kv->head_dim, false));
+        FO_TRY(check_rows(q_out, "fo_paged_append q_out", rows, kv->head_dim, true));
+        if (q->heads != q_out->heads || q->dtype != q_out->dtype || q->dtype != k->dtype)
+            return fail(FO_ERR_INVALID, "fo_paged_append: q and q_out must have one type, the keys', and as many heads");
+        in_place = q->data == q_out->data;
+        if (in_place && (q->row_stride != q_out->row_stride || q->head_stride != q_out->head_stride))
+            return fail(FO_ERR_INVALID, "fo_paged_append: in place, q and q_out must be laid out alike");
+    }
+    if (!ctx) return fail(FO_ERR_INVALID, "null context");
+    if (rows == 0) return FO_OK;
+    DeviceGuard guard(ctx->device);
+    a.kv = *kv;
+    a.batch = *batch;
+    a.k = *k;
+    a.v = *v;
+    a.err = ctx->dev_err;
+    if (q) {
+        a.q.x = *q;
+        a.q.out = *q_out;
+        a.q.rows = rows;
+        a.q.rope = a.rope;
+        a.q.axes = a.axes;
+        a.q.err = ctx->dev_err;
+        a.q.head_dim = kv->head_dim;
+        a.q.in_place = in_place;
+    }
+    cudaError_t e = by_axes ? fo_launch_paged_append_axes(&a, ctx->stream) : fo_launch_paged_append(&a, ctx->stream);
+    return e == cudaSuccess ? FO_OK : cuda_fail(e, "paged append launch");
+}
+
+// What all paged attentions ask of their arguments.
+int check_attention(const char *name, const fo_paged_kv *kv, const fo_paged_batch *batch, const fo_rows *q,
+                    const fo_rows *out, const float *sinks, float scale, int64_t window, const float *lse) {
+    FO_TRY(check_paged(kv, batch));
+    const int64_t rows = batch->total_rows;
+    if (!q || (!q->data && rows > 0) || !out || (!out->data && rows > 0)) return fail(FO_ERR_INVALID, "%s: null pointer", name);
+    FO_TRY(check_rows(q, "paged attention q", rows, kv->head_dim, false));
+    FO_TRY(check_rows(out, "paged attention out", rows, kv->head_dim, true));
+    if (q->heads != out->heads || q->dtype != out->dtype)
+        return fail(FO_ERR_INVALID, "%s: q and out must have one type and as many heads", name);
+    if (q->heads % kv->n_kv_heads != 0 || q->heads > 65535)
+        return fail(FO_ERR_INVALID, "%s: query heads must be a multiple of the KV heads", name);
+    if (!std::isfinite(scale)) return fail(FO_ERR_INVALID, "%s: scale must be finite", name);
+    if (window < 0) return fail(FO_ERR_INVALID, "%s: negative window", name);
+    if (!aligned4(sinks) || !aligned4(lse)) return fail(FO_ERR_INVALID, "%s: misaligned sinks or lse", name);
+    return FO_OK;
+}
+
+// The kernels number query rows and the tables' 8 KB tiles of keys, for every 48
+// query rows of a KV head, in 32 bits; `wide` query rows of a KV head in all, of
+// at most `units` sequences or groups.
+int check_tiles(const char *name, const fo_paged_kv *kv, const fo_paged_batch *batch, double wide, double units) {
+    const double tiles = kv->n_kv_heads * (wide / FO_PAGED_QUERIES + units) *
+                         ((double)batch->table_stride * kv->page_size * kv->head_dim / 8192 + 2);
+    if (wide > INT32_MAX) return fail(FO_ERR_CAPACITY, "%s: more than 2^31 query rows of a KV head", name);
+    if (tiles > INT32_MAX)
+        return fail(FO_ERR_CAPACITY, "%s: the batch's page tables have room for more than 2^31 tiles", name);
+    return FO_OK;
+}
+
+// One launch of a paged attention with a reach: few query rows of a KV head by
+// the one kernel, many by the other.
+int launch_reach(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch *batch, const fo_rows *q, const fo_rows *out,
+                 const float *sinks, float *lse, float scale, int32_t window, const fo_paged_reach &reach, bool few) {
+    FO_TRY(make_paged_parts(ctx));
+    cudaError_t e;
+    if (few) {
+        fo_paged_attention_launch a = {};
+        a.kv = *kv;
+        a.batch = *batch;
+        a.q = *q;
+        a.out = *out;
+        a.sinks = sinks;
+        a.lse = lse;
+        a.scale = scale;
+        a.window = window;
+        a.err = ctx->dev_err;
+        a.part_o = (float *)ctx->paged_parts.ptr;
+        a.part_ml = ctx->paged_part_ml();
+        a.counters = ctx->paged_counters();
+        a.reach = reach;
+        const bool plain = reach.n_groups == 0 && (reach.first == 0 || window == 0);
+        e = plain ? fo_launch_paged_attention(&a, ctx->sms, ctx->stream)
+                  : fo_launch_paged_attention_reach(&a, ctx->sms, ctx->stream);
+    } else {
+        FO_TRY(make_tile_parts(ctx));
+        fo_paged_tiles_launch a = {};
+        a.kv = *kv;
+        a.batch = *batch;
+        a.q = *q;
+        a.out = *out;
+        a.sinks = sinks;
+        a.lse = lse;
+        a.scale = scale;
+        a.window = window;
+        a.reach = reach;
+        a.err = ctx->dev_err;
+        a.part_o = (float *)ctx->tile_parts.ptr;
+        a.part_ml = ctx->tile_part_ml();
+        a.joins = ctx->tile_joins();
+        e = fo_launch_paged_tiles(&a, ctx->sms, ctx->stream);
+    }
+    return e == cudaSuccess ? FO_OK : cuda_fail(e, "paged attention launch");
+}
+
 }  // namespace
 
 int fo_rope_table(fo_ctx *ctx, float *table, int64_t positions, int32_t rot_dim, fo_rope_scaling s) {
@@ -1848,77 +2066,24 @@ int fo_rope_table(fo_ctx *ctx, float *table, int64_t positions, int32_t rot_dim,
 
 int fo_rope(fo_ctx *ctx, const fo_rows *x, const fo_rows *out, int64_t rows, int32_t head_dim,
             const fo_rope_spec *rope, int32_t transpose) {
-    if (rows < 0 || rows > INT32_MAX) return fail(FO_ERR_INVALID, "fo_rope: rows must be 0..2^31 - 1");
-    if (head_dim < 2 || head_dim > 256) return fail(FO_ERR_INVALID, "fo_rope: head_dim must be 2..256");
-    FO_TRY(check_rows(x, "fo_rope x", rows, head_dim, false));
-    FO_TRY(check_rows(out, "fo_rope out", rows, head_dim, true));
-    if (x->heads != out->heads || x->dtype != out->dtype)
-        return fail(FO_ERR_INVALID, "fo_rope: x and out must have one type and as many heads");
-    FO_TRY(check_rope(rope, head_dim));
-    const bool in_place = x->data == out->data;
-    if (in_place && (x->row_stride != out->row_stride || x->head_stride != out->head_stride))
-        return fail(FO_ERR_INVALID, "fo_rope: in place, x and out must be laid out alike");
-    if (!ctx) return fail(FO_ERR_INVALID, "null context");
-    DeviceGuard guard(ctx->device);
-    fo_rope_launch a = {};
-    a.x = *x;
-    a.out = *out;
-    a.rows = rows;
-    a.rope = *rope;
-    a.err = ctx->dev_err;
-    a.head_dim = head_dim;
-    a.transpose = transpose != 0;
-    a.in_place = in_place;
-    cudaError_t e = fo_launch_rope(&a, ctx->stream);
-    return e == cudaSuccess ? FO_OK : cuda_fail(e, "rope launch");
+    return rope_rows(ctx, x, out, rows, head_dim, rope, nullptr, transpose);
+}
+
+int fo_rope_by_axes(fo_ctx *ctx, const fo_rows *x, const fo_rows *out, int64_t rows, int32_t head_dim,
+                    const fo_rope_axes *rope, int32_t transpose) {
+    if (!rope) return fail(FO_ERR_INVALID, "rope: null axes");
+    return rope_rows(ctx, x, out, rows, head_dim, nullptr, rope, transpose);
 }
 
 int fo_paged_append(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch *batch, const fo_rows *k,
                     const fo_rows *v, const fo_rows *q, const fo_rows *q_out, const fo_rope_spec *rope) {
-    FO_TRY(check_paged(kv, batch));
-    const int64_t rows = batch->total_rows;
-    FO_TRY(check_rows(k, "fo_paged_append k", rows, kv->head_dim, false));
-    FO_TRY(check_rows(v, "fo_paged_append v", rows, kv->head_dim, false));
-    if (k->heads != kv->n_kv_heads || v->heads != kv->n_kv_heads)
-        return fail(FO_ERR_INVALID, "fo_paged_append: k and v must have the cache's heads");
-    if (k->dtype != v->dtype) return fail(FO_ERR_INVALID, "fo_paged_append: k and v must have one type");
-    if (rope) FO_TRY(check_rope(rope, kv->head_dim));
-    if ((q != nullptr) != (q_out != nullptr)) return fail(FO_ERR_INVALID, "fo_paged_append: q needs q_out");
-    bool in_place = false;
-    if (q) {
-        if (!rope) return fail(FO_ERR_INVALID, "fo_paged_append: queries are taken to be rotated, without rope there is nothing to do");
-        FO_TRY(check_rows(q, "fo_paged_append q", rows, kv->head_dim, false));
-        FO_TRY(check_rows(q_out, "fo_paged_append q_out", rows, kv->head_dim, true));
-        if (q->heads != q_out->heads || q->dtype != q_out->dtype || q->dtype != k->dtype)
-            return fail(FO_ERR_INVALID, "fo_paged_append: q and q_out must have one type, the keys', and as many heads");
-        in_place = q->data == q_out->data;
-        if (in_place && (q->row_stride != q_out->row_stride || q->head_stride != q_out->head_stride))
-            return fail(FO_ERR_INVALID, "fo_paged_append: in place, q and q_out must be laid out alike");
-    }
-    if (!ctx) return fail(FO_ERR_INVALID, "null context");
-    if (rows == 0) return FO_OK;
-    DeviceGuard guard(ctx->device);
-    fo_append_launch a = {};
-    a.kv = *kv;
-    a.batch = *batch;
-    a.k = *k;
-    a.v = *v;
-    a.err = ctx->dev_err;
-    if (rope) {
-        a.rope = *rope;
-        a.rotate = 1;
-    }
-    if (q) {
-        a.q.x = *q;
-        a.q.out = *q_out;
-        a.q.rows = rows;
-        a.q.rope = *rope;
-        a.q.err = ctx->dev_err;
-        a.q.head_dim = kv->head_dim;
-        a.q.in_place = in_place;
-    }
-    cudaError_t e = fo_launch_paged_append(&a, ctx->stream);
-    return e == cudaSuccess ? FO_OK : cuda_fail(e, "paged append launch");
+    return append_rows(ctx, kv, batch, k, v, q, q_out, rope, nullptr);
+}
+
+int fo_paged_append_by_axes(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch *batch, const fo_rows *k,
+                            const fo_rows *v, const fo_rows *q, const fo_rows *q_out, const fo_rope_axes *rope) {
+    if (!rope) return fail(FO_ERR_INVALID, "rope: null axes");
+    return append_rows(ctx, kv, batch, k, v, q, q_out, nullptr, rope);
 }
 
 int fo_paged_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch *batch, const fo_rows *q,
@@ -1962,6 +2127,63 @@ int fo_paged_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch 
     a.counters = ctx->paged_counters();
     cudaError_t e = fo_launch_paged_attention(&a, ctx->sms, ctx->stream);
     return e == cudaSuccess ? FO_OK : cuda_fail(e, "paged attention launch");
+}
+
+int fo_paged_window_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch *batch, const fo_rows *q,
+                              const float *sinks, float scale, int64_t window, int64_t first, const fo_rows *out,
+                              float *lse) {
+    const char *name = "fo_paged_window_attention";
+    FO_TRY(check_attention(name, kv, batch, q, out, sinks, scale, window, lse));
+    if (first < 0) return fail(FO_ERR_INVALID, "%s: negative number of first positions", name);
+    const int64_t group = q->heads / kv->n_kv_heads;
+    if (batch->max_rows * group > INT32_MAX) return fail(FO_ERR_CAPACITY, "%s: more than 2^31 query rows of a KV head", name);
+    FO_TRY(check_tiles(name, kv, batch, (double)batch->total_rows * group, (double)batch->n_seqs));
+    if (!ctx) return fail(FO_ERR_INVALID, "null context");
+    if (batch->total_rows == 0) return FO_OK;
+    DeviceGuard guard(ctx->device);
+    fo_paged_reach reach = {};
+    reach.first = (int32_t)std::min<int64_t>(first, INT32_MAX);
+    return launch_reach(ctx, kv, batch, q, out, sinks, lse, scale, window < INT32_MAX ? (int32_t)window : 0, reach,
+                        batch->max_rows * group <= FO_PAGED_FEW);
+}
+
+int fo_paged_prefix_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch *batch,
+                              const fo_paged_groups *groups, const fo_rows *q, const float *sinks, float scale,
+                              const fo_rows *out, float *lse) {
+    const char *name = "fo_paged_prefix_attention";
+    FO_TRY(check_attention(name, kv, batch, q, out, sinks, scale, 0, lse));
+    if (!groups) return fail(FO_ERR_INVALID, "%s: null groups", name);
+    if (groups->n_groups < 0 || groups->n_groups > 65535) return fail(FO_ERR_INVALID, "%s: 0 to 65,535 groups", name);
+    if (groups->n_groups > 0 && (!groups->seq_start || !groups->lens))
+        return fail(FO_ERR_INVALID, "%s: null groups' starts or lengths", name);
+    if (!aligned4(groups->seq_start) || !aligned4(groups->lens)) return fail(FO_ERR_INVALID, "%s: misaligned integers", name);
+    const int64_t group = q->heads / kv->n_kv_heads, rows = batch->total_rows, queries = batch->max_rows * group;
+    if (queries > INT32_MAX) return fail(FO_ERR_CAPACITY, "%s: more than 2^31 query rows of a KV head", name);
+    FO_TRY(check_tiles(name, kv, batch, (double)rows * group, (double)batch->n_seqs + groups->n_groups + 2));
+    if (!ctx) return fail(FO_ERR_INVALID, "null context");
+    if (rows == 0) return FO_OK;
+    DeviceGuard guard(ctx->device);
+    fo_paged_reach reach = {};
+    reach.group_start = groups->seq_start;
+    reach.group_lens = groups->lens;
+    reach.n_groups = (int32_t)groups->n_groups;
+    if (reach.n_groups == 0)
+        return launch_reach(ctx, kv, batch, q, out, sinks, lse, scale, 0, reach, queries <= FO_PAGED_FEW);
+    // Half a tile of query rows and more: the products bound the call, however
+    // often the beginning is read, so each sequence goes over all it sees.
+    if (queries >= FO_PAGED_ALONE) return launch_reach(ctx, kv, batch, q, out, sinks, lse, scale, 0, reach, false);
+    float *o = nullptr, *ml = nullptr;
+    FO_TRY(make_waiting(ctx, rows * q->heads, kv->head_dim, &o, &ml));
+    fo_paged_reach own = reach;
+    own.own_only = 1;
+    own.raw_o = o;
+    own.raw_ml = ml;
+    FO_TRY(launch_reach(ctx, kv, batch, q, out, nullptr, nullptr, scale, 0, own, queries <= FO_PAGED_FEW));
+    reach.over_groups = 1;
+    reach.prior_o = o;
+    reach.prior_ml = ml;
+    return launch_reach(ctx, kv, batch, q, out, sinks, lse, scale, 0, reach,
+                        rows * group <= FO_PAGED_FEW * groups->n_groups);
 }
 
 }  // extern "C"

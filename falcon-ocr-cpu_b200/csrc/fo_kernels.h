@@ -198,6 +198,16 @@ cudaError_t fo_launch_draft_attend(const int8_t *key_codes, const float *key_sca
 #define FO_DEVERR_POSITION 8u
 #define FO_DEVERR_VALUE 16u
 
+// Positions on several axes: row r's on axis a at [r * row_stride + a *
+// axis_stride], for the axes that pairs have (bits of `used`; 0: one position a
+// row, the rotation's own), and the axis of each pair, 2 bits.
+struct fo_axes_launch {
+    const int32_t *positions;
+    int64_t row_stride, axis_stride;
+    uint32_t used;
+    uint32_t pair_axis[8];
+};
+
 // Rotation of rows of heads (rope.cu); the launcher fills in the last line.
 struct fo_rope_launch {
     fo_rows x, out;
@@ -205,6 +215,7 @@ struct fo_rope_launch {
     fo_rope_spec rope;
     unsigned *err;
     int32_t head_dim, transpose, in_place;
+    struct fo_axes_launch axes;
     int32_t slots, head_blocks, block_x;
 };
 cudaError_t fo_launch_rope_table(float *table, int64_t positions, int32_t rot_dim, const fo_rope_scaling *scaling,
@@ -222,8 +233,27 @@ struct fo_append_launch {
     fo_rope_launch q;
     unsigned *err;
     int32_t rotate;
+    struct fo_axes_launch axes;
 };
 cudaError_t fo_launch_paged_append(const fo_append_launch *args, cudaStream_t stream);
+// With positions on several axes (paged_append_axes.cu).
+cudaError_t fo_launch_paged_append_axes(const fo_append_launch *args, cudaStream_t stream);
+
+// What the rows of a paged attention see beside the window's positions, and
+// where unfinished rows come from and go to (paged_reach.cuh).
+struct fo_paged_reach {
+    int32_t first;  // leading positions that stay in sight behind a window
+    // Groups of sequences: the positions before a group's length are in the pages
+    // of its first sequence.
+    const int32_t *group_start, *group_lens;
+    int32_t n_groups;  // 0: no sequence shares
+    int32_t over_groups;  // the call is over the groups' shared positions, each with all rows of its sequences
+    int32_t own_only;     // over each sequence's positions behind the shared ones
+    // Unfinished rows, [total_rows][heads][head_dim] sums and {maximum in log2
+    // units, sum of probabilities}: written in place of out, or joined.
+    float *raw_o, *raw_ml;
+    const float *prior_o, *prior_ml;
+};
 
 // Attention over the paged cache (paged_attention.cu).
 #define FO_PAGED_MAX_ROWS 64  // rows of one sequence
@@ -244,9 +274,37 @@ struct fo_paged_attention_launch {
     // holds, warps that share a tile, what 16-byte accesses may be used for, and
     // whether there are at most as many (sequence, KV head)s as blocks.
     int32_t group, queries, col_groups, q_vec, out_vec, evict_first, whole_units;
+    struct fo_paged_reach reach;  // fo_launch_paged_attention_reach alone
 };
 #define FO_PAGED_QUERIES 48  // queries that a block holds at most
 cudaError_t fo_launch_paged_attention(const fo_paged_attention_launch *args, int sms, cudaStream_t stream);
+// The same kernel with a reach (paged_attention_reach.cu).
+cudaError_t fo_launch_paged_attention_reach(const fo_paged_attention_launch *args, int sms, cudaStream_t stream);
+
+// Attention of many query rows over the paged cache on the 5th-generation
+// tensor cores (paged_tiles.cu).
+#define FO_TILES_QUERIES 256  // query rows of a block's unit at most
+#define FO_PAGED_ALONE 64     // query rows of a sequence from which on it reads a shared beginning by itself
+struct fo_paged_tiles_launch {
+    fo_paged_kv kv;
+    fo_paged_batch batch;
+    fo_rows q, out;
+    const float *sinks;
+    float *lse;
+    float scale;
+    int32_t window;  // 0: none
+    struct fo_paged_reach reach;
+    unsigned *err;
+    // Scratch of the context: a block's two unfinished parts, and which of them
+    // the second launch joins.
+    float *part_o;   // [2 sms][head_dim / 4][FO_TILES_QUERIES][4]
+    float *part_ml;  // [2 sms][FO_TILES_QUERIES][2]
+    int32_t *joins;  // [sms][8]
+    // Filled in by the launcher: query heads per KV head, units of queries per
+    // sequence, what 16-byte accesses may be used for.
+    int32_t group, q_units, q_vec, out_vec;
+};
+cudaError_t fo_launch_paged_tiles(const fo_paged_tiles_launch *args, int sms, cudaStream_t stream);
 
 // The bounded-wait self-test kernel (selftest.cu).
 cudaError_t fo_launch_bounded_wait(unsigned *err, unsigned long long limit_ns, cudaStream_t stream);

@@ -8,6 +8,33 @@
 namespace fo {
 
 constexpr int ROPE_THREADS = 256;
+
+// A row's entries of the rotation's table where its pairs stand on axes of their
+// own: NaN for an axis whose position lies outside the table.
+struct AxisEntries {
+    int p[FO_ROPE_MAX_AXES];
+    // Reads the row's positions; whether all that pairs have lie inside.
+    __device__ __forceinline__ bool read(const fo_axes_launch &a, int64_t positions, int64_t row) {
+        bool inside = true;
+#pragma unroll
+        for (int x = 0; x < FO_ROPE_MAX_AXES; x++) {
+            p[x] = -1;
+            if (a.used >> x & 1) p[x] = a.positions[row * a.row_stride + x * a.axis_stride];
+        }
+#pragma unroll
+        for (int x = 0; x < FO_ROPE_MAX_AXES; x++) {
+            if (p[x] >= positions) p[x] = -1;
+            if ((a.used >> x & 1) && p[x] < 0) inside = false;
+        }
+        return inside;
+    }
+    __device__ __forceinline__ float2 entry(const fo_axes_launch &a, const fo_rope_spec &rope, int pair) const {
+        const uint32_t axis = a.pair_axis[pair >> 4] >> (2 * (pair & 15)) & 3u;
+        const int low = axis & 1 ? p[1] : p[0], high = axis & 1 ? p[3] : p[2], at = axis & 2 ? high : low;
+        if (at < 0) return make_float2(NAN, NAN);
+        return load_entry(reinterpret_cast<const float2 *>(rope.table) + (int64_t)at * (rope.rot_dim / 2) + pair);
+    }
+};
 // Heads a thread takes with one read of its table entries: 64 or 128 bytes of
 // loads in flight for each thread.
 template <typename T, bool HALF>
@@ -44,7 +71,7 @@ inline bool rope_shape(fo_rope_launch *a) {
 
 // Block `block` of the rotation, thread t of ROPE_THREADS; `position(row, padded)` gives a row's
 // position, or sets padded (the row is copied as it is).
-template <typename T, bool HALF, bool VEC, typename Position>
+template <typename T, bool HALF, bool VEC, bool AXES, typename Position>
 __device__ __forceinline__ void rope_block(const fo_rope_launch &a, int64_t block, int t, Position position) {
     // block_x threads over (head block, slot), the others over rows.
     const int rows_per_block = ROPE_THREADS / a.block_x;
@@ -59,7 +86,14 @@ __device__ __forceinline__ void rope_block(const fo_rope_launch &a, int64_t bloc
     // which do not wait for its position.
     const float2 *entries = nullptr;
     bool inside = false, padded = false;
+    AxisEntries on_axes;
     auto look_up = [&]() {
+        if constexpr (AXES) {
+            if (inside) return;  // read
+            inside = true;
+            if (!on_axes.read(a.axes, a.rope.positions, row) && tx == 0) atomicOr(a.err, FO_DEVERR_POSITION);
+            return;
+        }
         if (entries) return;
         const int64_t p = position(row, padded);
         inside = p >= 0 && p < a.rope.positions;
@@ -67,8 +101,10 @@ __device__ __forceinline__ void rope_block(const fo_rope_launch &a, int64_t bloc
         entries = reinterpret_cast<const float2 *>(a.rope.table) + (inside ? p : 0) * h2;
     };
     auto entry = [&](int pair) {
-        float2 cs = load_entry(entries + pair);
-        if (!inside) cs = padded ? make_float2(1.0f, 0.0f) : make_float2(NAN, NAN);
+        float2 cs;
+        if constexpr (AXES) cs = on_axes.entry(a.axes, a.rope, pair);
+        else cs = load_entry(entries + pair);
+        if (!AXES && !inside) cs = padded ? make_float2(1.0f, 0.0f) : make_float2(NAN, NAN);
         if (a.transpose) cs.y = -cs.y;
         return cs;
     };

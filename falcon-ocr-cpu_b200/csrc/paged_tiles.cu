@@ -1,0 +1,1226 @@
+// paged_tiles.cu -- attention of many query rows of a KV head over the paged
+// 8-bit cache: prompts (over a window and first positions, or all of them), and
+// the shared beginning of a group of sequences, once for all their rows.
+//
+// For a query row q that sees positions j: s_j = scale * kscale * (q . kcode_j),
+// m = max s_j, out = sum_j e^(s_j - m) vscale vcode_j / (sum_j e^(s_j - m) +
+// e^(sink - m)).  With 128 query rows and more to a KV head the products bound
+// the call, so they belong on the 5th-generation tensor cores, in FP16 with FP32
+// sums: FP16 holds every int8 and every e4m3 code, so nothing of the cache is
+// rounded; a query row is taken relative to a power of two near its largest
+// element (exact for BF16's 8 bits; FP32 rows as the sum of two FP16, 22 bits);
+// a probability times its page's value scale, relative to the largest scale so
+// far and times 2^10, is one FP16 (11 bits) or two, down to 2^-24 of the row's
+// largest at full precision.  The sum of probabilities takes them unrounded.
+//
+// Work is a line of tiles of 128 positions, the tiles of a unit (128 or 256
+// query rows of one KV head) adjacent; each of at most one block per SM takes an
+// equal piece.  A block that holds a part of a unit leaves the rows' maxima, sums
+// and outputs in scratch, which a second, small launch joins (by all SMs: joined
+// by one of the unit's blocks, 8 units of 18 parts would wait for eight SMs'
+// share of L2).
+//
+// In a block:
+//   warp 12      walks the line: page numbers, scales, and bulk copies of the
+//                codes into a ring, 8 KB a slot; announces the segments (a unit's
+//                tiles in this block) to the other warps;
+//   warps 8-11   codes to FP16, into swizzled operand tiles (two of keys, two of
+//                values);
+//   warps 14-15  a segment's query rows to FP16 operands, and what each row sees;
+//   warp 13      issues S_t = Q_t K^T and O_t += P_t V, whichever is ready;
+//   warps 0-7    two softmax warpgroups, a thread to a query row: S from tensor
+//                memory, scales, mask, exponentials, P back to tensor memory, and
+//                at the end of a segment O.
+// The two warpgroups are two streams: of a unit of more than 128 query rows each
+// takes 128 of them over all tiles; of a smaller one, both take the same rows over
+// every other tile, and join at the end, so a few rows still keep two tiles in
+// flight.
+// Tensor memory (512 columns): S_t at 128 t; heads of 64 and BF16 rows: O_t at
+// 256 + 64 t, P_t at 384 + 64 t; else P_t in S_t's place and O_t at 256 + 128 t.
+// Every wait is bounded; on a timeout the block unwinds, waits for its own copies
+// and MMAs, frees tensor memory and reports through the error word.
+#include "paged_reach.cuh"
+#include "sm100.cuh"
+
+#include <algorithm>
+#include <atomic>
+#include <type_traits>
+
+namespace fo {
+using namespace sm100;
+
+constexpr int PT_TILE = 128;  // positions
+constexpr int PT_SOFTMAX = 8, PT_CONVERTERS = 4, PT_LOADERS = 2;
+constexpr int PT_PRODUCER = PT_SOFTMAX + PT_CONVERTERS, PT_ISSUER = PT_PRODUCER + 1, PT_LOADER = PT_ISSUER + 1;
+constexpr int PT_THREADS = 32 * (PT_LOADER + PT_LOADERS);
+// Registers a thread: launched with 128, the softmax warpgroups' two take what
+// the other two give up: 256 * 176 + 256 * 80 = 512 * 128.
+constexpr int PT_LAUNCH_REGS = 128, PT_SOFTMAX_REGS = 176, PT_OTHER_REGS = 80;
+static_assert(256 * PT_SOFTMAX_REGS + 256 * PT_OTHER_REGS == PT_THREADS * PT_LAUNCH_REGS, "register split");
+constexpr int PT_SEGS = 8;    // segments announced at a time
+constexpr int PT_METAS = 16;  // tiles whose scales are held: what the code ring and the operands can be ahead by, and more
+constexpr uint32_t PT_SLOT = 8192, PT_PANEL = 16384;  // a slot of codes; 128 rows of 64 FP16
+// Exponent bits of a power of two above x (x from 2^-116 to 2^126; what is smaller
+// is taken as that, relative to which FP16 holds less of it).
+constexpr int PT_LOWEST = 12;
+__device__ __forceinline__ int pt_above(float x) {
+    return min(max((int)(__float_as_uint(x) >> 23 & 255u) + 1, PT_LOWEST), 253);
+}
+
+// A row's maximum moves only when a score passes it by more than 2^4: P stays
+// below 2^15, FP16's range.
+constexpr float PT_SLACK = 4.0f;
+
+template <int D, bool F32>
+struct PtShape {
+    static constexpr int TERMS = 1 + F32;  // FP16 terms of a query and of a probability
+    static constexpr int Q_TILES = F32 && D == 128 ? 1 : 2;
+    static constexpr int QUERIES = 128 * Q_TILES;
+    static constexpr bool ALIAS = D == 128 || F32;  // P in S's place
+    static constexpr int PANELS = D / 64;
+    static constexpr uint32_t OPERAND = PANELS * PT_PANEL;  // 128 rows of D FP16
+    static constexpr uint32_t Q_BYTES = Q_TILES * TERMS * OPERAND;
+    static constexpr int Q_BUFS = D == 64 && !F32 ? 2 : 1;
+    static constexpr int PARTS = D / 64;  // slots of a tile's keys, or values
+    static constexpr int SLOTS = D == 64 ? 6 : 3;
+    static constexpr uint32_t OFF_K = Q_BUFS * Q_BYTES, OFF_V = OFF_K + 2 * OPERAND, OFF_CODES = OFF_V + 2 * OPERAND;
+    static constexpr uint32_t SMEM = OFF_CODES + SLOTS * PT_SLOT + 1024;
+};
+
+// A unit's tiles in this block, and the unit.
+struct PtSegment {
+    int n, base;     // tiles, and the first one's number in the block
+    int pair, last;  // two query tiles; the block's last segment
+    int head, first, q0, nq;  // KV head; the rows' first; the unit's queries [q0, q0 + nq) of them
+    int p0, end, flat;        // position of the first row; end of what is seen; rows look their positions up
+    int part;                 // scratch of an unfinished unit's part, -1: the unit is whole
+};
+
+struct PtMeta {
+    float ks[8], vs[8];  // keys' and values' scales of each 16 positions' page
+    int top;             // exponent bits of a power of two above the values' scales
+    int base;            // the tile's first position
+    int from, to;        // positions [from, to) that rows may see of it
+    unsigned pages;      // pages that were copied
+};
+
+template <int D, bool F32>
+struct PtShared {
+    using Shape = PtShape<D, F32>;
+    uint64_t code_full[Shape::SLOTS], code_empty[Shape::SLOTS];
+    uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
+    uint64_t s_full[2], s_read[2], p_full[2], o_full[2];
+    uint64_t q_full[2], q_free[2];
+    uint64_t seg_full[PT_SEGS], seg_free[PT_SEGS];
+    uint64_t meta_full[PT_METAS];
+    uint64_t x_full, x_free, done;
+    PtSegment seg[PT_SEGS];
+    PtMeta meta[PT_METAS];
+    float q_scale[Shape::Q_BUFS][Shape::QUERIES];
+    int q_high[Shape::Q_BUFS][Shape::QUERIES], q_low[Shape::Q_BUFS][Shape::QUERIES];
+    float xm[2][128], xl[2][128], xt[2][128];
+    int2 warp_sum[PT_THREADS / 32];
+    int begin_item, begin_base, abort;
+    uint32_t tmem;
+};
+
+// ------------------------------------------------------------------ the line
+// An item of the line: a unit of query rows of a sequence, for each KV head; or a
+// group, all of its units of query rows, for each KV head.
+struct PtItem {
+    int seq;          // whose row of the page table
+    int first, n;     // rows
+    int p0, end;      // position of the first row; end of what is seen
+    int low, t0, tf;  // first position seen behind the first ones; its tile; tiles of the first ones, which come before
+    int shared, leader;  // positions in another sequence's pages, and that sequence
+    int tiles, units;
+    int q0;           // the unit's first query (a sequence's)
+};
+
+template <int QUERIES>
+__device__ __forceinline__ PtItem pt_item(const fo_paged_tiles_launch &a, int index) {
+    PtItem x;
+    x.low = x.t0 = x.tf = x.q0 = x.p0 = x.shared = x.leader = 0;
+    if (a.reach.over_groups) {
+        const Group g = load_group(a.reach, a.batch, a.kv.page_size, index, a.err);
+        x.seq = g.leader;
+        x.first = g.first;
+        x.n = g.n;
+        x.end = g.len;
+        x.tiles = max((int)(((unsigned)g.len + PT_TILE - 1) / PT_TILE), 1);
+        x.units = (int)(((unsigned)(g.n * a.group) + QUERIES - 1) / QUERIES) * a.kv.n_kv_heads;
+        return x;
+    }
+    x.seq = index / a.q_units;
+    const Sequence s = load_sequence(a.batch, a.kv.page_size, x.seq, a.err);
+    x.q0 = (index - x.seq * a.q_units) * QUERIES;
+    x.first = s.first;
+    x.n = s.n;
+    x.p0 = s.len - s.n;
+    const int queries = s.n * a.group - x.q0;
+    x.units = queries > 0 ? a.kv.n_kv_heads : 0;
+    const int last = (x.q0 + min(queries, QUERIES) - 1) / a.group;
+    const int from = max(x.p0 + x.q0 / a.group, 0);
+    x.end = min(max(x.p0 + last + 1, 0), s.len);
+    int first = a.reach.first;
+    if (a.reach.n_groups > 0) {
+        // The tile that the shared positions end in comes twice, for each sequence's part of it.
+        const Shared g = shared_of(a.reach, a.batch, a.kv.page_size, x.seq, a.err);
+        x.shared = x.low = first = g.len;
+        x.leader = g.leader;
+    } else {
+        x.low = a.window > 0 ? max(from + 1 - a.window, 0) : 0;
+    }
+    x.t0 = x.low / PT_TILE;
+    x.tf = (int)(((unsigned)min(first, x.end) + PT_TILE - 1) / PT_TILE);
+    if (x.shared == 0) x.tf = min(x.tf, x.t0);
+    if (a.reach.own_only) x.tf = 0;
+    const int near = x.end > x.low ? (int)(((unsigned)x.end + PT_TILE - 1) / PT_TILE) - x.t0 : 0;
+    x.tiles = max(near + x.tf, 1);
+    return x;
+}
+
+// Sum of x over the block's earlier threads; `all` the whole block's.
+template <typename Shared_>
+__device__ __forceinline__ int pt_scan(int x, Shared_ &sh, int &all) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    int sum = x;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, sum, o);
+        if (lane >= o) sum += u;
+    }
+    __syncthreads();  // the last scan's sums have been read
+    if (lane == 31) sh.warp_sum[warp].x = sum;
+    __syncthreads();
+    int before = sum - x;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < PT_THREADS / 32; w++) {
+        const int y = sh.warp_sum[w].x;
+        if (w < warp) before += y;
+        all += y;
+    }
+    return before;
+}
+
+// ------------------------------------------------------------------- numbers
+__host__ __device__ constexpr uint32_t idesc_f16(uint32_t m, uint32_t n, uint32_t b_mn_major) {
+    return (1u << 4) | (b_mn_major << 16) | ((n >> 3) << 17) | ((m >> 4) << 24);
+}
+__device__ __forceinline__ uint32_t pt_f16x2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ uint32_t pt_sub_f16x2(uint32_t a, uint32_t b) {
+    uint32_t r;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+    return r;
+}
+// Four codes as four FP16 (exact).  int8: the byte of code + 128 under 1024's
+// exponent is 1024 + code + 128.
+template <int FORMAT>
+__device__ __forceinline__ uint2 pt_widen(uint32_t w) {
+    if constexpr (FORMAT == FO_PAGED_I8) {
+        const uint32_t u = w ^ 0x80808080u;
+        return make_uint2(pt_sub_f16x2(__byte_perm(u, 0x64646464u, 0x4140), 0x64806480u),
+                          pt_sub_f16x2(__byte_perm(u, 0x64646464u, 0x4342), 0x64806480u));
+    } else {
+        return make_uint2(e4m3x2_f16x2(w & 0xFFFFu), e4m3x2_f16x2(w >> 16));
+    }
+}
+
+// Writes 32 dimensions of a finished row.
+template <typename T>
+__device__ __forceinline__ void pt_store32(T *to, const float *v, bool vec) {
+    if (vec) {
+#pragma unroll
+        for (int i = 0; i < 32; i += 8) store8(to + i, v + i);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 32; i++) store1(to + i, v[i]);
+    }
+}
+
+template <int D, int FORMAT, bool F32>
+__global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid_constant__ fo_paged_tiles_launch a) {
+    using Shape = PtShape<D, F32>;
+    using T = typename std::conditional<F32, float, uint16_t>::type;
+    constexpr int QUERIES = Shape::QUERIES, TERMS = Shape::TERMS, PANELS = Shape::PANELS, PARTS = Shape::PARTS;
+    constexpr int SLOTS = Shape::SLOTS, Q_BUFS = Shape::Q_BUFS;
+    constexpr bool ALIAS = Shape::ALIAS;
+    extern __shared__ uint8_t pt_smem[];
+    __shared__ PtShared<D, F32> sh;
+    uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(pt_smem) + 1023) & ~uintptr_t(1023));
+    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    volatile int *abort_flag = &sh.abort;
+
+    if (warp == PT_ISSUER) {
+        if (lane < SLOTS) mbar_init(&sh.code_full[lane], 1), mbar_init(&sh.code_empty[lane], PT_CONVERTERS);
+        if (lane < 2) {
+            mbar_init(&sh.k_full[lane], PT_CONVERTERS), mbar_init(&sh.v_full[lane], PT_CONVERTERS);
+            mbar_init(&sh.k_empty[lane], 1), mbar_init(&sh.v_empty[lane], 1);
+            mbar_init(&sh.s_full[lane], 1), mbar_init(&sh.o_full[lane], 1);
+            mbar_init(&sh.s_read[lane], 4), mbar_init(&sh.p_full[lane], 4);
+            mbar_init(&sh.q_full[lane], PT_LOADERS), mbar_init(&sh.q_free[lane], 1 + PT_SOFTMAX);
+        }
+        if (lane < PT_SEGS) {
+            mbar_init(&sh.seg_full[lane], 1);
+            mbar_init(&sh.seg_free[lane], PT_SOFTMAX + PT_LOADERS + 1);
+        }
+        if (lane < PT_METAS) mbar_init(&sh.meta_full[lane], 1);
+        if (lane == 31) {
+            mbar_init(&sh.x_full, PT_SOFTMAX), mbar_init(&sh.x_free, PT_SOFTMAX), mbar_init(&sh.done, 1);
+            sh.abort = 0;
+        }
+        mbar_fence_init();
+        __syncwarp();
+        tmem_alloc(&sh.tmem, 512);
+    }
+    wait_for_prior_kernel();
+
+    // This block's piece [begin, end) of the line, and where it begins.  (The
+    // line's tiles are below 2^31, checked on the host.)
+    const int n_items = a.reach.over_groups ? a.reach.n_groups + 2 : (int)a.batch.n_seqs * a.q_units;
+    int per, begin, count;
+    {
+        auto work = [&](int index) {
+            if (index >= n_items) return 0;
+            const PtItem x = pt_item<QUERIES>(a, index);
+            return x.tiles * x.units;
+        };
+        int mine = work(tid), chunk, before = pt_scan(mine, sh, chunk), all = chunk;
+        for (int first = PT_THREADS; first < n_items; first += PT_THREADS) {
+            int more;
+            pt_scan(work(first + tid), sh, more);
+            all += more;
+        }
+        per = max((int)((unsigned)(all + gridDim.x - 1) / gridDim.x), 2);
+        begin = (int)min((long long)per * blockIdx.x, (long long)all);
+        count = (int)min((long long)per, (long long)all - begin);
+        if (count > 0) {
+            for (int first = 0, sum = 0;;) {
+                if (begin >= sum + before && begin < sum + before + mine) {
+                    sh.begin_item = first + tid;
+                    sh.begin_base = sum + before;
+                }
+                first += PT_THREADS;
+                if (first >= n_items) break;
+                sum += chunk;
+                mine = work(first + tid);
+                before = pt_scan(mine, sh, chunk);
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem;
+    if (count <= 0) {
+        if (tid == 0) a.joins[8 * blockIdx.x] = 0;
+        if (warp == PT_ISSUER) tmem_dealloc(tmem, 512);
+        return;
+    }
+
+    if (warp < PT_SOFTMAX) {
+        // -------------------------------------------------------------- softmax
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PT_SOFTMAX_REGS));
+        const int t = warp >> 2, wq = warp & 3, r = tid & 127;
+        const uint32_t at = tmem + ((uint32_t)(32 * wq) << 16);
+        const uint32_t s_at = at + 128 * t, p_at = ALIAS ? s_at : at + 384 + 64 * t;
+        auto o_at = [&](int stream) { return at + 256 + (ALIAS ? 128 : 64) * stream; };
+        int c = 0, x_phase = 0;  // tiles of this stream so far; joins of both streams
+        bool ok = true;
+        for (int s = 0; ok; s++) {
+            ok = __all_sync(0xffffffffu, mbar_wait(&sh.seg_full[s % PT_SEGS], (s / PT_SEGS) & 1, abort_flag, a.err));
+            if (!ok) break;
+            const PtSegment &seg = sh.seg[s % PT_SEGS];
+            const int n = seg.n, base = seg.base, pair = seg.pair, last = seg.last;
+            const int q = (pair ? 128 * t : 0) + r;  // of the unit's
+            const bool live = (pair ? 128 * t : 0) + 32 * wq < seg.nq;
+            ok = __all_sync(0xffffffffu, mbar_wait(&sh.q_full[s % Q_BUFS], (s / Q_BUFS) & 1, abort_flag, a.err));
+            if (!ok) break;
+            const float q_scale = sh.q_scale[s % Q_BUFS][q];
+            const int high = sh.q_high[s % Q_BUFS][q], low = sh.q_low[s % Q_BUFS][q];
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.q_free[s % Q_BUFS]);
+            float m = -INFINITY, l = 0.0f;
+            int top = PT_LOWEST;  // exponent bits of a power of two above the scales of the values that the row sees
+            bool any = false;
+            for (int i = pair ? 0 : t; i < n; i += pair ? 1 : 2, c++) {
+                const int k = base + i;
+                ok = __all_sync(0xffffffffu, mbar_wait(&sh.s_full[t], c & 1, abort_flag, a.err));
+                if (!ok) break;
+                if (!live) {
+                    // No query in this warp: whatever its lanes hold stays theirs.  (It arrives once
+                    // for each tile as the others do, not for the next one before they have for this.)
+                    if (lane == 0) mbar_arrive(&sh.s_read[t]);
+                    if (any) ok = __all_sync(0xffffffffu, mbar_wait(&sh.o_full[t], (c - 1) & 1, abort_flag, a.err));
+                    if (!ok) break;
+                    if (lane == 0) mbar_arrive(&sh.p_full[t]);
+                    __syncwarp();
+                    any = true;
+                    continue;
+                }
+                ok = __all_sync(0xffffffffu, mbar_wait(&sh.meta_full[k % PT_METAS], (k / PT_METAS) & 1, abort_flag, a.err));
+                if (!ok) break;
+                tc_fence_after();
+                uint32_t raw[128];
+                FO_TMEM_LD32(s_at + 0, (raw + 0));
+                FO_TMEM_LD32(s_at + 32, (raw + 32));
+                FO_TMEM_LD32(s_at + 64, (raw + 64));
+                FO_TMEM_LD32(s_at + 96, (raw + 96));
+                const PtMeta &meta = sh.meta[k % PT_METAS];
+                const int tile = meta.base;
+                int tile_top = meta.top;
+                float f[8];
+#pragma unroll
+                for (int g = 0; g < 8; g++) f[g] = meta.ks[g] * q_scale;
+                tmem_wait_ld();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.s_read[t]);
+                // Scores in log2 units, two at a time.
+                float2 x[64];
+#pragma unroll
+                for (int e = 0; e < 64; e++)
+                    x[e] = __fmul2_rn(make_float2(__uint_as_float(raw[2 * e]), __uint_as_float(raw[2 * e + 1])),
+                                      make_float2(f[e / 8], f[e / 8]));
+                const int hi = min(high, meta.to - 1), lo = max(low, meta.from);
+                const bool full = hi - tile >= PT_TILE - 1 && (lo <= tile || a.reach.first - tile >= PT_TILE);
+                if (!__all_sync(0xffffffffu, full)) {
+                    // Keys that the row sees, as bits.
+                    tile_top = PT_LOWEST;
+                    auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; };
+#pragma unroll
+                    for (int w = 0; w < 4; w++) {
+                        const int b = tile + 32 * w;
+                        // (Differences that cannot wrap: every one is of numbers from -1 up.)
+                        const uint32_t see = below(min(hi - b, 32) + 1) & (~below(lo - b) | below(a.reach.first - b));
+                        if (see & 0x0000FFFFu) tile_top = max(tile_top, pt_above(meta.vs[2 * w]));
+                        if (see & 0xFFFF0000u) tile_top = max(tile_top, pt_above(meta.vs[2 * w + 1]));
+#pragma unroll
+                        for (int e = 0; e < 16; e++) {
+                            if (!(see >> (2 * e) & 1)) x[16 * w + e].x = -INFINITY;
+                            if (!(see >> (2 * e + 1) & 1)) x[16 * w + e].y = -INFINITY;
+                        }
+                    }
+                }
+                float mx0 = x[0].x, mx1 = x[0].y, mx2 = x[1].x, mx3 = x[1].y;
+#pragma unroll
+                for (int e = 2; e < 64; e += 2) {
+                    mx0 = fmaxf(mx0, x[e].x);
+                    mx1 = fmaxf(mx1, x[e].y);
+                    mx2 = fmaxf(mx2, x[e + 1].x);
+                    mx3 = fmaxf(mx3, x[e + 1].y);
+                }
+                const float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3));
+                float factor = 1.0f;  // of what has been summed so far
+                if (!any) {
+                    m = mx;
+                    top = tile_top;
+                } else if (__any_sync(0xffffffffu, mx > m + PT_SLACK || tile_top > top)) {
+                    const float next = fmaxf(m, mx);
+                    const float alpha = next == -INFINITY ? 1.0f : ex2(m - next);
+                    l *= alpha;
+                    // (Beyond 2^-126 what was summed is nothing next to what comes.)
+                    factor = alpha * __uint_as_float((uint32_t)max(127 + top - max(top, tile_top), 0) << 23);
+                    m = next;
+                    top = max(top, tile_top);
+                }
+                // Values' scales times 2^10 / top; those of pages that the row does not see meet zeros.
+                const float inverse_top = __uint_as_float((uint32_t)(264 - top) << 23);
+#pragma unroll
+                for (int g = 0; g < 8; g++) f[g] = fminf(meta.vs[g] * inverse_top, FLT_MAX);
+                const float shift = m == -INFINITY ? 0.0f : m;
+                // P may be written, and O touched, once the PV before is complete.
+                uint32_t pk[64];
+                float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+                auto probabilities = [&](int e) {
+                    const float2 d = __fadd2_rn(x[e], make_float2(-shift, -shift));
+                    const float2 p = make_float2(ex2(d.x), ex2(d.y));
+                    sum[e & 1] = __fadd2_rn(sum[e & 1], p);
+                    return __fmul2_rn(p, make_float2(f[e / 8], f[e / 8]));
+                };
+                if constexpr (!F32) {
+#pragma unroll
+                    for (int e = 0; e < 64; e++) {
+                        const float2 p = probabilities(e);
+                        pk[e] = pt_f16x2(p.x, p.y);
+                    }
+                }
+                if (any) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(&sh.o_full[t], (c - 1) & 1, abort_flag, a.err));
+                    if (!ok) break;
+                    if (__any_sync(0xffffffffu, factor != 1.0f)) {
+                        tc_fence_after();
+#pragma unroll
+                        for (int h = 0; h < D / 16; h++) {
+                            uint32_t o[16];
+                            asm volatile(
+                                "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                                : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]), "=r"(o[4]), "=r"(o[5]), "=r"(o[6]), "=r"(o[7]),
+                                  "=r"(o[8]), "=r"(o[9]), "=r"(o[10]), "=r"(o[11]), "=r"(o[12]), "=r"(o[13]), "=r"(o[14]), "=r"(o[15])
+                                : "r"(o_at(t) + 16 * h)
+                                : "memory");
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
+                            asm volatile(
+                                "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
+                                ::"r"(o_at(t) + 16 * h),
+                                "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7]),
+                                "r"(o[8]), "r"(o[9]), "r"(o[10]), "r"(o[11]), "r"(o[12]), "r"(o[13]), "r"(o[14]), "r"(o[15])
+                                : "memory");
+                        }
+                        tmem_wait_st();
+                    }
+                }
+                if constexpr (!F32) {
+                    FO_TMEM_ST32(p_at, (pk + 0));
+                    FO_TMEM_ST32(p_at + 32, (pk + 32));
+                } else {
+                    // Two terms; half of the keys at a time, for the registers.
+#pragma unroll
+                    for (int h = 0; h < 2; h++) {
+#pragma unroll
+                        for (int e = 0; e < 32; e++) {
+                            const float2 p = probabilities(32 * h + e);
+                            pk[e] = pt_f16x2(p.x, p.y);
+                            const float2 b = f16x2_f32x2(pk[e]);
+                            pk[32 + e] = pt_f16x2(p.x - b.x, p.y - b.y);
+                        }
+                        FO_TMEM_ST32(p_at + 32 * h, (pk + 0));
+                        FO_TMEM_ST32(p_at + 64 + 32 * h, (pk + 32));
+                    }
+                }
+                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.p_full[t]);
+                any = true;
+            }
+            if (!ok) break;
+            // The segment's end.
+            if (any) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&sh.o_full[t], (c - 1) & 1, abort_flag, a.err));
+                if (!ok) break;
+                tc_fence_after();
+            }
+            // O times f0, and where both streams have these rows the other's times f1.
+            const float unit = __uint_as_float((uint32_t)(top - 10) << 23);  // of O
+            float f0 = unit, f1 = 0.0f;
+            int c0 = 0, c1 = D;  // this thread's dimensions
+            bool has0 = any, has1 = false;
+            int o_from = t;
+            if (!pair) {
+                sh.xm[t][r] = m;
+                sh.xl[t][r] = l;
+                sh.xt[t][r] = unit;
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.x_full);
+                ok = __all_sync(0xffffffffu, mbar_wait(&sh.x_full, x_phase, abort_flag, a.err));
+                if (!ok) break;
+                tc_fence_after();
+                const Joined j = join_parts(sh.xm[0][r], sh.xl[0][r], sh.xm[1][r], sh.xl[1][r]);
+                m = j.m;
+                l = j.l;
+                f0 = j.f0 * sh.xt[0][r];
+                f1 = j.f1 * sh.xt[1][r];
+                c0 = t * (D / 2);
+                c1 = c0 + D / 2;
+                has0 = true;
+                has1 = n > 1;
+                o_from = 0;
+            }
+            if (live) {
+                const bool mine = q < seg.nq;
+                const int qi = seg.q0 + q, row_of = qi / a.group, h = seg.head * a.group + qi - row_of * a.group;
+                const int64_t row = seg.first + row_of;
+                const int part = seg.part;
+                float inv = 0.0f, fp = 0.0f;
+                const int64_t at_row = row * a.q.heads + h;
+                if (mine && part < 0 && a.reach.raw_o) {
+                    if (pair || t == 0) reinterpret_cast<float2 *>(a.reach.raw_ml)[at_row] = make_float2(m, l);
+                } else if (mine && part < 0) {
+                    if (a.reach.prior_o) {
+                        const float2 prior = reinterpret_cast<const float2 *>(a.reach.prior_ml)[at_row];
+                        const Joined j = join_parts(m, l, prior.x, prior.y);
+                        m = j.m;
+                        l = j.l;
+                        f0 *= j.f0;
+                        f1 *= j.f0;
+                        fp = j.f1;
+                    }
+                    inv = inverse_sum(a.sinks, h, m, l);
+                    if (a.lse && (pair || t == 0)) a.lse[at_row] = log_sum(m, l);
+                } else if (mine && (pair || t == 0)) {
+                    reinterpret_cast<float2 *>(a.part_ml)[(int64_t)part * FO_TILES_QUERIES + q] = make_float2(m, l);
+                }
+#pragma unroll 1
+                for (int d = c0; d < c1; d += 32) {
+                    uint32_t o[32];
+                    float v[32];
+                    if (has0) {
+                        FO_TMEM_LD32(o_at(o_from) + d, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; e++) v[e] = __uint_as_float(o[e]) * f0;
+                    }
+                    if (has1) {
+                        FO_TMEM_LD32(o_at(1) + d, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; e++) v[e] = fmaf(__uint_as_float(o[e]), f1, v[e]);
+                    }
+                    if (!mine) continue;
+                    if (part >= 0) {
+                        float4 *to = reinterpret_cast<float4 *>(a.part_o) +
+                                     ((int64_t)part * (D / 4) + d / 4) * FO_TILES_QUERIES + q;
+#pragma unroll
+                        for (int e = 0; e < 8; e++)
+                            __stcg(to + e * FO_TILES_QUERIES,
+                                   make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]));
+                        continue;
+                    }
+                    if (a.reach.raw_o) {
+                        float4 *to = reinterpret_cast<float4 *>(a.reach.raw_o + at_row * D + d);
+#pragma unroll
+                        for (int e = 0; e < 8; e++) to[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+                        continue;
+                    }
+                    if (a.reach.prior_o) {
+                        const float4 *from = reinterpret_cast<const float4 *>(a.reach.prior_o + at_row * D + d);
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            const float4 y = __ldcg(from + e);
+                            v[4 * e] = fmaf(y.x, fp, v[4 * e]);
+                            v[4 * e + 1] = fmaf(y.y, fp, v[4 * e + 1]);
+                            v[4 * e + 2] = fmaf(y.z, fp, v[4 * e + 2]);
+                            v[4 * e + 3] = fmaf(y.w, fp, v[4 * e + 3]);
+                        }
+                    }
+#pragma unroll
+                    for (int e = 0; e < 32; e++) v[e] *= inv;
+                    pt_store32(static_cast<T *>(a.out.data) + row * a.out.row_stride + h * a.out.head_stride + d, v,
+                               a.out_vec);
+                }
+            }
+            if (!pair) {
+                // Neither stream goes on to write its O before the other has read it.
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.x_free);
+                ok = __all_sync(0xffffffffu, mbar_wait(&sh.x_free, x_phase, abort_flag, a.err));
+                x_phase ^= 1;
+                if (!ok) break;
+            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.seg_free[s % PT_SEGS]);
+            if (last) break;
+        }
+    } else if (warp < PT_PRODUCER) {
+        // ----------------------------------------------------------- converters
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PT_OTHER_REGS));
+        const int ct = tid - 32 * PT_SOFTMAX, log_page = 31 - __clz(a.kv.page_size);
+        constexpr int CHUNKS = D / 16;  // 16-byte chunks of a row's codes
+        int slot = 0, round = 0;
+        bool ok = true;
+        for (int k = 0; k < count && ok; k++) {
+#pragma unroll
+            for (int value = 0; value < 2; value++) {
+                uint64_t *full = value ? &sh.v_full[k & 1] : &sh.k_full[k & 1];
+                uint64_t *empty = value ? &sh.v_empty[k & 1] : &sh.k_empty[k & 1];
+                uint8_t *to = smem + (value ? Shape::OFF_V : Shape::OFF_K) + (k & 1) * Shape::OPERAND;
+                if (k > 1) ok = __all_sync(0xffffffffu, mbar_wait(empty, (k / 2 - 1) & 1, abort_flag, a.err));
+                if (!ok) break;
+#pragma unroll 1
+                for (int h = 0; h < PARTS; h++) {
+                    ok = __all_sync(0xffffffffu, mbar_wait(&sh.code_full[slot], round & 1, abort_flag, a.err));
+                    if (!ok) break;
+                    const uint4 *from = reinterpret_cast<const uint4 *>(smem + Shape::OFF_CODES + slot * PT_SLOT);
+                    const unsigned pages = sh.meta[k % PT_METAS].pages;
+                    const int row_from = sh.meta[k % PT_METAS].from - sh.meta[k % PT_METAS].base;
+                    const int row_to = sh.meta[k % PT_METAS].to - sh.meta[k % PT_METAS].base;
+                    uint4 w[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) w[j] = from[j * 128 + ct];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        const int u = j * 128 + ct, row = h * (PT_TILE / PARTS) + u / CHUNKS, chunk = u % CHUNKS;
+                        // Values that were not copied, or that no row sees, may be any bytes: an FP8 NaN
+                        // times a probability of 0 would be NaN.
+                        if (value && !(row >= row_from && row < row_to && (pages >> (row >> log_page) & 1)))
+                            w[j] = make_uint4(0, 0, 0, 0);
+                        const uint2 h0 = pt_widen<FORMAT>(w[j].x), h1 = pt_widen<FORMAT>(w[j].y);
+                        const uint2 h2 = pt_widen<FORMAT>(w[j].z), h3 = pt_widen<FORMAT>(w[j].w);
+                        uint8_t *line = to + (chunk >> 2) * PT_PANEL + row * 128;
+                        const int c16 = 2 * (chunk & 3), odd = chunk >> 2;  // which half first: other banks for the panels
+                        const uint4 lo = make_uint4(h0.x, h0.y, h1.x, h1.y), hi = make_uint4(h2.x, h2.y, h3.x, h3.y);
+                        *reinterpret_cast<uint4 *>(line + (((c16 + odd) ^ (row & 7)) << 4)) = odd ? hi : lo;
+                        *reinterpret_cast<uint4 *>(line + (((c16 + 1 - odd) ^ (row & 7)) << 4)) = odd ? lo : hi;
+                    }
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.code_empty[slot]);
+                    if (++slot == SLOTS) slot = 0, round++;
+                }
+                if (!ok) break;
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(full);
+            }
+        }
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PT_OTHER_REGS));
+        if (warp == PT_PRODUCER) {
+            // --------------------------------------------------------- producer
+            const int page = a.kv.page_size, log_page = 31 - __clz(page), pages = max(PT_TILE >> log_page, 1);
+            PtItem item = pt_item<QUERIES>(a, sh.begin_item);
+            int index = sh.begin_item;
+            int unit = (begin - sh.begin_base) / item.tiles, tile = (begin - sh.begin_base) - unit * item.tiles;
+            int segs = 0, ahead = 0, left = 0, head = 0;
+            bool ok = true;
+            if (lane == 0) a.joins[8 * blockIdx.x] = 0;
+            struct Next {
+                int base, from, to, head, id;  // the tile's positions [from, to) that rows may see
+                float ks, vs;
+                bool wanted, bad;  // rows see this lane's page; its number is outside the pool
+            };
+            auto fetch = [&]() {
+                Next x;
+                x.base = x.from = x.to = x.head = x.id = 0;
+                x.ks = x.vs = 0.0f;
+                x.wanted = x.bad = false;
+                if (ahead >= count || !ok) return x;
+                if (left == 0) {
+                    // A new segment: the rest of the unit, or of the block's piece.
+                    const int n = min(item.tiles - tile, count - ahead);
+                    left = n;
+                    const int heads = a.kv.n_kv_heads, q_unit = a.reach.over_groups ? unit / heads : 0;
+                    head = unit - q_unit * heads;
+                    if (segs >= PT_SEGS)
+                        ok = __all_sync(0xffffffffu, mbar_wait(&sh.seg_free[segs % PT_SEGS], (segs / PT_SEGS - 1) & 1,
+                                                               abort_flag, a.err));
+                    if (!ok) return x;
+                    if (lane == 0) {
+                        PtSegment &g = sh.seg[segs % PT_SEGS];
+                        g.n = n;
+                        g.base = ahead;
+                        g.head = head;
+                        g.first = item.first;
+                        g.q0 = item.q0 + q_unit * QUERIES;
+                        g.nq = min(item.n * a.group - g.q0, QUERIES);
+                        g.pair = Shape::Q_TILES == 2 && g.nq > 128;
+                        g.last = ahead + n == count;
+                        g.p0 = item.p0;
+                        g.end = item.end;
+                        g.flat = a.reach.over_groups;
+                        g.part = -1;
+                        if (n < item.tiles) {
+                            const int from = begin + ahead - tile;  // the unit's place in the line
+                            const int c0 = from / per, c1 = (from + item.tiles - 1) / per;
+                            g.part = 2 * (int)blockIdx.x + (c0 == (int)blockIdx.x ? 1 : 0);
+                            if (c0 == (int)blockIdx.x) {
+                                int *j = a.joins + 8 * blockIdx.x;
+                                j[1] = g.first;
+                                j[2] = g.q0;
+                                j[3] = g.head;
+                                j[4] = c1;
+                                j[0] = g.nq;
+                            }
+                        }
+                        mbar_arrive(&sh.seg_full[segs % PT_SEGS]);
+                    }
+                    __syncwarp();
+                    segs++;
+                }
+                const bool early = tile < item.tf;
+                x.base = (early ? tile : item.t0 + tile - item.tf) * PT_TILE;
+                x.head = head;
+                // Of a shared beginning, the first tiles' positions are the leader's and end with it, and the others
+                // begin behind it.
+                x.from = item.shared > 0 && !early ? item.shared : 0;
+                x.to = item.shared > 0 && early ? min(item.shared, item.end) : item.end;
+                const int off = lane << log_page;
+                if (lane < pages && off < x.to - x.base) {
+                    const int begins = (x.base + off) >> log_page << log_page;  // of the page
+                    const bool seen = item.shared > 0 ? early || page > item.shared - begins
+                                                      : begins < a.reach.first || page > item.low - begins;
+                    if (seen) {
+                        x.wanted = true;
+                        x.id = a.batch.page_table[(item.shared > 0 && early ? item.leader : item.seq) * a.batch.table_stride +
+                                                  (begins >> log_page)];
+                    }
+                }
+                ahead++;
+                left--;
+                if (++tile == item.tiles) {
+                    tile = 0;
+                    if (++unit == item.units) {
+                        unit = 0;
+                        if (ahead < count) {
+                            do item = pt_item<QUERIES>(a, ++index);
+                            while (item.units == 0 && index < n_items - 1);
+                        }
+                    }
+                }
+                return x;
+            };
+            auto scales = [&](Next &x) {
+                if (!x.wanted) return;
+                x.bad = x.id < 0 || x.id >= a.kv.n_pages;
+                if (x.bad) return;
+                const int64_t at = (int64_t)x.id * a.kv.n_kv_heads + x.head;
+                x.ks = a.kv.k_scales[at];
+                x.vs = a.kv.v_scales[at];
+            };
+            int slot = 0, round = 0, issued = 0;
+            Next now = fetch(), next = fetch();
+            scales(now);
+            for (int k = 0; k < count && ok; k++) {
+                const Next later = fetch();
+                scales(next);
+                if (!ok) break;
+                if (round > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh.code_empty[slot], (round - 1) & 1, abort_flag, a.err));
+                if (!ok) break;
+                // The tile's scales.  A page number outside the pool, or a scale that is not finite,
+                // gives NaN to the rows that see the page, by their scores.
+                const bool load = now.wanted && !now.bad, sane = load && fabsf(now.vs) <= FLT_MAX;
+                if (now.bad) atomicOr(a.err, FO_DEVERR_PAGED);
+                const float ks = now.wanted && !sane ? NAN : now.ks, vs = sane ? now.vs : 0.0f;
+                const float most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(vs))));
+                PtMeta &meta = sh.meta[k % PT_METAS];
+                const unsigned mask = __ballot_sync(0xffffffffu, load);
+                // Eight entries of 16 positions each; a page larger than that has several.
+                const int shift = log_page - 4;
+                const float ks8 = __shfl_sync(0xffffffffu, ks, lane < 8 ? min(lane >> shift, 31) : 0);
+                const float vs8 = __shfl_sync(0xffffffffu, vs, lane < 8 ? min(lane >> shift, 31) : 0);
+                if (lane < 8) {
+                    meta.ks[lane] = ks8;
+                    meta.vs[lane] = vs8;
+                }
+                if (lane == 8) meta.top = pt_above(most);
+                if (lane == 9) meta.base = now.base;
+                if (lane == 10) meta.pages = mask;
+                if (lane == 11) meta.from = now.from, meta.to = now.to;
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.meta_full[k % PT_METAS]);
+#pragma unroll 1
+                for (int p = 0; p < 2 * PARTS; p++) {
+                    if (p > 0 && round > 0) {
+                        ok = __all_sync(0xffffffffu, mbar_wait(&sh.code_empty[slot], (round - 1) & 1, abort_flag, a.err));
+                        if (!ok) break;
+                    }
+                    // This slot's rows [h, h + 128 / PARTS) of the tile's.
+                    constexpr int ROWS = PT_TILE / PARTS;
+                    const int h = p % PARTS * ROWS, rows = min(page, ROWS);
+                    const int at = page > ROWS ? 0 : (lane << log_page) - h;  // of this lane's page in the slot
+                    const bool here = load && at >= 0 && at < ROWS;
+                    const uint32_t n_here = __popc(__ballot_sync(0xffffffffu, here));
+                    if (lane == 0) mbar_expect_tx(&sh.code_full[slot], n_here * (uint32_t)(rows * D));
+                    __syncwarp();
+                    if (here) {
+                        const uint8_t *codes = static_cast<const uint8_t *>(p < PARTS ? a.kv.k_codes : a.kv.v_codes);
+                        codes += (((int64_t)now.id * a.kv.n_kv_heads + now.head) * page + (page > ROWS ? h : 0)) * D;
+                        bulk_g2s(smem + Shape::OFF_CODES + slot * PT_SLOT + at * D, codes, rows * D, &sh.code_full[slot]);
+                    }
+                    __syncwarp();
+                    issued++;
+                    if (++slot == SLOTS) slot = 0, round++;
+                }
+                now = next;
+                next = later;
+            }
+            if (lane == 0) {
+                // The copies in flight land before the block ends, also where another warp gave up.
+                for (int i = max(issued - SLOTS, 0); i < issued; i++)
+                    mbar_wait_drain(&sh.code_full[i % SLOTS], (i / SLOTS) & 1);
+            }
+        } else if (warp == PT_ISSUER) {
+            // ----------------------------------------------------------- issuer
+            // The whole warp runs the loop and its waits, so that addresses stay
+            // uniform; one elected lane issues.
+            const uint32_t base = smem_u32(smem);
+            constexpr uint32_t ID_S = idesc_f16(128, 128, 0), ID_PV = idesc_f16(128, 64, 1);
+            const uint64_t dQ = sdesc_sw128(base, 16, 1024), dK = sdesc_sw128(base + Shape::OFF_K, 16, 1024);
+            const uint64_t dV = sdesc_sw128(base + Shape::OFF_V, PT_PANEL, 1024);
+            constexpr uint32_t OPERAND16 = Shape::OPERAND >> 4, PANEL16 = PT_PANEL >> 4;
+            auto issue_s = [&](int t, int q_buf, int q_tile, int k) {
+                if (elect_one()) {
+                    uint32_t more = 0;
+#pragma unroll
+                    for (int x = 0; x < TERMS; x++) {
+                        const uint64_t q = dQ + q_buf * (Shape::Q_BYTES >> 4) + (q_tile * TERMS + x) * OPERAND16;
+                        const uint64_t b = dK + (k & 1) * OPERAND16;
+#pragma unroll
+                        for (int kk = 0; kk < D / 16; kk++) {
+                            const uint32_t off = (kk >> 2) * PANEL16 + 2 * (kk & 3);
+                            mma_bf16(tmem + 128 * t, q + off, b + off, ID_S, more);
+                            more = 1;
+                        }
+                    }
+                    mma_commit(&sh.s_full[t]);
+                }
+                __syncwarp();
+            };
+            auto issue_pv = [&](int t, int k, bool first) {
+                if (elect_one()) {
+                    const uint32_t p = tmem + (ALIAS ? 128 * t : 384 + 64 * t);
+#pragma unroll
+                    for (int x = 0; x < TERMS; x++)
+#pragma unroll
+                        for (int panel = 0; panel < PANELS; panel++) {
+                            const uint64_t b = dV + (k & 1) * OPERAND16 + panel * PANEL16;
+                            const uint32_t o = tmem + 256 + (ALIAS ? 128 : 64) * t + 64 * panel;
+#pragma unroll
+                            for (int kk = 0; kk < 8; kk++)
+                                mma_bf16_ts(o, p + 64 * x + 8 * kk, b + kk * (2048 >> 4), ID_PV, x > 0 || kk > 0 || !first);
+                        }
+                    mma_commit(&sh.o_full[t]);
+                }
+                __syncwarp();
+            };
+            auto commit = [&](uint64_t *bar) {
+                if (elect_one()) mma_commit(bar);
+                __syncwarp();
+            };
+            // A stream's place in the block's segments: the next tile of its own.
+            struct Place {
+                int seg, i, n, base, pair;
+                bool last, over;
+            };
+            auto enter = [&](Place &x, int t) {
+                while (x.i >= x.n) {
+                    if (x.last) {
+                        x.over = true;
+                        return false;
+                    }
+                    const int s = x.seg + 1;
+                    if (!__all_sync(0xffffffffu, mbar_test(&sh.seg_full[s % PT_SEGS], (s / PT_SEGS) & 1))) return false;
+                    const PtSegment &g = sh.seg[s % PT_SEGS];
+                    x.seg = s;
+                    x.n = g.n;
+                    x.base = g.base;
+                    x.pair = g.pair;
+                    x.last = g.last;
+                    x.i = x.pair ? 0 : t;
+                }
+                return true;
+            };
+            // Tiles that the stream is past.
+            auto past = [](const Place &x) { return x.base + min(x.i, x.n); };
+            Place ps[2], pv[2];
+#pragma unroll
+            for (int t = 0; t < 2; t++) ps[t] = pv[t] = {-1, 0, 0, 0, 0, false, false};
+            int ns[2] = {0, 0}, np[2] = {0, 0}, q_freed = 0, s_freed = 0;
+            // Tiles and segments whose operands are there, counted in order: a stream skips what is
+            // the other's alone, and a parity test cannot tell a phase from the one two before.
+            int k_there = 0, v_there = 0, q_there = 0;
+            auto count_up = [](int &there, uint64_t *full, int bufs) {
+                if (__all_sync(0xffffffffu, mbar_test(full + there % bufs, (there / bufs) & 1))) there++;
+            };
+            bool ok = true;
+            uint64_t t_last = globaltimer();
+            while (ok && !(pv[0].over && pv[1].over)) {
+                bool progress = false;
+                if (k_there < count) count_up(k_there, sh.k_full, 2);
+                if (v_there < k_there) count_up(v_there, sh.v_full, 2);
+                if (q_there < q_freed + Q_BUFS) count_up(q_there, sh.q_full, Q_BUFS);
+#pragma unroll
+                for (int t = 0; t < 2; t++) {
+                    Place &x = ps[t], &y = pv[t];
+                    if (!x.over && enter(x, t)) {
+                        const int k = x.base + x.i, s = x.seg;
+                        bool ready = k < k_there && s < q_there;
+                        if (ns[t] > 0) {
+                            if constexpr (ALIAS) ready = ready && np[t] == ns[t] && mbar_test(&sh.o_full[t], (ns[t] - 1) & 1);
+                            else ready = ready && mbar_test(&sh.s_read[t], (ns[t] - 1) & 1);
+                        }
+                        if (__all_sync(0xffffffffu, ready)) {
+                            tc_fence_after();
+                            issue_s(t, s % Q_BUFS, x.pair ? t : 0, k);
+                            ns[t]++;
+                            x.i += x.pair ? 1 : 2;
+                            // The last stream to want K(k) releases it.
+                            if (!x.pair || past(ps[t ^ 1]) > k) commit(&sh.k_empty[k & 1]);
+                            progress = true;
+                        }
+                    }
+                    if (!y.over && enter(y, t)) {
+                        const int k = y.base + y.i;
+                        const bool ready = k < v_there && np[t] < ns[t] && mbar_test(&sh.p_full[t], np[t] & 1);
+                        if (__all_sync(0xffffffffu, ready)) {
+                            tc_fence_after();
+                            issue_pv(t, k, y.i < (y.pair ? 1 : 2));
+                            np[t]++;
+                            y.i += y.pair ? 1 : 2;
+                            if (!y.pair || past(pv[t ^ 1]) > k) commit(&sh.v_empty[k & 1]);
+                            progress = true;
+                        }
+                    }
+                }
+                // Queries that both streams are done with, and segments.
+                auto behind = [](const Place &x, int s) { return x.seg > s || (x.seg == s && x.i >= x.n); };
+                if (behind(ps[0], q_freed) && behind(ps[1], q_freed)) {
+                    commit(&sh.q_free[q_freed % Q_BUFS]);
+                    q_freed++;
+                }
+                if (pv[0].seg > s_freed && pv[1].seg > s_freed) {
+                    if (lane == 0) mbar_arrive(&sh.seg_free[s_freed % PT_SEGS]);
+                    __syncwarp();
+                    s_freed++;
+                }
+                if (progress) {
+                    t_last = globaltimer();
+                } else if (globaltimer() - t_last > FO_WAIT_NS || *abort_flag) {
+                    if (lane == 0 && !*abort_flag) {
+                        *abort_flag = 1;
+                        atomicOr(a.err, FO_DEVERR_WAIT_TIMEOUT);
+                    }
+                    ok = false;
+                }
+                ok = __shfl_sync(0xffffffffu, ok, 0);
+            }
+            // Every issued MMA completes before tensor memory is released.
+            commit(&sh.done);
+            if (lane == 0) mbar_wait_drain(&sh.done, 0);
+            __syncwarp();
+        } else {
+            // ---------------------------------------------------------- queries
+            const int ql = tid - 32 * PT_LOADER;
+            bool ok = true;
+            for (int s = 0; ok; s++) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&sh.seg_full[s % PT_SEGS], (s / PT_SEGS) & 1, abort_flag, a.err));
+                if (!ok) break;
+                const PtSegment seg = sh.seg[s % PT_SEGS];
+                const int buf = s % Q_BUFS;
+                if (s >= Q_BUFS)
+                    ok = __all_sync(0xffffffffu, mbar_wait(&sh.q_free[buf], (s / Q_BUFS - 1) & 1, abort_flag, a.err));
+                if (!ok) break;
+#pragma unroll 1
+                for (int q = ql; q < (seg.pair ? 256 : 128); q += 32 * PT_LOADERS) {
+                    uint8_t *to = smem + buf * Shape::Q_BYTES + (q >> 7) * TERMS * Shape::OPERAND + (q & 127) * 128;
+                    const int swizzle = q & 7;
+                    const bool mine = q < seg.nq;
+                    const T *from = nullptr;
+                    float inv0 = 1.0f, inv1 = 1.0f, scale = 0.0f;
+                    int high = INT32_MAX, low = 0;  // rows that are none's see everything, and are not kept
+                    if (mine) {
+                        const int qi = seg.q0 + q, r = qi / a.group;
+                        const int64_t row = seg.first + r;
+                        from = static_cast<const T *>(a.q.data) + row * a.q.row_stride +
+                               (seg.head * a.group + qi - r * a.group) * a.q.head_stride;
+                        if (seg.flat) {
+                            high = min(place_of_row(a.batch, a.kv.page_size, (int)row, a.err), seg.end - 1);
+                        } else {
+                            high = max(seg.p0 + r, -1);
+                            low = a.window > 0 ? max(high + 1 - a.window, 0) : 0;
+                        }
+                        float top = 0.0f;
+                        bool finite = true;
+#pragma unroll 4
+                        for (int d = 0; d < D; d += 8) {
+                            float x[8];
+                            if (a.q_vec) {
+                                load8(from + d, x);
+                            } else {
+#pragma unroll
+                                for (int e = 0; e < 8; e++) x[e] = load1(from + d + e);
+                            }
+#pragma unroll
+                            for (int e = 0; e < 8; e++) {
+                                top = fmaxf(top, fabsf(x[e]));
+                                finite &= fabsf(x[e]) <= FLT_MAX;
+                            }
+                        }
+                        // A power of two brings the largest element to [2^14, 2^15), in two factors, so
+                        // that FP32's whole range of exponents can be brought there.
+                        const int e = max((int)(__float_as_uint(top) >> 23), 1);
+                        inv0 = __uint_as_float((uint32_t)(254 - (e + 1) / 2 - 63) << 23);
+                        inv1 = __uint_as_float((uint32_t)(254 - (e - (e + 1) / 2) - 64) << 23) * 16384.0f;
+                        scale = finite ? __uint_as_float((uint32_t)e << 23) * (1.0f / 16384.0f) * a.scale * REACH_LOG2E : NAN;
+                        if (!finite) inv0 = 0.0f;
+                    }
+                    sh.q_scale[buf][q] = scale;
+                    sh.q_high[buf][q] = high;
+                    sh.q_low[buf][q] = low;
+#pragma unroll 2
+                    for (int d = 0; d < D; d += 8) {
+                        float x[8];
+                        if (!mine || inv0 == 0.0f) {
+#pragma unroll
+                            for (int e = 0; e < 8; e++) x[e] = 0.0f;
+                        } else if (a.q_vec) {
+                            load8(from + d, x);
+                        } else {
+#pragma unroll
+                            for (int e = 0; e < 8; e++) x[e] = load1(from + d + e);
+                        }
+#pragma unroll
+                        for (int e = 0; e < 8; e++) x[e] = x[e] * inv0 * inv1;
+                        const int place = (d >> 6) * PT_PANEL + (((d >> 3 & 7) ^ swizzle) << 4);
+#pragma unroll
+                        for (int term = 0; term < TERMS; term++) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                w[e] = pt_f16x2(x[2 * e], x[2 * e + 1]);
+                                const float2 b = f16x2_f32x2(w[e]);
+                                x[2 * e] -= b.x;
+                                x[2 * e + 1] -= b.y;
+                            }
+                            *reinterpret_cast<uint4 *>(to + term * Shape::OPERAND + place) = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                    }
+                }
+                fence_proxy_async_smem();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&sh.q_full[buf]);
+                    mbar_arrive(&sh.seg_free[s % PT_SEGS]);
+                }
+                if (seg.last) break;
+            }
+        }
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == PT_ISSUER) tmem_dealloc(tmem, 512);
+}
+
+// ------------------------------------------------------------- the joining
+// The parts of the unit that begins in block blockIdx.x and goes on in others, in
+// the blocks' order: 32 of its queries, four dimensions to a thread.
+constexpr int PJ_QUERIES = 32, PJ_THREADS = 256;
+template <int D, bool F32>
+__global__ void __launch_bounds__(PJ_THREADS) paged_join_kernel(const __grid_constant__ fo_paged_tiles_launch a) {
+    using T = typename std::conditional<F32, float, uint16_t>::type;
+    wait_for_prior_kernel();
+    const int c0 = blockIdx.x;
+    const int4 j0 = __ldcg(reinterpret_cast<const int4 *>(a.joins) + 2 * c0);
+    const int nq = j0.x, q = blockIdx.y * PJ_QUERIES + (threadIdx.x & 31);
+    if (blockIdx.y * PJ_QUERIES >= nq || q >= nq) return;
+    const int first = j0.y, qi = j0.z + q, head = j0.w, c1 = __ldcg(a.joins + 8 * c0 + 4);
+    const int r = qi / a.group, h = head * a.group + qi - r * a.group;
+    const int64_t row = first + r, at_row = row * a.q.heads + h;
+    const float2 *mls = reinterpret_cast<const float2 *>(a.part_ml);
+    auto part = [&](int c) { return (int64_t)(2 * c + (c == c0 ? 1 : 0)); };
+    float2 prior = make_float2(-INFINITY, 0.0f);
+    if (a.reach.prior_o) prior = reinterpret_cast<const float2 *>(a.reach.prior_ml)[at_row];
+    float m = prior.x;
+#pragma unroll 4
+    for (int c = c0; c <= c1; c++) m = fmaxf(m, __ldcg(mls + part(c) * FO_TILES_QUERIES + q).x);
+    const float shift = m == -INFINITY ? 0.0f : m, fp = exp2f(prior.x - shift);
+    constexpr int QUADS = D / 4, STEP = PJ_THREADS / 32, MINE = QUADS / STEP;
+    const int quad0 = threadIdx.x >> 5;
+    float l = prior.y * fp;
+    float4 v[MINE];
+#pragma unroll
+    for (int i = 0; i < MINE; i++) {
+        v[i] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (a.reach.prior_o) {
+            const float4 y = __ldcg(reinterpret_cast<const float4 *>(a.reach.prior_o + at_row * D) + quad0 + STEP * i);
+            v[i] = make_float4(y.x * fp, y.y * fp, y.z * fp, y.w * fp);
+        }
+    }
+#pragma unroll 4
+    for (int c = c0; c <= c1; c++) {
+        const float2 ml = __ldcg(mls + part(c) * FO_TILES_QUERIES + q);
+        const float f = exp2f(ml.x - shift);
+        l = fmaf(ml.y, f, l);
+#pragma unroll
+        for (int i = 0; i < MINE; i++) {
+            const float4 y = __ldcg(reinterpret_cast<const float4 *>(a.part_o) +
+                                    (part(c) * QUADS + quad0 + STEP * i) * FO_TILES_QUERIES + q);
+            v[i] = make_float4(fmaf(y.x, f, v[i].x), fmaf(y.y, f, v[i].y), fmaf(y.z, f, v[i].z), fmaf(y.w, f, v[i].w));
+        }
+    }
+    if (a.reach.raw_o) {
+#pragma unroll
+        for (int i = 0; i < MINE; i++)
+            reinterpret_cast<float4 *>(a.reach.raw_o + at_row * D)[quad0 + STEP * i] = v[i];
+        if (quad0 == 0) reinterpret_cast<float2 *>(a.reach.raw_ml)[at_row] = make_float2(m, l);
+        return;
+    }
+    const float inv = inverse_sum(a.sinks, h, m, l);
+    T *out = static_cast<T *>(a.out.data) + row * a.out.row_stride + h * a.out.head_stride;
+#pragma unroll
+    for (int i = 0; i < MINE; i++) {
+        T *to = out + 4 * (quad0 + STEP * i);
+        const float4 y = make_float4(v[i].x * inv, v[i].y * inv, v[i].z * inv, v[i].w * inv);
+        if (!a.out_vec) {
+            store1(to, y.x);
+            store1(to + 1, y.y);
+            store1(to + 2, y.z);
+            store1(to + 3, y.w);
+        } else if constexpr (F32) {
+            *reinterpret_cast<float4 *>(to) = y;
+        } else {
+            *reinterpret_cast<uint2 *>(to) = make_uint2(bf16_pair(y.x, y.y), bf16_pair(y.z, y.w));
+        }
+    }
+    if (a.lse && quad0 == 0) a.lse[at_row] = log_sum(m, l);
+}
+
+template <int D, int FORMAT, bool F32>
+cudaError_t launch_tiles(const fo_paged_tiles_launch &in, int sms, cudaStream_t stream) {
+    fo_paged_tiles_launch a = in;
+    using Shape = PtShape<D, F32>;
+    static_assert(Shape::SMEM + sizeof(PtShared<D, F32>) <= 227 * 1024, "shared memory");
+    auto *kernel = paged_tiles_kernel<D, FORMAT, F32>;
+    // The attribute belongs to each device's context: set once per device.
+    static std::atomic<unsigned long long> configured{0};
+    int dev = 0;
+    cudaGetDevice(&dev);
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (!(configured.load() & bit)) {
+        cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::SMEM);
+        if (e != cudaSuccess) return e;
+        // The kernel's register split is only sound at the launch count that it
+        // was written for.
+        cudaFuncAttributes f;
+        e = cudaFuncGetAttributes(&f, kernel);
+        if (e != cudaSuccess) return e;
+        if (f.numRegs != PT_LAUNCH_REGS) return cudaErrorInvalidConfiguration;
+        configured.fetch_or(bit);
+    }
+    // No more blocks than the most tiles there can be for, two to a block.
+    const int64_t table = (a.batch.table_stride * a.kv.page_size + PT_TILE - 1) / PT_TILE;
+    const int64_t units = a.reach.over_groups
+                              ? (a.batch.total_rows * a.group + Shape::QUERIES - 1) / Shape::QUERIES + a.reach.n_groups + 2
+                              : a.batch.n_seqs * ((a.batch.max_rows * a.group + Shape::QUERIES - 1) / Shape::QUERIES);
+    const int64_t most = units * a.kv.n_kv_heads * table;
+    a.q_units = (int)((a.batch.max_rows * a.group + Shape::QUERIES - 1) / Shape::QUERIES);
+    const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(sms, (most + 1) / 2));
+    cudaError_t e = launch(kernel, dim3(grid), dim3(PT_THREADS), Shape::SMEM, stream, a);
+    if (e != cudaSuccess || grid == 1) return e;
+    return launch(paged_join_kernel<D, F32>, dim3(grid, Shape::QUERIES / PJ_QUERIES), dim3(PJ_THREADS), 0, stream, a);
+}
+
+template <int D>
+cudaError_t launch_tiles(const fo_paged_tiles_launch &a, int sms, cudaStream_t stream) {
+    if (a.q.dtype == FO_DT_F32)
+        return a.kv.format == FO_PAGED_I8 ? launch_tiles<D, FO_PAGED_I8, true>(a, sms, stream)
+                                          : launch_tiles<D, FO_PAGED_E4M3, true>(a, sms, stream);
+    return a.kv.format == FO_PAGED_I8 ? launch_tiles<D, FO_PAGED_I8, false>(a, sms, stream)
+                                      : launch_tiles<D, FO_PAGED_E4M3, false>(a, sms, stream);
+}
+
+}  // namespace fo
+
+extern "C" cudaError_t fo_launch_paged_tiles(const fo_paged_tiles_launch *args, int sms, cudaStream_t stream) {
+    fo_paged_tiles_launch a = *args;
+    if (a.batch.total_rows <= 0) return cudaSuccess;
+    a.group = a.q.heads / a.kv.n_kv_heads;
+    auto aligned = [](const fo_rows &r) {
+        const int64_t unit = r.dtype == FO_DT_F32 ? 4 : 8;  // elements in 16 bytes
+        return reinterpret_cast<uintptr_t>(r.data) % 16 == 0 && r.row_stride % unit == 0 && r.head_stride % unit == 0;
+    };
+    a.q_vec = aligned(a.q);
+    a.out_vec = aligned(a.out);
+    return a.kv.head_dim == 64 ? fo::launch_tiles<64>(a, sms, stream) : fo::launch_tiles<128>(a, sms, stream);
+}

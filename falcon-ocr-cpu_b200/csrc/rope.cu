@@ -42,13 +42,20 @@ __global__ void __launch_bounds__(256) rope_table_kernel(float2 *table, int64_t 
     }
 }
 
-template <typename T, bool HALF, bool VEC>
+template <typename T, bool HALF, bool VEC, bool AXES>
 __global__ void __launch_bounds__(ROPE_THREADS, 3) rope_kernel(const __grid_constant__ fo_rope_launch a) {
     wait_for_prior_kernel();
-    rope_block<T, HALF, VEC>(a, blockIdx.x, threadIdx.x, [&](int64_t row, bool &padded) {
+    rope_block<T, HALF, VEC, AXES>(a, blockIdx.x, threadIdx.x, [&](int64_t row, bool &padded) {
         padded = false;
         return a.rope.row_positions ? (int64_t)a.rope.row_positions[row] : row;
     });
+}
+
+template <typename T, bool AXES>
+cudaError_t launch_rope(const fo_rope_launch &a, unsigned grid, bool half, bool vec, cudaStream_t stream) {
+    auto go = [&](auto *kernel) { return launch(kernel, grid, ROPE_THREADS, 0, stream, a); };
+    if (half) return vec ? go(rope_kernel<T, true, true, AXES>) : go(rope_kernel<T, true, false, AXES>);
+    return vec ? go(rope_kernel<T, false, true, AXES>) : go(rope_kernel<T, false, false, AXES>);
 }
 
 }  // namespace fo
@@ -68,16 +75,11 @@ extern "C" cudaError_t fo_launch_rope(const fo_rope_launch *args, cudaStream_t s
     fo_rope_launch a = *args;
     const bool vec = fo::rope_shape(&a);
     const int rows = fo::ROPE_THREADS / a.block_x;
-    const unsigned grid = (unsigned)((a.rows + rows - 1) / rows), block = fo::ROPE_THREADS;
-    const bool half = a.rope.layout == FO_ROPE_HALF;
-    cudaError_t e = cudaSuccess;
-    auto go = [&](auto *kernel) { e = fo::launch(kernel, grid, block, 0, stream, a); };
-    if (a.x.dtype == FO_DT_F32) {
-        if (half) vec ? go(fo::rope_kernel<float, true, true>) : go(fo::rope_kernel<float, true, false>);
-        else vec ? go(fo::rope_kernel<float, false, true>) : go(fo::rope_kernel<float, false, false>);
-    } else {
-        if (half) vec ? go(fo::rope_kernel<uint16_t, true, true>) : go(fo::rope_kernel<uint16_t, true, false>);
-        else vec ? go(fo::rope_kernel<uint16_t, false, true>) : go(fo::rope_kernel<uint16_t, false, false>);
-    }
-    return e;
+    const unsigned grid = (unsigned)((a.rows + rows - 1) / rows);
+    const bool half = a.rope.layout == FO_ROPE_HALF, f32 = a.x.dtype == FO_DT_F32;
+    if (a.axes.used)
+        return f32 ? fo::launch_rope<float, true>(a, grid, half, vec, stream)
+                   : fo::launch_rope<uint16_t, true>(a, grid, half, vec, stream);
+    return f32 ? fo::launch_rope<float, false>(a, grid, half, vec, stream)
+               : fo::launch_rope<uint16_t, false>(a, grid, half, vec, stream);
 }

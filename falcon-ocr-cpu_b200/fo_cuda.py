@@ -4,8 +4,10 @@ reference's attention operator interface for tests and benchmarks:
 * ``attention_with``          kernels::attention_with (src/kernels/attention/mod.rs:256-311)
 * ``attention_prefill_bf16``  kernels::attention_prefill_bf16 (mod.rs:321-349)
 * ``rope``, ``PagedKv``, ``paged_append``, ``paged_attention``  rotary positions
-  and a paged 8-bit cache for many sequences (no counterpart); without ``ctx``
-  these run on torch's current stream
+  and a paged 8-bit cache for many sequences (no counterpart); ``RopeAxes``
+  positions on several axes, ``paged_window_attention`` windows with first
+  positions and prompts, ``paged_prefix_attention`` shared beginnings; without
+  ``ctx`` these run on torch's current stream
 * ``SplitPrefix``             quant::kv::SplitPrefix (src/quant/kv.rs:155-972):
   ``from_compact``, ``append``, ``truncate_tail``, ``tail_len``, ``bytes``,
   ``attention_decode``, ``attention_decode_rows``; ``decode_batch`` for pages.
@@ -103,6 +105,7 @@ class Rows(ctypes.Structure):
 
 _PACK_ROWS = struct.Struct("=QqqiI").pack  # Rows and RopeSpec as bytes: a third of a Structure's time
 _PACK_ROPE = struct.Struct("=QqQii").pack
+_PACK_AXES = struct.Struct("=QqQqqiii128s4x").pack  # RopeAxesSpec
 
 
 class RopeScaling(ctypes.Structure):
@@ -118,6 +121,13 @@ class RopeSpec(ctypes.Structure):
                 ("rot_dim", ctypes.c_int32), ("layout", ctypes.c_int32)]
 
 
+class RopeAxesSpec(ctypes.Structure):
+    """fo_rope_axes"""
+    _fields_ = [("table", ctypes.c_void_p), ("positions", ctypes.c_int64), ("row_positions", ctypes.c_void_p),
+                ("row_stride", ctypes.c_int64), ("axis_stride", ctypes.c_int64), ("rot_dim", ctypes.c_int32),
+                ("layout", ctypes.c_int32), ("n_axes", ctypes.c_int32), ("pair_axis", ctypes.c_uint8 * 128)]
+
+
 class PagedPool(ctypes.Structure):
     """fo_paged_kv"""
     _fields_ = [("k_codes", ctypes.c_void_p), ("v_codes", ctypes.c_void_p), ("k_scales", ctypes.c_void_p),
@@ -130,6 +140,11 @@ class PagedSequences(ctypes.Structure):
     _fields_ = [("page_table", ctypes.c_void_p), ("lens", ctypes.c_void_p), ("row_start", ctypes.c_void_p),
                 ("table_stride", ctypes.c_int64), ("n_seqs", ctypes.c_int64), ("max_rows", ctypes.c_int64),
                 ("total_rows", ctypes.c_int64)]
+
+
+class PagedPrefixes(ctypes.Structure):
+    """fo_paged_groups"""
+    _fields_ = [("seq_start", ctypes.c_void_p), ("lens", ctypes.c_void_p), ("n_groups", ctypes.c_int64)]
 
 
 ROPE_LAYOUTS = {"interleaved": 0, "half": 1}
@@ -150,7 +165,8 @@ EXPORTS = [
     "fo_i8_decode_batch", "fo_draft_kv_create", "fo_draft_kv_destroy", "fo_draft_kv_push", "fo_draft_kv_len",
     "fo_draft_kv_bytes", "fo_draft_kv_records", "fo_draft_attend", "fo_peer_block_register",
     "fo_peer_block_destroy", "fo_sharded_prefill_bf16_peers", "fo_rope_table", "fo_rope", "fo_paged_append",
-    "fo_paged_attention",
+    "fo_paged_attention", "fo_rope_by_axes", "fo_paged_append_by_axes", "fo_paged_window_attention",
+    "fo_paged_prefix_attention",
 ]
 
 _lib: Optional[ctypes.CDLL] = None
@@ -227,6 +243,10 @@ def lib() -> ctypes.CDLL:
         "fo_rope": (I, [P, P, P, I64, I32, P, I32]),
         "fo_paged_append": (I, [P, P, P, P, P, P, P, P]),
         "fo_paged_attention": (I, [P, P, P, P, P, ctypes.c_float, I64, P, P]),
+        "fo_rope_by_axes": (I, [P, P, P, I64, I32, P, I32]),
+        "fo_paged_append_by_axes": (I, [P, P, P, P, P, P, P, P]),
+        "fo_paged_window_attention": (I, [P, P, P, P, P, ctypes.c_float, I64, I64, P, P]),
+        "fo_paged_prefix_attention": (I, [P, P, P, P, P, P, ctypes.c_float, P, P]),
     }
     for name, (res, args) in sigs.items():
         fn = getattr(L, name)
@@ -809,6 +829,8 @@ def rope_table(table, theta=10000.0, scaling="none", factor=1.0, original_positi
 class Rope:
     """A rope table and the layout of the pairs that it turns."""
 
+    rope_call, append_call = "fo_rope", "fo_paged_append"
+
     def __init__(self, table, layout="interleaved"):
         if not _on_device(table) or not table.is_contiguous() or table.dim() != 3 or table.shape[2] != 2 or \
                 str(table.dtype) != "torch.float32":
@@ -828,10 +850,40 @@ class Rope:
         return _PACK_ROPE(table, n, _device_ints(positions, "positions", device), rot_dim, layout)
 
 
+class RopeAxes(Rope):
+    """A rope table whose pairs turn by positions on several axes (time, height
+    and width, say): `axes` names each of the rot_dim / 2 pairs' axis, 0 to 3.
+    Calls with it want `positions` [axes][rows] int32, in any strides."""
+
+    rope_call, append_call = "fo_rope_by_axes", "fo_paged_append_by_axes"
+
+    def __init__(self, table, axes, layout="interleaved"):
+        super().__init__(table, layout)
+        axes = [int(a) for a in axes]
+        if len(axes) != table.shape[1] or len(axes) > 128 or min(axes) < 0 or max(axes) > 3:
+            raise FoError("rope axes: an axis of 0 to 3 for each pair of the table, 128 pairs at most")
+        self.n_axes, self.pair_axis = max(axes) + 1, bytes(axes)
+
+    def at(self, positions, rows: int, device: int) -> bytes:
+        if self.device != device:
+            raise FoError(f"the rope table is on GPU {self.device}, the call on GPU {device}")
+        if positions is None or positions.dim() != 2 or positions.shape[0] < self.n_axes or positions.shape[1] != rows:
+            raise FoError("positions on axes must be [axes][rows]")
+        if not positions.is_cuda or positions.dtype != _torch().int32:
+            raise FoError("positions must be a CUDA tensor of int32")
+        if positions.get_device() != device:
+            raise FoError(f"positions is on GPU {positions.get_device()}, the call on GPU {device}")
+        table, n, rot_dim, layout = self.spec
+        axis_stride, row_stride = positions.stride()
+        return _PACK_AXES(table, n, positions.data_ptr(), row_stride, axis_stride, rot_dim, layout, self.n_axes,
+                          self.pair_axis)
+
+
 def rope(x, out, rope: Rope, positions=None, inverse=False, ctx=None):
     """fo_rope: rows x [rows][heads][head_dim] rotated into `out` (x itself is
-    allowed) at `positions` [rows] int32 (None: the row's number).  inverse:
-    the transposed rotation, which takes a gradient back."""
+    allowed) at `positions` [rows] int32 (None: the row's number), or with a
+    RopeAxes (fo_rope_by_axes) at `positions` [axes][rows].  inverse: the
+    transposed rotation, which takes a gradient back."""
     device = x.get_device()
     a, b = _rows(x, "x", device), _rows(out, "out", device)
     shape = x.shape
@@ -839,7 +891,8 @@ def rope(x, out, rope: Rope, positions=None, inverse=False, ctx=None):
         raise FoError("rope: x and out must have one shape")
     rows, _, dim = shape
     ctx = _context(ctx, device)
-    check(lib().fo_rope(ctx.handle, a, b, rows, dim, rope.at(positions, rows, device), 1 if inverse else 0))
+    call = getattr(lib(), rope.rope_call)
+    check(call(ctx.handle, a, b, rows, dim, rope.at(positions, rows, device), 1 if inverse else 0))
     return out
 
 
@@ -912,7 +965,8 @@ def paged_append(kv: PagedKv, batch: PagedBatch, k, v, rope: Optional[Rope] = No
                  q_out=None, ctx=None):
     """fo_paged_append: rows k, v [rows][kv heads][head dim] into the batch's
     pages, keys rotated on the way when `rope` is given (at `positions`, else
-    at their place in the cache), and queries q rotated into q_out."""
+    at their place in the cache; with a RopeAxes, fo_paged_append_by_axes, at
+    `positions` [axes][rows]), and queries q rotated into q_out."""
     device = _paged_device(kv, batch)
     rk, rv = _rows(k, "k", device), _rows(v, "v", device)
     rows, _, dim = shape = k.shape
@@ -927,8 +981,9 @@ def paged_append(kv: PagedKv, batch: PagedBatch, k, v, rope: Optional[Rope] = No
     if rope is None and positions is not None:
         raise FoError("paged_append: positions are the rotation's, without rope there is nothing to do with them")
     ctx = _context(ctx, device)
-    check(lib().fo_paged_append(ctx.handle, kv.ref, batch.of(rows), rk, rv, rq, ro,
-                                None if rope is None else rope.at(positions, rows, device)))
+    call = getattr(lib(), "fo_paged_append" if rope is None else rope.append_call)
+    check(call(ctx.handle, kv.ref, batch.of(rows), rk, rv, rq, ro,
+               None if rope is None else rope.at(positions, rows, device)))
 
 
 def paged_attention(kv: PagedKv, batch: PagedBatch, q, out, sinks=None, scale=None, window=0, lse=None, ctx=None):
@@ -944,6 +999,59 @@ def paged_attention(kv: PagedKv, batch: PagedBatch, q, out, sinks=None, scale=No
                                    None if sinks is None else _floats(sinks, heads, "sinks", device),
                                    kv.scale if scale is None else scale, window, ro,
                                    None if lse is None else _floats(lse, rows * heads, "lse", device)))
+    return out
+
+
+def paged_window_attention(kv: PagedKv, batch: PagedBatch, q, out, window=0, first=0, sinks=None, scale=None,
+                           lse=None, ctx=None):
+    """fo_paged_window_attention: as paged_attention, for any number of rows
+    (a prompt's too), over the newest `window` positions (0: all) and the
+    `first` ones, which stay in sight behind them."""
+    device = _paged_device(kv, batch)
+    rq, ro = _rows(q, "q", device), _rows(out, "out", device)
+    rows, heads, dim = shape = q.shape
+    if dim != kv.head_dim or out.shape != shape:
+        raise FoError("paged_window_attention: q and out must be [rows][heads][head dim] of the cache's width")
+    ctx = _context(ctx, device)
+    check(lib().fo_paged_window_attention(ctx.handle, kv.ref, batch.of(rows), rq,
+                                          None if sinks is None else _floats(sinks, heads, "sinks", device),
+                                          kv.scale if scale is None else scale, window, first, ro,
+                                          None if lse is None else _floats(lse, rows * heads, "lse", device)))
+    return out
+
+
+class PagedGroups:
+    """Groups of a batch's sequences that share their beginnings
+    (fo_paged_groups): seq_start [groups + 1] and lens [groups] int32.  Group
+    g's sequences seq_start[g] .. seq_start[g + 1] - 1 have their positions
+    below lens[g] in the pages of the first of them.  The tensors are the
+    caller's and may change between calls."""
+
+    def __init__(self, seq_start, lens):
+        if seq_start.numel() != lens.numel() + 1:
+            raise FoError("seq_start must have one entry more than there are groups")
+        self.keep, self.device = (seq_start, lens), lens.get_device()
+        self.groups = PagedPrefixes(_device_ints(seq_start, "seq_start", self.device),
+                                    _device_ints(lens, "lens", self.device), lens.numel())
+        self.ref = ctypes.byref(self.groups)
+
+
+def paged_prefix_attention(kv: PagedKv, batch: PagedBatch, groups: PagedGroups, q, out, sinks=None, scale=None,
+                           lse=None, ctx=None):
+    """fo_paged_prefix_attention: paged_attention of sequences whose groups
+    share their beginnings, which are read once for a group."""
+    device = _paged_device(kv, batch)
+    if groups.device != device:
+        raise FoError(f"the groups are on GPU {groups.device}, the call on GPU {device}")
+    rq, ro = _rows(q, "q", device), _rows(out, "out", device)
+    rows, heads, dim = shape = q.shape
+    if dim != kv.head_dim or out.shape != shape:
+        raise FoError("paged_prefix_attention: q and out must be [rows][heads][head dim] of the cache's width")
+    ctx = _context(ctx, device)
+    check(lib().fo_paged_prefix_attention(ctx.handle, kv.ref, batch.of(rows), groups.ref, rq,
+                                          None if sinks is None else _floats(sinks, heads, "sinks", device),
+                                          kv.scale if scale is None else scale, ro,
+                                          None if lse is None else _floats(lse, rows * heads, "lse", device)))
     return out
 
 

@@ -526,6 +526,28 @@ int fo_rope_table(fo_ctx *ctx, float *table, int64_t positions, int32_t rot_dim,
 int fo_rope(fo_ctx *ctx, const fo_rows *x, const fo_rows *out, int64_t rows, int32_t head_dim,
             const fo_rope_spec *rope, int32_t transpose);
 
+/* Rotary positions on several axes (time, height and width of an image's or a
+ * video's tokens): pair i of a head turns by its own axis's position, and text
+ * stands at one position on all of them.  The table has an entry for every
+ * position and pair, as fo_rope_table fills it (or the caller, where an axis's
+ * frequencies are its own). */
+#define FO_ROPE_MAX_AXES 4
+typedef struct {
+    const float *table;           /* [positions][rot_dim / 2]{cos, sin} */
+    int64_t positions;
+    const int32_t *row_positions; /* row r's position on axis a at [r * row_stride + a * axis_stride] */
+    int64_t row_stride, axis_stride;
+    int32_t rot_dim;              /* even, at most the head's width and 256 */
+    int32_t layout;               /* FO_ROPE_INTERLEAVED | FO_ROPE_HALF */
+    int32_t n_axes;               /* 1 .. FO_ROPE_MAX_AXES */
+    uint8_t pair_axis[128];       /* the axis of each of the rot_dim / 2 pairs */
+} fo_rope_axes;
+
+/* fo_rope with positions on several axes.  A pair whose axis's position lies
+ * outside the table becomes NaN, and the error word says so. */
+int fo_rope_by_axes(fo_ctx *ctx, const fo_rows *x, const fo_rows *out, int64_t rows, int32_t head_dim,
+                    const fo_rope_axes *rope, int32_t transpose);
+
 #define FO_PAGED_I8 0   /* codes -127..127 */
 #define FO_PAGED_E4M3 1 /* FP8 e4m3, finite codes only */
 
@@ -574,6 +596,11 @@ typedef struct {
 int fo_paged_append(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch *batch, const fo_rows *k,
                     const fo_rows *v, const fo_rows *q, const fo_rows *q_out, const fo_rope_spec *rope);
 
+/* fo_paged_append with positions on several axes, of every row of the call
+ * (they say how rows are rotated; where they are stored goes by the batch). */
+int fo_paged_append_by_axes(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch *batch, const fo_rows *k,
+                            const fo_rows *v, const fo_rows *q, const fo_rows *q_out, const fo_rope_axes *rope);
+
 /* Attention of the batch's query rows over their sequences' cached positions:
  * the row at position p sees positions 0 .. p, or the newest `window` of them
  * (0: all).  q and out have one type and n_heads heads, a multiple of
@@ -597,6 +624,50 @@ int fo_paged_append(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch *ba
  * (FO_ERR_CAPACITY). */
 int fo_paged_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch *batch, const fo_rows *q,
                        const float *sinks, float scale, int64_t window, const fo_rows *out, float *lse);
+
+/* fo_paged_attention over a window and a few first positions that stay in
+ * sight behind it, for any number of rows (a decode step's, or a whole
+ * prompt's): the row at position p sees the positions j <= p with j < first or
+ * p - j < window (window 0: all of them).  Pages that no row sees are not read.
+ * Rows that see nothing, and rows that are not finite, as there.
+ *
+ * Few query rows of a KV head (up to FO_PAGED_FEW) are computed as
+ * fo_paged_attention's; more as FP16 products with FP32 sums: codes are exact, a
+ * query element is held to 2^-11 (FP32 rows: 2^-22) of itself, which BF16 rows'
+ * are exactly, or to 2^-39 of the largest of its row and head; a probability to
+ * 2^-11 (2^-22) of itself, or to 2^-35 of its row's largest.  The sum of
+ * probabilities has no such rounding.
+ *
+ * A sequence's rows times the query heads of a KV head are at most 2^31 - 1,
+ * and so are the tiles of 8 KB of keys that the page tables have room for, of
+ * all KV heads and for every 48 query rows of one (FO_ERR_CAPACITY). */
+#define FO_PAGED_FEW 16
+int fo_paged_window_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch *batch, const fo_rows *q,
+                              const float *sinks, float scale, int64_t window, int64_t first, const fo_rows *out,
+                              float *lse);
+
+/* Groups of sequences that share their beginnings: group g is the sequences
+ * seq_start[g] .. seq_start[g + 1] - 1 (n_groups + 1 ascending numbers), and
+ * their positions 0 .. lens[g] - 1 are in the pages that the FIRST of them has
+ * in the page table; what the others have there is not read, but for the page
+ * that position lens[g] falls into, where each has its own from that position
+ * on.  Sequences before the first group and behind the last share nothing. */
+typedef struct {
+    const int32_t *seq_start; /* [n_groups + 1] */
+    const int32_t *lens;      /* [n_groups] */
+    int64_t n_groups;
+} fo_paged_groups;
+
+/* Attention of rows whose sequences share their beginnings, which are read once
+ * for all rows of a group: the row at position p sees positions 0 .. p, as in
+ * fo_paged_attention without a window.  Rounding and limits as in
+ * fo_paged_window_attention.  Where a KV head has fewer than 64 query rows of a
+ * sequence, unfinished rows wait in the context's scratch, total_rows *
+ * n_heads * (head_dim + 2) floats: a call that needs more of it than any before
+ * makes it, which a graph's capture refuses (what graphs use is kept). */
+int fo_paged_prefix_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch *batch,
+                              const fo_paged_groups *groups, const fo_rows *q, const float *sinks, float scale,
+                              const fo_rows *out, float *lse);
 
 #ifdef __cplusplus
 }
