@@ -231,15 +231,15 @@ __device__ __forceinline__ uint2 pt_widen(uint32_t w) {
     }
 }
 
-// Writes 32 dimensions of a finished row.
+// Writes 16 dimensions of a finished row.
 template <typename T>
-__device__ __forceinline__ void pt_store32(T *to, const float *v, bool vec) {
+__device__ __forceinline__ void pt_store16(T *to, const float *v, bool vec) {
     if (vec) {
 #pragma unroll
-        for (int i = 0; i < 32; i += 8) store8(to + i, v + i);
+        for (int i = 0; i < 16; i += 8) store8(to + i, v + i);
     } else {
 #pragma unroll
-        for (int i = 0; i < 32; i++) store1(to + i, v[i]);
+        for (int i = 0; i < 16; i++) store1(to + i, v[i]);
     }
 }
 
@@ -366,56 +366,54 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 ok = __all_sync(0xffffffffu, mbar_wait(&sh.meta_full[k % PT_METAS], (k / PT_METAS) & 1, abort_flag, a.err));
                 if (!ok) break;
                 tc_fence_after();
-                uint32_t raw[128];
-                FO_TMEM_LD32(s_at + 0, (raw + 0));
-                FO_TMEM_LD32(s_at + 32, (raw + 32));
-                FO_TMEM_LD32(s_at + 64, (raw + 64));
-                FO_TMEM_LD32(s_at + 96, (raw + 96));
                 const PtMeta &meta = sh.meta[k % PT_METAS];
                 const int tile = meta.base;
                 int tile_top = meta.top;
-                float f[8];
-#pragma unroll
-                for (int g = 0; g < 8; g++) f[g] = meta.ks[g] * q_scale;
-                tmem_wait_ld();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.s_read[t]);
-                // Scores in log2 units, two at a time.
-                float2 x[64];
-#pragma unroll
-                for (int e = 0; e < 64; e++)
-                    x[e] = __fmul2_rn(make_float2(__uint_as_float(raw[2 * e]), __uint_as_float(raw[2 * e + 1])),
-                                      make_float2(f[e / 8], f[e / 8]));
                 const int hi = min(high, meta.to - 1), lo = max(low, meta.from);
-                const bool full = hi - tile >= PT_TILE - 1 && (lo <= tile || a.reach.first - tile >= PT_TILE);
-                if (!__all_sync(0xffffffffu, full)) {
-                    // Keys that the row sees, as bits.
-                    tile_top = PT_LOWEST;
-                    auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; };
+                const bool full = __all_sync(
+                    0xffffffffu, hi - tile >= PT_TILE - 1 && (lo <= tile || a.reach.first - tile >= PT_TILE));
+                // Of 32 keys, those that the row sees, as bits.  (Differences that cannot wrap: every
+                // one is of numbers from -1 up.)
+                auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; };
+                auto seen = [&](int w) {
+                    const int b = tile + 32 * w;
+                    return below(min(hi - b, 32) + 1) & (~below(lo - b) | below(a.reach.first - b));
+                };
+                // The row's largest score, in log2 units, 32 keys at a time: the loops are short, since
+                // code of every kind runs on an SM at once and what does not stay in its instruction
+                // cache costs more than the exponentials (the row held in registers and all of it
+                // unrolled: 274 us where this takes MEASURED).
+                float mx = -INFINITY;
+                if (!full) tile_top = PT_LOWEST;
+#pragma unroll 1
+                for (int w = 0; w < 4; w++) {
+                    uint32_t raw[32];
+                    FO_TMEM_LD32(s_at + 32 * w, raw);
+                    const float f0 = meta.ks[2 * w] * q_scale, f1 = meta.ks[2 * w + 1] * q_scale;
+                    float2 x[16];
+                    tmem_wait_ld();
 #pragma unroll
-                    for (int w = 0; w < 4; w++) {
-                        const int b = tile + 32 * w;
-                        // (Differences that cannot wrap: every one is of numbers from -1 up.)
-                        const uint32_t see = below(min(hi - b, 32) + 1) & (~below(lo - b) | below(a.reach.first - b));
+                    for (int e = 0; e < 16; e++)
+                        x[e] = __fmul2_rn(make_float2(__uint_as_float(raw[2 * e]), __uint_as_float(raw[2 * e + 1])),
+                                          e < 8 ? make_float2(f0, f0) : make_float2(f1, f1));
+                    if (!full) {
+                        const uint32_t see = seen(w);
                         if (see & 0x0000FFFFu) tile_top = max(tile_top, pt_above(meta.vs[2 * w]));
                         if (see & 0xFFFF0000u) tile_top = max(tile_top, pt_above(meta.vs[2 * w + 1]));
 #pragma unroll
                         for (int e = 0; e < 16; e++) {
-                            if (!(see >> (2 * e) & 1)) x[16 * w + e].x = -INFINITY;
-                            if (!(see >> (2 * e + 1) & 1)) x[16 * w + e].y = -INFINITY;
+                            if (!(see >> (2 * e) & 1)) x[e].x = -INFINITY;
+                            if (!(see >> (2 * e + 1) & 1)) x[e].y = -INFINITY;
                         }
                     }
-                }
-                float mx0 = x[0].x, mx1 = x[0].y, mx2 = x[1].x, mx3 = x[1].y;
+                    float m0 = fmaxf(x[0].x, x[0].y), m1 = fmaxf(x[1].x, x[1].y);
 #pragma unroll
-                for (int e = 2; e < 64; e += 2) {
-                    mx0 = fmaxf(mx0, x[e].x);
-                    mx1 = fmaxf(mx1, x[e].y);
-                    mx2 = fmaxf(mx2, x[e + 1].x);
-                    mx3 = fmaxf(mx3, x[e + 1].y);
+                    for (int e = 2; e < 16; e += 2) {
+                        m0 = fmaxf(m0, fmaxf(x[e].x, x[e].y));
+                        m1 = fmaxf(m1, fmaxf(x[e + 1].x, x[e + 1].y));
+                    }
+                    mx = fmaxf(mx, fmaxf(m0, m1));
                 }
-                const float mx = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3));
                 float factor = 1.0f;  // of what has been summed so far
                 if (!any) {
                     m = mx;
@@ -429,77 +427,78 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                     m = next;
                     top = max(top, tile_top);
                 }
-                // Values' scales times 2^10 / top; those of pages that the row does not see meet zeros.
-                const float inverse_top = __uint_as_float((uint32_t)(264 - top) << 23);
-#pragma unroll
-                for (int g = 0; g < 8; g++) f[g] = fminf(meta.vs[g] * inverse_top, FLT_MAX);
                 const float shift = m == -INFINITY ? 0.0f : m;
                 // P may be written, and O touched, once the PV before is complete.
-                uint32_t pk[64];
-                float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
-                auto probabilities = [&](int e) {
-                    const float2 d = __fadd2_rn(x[e], make_float2(-shift, -shift));
-                    const float2 p = make_float2(ex2(d.x), ex2(d.y));
-                    sum[e & 1] = __fadd2_rn(sum[e & 1], p);
-                    return __fmul2_rn(p, make_float2(f[e / 8], f[e / 8]));
-                };
-                if constexpr (!F32) {
-#pragma unroll
-                    for (int e = 0; e < 64; e++) {
-                        const float2 p = probabilities(e);
-                        pk[e] = pt_f16x2(p.x, p.y);
-                    }
-                }
                 if (any) {
                     ok = __all_sync(0xffffffffu, mbar_wait(&sh.o_full[t], (c - 1) & 1, abort_flag, a.err));
                     if (!ok) break;
                     if (__any_sync(0xffffffffu, factor != 1.0f)) {
                         tc_fence_after();
-#pragma unroll
-                        for (int h = 0; h < D / 16; h++) {
+#pragma unroll 1
+                        for (int d = 0; d < D; d += 16) {
                             uint32_t o[16];
-                            asm volatile(
-                                "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                                : "=r"(o[0]), "=r"(o[1]), "=r"(o[2]), "=r"(o[3]), "=r"(o[4]), "=r"(o[5]), "=r"(o[6]), "=r"(o[7]),
-                                  "=r"(o[8]), "=r"(o[9]), "=r"(o[10]), "=r"(o[11]), "=r"(o[12]), "=r"(o[13]), "=r"(o[14]), "=r"(o[15])
-                                : "r"(o_at(t) + 16 * h)
-                                : "memory");
+                            FO_TMEM_LD16(o_at(t) + d, o);
                             tmem_wait_ld();
 #pragma unroll
                             for (int e = 0; e < 16; e++) o[e] = __float_as_uint(__uint_as_float(o[e]) * factor);
-                            asm volatile(
-                                "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
-                                ::"r"(o_at(t) + 16 * h),
-                                "r"(o[0]), "r"(o[1]), "r"(o[2]), "r"(o[3]), "r"(o[4]), "r"(o[5]), "r"(o[6]), "r"(o[7]),
-                                "r"(o[8]), "r"(o[9]), "r"(o[10]), "r"(o[11]), "r"(o[12]), "r"(o[13]), "r"(o[14]), "r"(o[15])
-                                : "memory");
+                            FO_TMEM_ST16(o_at(t) + d, o);
                         }
-                        tmem_wait_st();
                     }
                 }
-                if constexpr (!F32) {
-                    FO_TMEM_ST32(p_at, (pk + 0));
-                    FO_TMEM_ST32(p_at + 32, (pk + 32));
-                } else {
-                    // Two terms; half of the keys at a time, for the registers.
+                // Values' scales are taken times 2^10 / top; those of pages that the row does not see meet
+                // zeros.
+                const float inverse_top = __uint_as_float((uint32_t)(264 - top) << 23);
+                float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll 1
+                for (int w = 0; w < 4; w++) {
+                    uint32_t raw[32];
+                    FO_TMEM_LD32(s_at + 32 * w, raw);
+                    const float f0 = meta.ks[2 * w] * q_scale, f1 = meta.ks[2 * w + 1] * q_scale;
+                    const float v0 = fminf(meta.vs[2 * w] * inverse_top, FLT_MAX);
+                    const float v1 = fminf(meta.vs[2 * w + 1] * inverse_top, FLT_MAX);
+                    const uint32_t see = full ? 0xFFFFFFFFu : seen(w);
+                    tmem_wait_ld();
+                    float2 p[16];
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
+                    for (int e = 0; e < 16; e++) {
+                        const float2 x = __ffma2_rn(make_float2(__uint_as_float(raw[2 * e]), __uint_as_float(raw[2 * e + 1])),
+                                                    e < 8 ? make_float2(f0, f0) : make_float2(f1, f1),
+                                                    make_float2(-shift, -shift));
+                        p[e] = make_float2(ex2(x.x), ex2(x.y));
+                    }
+                    if (!full) {
 #pragma unroll
-                        for (int e = 0; e < 32; e++) {
-                            const float2 p = probabilities(32 * h + e);
-                            pk[e] = pt_f16x2(p.x, p.y);
-                            const float2 b = f16x2_f32x2(pk[e]);
-                            pk[32 + e] = pt_f16x2(p.x - b.x, p.y - b.y);
+                        for (int e = 0; e < 16; e++) {
+                            if (!(see >> (2 * e) & 1)) p[e].x = 0.0f;
+                            if (!(see >> (2 * e + 1) & 1)) p[e].y = 0.0f;
                         }
-                        FO_TMEM_ST32(p_at + 32 * h, (pk + 0));
-                        FO_TMEM_ST32(p_at + 64 + 32 * h, (pk + 32));
+                    }
+                    uint32_t hi_term[16];
+#pragma unroll
+                    for (int e = 0; e < 16; e++) {
+                        sum = __fadd2_rn(sum, p[e]);
+                        p[e] = __fmul2_rn(p[e], e < 8 ? make_float2(v0, v0) : make_float2(v1, v1));
+                        hi_term[e] = pt_f16x2(p[e].x, p[e].y);
+                    }
+                    // (In S's place P's columns are of keys that have been read.)
+                    FO_TMEM_ST16(p_at + 16 * TERMS * w, hi_term);
+                    if constexpr (F32) {
+#pragma unroll
+                        for (int e = 0; e < 16; e++) {
+                            const float2 b = f16x2_f32x2(hi_term[e]);
+                            hi_term[e] = pt_f16x2(p[e].x - b.x, p[e].y - b.y);
+                        }
+                        FO_TMEM_ST16(p_at + 16 * TERMS * w + 16, hi_term);
                     }
                 }
-                l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                l += sum.x + sum.y;
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.p_full[t]);
+                if (lane == 0) {
+                    mbar_arrive(&sh.s_read[t]);
+                    mbar_arrive(&sh.p_full[t]);
+                }
                 any = true;
             }
             if (!ok) break;
@@ -561,41 +560,36 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                     reinterpret_cast<float2 *>(a.part_ml)[(int64_t)part * FO_TILES_QUERIES + q] = make_float2(m, l);
                 }
 #pragma unroll 1
-                for (int d = c0; d < c1; d += 32) {
-                    uint32_t o[32];
-                    float v[32];
+                for (int d = c0; d < c1; d += 16) {
+                    uint32_t o[16];
+                    float v[16];
                     if (has0) {
-                        FO_TMEM_LD32(o_at(o_from) + d, o);
+                        FO_TMEM_LD16(o_at(o_from) + d, o);
                         tmem_wait_ld();
 #pragma unroll
-                        for (int e = 0; e < 32; e++) v[e] = __uint_as_float(o[e]) * f0;
+                        for (int e = 0; e < 16; e++) v[e] = __uint_as_float(o[e]) * f0;
                     }
                     if (has1) {
-                        FO_TMEM_LD32(o_at(1) + d, o);
+                        FO_TMEM_LD16(o_at(1) + d, o);
                         tmem_wait_ld();
 #pragma unroll
-                        for (int e = 0; e < 32; e++) v[e] = fmaf(__uint_as_float(o[e]), f1, v[e]);
+                        for (int e = 0; e < 16; e++) v[e] = fmaf(__uint_as_float(o[e]), f1, v[e]);
                     }
                     if (!mine) continue;
-                    if (part >= 0) {
-                        float4 *to = reinterpret_cast<float4 *>(a.part_o) +
-                                     ((int64_t)part * (D / 4) + d / 4) * FO_TILES_QUERIES + q;
+                    if (part >= 0 || a.reach.raw_o) {
+                        const int64_t step = part >= 0 ? FO_TILES_QUERIES : 1;
+                        float4 *to = part >= 0 ? reinterpret_cast<float4 *>(a.part_o) +
+                                                     ((int64_t)part * (D / 4) + d / 4) * FO_TILES_QUERIES + q
+                                               : reinterpret_cast<float4 *>(a.reach.raw_o + at_row * D + d);
 #pragma unroll
-                        for (int e = 0; e < 8; e++)
-                            __stcg(to + e * FO_TILES_QUERIES,
-                                   make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]));
-                        continue;
-                    }
-                    if (a.reach.raw_o) {
-                        float4 *to = reinterpret_cast<float4 *>(a.reach.raw_o + at_row * D + d);
-#pragma unroll
-                        for (int e = 0; e < 8; e++) to[e] = make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]);
+                        for (int e = 0; e < 4; e++)
+                            __stcg(to + e * step, make_float4(v[4 * e], v[4 * e + 1], v[4 * e + 2], v[4 * e + 3]));
                         continue;
                     }
                     if (a.reach.prior_o) {
                         const float4 *from = reinterpret_cast<const float4 *>(a.reach.prior_o + at_row * D + d);
 #pragma unroll
-                        for (int e = 0; e < 8; e++) {
+                        for (int e = 0; e < 4; e++) {
                             const float4 y = __ldcg(from + e);
                             v[4 * e] = fmaf(y.x, fp, v[4 * e]);
                             v[4 * e + 1] = fmaf(y.y, fp, v[4 * e + 1]);
@@ -604,8 +598,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                         }
                     }
 #pragma unroll
-                    for (int e = 0; e < 32; e++) v[e] *= inv;
-                    pt_store32(static_cast<T *>(a.out.data) + row * a.out.row_stride + h * a.out.head_stride + d, v,
+                    for (int e = 0; e < 16; e++) v[e] *= inv;
+                    pt_store16(static_cast<T *>(a.out.data) + row * a.out.row_stride + h * a.out.head_stride + d, v,
                                a.out_vec);
                 }
             }
@@ -630,7 +624,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
         int slot = 0, round = 0;
         bool ok = true;
         for (int k = 0; k < count && ok; k++) {
-#pragma unroll
+#pragma unroll 1
             for (int value = 0; value < 2; value++) {
                 uint64_t *full = value ? &sh.v_full[k & 1] : &sh.k_full[k & 1];
                 uint64_t *empty = value ? &sh.v_empty[k & 1] : &sh.k_empty[k & 1];
@@ -851,11 +845,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
             auto issue_s = [&](int t, int q_buf, int q_tile, int k) {
                 if (elect_one()) {
                     uint32_t more = 0;
-#pragma unroll
+#pragma unroll 1
                     for (int x = 0; x < TERMS; x++) {
                         const uint64_t q = dQ + q_buf * (Shape::Q_BYTES >> 4) + (q_tile * TERMS + x) * OPERAND16;
                         const uint64_t b = dK + (k & 1) * OPERAND16;
-#pragma unroll
+#pragma unroll 2
                         for (int kk = 0; kk < D / 16; kk++) {
                             const uint32_t off = (kk >> 2) * PANEL16 + 2 * (kk & 3);
                             mma_bf16(tmem + 128 * t, q + off, b + off, ID_S, more);
@@ -869,15 +863,16 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
             auto issue_pv = [&](int t, int k, bool first) {
                 if (elect_one()) {
                     const uint32_t p = tmem + (ALIAS ? 128 * t : 384 + 64 * t);
-#pragma unroll
+#pragma unroll 1
                     for (int x = 0; x < TERMS; x++)
-#pragma unroll
+#pragma unroll 1
                         for (int panel = 0; panel < PANELS; panel++) {
                             const uint64_t b = dV + (k & 1) * OPERAND16 + panel * PANEL16;
                             const uint32_t o = tmem + 256 + (ALIAS ? 128 : 64) * t + 64 * panel;
-#pragma unroll
+#pragma unroll 2
                             for (int kk = 0; kk < 8; kk++)
-                                mma_bf16_ts(o, p + 64 * x + 8 * kk, b + kk * (2048 >> 4), ID_PV, x > 0 || kk > 0 || !first);
+                                mma_bf16_ts(o, p + 16 * (x + TERMS * (kk >> 1)) + 8 * (kk & 1), b + kk * (2048 >> 4), ID_PV,
+                                            x > 0 || kk > 0 || !first);
                         }
                     mma_commit(&sh.o_full[t]);
                 }

@@ -242,6 +242,23 @@ __device__ __forceinline__ uint64_t sdesc_sw64(uint32_t smem_addr, uint32_t lbo_
         "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])                                                              \
         : "memory")
 
+// The same, 16 columns.
+#define FO_TMEM_LD16(taddr, r)                                                                                     \
+    asm volatile(                                                                                                  \
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"     \
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), \
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])                  \
+        : "r"(taddr)                                                                                               \
+        : "memory")
+
+#define FO_TMEM_ST16(taddr, r)                                                                                     \
+    asm volatile(                                                                                                  \
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::  \
+            "r"(taddr),                                                                                            \
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), \
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])                                      \
+        : "memory")
+
 // One 32-bit column of this warp's 32 TMEM lanes.
 __device__ __forceinline__ uint32_t tmem_ld1(uint32_t taddr) {
     uint32_t r;
