@@ -50,9 +50,9 @@ namespace fo {
 using namespace sm100;
 
 constexpr int PT_TILE = 128;  // positions
-constexpr int PT_SOFTMAX = 8, PT_CONVERTERS = 4, PT_LOADERS = 2;
-constexpr int PT_PRODUCER = PT_SOFTMAX + PT_CONVERTERS, PT_ISSUER = PT_PRODUCER + 1, PT_LOADER = PT_ISSUER + 1;
-constexpr int PT_THREADS = 32 * (PT_LOADER + PT_LOADERS);
+constexpr int PT_SOFTMAX = 8, PT_CONVERTERS = 4;
+constexpr int PT_PRODUCER = PT_SOFTMAX + PT_CONVERTERS, PT_ISSUER = PT_PRODUCER + 1;  // two issuers, and a warp that idles
+constexpr int PT_THREADS = 512;
 // Registers a thread: launched with 128, the softmax warpgroups' two take what
 // the other two give up: 256 * 176 + 256 * 80 = 512 * 128.
 constexpr int PT_LAUNCH_REGS = 128, PT_SOFTMAX_REGS = 176, PT_OTHER_REGS = 80;
@@ -80,10 +80,9 @@ struct PtShape {
     static constexpr int PANELS = D / 64;
     static constexpr uint32_t OPERAND = PANELS * PT_PANEL;  // 128 rows of D FP16
     static constexpr uint32_t Q_BYTES = Q_TILES * TERMS * OPERAND;
-    static constexpr int Q_BUFS = D == 64 && !F32 ? 2 : 1;
     static constexpr int PARTS = D / 64;  // slots of a tile's keys, or values
     static constexpr int SLOTS = D == 64 ? 6 : 3;
-    static constexpr uint32_t OFF_K = Q_BUFS * Q_BYTES, OFF_V = OFF_K + 2 * OPERAND, OFF_CODES = OFF_V + 2 * OPERAND;
+    static constexpr uint32_t OFF_K = Q_BYTES, OFF_V = OFF_K + 2 * OPERAND, OFF_CODES = OFF_V + 2 * OPERAND;
     static constexpr uint32_t SMEM = OFF_CODES + SLOTS * PT_SLOT + 1024;
 };
 
@@ -109,15 +108,14 @@ struct PtShared {
     using Shape = PtShape<D, F32>;
     uint64_t code_full[Shape::SLOTS], code_empty[Shape::SLOTS];
     uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
-    uint64_t s_full[2], s_read[2], p_full[2], o_full[2];
-    uint64_t q_full[2], q_free[2];
+    uint64_t s_full[2], p_full[2], o_full[2];
+    uint64_t q_full[2], q_both;  // a stream's queries are there; those of the first that the second uses too
     uint64_t seg_full[PT_SEGS], seg_free[PT_SEGS];
     uint64_t meta_full[PT_METAS];
     uint64_t x_full, x_free, done;
     PtSegment seg[PT_SEGS];
     PtMeta meta[PT_METAS];
-    float q_scale[Shape::Q_BUFS][Shape::QUERIES];
-    int q_high[Shape::Q_BUFS][Shape::QUERIES], q_low[Shape::Q_BUFS][Shape::QUERIES];
+    int k_tile[2], v_tile[2];  // the tile that the operands are, or will be, of
     float xm[2][128], xl[2][128], xt[2][128];
     int2 warp_sum[PT_THREADS / 32];
     int begin_item, begin_base, abort;
@@ -248,7 +246,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
     using Shape = PtShape<D, F32>;
     using T = typename std::conditional<F32, float, uint16_t>::type;
     constexpr int QUERIES = Shape::QUERIES, TERMS = Shape::TERMS, PANELS = Shape::PANELS, PARTS = Shape::PARTS;
-    constexpr int SLOTS = Shape::SLOTS, Q_BUFS = Shape::Q_BUFS;
+    constexpr int SLOTS = Shape::SLOTS;
     constexpr bool ALIAS = Shape::ALIAS;
     extern __shared__ uint8_t pt_smem[];
     __shared__ PtShared<D, F32> sh;
@@ -260,18 +258,16 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
         if (lane < SLOTS) mbar_init(&sh.code_full[lane], 1), mbar_init(&sh.code_empty[lane], PT_CONVERTERS);
         if (lane < 2) {
             mbar_init(&sh.k_full[lane], PT_CONVERTERS), mbar_init(&sh.v_full[lane], PT_CONVERTERS);
-            mbar_init(&sh.k_empty[lane], 1), mbar_init(&sh.v_empty[lane], 1);
+            mbar_init(&sh.k_empty[lane], 2), mbar_init(&sh.v_empty[lane], 2);
             mbar_init(&sh.s_full[lane], 1), mbar_init(&sh.o_full[lane], 1);
-            mbar_init(&sh.s_read[lane], 4), mbar_init(&sh.p_full[lane], 4);
-            mbar_init(&sh.q_full[lane], PT_LOADERS), mbar_init(&sh.q_free[lane], 1 + PT_SOFTMAX);
+            mbar_init(&sh.p_full[lane], 4), mbar_init(&sh.q_full[lane], 4);
+            sh.k_tile[lane] = sh.v_tile[lane] = -1;
         }
-        if (lane < PT_SEGS) {
-            mbar_init(&sh.seg_full[lane], 1);
-            mbar_init(&sh.seg_free[lane], PT_SOFTMAX + PT_LOADERS + 1);
-        }
+        if (lane < PT_SEGS) mbar_init(&sh.seg_full[lane], 1), mbar_init(&sh.seg_free[lane], PT_SOFTMAX + 2);
         if (lane < PT_METAS) mbar_init(&sh.meta_full[lane], 1);
         if (lane == 31) {
-            mbar_init(&sh.x_full, PT_SOFTMAX), mbar_init(&sh.x_free, PT_SOFTMAX), mbar_init(&sh.done, 1);
+            mbar_init(&sh.x_full, PT_SOFTMAX), mbar_init(&sh.x_free, PT_SOFTMAX), mbar_init(&sh.done, 2);
+            mbar_init(&sh.q_both, 4);
             sh.abort = 0;
         }
         mbar_fence_init();
@@ -330,7 +326,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
         const uint32_t at = tmem + ((uint32_t)(32 * wq) << 16);
         const uint32_t s_at = at + 128 * t, p_at = ALIAS ? s_at : at + 384 + 64 * t;
         auto o_at = [&](int stream) { return at + 256 + (ALIAS ? 128 : 64) * stream; };
-        int c = 0, x_phase = 0;  // tiles of this stream so far; joins of both streams
+        int c = 0, x_phase = 0, both_phase = 0;  // tiles of this stream so far; joins of both streams; queries of both
         bool ok = true;
         for (int s = 0; ok; s++) {
             ok = __all_sync(0xffffffffu, mbar_wait(&sh.seg_full[s % PT_SEGS], (s / PT_SEGS) & 1, abort_flag, a.err));
@@ -339,12 +335,92 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
             const int n = seg.n, base = seg.base, pair = seg.pair, last = seg.last;
             const int q = (pair ? 128 * t : 0) + r;  // of the unit's
             const bool live = (pair ? 128 * t : 0) + 32 * wq < seg.nq;
-            ok = __all_sync(0xffffffffu, mbar_wait(&sh.q_full[s % Q_BUFS], (s / Q_BUFS) & 1, abort_flag, a.err));
-            if (!ok) break;
-            const float q_scale = sh.q_scale[s % Q_BUFS][q];
-            const int high = sh.q_high[s % Q_BUFS][q], low = sh.q_low[s % Q_BUFS][q];
+            // The row's queries, as operands, and what it sees.  (Rows that are none's see everything,
+            // and are not kept.)
+            const bool own = pair || t == 0 || n > 1;  // this stream has tiles
+            const bool mine = q < seg.nq;
+            float q_scale = 0.0f;
+            int high = INT32_MAX, low = 0;
+            if (own && live) {
+                const T *from = nullptr;
+                float inv0 = 0.0f, inv1 = 1.0f;
+                if (mine) {
+                    const int qi = seg.q0 + q, row_of = qi / a.group;
+                    const int64_t row = seg.first + row_of;
+                    from = static_cast<const T *>(a.q.data) + row * a.q.row_stride +
+                           (seg.head * a.group + qi - row_of * a.group) * a.q.head_stride;
+                    if (seg.flat) {
+                        high = min(place_of_row(a.batch, a.kv.page_size, (int)row, a.err), seg.end - 1);
+                    } else {
+                        high = max(seg.p0 + row_of, -1);
+                        low = a.window > 0 ? max(high + 1 - a.window, 0) : 0;
+                    }
+                }
+                auto load = [&](int d, float (&x)[8]) {
+                    if (a.q_vec) {
+                        load8(from + d, x);
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 8; e++) x[e] = load1(from + d + e);
+                    }
+                };
+                if (mine) {
+                    float most = 0.0f;
+                    bool finite = true;
+#pragma unroll 4
+                    for (int d = 0; d < D; d += 8) {
+                        float x[8];
+                        load(d, x);
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            most = fmaxf(most, fabsf(x[e]));
+                            finite &= fabsf(x[e]) <= FLT_MAX;
+                        }
+                    }
+                    // A power of two brings the largest element to [2^14, 2^15), in two factors, so
+                    // that FP32's whole range of exponents can be brought there.
+                    const int e = max((int)(__float_as_uint(most) >> 23), 1);
+                    inv0 = finite ? __uint_as_float((uint32_t)(254 - (e + 1) / 2 - 63) << 23) : 0.0f;
+                    inv1 = __uint_as_float((uint32_t)(254 - (e - (e + 1) / 2) - 64) << 23) * 16384.0f;
+                    q_scale = finite ? __uint_as_float((uint32_t)e << 23) * (1.0f / 16384.0f) * a.scale * REACH_LOG2E : NAN;
+                }
+                if (pair || t == 0) {
+                    uint8_t *to = smem + (pair ? t : 0) * TERMS * Shape::OPERAND + r * 128;
+#pragma unroll 1
+                    for (int d = 0; d < D; d += 8) {
+                        float x[8] = {};
+                        if (inv0 != 0.0f) load(d, x);
+#pragma unroll
+                        for (int e = 0; e < 8; e++) x[e] = x[e] * inv0 * inv1;
+                        const int place = (d >> 6) * PT_PANEL + (((d >> 3 & 7) ^ (r & 7)) << 4);
+#pragma unroll
+                        for (int term = 0; term < TERMS; term++) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int e = 0; e < 4; e++) {
+                                w[e] = pt_f16x2(x[2 * e], x[2 * e + 1]);
+                                const float2 b = f16x2_f32x2(w[e]);
+                                x[2 * e] -= b.x;
+                                x[2 * e + 1] -= b.y;
+                            }
+                            *reinterpret_cast<uint4 *>(to + term * Shape::OPERAND + place) = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
+                    }
+                    fence_proxy_async_smem();
+                }
+            }
             __syncwarp();
-            if (lane == 0) mbar_arrive(&sh.q_free[s % Q_BUFS]);
+            if (pair || t == 0) {
+                if (lane == 0) {
+                    mbar_arrive(&sh.q_full[t]);
+                    if (!pair && n > 1) mbar_arrive(&sh.q_both);
+                }
+            } else if (own) {
+                ok = __all_sync(0xffffffffu, mbar_wait(&sh.q_both, both_phase, abort_flag, a.err));
+                if (!ok) break;
+                if (lane == 0) mbar_arrive(&sh.q_full[t]);
+            }
+            if (!pair && n > 1) both_phase ^= 1;
             float m = -INFINITY, l = 0.0f;
             int top = PT_LOWEST;  // exponent bits of a power of two above the scales of the values that the row sees
             bool any = false;
@@ -355,7 +431,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 if (!live) {
                     // No query in this warp: whatever its lanes hold stays theirs.  (It arrives once
                     // for each tile as the others do, not for the next one before they have for this.)
-                    if (lane == 0) mbar_arrive(&sh.s_read[t]);
                     if (any) ok = __all_sync(0xffffffffu, mbar_wait(&sh.o_full[t], (c - 1) & 1, abort_flag, a.err));
                     if (!ok) break;
                     if (lane == 0) mbar_arrive(&sh.p_full[t]);
@@ -495,10 +570,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(&sh.s_read[t]);
-                    mbar_arrive(&sh.p_full[t]);
-                }
+                if (lane == 0) mbar_arrive(&sh.p_full[t]);
                 any = true;
             }
             if (!ok) break;
@@ -536,7 +608,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 o_from = 0;
             }
             if (live) {
-                const bool mine = q < seg.nq;
                 const int qi = seg.q0 + q, row_of = qi / a.group, h = seg.head * a.group + qi - row_of * a.group;
                 const int64_t row = seg.first + row_of;
                 const int part = seg.part;
@@ -631,6 +702,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 uint8_t *to = smem + (value ? Shape::OFF_V : Shape::OFF_K) + (k & 1) * Shape::OPERAND;
                 if (k > 1) ok = __all_sync(0xffffffffu, mbar_wait(empty, (k / 2 - 1) & 1, abort_flag, a.err));
                 if (!ok) break;
+                if (ct == 0) *(volatile int *)(value ? &sh.v_tile[k & 1] : &sh.k_tile[k & 1]) = k;
 #pragma unroll 1
                 for (int h = 0; h < PARTS; h++) {
                     ok = __all_sync(0xffffffffu, mbar_wait(&sh.code_full[slot], round & 1, abort_flag, a.err));
@@ -833,23 +905,30 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 for (int i = max(issued - SLOTS, 0); i < issued; i++)
                     mbar_wait_drain(&sh.code_full[i % SLOTS], (i / SLOTS) & 1);
             }
-        } else if (warp == PT_ISSUER) {
-            // ----------------------------------------------------------- issuer
-            // The whole warp runs the loop and its waits, so that addresses stay
-            // uniform; one elected lane issues.
+        } else if (warp < PT_ISSUER + 2) {
+            // ---------------------------------------------------------- issuers
+            // A warp for each stream, whose code is the same and short (one for both, polling whatever
+            // could be ready, fetched its long loop anew each time: up to 3,000 cycles from a P to its
+            // MMA).  The whole warp runs the loop and its waits, so that addresses stay uniform; one
+            // elected lane issues.
+            const int t = warp - PT_ISSUER;
             const uint32_t base = smem_u32(smem);
             constexpr uint32_t ID_S = idesc_f16(128, 128, 0), ID_PV = idesc_f16(128, 64, 1);
             const uint64_t dQ = sdesc_sw128(base, 16, 1024), dK = sdesc_sw128(base + Shape::OFF_K, 16, 1024);
             const uint64_t dV = sdesc_sw128(base + Shape::OFF_V, PT_PANEL, 1024);
             constexpr uint32_t OPERAND16 = Shape::OPERAND >> 4, PANEL16 = PT_PANEL >> 4;
-            auto issue_s = [&](int t, int q_buf, int q_tile, int k) {
+            struct Tile {
+                int k, pair;
+                bool first;  // of its segment's in this stream
+            };
+            auto issue_s = [&](const Tile &x) {
                 if (elect_one()) {
                     uint32_t more = 0;
 #pragma unroll 1
-                    for (int x = 0; x < TERMS; x++) {
-                        const uint64_t q = dQ + q_buf * (Shape::Q_BYTES >> 4) + (q_tile * TERMS + x) * OPERAND16;
-                        const uint64_t b = dK + (k & 1) * OPERAND16;
-#pragma unroll 2
+                    for (int term = 0; term < TERMS; term++) {
+                        const uint64_t q = dQ + ((x.pair ? t : 0) * TERMS + term) * OPERAND16;
+                        const uint64_t b = dK + (x.k & 1) * OPERAND16;
+#pragma unroll
                         for (int kk = 0; kk < D / 16; kk++) {
                             const uint32_t off = (kk >> 2) * PANEL16 + 2 * (kk & 3);
                             mma_bf16(tmem + 128 * t, q + off, b + off, ID_S, more);
@@ -857,228 +936,129 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                         }
                     }
                     mma_commit(&sh.s_full[t]);
+                    // A tile that is this stream's alone is released for both.
+                    mma_commit(&sh.k_empty[x.k & 1]);
+                    if (!x.pair) mma_commit(&sh.k_empty[x.k & 1]);
                 }
                 __syncwarp();
             };
-            auto issue_pv = [&](int t, int k, bool first) {
+            auto issue_pv = [&](const Tile &x) {
                 if (elect_one()) {
                     const uint32_t p = tmem + (ALIAS ? 128 * t : 384 + 64 * t);
 #pragma unroll 1
-                    for (int x = 0; x < TERMS; x++)
-#pragma unroll 1
-                        for (int panel = 0; panel < PANELS; panel++) {
-                            const uint64_t b = dV + (k & 1) * OPERAND16 + panel * PANEL16;
-                            const uint32_t o = tmem + 256 + (ALIAS ? 128 : 64) * t + 64 * panel;
-#pragma unroll 2
-                            for (int kk = 0; kk < 8; kk++)
-                                mma_bf16_ts(o, p + 16 * (x + TERMS * (kk >> 1)) + 8 * (kk & 1), b + kk * (2048 >> 4), ID_PV,
-                                            x > 0 || kk > 0 || !first);
-                        }
+                    for (int y = 0; y < TERMS * PANELS; y++) {
+                        const int term = y / PANELS, panel = y % PANELS;
+                        const uint64_t b = dV + (x.k & 1) * OPERAND16 + panel * PANEL16;
+                        const uint32_t o = tmem + 256 + (ALIAS ? 128 : 64) * t + 64 * panel;
+#pragma unroll
+                        for (int kk = 0; kk < 8; kk++)
+                            mma_bf16_ts(o, p + 16 * (term + TERMS * (kk >> 1)) + 8 * (kk & 1), b + kk * (2048 >> 4), ID_PV,
+                                        term > 0 || kk > 0 || !x.first);
+                    }
                     mma_commit(&sh.o_full[t]);
+                    mma_commit(&sh.v_empty[x.k & 1]);
+                    if (!x.pair) mma_commit(&sh.v_empty[x.k & 1]);
                 }
                 __syncwarp();
             };
-            auto commit = [&](uint64_t *bar) {
-                if (elect_one()) mma_commit(bar);
-                __syncwarp();
-            };
-            // A stream's place in the block's segments: the next tile of its own.
-            struct Place {
-                int seg, i, n, base, pair;
-                bool last, over;
-            };
-            auto enter = [&](Place &x, int t) {
-                while (x.i >= x.n) {
-                    if (x.last) {
-                        x.over = true;
-                        return false;
-                    }
-                    const int s = x.seg + 1;
-                    if (!__all_sync(0xffffffffu, mbar_test(&sh.seg_full[s % PT_SEGS], (s / PT_SEGS) & 1))) return false;
-                    const PtSegment &g = sh.seg[s % PT_SEGS];
-                    x.seg = s;
-                    x.n = g.n;
-                    x.base = g.base;
-                    x.pair = g.pair;
-                    x.last = g.last;
-                    x.i = x.pair ? 0 : t;
-                }
-                return true;
-            };
-            // Tiles that the stream is past.
-            auto past = [](const Place &x) { return x.base + min(x.i, x.n); };
-            Place ps[2], pv[2];
-#pragma unroll
-            for (int t = 0; t < 2; t++) ps[t] = pv[t] = {-1, 0, 0, 0, 0, false, false};
-            int ns[2] = {0, 0}, np[2] = {0, 0}, q_freed = 0, s_freed = 0;
-            // Tiles and segments whose operands are there, counted in order: a stream skips what is
-            // the other's alone, and a parity test cannot tell a phase from the one two before.
-            int k_there = 0, v_there = 0, q_there = 0;
-            auto count_up = [](int &there, uint64_t *full, int bufs) {
-                if (__all_sync(0xffffffffu, mbar_test(full + there % bufs, (there / bufs) & 1))) there++;
-            };
-            bool ok = true;
-            uint64_t t_last = globaltimer();
-            while (ok && !(pv[0].over && pv[1].over)) {
-                bool progress = false;
-                if (k_there < count) count_up(k_there, sh.k_full, 2);
-                if (v_there < k_there) count_up(v_there, sh.v_full, 2);
-                if (q_there < q_freed + Q_BUFS) count_up(q_there, sh.q_full, Q_BUFS);
-#pragma unroll
-                for (int t = 0; t < 2; t++) {
-                    Place &x = ps[t], &y = pv[t];
-                    if (!x.over && enter(x, t)) {
-                        const int k = x.base + x.i, s = x.seg;
-                        bool ready = k < k_there && s < q_there;
-                        if (ns[t] > 0) {
-                            if constexpr (ALIAS) ready = ready && np[t] == ns[t] && mbar_test(&sh.o_full[t], (ns[t] - 1) & 1);
-                            else ready = ready && mbar_test(&sh.s_read[t], (ns[t] - 1) & 1);
-                        }
-                        if (__all_sync(0xffffffffu, ready)) {
-                            tc_fence_after();
-                            issue_s(t, s % Q_BUFS, x.pair ? t : 0, k);
-                            ns[t]++;
-                            x.i += x.pair ? 1 : 2;
-                            // The last stream to want K(k) releases it.
-                            if (!x.pair || past(ps[t ^ 1]) > k) commit(&sh.k_empty[k & 1]);
-                            progress = true;
-                        }
-                    }
-                    if (!y.over && enter(y, t)) {
-                        const int k = y.base + y.i;
-                        const bool ready = k < v_there && np[t] < ns[t] && mbar_test(&sh.p_full[t], np[t] & 1);
-                        if (__all_sync(0xffffffffu, ready)) {
-                            tc_fence_after();
-                            issue_pv(t, k, y.i < (y.pair ? 1 : 2));
-                            np[t]++;
-                            y.i += y.pair ? 1 : 2;
-                            if (!y.pair || past(pv[t ^ 1]) > k) commit(&sh.v_empty[k & 1]);
-                            progress = true;
-                        }
-                    }
-                }
-                // Queries that both streams are done with, and segments.
-                auto behind = [](const Place &x, int s) { return x.seg > s || (x.seg == s && x.i >= x.n); };
-                if (behind(ps[0], q_freed) && behind(ps[1], q_freed)) {
-                    commit(&sh.q_free[q_freed % Q_BUFS]);
-                    q_freed++;
-                }
-                if (pv[0].seg > s_freed && pv[1].seg > s_freed) {
-                    if (lane == 0) mbar_arrive(&sh.seg_free[s_freed % PT_SEGS]);
-                    __syncwarp();
-                    s_freed++;
-                }
-                if (progress) {
-                    t_last = globaltimer();
-                } else if (globaltimer() - t_last > FO_WAIT_NS || *abort_flag) {
-                    if (lane == 0 && !*abort_flag) {
+            // Waits for tile k's operands.  A stream skips tiles that are the other's, and a parity wait
+            // cannot tell a phase from the one two before; once the operands' tile number is k, the phase
+            // before is over.
+            auto there = [&](uint64_t *full, const int *number, int k) {
+                const uint32_t phase = (k >> 1) & 1;
+                uint64_t t0 = 0;
+                for (uint32_t it = 1;; it++) {
+                    if (!mbar_wait(full + (k & 1), phase, abort_flag, a.err)) return false;
+                    if (*(const volatile int *)(number + (k & 1)) == k)
+                        return mbar_wait(full + (k & 1), phase, abort_flag, a.err);
+                    if ((it & 63) != 0) continue;
+                    if (*abort_flag) return false;
+                    if (t0 == 0) t0 = globaltimer();
+                    if (globaltimer() - t0 > FO_WAIT_NS) {
                         *abort_flag = 1;
                         atomicOr(a.err, FO_DEVERR_WAIT_TIMEOUT);
+                        return false;
                     }
-                    ok = false;
                 }
-                ok = __shfl_sync(0xffffffffu, ok, 0);
+            };
+            // The stream's place: the next tile of its own is i of segment seg.
+            int seg = -1, i = 0, n = 0, first = 0, pair = 0, loads = 0;
+            bool last = false, ok = true;
+            // Goes on to the next segment with a tile of this stream's; false after the last one.
+            auto enter = [&]() {
+                while (i >= n) {
+                    if (seg >= 0) {
+                        if (lane == 0) mbar_arrive(&sh.seg_free[seg % PT_SEGS]);
+                        __syncwarp();
+                    }
+                    if (last) return false;
+                    seg++;
+                    ok = __all_sync(0xffffffffu, mbar_wait(&sh.seg_full[seg % PT_SEGS], (seg / PT_SEGS) & 1, abort_flag, a.err));
+                    if (!ok) return false;
+                    const PtSegment &g = sh.seg[seg % PT_SEGS];
+                    n = g.n;
+                    first = g.base;
+                    pair = g.pair;
+                    last = g.last;
+                    i = pair ? 0 : t;
+                }
+                ok = __all_sync(0xffffffffu, mbar_wait(&sh.q_full[t], loads & 1, abort_flag, a.err));
+                loads++;
+                return ok;
+            };
+            auto take = [&]() {
+                const Tile x = {first + i, pair, i < (pair ? 1 : 2)};
+                i += pair ? 1 : 2;
+                return x;
+            };
+            bool more = enter();
+            Tile now = {};
+            if (more) {
+                now = take();
+                ok = __all_sync(0xffffffffu, there(sh.k_full, sh.k_tile, now.k));
+                tc_fence_after();
+                if (ok) issue_s(now);
+            }
+            for (int c = 0; more && ok; c++) {
+                Tile next = {};
+                bool issued = false;
+                const bool same = i < n;  // the next tile is of the same segment
+                if (same) next = take();
+                ok = __all_sync(0xffffffffu, mbar_wait(&sh.p_full[t], c & 1, abort_flag, a.err));
+                if (!ok) break;
+                tc_fence_after();
+                if (!ALIAS && same) {
+                    // S first, if its keys are there: it is what the softmax waits for next.
+                    issued = __all_sync(0xffffffffu, *(volatile int *)&sh.k_tile[next.k & 1] == next.k &&
+                                                         mbar_test(&sh.k_full[next.k & 1], (next.k >> 1) & 1));
+                    if (issued) {
+                        tc_fence_after();
+                        issue_s(next);
+                    }
+                }
+                ok = __all_sync(0xffffffffu, there(sh.v_full, sh.v_tile, now.k));
+                if (!ok) break;
+                tc_fence_after();
+                issue_pv(now);
+                if (!issued) {
+                    if (!same) {
+                        more = enter();
+                        if (!more) break;
+                        next = take();
+                    }
+                    ok = __all_sync(0xffffffffu, there(sh.k_full, sh.k_tile, next.k));
+                    if (ok && ALIAS) ok = __all_sync(0xffffffffu, mbar_wait(&sh.o_full[t], c & 1, abort_flag, a.err));
+                    if (!ok) break;
+                    tc_fence_after();
+                    issue_s(next);
+                }
+                now = next;
             }
             // Every issued MMA completes before tensor memory is released.
-            commit(&sh.done);
+            if (elect_one()) mma_commit(&sh.done);
+            __syncwarp();
             if (lane == 0) mbar_wait_drain(&sh.done, 0);
             __syncwarp();
-        } else {
-            // ---------------------------------------------------------- queries
-            const int ql = tid - 32 * PT_LOADER;
-            bool ok = true;
-            for (int s = 0; ok; s++) {
-                ok = __all_sync(0xffffffffu, mbar_wait(&sh.seg_full[s % PT_SEGS], (s / PT_SEGS) & 1, abort_flag, a.err));
-                if (!ok) break;
-                const PtSegment seg = sh.seg[s % PT_SEGS];
-                const int buf = s % Q_BUFS;
-                if (s >= Q_BUFS)
-                    ok = __all_sync(0xffffffffu, mbar_wait(&sh.q_free[buf], (s / Q_BUFS - 1) & 1, abort_flag, a.err));
-                if (!ok) break;
-#pragma unroll 1
-                for (int q = ql; q < (seg.pair ? 256 : 128); q += 32 * PT_LOADERS) {
-                    uint8_t *to = smem + buf * Shape::Q_BYTES + (q >> 7) * TERMS * Shape::OPERAND + (q & 127) * 128;
-                    const int swizzle = q & 7;
-                    const bool mine = q < seg.nq;
-                    const T *from = nullptr;
-                    float inv0 = 1.0f, inv1 = 1.0f, scale = 0.0f;
-                    int high = INT32_MAX, low = 0;  // rows that are none's see everything, and are not kept
-                    if (mine) {
-                        const int qi = seg.q0 + q, r = qi / a.group;
-                        const int64_t row = seg.first + r;
-                        from = static_cast<const T *>(a.q.data) + row * a.q.row_stride +
-                               (seg.head * a.group + qi - r * a.group) * a.q.head_stride;
-                        if (seg.flat) {
-                            high = min(place_of_row(a.batch, a.kv.page_size, (int)row, a.err), seg.end - 1);
-                        } else {
-                            high = max(seg.p0 + r, -1);
-                            low = a.window > 0 ? max(high + 1 - a.window, 0) : 0;
-                        }
-                        float top = 0.0f;
-                        bool finite = true;
-#pragma unroll 4
-                        for (int d = 0; d < D; d += 8) {
-                            float x[8];
-                            if (a.q_vec) {
-                                load8(from + d, x);
-                            } else {
-#pragma unroll
-                                for (int e = 0; e < 8; e++) x[e] = load1(from + d + e);
-                            }
-#pragma unroll
-                            for (int e = 0; e < 8; e++) {
-                                top = fmaxf(top, fabsf(x[e]));
-                                finite &= fabsf(x[e]) <= FLT_MAX;
-                            }
-                        }
-                        // A power of two brings the largest element to [2^14, 2^15), in two factors, so
-                        // that FP32's whole range of exponents can be brought there.
-                        const int e = max((int)(__float_as_uint(top) >> 23), 1);
-                        inv0 = __uint_as_float((uint32_t)(254 - (e + 1) / 2 - 63) << 23);
-                        inv1 = __uint_as_float((uint32_t)(254 - (e - (e + 1) / 2) - 64) << 23) * 16384.0f;
-                        scale = finite ? __uint_as_float((uint32_t)e << 23) * (1.0f / 16384.0f) * a.scale * REACH_LOG2E : NAN;
-                        if (!finite) inv0 = 0.0f;
-                    }
-                    sh.q_scale[buf][q] = scale;
-                    sh.q_high[buf][q] = high;
-                    sh.q_low[buf][q] = low;
-#pragma unroll 2
-                    for (int d = 0; d < D; d += 8) {
-                        float x[8];
-                        if (!mine || inv0 == 0.0f) {
-#pragma unroll
-                            for (int e = 0; e < 8; e++) x[e] = 0.0f;
-                        } else if (a.q_vec) {
-                            load8(from + d, x);
-                        } else {
-#pragma unroll
-                            for (int e = 0; e < 8; e++) x[e] = load1(from + d + e);
-                        }
-#pragma unroll
-                        for (int e = 0; e < 8; e++) x[e] = x[e] * inv0 * inv1;
-                        const int place = (d >> 6) * PT_PANEL + (((d >> 3 & 7) ^ swizzle) << 4);
-#pragma unroll
-                        for (int term = 0; term < TERMS; term++) {
-                            uint32_t w[4];
-#pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                w[e] = pt_f16x2(x[2 * e], x[2 * e + 1]);
-                                const float2 b = f16x2_f32x2(w[e]);
-                                x[2 * e] -= b.x;
-                                x[2 * e + 1] -= b.y;
-                            }
-                            *reinterpret_cast<uint4 *>(to + term * Shape::OPERAND + place) = make_uint4(w[0], w[1], w[2], w[3]);
-                        }
-                    }
-                }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(&sh.q_full[buf]);
-                    mbar_arrive(&sh.seg_free[s % PT_SEGS]);
-                }
-                if (seg.last) break;
-            }
         }
     }
     tc_fence_before();
