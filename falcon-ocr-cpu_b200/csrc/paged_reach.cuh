@@ -114,11 +114,8 @@ __device__ __forceinline__ Joined join_parts(float m0, float l0, float m1, float
     return j;
 }
 // 1 / (sum + the sink's term), 0 for a row that has seen nothing.
-__device__ __forceinline__ float inverse_sum(const float *sinks, int head, float m, float l) {
-    if (l == 0.0f) return 0.0f;
-    float sum = l;
-    if (sinks) sum += exp2f(fmaf(sinks[head], REACH_LOG2E, -m));
-    return 1.0f / sum;
+__device__ __forceinline__ float inverse_sum(float sink, float m, float l) {
+    return l == 0.0f ? 0.0f : 1.0f / (l + exp2f(fmaf(sink, REACH_LOG2E, -m)));
 }
 __device__ __forceinline__ float log_sum(float m, float l) {
     return l == 0.0f ? -INFINITY : (m + log2f(l)) * REACH_LN2;

@@ -54,8 +54,8 @@ constexpr int PT_SOFTMAX = 8, PT_CONVERTERS = 4;
 constexpr int PT_PRODUCER = PT_SOFTMAX + PT_CONVERTERS, PT_ISSUER = PT_PRODUCER + 1;  // two issuers, and a warp that idles
 constexpr int PT_THREADS = 512;
 // Registers a thread: launched with 128, the softmax warpgroups' two take what
-// the other two give up: 256 * 176 + 256 * 80 = 512 * 128.
-constexpr int PT_LAUNCH_REGS = 128, PT_SOFTMAX_REGS = 176, PT_OTHER_REGS = 80;
+// the other two give up: 256 * 184 + 256 * 72 = 512 * 128.
+constexpr int PT_LAUNCH_REGS = 128, PT_SOFTMAX_REGS = 184, PT_OTHER_REGS = 72;
 static_assert(256 * PT_SOFTMAX_REGS + 256 * PT_OTHER_REGS == PT_THREADS * PT_LAUNCH_REGS, "register split");
 constexpr int PT_SEGS = 8;    // segments announced at a time
 constexpr int PT_METAS = 16;  // tiles whose scales are held: what the code ring and the operands can be ahead by, and more
@@ -98,6 +98,7 @@ struct PtSegment {
 struct PtMeta {
     float ks[8], vs[8];  // keys' and values' scales of each 16 positions' page
     int top;             // exponent bits of a power of two above the values' scales
+    int plain;           // the keys' scales are numbers from 0 up
     int base;            // the tile's first position
     int from, to;        // positions [from, to) that rows may see of it
     unsigned pages;      // pages that were copied
@@ -108,7 +109,7 @@ struct PtShared {
     using Shape = PtShape<D, F32>;
     uint64_t code_full[Shape::SLOTS], code_empty[Shape::SLOTS];
     uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
-    uint64_t s_full[2], p_full[2], o_full[2];
+    uint64_t s_full[2], s_read[2], p_full[2], o_full[2];
     uint64_t q_full[2], q_both;  // a stream's queries are there; those of the first that the second uses too
     uint64_t seg_full[PT_SEGS], seg_free[PT_SEGS];
     uint64_t meta_full[PT_METAS];
@@ -260,7 +261,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
             mbar_init(&sh.k_full[lane], PT_CONVERTERS), mbar_init(&sh.v_full[lane], PT_CONVERTERS);
             mbar_init(&sh.k_empty[lane], 2), mbar_init(&sh.v_empty[lane], 2);
             mbar_init(&sh.s_full[lane], 1), mbar_init(&sh.o_full[lane], 1);
-            mbar_init(&sh.p_full[lane], 4), mbar_init(&sh.q_full[lane], 4);
+            mbar_init(&sh.s_read[lane], 4), mbar_init(&sh.p_full[lane], 4), mbar_init(&sh.q_full[lane], 4);
             sh.k_tile[lane] = sh.v_tile[lane] = -1;
         }
         if (lane < PT_SEGS) mbar_init(&sh.seg_full[lane], 1), mbar_init(&sh.seg_free[lane], PT_SOFTMAX + 2);
@@ -339,59 +340,68 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
             // and are not kept.)
             const bool own = pair || t == 0 || n > 1;  // this stream has tiles
             const bool mine = q < seg.nq;
-            float q_scale = 0.0f;
-            int high = INT32_MAX, low = 0;
+            float q_scale = 0.0f, sink = -INFINITY;
+            int high = INT32_MAX, low = 0, h = 0;
+            int64_t row = 0;
+            if (mine) {
+                const int qi = seg.q0 + q, row_of = qi / a.group;
+                row = seg.first + row_of;
+                h = seg.head * a.group + qi - row_of * a.group;
+                if (a.sinks) sink = a.sinks[h];
+                if (seg.flat) {
+                    high = min(place_of_row(a.batch, a.kv.page_size, (int)row, a.err), seg.end - 1);
+                } else {
+                    high = max(seg.p0 + row_of, -1);
+                    low = a.window > 0 ? max(high + 1 - a.window, 0) : 0;
+                }
+            }
             if (own && live) {
-                const T *from = nullptr;
-                float inv0 = 0.0f, inv1 = 1.0f;
-                if (mine) {
-                    const int qi = seg.q0 + q, row_of = qi / a.group;
-                    const int64_t row = seg.first + row_of;
-                    from = static_cast<const T *>(a.q.data) + row * a.q.row_stride +
-                           (seg.head * a.group + qi - row_of * a.group) * a.q.head_stride;
-                    if (seg.flat) {
-                        high = min(place_of_row(a.batch, a.kv.page_size, (int)row, a.err), seg.end - 1);
+                // The whole row in registers, every load in flight at once.
+                Raw8<T> raw[D / 8];
+                const T *from = static_cast<const T *>(a.q.data) + row * a.q.row_stride + h * a.q.head_stride;
+#pragma unroll
+                for (int d = 0; d < D / 8; d++) {
+                    if (!mine) {
+#pragma unroll
+                        for (int e = 0; e < (int)sizeof(T) / 2; e++) raw[d].w[e] = make_uint4(0, 0, 0, 0);
+                    } else if (a.q_vec) {
+                        raw[d] = load_raw8(from + 8 * d);
                     } else {
-                        high = max(seg.p0 + row_of, -1);
-                        low = a.window > 0 ? max(high + 1 - a.window, 0) : 0;
+#pragma unroll
+                        for (int e = 0; e < 8; e++) reinterpret_cast<T *>(raw[d].w)[e] = from[8 * d + e];
                     }
                 }
-                auto load = [&](int d, float (&x)[8]) {
-                    if (a.q_vec) {
-                        load8(from + d, x);
-                    } else {
+                // The largest magnitude, as bits, which are in its order (NaN above infinity): of FP32,
+                // or of two BF16 at once.
+                uint32_t most = 0;
 #pragma unroll
-                        for (int e = 0; e < 8; e++) x[e] = load1(from + d + e);
-                    }
-                };
-                if (mine) {
-                    float most = 0.0f;
-                    bool finite = true;
-#pragma unroll 4
-                    for (int d = 0; d < D; d += 8) {
-                        float x[8];
-                        load(d, x);
+                for (int d = 0; d < D / 8; d++)
 #pragma unroll
-                        for (int e = 0; e < 8; e++) {
-                            most = fmaxf(most, fabsf(x[e]));
-                            finite &= fabsf(x[e]) <= FLT_MAX;
+                    for (int e = 0; e < (int)sizeof(T) / 2; e++) {
+                        const uint4 w = raw[d].w[e];
+                        if constexpr (F32) {
+                            most = max(most, max(max(w.x & 0x7FFFFFFFu, w.y & 0x7FFFFFFFu),
+                                                 max(w.z & 0x7FFFFFFFu, w.w & 0x7FFFFFFFu)));
+                        } else {
+                            most = __vmaxu2(most, __vmaxu2(__vmaxu2(w.x & 0x7FFF7FFFu, w.y & 0x7FFF7FFFu),
+                                                           __vmaxu2(w.z & 0x7FFF7FFFu, w.w & 0x7FFF7FFFu)));
                         }
                     }
-                    // A power of two brings the largest element to [2^14, 2^15), in two factors, so
-                    // that FP32's whole range of exponents can be brought there.
-                    const int e = max((int)(__float_as_uint(most) >> 23), 1);
-                    inv0 = finite ? __uint_as_float((uint32_t)(254 - (e + 1) / 2 - 63) << 23) : 0.0f;
-                    inv1 = __uint_as_float((uint32_t)(254 - (e - (e + 1) / 2) - 64) << 23) * 16384.0f;
-                    q_scale = finite ? __uint_as_float((uint32_t)e << 23) * (1.0f / 16384.0f) * a.scale * REACH_LOG2E : NAN;
-                }
+                if constexpr (!F32) most = max(most & 0xFFFFu, most >> 16) << 16;
+                const bool finite = most < 0x7F800000u;
+                // A power of two brings the largest element to [2^14, 2^15); 2^126 at most, which still
+                // brings the least rows to where FP16 holds BF16's 8 bits.
+                const int e = max((int)(most >> 23), 15);
+                const float up = finite ? __uint_as_float((uint32_t)(268 - e) << 23) : 0.0f;
+                q_scale = finite ? __uint_as_float((uint32_t)max(e - 14, 1) << 23) * a.scale * REACH_LOG2E : NAN;
                 if (pair || t == 0) {
                     uint8_t *to = smem + (pair ? t : 0) * TERMS * Shape::OPERAND + r * 128;
-#pragma unroll 1
-                    for (int d = 0; d < D; d += 8) {
-                        float x[8] = {};
-                        if (inv0 != 0.0f) load(d, x);
 #pragma unroll
-                        for (int e = 0; e < 8; e++) x[e] = x[e] * inv0 * inv1;
+                    for (int d = 0; d < D; d += 8) {
+                        float x[8];
+                        unpack8(raw[d / 8], x);
+#pragma unroll
+                        for (int e = 0; e < 8; e++) x[e] = finite ? x[e] * up : 0.0f;
                         const int place = (d >> 6) * PT_PANEL + (((d >> 3 & 7) ^ (r & 7)) << 4);
 #pragma unroll
                         for (int term = 0; term < TERMS; term++) {
@@ -399,9 +409,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
 #pragma unroll
                             for (int e = 0; e < 4; e++) {
                                 w[e] = pt_f16x2(x[2 * e], x[2 * e + 1]);
-                                const float2 b = f16x2_f32x2(w[e]);
-                                x[2 * e] -= b.x;
-                                x[2 * e + 1] -= b.y;
+                                if constexpr (F32) {
+                                    const float2 b = f16x2_f32x2(w[e]);
+                                    x[2 * e] -= b.x;
+                                    x[2 * e + 1] -= b.y;
+                                }
                             }
                             *reinterpret_cast<uint4 *>(to + term * Shape::OPERAND + place) = make_uint4(w[0], w[1], w[2], w[3]);
                         }
@@ -433,7 +445,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                     // for each tile as the others do, not for the next one before they have for this.)
                     if (any) ok = __all_sync(0xffffffffu, mbar_wait(&sh.o_full[t], (c - 1) & 1, abort_flag, a.err));
                     if (!ok) break;
-                    if (lane == 0) mbar_arrive(&sh.p_full[t]);
+                    if (lane == 0) mbar_arrive(&sh.s_read[t]), mbar_arrive(&sh.p_full[t]);
                     __syncwarp();
                     any = true;
                     continue;
@@ -441,53 +453,57 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 ok = __all_sync(0xffffffffu, mbar_wait(&sh.meta_full[k % PT_METAS], (k / PT_METAS) & 1, abort_flag, a.err));
                 if (!ok) break;
                 tc_fence_after();
+                uint32_t raw[128];
+                FO_TMEM_LD32(s_at + 0, (raw + 0));
+                FO_TMEM_LD32(s_at + 32, (raw + 32));
+                FO_TMEM_LD32(s_at + 64, (raw + 64));
+                FO_TMEM_LD32(s_at + 96, (raw + 96));
                 const PtMeta &meta = sh.meta[k % PT_METAS];
                 const int tile = meta.base;
                 int tile_top = meta.top;
-                const int hi = min(high, meta.to - 1), lo = max(low, meta.from);
-                const bool full = __all_sync(
-                    0xffffffffu, hi - tile >= PT_TILE - 1 && (lo <= tile || a.reach.first - tile >= PT_TILE));
-                // Of 32 keys, those that the row sees, as bits.  (Differences that cannot wrap: every
-                // one is of numbers from -1 up.)
-                auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; };
-                auto seen = [&](int w) {
-                    const int b = tile + 32 * w;
-                    return below(min(hi - b, 32) + 1) & (~below(lo - b) | below(a.reach.first - b));
-                };
-                // The row's largest score, in log2 units, 32 keys at a time: the loops are short, since
-                // code of every kind runs on an SM at once and what does not stay in its instruction
-                // cache costs more than the exponentials (the row held in registers and all of it
-                // unrolled: 274 us where this takes MEASURED).
-                float mx = -INFINITY;
-                if (!full) tile_top = PT_LOWEST;
-#pragma unroll 1
-                for (int w = 0; w < 4; w++) {
-                    uint32_t raw[32];
-                    FO_TMEM_LD32(s_at + 32 * w, raw);
-                    const float f0 = meta.ks[2 * w] * q_scale, f1 = meta.ks[2 * w + 1] * q_scale;
-                    float2 x[16];
-                    tmem_wait_ld();
+                float f[8];  // of 16 keys' scores: log2 units
 #pragma unroll
-                    for (int e = 0; e < 16; e++)
-                        x[e] = __fmul2_rn(make_float2(__uint_as_float(raw[2 * e]), __uint_as_float(raw[2 * e + 1])),
-                                          e < 8 ? make_float2(f0, f0) : make_float2(f1, f1));
-                    if (!full) {
-                        const uint32_t see = seen(w);
+                for (int g = 0; g < 8; g++) f[g] = meta.ks[g] * q_scale;
+                const int hi = min(high, meta.to - 1), lo = max(low, meta.from);
+                const bool simple = __all_sync(0xffffffffu, hi - tile >= PT_TILE - 1 &&
+                                                                (lo <= tile || a.reach.first - tile >= PT_TILE) &&
+                                                                meta.plain && q_scale >= 0.0f);
+                tmem_wait_ld();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.s_read[t]);
+                if (!simple) {
+                    // Scores themselves, those of keys that the row does not see -infinity.
+                    auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; };
+                    tile_top = PT_LOWEST;
+#pragma unroll
+                    for (int w = 0; w < 4; w++) {
+                        // Keys that the row sees, as bits.  (Differences that cannot wrap: every one is of
+                        // numbers from -1 up.)
+                        const int b = tile + 32 * w;
+                        const uint32_t see = below(min(hi - b, 32) + 1) & (~below(lo - b) | below(a.reach.first - b));
                         if (see & 0x0000FFFFu) tile_top = max(tile_top, pt_above(meta.vs[2 * w]));
                         if (see & 0xFFFF0000u) tile_top = max(tile_top, pt_above(meta.vs[2 * w + 1]));
 #pragma unroll
-                        for (int e = 0; e < 16; e++) {
-                            if (!(see >> (2 * e) & 1)) x[e].x = -INFINITY;
-                            if (!(see >> (2 * e + 1) & 1)) x[e].y = -INFINITY;
+                        for (int e = 0; e < 32; e++) {
+                            const float x = __uint_as_float(raw[32 * w + e]) * f[2 * w + e / 16];
+                            raw[32 * w + e] = see >> e & 1 ? __float_as_uint(x) : 0xFF800000u;
                         }
                     }
-                    float m0 = fmaxf(x[0].x, x[0].y), m1 = fmaxf(x[1].x, x[1].y);
 #pragma unroll
-                    for (int e = 2; e < 16; e += 2) {
-                        m0 = fmaxf(m0, fmaxf(x[e].x, x[e].y));
-                        m1 = fmaxf(m1, fmaxf(x[e + 1].x, x[e + 1].y));
+                    for (int g = 0; g < 8; g++) f[g] = 1.0f;
+                }
+                // The row's largest score.
+                float mx = -INFINITY;
+#pragma unroll
+                for (int g = 0; g < 8; g++) {
+                    float m0 = -INFINITY, m1 = -INFINITY;
+#pragma unroll
+                    for (int e = 0; e < 16; e += 4) {
+                        m0 = fmaxf(fmaxf(m0, __uint_as_float(raw[16 * g + e])), __uint_as_float(raw[16 * g + e + 1]));
+                        m1 = fmaxf(fmaxf(m1, __uint_as_float(raw[16 * g + e + 2])), __uint_as_float(raw[16 * g + e + 3]));
                     }
-                    mx = fmaxf(mx, fmaxf(m0, m1));
+                    mx = fmaxf(mx, fmaxf(m0, m1) * f[g]);
                 }
                 float factor = 1.0f;  // of what has been summed so far
                 if (!any) {
@@ -524,46 +540,31 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 // zeros.
                 const float inverse_top = __uint_as_float((uint32_t)(264 - top) << 23);
                 float2 sum = make_float2(0.0f, 0.0f);
-#pragma unroll 1
+#pragma unroll
                 for (int w = 0; w < 4; w++) {
-                    uint32_t raw[32];
-                    FO_TMEM_LD32(s_at + 32 * w, raw);
-                    const float f0 = meta.ks[2 * w] * q_scale, f1 = meta.ks[2 * w + 1] * q_scale;
                     const float v0 = fminf(meta.vs[2 * w] * inverse_top, FLT_MAX);
                     const float v1 = fminf(meta.vs[2 * w + 1] * inverse_top, FLT_MAX);
-                    const uint32_t see = full ? 0xFFFFFFFFu : seen(w);
-                    tmem_wait_ld();
                     float2 p[16];
+                    uint32_t term[16];
 #pragma unroll
                     for (int e = 0; e < 16; e++) {
-                        const float2 x = __ffma2_rn(make_float2(__uint_as_float(raw[2 * e]), __uint_as_float(raw[2 * e + 1])),
-                                                    e < 8 ? make_float2(f0, f0) : make_float2(f1, f1),
-                                                    make_float2(-shift, -shift));
+                        const float g = f[2 * w + e / 8], v = e < 8 ? v0 : v1;
+                        const float2 x = __ffma2_rn(make_float2(__uint_as_float(raw[32 * w + 2 * e]),
+                                                                __uint_as_float(raw[32 * w + 2 * e + 1])),
+                                                    make_float2(g, g), make_float2(-shift, -shift));
                         p[e] = make_float2(ex2(x.x), ex2(x.y));
-                    }
-                    if (!full) {
-#pragma unroll
-                        for (int e = 0; e < 16; e++) {
-                            if (!(see >> (2 * e) & 1)) p[e].x = 0.0f;
-                            if (!(see >> (2 * e + 1) & 1)) p[e].y = 0.0f;
-                        }
-                    }
-                    uint32_t hi_term[16];
-#pragma unroll
-                    for (int e = 0; e < 16; e++) {
                         sum = __fadd2_rn(sum, p[e]);
-                        p[e] = __fmul2_rn(p[e], e < 8 ? make_float2(v0, v0) : make_float2(v1, v1));
-                        hi_term[e] = pt_f16x2(p[e].x, p[e].y);
+                        p[e] = __fmul2_rn(p[e], make_float2(v, v));
+                        term[e] = pt_f16x2(p[e].x, p[e].y);
                     }
-                    // (In S's place P's columns are of keys that have been read.)
-                    FO_TMEM_ST16(p_at + 16 * TERMS * w, hi_term);
+                    FO_TMEM_ST16(p_at + 16 * TERMS * w, term);
                     if constexpr (F32) {
 #pragma unroll
                         for (int e = 0; e < 16; e++) {
-                            const float2 b = f16x2_f32x2(hi_term[e]);
-                            hi_term[e] = pt_f16x2(p[e].x - b.x, p[e].y - b.y);
+                            const float2 b = f16x2_f32x2(term[e]);
+                            term[e] = pt_f16x2(p[e].x - b.x, p[e].y - b.y);
                         }
-                        FO_TMEM_ST16(p_at + 16 * TERMS * w + 16, hi_term);
+                        FO_TMEM_ST16(p_at + 16 * TERMS * w + 16, term);
                     }
                 }
                 l += sum.x + sum.y;
@@ -608,8 +609,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 o_from = 0;
             }
             if (live) {
-                const int qi = seg.q0 + q, row_of = qi / a.group, h = seg.head * a.group + qi - row_of * a.group;
-                const int64_t row = seg.first + row_of;
                 const int part = seg.part;
                 float inv = 0.0f, fp = 0.0f;
                 const int64_t at_row = row * a.q.heads + h;
@@ -625,13 +624,31 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                         f1 *= j.f0;
                         fp = j.f1;
                     }
-                    inv = inverse_sum(a.sinks, h, m, l);
+                    inv = inverse_sum(sink, m, l);
                     if (a.lse && (pair || t == 0)) a.lse[at_row] = log_sum(m, l);
                 } else if (mine && (pair || t == 0)) {
                     reinterpret_cast<float2 *>(a.part_ml)[(int64_t)part * FO_TILES_QUERIES + q] = make_float2(m, l);
                 }
+                T *out = static_cast<T *>(a.out.data) + row * a.out.row_stride + h * a.out.head_stride;
+                // Finished rows of one stream, as most are, 32 dimensions at a time.
+                const bool simple = !has1 && part < 0 && !a.reach.raw_o && !a.reach.prior_o && a.out_vec;
+                if (simple) {
+                    const float scale = f0 * inv;
 #pragma unroll 1
-                for (int d = c0; d < c1; d += 16) {
+                    for (int d = c0; d < c1; d += 32) {
+                        uint32_t o[32];
+                        float v[32];
+                        FO_TMEM_LD32(o_at(o_from) + d, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; e++) v[e] = __uint_as_float(o[e]) * scale;
+                        if (!mine) continue;
+#pragma unroll
+                        for (int e = 0; e < 32; e += 8) store8(out + d + e, v + e);
+                    }
+                }
+#pragma unroll 1
+                for (int d = simple ? c1 : c0; d < c1; d += 16) {
                     uint32_t o[16];
                     float v[16];
                     if (has0) {
@@ -670,8 +687,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                     }
 #pragma unroll
                     for (int e = 0; e < 16; e++) v[e] *= inv;
-                    pt_store16(static_cast<T *>(a.out.data) + row * a.out.row_stride + h * a.out.head_stride + d, v,
-                               a.out_vec);
+                    pt_store16(out + d, v, a.out_vec);
                 }
             }
             if (!pair) {
@@ -868,7 +884,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                     meta.ks[lane] = ks8;
                     meta.vs[lane] = vs8;
                 }
-                if (lane == 8) meta.top = pt_above(most);
+                const bool plain = __all_sync(0xffffffffu, ks >= 0.0f);
+                if (lane == 8) meta.top = pt_above(most), meta.plain = plain;
                 if (lane == 9) meta.base = now.base;
                 if (lane == 10) meta.pages = mask;
                 if (lane == 11) meta.from = now.from, meta.to = now.to;
@@ -1024,11 +1041,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 bool issued = false;
                 const bool same = i < n;  // the next tile is of the same segment
                 if (same) next = take();
-                ok = __all_sync(0xffffffffu, mbar_wait(&sh.p_full[t], c & 1, abort_flag, a.err));
-                if (!ok) break;
-                tc_fence_after();
                 if (!ALIAS && same) {
-                    // S first, if its keys are there: it is what the softmax waits for next.
+                    // The next S is computed while the softmax is at this one, which it holds in
+                    // registers, if its keys are there.
+                    ok = __all_sync(0xffffffffu, mbar_wait(&sh.s_read[t], c & 1, abort_flag, a.err));
+                    if (!ok) break;
                     issued = __all_sync(0xffffffffu, *(volatile int *)&sh.k_tile[next.k & 1] == next.k &&
                                                          mbar_test(&sh.k_full[next.k & 1], (next.k >> 1) & 1));
                     if (issued) {
@@ -1036,6 +1053,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                         issue_s(next);
                     }
                 }
+                ok = __all_sync(0xffffffffu, mbar_wait(&sh.p_full[t], c & 1, abort_flag, a.err));
+                if (!ok) break;
+                tc_fence_after();
                 ok = __all_sync(0xffffffffu, there(sh.v_full, sh.v_tile, now.k));
                 if (!ok) break;
                 tc_fence_after();
@@ -1121,7 +1141,7 @@ __global__ void __launch_bounds__(PJ_THREADS) paged_join_kernel(const __grid_con
         if (quad0 == 0) reinterpret_cast<float2 *>(a.reach.raw_ml)[at_row] = make_float2(m, l);
         return;
     }
-    const float inv = inverse_sum(a.sinks, h, m, l);
+    const float inv = inverse_sum(a.sinks ? a.sinks[h] : -INFINITY, m, l);
     T *out = static_cast<T *>(a.out.data) + row * a.out.row_stride + h * a.out.head_stride;
 #pragma unroll
     for (int i = 0; i < MINE; i++) {
