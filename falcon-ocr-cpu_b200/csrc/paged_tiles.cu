@@ -98,7 +98,7 @@ struct PtSegment {
 struct PtMeta {
     float ks[8], vs[8];  // keys' and values' scales of each 16 positions' page
     int top;             // exponent bits of a power of two above the values' scales
-    int plain;           // the keys' scales are numbers from 0 up
+    int plain;           // the keys' scales are numbers above 0
     int base;            // the tile's first position
     int from, to;        // positions [from, to) that rows may see of it
     unsigned pages;      // pages that were copied
@@ -113,7 +113,8 @@ struct PtShared {
     uint64_t q_full[2], q_both;  // a stream's queries are there; those of the first that the second uses too
     uint64_t seg_full[PT_SEGS], seg_free[PT_SEGS];
     uint64_t meta_full[PT_METAS];
-    uint64_t x_full, x_free, done;
+    uint64_t x_full, x_free, done, ended;
+    uint64_t turn[2][4];  // the exponentials of a stream's warp are done
     PtSegment seg[PT_SEGS];
     PtMeta meta[PT_METAS];
     int k_tile[2], v_tile[2];  // the tile that the operands are, or will be, of
@@ -122,6 +123,16 @@ struct PtShared {
     int begin_item, begin_base, abort;
     uint32_t tmem;
 };
+
+// Waits for `phase` of `bar`, all lanes of a warp; false when the block gives up.  The bound
+// is kept by a warp that does nothing else (the last one): when no tile has come
+// along for FO_WAIT_NS it raises the flag.  (A clock in every wait is 60
+// instructions each, of the few thousand that stay in the instruction cache.)
+__device__ __forceinline__ bool pt_wait(uint64_t *bar, uint32_t phase, volatile int *abort_flag) {
+    bool ok = true;
+    while (!mbar_try_wait(bar, phase) && (ok = !*abort_flag)) {}
+    return __all_sync(0xffffffffu, ok);
+}
 
 // ------------------------------------------------------------------ the line
 // An item of the line: a unit of query rows of a sequence, for each KV head; or a
@@ -268,7 +279,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
         if (lane < PT_METAS) mbar_init(&sh.meta_full[lane], 1);
         if (lane == 31) {
             mbar_init(&sh.x_full, PT_SOFTMAX), mbar_init(&sh.x_free, PT_SOFTMAX), mbar_init(&sh.done, 2);
-            mbar_init(&sh.q_both, 4);
+            mbar_init(&sh.q_both, 4), mbar_init(&sh.ended, PT_THREADS / 32 - 1);
+            for (int i = 0; i < 8; i++) mbar_init(&sh.turn[i & 1][i >> 1], 1);
             sh.abort = 0;
         }
         mbar_fence_init();
@@ -280,35 +292,37 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
     // This block's piece [begin, end) of the line, and where it begins.  (The
     // line's tiles are below 2^31, checked on the host.)
     const int n_items = a.reach.over_groups ? a.reach.n_groups + 2 : (int)a.batch.n_seqs * a.q_units;
-    int per, begin, count;
-    {
-        auto work = [&](int index) {
-            if (index >= n_items) return 0;
-            const PtItem x = pt_item<QUERIES>(a, index);
-            return x.tiles * x.units;
-        };
-        int mine = work(tid), chunk, before = pt_scan(mine, sh, chunk), all = chunk;
-        for (int first = PT_THREADS; first < n_items; first += PT_THREADS) {
-            int more;
-            pt_scan(work(first + tid), sh, more);
-            all += more;
+    int per = 0, begin = 0, count = 0;
+    // The line's length first, then the item that the piece begins in; with no more items than
+    // threads at one go.
+#pragma unroll 1
+    for (bool known = false;;) {
+        int all = 0;
+#pragma unroll 1
+        for (int first = 0; first < n_items; first += PT_THREADS) {
+            int mine = 0, chunk;
+            if (first + tid < n_items) {
+                const PtItem x = pt_item<QUERIES>(a, first + tid);
+                mine = x.tiles * x.units;
+            }
+            const int before = all + pt_scan(mine, sh, chunk);
+            all += chunk;
+            if (!known && n_items <= PT_THREADS) {
+                known = true;
+                per = max((int)((unsigned)(all + gridDim.x - 1) / gridDim.x), 2);
+                begin = (int)min((long long)per * blockIdx.x, (long long)all);
+                count = (int)min((long long)per, (long long)all - begin);
+            }
+            if (known && begin >= before && begin < before + mine) {
+                sh.begin_item = first + tid;
+                sh.begin_base = before;
+            }
         }
+        if (known) break;
+        known = true;
         per = max((int)((unsigned)(all + gridDim.x - 1) / gridDim.x), 2);
         begin = (int)min((long long)per * blockIdx.x, (long long)all);
         count = (int)min((long long)per, (long long)all - begin);
-        if (count > 0) {
-            for (int first = 0, sum = 0;;) {
-                if (begin >= sum + before && begin < sum + before + mine) {
-                    sh.begin_item = first + tid;
-                    sh.begin_base = sum + before;
-                }
-                first += PT_THREADS;
-                if (first >= n_items) break;
-                sum += chunk;
-                mine = work(first + tid);
-                before = pt_scan(mine, sh, chunk);
-            }
-        }
     }
     tc_fence_before();
     __syncthreads();
@@ -327,10 +341,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
         const uint32_t at = tmem + ((uint32_t)(32 * wq) << 16);
         const uint32_t s_at = at + 128 * t, p_at = ALIAS ? s_at : at + 384 + 64 * t;
         auto o_at = [&](int stream) { return at + 256 + (ALIAS ? 128 : 64) * stream; };
+        int turns = 0;  // tiles that this warp and the other stream's have taken turns at
         int c = 0, x_phase = 0, both_phase = 0;  // tiles of this stream so far; joins of both streams; queries of both
         bool ok = true;
         for (int s = 0; ok; s++) {
-            ok = __all_sync(0xffffffffu, mbar_wait(&sh.seg_full[s % PT_SEGS], (s / PT_SEGS) & 1, abort_flag, a.err));
+            ok = pt_wait(&sh.seg_full[s % PT_SEGS], (s / PT_SEGS) & 1, abort_flag);
             if (!ok) break;
             const PtSegment &seg = sh.seg[s % PT_SEGS];
             const int n = seg.n, base = seg.base, pair = seg.pair, last = seg.last;
@@ -396,26 +411,44 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 q_scale = finite ? __uint_as_float((uint32_t)max(e - 14, 1) << 23) * a.scale * REACH_LOG2E : NAN;
                 if (pair || t == 0) {
                     uint8_t *to = smem + (pair ? t : 0) * TERMS * Shape::OPERAND + r * 128;
+                    auto place = [&](int d) { return (d >> 6) * PT_PANEL + (((d >> 3 & 7) ^ (r & 7)) << 4); };
+                    if constexpr (!F32) {
+                        // As they are into their places, and there to FP16 (a short loop, for the
+                        // instruction cache).
 #pragma unroll
-                    for (int d = 0; d < D; d += 8) {
-                        float x[8];
-                        unpack8(raw[d / 8], x);
+                        for (int d = 0; d < D; d += 8) *reinterpret_cast<uint4 *>(to + place(d)) = raw[d / 8].w[0];
+#pragma unroll 1
+                        for (int d = 0; d < D; d += 8) {
+                            uint4 *at = reinterpret_cast<uint4 *>(to + place(d));
+                            Raw8<T> y;
+                            y.w[0] = *at;
+                            float x[8];
+                            unpack8(y, x);
 #pragma unroll
-                        for (int e = 0; e < 8; e++) x[e] = finite ? x[e] * up : 0.0f;
-                        const int place = (d >> 6) * PT_PANEL + (((d >> 3 & 7) ^ (r & 7)) << 4);
+                            for (int e = 0; e < 8; e++) x[e] = finite ? x[e] * up : 0.0f;
+                            *at = make_uint4(pt_f16x2(x[0], x[1]), pt_f16x2(x[2], x[3]), pt_f16x2(x[4], x[5]),
+                                             pt_f16x2(x[6], x[7]));
+                        }
+                    } else {
 #pragma unroll
-                        for (int term = 0; term < TERMS; term++) {
-                            uint32_t w[4];
+                        for (int d = 0; d < D; d += 8) {
+                            float x[8];
+                            unpack8(raw[d / 8], x);
 #pragma unroll
-                            for (int e = 0; e < 4; e++) {
-                                w[e] = pt_f16x2(x[2 * e], x[2 * e + 1]);
-                                if constexpr (F32) {
+                            for (int e = 0; e < 8; e++) x[e] = finite ? x[e] * up : 0.0f;
+#pragma unroll
+                            for (int term = 0; term < 2; term++) {
+                                uint32_t w[4];
+#pragma unroll
+                                for (int e = 0; e < 4; e++) {
+                                    w[e] = pt_f16x2(x[2 * e], x[2 * e + 1]);
                                     const float2 b = f16x2_f32x2(w[e]);
                                     x[2 * e] -= b.x;
                                     x[2 * e + 1] -= b.y;
                                 }
+                                *reinterpret_cast<uint4 *>(to + term * Shape::OPERAND + place(d)) =
+                                    make_uint4(w[0], w[1], w[2], w[3]);
                             }
-                            *reinterpret_cast<uint4 *>(to + term * Shape::OPERAND + place) = make_uint4(w[0], w[1], w[2], w[3]);
                         }
                     }
                     fence_proxy_async_smem();
@@ -428,7 +461,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                     if (!pair && n > 1) mbar_arrive(&sh.q_both);
                 }
             } else if (own) {
-                ok = __all_sync(0xffffffffu, mbar_wait(&sh.q_both, both_phase, abort_flag, a.err));
+                ok = pt_wait(&sh.q_both, both_phase, abort_flag);
                 if (!ok) break;
                 if (lane == 0) mbar_arrive(&sh.q_full[t]);
             }
@@ -436,47 +469,39 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
             float m = -INFINITY, l = 0.0f;
             int top = PT_LOWEST;  // exponent bits of a power of two above the scales of the values that the row sees
             bool any = false;
+            const bool turning = pair && 128 + 32 * wq < seg.nq;  // both have queries
             for (int i = pair ? 0 : t; i < n; i += pair ? 1 : 2, c++) {
                 const int k = base + i;
-                ok = __all_sync(0xffffffffu, mbar_wait(&sh.s_full[t], c & 1, abort_flag, a.err));
+                ok = pt_wait(&sh.s_full[t], c & 1, abort_flag);
                 if (!ok) break;
                 if (!live) {
                     // No query in this warp: whatever its lanes hold stays theirs.  (It arrives once
                     // for each tile as the others do, not for the next one before they have for this.)
-                    if (any) ok = __all_sync(0xffffffffu, mbar_wait(&sh.o_full[t], (c - 1) & 1, abort_flag, a.err));
+                    if (any) ok = pt_wait(&sh.o_full[t], (c - 1) & 1, abort_flag);
                     if (!ok) break;
                     if (lane == 0) mbar_arrive(&sh.s_read[t]), mbar_arrive(&sh.p_full[t]);
                     __syncwarp();
                     any = true;
                     continue;
                 }
-                ok = __all_sync(0xffffffffu, mbar_wait(&sh.meta_full[k % PT_METAS], (k / PT_METAS) & 1, abort_flag, a.err));
+                ok = pt_wait(&sh.meta_full[k % PT_METAS], (k / PT_METAS) & 1, abort_flag);
                 if (!ok) break;
                 tc_fence_after();
-                uint32_t raw[128];
-                FO_TMEM_LD32(s_at + 0, (raw + 0));
-                FO_TMEM_LD32(s_at + 32, (raw + 32));
-                FO_TMEM_LD32(s_at + 64, (raw + 64));
-                FO_TMEM_LD32(s_at + 96, (raw + 96));
                 const PtMeta &meta = sh.meta[k % PT_METAS];
                 const int tile = meta.base;
                 int tile_top = meta.top;
-                float f[8];  // of 16 keys' scores: log2 units
-#pragma unroll
-                for (int g = 0; g < 8; g++) f[g] = meta.ks[g] * q_scale;
                 const int hi = min(high, meta.to - 1), lo = max(low, meta.from);
-                const bool simple = __all_sync(0xffffffffu, hi - tile >= PT_TILE - 1 &&
-                                                                (lo <= tile || a.reach.first - tile >= PT_TILE) &&
-                                                                meta.plain && q_scale >= 0.0f);
-                tmem_wait_ld();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.s_read[t]);
-                if (!simple) {
-                    // Scores themselves, those of keys that the row does not see -infinity.
+                const bool plain = __all_sync(0xffffffffu, meta.plain && q_scale > 0.0f);
+                const bool all = hi - tile >= PT_TILE - 1 && (lo <= tile || a.reach.first - tile >= PT_TILE);
+                if (!__all_sync(0xffffffffu, plain && all)) {
+                    // Scores of keys that the row does not see become -infinity in tensor memory, 32 keys
+                    // at a time, where a row of the warp does not see them all.  (Code of every kind runs
+                    // on an SM at once, and what does not stay in its instruction cache costs more than
+                    // these round trips: 128 masks in line took 3,000 cycles.)  Scales that would make
+                    // something else of -infinity are multiplied here.
                     auto below = [](int n) { return n <= 0 ? 0u : n >= 32 ? 0xFFFFFFFFu : (1u << n) - 1u; };
                     tile_top = PT_LOWEST;
-#pragma unroll
+#pragma unroll 1
                     for (int w = 0; w < 4; w++) {
                         // Keys that the row sees, as bits.  (Differences that cannot wrap: every one is of
                         // numbers from -1 up.)
@@ -484,15 +509,33 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                         const uint32_t see = below(min(hi - b, 32) + 1) & (~below(lo - b) | below(a.reach.first - b));
                         if (see & 0x0000FFFFu) tile_top = max(tile_top, pt_above(meta.vs[2 * w]));
                         if (see & 0xFFFF0000u) tile_top = max(tile_top, pt_above(meta.vs[2 * w + 1]));
+                        if (__all_sync(0xffffffffu, plain && see == 0xFFFFFFFFu)) continue;
+                        uint32_t x[32];
+                        FO_TMEM_LD32(s_at + 32 * w, x);
+                        const float f0 = plain ? 1.0f : meta.ks[2 * w] * q_scale;
+                        const float f1 = plain ? 1.0f : meta.ks[2 * w + 1] * q_scale;
+                        tmem_wait_ld();
 #pragma unroll
                         for (int e = 0; e < 32; e++) {
-                            const float x = __uint_as_float(raw[32 * w + e]) * f[2 * w + e / 16];
-                            raw[32 * w + e] = see >> e & 1 ? __float_as_uint(x) : 0xFF800000u;
+                            const float y = __uint_as_float(x[e]) * (e < 16 ? f0 : f1);
+                            x[e] = see >> e & 1 ? __float_as_uint(y) : 0xFF800000u;
                         }
+                        FO_TMEM_ST32(s_at + 32 * w, x);
+                        tmem_wait_st();
                     }
-#pragma unroll
-                    for (int g = 0; g < 8; g++) f[g] = 1.0f;
                 }
+                uint32_t raw[128];
+                FO_TMEM_LD32(s_at + 0, (raw + 0));
+                FO_TMEM_LD32(s_at + 32, (raw + 32));
+                FO_TMEM_LD32(s_at + 64, (raw + 64));
+                FO_TMEM_LD32(s_at + 96, (raw + 96));
+                float f[8];  // of 16 keys' scores: log2 units
+#pragma unroll
+                for (int g = 0; g < 8; g++) f[g] = plain ? meta.ks[g] * q_scale : 1.0f;
+                tmem_wait_ld();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.s_read[t]);
                 // The row's largest score.
                 float mx = -INFINITY;
 #pragma unroll
@@ -521,7 +564,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 const float shift = m == -INFINITY ? 0.0f : m;
                 // P may be written, and O touched, once the PV before is complete.
                 if (any) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(&sh.o_full[t], (c - 1) & 1, abort_flag, a.err));
+                    ok = pt_wait(&sh.o_full[t], (c - 1) & 1, abort_flag);
                     if (!ok) break;
                     if (__any_sync(0xffffffffu, factor != 1.0f)) {
                         tc_fence_after();
@@ -535,6 +578,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                             FO_TMEM_ST16(o_at(t) + d, o);
                         }
                     }
+                }
+                // The two streams' warps of an SM's quarter take turns at the exponentials, which its special
+                // function unit bounds; the one that is not at them does the rest.
+                if (turning && (t == 1 || turns > 0)) {
+                    ok = pt_wait(&sh.turn[t ^ 1][wq], (t == 1 ? turns : turns - 1) & 1, abort_flag);
+                    if (!ok) break;
                 }
                 // Values' scales are taken times 2^10 / top; those of pages that the row does not see meet
                 // zeros.
@@ -568,6 +617,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                     }
                 }
                 l += sum.x + sum.y;
+                if (turning) {
+                    if (lane == 0) mbar_arrive(&sh.turn[t][wq]);
+                    turns++;
+                }
                 tmem_wait_st();
                 tc_fence_before();
                 __syncwarp();
@@ -577,7 +630,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
             if (!ok) break;
             // The segment's end.
             if (any) {
-                ok = __all_sync(0xffffffffu, mbar_wait(&sh.o_full[t], (c - 1) & 1, abort_flag, a.err));
+                ok = pt_wait(&sh.o_full[t], (c - 1) & 1, abort_flag);
                 if (!ok) break;
                 tc_fence_after();
             }
@@ -594,7 +647,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.x_full);
-                ok = __all_sync(0xffffffffu, mbar_wait(&sh.x_full, x_phase, abort_flag, a.err));
+                ok = pt_wait(&sh.x_full, x_phase, abort_flag);
                 if (!ok) break;
                 tc_fence_after();
                 const Joined j = join_parts(sh.xm[0][r], sh.xl[0][r], sh.xm[1][r], sh.xl[1][r]);
@@ -633,6 +686,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 // Finished rows of one stream, as most are, 32 dimensions at a time.
                 const bool simple = !has1 && part < 0 && !a.reach.raw_o && !a.reach.prior_o && a.out_vec;
                 if (simple) {
+                    // BF16 rows of a pair by way of the queries' place, which this warp is done with, so
+                    // that eight lanes write 128 bytes of a row.
+                    const bool staged = !F32 && pair;
+                    uint8_t *stage = smem + t * TERMS * Shape::OPERAND + 32 * wq * 128;
                     const float scale = f0 * inv;
 #pragma unroll 1
                     for (int d = c0; d < c1; d += 32) {
@@ -642,9 +699,30 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                         tmem_wait_ld();
 #pragma unroll
                         for (int e = 0; e < 32; e++) v[e] = __uint_as_float(o[e]) * scale;
-                        if (!mine) continue;
+                        if (staged) {
 #pragma unroll
-                        for (int e = 0; e < 32; e += 8) store8(out + d + e, v + e);
+                            for (int e = 0; e < 32; e += 8)
+                                store8(reinterpret_cast<T *>(stage + (d >> 6) * PT_PANEL + lane * 128 +
+                                                             ((((d + e) >> 3 & 7) ^ (lane & 7)) << 4)),
+                                       v + e);
+                        } else if (mine) {
+#pragma unroll
+                            for (int e = 0; e < 32; e += 8) store8(out + d + e, v + e);
+                        }
+                    }
+                    if (staged) {
+                        const long long at_out = row * a.out.row_stride + h * a.out.head_stride;
+                        __syncwarp();
+#pragma unroll 1
+                        for (int x = 0; x < 8 * PANELS; x++) {
+                            const int from = (x & 7) * 4 + (lane >> 3), chunk = lane & 7;  // of the warp's rows
+                            const long long to = __shfl_sync(0xffffffffu, at_out, from);
+                            const uint4 y = *reinterpret_cast<const uint4 *>(stage + (x >> 3) * PT_PANEL + from * 128 +
+                                                                             ((chunk ^ (from & 7)) << 4));
+                            if (q - lane + from < seg.nq)
+                                *reinterpret_cast<uint4 *>(static_cast<T *>(a.out.data) + to + (x >> 3) * 64 + 8 * chunk) = y;
+                        }
+                        __syncwarp();
                     }
                 }
 #pragma unroll 1
@@ -695,7 +773,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.x_free);
-                ok = __all_sync(0xffffffffu, mbar_wait(&sh.x_free, x_phase, abort_flag, a.err));
+                ok = pt_wait(&sh.x_free, x_phase, abort_flag);
                 x_phase ^= 1;
                 if (!ok) break;
             }
@@ -716,12 +794,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 uint64_t *full = value ? &sh.v_full[k & 1] : &sh.k_full[k & 1];
                 uint64_t *empty = value ? &sh.v_empty[k & 1] : &sh.k_empty[k & 1];
                 uint8_t *to = smem + (value ? Shape::OFF_V : Shape::OFF_K) + (k & 1) * Shape::OPERAND;
-                if (k > 1) ok = __all_sync(0xffffffffu, mbar_wait(empty, (k / 2 - 1) & 1, abort_flag, a.err));
+                if (k > 1) ok = pt_wait(empty, (k / 2 - 1) & 1, abort_flag);
                 if (!ok) break;
                 if (ct == 0) *(volatile int *)(value ? &sh.v_tile[k & 1] : &sh.k_tile[k & 1]) = k;
 #pragma unroll 1
                 for (int h = 0; h < PARTS; h++) {
-                    ok = __all_sync(0xffffffffu, mbar_wait(&sh.code_full[slot], round & 1, abort_flag, a.err));
+                    ok = pt_wait(&sh.code_full[slot], round & 1, abort_flag);
                     if (!ok) break;
                     const uint4 *from = reinterpret_cast<const uint4 *>(smem + Shape::OFF_CODES + slot * PT_SLOT);
                     const unsigned pages = sh.meta[k % PT_METAS].pages;
@@ -760,9 +838,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
         if (warp == PT_PRODUCER) {
             // --------------------------------------------------------- producer
             const int page = a.kv.page_size, log_page = 31 - __clz(page), pages = max(PT_TILE >> log_page, 1);
-            PtItem item = pt_item<QUERIES>(a, sh.begin_item);
-            int index = sh.begin_item;
-            int unit = (begin - sh.begin_base) / item.tiles, tile = (begin - sh.begin_base) - unit * item.tiles;
+            PtItem item;
+            item.units = 0;
+            int index = sh.begin_item - 1, unit = 0, tile = 0;
             int segs = 0, ahead = 0, left = 0, head = 0;
             bool ok = true;
             if (lane == 0) a.joins[8 * blockIdx.x] = 0;
@@ -777,6 +855,15 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 x.ks = x.vs = 0.0f;
                 x.wanted = x.bad = false;
                 if (ahead >= count || !ok) return x;
+                if (unit == item.units) {
+                    do item = pt_item<QUERIES>(a, ++index);
+                    while (item.units == 0 && index < n_items - 1);
+                    unit = 0;
+                    if (ahead == 0) {
+                        unit = (begin - sh.begin_base) / item.tiles;
+                        tile = (begin - sh.begin_base) - unit * item.tiles;
+                    }
+                }
                 if (left == 0) {
                     // A new segment: the rest of the unit, or of the block's piece.
                     const int n = min(item.tiles - tile, count - ahead);
@@ -784,8 +871,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                     const int heads = a.kv.n_kv_heads, q_unit = a.reach.over_groups ? unit / heads : 0;
                     head = unit - q_unit * heads;
                     if (segs >= PT_SEGS)
-                        ok = __all_sync(0xffffffffu, mbar_wait(&sh.seg_free[segs % PT_SEGS], (segs / PT_SEGS - 1) & 1,
-                                                               abort_flag, a.err));
+                        ok = pt_wait(&sh.seg_free[segs % PT_SEGS], (segs / PT_SEGS - 1) & 1, abort_flag);
                     if (!ok) return x;
                     if (lane == 0) {
                         PtSegment &g = sh.seg[segs % PT_SEGS];
@@ -841,13 +927,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 left--;
                 if (++tile == item.tiles) {
                     tile = 0;
-                    if (++unit == item.units) {
-                        unit = 0;
-                        if (ahead < count) {
-                            do item = pt_item<QUERIES>(a, ++index);
-                            while (item.units == 0 && index < n_items - 1);
-                        }
-                    }
+                    unit++;
                 }
                 return x;
             };
@@ -860,19 +940,24 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 x.vs = a.kv.v_scales[at];
             };
             int slot = 0, round = 0, issued = 0;
-            Next now = fetch(), next = fetch();
-            scales(now);
-            for (int k = 0; k < count && ok; k++) {
-                const Next later = fetch();
+            Next now = {}, next = {}, later = {};
+            // Page numbers two tiles ahead, scales one.
+#pragma unroll 1
+            for (int k = -2; k < count && ok; k++) {
+                now = next;
+                next = later;
+                later = fetch();
                 scales(next);
+                if (k < 0) continue;
                 if (!ok) break;
-                if (round > 0) ok = __all_sync(0xffffffffu, mbar_wait(&sh.code_empty[slot], (round - 1) & 1, abort_flag, a.err));
+                if (round > 0) ok = pt_wait(&sh.code_empty[slot], (round - 1) & 1, abort_flag);
                 if (!ok) break;
                 // The tile's scales.  A page number outside the pool, or a scale that is not finite,
                 // gives NaN to the rows that see the page, by their scores.
                 const bool load = now.wanted && !now.bad, sane = load && fabsf(now.vs) <= FLT_MAX;
                 if (now.bad) atomicOr(a.err, FO_DEVERR_PAGED);
-                const float ks = now.wanted && !sane ? NAN : now.ks, vs = sane ? now.vs : 0.0f;
+                // (That of a page that no row sees is never used.)
+                const float ks = !now.wanted ? 1.0f : !sane ? NAN : now.ks, vs = sane ? now.vs : 0.0f;
                 const float most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(fabsf(vs))));
                 PtMeta &meta = sh.meta[k % PT_METAS];
                 const unsigned mask = __ballot_sync(0xffffffffu, load);
@@ -884,7 +969,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                     meta.ks[lane] = ks8;
                     meta.vs[lane] = vs8;
                 }
-                const bool plain = __all_sync(0xffffffffu, ks >= 0.0f);
+                const bool plain = __all_sync(0xffffffffu, ks > 0.0f);
                 if (lane == 8) meta.top = pt_above(most), meta.plain = plain;
                 if (lane == 9) meta.base = now.base;
                 if (lane == 10) meta.pages = mask;
@@ -894,7 +979,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
 #pragma unroll 1
                 for (int p = 0; p < 2 * PARTS; p++) {
                     if (p > 0 && round > 0) {
-                        ok = __all_sync(0xffffffffu, mbar_wait(&sh.code_empty[slot], (round - 1) & 1, abort_flag, a.err));
+                        ok = pt_wait(&sh.code_empty[slot], (round - 1) & 1, abort_flag);
                         if (!ok) break;
                     }
                     // This slot's rows [h, h + 128 / PARTS) of the tile's.
@@ -914,8 +999,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                     issued++;
                     if (++slot == SLOTS) slot = 0, round++;
                 }
-                now = next;
-                next = later;
             }
             if (lane == 0) {
                 // The copies in flight land before the block ends, also where another warp gave up.
@@ -982,20 +1065,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
             // cannot tell a phase from the one two before; once the operands' tile number is k, the phase
             // before is over.
             auto there = [&](uint64_t *full, const int *number, int k) {
-                const uint32_t phase = (k >> 1) & 1;
-                uint64_t t0 = 0;
-                for (uint32_t it = 1;; it++) {
-                    if (!mbar_wait(full + (k & 1), phase, abort_flag, a.err)) return false;
-                    if (*(const volatile int *)(number + (k & 1)) == k)
-                        return mbar_wait(full + (k & 1), phase, abort_flag, a.err);
-                    if ((it & 63) != 0) continue;
-                    if (*abort_flag) return false;
-                    if (t0 == 0) t0 = globaltimer();
-                    if (globaltimer() - t0 > FO_WAIT_NS) {
-                        *abort_flag = 1;
-                        atomicOr(a.err, FO_DEVERR_WAIT_TIMEOUT);
-                        return false;
-                    }
+                for (;;) {
+                    if (!pt_wait(full + (k & 1), (k >> 1) & 1, abort_flag)) return false;
+                    if (__all_sync(0xffffffffu, *(const volatile int *)(number + (k & 1)) == k))
+                        return pt_wait(full + (k & 1), (k >> 1) & 1, abort_flag);
+                    if (__any_sync(0xffffffffu, *abort_flag)) return false;
                 }
             };
             // The stream's place: the next tile of its own is i of segment seg.
@@ -1010,7 +1084,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                     }
                     if (last) return false;
                     seg++;
-                    ok = __all_sync(0xffffffffu, mbar_wait(&sh.seg_full[seg % PT_SEGS], (seg / PT_SEGS) & 1, abort_flag, a.err));
+                    ok = pt_wait(&sh.seg_full[seg % PT_SEGS], (seg / PT_SEGS) & 1, abort_flag);
                     if (!ok) return false;
                     const PtSegment &g = sh.seg[seg % PT_SEGS];
                     n = g.n;
@@ -1019,7 +1093,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                     last = g.last;
                     i = pair ? 0 : t;
                 }
-                ok = __all_sync(0xffffffffu, mbar_wait(&sh.q_full[t], loads & 1, abort_flag, a.err));
+                ok = pt_wait(&sh.q_full[t], loads & 1, abort_flag);
                 loads++;
                 return ok;
             };
@@ -1032,7 +1106,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
             Tile now = {};
             if (more) {
                 now = take();
-                ok = __all_sync(0xffffffffu, there(sh.k_full, sh.k_tile, now.k));
+                ok = (there(sh.k_full, sh.k_tile, now.k));
                 tc_fence_after();
                 if (ok) issue_s(now);
             }
@@ -1044,7 +1118,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 if (!ALIAS && same) {
                     // The next S is computed while the softmax is at this one, which it holds in
                     // registers, if its keys are there.
-                    ok = __all_sync(0xffffffffu, mbar_wait(&sh.s_read[t], c & 1, abort_flag, a.err));
+                    ok = pt_wait(&sh.s_read[t], c & 1, abort_flag);
                     if (!ok) break;
                     issued = __all_sync(0xffffffffu, *(volatile int *)&sh.k_tile[next.k & 1] == next.k &&
                                                          mbar_test(&sh.k_full[next.k & 1], (next.k >> 1) & 1));
@@ -1053,10 +1127,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                         issue_s(next);
                     }
                 }
-                ok = __all_sync(0xffffffffu, mbar_wait(&sh.p_full[t], c & 1, abort_flag, a.err));
+                ok = pt_wait(&sh.p_full[t], c & 1, abort_flag);
                 if (!ok) break;
                 tc_fence_after();
-                ok = __all_sync(0xffffffffu, there(sh.v_full, sh.v_tile, now.k));
+                ok = (there(sh.v_full, sh.v_tile, now.k));
                 if (!ok) break;
                 tc_fence_after();
                 issue_pv(now);
@@ -1066,8 +1140,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                         if (!more) break;
                         next = take();
                     }
-                    ok = __all_sync(0xffffffffu, there(sh.k_full, sh.k_tile, next.k));
-                    if (ok && ALIAS) ok = __all_sync(0xffffffffu, mbar_wait(&sh.o_full[t], c & 1, abort_flag, a.err));
+                    ok = (there(sh.k_full, sh.k_tile, next.k));
+                    if (ok && ALIAS) ok = pt_wait(&sh.o_full[t], c & 1, abort_flag);
                     if (!ok) break;
                     tc_fence_after();
                     issue_s(next);
@@ -1079,8 +1153,24 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
             __syncwarp();
             if (lane == 0) mbar_wait_drain(&sh.done, 0);
             __syncwarp();
+        } else {
+            // ---------------------------------------------------------- the bound
+            uint64_t t0 = globaltimer();
+            int seen = 0;
+            while (!mbar_try_wait(&sh.ended, 0)) {
+                __nanosleep(500);
+                const int now = *(volatile int *)&sh.k_tile[0] + *(volatile int *)&sh.k_tile[1];
+                if (now != seen) t0 = globaltimer();
+                seen = now;
+                if (globaltimer() - t0 <= FO_WAIT_NS) continue;
+                *abort_flag = 1;
+                if (lane == 0) atomicOr(a.err, FO_DEVERR_WAIT_TIMEOUT);
+                break;
+            }
+            __syncwarp();
         }
     }
+    if (warp < PT_THREADS / 32 - 1 && lane == 0) mbar_arrive(&sh.ended);
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
