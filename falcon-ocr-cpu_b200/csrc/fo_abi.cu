@@ -1843,10 +1843,11 @@ int make_tile_parts(fo_ctx *ctx) {
     return FO_OK;
 }
 
-// Room for `rows` rows of `dim` that wait to be joined: sums, then {maximum, sum}.
-int make_waiting(fo_ctx *ctx, int64_t rows, int64_t dim, float **o, float **ml) {
+// Room for `rows` rows of `dim` that wait to be joined: sums, {maximum, sum}, and
+// where a row's parts are.
+int make_waiting(fo_ctx *ctx, int64_t rows, int64_t dim, float **o, float **ml, int32_t **parts_of) {
     std::lock_guard<std::mutex> lock(ctx->paged_mutex);
-    const size_t need = (size_t)rows * (size_t)(dim + 2) * 4;
+    const size_t need = (size_t)rows * (size_t)(dim + 4) * 4;
     if (ctx->waiting.empty() || ctx->waiting.back().bytes < need) {
         FO_TRY(refuse_capture(ctx->stream, "an attention of shared beginnings that needs more scratch than any before"));
         // Twice the last one at least, so that all of them are at most twice the largest.
@@ -1857,6 +1858,7 @@ int make_waiting(fo_ctx *ctx, int64_t rows, int64_t dim, float **o, float **ml) 
     }
     *o = (float *)ctx->waiting.back().ptr;
     *ml = *o + rows * dim;
+    *parts_of = (int32_t *)(*ml + rows * 2);
     return FO_OK;
 }
 
@@ -2173,17 +2175,44 @@ int fo_paged_prefix_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged
     // often the beginning is read, so each sequence goes over all it sees.
     if (queries >= FO_PAGED_ALONE) return launch_reach(ctx, kv, batch, q, out, sinks, lse, scale, 0, reach, false);
     float *o = nullptr, *ml = nullptr;
-    FO_TRY(make_waiting(ctx, rows * q->heads, kv->head_dim, &o, &ml));
+    int32_t *parts_of = nullptr;
+    FO_TRY(make_waiting(ctx, rows * q->heads, kv->head_dim, &o, &ml, &parts_of));
+    const bool few = rows * group <= FO_PAGED_FEW * groups->n_groups;  // of the average group
+    if (queries <= FO_PAGED_FEW) {
+        // The shared positions, then each sequence's own.
+        fo_paged_reach shared = reach;
+        shared.over_groups = 1;
+        shared.raw_o = o;
+        shared.raw_ml = ml;
+        if (!few) shared.parts_of = parts_of;
+        FO_TRY(launch_reach(ctx, kv, batch, q, out, nullptr, nullptr, scale, 0, shared, few));
+        fo_paged_own_launch a = {};
+        a.kv = *kv;
+        a.batch = *batch;
+        a.q = *q;
+        a.out = *out;
+        a.sinks = sinks;
+        a.lse = lse;
+        a.scale = scale;
+        a.reach = reach;
+        a.reach.prior_o = o;
+        a.reach.prior_ml = ml;
+        a.reach.parts_of = shared.parts_of;
+        a.part_o = (float *)ctx->tile_parts.ptr;
+        a.part_ml = ctx->tile_part_ml();
+        a.err = ctx->dev_err;
+        cudaError_t e = fo_launch_paged_own(&a, ctx->sms, ctx->stream);
+        return e == cudaSuccess ? FO_OK : cuda_fail(e, "paged attention launch");
+    }
     fo_paged_reach own = reach;
     own.own_only = 1;
     own.raw_o = o;
     own.raw_ml = ml;
-    FO_TRY(launch_reach(ctx, kv, batch, q, out, nullptr, nullptr, scale, 0, own, queries <= FO_PAGED_FEW));
+    FO_TRY(launch_reach(ctx, kv, batch, q, out, nullptr, nullptr, scale, 0, own, false));
     reach.over_groups = 1;
     reach.prior_o = o;
     reach.prior_ml = ml;
-    return launch_reach(ctx, kv, batch, q, out, sinks, lse, scale, 0, reach,
-                        rows * group <= FO_PAGED_FEW * groups->n_groups);
+    return launch_reach(ctx, kv, batch, q, out, sinks, lse, scale, 0, reach, few);
 }
 
 }  // extern "C"

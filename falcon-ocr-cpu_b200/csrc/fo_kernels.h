@@ -253,6 +253,9 @@ struct fo_paged_reach {
     // units, sum of probabilities}: written in place of out, or joined.
     float *raw_o, *raw_ml;
     const float *prior_o, *prior_ml;
+    // Many query rows over groups: where a row's sums are, {first block whose part
+    // it has, last one | its number in the unit << 16}, or {-1, ..}: in raw_o.
+    int32_t *parts_of;
 };
 
 // Attention over the paged cache (paged_attention.cu).
@@ -305,6 +308,22 @@ struct fo_paged_tiles_launch {
     int32_t group, q_units, q_vec, out_vec;
 };
 cudaError_t fo_launch_paged_tiles(const fo_paged_tiles_launch *args, int sms, cudaStream_t stream);
+
+// Each sequence's positions behind the shared ones, for FO_PAGED_FEW query rows of
+// a KV head at most, joined with what the shared ones gave (paged_own.cu).
+struct fo_paged_own_launch {
+    fo_paged_kv kv;
+    fo_paged_batch batch;
+    fo_rows q, out;
+    const float *sinks;
+    float *lse;
+    float scale;
+    struct fo_paged_reach reach;  // prior_o, prior_ml, parts_of
+    const float *part_o, *part_ml;  // of fo_paged_tiles_launch
+    unsigned *err;
+    int32_t group, q_warps, q_vec, out_vec, parts;  // filled in by the launcher
+};
+cudaError_t fo_launch_paged_own(const fo_paged_own_launch *args, int sms, cudaStream_t stream);
 
 // The bounded-wait self-test kernel (selftest.cu).
 cudaError_t fo_launch_bounded_wait(unsigned *err, unsigned long long limit_ns, cudaStream_t stream);

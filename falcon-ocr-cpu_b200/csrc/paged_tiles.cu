@@ -92,6 +92,7 @@ struct PtSegment {
     int pair, last;  // two query tiles; the block's last segment
     int head, first, q0, nq;  // KV head; the rows' first; the unit's queries [q0, q0 + nq) of them
     int p0, end, flat;        // position of the first row; end of what is seen; rows look their positions up
+    int c1;                   // the last block that has tiles of the unit
     int part;                 // scratch of an unfinished unit's part, -1: the unit is whole
 };
 
@@ -682,6 +683,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 } else if (mine && (pair || t == 0)) {
                     reinterpret_cast<float2 *>(a.part_ml)[(int64_t)part * FO_TILES_QUERIES + q] = make_float2(m, l);
                 }
+                // Where the row's sums are, by the block that its unit begins in.
+                if (mine && a.reach.parts_of && (pair || t == 0) && (part < 0 || part & 1))
+                    reinterpret_cast<int2 *>(a.reach.parts_of)[at_row] = make_int2(part < 0 ? -1 : (int)blockIdx.x, seg.c1 | q << 16);
                 T *out = static_cast<T *>(a.out.data) + row * a.out.row_stride + h * a.out.head_stride;
                 // Finished rows of one stream, as most are, 32 dimensions at a time.
                 const bool simple = !has1 && part < 0 && !a.reach.raw_o && !a.reach.prior_o && a.out_vec;
@@ -887,10 +891,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                         g.end = item.end;
                         g.flat = a.reach.over_groups;
                         g.part = -1;
+                        g.c1 = 0;
                         if (n < item.tiles) {
                             const int from = begin + ahead - tile;  // the unit's place in the line
                             const int c0 = from / per, c1 = (from + item.tiles - 1) / per;
                             g.part = 2 * (int)blockIdx.x + (c0 == (int)blockIdx.x ? 1 : 0);
+                            g.c1 = c1;
                             if (c0 == (int)blockIdx.x) {
                                 int *j = a.joins + 8 * blockIdx.x;
                                 j[1] = g.first;
@@ -1282,7 +1288,7 @@ cudaError_t launch_tiles(const fo_paged_tiles_launch &in, int sms, cudaStream_t 
     a.q_units = (int)((a.batch.max_rows * a.group + Shape::QUERIES - 1) / Shape::QUERIES);
     const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(sms, (most + 1) / 2));
     cudaError_t e = launch(kernel, dim3(grid), dim3(PT_THREADS), Shape::SMEM, stream, a);
-    if (e != cudaSuccess || grid == 1) return e;
+    if (e != cudaSuccess || grid == 1 || a.reach.parts_of) return e;
     return launch(paged_join_kernel<D, F32>, dim3(grid, Shape::QUERIES / PJ_QUERIES), dim3(PJ_THREADS), 0, stream, a);
 }
 

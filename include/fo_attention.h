@@ -663,7 +663,7 @@ typedef struct {
  * fo_paged_attention without a window.  Rounding and limits as in
  * fo_paged_window_attention.  Where a KV head has fewer than 64 query rows of a
  * sequence, unfinished rows wait in the context's scratch, total_rows *
- * n_heads * (head_dim + 2) floats: a call that needs more of it than any before
+ * n_heads * (head_dim + 4) floats: a call that needs more of it than any before
  * makes it, which a graph's capture refuses (what graphs use is kept). */
 int fo_paged_prefix_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch *batch,
                               const fo_paged_groups *groups, const fo_rows *q, const float *sinks, float scale,
