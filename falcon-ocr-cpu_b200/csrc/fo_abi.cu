@@ -2177,31 +2177,39 @@ int fo_paged_prefix_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged
     float *o = nullptr, *ml = nullptr;
     int32_t *parts_of = nullptr;
     FO_TRY(make_waiting(ctx, rows * q->heads, kv->head_dim, &o, &ml, &parts_of));
-    const bool few = rows * group <= FO_PAGED_FEW * groups->n_groups;  // of the average group
+    // Of the average group, few query rows; and few groups, since any of them may have all rows.
+    const bool few = rows * group <= FO_PAGED_FEW * groups->n_groups && groups->n_groups <= 16;
     if (queries <= FO_PAGED_FEW) {
         // The shared positions, then each sequence's own.
-        fo_paged_reach shared = reach;
-        shared.over_groups = 1;
-        shared.raw_o = o;
-        shared.raw_ml = ml;
-        if (!few) shared.parts_of = parts_of;
-        FO_TRY(launch_reach(ctx, kv, batch, q, out, nullptr, nullptr, scale, 0, shared, few));
-        fo_paged_own_launch a = {};
+        fo_paged_few_launch a = {};
         a.kv = *kv;
         a.batch = *batch;
         a.q = *q;
         a.out = *out;
-        a.sinks = sinks;
-        a.lse = lse;
         a.scale = scale;
+        a.err = ctx->dev_err;
+        fo_paged_reach shared = reach;
+        shared.over_groups = 1;
+        shared.raw_o = o;
+        shared.raw_ml = ml;
+        if (few) {
+            FO_TRY(make_paged_parts(ctx));
+            a.reach = shared;
+            cudaError_t e = fo_launch_paged_few(&a, ctx->sms, ctx->stream);
+            if (e != cudaSuccess) return cuda_fail(e, "paged attention launch");
+        } else {
+            shared.parts_of = parts_of;
+            FO_TRY(launch_reach(ctx, kv, batch, q, out, nullptr, nullptr, scale, 0, shared, false));
+            a.part_o = (float *)ctx->tile_parts.ptr;
+            a.part_ml = ctx->tile_part_ml();
+        }
         a.reach = reach;
         a.reach.prior_o = o;
         a.reach.prior_ml = ml;
         a.reach.parts_of = shared.parts_of;
-        a.part_o = (float *)ctx->tile_parts.ptr;
-        a.part_ml = ctx->tile_part_ml();
-        a.err = ctx->dev_err;
-        cudaError_t e = fo_launch_paged_own(&a, ctx->sms, ctx->stream);
+        a.sinks = sinks;
+        a.lse = lse;
+        cudaError_t e = fo_launch_paged_few(&a, ctx->sms, ctx->stream);
         return e == cudaSuccess ? FO_OK : cuda_fail(e, "paged attention launch");
     }
     fo_paged_reach own = reach;
@@ -2212,7 +2220,7 @@ int fo_paged_prefix_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged
     reach.over_groups = 1;
     reach.prior_o = o;
     reach.prior_ml = ml;
-    return launch_reach(ctx, kv, batch, q, out, sinks, lse, scale, 0, reach, few);
+    return launch_reach(ctx, kv, batch, q, out, sinks, lse, scale, 0, reach, false);
 }
 
 }  // extern "C"

@@ -309,21 +309,22 @@ struct fo_paged_tiles_launch {
 };
 cudaError_t fo_launch_paged_tiles(const fo_paged_tiles_launch *args, int sms, cudaStream_t stream);
 
-// Each sequence's positions behind the shared ones, for FO_PAGED_FEW query rows of
-// a KV head at most, joined with what the shared ones gave (paged_own.cu).
-struct fo_paged_own_launch {
+// Few query rows where sequences share their beginnings (paged_few.cu): groups'
+// rows over the shared positions into raw_o, or each sequence's rows over its own
+// positions joined with what the shared ones gave.
+struct fo_paged_few_launch {
     fo_paged_kv kv;
     fo_paged_batch batch;
     fo_rows q, out;
     const float *sinks;
     float *lse;
     float scale;
-    struct fo_paged_reach reach;  // prior_o, prior_ml, parts_of
+    struct fo_paged_reach reach;
     const float *part_o, *part_ml;  // of fo_paged_tiles_launch
     unsigned *err;
-    int32_t group, q_warps, q_vec, out_vec, parts;  // filled in by the launcher
+    int32_t group, q_units, q_vec, out_vec, parts;  // filled in by the launcher
 };
-cudaError_t fo_launch_paged_own(const fo_paged_own_launch *args, int sms, cudaStream_t stream);
+cudaError_t fo_launch_paged_few(const fo_paged_few_launch *args, int sms, cudaStream_t stream);
 
 // The bounded-wait self-test kernel (selftest.cu).
 cudaError_t fo_launch_bounded_wait(unsigned *err, unsigned long long limit_ns, cudaStream_t stream);
