@@ -322,7 +322,7 @@ struct fo_paged_few_launch {
     struct fo_paged_reach reach;
     const float *part_o, *part_ml;  // of fo_paged_tiles_launch
     unsigned *err;
-    int32_t group, q_units, q_vec, out_vec, parts;  // filled in by the launcher
+    int32_t group, q_units, q_vec, out_vec, parts, warps;  // filled in by the launcher
 };
 cudaError_t fo_launch_paged_few(const fo_paged_few_launch *args, int sms, cudaStream_t stream);
 

@@ -6,7 +6,7 @@
 // kscale * (q . kcode_j), and the sums of e^(s_j - m) and e^(s_j - m) vscale vcode_j.
 // Such ranges are short and there are many (64 sequences' own 500 positions are 512
 // units of 64 KB), so latency bounds them, and what a kernel does once for a unit:
-// the units are spread as thinly as they go, eight warps to a block, 16 positions
+// the units are spread as thinly as they go, eight or four warps to a block, 16 positions
 // to a warp at a time, the blocks of a cluster sharing a unit where there are
 // few, lanes' parts joined once at the end, by way of distributed shared memory.
 // (paged_attention.cuh's kernel goes from unit to unit with blocks of sixteen
@@ -30,7 +30,7 @@
 
 namespace fo {
 
-constexpr int PF_WARPS = 8, PF_THREADS = 32 * PF_WARPS;
+constexpr int PF_WARPS = 8, PF_THREADS = 32 * PF_WARPS;  // of a block at most
 constexpr int PF_LOWEST = 12;       // exponent bits of the least power of two that scales are relative to
 constexpr float PF_SLACK = 4.0f;    // log2: what a score may pass the maximum by before that moves
 
@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(PF_THREADS, F32 && NT == 2 ? 1 : 2)
 
     // Steps of 16 positions, of one page; the next step's codes and scales on their way while one
     // is computed, and the page number of the one after.
-    const int base = from & ~15, steps = to > from ? (to - base + 15) / 16 : 0, stride = PF_WARPS * blocks;
+    const int base = from & ~15, steps = to > from ? (to - base + 15) / 16 : 0, stride = a.warps * blocks;
     const int32_t *table = a.batch.page_table + seq * a.batch.table_stride;
     struct Step {
         uint4 k[HALVES][2];  // keys g and g + 8, dimensions 16 t ..
@@ -367,14 +367,14 @@ __global__ void __launch_bounds__(PF_THREADS, F32 && NT == 2 ? 1 : 2)
     __syncthreads();
     // The block's warps.
 #pragma unroll 1
-    for (int y = threadIdx.x; y < n_queries * D; y += PF_THREADS) {
+    for (int y = threadIdx.x; y < n_queries * D; y += blockDim.x) {
         const int qi = y / D, d = y % D;
         float high = -INFINITY, sum = 0.0f, v = 0.0f;
-#pragma unroll
-        for (int w = 0; w < PF_WARPS; w++) high = fmaxf(high, sh.ml[w][qi][0]);
+#pragma unroll 4
+        for (int w = 0; w < a.warps; w++) high = fmaxf(high, sh.ml[w][qi][0]);
         const float shift = high == -INFINITY ? 0.0f : high;
-#pragma unroll
-        for (int w = 0; w < PF_WARPS; w++) {
+#pragma unroll 4
+        for (int w = 0; w < a.warps; w++) {
             const float f = sm100::ex2(sh.ml[w][qi][0] - shift);
             sum = fmaf(sh.ml[w][qi][1], f, sum);
             v = fmaf(sh.o[w][qi][d], f, v);
@@ -386,7 +386,7 @@ __global__ void __launch_bounds__(PF_THREADS, F32 && NT == 2 ? 1 : 2)
     else __syncthreads();
     // The cluster's blocks, and what the shared positions gave: four dimensions of a query at a time.
 #pragma unroll 1
-    for (int y = rank * PF_THREADS + threadIdx.x; y < n_queries * (D / 4); y += blocks * PF_THREADS) {
+    for (int y = rank * blockDim.x + threadIdx.x; y < n_queries * (D / 4); y += blocks * blockDim.x) {
         const int qi = y / (D / 4), quad = y % (D / 4), r = (q0 + qi) / a.group, h = head * a.group + q0 + qi - r * a.group;
         const int64_t row = first + r, at_row = row * a.q.heads + h;
         float high = -INFINITY, sum = 0.0f;
@@ -400,7 +400,7 @@ __global__ void __launch_bounds__(PF_THREADS, F32 && NT == 2 ? 1 : 2)
                             fmaf(z.w, f, v.w * keep));
             high = up;
         };
-#pragma unroll 1
+#pragma unroll 4
         for (int c = 0; c < blocks; c++) {
             const float *z = &sh.block_o[qi][4 * quad];
             add(pf_remote(&sh.block_ml[qi][0], c), pf_remote(&sh.block_ml[qi][1], c),
@@ -472,14 +472,16 @@ cudaError_t launch_few(const fo_paged_few_launch &in, int sms, cudaStream_t stre
     a.q_units = (int)((queries + 8 * NT - 1) / (8 * NT));
     const int64_t units = items * a.q_units * a.kv.n_kv_heads;
     if (units > 0x7FFFFFFF) return cudaErrorInvalidValue;
-    // Blocks that share a unit: as many as there are SMs for, two blocks to an SM.  (Of groups,
+    // Blocks that share a unit: as many as there are SMs for, two blocks of eight warps to an SM; and
+    // with units enough, blocks of four warps, of which twice as many run at once.  (Of groups,
     // the two that stand for sequences outside them have next to nothing to do.)
     const int64_t busy = a.reach.over_groups ? (int64_t)a.reach.n_groups * a.kv.n_kv_heads : units;
     int blocks = 1;
     while (blocks < 8 && 2 * blocks * busy <= 2 * sms) blocks *= 2;
+    a.warps = busy > 2 * sms ? 4 : 8;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)units, (unsigned)blocks);
-    cfg.blockDim = dim3(PF_THREADS);
+    cfg.blockDim = dim3(32 * a.warps);
     cfg.dynamicSmemBytes = SMEM;
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];

@@ -110,7 +110,7 @@ struct PtShared {
     using Shape = PtShape<D, F32>;
     uint64_t code_full[Shape::SLOTS], code_empty[Shape::SLOTS];
     uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
-    uint64_t s_full[2], s_read[2], p_full[2], o_full[2];
+    uint64_t s_full[2], s_read[2], p_half[2], p_full[2], o_full[2];
     uint64_t q_full[2], q_both;  // a stream's queries are there; those of the first that the second uses too
     uint64_t seg_full[PT_SEGS], seg_free[PT_SEGS];
     uint64_t meta_full[PT_METAS];
@@ -119,7 +119,7 @@ struct PtShared {
     PtSegment seg[PT_SEGS];
     PtMeta meta[PT_METAS];
     int k_tile[2], v_tile[2];  // the tile that the operands are, or will be, of
-    float xm[2][128], xl[2][128], xt[2][128];
+    float xm[2][128], xl[2][128], xt[2][128], q_scale[128];
     int2 warp_sum[PT_THREADS / 32];
     int begin_item, begin_base, abort;
     uint32_t tmem;
@@ -273,7 +273,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
             mbar_init(&sh.k_full[lane], PT_CONVERTERS), mbar_init(&sh.v_full[lane], PT_CONVERTERS);
             mbar_init(&sh.k_empty[lane], 2), mbar_init(&sh.v_empty[lane], 2);
             mbar_init(&sh.s_full[lane], 1), mbar_init(&sh.o_full[lane], 1);
-            mbar_init(&sh.s_read[lane], 4), mbar_init(&sh.p_full[lane], 4), mbar_init(&sh.q_full[lane], 4);
+            mbar_init(&sh.s_read[lane], 4), mbar_init(&sh.p_full[lane], 4), mbar_init(&sh.q_full[lane], 4), mbar_init(&sh.p_half[lane], 4);
             sh.k_tile[lane] = sh.v_tile[lane] = -1;
         }
         if (lane < PT_SEGS) mbar_init(&sh.seg_full[lane], 1), mbar_init(&sh.seg_free[lane], PT_SOFTMAX + 2);
@@ -371,38 +371,57 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                     low = a.window > 0 ? max(high + 1 - a.window, 0) : 0;
                 }
             }
-            if (own && live) {
-                // The whole row in registers, every load in flight at once.
-                Raw8<T> raw[D / 8];
-                const T *from = static_cast<const T *>(a.q.data) + row * a.q.row_stride + h * a.q.head_stride;
+            if (live && (pair || t == 0)) {
+                // The warp's rows as they are into their places, 16 bytes to a lane and neighbouring
+                // lanes in a row; then each thread its own row to FP16 operands there.  FP32 rows lie
+                // where their two terms will be.
+                constexpr int CHUNKS = D * (int)sizeof(T) / 16;
+                uint8_t *rows = smem + t * TERMS * Shape::OPERAND + 32 * wq * 128;
+                auto place = [&](int of, int chunk) {
+                    return reinterpret_cast<uint4 *>(rows + (chunk >> 3) * PT_PANEL + of * 128 + (((chunk & 7) ^ (of & 7)) << 4));
+                };
+                const T *data = static_cast<const T *>(a.q.data);
+                const long long at_q = row * a.q.row_stride + h * a.q.head_stride;
+                constexpr int FLIGHT = 8;
+#pragma unroll 1
+                for (int x0 = 0; x0 < CHUNKS; x0 += FLIGHT) {
+                    uint4 y[FLIGHT];
 #pragma unroll
-                for (int d = 0; d < D / 8; d++) {
-                    if (!mine) {
+                    for (int x = 0; x < FLIGHT; x++) {
+                        const int of = ((x0 + x) * 32 + lane) / CHUNKS, chunk = ((x0 + x) * 32 + lane) % CHUNKS;
+                        const T *from = data + __shfl_sync(0xffffffffu, at_q, of) + chunk * (16 / (int)sizeof(T));
+                        y[x] = make_uint4(0, 0, 0, 0);
+                        if (q - lane + of >= seg.nq) continue;
+                        if (a.q_vec) {
+                            y[x] = *reinterpret_cast<const uint4 *>(from);
+                        } else {
+                            T z[16 / sizeof(T)];
 #pragma unroll
-                        for (int e = 0; e < (int)sizeof(T) / 2; e++) raw[d].w[e] = make_uint4(0, 0, 0, 0);
-                    } else if (a.q_vec) {
-                        raw[d] = load_raw8(from + 8 * d);
-                    } else {
-#pragma unroll
-                        for (int e = 0; e < 8; e++) reinterpret_cast<T *>(raw[d].w)[e] = from[8 * d + e];
+                            for (int e = 0; e < 16 / (int)sizeof(T); e++) z[e] = from[e];
+                            memcpy(&y[x], z, 16);
+                        }
                     }
+#pragma unroll
+                    for (int x = 0; x < FLIGHT; x++)
+                        *place(((x0 + x) * 32 + lane) / CHUNKS, ((x0 + x) * 32 + lane) % CHUNKS) = y[x];
                 }
+                __syncwarp();
                 // The largest magnitude, as bits, which are in its order (NaN above infinity): of FP32,
                 // or of two BF16 at once.
                 uint32_t most = 0;
-#pragma unroll
-                for (int d = 0; d < D / 8; d++)
-#pragma unroll
-                    for (int e = 0; e < (int)sizeof(T) / 2; e++) {
-                        const uint4 w = raw[d].w[e];
-                        if constexpr (F32) {
-                            most = max(most, max(max(w.x & 0x7FFFFFFFu, w.y & 0x7FFFFFFFu),
-                                                 max(w.z & 0x7FFFFFFFu, w.w & 0x7FFFFFFFu)));
-                        } else {
-                            most = __vmaxu2(most, __vmaxu2(__vmaxu2(w.x & 0x7FFF7FFFu, w.y & 0x7FFF7FFFu),
-                                                           __vmaxu2(w.z & 0x7FFF7FFFu, w.w & 0x7FFF7FFFu)));
-                        }
+                uint4 raw[F32 ? CHUNKS : 1];
+#pragma unroll(F32 ? CHUNKS : 2)
+                for (int x = 0; x < CHUNKS; x++) {
+                    const uint4 w = *place(lane, x);
+                    if constexpr (F32) {
+                        raw[x] = w;
+                        most = max(most, max(max(w.x & 0x7FFFFFFFu, w.y & 0x7FFFFFFFu),
+                                             max(w.z & 0x7FFFFFFFu, w.w & 0x7FFFFFFFu)));
+                    } else {
+                        most = __vmaxu2(most, __vmaxu2(__vmaxu2(w.x & 0x7FFF7FFFu, w.y & 0x7FFF7FFFu),
+                                                       __vmaxu2(w.z & 0x7FFF7FFFu, w.w & 0x7FFF7FFFu)));
                     }
+                }
                 if constexpr (!F32) most = max(most & 0xFFFFu, most >> 16) << 16;
                 const bool finite = most < 0x7F800000u;
                 // A power of two brings the largest element to [2^14, 2^15); 2^126 at most, which still
@@ -410,50 +429,38 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 const int e = max((int)(most >> 23), 15);
                 const float up = finite ? __uint_as_float((uint32_t)(268 - e) << 23) : 0.0f;
                 q_scale = finite ? __uint_as_float((uint32_t)max(e - 14, 1) << 23) * a.scale * REACH_LOG2E : NAN;
-                if (pair || t == 0) {
-                    uint8_t *to = smem + (pair ? t : 0) * TERMS * Shape::OPERAND + r * 128;
-                    auto place = [&](int d) { return (d >> 6) * PT_PANEL + (((d >> 3 & 7) ^ (r & 7)) << 4); };
-                    if constexpr (!F32) {
-                        // As they are into their places, and there to FP16 (a short loop, for the
-                        // instruction cache).
-#pragma unroll
-                        for (int d = 0; d < D; d += 8) *reinterpret_cast<uint4 *>(to + place(d)) = raw[d / 8].w[0];
+                if constexpr (!F32) {
 #pragma unroll 1
-                        for (int d = 0; d < D; d += 8) {
-                            uint4 *at = reinterpret_cast<uint4 *>(to + place(d));
-                            Raw8<T> y;
-                            y.w[0] = *at;
-                            float x[8];
-                            unpack8(y, x);
+                    for (int x = 0; x < CHUNKS; x++) {
+                        Raw8<T> w;
+                        w.w[0] = *place(lane, x);
+                        float y[8];
+                        unpack8(w, y);
 #pragma unroll
-                            for (int e = 0; e < 8; e++) x[e] = finite ? x[e] * up : 0.0f;
-                            *at = make_uint4(pt_f16x2(x[0], x[1]), pt_f16x2(x[2], x[3]), pt_f16x2(x[4], x[5]),
-                                             pt_f16x2(x[6], x[7]));
-                        }
-                    } else {
-#pragma unroll
-                        for (int d = 0; d < D; d += 8) {
-                            float x[8];
-                            unpack8(raw[d / 8], x);
-#pragma unroll
-                            for (int e = 0; e < 8; e++) x[e] = finite ? x[e] * up : 0.0f;
-#pragma unroll
-                            for (int term = 0; term < 2; term++) {
-                                uint32_t w[4];
-#pragma unroll
-                                for (int e = 0; e < 4; e++) {
-                                    w[e] = pt_f16x2(x[2 * e], x[2 * e + 1]);
-                                    const float2 b = f16x2_f32x2(w[e]);
-                                    x[2 * e] -= b.x;
-                                    x[2 * e + 1] -= b.y;
-                                }
-                                *reinterpret_cast<uint4 *>(to + term * Shape::OPERAND + place(d)) =
-                                    make_uint4(w[0], w[1], w[2], w[3]);
-                            }
-                        }
+                        for (int e = 0; e < 8; e++) y[e] = finite ? y[e] * up : 0.0f;
+                        *place(lane, x) = make_uint4(pt_f16x2(y[0], y[1]), pt_f16x2(y[2], y[3]), pt_f16x2(y[4], y[5]),
+                                                     pt_f16x2(y[6], y[7]));
                     }
-                    fence_proxy_async_smem();
+                } else {
+#pragma unroll
+                    for (int x = 0; x < CHUNKS / 2; x++) {
+                        const uint32_t w[8] = {raw[2 * x].x, raw[2 * x].y, raw[2 * x].z, raw[2 * x].w,
+                                               raw[2 * x + 1].x, raw[2 * x + 1].y, raw[2 * x + 1].z, raw[2 * x + 1].w};
+                        uint32_t hi[4], lo[4];
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            const float u = finite ? __uint_as_float(w[2 * e]) * up : 0.0f;
+                            const float v = finite ? __uint_as_float(w[2 * e + 1]) * up : 0.0f;
+                            hi[e] = pt_f16x2(u, v);
+                            const float2 b = f16x2_f32x2(hi[e]);
+                            lo[e] = pt_f16x2(u - b.x, v - b.y);
+                        }
+                        *place(lane, x) = make_uint4(hi[0], hi[1], hi[2], hi[3]);
+                        *place(lane, x + CHUNKS / 2) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
+                    }
                 }
+                if (!pair) sh.q_scale[r] = q_scale;
+                fence_proxy_async_smem();
             }
             __syncwarp();
             if (pair || t == 0) {
@@ -464,6 +471,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
             } else if (own) {
                 ok = pt_wait(&sh.q_both, both_phase, abort_flag);
                 if (!ok) break;
+                if (live) q_scale = sh.q_scale[r];
                 if (lane == 0) mbar_arrive(&sh.q_full[t]);
             }
             if (!pair && n > 1) both_phase ^= 1;
@@ -480,7 +488,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                     // for each tile as the others do, not for the next one before they have for this.)
                     if (any) ok = pt_wait(&sh.o_full[t], (c - 1) & 1, abort_flag);
                     if (!ok) break;
-                    if (lane == 0) mbar_arrive(&sh.s_read[t]), mbar_arrive(&sh.p_full[t]);
+                    if (lane == 0) mbar_arrive(&sh.s_read[t]), mbar_arrive(&sh.p_half[t]), mbar_arrive(&sh.p_full[t]);
                     __syncwarp();
                     any = true;
                     continue;
@@ -564,8 +572,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 }
                 const float shift = m == -INFINITY ? 0.0f : m;
                 // P may be written, and O touched, once the PV before is complete.
+                // (In S's place, S would not be there before.)
                 if (any) {
-                    ok = pt_wait(&sh.o_full[t], (c - 1) & 1, abort_flag);
+                    if (!ALIAS) ok = pt_wait(&sh.o_full[t], (c - 1) & 1, abort_flag);
                     if (!ok) break;
                     if (__any_sync(0xffffffffu, factor != 1.0f)) {
                         tc_fence_after();
@@ -608,6 +617,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                         term[e] = pt_f16x2(p[e].x, p[e].y);
                     }
                     FO_TMEM_ST16(p_at + 16 * TERMS * w, term);
+                    if (w == 2) {
+                        // The first half is multiplied while the second is computed.
+                        tmem_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sh.p_half[t]);
+                    }
                     if constexpr (F32) {
 #pragma unroll
                         for (int e = 0; e < 16; e++) {
@@ -1019,7 +1035,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
             // elected lane issues.
             const int t = warp - PT_ISSUER;
             const uint32_t base = smem_u32(smem);
-            constexpr uint32_t ID_S = idesc_f16(128, 128, 0), ID_PV = idesc_f16(128, 64, 1);
+            constexpr uint32_t ID_S = idesc_f16(128, 128, 0), ID_PV = idesc_f16(128, D, 1);
             const uint64_t dQ = sdesc_sw128(base, 16, 1024), dK = sdesc_sw128(base + Shape::OFF_K, 16, 1024);
             const uint64_t dV = sdesc_sw128(base + Shape::OFF_V, PT_PANEL, 1024);
             constexpr uint32_t OPERAND16 = Shape::OPERAND >> 4, PANEL16 = PT_PANEL >> 4;
@@ -1048,22 +1064,24 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 }
                 __syncwarp();
             };
-            auto issue_pv = [&](const Tile &x) {
+            // Half h of the keys.
+            auto issue_pv = [&](const Tile &x, int h) {
                 if (elect_one()) {
-                    const uint32_t p = tmem + (ALIAS ? 128 * t : 384 + 64 * t);
+                    const uint32_t p = tmem + (ALIAS ? 128 * t : 384 + 64 * t), o = tmem + 256 + (ALIAS ? 128 : 64) * t;
+                    const uint64_t b = dV + (x.k & 1) * OPERAND16;
 #pragma unroll 1
-                    for (int y = 0; y < TERMS * PANELS; y++) {
-                        const int term = y / PANELS, panel = y % PANELS;
-                        const uint64_t b = dV + (x.k & 1) * OPERAND16 + panel * PANEL16;
-                        const uint32_t o = tmem + 256 + (ALIAS ? 128 : 64) * t + 64 * panel;
+                    for (int term = 0; term < TERMS; term++)
 #pragma unroll
-                        for (int kk = 0; kk < 8; kk++)
+                        for (int y = 0; y < 4; y++) {
+                            const int kk = 4 * h + y;
                             mma_bf16_ts(o, p + 16 * (term + TERMS * (kk >> 1)) + 8 * (kk & 1), b + kk * (2048 >> 4), ID_PV,
                                         term > 0 || kk > 0 || !x.first);
+                        }
+                    if (h == 1) {
+                        mma_commit(&sh.o_full[t]);
+                        mma_commit(&sh.v_empty[x.k & 1]);
+                        if (!x.pair) mma_commit(&sh.v_empty[x.k & 1]);
                     }
-                    mma_commit(&sh.o_full[t]);
-                    mma_commit(&sh.v_empty[x.k & 1]);
-                    if (!x.pair) mma_commit(&sh.v_empty[x.k & 1]);
                 }
                 __syncwarp();
             };
@@ -1112,7 +1130,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
             Tile now = {};
             if (more) {
                 now = take();
-                ok = (there(sh.k_full, sh.k_tile, now.k));
+                ok = there(sh.k_full, sh.k_tile, now.k);
                 tc_fence_after();
                 if (ok) issue_s(now);
             }
@@ -1133,20 +1151,21 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                         issue_s(next);
                     }
                 }
+                ok = there(sh.v_full, sh.v_tile, now.k) && pt_wait(&sh.p_half[t], c & 1, abort_flag);
+                if (!ok) break;
+                tc_fence_after();
+                issue_pv(now, 0);
                 ok = pt_wait(&sh.p_full[t], c & 1, abort_flag);
                 if (!ok) break;
                 tc_fence_after();
-                ok = (there(sh.v_full, sh.v_tile, now.k));
-                if (!ok) break;
-                tc_fence_after();
-                issue_pv(now);
+                issue_pv(now, 1);
                 if (!issued) {
                     if (!same) {
                         more = enter();
                         if (!more) break;
                         next = take();
                     }
-                    ok = (there(sh.k_full, sh.k_tile, next.k));
+                    ok = there(sh.k_full, sh.k_tile, next.k);
                     if (ok && ALIAS) ok = pt_wait(&sh.o_full[t], c & 1, abort_flag);
                     if (!ok) break;
                     tc_fence_after();
