@@ -60,6 +60,12 @@ static_assert(256 * PT_SOFTMAX_REGS + 256 * PT_OTHER_REGS == PT_THREADS * PT_LAU
 constexpr int PT_SEGS = 8;    // segments announced at a time
 constexpr int PT_METAS = 16;  // tiles whose scales are held: what the code ring and the operands can be ahead by, and more
 constexpr uint32_t PT_SLOT = 8192, PT_PANEL = 16384;  // a slot of codes; 128 rows of 64 FP16
+// What beginning with a unit costs, in tiles: its place in the line is so much longer.
+// (Queries, first scores, output: 9,000 cycles, where a tile of 256 rows takes 4,500.
+// With none, the blocks of a prompt's first, short units took twice as long as
+// the others.)
+constexpr int PT_START = 2;
+
 // Exponent bits of a power of two above x (x from 2^-116 to 2^126; what is smaller
 // is taken as that, relative to which FP16 holds less of it).
 constexpr int PT_LOWEST = 12;
@@ -121,7 +127,7 @@ struct PtShared {
     int k_tile[2], v_tile[2];  // the tile that the operands are, or will be, of
     float xm[2][128], xl[2][128], xt[2][128], q_scale[128];
     int2 warp_sum[PT_THREADS / 32];
-    int begin_item, begin_base, abort;
+    int begin_item, begin_base, first_tile, last_tile, abort;
     uint32_t tmem;
 };
 
@@ -193,24 +199,24 @@ __device__ __forceinline__ PtItem pt_item(const fo_paged_tiles_launch &a, int in
 
 // Sum of x over the block's earlier threads; `all` the whole block's.
 template <typename Shared_>
-__device__ __forceinline__ int pt_scan(int x, Shared_ &sh, int &all) {
+__device__ __forceinline__ int2 pt_scan(int2 x, Shared_ &sh, int2 &all) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    int sum = x;
+    int2 sum = x;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
-        const int u = __shfl_up_sync(0xffffffffu, sum, o);
-        if (lane >= o) sum += u;
+        const int u = __shfl_up_sync(0xffffffffu, sum.x, o), v = __shfl_up_sync(0xffffffffu, sum.y, o);
+        if (lane >= o) sum.x += u, sum.y += v;
     }
     __syncthreads();  // the last scan's sums have been read
-    if (lane == 31) sh.warp_sum[warp].x = sum;
+    if (lane == 31) sh.warp_sum[warp] = sum;
     __syncthreads();
-    int before = sum - x;
-    all = 0;
-#pragma unroll
+    int2 before = make_int2(sum.x - x.x, sum.y - x.y);
+    all = make_int2(0, 0);
+#pragma unroll 1
     for (int w = 0; w < PT_THREADS / 32; w++) {
-        const int y = sh.warp_sum[w].x;
-        if (w < warp) before += y;
-        all += y;
+        const int2 y = sh.warp_sum[w];
+        if (w < warp) before.x += y.x, before.y += y.y;
+        all.x += y.x, all.y += y.y;
     }
     return before;
 }
@@ -291,44 +297,54 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
     wait_for_prior_kernel();
 
     // This block's piece [begin, end) of the line, and where it begins.  (The
-    // line's tiles are below 2^31, checked on the host.)
+    // line is shorter than 2^31, checked on the host.)
     const int n_items = a.reach.over_groups ? a.reach.n_groups + 2 : (int)a.batch.n_seqs * a.q_units;
-    int per = 0, begin = 0, count = 0;
+    int per = 0, begin = 0, end = 0;
     // The line's length first, then the item that the piece begins in; with no more items than
     // threads at one go.
 #pragma unroll 1
     for (bool known = false;;) {
-        int all = 0;
+        int2 all = make_int2(0, 0);  // length of the line, and tiles
 #pragma unroll 1
         for (int first = 0; first < n_items; first += PT_THREADS) {
-            int mine = 0, chunk;
+            int2 mine = make_int2(0, 0), chunk;
+            PtItem x;
             if (first + tid < n_items) {
-                const PtItem x = pt_item<QUERIES>(a, first + tid);
-                mine = x.tiles * x.units;
+                x = pt_item<QUERIES>(a, first + tid);
+                mine = make_int2((x.tiles + PT_START) * x.units, x.tiles * x.units);
             }
-            const int before = all + pt_scan(mine, sh, chunk);
-            all += chunk;
+            int2 before = pt_scan(mine, sh, chunk);
+            before.x += all.x, before.y += all.y;
+            all.x += chunk.x, all.y += chunk.y;
             if (!known && n_items <= PT_THREADS) {
                 known = true;
-                per = max((int)((unsigned)(all + gridDim.x - 1) / gridDim.x), 2);
-                begin = (int)min((long long)per * blockIdx.x, (long long)all);
-                count = (int)min((long long)per, (long long)all - begin);
+                per = max((int)((unsigned)(all.x + gridDim.x - 1) / gridDim.x), 2 + PT_START);
+                begin = (int)min((long long)per * blockIdx.x, (long long)all.x);
+                end = (int)min((long long)begin + per, (long long)all.x);
             }
-            if (known && begin >= before && begin < before + mine) {
+            // Tiles before a place of the line in this thread's item.
+            auto tiles = [&](int at, int unit) {
+                return before.y + unit * x.tiles + max(at - before.x - unit * (x.tiles + PT_START) - PT_START, 0);
+            };
+            if (known && begin >= before.x && begin < before.x + mine.x) {
                 sh.begin_item = first + tid;
-                sh.begin_base = before;
+                sh.begin_base = before.x;
+                sh.first_tile = tiles(begin, (begin - before.x) / (x.tiles + PT_START));
             }
+            if (known && end > before.x && end <= before.x + mine.x)
+                sh.last_tile = tiles(end, (end - 1 - before.x) / (x.tiles + PT_START));
         }
         if (known) break;
         known = true;
-        per = max((int)((unsigned)(all + gridDim.x - 1) / gridDim.x), 2);
-        begin = (int)min((long long)per * blockIdx.x, (long long)all);
-        count = (int)min((long long)per, (long long)all - begin);
+        per = max((int)((unsigned)(all.x + gridDim.x - 1) / gridDim.x), 2 + PT_START);
+        begin = (int)min((long long)per * blockIdx.x, (long long)all.x);
+        end = (int)min((long long)begin + per, (long long)all.x);
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
     const uint32_t tmem = sh.tmem;
+    const int count = begin < end ? sh.last_tile - sh.first_tile : 0;
     if (count <= 0) {
         if (tid == 0) a.joins[8 * blockIdx.x] = 0;
         if (warp == PT_ISSUER) tmem_dealloc(tmem, 512);
@@ -862,6 +878,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
             item.units = 0;
             int index = sh.begin_item - 1, unit = 0, tile = 0;
             int segs = 0, ahead = 0, left = 0, head = 0;
+            int at_unit = 0;  // the unit's place in the line
             bool ok = true;
             if (lane == 0) a.joins[8 * blockIdx.x] = 0;
             struct Next {
@@ -880,8 +897,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                     while (item.units == 0 && index < n_items - 1);
                     unit = 0;
                     if (ahead == 0) {
-                        unit = (begin - sh.begin_base) / item.tiles;
-                        tile = (begin - sh.begin_base) - unit * item.tiles;
+                        at_unit = sh.begin_base;
+                        unit = (begin - at_unit) / (item.tiles + PT_START);
+                        at_unit += unit * (item.tiles + PT_START);
+                        tile = max(begin - at_unit - PT_START, 0);
                     }
                 }
                 if (left == 0) {
@@ -909,7 +928,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                         g.part = -1;
                         g.c1 = 0;
                         if (n < item.tiles) {
-                            const int from = begin + ahead - tile;  // the unit's place in the line
+                            const int from = at_unit + PT_START;
                             const int c0 = from / per, c1 = (from + item.tiles - 1) / per;
                             g.part = 2 * (int)blockIdx.x + (c0 == (int)blockIdx.x ? 1 : 0);
                             g.c1 = c1;
@@ -950,6 +969,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 if (++tile == item.tiles) {
                     tile = 0;
                     unit++;
+                    at_unit += item.tiles + PT_START;
                 }
                 return x;
             };
