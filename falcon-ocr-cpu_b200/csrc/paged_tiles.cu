@@ -549,29 +549,49 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                         tmem_wait_st();
                     }
                 }
-                uint32_t raw[128];
-                FO_TMEM_LD32(s_at + 0, (raw + 0));
-                FO_TMEM_LD32(s_at + 32, (raw + 32));
-                FO_TMEM_LD32(s_at + 64, (raw + 64));
-                FO_TMEM_LD32(s_at + 96, (raw + 96));
-                float f[8];  // of 16 keys' scores: log2 units
-#pragma unroll
-                for (int g = 0; g < 8; g++) f[g] = plain ? meta.ks[g] * q_scale : 1.0f;
-                tmem_wait_ld();
-                tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&sh.s_read[t]);
-                // The row's largest score.
+                // What 32 keys of a row need: their scores' factors (log2 units), the largest score, and
+                // the probabilities.
+                auto factor_of = [&](int g) { return plain ? meta.ks[g] * q_scale : 1.0f; };
                 float mx = -INFINITY;
+                auto largest = [&](const uint32_t *raw, int w) {
 #pragma unroll
-                for (int g = 0; g < 8; g++) {
-                    float m0 = -INFINITY, m1 = -INFINITY;
+                    for (int g = 0; g < 2; g++) {
+                        float m0 = -INFINITY, m1 = -INFINITY;
 #pragma unroll
-                    for (int e = 0; e < 16; e += 4) {
-                        m0 = fmaxf(fmaxf(m0, __uint_as_float(raw[16 * g + e])), __uint_as_float(raw[16 * g + e + 1]));
-                        m1 = fmaxf(fmaxf(m1, __uint_as_float(raw[16 * g + e + 2])), __uint_as_float(raw[16 * g + e + 3]));
+                        for (int e = 16 * g; e < 16 * g + 16; e += 4) {
+                            m0 = fmaxf(fmaxf(m0, __uint_as_float(raw[e])), __uint_as_float(raw[e + 1]));
+                            m1 = fmaxf(fmaxf(m1, __uint_as_float(raw[e + 2])), __uint_as_float(raw[e + 3]));
+                        }
+                        mx = fmaxf(mx, fmaxf(m0, m1) * factor_of(2 * w + g));
                     }
-                    mx = fmaxf(mx, fmaxf(m0, m1) * f[g]);
+                };
+                // Where S has its place to itself the row is held in registers, so that the next S can
+                // be computed meanwhile.  Where P takes that place S is read twice, in short loops: what
+                // is run over and over has to stay in the instruction cache (heads of 128: 2,621 us
+                // with the row in registers and all in line, MEASURED so).
+                uint32_t raw[ALIAS ? 64 : 128];
+                if constexpr (!ALIAS) {
+                    FO_TMEM_LD32(s_at + 0, (raw + 0));
+                    FO_TMEM_LD32(s_at + 32, (raw + 32));
+                    FO_TMEM_LD32(s_at + 64, (raw + 64));
+                    FO_TMEM_LD32(s_at + 96, (raw + 96));
+                    tmem_wait_ld();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.s_read[t]);
+#pragma unroll
+                    for (int w = 0; w < 4; w++) largest(raw + 32 * w, w);
+                } else {
+                    FO_TMEM_LD32(s_at, raw);
+#pragma unroll 1
+                    for (int w = 0; w < 4; w += 2) {
+                        tmem_wait_ld();
+                        FO_TMEM_LD32(s_at + 32 * w + 32, (raw + 32));
+                        largest(raw, w);
+                        tmem_wait_ld();
+                        FO_TMEM_LD32(s_at + (32 * w + 64) % 128, raw);  // (at last the first keys again)
+                        largest(raw + 32, w + 1);
+                    }
                 }
                 float factor = 1.0f;  // of what has been summed so far
                 if (!any) {
@@ -615,17 +635,16 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 // zeros.
                 const float inverse_top = __uint_as_float((uint32_t)(264 - top) << 23);
                 float2 sum = make_float2(0.0f, 0.0f);
-#pragma unroll
-                for (int w = 0; w < 4; w++) {
+                auto probabilities = [&](const uint32_t *raw, int w) {
+                    const float f0 = factor_of(2 * w), f1 = factor_of(2 * w + 1);
                     const float v0 = fminf(meta.vs[2 * w] * inverse_top, FLT_MAX);
                     const float v1 = fminf(meta.vs[2 * w + 1] * inverse_top, FLT_MAX);
                     float2 p[16];
                     uint32_t term[16];
 #pragma unroll
                     for (int e = 0; e < 16; e++) {
-                        const float g = f[2 * w + e / 8], v = e < 8 ? v0 : v1;
-                        const float2 x = __ffma2_rn(make_float2(__uint_as_float(raw[32 * w + 2 * e]),
-                                                                __uint_as_float(raw[32 * w + 2 * e + 1])),
+                        const float g = e < 8 ? f0 : f1, v = e < 8 ? v0 : v1;
+                        const float2 x = __ffma2_rn(make_float2(__uint_as_float(raw[2 * e]), __uint_as_float(raw[2 * e + 1])),
                                                     make_float2(g, g), make_float2(-shift, -shift));
                         p[e] = make_float2(ex2(x.x), ex2(x.y));
                         sum = __fadd2_rn(sum, p[e]);
@@ -633,13 +652,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                         term[e] = pt_f16x2(p[e].x, p[e].y);
                     }
                     FO_TMEM_ST16(p_at + 16 * TERMS * w, term);
-                    if (w == 2) {
-                        // The first half is multiplied while the second is computed.
-                        tmem_wait_st();
-                        tc_fence_before();
-                        __syncwarp();
-                        if (lane == 0) mbar_arrive(&sh.p_half[t]);
-                    }
                     if constexpr (F32) {
 #pragma unroll
                         for (int e = 0; e < 16; e++) {
@@ -647,6 +659,31 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                             term[e] = pt_f16x2(p[e].x - b.x, p[e].y - b.y);
                         }
                         FO_TMEM_ST16(p_at + 16 * TERMS * w + 16, term);
+                    }
+                };
+                auto half = [&]() {
+                    // The first half is multiplied while the second is computed.
+                    tmem_wait_st();
+                    tc_fence_before();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&sh.p_half[t]);
+                };
+                if constexpr (!ALIAS) {
+#pragma unroll
+                    for (int w = 0; w < 4; w++) {
+                        probabilities(raw + 32 * w, w);
+                        if (w == 2) half();
+                    }
+                } else {
+#pragma unroll 1
+                    for (int w = 0; w < 4; w += 2) {
+                        tmem_wait_ld();
+                        FO_TMEM_LD32(s_at + 32 * w + 32, (raw + 32));
+                        probabilities(raw, w);
+                        if (w == 2) half();
+                        tmem_wait_ld();
+                        if (w == 0) FO_TMEM_LD32(s_at + 64, raw);
+                        probabilities(raw + 32, w + 1);
                     }
                 }
                 l += sum.x + sum.y;
