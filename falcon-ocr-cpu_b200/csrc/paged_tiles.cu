@@ -82,7 +82,7 @@ struct PtShape {
     static constexpr int TERMS = 1 + F32;  // FP16 terms of a query and of a probability
     static constexpr int Q_TILES = F32 && D == 128 ? 1 : 2;
     static constexpr int QUERIES = 128 * Q_TILES;
-    static constexpr bool ALIAS = D == 128 || F32;  // P in S's place
+    static constexpr bool OWN_P = D == 64 && !F32;  // P has columns of its own, else S's
     static constexpr int PANELS = D / 64;
     static constexpr uint32_t OPERAND = PANELS * PT_PANEL;  // 128 rows of D FP16
     static constexpr uint32_t Q_BYTES = Q_TILES * TERMS * OPERAND;
@@ -116,7 +116,7 @@ struct PtShared {
     using Shape = PtShape<D, F32>;
     uint64_t code_full[Shape::SLOTS], code_empty[Shape::SLOTS];
     uint64_t k_full[2], k_empty[2], v_full[2], v_empty[2];
-    uint64_t s_full[2], s_read[2], p_half[2], p_full[2], o_full[2];
+    uint64_t s_full[2], p_half[2], p_full[2], o_full[2];
     uint64_t q_full[2], q_both;  // a stream's queries are there; those of the first that the second uses too
     uint64_t seg_full[PT_SEGS], seg_free[PT_SEGS];
     uint64_t meta_full[PT_METAS];
@@ -266,7 +266,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
     using T = typename std::conditional<F32, float, uint16_t>::type;
     constexpr int QUERIES = Shape::QUERIES, TERMS = Shape::TERMS, PANELS = Shape::PANELS, PARTS = Shape::PARTS;
     constexpr int SLOTS = Shape::SLOTS;
-    constexpr bool ALIAS = Shape::ALIAS;
+    constexpr bool OWN_P = Shape::OWN_P;
     extern __shared__ uint8_t pt_smem[];
     __shared__ PtShared<D, F32> sh;
     uint8_t *smem = reinterpret_cast<uint8_t *>((reinterpret_cast<uintptr_t>(pt_smem) + 1023) & ~uintptr_t(1023));
@@ -279,7 +279,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
             mbar_init(&sh.k_full[lane], PT_CONVERTERS), mbar_init(&sh.v_full[lane], PT_CONVERTERS);
             mbar_init(&sh.k_empty[lane], 2), mbar_init(&sh.v_empty[lane], 2);
             mbar_init(&sh.s_full[lane], 1), mbar_init(&sh.o_full[lane], 1);
-            mbar_init(&sh.s_read[lane], 4), mbar_init(&sh.p_full[lane], 4), mbar_init(&sh.q_full[lane], 4), mbar_init(&sh.p_half[lane], 4);
+            mbar_init(&sh.p_full[lane], 4), mbar_init(&sh.q_full[lane], 4), mbar_init(&sh.p_half[lane], 4);
             sh.k_tile[lane] = sh.v_tile[lane] = -1;
         }
         if (lane < PT_SEGS) mbar_init(&sh.seg_full[lane], 1), mbar_init(&sh.seg_free[lane], PT_SOFTMAX + 2);
@@ -356,8 +356,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PT_SOFTMAX_REGS));
         const int t = warp >> 2, wq = warp & 3, r = tid & 127;
         const uint32_t at = tmem + ((uint32_t)(32 * wq) << 16);
-        const uint32_t s_at = at + 128 * t, p_at = ALIAS ? s_at : at + 384 + 64 * t;
-        auto o_at = [&](int stream) { return at + 256 + (ALIAS ? 128 : 64) * stream; };
+        const uint32_t s_at = at + 128 * t, p_at = OWN_P ? at + 384 + 64 * t : s_at;
+        auto o_at = [&](int stream) { return at + 256 + (OWN_P ? 64 : 128) * stream; };
         int turns = 0;  // tiles that this warp and the other stream's have taken turns at
         int c = 0, x_phase = 0, both_phase = 0;  // tiles of this stream so far; joins of both streams; queries of both
         bool ok = true;
@@ -504,7 +504,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                     // for each tile as the others do, not for the next one before they have for this.)
                     if (any) ok = pt_wait(&sh.o_full[t], (c - 1) & 1, abort_flag);
                     if (!ok) break;
-                    if (lane == 0) mbar_arrive(&sh.s_read[t]), mbar_arrive(&sh.p_half[t]), mbar_arrive(&sh.p_full[t]);
+                    if (lane == 0) mbar_arrive(&sh.p_half[t]), mbar_arrive(&sh.p_full[t]);
                     __syncwarp();
                     any = true;
                     continue;
@@ -565,33 +565,19 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                         mx = fmaxf(mx, fmaxf(m0, m1) * factor_of(2 * w + g));
                     }
                 };
-                // Where S has its place to itself the row is held in registers, so that the next S can
-                // be computed meanwhile.  Where P takes that place S is read twice, in short loops: what
-                // is run over and over has to stay in the instruction cache (heads of 128: 2,621 us
-                // with the row in registers and all in line, MEASURED so).
-                uint32_t raw[ALIAS ? 64 : 128];
-                if constexpr (!ALIAS) {
-                    FO_TMEM_LD32(s_at + 0, (raw + 0));
-                    FO_TMEM_LD32(s_at + 32, (raw + 32));
-                    FO_TMEM_LD32(s_at + 64, (raw + 64));
-                    FO_TMEM_LD32(s_at + 96, (raw + 96));
-                    tmem_wait_ld();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sh.s_read[t]);
-#pragma unroll
-                    for (int w = 0; w < 4; w++) largest(raw + 32 * w, w);
-                } else {
-                    FO_TMEM_LD32(s_at, raw);
+                // S is read twice, in short loops: what is run over and over has to stay in the instruction
+                // cache (with the row in registers and all of it in line: 123 us for a page's prompt where
+                // this takes MEASURED, 2,621 for ragged prompts with heads of 128 against MEASURED).
+                uint32_t raw[64];
+                FO_TMEM_LD32(s_at, raw);
 #pragma unroll 1
-                    for (int w = 0; w < 4; w += 2) {
-                        tmem_wait_ld();
-                        FO_TMEM_LD32(s_at + 32 * w + 32, (raw + 32));
-                        largest(raw, w);
-                        tmem_wait_ld();
-                        FO_TMEM_LD32(s_at + (32 * w + 64) % 128, raw);  // (at last the first keys again)
-                        largest(raw + 32, w + 1);
-                    }
+                for (int w = 0; w < 4; w += 2) {
+                    tmem_wait_ld();
+                    FO_TMEM_LD32(s_at + 32 * w + 32, (raw + 32));
+                    largest(raw, w);
+                    tmem_wait_ld();
+                    FO_TMEM_LD32(s_at + (32 * w + 64) % 128, raw);  // (at last the first keys again)
+                    largest(raw + 32, w + 1);
                 }
                 float factor = 1.0f;  // of what has been summed so far
                 if (!any) {
@@ -610,7 +596,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 // P may be written, and O touched, once the PV before is complete.
                 // (In S's place, S would not be there before.)
                 if (any) {
-                    if (!ALIAS) ok = pt_wait(&sh.o_full[t], (c - 1) & 1, abort_flag);
+                    if (OWN_P) ok = pt_wait(&sh.o_full[t], (c - 1) & 1, abort_flag);
                     if (!ok) break;
                     if (__any_sync(0xffffffffu, factor != 1.0f)) {
                         tc_fence_after();
@@ -661,30 +647,21 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                         FO_TMEM_ST16(p_at + 16 * TERMS * w + 16, term);
                     }
                 };
-                auto half = [&]() {
-                    // The first half is multiplied while the second is computed.
-                    tmem_wait_st();
-                    tc_fence_before();
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&sh.p_half[t]);
-                };
-                if constexpr (!ALIAS) {
-#pragma unroll
-                    for (int w = 0; w < 4; w++) {
-                        probabilities(raw + 32 * w, w);
-                        if (w == 2) half();
-                    }
-                } else {
 #pragma unroll 1
-                    for (int w = 0; w < 4; w += 2) {
-                        tmem_wait_ld();
-                        FO_TMEM_LD32(s_at + 32 * w + 32, (raw + 32));
-                        probabilities(raw, w);
-                        if (w == 2) half();
-                        tmem_wait_ld();
-                        if (w == 0) FO_TMEM_LD32(s_at + 64, raw);
-                        probabilities(raw + 32, w + 1);
+                for (int w = 0; w < 4; w += 2) {
+                    tmem_wait_ld();
+                    FO_TMEM_LD32(s_at + 32 * w + 32, (raw + 32));
+                    probabilities(raw, w);
+                    if (w == 2) {
+                        // The first half is multiplied while the second is computed.
+                        tmem_wait_st();
+                        tc_fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&sh.p_half[t]);
                     }
+                    tmem_wait_ld();
+                    if (w == 0) FO_TMEM_LD32(s_at + 64, raw);
+                    probabilities(raw + 32, w + 1);
                 }
                 l += sum.x + sum.y;
                 if (turning) {
@@ -1124,7 +1101,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
             // Half h of the keys.
             auto issue_pv = [&](const Tile &x, int h) {
                 if (elect_one()) {
-                    const uint32_t p = tmem + (ALIAS ? 128 * t : 384 + 64 * t), o = tmem + 256 + (ALIAS ? 128 : 64) * t;
+                    const uint32_t p = tmem + (OWN_P ? 384 + 64 * t : 128 * t), o = tmem + 256 + (OWN_P ? 64 : 128) * t;
                     const uint64_t b = dV + (x.k & 1) * OPERAND16;
 #pragma unroll 1
                     for (int term = 0; term < TERMS; term++)
@@ -1196,18 +1173,6 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 bool issued = false;
                 const bool same = i < n;  // the next tile is of the same segment
                 if (same) next = take();
-                if (!ALIAS && same) {
-                    // The next S is computed while the softmax is at this one, which it holds in
-                    // registers, if its keys are there.
-                    ok = pt_wait(&sh.s_read[t], c & 1, abort_flag);
-                    if (!ok) break;
-                    issued = __all_sync(0xffffffffu, *(volatile int *)&sh.k_tile[next.k & 1] == next.k &&
-                                                         mbar_test(&sh.k_full[next.k & 1], (next.k >> 1) & 1));
-                    if (issued) {
-                        tc_fence_after();
-                        issue_s(next);
-                    }
-                }
                 ok = there(sh.v_full, sh.v_tile, now.k) && pt_wait(&sh.p_half[t], c & 1, abort_flag);
                 if (!ok) break;
                 tc_fence_after();
@@ -1215,6 +1180,15 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 ok = pt_wait(&sh.p_full[t], c & 1, abort_flag);
                 if (!ok) break;
                 tc_fence_after();
+                if (OWN_P && same) {
+                    // S first, if its keys are there: it is what the softmax waits for next.
+                    issued = __all_sync(0xffffffffu, *(volatile int *)&sh.k_tile[next.k & 1] == next.k &&
+                                                         mbar_test(&sh.k_full[next.k & 1], (next.k >> 1) & 1));
+                    if (issued) {
+                        tc_fence_after();
+                        issue_s(next);
+                    }
+                }
                 issue_pv(now, 1);
                 if (!issued) {
                     if (!same) {
@@ -1223,7 +1197,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                         next = take();
                     }
                     ok = there(sh.k_full, sh.k_tile, next.k);
-                    if (ok && ALIAS) ok = pt_wait(&sh.o_full[t], c & 1, abort_flag);
+                    if (ok && !OWN_P) ok = pt_wait(&sh.o_full[t], c & 1, abort_flag);
                     if (!ok) break;
                     tc_fence_after();
                     issue_s(next);
