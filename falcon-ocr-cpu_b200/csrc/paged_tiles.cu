@@ -494,7 +494,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
             float m = -INFINITY, l = 0.0f;
             int top = PT_LOWEST;  // exponent bits of a power of two above the scales of the values that the row sees
             bool any = false;
-            const bool turning = pair && 128 + 32 * wq < seg.nq;  // both have queries
+            // Turns, where both have queries.  (With P in columns of its own the streams do better without:
+            // a page's prompt 106.6 us, with 110.1; heads of 128 the other way, 2,443 and 2,375.)
+            const bool turning = !OWN_P && pair && 128 + 32 * wq < seg.nq;
             for (int i = pair ? 0 : t; i < n; i += pair ? 1 : 2, c++) {
                 const int k = base + i;
                 ok = pt_wait(&sh.s_full[t], c & 1, abort_flag);
