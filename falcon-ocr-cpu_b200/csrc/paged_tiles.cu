@@ -553,9 +553,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 }
                 // What 32 keys of a row need: their scores' factors (log2 units), the largest score, and
                 // the probabilities.
-                auto factor_of = [&](int g) { return plain ? meta.ks[g] * q_scale : 1.0f; };
+                // (Read before the scores are waited for.)
+                auto factors = [&](int w) {
+                    const float2 ks = *reinterpret_cast<const float2 *>(&meta.ks[2 * w]);
+                    return plain ? make_float2(ks.x * q_scale, ks.y * q_scale) : make_float2(1.0f, 1.0f);
+                };
                 float mx = -INFINITY;
-                auto largest = [&](const uint32_t *raw, int w) {
+                auto largest = [&](const uint32_t *raw, float2 f) {
 #pragma unroll
                     for (int g = 0; g < 2; g++) {
                         float m0 = -INFINITY, m1 = -INFINITY;
@@ -564,7 +568,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                             m0 = fmaxf(fmaxf(m0, __uint_as_float(raw[e])), __uint_as_float(raw[e + 1]));
                             m1 = fmaxf(fmaxf(m1, __uint_as_float(raw[e + 2])), __uint_as_float(raw[e + 3]));
                         }
-                        mx = fmaxf(mx, fmaxf(m0, m1) * factor_of(2 * w + g));
+                        mx = fmaxf(mx, fmaxf(m0, m1) * (g ? f.y : f.x));
                     }
                 };
                 // S is read twice, in short loops: what is run over and over has to stay in the instruction
@@ -574,12 +578,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 FO_TMEM_LD32(s_at, raw);
 #pragma unroll 1
                 for (int w = 0; w < 4; w += 2) {
+                    const float2 f0 = factors(w), f1 = factors(w + 1);
                     tmem_wait_ld();
                     FO_TMEM_LD32(s_at + 32 * w + 32, (raw + 32));
-                    largest(raw, w);
+                    largest(raw, f0);
                     tmem_wait_ld();
                     FO_TMEM_LD32(s_at + (32 * w + 64) % 128, raw);  // (at last the first keys again)
-                    largest(raw + 32, w + 1);
+                    largest(raw + 32, f1);
                 }
                 float factor = 1.0f;  // of what has been summed so far
                 if (!any) {
@@ -623,15 +628,16 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 // zeros.
                 const float inverse_top = __uint_as_float((uint32_t)(264 - top) << 23);
                 float2 sum = make_float2(0.0f, 0.0f);
-                auto probabilities = [&](const uint32_t *raw, int w) {
-                    const float f0 = factor_of(2 * w), f1 = factor_of(2 * w + 1);
-                    const float v0 = fminf(meta.vs[2 * w] * inverse_top, FLT_MAX);
-                    const float v1 = fminf(meta.vs[2 * w + 1] * inverse_top, FLT_MAX);
+                auto values = [&](int w) {
+                    const float2 vs = *reinterpret_cast<const float2 *>(&meta.vs[2 * w]);
+                    return make_float2(fminf(vs.x * inverse_top, FLT_MAX), fminf(vs.y * inverse_top, FLT_MAX));
+                };
+                auto probabilities = [&](const uint32_t *raw, int w, float2 f, float2 vs) {
                     float2 p[16];
                     uint32_t term[16];
 #pragma unroll
                     for (int e = 0; e < 16; e++) {
-                        const float g = e < 8 ? f0 : f1, v = e < 8 ? v0 : v1;
+                        const float g = e < 8 ? f.x : f.y, v = e < 8 ? vs.x : vs.y;
                         const float2 x = __ffma2_rn(make_float2(__uint_as_float(raw[2 * e]), __uint_as_float(raw[2 * e + 1])),
                                                     make_float2(g, g), make_float2(-shift, -shift));
                         p[e] = make_float2(ex2(x.x), ex2(x.y));
@@ -651,9 +657,10 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 };
 #pragma unroll 1
                 for (int w = 0; w < 4; w += 2) {
+                    const float2 f0 = factors(w), f1 = factors(w + 1), v0 = values(w), v1 = values(w + 1);
                     tmem_wait_ld();
                     FO_TMEM_LD32(s_at + 32 * w + 32, (raw + 32));
-                    probabilities(raw, w);
+                    probabilities(raw, w, f0, v0);
                     if (w == 2) {
                         // The first half is multiplied while the second is computed.
                         tmem_wait_st();
@@ -663,7 +670,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                     }
                     tmem_wait_ld();
                     if (w == 0) FO_TMEM_LD32(s_at + 64, raw);
-                    probabilities(raw + 32, w + 1);
+                    probabilities(raw + 32, w + 1, f1, v1);
                 }
                 l += sum.x + sum.y;
                 if (turning) {
