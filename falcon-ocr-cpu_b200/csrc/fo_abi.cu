@@ -187,7 +187,7 @@ struct fo_ctx {
     // use is kept).
     DevBuf tile_parts;
     std::vector<DevBuf> waiting;
-    float *tile_part_ml() const { return (float *)tile_parts.ptr + (size_t)2 * sms * FO_TILES_QUERIES * 128; }
+    float *tile_part_ml() const { return (float *)tile_parts.ptr + (size_t)3 * sms * FO_TILES_QUERIES * 128; }
     int32_t *tile_joins() const { return (int32_t *)(tile_part_ml() + (size_t)2 * sms * FO_TILES_QUERIES * 2); }
     size_t paged_part_rows() const { return (size_t)2 * sms * FO_PAGED_QUERIES; }
     float *paged_part_ml() const { return (float *)paged_parts.ptr + paged_part_rows() * 128; }
@@ -1838,8 +1838,8 @@ int make_tile_parts(fo_ctx *ctx) {
     std::lock_guard<std::mutex> lock(ctx->paged_mutex);
     if (ctx->tile_parts.ptr) return FO_OK;
     FO_TRY(refuse_capture(ctx->stream, "a context's first attention of many query rows makes its scratch and"));
-    const size_t rows = (size_t)2 * ctx->sms * FO_TILES_QUERIES;
-    FO_CUDA(ctx->tile_parts.ensure(rows * (128 + 2) * 4 + (size_t)ctx->sms * 32), "cudaMalloc(attention parts)");
+    const size_t rows = (size_t)ctx->sms * FO_TILES_QUERIES;
+    FO_CUDA(ctx->tile_parts.ensure(rows * (3 * 128 + 2 * 2) * 4 + (size_t)ctx->sms * 32), "cudaMalloc(attention parts)");
     return FO_OK;
 }
 

@@ -298,9 +298,9 @@ struct fo_paged_tiles_launch {
     int32_t window;  // 0: none
     struct fo_paged_reach reach;
     unsigned *err;
-    // Scratch of the context: a block's two unfinished parts, and which of them
-    // the second launch joins.
-    float *part_o;   // [2 sms][head_dim / 4][FO_TILES_QUERIES][4]
+    // Scratch of the context: a block's two unfinished parts, its sums outside tensor
+    // memory, and which of the parts the second launch joins.
+    float *part_o;   // [2 sms, and one more a block][head_dim / 4][FO_TILES_QUERIES][4]
     float *part_ml;  // [2 sms][FO_TILES_QUERIES][2]
     int32_t *joins;  // [sms][8]
     // Filled in by the launcher: query heads per KV head, units of queries per

@@ -66,6 +66,13 @@ constexpr uint32_t PT_SLOT = 8192, PT_PANEL = 16384;  // a slot of codes; 128 ro
 // the others.)
 constexpr int PT_START = 2;
 
+// FP32 rows: tiles after which O is taken out of tensor memory and added to by ordinary
+// FP32.  The tensor core's sums are truncated: a tile's sixteen additions leave 1e-7
+// less of what is there (40 sequences over 16,384 positions came out 1.4e-5 too
+// small; MEASURED so), which BF16 rows, at half of that and 2^-9 of rounding, do not
+// notice below millions of positions.
+constexpr int PT_KEEP = 4;
+
 // Exponent bits of a power of two above x (x from 2^-116 to 2^126; what is smaller
 // is taken as that, relative to which FP16 holds less of it).
 constexpr int PT_LOWEST = 12;
@@ -494,6 +501,48 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
             float m = -INFINITY, l = 0.0f;
             int top = PT_LOWEST;  // exponent bits of a power of two above the scales of the values that the row sees
             bool any = false;
+            // FP32 rows: what was summed up to a few tiles ago is outside tensor memory, relative to
+            // these.
+            bool kept = false;
+            float kept_m = 0.0f;
+            int kept_top = 0;
+            float4 *keep = reinterpret_cast<float4 *>(a.part_o) +
+                           (int64_t)(2 * gridDim.x + blockIdx.x) * (D / 4) * FO_TILES_QUERIES + 128 * t + r;
+            // O and the sums kept, into what is kept or (`back`) into O.
+            auto move = [&](bool back) {
+                const float f = !kept ? 0.0f
+                                      : (m == -INFINITY ? 1.0f : ex2(kept_m - m)) *
+                                            __uint_as_float((uint32_t)max(127 + kept_top - top, 0) << 23);
+                tc_fence_after();
+#pragma unroll 1
+                for (int d = 0; d < D; d += 16) {
+                    uint32_t o[16];
+                    FO_TMEM_LD16(o_at(t) + d, o);
+                    float4 y[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        y[e] = kept ? __ldcg(keep + (d / 4 + e) * FO_TILES_QUERIES) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        y[e].x = fmaf(y[e].x, f, __uint_as_float(o[4 * e]));
+                        y[e].y = fmaf(y[e].y, f, __uint_as_float(o[4 * e + 1]));
+                        y[e].z = fmaf(y[e].z, f, __uint_as_float(o[4 * e + 2]));
+                        y[e].w = fmaf(y[e].w, f, __uint_as_float(o[4 * e + 3]));
+                        if (!back) {
+                            __stcg(keep + (d / 4 + e) * FO_TILES_QUERIES, y[e]);
+                        } else {
+                            o[4 * e] = __float_as_uint(y[e].x), o[4 * e + 1] = __float_as_uint(y[e].y);
+                            o[4 * e + 2] = __float_as_uint(y[e].z), o[4 * e + 3] = __float_as_uint(y[e].w);
+                        }
+                    }
+                    if (back) FO_TMEM_ST16(o_at(t) + d, o);
+                }
+                if (back) tmem_wait_st();
+                kept = true;
+                kept_m = m;
+                kept_top = top;
+            };
             // Turns, where both have queries.  (With P in columns of its own the streams do better without:
             // a page's prompt 106.6 us, with 110.1; heads of 128 the other way, 2,443 and 2,375.)
             const bool turning = !OWN_P && pair && 128 + 32 * wq < seg.nq;
@@ -586,6 +635,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                     FO_TMEM_LD32(s_at + (32 * w + 64) % 128, raw);  // (at last the first keys again)
                     largest(raw + 32, f1);
                 }
+                if (F32 && any && i / (pair ? 1 : 2) % PT_KEEP == 0) move(false);
                 float factor = 1.0f;  // of what has been summed so far
                 if (!any) {
                     m = mx;
@@ -605,7 +655,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 if (any) {
                     if (OWN_P) ok = pt_wait(&sh.o_full[t], (c - 1) & 1, abort_flag);
                     if (!ok) break;
-                    if (__any_sync(0xffffffffu, factor != 1.0f)) {
+                    if (__any_sync(0xffffffffu, factor != 1.0f) && !(F32 && i / (pair ? 1 : 2) % PT_KEEP == 0)) {
                         tc_fence_after();
 #pragma unroll 1
                         for (int d = 0; d < D; d += 16) {
@@ -690,6 +740,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 if (!ok) break;
                 tc_fence_after();
             }
+            if (F32 && live && kept) move(true);
             // O times f0, and where both streams have these rows the other's times f1.
             const float unit = __uint_as_float((uint32_t)(top - 10) << 23);  // of O
             float f0 = unit, f1 = 0.0f;
@@ -1084,13 +1135,13 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
             constexpr uint32_t OPERAND16 = Shape::OPERAND >> 4, PANEL16 = PT_PANEL >> 4;
             struct Tile {
                 int k, pair;
-                bool first;  // of its segment's in this stream
+                bool first;  // of its segment's in this stream, or since O was taken away
             };
             auto issue_s = [&](const Tile &x) {
                 if (elect_one()) {
                     uint32_t more = 0;
 #pragma unroll 1
-                    for (int term = 0; term < TERMS; term++) {
+                    for (int term = TERMS - 1; term >= 0; term--) {
                         const uint64_t q = dQ + ((x.pair ? t : 0) * TERMS + term) * OPERAND16;
                         const uint64_t b = dK + (x.k & 1) * OPERAND16;
 #pragma unroll
@@ -1113,12 +1164,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                     const uint32_t p = tmem + (OWN_P ? 384 + 64 * t : 128 * t), o = tmem + 256 + (OWN_P ? 64 : 128) * t;
                     const uint64_t b = dV + (x.k & 1) * OPERAND16;
 #pragma unroll 1
-                    for (int term = 0; term < TERMS; term++)
+                    for (int term = TERMS - 1; term >= 0; term--)  // the small terms while the sum is
 #pragma unroll
                         for (int y = 0; y < 4; y++) {
                             const int kk = 4 * h + y;
                             mma_bf16_ts(o, p + 16 * (term + TERMS * (kk >> 1)) + 8 * (kk & 1), b + kk * (2048 >> 4), ID_PV,
-                                        term > 0 || kk > 0 || !x.first);
+                                        term < TERMS - 1 || kk > 0 || !x.first);
                         }
                     if (h == 1) {
                         mma_commit(&sh.o_full[t]);
@@ -1165,7 +1216,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 return ok;
             };
             auto take = [&]() {
-                const Tile x = {first + i, pair, i < (pair ? 1 : 2)};
+                const Tile x = {first + i, pair, F32 ? i / (pair ? 1 : 2) % PT_KEEP == 0 : i < (pair ? 1 : 2)};
                 i += pair ? 1 : 2;
                 return x;
             };
