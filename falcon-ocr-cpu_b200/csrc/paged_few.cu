@@ -43,14 +43,23 @@ __device__ __forceinline__ void pf_cluster_sync() {
     asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
     asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
-// A float of another block's shared memory, at this block's address.
-__device__ __forceinline__ float pf_remote(const float *p, uint32_t rank) {
-    const uint32_t at = (uint32_t)__cvta_generic_to_shared(p);
-    float x;
-    asm volatile("{\n\t.reg .b32 r;\n\tmapa.shared::cluster.u32 r, %1, %2;\n\tld.shared::cluster.f32 %0, [r];\n\t}"
-                 : "=f"(x)
-                 : "r"(at), "r"(rank)
-                 : "memory");
+// Another block's shared memory, at this block's address.  (In order with the cluster's
+// barriers, which are volatile too; ordinary loads may pass.)
+__device__ __forceinline__ uint32_t pf_at(const void *p, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"((uint32_t)__cvta_generic_to_shared(p)), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ float2 pf_remote2(const float *p, uint32_t rank) {
+    float2 x;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(x.x), "=f"(x.y) : "r"(pf_at(p, rank)));
+    return x;
+}
+__device__ __forceinline__ float4 pf_remote4(const float *p, uint32_t rank) {
+    float4 x;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
+                 : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w)
+                 : "r"(pf_at(p, rank)));
     return x;
 }
 __device__ __forceinline__ void pf_mma(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
@@ -400,11 +409,19 @@ __global__ void __launch_bounds__(PF_THREADS, F32 && NT == 2 ? 1 : 2)
                             fmaf(z.w, f, v.w * keep));
             high = up;
         };
-#pragma unroll 4
-        for (int c = 0; c < blocks; c++) {
-            const float *z = &sh.block_o[qi][4 * quad];
-            add(pf_remote(&sh.block_ml[qi][0], c), pf_remote(&sh.block_ml[qi][1], c),
-                make_float4(pf_remote(z, c), pf_remote(z + 1, c), pf_remote(z + 2, c), pf_remote(z + 3, c)));
+        // (Four blocks' at once: one after the other they took half of a call's time.)
+#pragma unroll 1
+        for (int c = 0; c < blocks; c += 4) {
+            float2 ml[4];
+            float4 z[4];
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                ml[e] = pf_remote2(sh.block_ml[qi], min(c + e, blocks - 1));
+                z[e] = pf_remote4(&sh.block_o[qi][4 * quad], min(c + e, blocks - 1));
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                if (c + e < blocks) add(ml[e].x, ml[e].y, z[e]);
         }
         if (a.reach.raw_o) {
             reinterpret_cast<float4 *>(a.reach.raw_o + at_row * D)[quad] = v;
