@@ -94,12 +94,33 @@ __device__ __forceinline__ uint32_t pf_widen(uint32_t pair) {
     }
 }
 
+// Copies into shared memory: 16 bytes, none of them read and zeros written where `bytes`
+// is 0, and 4.
+__device__ __forceinline__ void pf_copy16(void *to, const void *from, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from),
+                 "r"(bytes)
+                 : "memory");
+}
+__device__ __forceinline__ void pf_copy4(void *to, const void *from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from)
+                 : "memory");
+}
+
+// Steps of a warp that are on their way or computed, and later its part.
+template <int D>
+struct PfShape {
+    static constexpr int STAGES = D == 64 ? 4 : 3;
+    static constexpr int STAGE = 2 * 16 * D + 16;  // 16 positions' keys and values, and their page's scales
+};
 template <int D, int NT>
 struct PfShared {
-    float o[PF_WARPS][8 * NT][D];
-    float ml[PF_WARPS][8 * NT][2];
-    float block_o[8 * NT][D], block_ml[8 * NT][2];
+    float block_o[8 * NT][D], block_ml[8 * NT][2], ml[PF_WARPS][8 * NT][2];
+    // [warps][STAGES * STAGE], a warp's part [8 * NT][D] in its own
 };
+template <int D, int NT>
+__host__ __device__ constexpr int pf_smem(int warps) {
+    return (int)sizeof(PfShared<D, NT>) + warps * PfShape<D>::STAGES * PfShape<D>::STAGE;
+}
 
 // NT: n8 tiles of queries.
 template <int D, int FORMAT, bool F32, int NT>
@@ -107,10 +128,16 @@ __global__ void __launch_bounds__(PF_THREADS, F32 && NT == 2 ? 1 : 2)
     paged_few_kernel(const __grid_constant__ fo_paged_few_launch a) {
     using T = typename std::conditional<F32, float, uint16_t>::type;
     constexpr int TERMS = 1 + F32, HALVES = D / 64, KQ = 4 * HALVES;
-    extern __shared__ __align__(16) uint8_t pf_smem[];
-    PfShared<D, NT> &sh = *reinterpret_cast<PfShared<D, NT> *>(pf_smem);
+    constexpr int STAGES = PfShape<D>::STAGES, STAGE = PfShape<D>::STAGE;
+    static_assert(8 * NT * D * 4 <= STAGES * STAGE && sizeof(PfShared<D, NT>) % 16 == 0, "a warp's part");
+    extern __shared__ __align__(16) uint8_t pf_memory[];
+    PfShared<D, NT> &sh = *reinterpret_cast<PfShared<D, NT> *>(pf_memory);
     wait_for_prior_kernel();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
+    uint8_t *stages = pf_memory + sizeof(PfShared<D, NT>) + warp * STAGES * STAGE;
+    auto part_of = [&](int w) {
+        return reinterpret_cast<float *>(pf_memory + sizeof(PfShared<D, NT>) + w * STAGES * STAGE);
+    };
     const int heads = a.kv.n_kv_heads, page = a.kv.page_size, log_page = 31 - __clz(page);
     const int blocks = gridDim.y, rank = blocks > 1 ? (int)pf_cluster_rank() : 0;
     // The unit: rows [first, first + n) of a sequence or a group, positions [from, to), queries from q0 on.
@@ -203,60 +230,71 @@ __global__ void __launch_bounds__(PF_THREADS, F32 && NT == 2 ? 1 : 2)
 #pragma unroll
         for (int e = 0; e < 4; e++) o[d][e] = 0.0f;
 
-    // Steps of 16 positions, of one page; the next step's codes and scales on their way while one
-    // is computed, and the page number of the one after.
+    // Steps of 16 positions, of one page, several on their way at once (one ahead, in registers,
+    // left each step waiting 2,000 cycles for its own), and the page numbers of those after them.
     const int base = from & ~15, steps = to > from ? (to - base + 15) / 16 : 0, stride = a.warps * blocks;
     const int32_t *table = a.batch.page_table + seq * a.batch.table_stride;
-    struct Step {
-        uint4 k[HALVES][2];  // keys g and g + 8, dimensions 16 t ..
-        uint2 v[HALVES][4];  // positions 2 t, 2 t + 1, 2 t + 8, 2 t + 9, dimensions 8 g ..
-        float ks, vs;
-    };
     auto ask = [&](int at) { return at < steps ? table[((int64_t)base + 16 * (int64_t)at) >> log_page] : 0; };
-    auto load = [&](int at, int id, Step &x) {
-        x.ks = x.vs = 0.0f;
+    auto load = [&](int at, int id, int stage) {
+        if (at < steps) {
+            uint8_t *to_k = stages + stage * STAGE;
+            float *scales = reinterpret_cast<float *>(to_k + 32 * D);
+            const int pos = base + 16 * at;
+            const bool valid = id >= 0 && id < a.kv.n_pages;
+            const int64_t tile = (int64_t)(valid ? id : 0) * heads + head, codes = (tile * page + (pos & (page - 1))) * D;
+            const uint8_t *k = static_cast<const uint8_t *>(a.kv.k_codes) + codes, *v = static_cast<const uint8_t *>(a.kv.v_codes) + codes;
 #pragma unroll
-        for (int h = 0; h < HALVES; h++) {
-            x.k[h][0] = x.k[h][1] = make_uint4(0, 0, 0, 0);
-#pragma unroll
-            for (int e = 0; e < 4; e++) x.v[h][e] = make_uint2(0, 0);
-        }
-        if (at >= steps) return;
-        if (id < 0 || id >= a.kv.n_pages) {
-            // The rows that see the page get NaN, by their scores.
-            atomicOr(a.err, FO_DEVERR_PAGED);
-            x.ks = NAN;
-            return;
-        }
-        const int pos = base + 16 * at;
-        const int64_t tile = (int64_t)id * heads + head, codes = (tile * page + (pos & (page - 1))) * D;
-        const uint8_t *k = static_cast<const uint8_t *>(a.kv.k_codes) + codes + 16 * t;
-        const uint8_t *v = static_cast<const uint8_t *>(a.kv.v_codes) + codes + 8 * g;
-#pragma unroll
-        for (int h = 0; h < HALVES; h++) {
-            x.k[h][0] = *reinterpret_cast<const uint4 *>(k + g * D + 64 * h);
-            x.k[h][1] = *reinterpret_cast<const uint4 *>(k + (g + 8) * D + 64 * h);
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
+            for (int x = lane; x < D; x += 32) {
                 // Values that no row sees may be any bytes: an FP8 NaN times a probability of 0 would be NaN.
-                const int row = 2 * t + (e & 1) + 8 * (e >> 1);
-                if (row >= from - pos && row < to - pos) x.v[h][e] = *reinterpret_cast<const uint2 *>(v + row * D + 64 * h);
+                const int row = x / (D / 16);
+                const bool seen = valid && row >= from - pos && row < to - pos;
+                pf_copy16(to_k + 16 * x, k + 16 * x, valid ? 16 : 0);
+                pf_copy16(to_k + 16 * D + 16 * x, v + 16 * x, seen ? 16 : 0);
+            }
+            if (valid) {
+                if (lane < 2) pf_copy4(scales + lane, (lane ? a.kv.v_scales : a.kv.k_scales) + tile);
+            } else if (lane == 0) {
+                // The rows that see the page get NaN, by their scores.
+                atomicOr(a.err, FO_DEVERR_PAGED);
+                scales[0] = NAN;
+                scales[1] = 0.0f;
             }
         }
-        x.ks = a.kv.k_scales[tile];
-        x.vs = a.kv.v_scales[tile];
-        if (!(fabsf(x.vs) <= FLT_MAX)) x.ks = NAN, x.vs = 0.0f;
+        asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    int i = warp * blocks + rank;
-    const int id0 = ask(i);
-    int id1 = ask(i + stride);
-    Step now, next;
-    load(i, id0, now);
+    int i = warp * blocks + rank, ids[STAGES + 1];
+#pragma unroll
+    for (int x = 0; x <= STAGES; x++) ids[x] = ask(i + x * stride);
+#pragma unroll
+    for (int x = 0; x < STAGES - 1; x++) load(i + x * stride, ids[x], x);
+    int id0 = ids[STAGES - 1], id1 = ids[STAGES];
 #pragma unroll 1
-    for (; i < steps; i += stride) {
-        load(i + stride, id1, next);
-        id1 = ask(i + 2 * stride);
+    for (int stage = 0; i < steps; i += stride) {
+        load(i + (STAGES - 1) * stride, id0, stage == 0 ? STAGES - 1 : stage - 1);
+        id0 = id1;
+        id1 = ask(i + (STAGES + 1) * stride);
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+        __syncwarp();
         const int pos = base + 16 * i;
+        struct {
+            uint4 k[HALVES][2];  // keys g and g + 8, dimensions 16 t ..
+            uint2 v[HALVES][4];  // positions 2 t, 2 t + 1, 2 t + 8, 2 t + 9, dimensions 8 g ..
+            float ks, vs;
+        } now;
+        const uint8_t *at = stages + stage * STAGE;
+#pragma unroll
+        for (int h = 0; h < HALVES; h++) {
+            now.k[h][0] = *reinterpret_cast<const uint4 *>(at + g * D + 64 * h + 16 * t);
+            now.k[h][1] = *reinterpret_cast<const uint4 *>(at + (g + 8) * D + 64 * h + 16 * t);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                now.v[h][e] = *reinterpret_cast<const uint2 *>(at + (16 + 2 * t + (e & 1) + 8 * (e >> 1)) * D + 64 * h + 8 * g);
+        }
+        now.ks = *reinterpret_cast<const float *>(at + 32 * D);
+        now.vs = *reinterpret_cast<const float *>(at + 32 * D + 4);
+        if (!(fabsf(now.vs) <= FLT_MAX)) now.ks = NAN, now.vs = 0.0f;
+        __syncwarp();  // the stage may be written again
+        stage = stage == STAGES - 1 ? 0 : stage + 1;
         // Scores in log2 units: keys g and g + 8, columns 2 t and 2 t + 1 of a tile.
         float c[NT][4];
 #pragma unroll
@@ -348,10 +386,12 @@ __global__ void __launch_bounds__(PF_THREADS, F32 && NT == 2 ? 1 : 2)
 #pragma unroll
                 for (int z = 0; z < TERMS; z++) pf_mma(o[8 * h + j], p[z][0], p[z][1], p[z][2], p[z][3], b0, b1);
             }
-        now = next;
     }
 
-    // This warp's part.
+    // This warp's part, in place of its stages.
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+    __syncwarp();
+    float *part = part_of(warp);
 #pragma unroll
     for (int x = 0; x < NT; x++) {
 #pragma unroll
@@ -369,27 +409,29 @@ __global__ void __launch_bounds__(PF_THREADS, F32 && NT == 2 ? 1 : 2)
             for (int e = 0; e < 2; e++)
 #pragma unroll
                 for (int j = 0; j < 8; j += 4)
-                    *reinterpret_cast<float4 *>(&sh.o[warp][8 * x + g][64 * h + 8 * (2 * t + e) + j]) =
+                    *reinterpret_cast<float4 *>(part + (8 * x + g) * D + 64 * h + 8 * (2 * t + e) + j) =
                         make_float4(o[8 * h + j][2 * x + e] * unit, o[8 * h + j + 1][2 * x + e] * unit,
                                     o[8 * h + j + 2][2 * x + e] * unit, o[8 * h + j + 3][2 * x + e] * unit);
     }
     __syncthreads();
     // The block's warps.
 #pragma unroll 1
-    for (int y = threadIdx.x; y < n_queries * D; y += blockDim.x) {
-        const int qi = y / D, d = y % D;
-        float high = -INFINITY, sum = 0.0f, v = 0.0f;
+    for (int y = threadIdx.x; y < n_queries * (D / 4); y += blockDim.x) {
+        const int qi = y / (D / 4), quad = y % (D / 4);
+        float high = -INFINITY, sum = 0.0f;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 4
         for (int w = 0; w < a.warps; w++) high = fmaxf(high, sh.ml[w][qi][0]);
         const float shift = high == -INFINITY ? 0.0f : high;
 #pragma unroll 4
         for (int w = 0; w < a.warps; w++) {
             const float f = sm100::ex2(sh.ml[w][qi][0] - shift);
+            const float4 z = *reinterpret_cast<const float4 *>(part_of(w) + qi * D + 4 * quad);
             sum = fmaf(sh.ml[w][qi][1], f, sum);
-            v = fmaf(sh.o[w][qi][d], f, v);
+            v = make_float4(fmaf(z.x, f, v.x), fmaf(z.y, f, v.y), fmaf(z.z, f, v.z), fmaf(z.w, f, v.w));
         }
-        sh.block_o[qi][d] = v;
-        if (d == 0) sh.block_ml[qi][0] = high, sh.block_ml[qi][1] = sum;
+        *reinterpret_cast<float4 *>(&sh.block_o[qi][4 * quad]) = v;
+        if (quad == 0) sh.block_ml[qi][0] = high, sh.block_ml[qi][1] = sum;
     }
     if (blocks > 1) pf_cluster_sync();
     else __syncthreads();
@@ -441,7 +483,7 @@ __global__ void __launch_bounds__(PF_THREADS, F32 && NT == 2 ? 1 : 2)
             const float2 ml = __ldcg(reinterpret_cast<const float2 *>(a.reach.prior_ml) + at_row);
             add(ml.x, ml.y, __ldcg(reinterpret_cast<const float4 *>(a.reach.prior_o + at_row * D) + quad));
         }
-#pragma unroll 4
+#pragma unroll 6
         for (int c = c0; c <= c1; c++) {
             const int64_t part = 2 * c + (c == c0 ? 1 : 0);
             const float2 ml = __ldcg(reinterpret_cast<const float2 *>(a.part_ml) + part * FO_TILES_QUERIES + unit_q);
@@ -470,7 +512,7 @@ template <int D, int FORMAT, bool F32, int NT>
 cudaError_t launch_few(const fo_paged_few_launch &in, int sms, cudaStream_t stream) {
     fo_paged_few_launch a = in;
     auto *kernel = paged_few_kernel<D, FORMAT, F32, NT>;
-    constexpr int SMEM = sizeof(PfShared<D, NT>);
+    constexpr int SMEM = pf_smem<D, NT>(PF_WARPS);
     if constexpr (SMEM > 48 * 1024) {
         // The attribute belongs to each device's context: set once per device.
         static std::atomic<unsigned long long> configured{0};
@@ -499,7 +541,7 @@ cudaError_t launch_few(const fo_paged_few_launch &in, int sms, cudaStream_t stre
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)units, (unsigned)blocks);
     cfg.blockDim = dim3(32 * a.warps);
-    cfg.dynamicSmemBytes = SMEM;
+    cfg.dynamicSmemBytes = pf_smem<D, NT>(a.warps);
     cfg.stream = stream;
     cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
