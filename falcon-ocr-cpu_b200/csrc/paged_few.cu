@@ -96,14 +96,11 @@ __device__ __forceinline__ uint32_t pf_widen(uint32_t pair) {
 
 // Copies into shared memory: 16 bytes, none of them read and zeros written where `bytes`
 // is 0, and 4.
-__device__ __forceinline__ void pf_copy16(void *to, const void *from, int bytes) {
-    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from),
-                 "r"(bytes)
-                 : "memory");
+__device__ __forceinline__ void pf_copy16(uint32_t to, const void *from, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
 }
-__device__ __forceinline__ void pf_copy4(void *to, const void *from) {
-    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"((uint32_t)__cvta_generic_to_shared(to)), "l"(from)
-                 : "memory");
+__device__ __forceinline__ void pf_copy4(uint32_t to, const void *from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
 }
 
 // Steps of a warp that are on their way or computed, and later its part.
@@ -235,42 +232,51 @@ __global__ void __launch_bounds__(PF_THREADS, F32 && NT == 2 ? 1 : 2)
     const int base = from & ~15, steps = to > from ? (to - base + 15) / 16 : 0, stride = a.warps * blocks;
     const int32_t *table = a.batch.page_table + seq * a.batch.table_stride;
     auto ask = [&](int at) { return at < steps ? table[((int64_t)base + 16 * (int64_t)at) >> log_page] : 0; };
+    const uint32_t page_bytes = (uint32_t)(page * D), to_stages = (uint32_t)__cvta_generic_to_shared(stages) + 16 * lane;
+    const uint8_t *my_k = static_cast<const uint8_t *>(a.kv.k_codes) + (int64_t)head * page_bytes + 16 * lane;
+    const uint8_t *my_v = static_cast<const uint8_t *>(a.kv.v_codes) + (int64_t)head * page_bytes + 16 * lane;
+    const float *my_scales = (lane & 1 ? a.kv.v_scales : a.kv.k_scales) + head;
     auto load = [&](int at, int id, int stage) {
         if (at < steps) {
-            uint8_t *to_k = stages + stage * STAGE;
-            float *scales = reinterpret_cast<float *>(to_k + 32 * D);
+            const uint32_t to_k = to_stages + stage * STAGE;
             const int pos = base + 16 * at;
-            const bool valid = id >= 0 && id < a.kv.n_pages;
-            const int64_t tile = (int64_t)(valid ? id : 0) * heads + head, codes = (tile * page + (pos & (page - 1))) * D;
-            const uint8_t *k = static_cast<const uint8_t *>(a.kv.k_codes) + codes, *v = static_cast<const uint8_t *>(a.kv.v_codes) + codes;
+            if (id >= 0 && id < a.kv.n_pages) {
+                const int64_t codes = (int64_t)id * ((int64_t)heads * page_bytes) + (pos & (page - 1)) * D;
 #pragma unroll
-            for (int x = lane; x < D; x += 32) {
-                // Values that no row sees may be any bytes: an FP8 NaN times a probability of 0 would be NaN.
-                const int row = x / (D / 16);
-                const bool seen = valid && row >= from - pos && row < to - pos;
-                pf_copy16(to_k + 16 * x, k + 16 * x, valid ? 16 : 0);
-                pf_copy16(to_k + 16 * D + 16 * x, v + 16 * x, seen ? 16 : 0);
-            }
-            if (valid) {
-                if (lane < 2) pf_copy4(scales + lane, (lane ? a.kv.v_scales : a.kv.k_scales) + tile);
-            } else if (lane == 0) {
+                for (int x = 0; x < D; x += 32) {
+                    // Values that no row sees may be any bytes: an FP8 NaN times a probability of 0 would be NaN.
+                    const int row = (x + lane) / (D / 16) + pos;
+                    pf_copy16(to_k + 16 * x, my_k + codes + 16 * x, 16);
+                    pf_copy16(to_k + 16 * D + 16 * x, my_v + codes + 16 * x, row >= from && row < to ? 16 : 0);
+                }
+                if (lane < 2) pf_copy4(to_k + 32 * D - 12 * lane, my_scales + (int64_t)id * heads);
+            } else {
+#pragma unroll
+                for (int x = 0; x < 2 * D; x += 32) pf_copy16(to_k + 16 * x, my_k, 0);
+                if (lane > 0) return;
+                float *scales = reinterpret_cast<float *>(stages + stage * STAGE + 32 * D);
+
                 // The rows that see the page get NaN, by their scores.
                 atomicOr(a.err, FO_DEVERR_PAGED);
                 scales[0] = NAN;
                 scales[1] = 0.0f;
             }
         }
-        asm volatile("cp.async.commit_group;" ::: "memory");
     };
+    auto commit = []() { asm volatile("cp.async.commit_group;" ::: "memory"); };
     int i = warp * blocks + rank, ids[STAGES + 1];
 #pragma unroll
     for (int x = 0; x <= STAGES; x++) ids[x] = ask(i + x * stride);
 #pragma unroll
-    for (int x = 0; x < STAGES - 1; x++) load(i + x * stride, ids[x], x);
+    for (int x = 0; x < STAGES - 1; x++) {
+        load(i + x * stride, ids[x], x);
+        commit();
+    }
     int id0 = ids[STAGES - 1], id1 = ids[STAGES];
 #pragma unroll 1
     for (int stage = 0; i < steps; i += stride) {
         load(i + (STAGES - 1) * stride, id0, stage == 0 ? STAGES - 1 : stage - 1);
+        commit();
         id0 = id1;
         id1 = ask(i + (STAGES + 1) * stride);
         asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
@@ -513,14 +519,15 @@ cudaError_t launch_few(const fo_paged_few_launch &in, int sms, cudaStream_t stre
     fo_paged_few_launch a = in;
     auto *kernel = paged_few_kernel<D, FORMAT, F32, NT>;
     constexpr int SMEM = pf_smem<D, NT>(PF_WARPS);
-    if constexpr (SMEM > 48 * 1024) {
-        // The attribute belongs to each device's context: set once per device.
+    {
+        // The attributes belong to each device's context: set once per device.
         static std::atomic<unsigned long long> configured{0};
         int dev = 0;
         cudaGetDevice(&dev);
         const unsigned long long bit = 1ull << (dev & 63);
         if (!(configured.load() & bit)) {
             cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM);
+            if (e == cudaSuccess) e = cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1);
             if (e != cudaSuccess) return e;
             configured.fetch_or(bit);
         }
@@ -537,6 +544,10 @@ cudaError_t launch_few(const fo_paged_few_launch &in, int sms, cudaStream_t stre
     const int64_t busy = a.reach.over_groups ? (int64_t)a.reach.n_groups * a.kv.n_kv_heads : units;
     int blocks = 1;
     while (blocks < 8 && 2 * blocks * busy <= 2 * sms) blocks *= 2;
+    // Sixteen, which want that many SMs next to each other, for no more units than there are such
+    // neighbourhoods: 8 units over 6,544 positions 20.2 us with sixteen, 23.2 with eight; 16 units
+    // 37.0 and 33.2.
+    if (blocks == 8 && 16 * busy <= sms) blocks = 16;
     a.warps = busy > 2 * sms ? 4 : 8;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3((unsigned)units, (unsigned)blocks);
