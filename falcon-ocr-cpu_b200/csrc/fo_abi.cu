@@ -1991,12 +1991,20 @@ int check_attention(const char *name, const fo_paged_kv *kv, const fo_paged_batc
 // at most `units` sequences or groups.
 int check_tiles(const char *name, const fo_paged_kv *kv, const fo_paged_batch *batch, double wide, double units) {
     const double tiles = kv->n_kv_heads * (wide / FO_PAGED_QUERIES + units) *
-                         ((double)batch->table_stride * kv->page_size * kv->head_dim / 8192 + 2);
+                         ((double)batch->table_stride * kv->page_size * kv->head_dim / 8192 + 4);
     if (wide > INT32_MAX) return fail(FO_ERR_CAPACITY, "%s: more than 2^31 query rows of a KV head", name);
     if (tiles > INT32_MAX)
         return fail(FO_ERR_CAPACITY, "%s: the batch's page tables have room for more than 2^31 tiles", name);
     return FO_OK;
 }
+
+// Query rows of a KV head up to which paged_attention.cuh is the faster kernel for
+// sequences by themselves.  48 sequences in a window of 4,096, int8, BF16, in
+// microseconds by query rows, that kernel / paged_tiles.cu's:
+//   heads of 64   16: 83 / 217   24: 109 / 217   40: 196 / 217   64: 290 / 219
+//   heads of 128  16: 125 / 291  24: 176 / 291   40: 313 / 295   64: 515 / 297
+// (25 to 48 take as long as 40; with e4m3 codes and FP32 rows the order is the same.)
+int64_t alone_few(int32_t head_dim) { return head_dim == 64 ? 48 : 24; }
 
 // One launch of a paged attention with a reach: few query rows of a KV head by
 // the one kernel, many by the other.
@@ -2146,7 +2154,7 @@ int fo_paged_window_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged
     fo_paged_reach reach = {};
     reach.first = (int32_t)std::min<int64_t>(first, INT32_MAX);
     return launch_reach(ctx, kv, batch, q, out, sinks, lse, scale, window < INT32_MAX ? (int32_t)window : 0, reach,
-                        batch->max_rows * group <= FO_PAGED_FEW);
+                        batch->max_rows * group <= alone_few(kv->head_dim));
 }
 
 int fo_paged_prefix_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch *batch,
@@ -2170,7 +2178,7 @@ int fo_paged_prefix_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged
     reach.group_lens = groups->lens;
     reach.n_groups = (int32_t)groups->n_groups;
     if (reach.n_groups == 0)
-        return launch_reach(ctx, kv, batch, q, out, sinks, lse, scale, 0, reach, queries <= FO_PAGED_FEW);
+        return launch_reach(ctx, kv, batch, q, out, sinks, lse, scale, 0, reach, queries <= alone_few(kv->head_dim));
     // Half a tile of query rows and more: the products bound the call, however
     // often the beginning is read, so each sequence goes over all it sees.
     if (queries >= FO_PAGED_ALONE) return launch_reach(ctx, kv, batch, q, out, sinks, lse, scale, 0, reach, false);

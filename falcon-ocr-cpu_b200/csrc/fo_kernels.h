@@ -287,6 +287,7 @@ cudaError_t fo_launch_paged_attention_reach(const fo_paged_attention_launch *arg
 // Attention of many query rows over the paged cache on the 5th-generation
 // tensor cores (paged_tiles.cu).
 #define FO_TILES_QUERIES 256  // query rows of a block's unit at most
+#define FO_PAGED_FEW 16       // query rows of a sequence up to which shared beginnings go by paged_few.cu
 #define FO_PAGED_ALONE 64     // query rows of a sequence from which on it reads a shared beginning by itself
 struct fo_paged_tiles_launch {
     fo_paged_kv kv;
@@ -304,7 +305,8 @@ struct fo_paged_tiles_launch {
     float *part_ml;  // [2 sms][FO_TILES_QUERIES][2]
     int32_t *joins;  // [sms][8]
     // Filled in by the launcher: query heads per KV head, units of queries per
-    // sequence, what 16-byte accesses may be used for.
+    // sequence (0: numbered by the rows before it), what 16-byte accesses may be used
+    // for.
     int32_t group, q_units, q_vec, out_vec;
 };
 cudaError_t fo_launch_paged_tiles(const fo_paged_tiles_launch *args, int sms, cudaStream_t stream);

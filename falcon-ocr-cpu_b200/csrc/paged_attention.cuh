@@ -71,13 +71,12 @@
 //
 // With REACH (paged_attention_reach.cu; the variants without it are unchanged
 // by it) a row also sees a few first positions behind its window, whose tiles
-// come before the window's in the line; or its sequence's positions behind a
-// beginning that it shares; or the units are the groups of sequences that share
-// a beginning, all their rows over it; and rows are written unfinished, or joined
-// with unfinished ones of another call.
+// come before the window's in the line.  64 sequences in a window of 4,096 with
+// 16 first positions, 2 query rows to each of 8 KV heads of 64: 58 us against a
+// floor of 41; a unit's change costs some 3 us and a unit here is short.
 #pragma once
 
-#include "paged_reach.cuh"
+#include "paged.cuh"
 #include "sm100.cuh"
 
 #include <algorithm>
@@ -203,19 +202,9 @@ __device__ __forceinline__ int pa_tile(const fo_paged_attention_launch &a, const
 template <int TILE, bool REACH>
 __device__ __forceinline__ PaWork pa_work(const fo_paged_attention_launch &a, int seq) {
     PaWork w;
-    if (REACH && a.reach.over_groups) {
-        const Group g = load_group(a.reach, a.batch, a.kv.page_size, seq, a.err);
-        w.s.first = g.first;
-        w.s.n = g.n;
-        w.s.len = g.len;
-        w.low = 0;
-    } else {
-        w.s = load_sequence(a.batch, a.kv.page_size, seq, a.err);
-        const int p0 = max(w.s.len - w.s.n, 0);
-        w.low = a.window > 0 ? max(p0 + 1 - a.window, 0) : 0;
-        if (REACH && a.reach.own_only)
-            w.low = min(shared_of(a.reach, a.batch, a.kv.page_size, seq, a.err).len, w.s.len);
-    }
+    w.s = load_sequence(a.batch, a.kv.page_size, seq, a.err);
+    const int p0 = max(w.s.len - w.s.n, 0);
+    w.low = a.window > 0 ? max(p0 + 1 - a.window, 0) : 0;
     w.t0 = w.low / TILE;
     w.tiles = (int)(((unsigned)w.s.len + TILE - 1) / TILE) - w.t0;
     if constexpr (REACH) w.tiles += pa_early<TILE>(a, w);
@@ -223,12 +212,6 @@ __device__ __forceinline__ PaWork pa_work(const fo_paged_attention_launch &a, in
     const int queries = w.s.n * a.group;
     w.groups = queries <= a.queries ? queries > 0 : (queries + FO_PAGED_QUERIES - 1) / FO_PAGED_QUERIES;
     return w;
-}
-
-// Sequences of the line.
-template <bool REACH>
-__device__ __forceinline__ int pa_sequences(const fo_paged_attention_launch &a) {
-    return REACH && a.reach.over_groups ? a.reach.n_groups + 2 : (int)a.batch.n_seqs;
 }
 
 // A place in the line: a sequence, a unit of it (KV head, group of queries)
@@ -248,7 +231,7 @@ struct PaCursor {
         if (++unit < a.kv.n_kv_heads * w.groups) return;
         unit = 0;
         do {
-            if (++seq >= pa_sequences<REACH>(a)) return;
+            if (++seq >= (int)a.batch.n_seqs) return;
             w = pa_work<TILE, REACH>(a, seq);
         } while (w.groups == 0);
     }
@@ -354,28 +337,11 @@ __device__ __forceinline__ PaUnit pa_unit(const fo_paged_attention_launch &a, co
 
 // Four dimensions of a query's output from their sum v, the sum ll of the
 // probabilities and the maximum mm that both are relative to.
-template <int D, bool F32, bool REACH>
+template <int D, bool F32>
 __device__ __forceinline__ void pa_write(const fo_paged_attention_launch &a, const PaUnit &u, int qi, int quad, float4 v,
                                          float mm, float ll) {
     using T = typename std::conditional<F32, float, uint16_t>::type;
     const int q = u.q0 + qi, r = q / a.group, h = u.head * a.group + q - r * a.group;
-    if constexpr (REACH) {
-        const int64_t at_row = (int64_t)(u.first + r) * a.q.heads + h;
-        if (a.reach.raw_o) {
-            reinterpret_cast<float4 *>(a.reach.raw_o + at_row * D)[quad] = v;
-            if (quad == 0) reinterpret_cast<float2 *>(a.reach.raw_ml)[at_row] = make_float2(mm, ll);
-            return;
-        }
-        if (a.reach.prior_o) {
-            const float2 ml = reinterpret_cast<const float2 *>(a.reach.prior_ml)[at_row];
-            const float4 x = reinterpret_cast<const float4 *>(a.reach.prior_o + at_row * D)[quad];
-            const Joined j = join_parts(mm, ll, ml.x, ml.y);
-            v = make_float4(fmaf(x.x, j.f1, v.x * j.f0), fmaf(x.y, j.f1, v.y * j.f0), fmaf(x.z, j.f1, v.z * j.f0),
-                            fmaf(x.w, j.f1, v.w * j.f0));
-            mm = j.m;
-            ll = j.l;
-        }
-    }
     float sum = ll;
     if (a.sinks) sum += sm100::ex2(fmaf(a.sinks[h], PA_LOG2E, -mm));
     const float inv = ll == 0.0f ? 0.0f : 1.0f / sum;
@@ -397,7 +363,7 @@ __device__ __forceinline__ void pa_write(const fo_paged_attention_launch &a, con
 // The blocks' parts of a unit joined in their order, by warp `rank` of `warps`
 // (all of them in the last block to come), a query at a time: the maxima and
 // sums a block to a lane, then four dimensions to a lane.
-template <int D, bool F32, bool REACH>
+template <int D, bool F32>
 __device__ __forceinline__ void pa_join_blocks(const fo_paged_attention_launch &a, const PaUnit &u, int rank, int warps) {
     constexpr int QUADS = D / 4, SETS = 32 / QUADS;  // lanes that share a quad take every SETS-th block
     const int lane = threadIdx.x & 31, quad = lane % QUADS, set = lane / QUADS;
@@ -440,7 +406,7 @@ __device__ __forceinline__ void pa_join_blocks(const fo_paged_attention_launch &
             v.z += __shfl_xor_sync(0xffffffffu, v.z, 16);
             v.w += __shfl_xor_sync(0xffffffffu, v.w, 16);
         }
-        if (set == 0) pa_write<D, F32, REACH>(a, u, qi, quad, v, mm, lost ? NAN : ll);
+        if (set == 0) pa_write<D, F32>(a, u, qi, quad, v, mm, lost ? NAN : ll);
     }
 }
 
@@ -507,11 +473,7 @@ __device__ __forceinline__ void pa_epilogue(const fo_paged_attention_launch &a, 
             if (t == 0) {
                 const bool good = (all_finite >> (lane & 28) & 15) == 15;
                 sh.q_scale[qi] = good ? __uint_as_float((uint32_t)e << 23) / up * a.scale * PA_LOG2E : NAN;
-                int pos = q ? u.w.s.len - u.w.s.n + r : -1;
-                // Over a group's shared positions: as far as the row sees of them, if it is a row.
-                if (REACH && a.reach.over_groups)
-                    pos = min(q ? place_of_row(a.batch, a.kv.page_size, u.w.s.first + r, a.err) : INT32_MAX, u.w.s.len - 1);
-                sh.q_pos[qi] = pos;
+                sh.q_pos[qi] = q ? u.w.s.len - u.w.s.n + r : -1;
             }
             uint2 *to = q_ops + tile * (Shape::Q_TILE / 8) + lane;
 #pragma unroll 1
@@ -592,7 +554,7 @@ __device__ __forceinline__ void pa_epilogue(const fo_paged_attention_launch &a, 
             }
             if (lost) ll = NAN;
             if (u.alone) {
-                pa_write<D, F32, REACH>(a, u, qi, quad, v, mm, ll);
+                pa_write<D, F32>(a, u, qi, quad, v, mm, ll);
             } else {
                 const int64_t at_me = u.part(a, blockIdx.x, qi);
                 __stcg(reinterpret_cast<float4 *>(a.part_o + at_me * D) + quad, v);
@@ -622,7 +584,7 @@ __device__ __forceinline__ void pa_epilogue(const fo_paged_attention_launch &a, 
             }
             if (!sm100::mbar_wait(&sh.shared_go[last], 0, &sh.abort, a.err)) return;
             if (sh.joins[last])
-                pa_join_blocks<D, F32, REACH>(a, u, me, last ? PA_EPILOGUES + PA_CONSUMERS : PA_EPILOGUES);
+                pa_join_blocks<D, F32>(a, u, me, last ? PA_EPILOGUES + PA_CONSUMERS : PA_EPILOGUES);
         }
         i += n;
         at.advance(a, n);
@@ -674,7 +636,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
     // line's tiles are below 2^31, checked on the host.)
     // No more units than blocks, and short ones: a block for each, since handing a
     // part on to another block takes longer (about 4 us) than these tiles.
-    const int n_seqs = pa_sequences<REACH>(a), few = 4 * key_groups;
+    const int n_seqs = (int)a.batch.n_seqs, few = 4 * key_groups;
     PaCursor<TILE, REACH> at;
     int per = 0, begin = 0, end, base;
     bool whole = false;
@@ -805,9 +767,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                 (int64_t)pa_tile<TILE, REACH>(a, at.w, at.tile + skip + PA_PRODUCERS * off) * TILE + (j << log_page);
             const int64_t begins = pos >> log_page << log_page;
             if (off < b.n && pos < at.w.s.len && (begins + page > at.w.low || (REACH && begins < a.reach.first))) {
-                int seq = at.seq;
-                if (REACH && a.reach.over_groups) seq = a.reach.group_start[seq - 1];
-                b.id = a.batch.page_table[seq * a.batch.table_stride + (pos >> log_page)];
+                b.id = a.batch.page_table[at.seq * a.batch.table_stride + (pos >> log_page)];
                 b.row = (int)(pos - begins);
                 b.wanted = true;
             }
@@ -871,8 +831,21 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                 if (here) {
                     // A page number outside the pool gives NaN; a page that no row
                     // sees has scales of 0.
-                    sh.scales[slot][j] = now.bad ? NAN : now.ks;
-                    sh.scales[slot][8 + j] = now.bad ? NAN : now.vs;
+                    if constexpr (REACH) {
+                        // Like values that are not finite, by the scores: rows that do not see the page are
+                        // not changed by it.
+                        const bool lost = now.bad || !(fabsf(now.vs) <= FLT_MAX);
+                        sh.scales[slot][j] = lost ? NAN : now.ks;
+                        sh.scales[slot][8 + j] = lost ? 0.0f : now.vs;
+                        if (now.bad) {
+                            uint4 *vt = reinterpret_cast<uint4 *>(tiles + slot * Shape::STAGE + Shape::TILE_BYTES + j * bytes);
+                            for (uint32_t x = 0; x < bytes / 16; x++) vt[x] = make_uint4(0, 0, 0, 0);
+                            sm100::fence_proxy_async_smem();  // these before the next copy
+                        }
+                    } else {
+                        sh.scales[slot][j] = now.bad ? NAN : now.ks;
+                        sh.scales[slot][8 + j] = now.bad ? NAN : now.vs;
+                    }
                     if (now.bad) atomicOr(a.err, FO_DEVERR_PAGED);
                 }
                 __syncwarp();
@@ -921,7 +894,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         const int n = min(here.left(), count - i);
         const int n_queries = min(here.w.s.n * a.group - here.group() * a.queries, a.queries);  // of this unit
         const int len = here.w.s.len, low = here.w.low;
-        int p_first = len - here.w.s.n;  // positions of the sequence's first row and of its last
+        const int p_first = len - here.w.s.n;  // positions of the sequence's first row and of its last
         const int p_last = p_first + here.w.s.n - 1;
         const int tile0 = here.w.t0 + here.tile - i;
         // The queries as B operands.
@@ -944,15 +917,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         }
         float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f}, o[MT][4] = {};
         // Tiles all of whose positions every row sees need no mask.
-        int low_last = a.window > 0 ? max(p_last + 1 - a.window, 0) : 0;
-        if constexpr (REACH) {
-            low_last = max(low_last, low);
-            if (a.reach.over_groups) {  // the warp's rows are of several sequences
-                p_first = min(q_pos[0], q_pos[1]);
-                p_first = min(p_first, __shfl_xor_sync(0xffffffffu, p_first, 1));
-                p_first = min(p_first, __shfl_xor_sync(0xffffffffu, p_first, 2));
-            }
-        }
+        const int low_last = a.window > 0 ? max(p_last + 1 - a.window, 0) : 0;
         bool any = false;
 
         int k = i + (key_group - i % key_groups + key_groups) % key_groups;
@@ -974,18 +939,13 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
             if constexpr (!I8) {
                 // Rows beyond the sequence, or of pages that no row sees, may hold any
                 // bytes: an FP8 NaN times a probability of 0 would be NaN.
-                // (Behind a shared beginning, rows of the page that it ends in, too.)
-                int lo_row = max((low >> log_page << log_page) - pos0, 0);
-                const int hi_row = min(len - pos0, HALF);
-                int early = 0;  // rows of the first positions' pages, which are there
-                if constexpr (REACH) {
-                    if (a.reach.own_only) lo_row = max(low - pos0, 0);
-                    else early = ((a.reach.first + page - 1) >> log_page << log_page) - pos0;
-                }
+                // (The first positions' pages are there, behind a window too.)
+                const int lo_row = max((low >> log_page << log_page) - pos0, 0), hi_row = min(len - pos0, HALF);
                 if (lo_row > 0 || hi_row < HALF) {
                     for (int x = lane; x < HALF * D / 16; x += 32) {
                         const int row = x / (D / 16);
-                        if ((row < lo_row && (!REACH || row >= early)) || row >= hi_row) reinterpret_cast<uint4 *>(vt)[x] = make_uint4(0, 0, 0, 0);
+                        const bool unseen = row < lo_row && (!REACH || (pos0 + row) >> log_page << log_page >= a.reach.first);
+                        if (unseen || row >= hi_row) reinterpret_cast<uint4 *>(vt)[x] = make_uint4(0, 0, 0, 0);
                     }
                     sm100::fence_proxy_async_smem();  // these before the next copy
                     __syncwarp();
@@ -1059,7 +1019,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                         for (int e = 0; e < 4; e++) {
                             const int pos = pos0 + 16 * (m0 + mt) + (e < 2 ? k0 : 8 + k1), p = q_pos[e & 1];
                             bool seen = pos <= p && (a.window == 0 || p - pos < a.window);
-                            if constexpr (REACH) seen = (seen && pos >= low) || (pos <= p && pos < a.reach.first);
+                            if constexpr (REACH) seen |= pos <= p && pos < a.reach.first;
                             if (!seen) sc[e] = -INFINITY;
                         }
                     }
@@ -1307,7 +1267,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
         if (i + n == count && !(was.at.tile == 0 && n == was.at.w.tiles)) {
             if (!sm100::mbar_wait(&sh.shared_go[1], 0, &sh.abort, a.err)) return;
             if (sh.joins[1])
-                pa_join_blocks<D, F32, REACH>(a, pa_unit(a, was.at, was.begin + i, n, was.per), PA_EPILOGUES + warp,
+                pa_join_blocks<D, F32>(a, pa_unit(a, was.at, was.begin + i, n, was.per), PA_EPILOGUES + warp,
                                               PA_EPILOGUES + PA_CONSUMERS);
         }
         i += n;
@@ -1389,10 +1349,8 @@ cudaError_t launch_attention(const fo_paged_attention_launch &args, int sms, cud
     a.group = a.q.heads / a.kv.n_kv_heads;
     // A warp takes the queries of one n8 tile; beyond that 2, 3 or 6 warps share
     // each half of a tile; beyond that a (sequence, KV head) is read once for
-    // each group of queries.  (A group of sequences may have all rows of the call.)
-    const bool over_groups = REACH && a.reach.over_groups;
-    const int64_t seqs = over_groups ? a.reach.n_groups + 2 : a.batch.n_seqs;
-    const int64_t queries = (over_groups ? a.batch.total_rows : a.batch.max_rows) * a.group;
+    // each group of queries.
+    const int64_t queries = a.batch.max_rows * a.group;
     a.col_groups = queries <= 8 ? 1 : queries <= 16 ? 2 : queries <= 24 ? 3 : 6;
     a.queries = 8 * a.col_groups;
     a.evict_first = queries <= a.queries;
@@ -1404,10 +1362,10 @@ cudaError_t launch_attention(const fo_paged_attention_launch &args, int sms, cud
     a.out_vec = aligned(a.out, a.q.dtype == FO_DT_F32 ? 16 : 8);
     // No more blocks than the most tiles there can be for, one for each group
     // of consumer warps.
-    const int64_t units = seqs * a.kv.n_kv_heads * ((queries + a.queries - 1) / a.queries);
+    const int64_t units = a.batch.n_seqs * a.kv.n_kv_heads * ((queries + a.queries - 1) / a.queries);
     const int64_t most = units * ((a.batch.table_stride * a.kv.page_size * a.kv.head_dim + 8191) / 8192 + REACH);
     const int64_t groups = PA_CONSUMERS / 2 / a.col_groups;
-    a.whole_units = units <= sms && seqs <= PA_THREADS;
+    a.whole_units = units <= sms && a.batch.n_seqs <= PA_THREADS;
     int64_t blocks = std::min<int64_t>(sms, (most + groups - 1) / groups);
     if (a.whole_units) blocks = std::max(blocks, units);
     const unsigned grid = (unsigned)std::max<int64_t>(1, blocks);

@@ -10,6 +10,8 @@
 // position is known.  Measured: 32,771 rows x 40 heads x 128 BF16 119 us (5.8
 // TB/s, 0.90 of the measured copy bandwidth), 6,544 rows x 24 x 64 FP32 16.6 us
 // (4.9 TB/s; a launch that does next to nothing takes 2.4 us), 8 rows 2.4 us.
+// By positions on several axes (a variant): 32,771 x 40 x 128 BF16 on three axes 114 us
+// in a CUDA graph (6.0 TB/s, 0.92), 8 rows 3.0.
 #include "paged_rope.cuh"
 
 namespace fo {

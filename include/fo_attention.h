@@ -629,9 +629,11 @@ int fo_paged_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch 
  * sight behind it, for any number of rows (a decode step's, or a whole
  * prompt's): the row at position p sees the positions j <= p with j < first or
  * p - j < window (window 0: all of them).  Pages that no row sees are not read.
- * Rows that see nothing, and rows that are not finite, as there.
+ * Rows that see nothing, and rows that are not finite, as there; a page number
+ * outside the pool and a scale that is not finite give NaN.
  *
- * Few query rows of a KV head (up to FO_PAGED_FEW) are computed as
+ * Few query rows of a KV head (a sequence's rows times the query heads of one:
+ * up to 48 with a head_dim of 64, up to 24 with 128) are computed as
  * fo_paged_attention's; more as FP16 products with FP32 sums: codes are exact, a
  * query element is held to 2^-11 (FP32 rows: 2^-22) of itself, which BF16 rows'
  * are exactly, or to 2^-39 of the largest of its row and head; a probability to
@@ -641,7 +643,6 @@ int fo_paged_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch 
  * A sequence's rows times the query heads of a KV head are at most 2^31 - 1,
  * and so are the tiles of 8 KB of keys that the page tables have room for, of
  * all KV heads and for every 48 query rows of one (FO_ERR_CAPACITY). */
-#define FO_PAGED_FEW 16
 int fo_paged_window_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch *batch, const fo_rows *q,
                               const float *sinks, float scale, int64_t window, int64_t first, const fo_rows *out,
                               float *lse);
@@ -660,8 +661,8 @@ typedef struct {
 
 /* Attention of rows whose sequences share their beginnings, which are read once
  * for all rows of a group: the row at position p sees positions 0 .. p, as in
- * fo_paged_attention without a window.  Rounding and limits as in
- * fo_paged_window_attention.  Where a KV head has fewer than 64 query rows of a
+ * fo_paged_attention without a window.  Limits as in fo_paged_window_attention,
+ * rounding as of many query rows there.  Where a KV head has fewer than 64 query rows of a
  * sequence, unfinished rows wait in the context's scratch, total_rows *
  * n_heads * (head_dim + 4) floats: a call that needs more of it than any before
  * makes it, which a graph's capture refuses (what graphs use is kept). */

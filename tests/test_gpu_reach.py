@@ -122,6 +122,22 @@ def test_prompt_windows(window, first, dim):
     window_case(4, "e4m3", dim, 128, 1, 4, "f32", [333], [60], window=window, first=first)
 
 
+@pytest.mark.parametrize("dim,group,rows", [(64, 8, 3), (64, 5, 8), (64, 8, 6), (64, 7, 7), (128, 6, 4), (128, 5, 5)])
+@pytest.mark.parametrize("fmt,dtype", [("i8", "bf16"), ("e4m3", "f32")])
+def test_rows_on_both_sides_of_the_kernels_limits(dim, group, rows, fmt, dtype):
+    """24, 40, 48 and 49 query rows of a KV head; 24 and 25."""
+    lens = [1, rows, rows + 1, 130, 257, 700]
+    window_case(18, fmt, dim, 32, 2, group, dtype, lens, [min(n, rows) for n in lens], window=90, first=17, ragged=True)
+
+
+@pytest.mark.parametrize("rows", [1, 60])
+@pytest.mark.parametrize("first", [1000, 2 ** 31 - 1, 2 ** 40])
+def test_more_first_positions_than_there_are(rows, first):
+    """Nothing wraps, and what lies before the window stays in sight."""
+    for fmt, dim, page in (("e4m3", 64, 128), ("e4m3", 128, 16), ("i8", 64, 64)):
+        window_case(19, fmt, dim, page, 2, 2, "bf16", [100, 400, 999], [rows] * 3, window=50, first=first)
+
+
 @pytest.mark.parametrize("window,first", [(1, 0), (1, 1), (2, 130), (64, 4), (100, 16), (200, 65), (5000, 7), (0, 9)])
 @pytest.mark.parametrize("fmt", ["i8", "e4m3"])
 @pytest.mark.parametrize("page", [16, 64, 128])
@@ -273,6 +289,39 @@ def test_bad_tables_are_reported():
         assert np.isfinite(got[:rows]).all()
         for r in range(rows):  # NaN where the page is in sight, and only there
             assert np.isnan(got[rows + r]).all() == (60 - rows + r >= 32)
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("what", ["number", "k", "v"])
+@pytest.mark.parametrize("rows", [24, 40, 60])
+def test_a_bad_page_is_lost_to_the_rows_that_see_it_alone(fmt, what, rows):
+    """A page number outside the pool, a key's scale of NaN, a value's that is infinite: the rows before that page, and those
+    whose window is behind it, come out as without it."""
+    for n, window, first in ((70, 1000, 1), (120, 30, 5)):
+        rng = np.random.default_rng(25)
+        cache = Cache(rng, fmt, 64, 16, 1, [n])
+        values, page = [cache.values(i, 0) for i in range(2)], 3
+        at = int(cache.table[0, page])
+        kv = cache.on_device()
+        if what == "number":
+            cache.table[0, page] = 1 << 30
+        else:
+            cache.dev[2 if what == "k" else 3][at] = math.nan if what == "k" else math.inf
+        q, _ = rows_of(rng, rows, 2, 64, "bf16")
+        out, lse = torch.empty_like(q), torch.empty(rows, 2, device="cuda")
+        ctx = F.Context(0)
+        F.paged_window_attention(kv, cache.batch([rows], False), q, out, window=window, first=first, lse=lse, ctx=ctx)
+        if what == "number" and n == 70:
+            with pytest.raises(F.FoError, match="page table"):
+                ctx.synchronize()
+        torch.cuda.synchronize()
+        ctx.close()
+        place = np.arange(n - rows, n)
+        sees = (place >= 48) & (place - 63 < window)
+        assert sees.any() or n > 70
+        assert not np.isfinite(out.float().cpu().numpy()[sees]).any()
+        check_rows(out, lse, q.double().cpu().numpy(), [rows], [n], lambda b: values, lambda p: seen_of(p, window, first), None,
+                   0.125, "bf16", only={(0, int(r)) for r in np.nonzero(~sees)[0]})
 
 
 # -------------------------------------------------------------- shared beginnings
