@@ -26,11 +26,12 @@
 //                tiles in this block) to the other warps;
 //   warps 8-11   codes to FP16, into swizzled operand tiles (two of keys, two of
 //                values);
-//   warps 14-15  a segment's query rows to FP16 operands, and what each row sees;
-//   warp 13      issues S_t = Q_t K^T and O_t += P_t V, whichever is ready;
-//   warps 0-7    two softmax warpgroups, a thread to a query row: S from tensor
-//                memory, scales, mask, exponentials, P back to tensor memory, and
-//                at the end of a segment O.
+//   warps 13-14  an issuer for each stream, S_t = Q_t K^T and O_t += P_t V;
+//   warp 15      keeps the bound of all other warps' waits;
+//   warps 0-7    two softmax warpgroups, a thread to a query row: a segment's query
+//                rows to FP16 operands, S from tensor memory, scales, mask,
+//                exponentials, P back to tensor memory, and at the end of a
+//                segment O.
 // The two warpgroups are two streams: of a unit of more than 128 query rows each
 // takes 128 of them over all tiles; of a smaller one, both take the same rows over
 // every other tile, and join at the end, so a few rows still keep two tiles in
@@ -39,6 +40,18 @@
 // 256 + 64 t, P_t at 384 + 64 t; else P_t in S_t's place and O_t at 256 + 128 t.
 // Every wait is bounded; on a timeout the block unwinds, waits for its own copies
 // and MMAs, frees tensor memory and reports through the error word.
+//
+// Measured (CUDA graph): a prompt of 6,544 rows in windows of 1,024 with 64 first
+// positions, 2 query heads to each of 8 KV heads of 64, int8: 105 us, 0.16 of the
+// measured FP16 peak; 16 ragged prompts of up to 4,096 rows, 4 query heads to each of
+// 8 of 128, windows of 2,048 with 128, e4m3: 2,345 us, 0.36; 48 questions of up to 96
+// rows to 4 documents of up to 9,001, the same heads: 653 us, 0.26.  Of the
+// prompt, profiled: 48.1 M warp instructions, 1.8 a cycle and SM, 92 % of the
+// instructions found in the instruction cache.  With heads of 128 a pair of tiles
+// takes 6,000 cycles, of which the products are 2,050: a stream waits 1,850 for its S,
+// finds maxima in 1,100 and takes exponentials for 2,300, and as P lies in S's place
+// the next S cannot be there before P V is done.  Heads of 64 have columns for both.
+// Beginning with a unit takes 9,000 to 17,000 cycles.
 #include "paged_reach.cuh"
 #include "sm100.cuh"
 
@@ -69,7 +82,7 @@ constexpr int PT_START = 2;
 // FP32 rows: tiles after which O is taken out of tensor memory and added to by ordinary
 // FP32.  The tensor core's sums are truncated: a tile's sixteen additions leave 1e-7
 // less of what is there (40 sequences over 16,384 positions came out 1.4e-5 too
-// small; MEASURED so), which BF16 rows, at half of that and 2^-9 of rounding, do not
+// small; 1.0e-6 so), which BF16 rows, at half of that and 2^-9 of rounding, do not
 // notice below millions of positions.
 constexpr int PT_KEEP = 4;
 
@@ -175,14 +188,34 @@ __device__ __forceinline__ PtItem pt_item(const fo_paged_tiles_launch &a, int in
         x.units = (int)(((unsigned)(g.n * a.group) + QUERIES - 1) / QUERIES) * a.kv.n_kv_heads;
         return x;
     }
-    x.seq = index / a.q_units;
+    int unit;  // of the sequence's
+    if (a.q_units) {
+        x.seq = index / a.q_units;
+        unit = index - x.seq * a.q_units;
+    } else {
+        // The last sequence that begins at or before the number.
+        auto begins = [&](int seq) { return (int)((long long)a.batch.row_start[seq] * a.group / QUERIES) + seq; };
+        int lo = 0, hi = (int)a.batch.n_seqs - 1;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) >> 1;
+            if (begins(mid) <= index) lo = mid;
+            else hi = mid - 1;
+        }
+        x.seq = lo;
+        unit = index - begins(lo);
+    }
     const Sequence s = load_sequence(a.batch, a.kv.page_size, x.seq, a.err);
-    x.q0 = (index - x.seq * a.q_units) * QUERIES;
     x.first = s.first;
     x.n = s.n;
     x.p0 = s.len - s.n;
+    if (unit < 0 || (long long)unit * QUERIES >= (long long)s.n * a.group) {
+        x.end = x.units = 0;
+        x.tiles = 1;
+        return x;
+    }
+    x.q0 = unit * QUERIES;
     const int queries = s.n * a.group - x.q0;
-    x.units = queries > 0 ? a.kv.n_kv_heads : 0;
+    x.units = a.kv.n_kv_heads;
     const int last = (x.q0 + min(queries, QUERIES) - 1) / a.group;
     const int from = max(x.p0 + x.q0 / a.group, 0);
     x.end = min(max(x.p0 + last + 1, 0), s.len);
@@ -305,7 +338,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
 
     // This block's piece [begin, end) of the line, and where it begins.  (The
     // line is shorter than 2^31, checked on the host.)
-    const int n_items = a.reach.over_groups ? a.reach.n_groups + 2 : (int)a.batch.n_seqs * a.q_units;
+    const int n_items = a.reach.over_groups ? a.reach.n_groups + 2
+                        : a.q_units         ? (int)a.batch.n_seqs * a.q_units
+                                            : (int)(a.batch.total_rows * a.group / QUERIES + a.batch.n_seqs);
     int per = 0, begin = 0, end = 0;
     // The line's length first, then the item that the piece begins in; with no more items than
     // threads at one go.
@@ -317,6 +352,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
             int2 mine = make_int2(0, 0), chunk;
             PtItem x;
             if (first + tid < n_items) {
+                // (Not every sequence whose rows are wrong is found by number.)
+                if (!a.q_units && first + tid < (int)a.batch.n_seqs)
+                    load_sequence(a.batch, a.kv.page_size, first + tid, a.err);
                 x = pt_item<QUERIES>(a, first + tid);
                 mine = make_int2((x.tiles + PT_START) * x.units, x.tiles * x.units);
             }
@@ -622,7 +660,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 };
                 // S is read twice, in short loops: what is run over and over has to stay in the instruction
                 // cache (with the row in registers and all of it in line: 123 us for a page's prompt where
-                // this takes MEASURED, 2,621 for ragged prompts with heads of 128 against MEASURED).
+                // this takes 110, 2,621 for ragged prompts with heads of 128 against 2,375).
                 uint32_t raw[64];
                 FO_TMEM_LD32(s_at, raw);
 #pragma unroll 1
@@ -1391,11 +1429,19 @@ cudaError_t launch_tiles(const fo_paged_tiles_launch &in, int sms, cudaStream_t 
     }
     // No more blocks than the most tiles there can be for, two to a block.
     const int64_t table = (a.batch.table_stride * a.kv.page_size + PT_TILE - 1) / PT_TILE;
+    a.q_units = (int)((a.batch.max_rows * a.group + Shape::QUERIES - 1) / Shape::QUERIES);
+    // Ragged sequences of up to so many units: as many numbers for each, those behind a
+    // sequence's rows for nothing.  Of more, a number is the rows before the sequence in
+    // units, and the sequences before it: floor(first / Q) + b + floor(n / Q) + 1 is at most
+    // the next one's floor((first + n) / Q) + b + 1, so they are in order, and there is
+    // hardly one that is nothing's; finding the sequence takes a search.
+    constexpr int MOST_UNITS = 4;
+    if (a.batch.row_start && !a.reach.over_groups && a.q_units > MOST_UNITS) a.q_units = 0;
     const int64_t units = a.reach.over_groups
                               ? (a.batch.total_rows * a.group + Shape::QUERIES - 1) / Shape::QUERIES + a.reach.n_groups + 2
-                              : a.batch.n_seqs * ((a.batch.max_rows * a.group + Shape::QUERIES - 1) / Shape::QUERIES);
+                          : a.q_units ? a.batch.n_seqs * a.q_units
+                                      : a.batch.total_rows * a.group / Shape::QUERIES + a.batch.n_seqs;
     const int64_t most = units * a.kv.n_kv_heads * table;
-    a.q_units = (int)((a.batch.max_rows * a.group + Shape::QUERIES - 1) / Shape::QUERIES);
     const unsigned grid = (unsigned)std::max<int64_t>(1, std::min<int64_t>(sms, (most + 1) / 2));
     cudaError_t e = launch(kernel, dim3(grid), dim3(PT_THREADS), Shape::SMEM, stream, a);
     if (e != cudaSuccess || grid == 1 || a.reach.parts_of) return e;

@@ -122,6 +122,35 @@ def test_prompt_windows(window, first, dim):
     window_case(4, "e4m3", dim, 128, 1, 4, "f32", [333], [60], window=window, first=first)
 
 
+@pytest.mark.parametrize("dim,dtype", [(64, "bf16"), (64, "f32"), (128, "bf16"), (128, "f32")])
+def test_long_prompts_beside_short_ones(dim, dtype):
+    """Sequences of more units than four, of few, of one row and of none in one batch; more units than threads."""
+    lens = [1300, 5, 0, 1900, 700, 1, 0, 300, 2600, 9]
+    rows = [1300, 1, 0, 1400, 700, 1, 0, 1, 1301, 9]
+    rng = np.random.default_rng(26)
+    some = {(b, int(r)) for b, n in enumerate(rows) if n for r in {0, n - 1, *rng.integers(0, n, 12), *range(127, n, 384)}}
+    window_case(26, "i8", dim, 64, 1, 2, dtype, lens, rows, window=200, first=70, ragged=True, only=some)
+    many = [3] * 500 + [1200] + [2] * 40
+    some = {(b, r) for b in (0, 1, 250, 499, 501, 540) for r in (0, 1)} | {(500, r) for r in (0, 600, 1199)}
+    window_case(27, "e4m3", dim, 16, 1, 1, dtype, many, many, window=30, first=2, ragged=True, only=some)
+
+
+def test_rows_out_of_order_are_reported():
+    """Of long prompts: the sequence whose rows end before they begin, and nothing else, is left out."""
+    rng = np.random.default_rng(28)
+    cache = Cache(rng, "i8", 64, 16, 1, [2000, 50, 110])
+    start = dev(np.array([0, 2000, 1990, 2100], np.int32))
+    batch = F.PagedBatch(dev(cache.table), dev(np.array(cache.lens, np.int32)), rows=2000, row_start=start)
+    q, _ = rows_of(rng, 2100, 1, 64, "bf16")
+    out = torch.empty_like(q)
+    ctx = F.Context(0)
+    F.paged_window_attention(cache.on_device(), batch, q, out, window=100, first=1, ctx=ctx)
+    with pytest.raises(F.FoError, match="page table"):
+        ctx.synchronize()
+    ctx.synchronize()
+    ctx.close()
+
+
 @pytest.mark.parametrize("dim,group,rows", [(64, 8, 3), (64, 5, 8), (64, 8, 6), (64, 7, 7), (128, 6, 4), (128, 5, 5)])
 @pytest.mark.parametrize("fmt,dtype", [("i8", "bf16"), ("e4m3", "f32")])
 def test_rows_on_both_sides_of_the_kernels_limits(dim, group, rows, fmt, dtype):
