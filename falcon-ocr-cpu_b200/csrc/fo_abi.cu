@@ -2027,7 +2027,7 @@ int launch_reach(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch *batch
         a.part_ml = ctx->paged_part_ml();
         a.counters = ctx->paged_counters();
         a.reach = reach;
-        const bool plain = reach.n_groups == 0 && (reach.first == 0 || window == 0);
+        const bool plain = reach.few == 0 && (reach.first == 0 || window == 0);
         e = plain ? fo_launch_paged_attention(&a, ctx->sms, ctx->stream)
                   : fo_launch_paged_attention_reach(&a, ctx->sms, ctx->stream);
     } else {
@@ -2049,6 +2049,30 @@ int launch_reach(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch *batch
         e = fo_launch_paged_tiles(&a, ctx->sms, ctx->stream);
     }
     return e == cudaSuccess ? FO_OK : cuda_fail(e, "paged attention launch");
+}
+
+// Sequences by themselves.  A ragged batch that can hold eight and more sequences of
+// a decode step's query rows beside longer ones takes both kernels, since those rows
+// are a tile of 128 in paged_tiles.cu: 256 sequences of one row (2 query rows of each of 8
+// KV heads of 64) beside a prompt of 4,096, windows of 1,024, 182 us against 526, 63 beside
+// 2,048 79 against 153; a batch that turns out to have none pays for a launch (16
+// sequences of up to 1,024 rows 167 us against 163).
+int launch_alone(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch *batch, const fo_rows *q, const fo_rows *out,
+                 const float *sinks, float *lse, float scale, int32_t window, fo_paged_reach reach) {
+    const int64_t group = q->heads / kv->n_kv_heads, queries = batch->max_rows * group;
+    const bool all_few = queries <= alone_few(kv->head_dim);
+    if (!all_few && batch->row_start && group <= 16) {
+        // As many as can be of few rows where the others have max_rows.
+        const int64_t few = group <= 8 ? 8 : 16, rows = few / group;
+        if (batch->n_seqs * batch->max_rows - batch->total_rows >= 8 * (batch->max_rows - rows)) {
+            reach.few = (int32_t)few;
+            // Before anything is launched, or captured.
+            FO_TRY(make_paged_parts(ctx));
+            FO_TRY(make_tile_parts(ctx));
+            FO_TRY(launch_reach(ctx, kv, batch, q, out, sinks, lse, scale, window, reach, true));
+        }
+    }
+    return launch_reach(ctx, kv, batch, q, out, sinks, lse, scale, window, reach, all_few);
 }
 
 }  // namespace
@@ -2153,8 +2177,7 @@ int fo_paged_window_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged
     DeviceGuard guard(ctx->device);
     fo_paged_reach reach = {};
     reach.first = (int32_t)std::min<int64_t>(first, INT32_MAX);
-    return launch_reach(ctx, kv, batch, q, out, sinks, lse, scale, window < INT32_MAX ? (int32_t)window : 0, reach,
-                        batch->max_rows * group <= alone_few(kv->head_dim));
+    return launch_alone(ctx, kv, batch, q, out, sinks, lse, scale, window < INT32_MAX ? (int32_t)window : 0, reach);
 }
 
 int fo_paged_prefix_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch *batch,
@@ -2177,11 +2200,12 @@ int fo_paged_prefix_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged
     reach.group_start = groups->seq_start;
     reach.group_lens = groups->lens;
     reach.n_groups = (int32_t)groups->n_groups;
-    if (reach.n_groups == 0)
-        return launch_reach(ctx, kv, batch, q, out, sinks, lse, scale, 0, reach, queries <= alone_few(kv->head_dim));
-    // Half a tile of query rows and more: the products bound the call, however
-    // often the beginning is read, so each sequence goes over all it sees.
-    if (queries >= FO_PAGED_ALONE) return launch_reach(ctx, kv, batch, q, out, sinks, lse, scale, 0, reach, false);
+    if (reach.n_groups == 0) return launch_alone(ctx, kv, batch, q, out, sinks, lse, scale, 0, reach);
+    // Half a tile of query rows and more a sequence: the products bound the call, however
+    // often the beginning is read, so each sequence goes over all it sees.  (Where
+    // they are few on average, a sequence of few among them would take a tile of its
+    // own over all of the beginning.)
+    if (rows * group >= FO_PAGED_ALONE * batch->n_seqs) return launch_reach(ctx, kv, batch, q, out, sinks, lse, scale, 0, reach, false);
     float *o = nullptr, *ml = nullptr;
     int32_t *parts_of = nullptr;
     FO_TRY(make_waiting(ctx, rows * q->heads, kv->head_dim, &o, &ml, &parts_of));

@@ -243,6 +243,9 @@ cudaError_t fo_launch_paged_append_axes(const fo_append_launch *args, cudaStream
 // where unfinished rows come from and go to (paged_reach.cuh).
 struct fo_paged_reach {
     int32_t first;  // leading positions that stay in sight behind a window
+    // Above 0: sequences of up to so many query rows of a KV head are
+    // paged_attention.cuh's, others paged_tiles.cu's, and each leaves out the other's.
+    int32_t few;
     // Groups of sequences: the positions before a group's length are in the pages
     // of its first sequence.
     const int32_t *group_start, *group_lens;

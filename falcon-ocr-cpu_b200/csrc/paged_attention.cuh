@@ -210,6 +210,10 @@ __device__ __forceinline__ PaWork pa_work(const fo_paged_attention_launch &a, in
     if constexpr (REACH) w.tiles += pa_early<TILE>(a, w);
     w.tiles = max(w.tiles, 1);
     const int queries = w.s.n * a.group;
+    if (REACH && a.reach.few > 0 && queries > a.reach.few) {
+        w.groups = 0;
+        return w;
+    }
     w.groups = queries <= a.queries ? queries > 0 : (queries + FO_PAGED_QUERIES - 1) / FO_PAGED_QUERIES;
     return w;
 }
@@ -1350,7 +1354,8 @@ cudaError_t launch_attention(const fo_paged_attention_launch &args, int sms, cud
     // A warp takes the queries of one n8 tile; beyond that 2, 3 or 6 warps share
     // each half of a tile; beyond that a (sequence, KV head) is read once for
     // each group of queries.
-    const int64_t queries = a.batch.max_rows * a.group;
+    int64_t queries = a.batch.max_rows * a.group;
+    if (REACH && a.reach.few > 0) queries = std::min<int64_t>(queries, a.reach.few);
     a.col_groups = queries <= 8 ? 1 : queries <= 16 ? 2 : queries <= 24 ? 3 : 6;
     a.queries = 8 * a.col_groups;
     a.evict_first = queries <= a.queries;

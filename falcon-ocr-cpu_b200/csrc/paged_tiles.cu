@@ -208,7 +208,7 @@ __device__ __forceinline__ PtItem pt_item(const fo_paged_tiles_launch &a, int in
     x.first = s.first;
     x.n = s.n;
     x.p0 = s.len - s.n;
-    if (unit < 0 || (long long)unit * QUERIES >= (long long)s.n * a.group) {
+    if (unit < 0 || (long long)unit * QUERIES >= (long long)s.n * a.group || s.n * a.group <= a.reach.few) {
         x.end = x.units = 0;
         x.tiles = 1;
         return x;

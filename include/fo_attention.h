@@ -633,8 +633,9 @@ int fo_paged_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch 
  * outside the pool and a scale that is not finite give NaN.
  *
  * Few query rows of a KV head (a sequence's rows times the query heads of one:
- * up to 48 with a head_dim of 64, up to 24 with 128) are computed as
- * fo_paged_attention's; more as FP16 products with FP32 sums: codes are exact, a
+ * up to 48 with a head_dim of 64, up to 24 with 128; beside longer sequences up
+ * to 8, or 16 where a KV head has more than 8 query heads, and only if the batch
+ * can hold eight such) are computed as fo_paged_attention's; more as FP16 products with FP32 sums: codes are exact, a
  * query element is held to 2^-11 (FP32 rows: 2^-22) of itself, which BF16 rows'
  * are exactly, or to 2^-39 of the largest of its row and head; a probability to
  * 2^-11 (2^-22) of itself, or to 2^-35 of its row's largest.  The sum of
@@ -663,7 +664,7 @@ typedef struct {
  * for all rows of a group: the row at position p sees positions 0 .. p, as in
  * fo_paged_attention without a window.  Limits as in fo_paged_window_attention,
  * rounding as of many query rows there.  Where a KV head has fewer than 64 query rows of a
- * sequence, unfinished rows wait in the context's scratch, total_rows *
+ * sequence on average, unfinished rows wait in the context's scratch, total_rows *
  * n_heads * (head_dim + 4) floats: a call that needs more of it than any before
  * makes it, which a graph's capture refuses (what graphs use is kept). */
 int fo_paged_prefix_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch *batch,

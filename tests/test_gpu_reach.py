@@ -135,6 +135,27 @@ def test_long_prompts_beside_short_ones(dim, dtype):
     window_case(27, "e4m3", dim, 16, 1, 1, dtype, many, many, window=30, first=2, ragged=True, only=some)
 
 
+@pytest.mark.parametrize("group", [1, 2, 8, 16])
+@pytest.mark.parametrize("fmt,dim,dtype", [("i8", 64, "bf16"), ("e4m3", 128, "f32"), ("e4m3", 64, "bf16"), ("i8", 128, "bf16")])
+@pytest.mark.parametrize("window,first", [(90, 17), (0, 0), (60, 0), (1, 1)])
+def test_a_decode_step_beside_prompts(group, fmt, dim, dtype, window, first):
+    """Sequences of few rows go to one kernel and the others to the other: every row is written by one of them."""
+    rows = [1, 1, 200, 1, 0, 1, 4, 1, 5, 8, 9, 1, 130, 1, 1, 2, 1, 0]
+    lens = [1, 700, 200, 40, 0, 130, 90, 300, 3, 8, 500, 17, 333, 64, 65, 1, 999, 5]
+    some = {(b, r) for b, n in enumerate(rows) for r in range(n) if r < 9 or r % 31 == 0 or r == n - 1}
+    window_case(29, fmt, dim, 32, 1, group, dtype, lens, rows, window=window, first=first, ragged=True, only=some)
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, "bf16"), (128, "bf16"), (64, "f32"), (128, "f32")])
+@pytest.mark.parametrize("long", [40, 700])
+def test_shared_beginnings_of_a_decode_step_beside_prompts(dim, dtype, long):
+    """Few rows on average and many at most: long prompts of several units beside single rows, in and out of groups."""
+    rows = [1] * 14 + [long, 1, 0, 5] + [1] * 30 + [long // 2]
+    own = [40 + 13 * (b % 5) + n for b, n in enumerate(rows)]
+    some = {(b, r) for b, n in enumerate(rows) for r in range(n) if r < 2 or r % 97 == 0 or r == n - 1}
+    prefix_case(30, "i8", dim, 32, 1, 2, dtype, [2, 12, 30, 30, 44], [333, 200, 0, 64], own, rows, ragged=True, only=some)
+
+
 def test_rows_out_of_order_are_reported():
     """Of long prompts: the sequence whose rows end before they begin, and nothing else, is left out."""
     rng = np.random.default_rng(28)
