@@ -2211,7 +2211,15 @@ int fo_paged_prefix_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged
     FO_TRY(make_waiting(ctx, rows * q->heads, kv->head_dim, &o, &ml, &parts_of));
     // Of the average group, few query rows; and few groups, since any of them may have all rows.
     const bool few = rows * group <= FO_PAGED_FEW * groups->n_groups && groups->n_groups <= 16;
-    if (queries <= FO_PAGED_FEW) {
+    FO_TRY(make_paged_parts(ctx));
+    // More rows than one of paged_few.cu's units holds: still by that kernel, two launches in
+    // place of four, where its units are few and no sequence's own positions can be many.
+    // 4 sequences of 40 query rows with some 100 of their own, 31 us against 45; 8 of 20 with
+    // 500, 36 and 51; heads of 128 42 and 59, 52 and 66.  But 12 of 40 with 3,000 72 and 76,
+    // heads of 128 (not taken) 159 and 103; 8 of 40 with 5,000 (not taken) 94 and 73.
+    const int64_t units = batch->n_seqs * kv->n_kv_heads * ((queries + FO_PAGED_FEW - 1) / FO_PAGED_FEW);
+    const bool small = units * kv->head_dim <= 128 * ctx->sms && batch->table_stride * kv->page_size <= 8192;
+    if (queries <= FO_PAGED_FEW || small) {
         // The shared positions, then each sequence's own.
         fo_paged_few_launch a = {};
         a.kv = *kv;
@@ -2225,7 +2233,6 @@ int fo_paged_prefix_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged
         shared.raw_o = o;
         shared.raw_ml = ml;
         if (few) {
-            FO_TRY(make_paged_parts(ctx));
             a.reach = shared;
             cudaError_t e = fo_launch_paged_few(&a, ctx->sms, ctx->stream);
             if (e != cudaSuccess) return cuda_fail(e, "paged attention launch");

@@ -290,8 +290,8 @@ cudaError_t fo_launch_paged_attention_reach(const fo_paged_attention_launch *arg
 // Attention of many query rows over the paged cache on the 5th-generation
 // tensor cores (paged_tiles.cu).
 #define FO_TILES_QUERIES 256  // query rows of a block's unit at most
-#define FO_PAGED_FEW 16       // query rows of a sequence up to which shared beginnings go by paged_few.cu
-#define FO_PAGED_ALONE 64     // query rows of a sequence from which on it reads a shared beginning by itself
+#define FO_PAGED_FEW 16       // query rows of a unit of paged_few.cu
+#define FO_PAGED_ALONE 64     // query rows of a sequence, on average, from which on each reads a shared beginning by itself
 struct fo_paged_tiles_launch {
     fo_paged_kv kv;
     fo_paged_batch batch;

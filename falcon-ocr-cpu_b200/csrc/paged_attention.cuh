@@ -72,7 +72,7 @@
 // With REACH (paged_attention_reach.cu; the variants without it are unchanged
 // by it) a row also sees a few first positions behind its window, whose tiles
 // come before the window's in the line.  64 sequences in a window of 4,096 with
-// 16 first positions, 2 query rows to each of 8 KV heads of 64: 58 us against a
+// 16 first positions, 2 query rows to each of 8 KV heads of 64: 60 us against a
 // floor of 41; a unit's change costs some 3 us and a unit here is short.
 #pragma once
 

@@ -156,6 +156,17 @@ def test_shared_beginnings_of_a_decode_step_beside_prompts(dim, dtype, long):
     prefix_case(30, "i8", dim, 32, 1, 2, dtype, [2, 12, 30, 30, 44], [333, 200, 0, 64], own, rows, ragged=True, only=some)
 
 
+@pytest.mark.parametrize("dim,dtype", [(64, "bf16"), (128, "bf16"), (64, "f32"), (128, "f32")])
+@pytest.mark.parametrize("ragged", [False, True])
+def test_shared_beginnings_of_many_sequences_with_several_rows(dim, dtype, ragged):
+    """20 query rows of a sequence: more sequences than one kernel takes, and as many as it does."""
+    for fmt, seqs in (("i8", 110), ("e4m3", 7)):
+        rows = [5 - b % 3 * ragged for b in range(seqs)]
+        own = [n + 11 * b % 70 for b, n in enumerate(rows)]
+        some = {(b, r) for b in range(0, seqs, 7) for r in range(rows[b])}
+        prefix_case(31, fmt, dim, 16, 2, 4, dtype, [0, 3, seqs - 2], [100, 140], own, rows, ragged=ragged, only=some)
+
+
 def test_rows_out_of_order_are_reported():
     """Of long prompts: the sequence whose rows end before they begin, and nothing else, is left out."""
     rng = np.random.default_rng(28)
