@@ -688,6 +688,45 @@ def test_serving_steps_in_a_graph():
         assert torch.equal(a, b) and a.isfinite().all()
 
 
+def test_two_streams_at_once_and_a_graph_beside():
+    """Each stream's context has scratch of its own: calls side by side, and a replayed graph of both kernels of a ragged
+    batch, give what each gives alone."""
+    rng = np.random.default_rng(62)
+    rows = [1] * 12 + [600] + [1] * 4
+    cache = Cache(rng, "e4m3", 64, 32, 2, [700 + 40 * b for b in range(17)])
+    kv, batch = cache.on_device(), cache.batch(rows, True)
+    step = cache.batch([3] * 17, False)
+    groups = F.PagedGroups(dev(np.array([0, 9, 17], np.int32)), dev(np.array([600, 333], np.int32)))
+    q, _ = rows_of(rng, sum(rows), 4, 64, "bf16")
+    few, _ = rows_of(rng, 51, 4, 64, "bf16")
+    window = lambda out: F.paged_window_attention(kv, batch, q, out, window=300, first=20)  # noqa: E731
+    prefix = lambda out: F.paged_prefix_attention(kv, step, groups, few, out)  # noqa: E731
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    expected = []
+    for call, x in ((window, q), (prefix, few), (window, q)):
+        with torch.cuda.stream(streams[len(expected)]):
+            out = torch.empty_like(x)
+            call(out)
+            expected.append(out)
+    torch.cuda.synchronize()
+    assert torch.equal(expected[0], expected[2])
+    graph, replayed = torch.cuda.CUDAGraph(), torch.empty_like(q)
+    with torch.cuda.graph(graph, stream=streams[2]):
+        window(replayed)
+    outs = [torch.empty_like(q) for _ in range(20)], [torch.empty_like(few) for _ in range(20)]
+    torch.cuda.synchronize()
+    for i in range(20):
+        with torch.cuda.stream(streams[0]):
+            window(outs[0][i])
+        with torch.cuda.stream(streams[1]):
+            prefix(outs[1][i])
+        with torch.cuda.stream(streams[2]):
+            graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, expected[0]) for x in outs[0]) and all(torch.equal(x, expected[1]) for x in outs[1])
+    assert torch.equal(replayed, expected[0])
+
+
 def test_first_calls_inside_a_capture_are_refused():
     rng = np.random.default_rng(61)
     cache = Cache(rng, "i8", 64, 16, 1, [60] * 20)
