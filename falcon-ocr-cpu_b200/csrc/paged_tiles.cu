@@ -46,7 +46,7 @@
 // measured FP16 peak; 16 ragged prompts of up to 4,096 rows, 4 query heads to each of
 // 8 of 128, windows of 2,048 with 128, e4m3: 2,345 us, 0.36; 48 questions of up to 96
 // rows to 4 documents of up to 9,001, the same heads: 653 us, 0.26.  Of the
-// prompt, profiled: 48.1 M warp instructions, 1.8 a cycle and SM, 92 % of the
+// prompt, profiled: 47.1 M warp instructions, 1.8 a cycle and SM, 92 % of the
 // instructions found in the instruction cache.  With heads of 128 a pair of tiles
 // takes 6,000 cycles, of which the products are 2,050: a stream waits 1,850 for its S,
 // finds maxima in 1,100 and takes exponentials for 2,300, and as P lies in S's place

@@ -653,7 +653,9 @@ int fo_paged_window_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged
  * their positions 0 .. lens[g] - 1 are in the pages that the FIRST of them has
  * in the page table; what the others have there is not read, but for the page
  * that position lens[g] falls into, where each has its own from that position
- * on.  Sequences before the first group and behind the last share nothing. */
+ * on.  Sequences before the first group and behind the last share nothing.
+ * Starts that do not ascend within the batch and lengths beyond the page table are
+ * reported by the error word; what the rows of such groups hold is undefined. */
 typedef struct {
     const int32_t *seq_start; /* [n_groups + 1] */
     const int32_t *lens;      /* [n_groups] */
