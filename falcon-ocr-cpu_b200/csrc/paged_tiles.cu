@@ -125,7 +125,7 @@ struct PtSegment {
 struct PtMeta {
     float ks[8], vs[8];  // keys' and values' scales of each 16 positions' page
     int top;             // exponent bits of a power of two above the values' scales
-    int plain;           // the keys' scales are numbers above 0
+    float least;         // the least of the keys' scales, 0: one is not a number above 0
     int base;            // the tile's first position
     int from, to;        // positions [from, to) that rows may see of it
     unsigned pages;      // pages that were copied
@@ -520,6 +520,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                         *place(lane, x + CHUNKS / 2) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                     }
                 }
+                // Zeros, and rows of no query, have scores of 0 at any scale; at this one they go the short way.
+                if (most == 0) q_scale = a.scale * REACH_LOG2E;
                 if (!pair) sh.q_scale[r] = q_scale;
                 fence_proxy_async_smem();
             }
@@ -605,7 +607,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 const int tile = meta.base;
                 int tile_top = meta.top;
                 const int hi = min(high, meta.to - 1), lo = max(low, meta.from);
-                const bool plain = __all_sync(0xffffffffu, meta.plain && q_scale > 0.0f);
+                // The scores' factors will multiply -infinity too, of which a product that underflows to 0
+                // would make NaN.
+                const bool plain = __all_sync(0xffffffffu, meta.least * q_scale >= FLT_MIN);
                 const bool all = hi - tile >= PT_TILE - 1 && (lo <= tile || a.reach.first - tile >= PT_TILE);
                 if (!__all_sync(0xffffffffu, plain && all)) {
                     // Scores of keys that the row does not see become -infinity in tensor memory, 32 keys
@@ -1123,8 +1127,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                     meta.ks[lane] = ks8;
                     meta.vs[lane] = vs8;
                 }
-                const bool plain = __all_sync(0xffffffffu, ks > 0.0f);
-                if (lane == 8) meta.top = pt_above(most), meta.plain = plain;
+                // (Numbers above 0 are in their bits' order.)
+                const float least = __uint_as_float(__reduce_min_sync(0xffffffffu, ks > 0.0f ? __float_as_uint(ks) : 0u));
+                if (lane == 8) meta.top = pt_above(most), meta.least = least;
                 if (lane == 9) meta.base = now.base;
                 if (lane == 10) meta.pages = mask;
                 if (lane == 11) meta.from = now.from, meta.to = now.to;
