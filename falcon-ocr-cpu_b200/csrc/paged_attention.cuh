@@ -838,7 +838,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                     if constexpr (REACH) {
                         // Like values that are not finite, by the scores: rows that do not see the page are
                         // not changed by it.
-                        const bool lost = now.bad || !(fabsf(now.vs) <= FLT_MAX);
+                        const bool lost = now.bad || !(fabsf(now.ks) <= FLT_MAX && fabsf(now.vs) <= FLT_MAX);
                         sh.scales[slot][j] = lost ? NAN : now.ks;
                         sh.scales[slot][8 + j] = lost ? 0.0f : now.vs;
                         if (now.bad) {

@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(PF_THREADS, F32 && NT == 2 ? 1 : 2)
         }
         now.ks = *reinterpret_cast<const float *>(at + 32 * D);
         now.vs = *reinterpret_cast<const float *>(at + 32 * D + 4);
-        if (!(fabsf(now.vs) <= FLT_MAX)) now.ks = NAN, now.vs = 0.0f;
+        if (!(fabsf(now.ks) <= FLT_MAX && fabsf(now.vs) <= FLT_MAX)) now.ks = NAN, now.vs = 0.0f;
         __syncwarp();  // the stage may be written again
         stage = stage == STAGES - 1 ? 0 : stage + 1;
         // Scores in log2 units: keys g and g + 8, columns 2 t and 2 t + 1 of a tile.

@@ -1112,7 +1112,8 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 if (!ok) break;
                 // The tile's scales.  A page number outside the pool, or a scale that is not finite,
                 // gives NaN to the rows that see the page, by their scores.
-                const bool load = now.wanted && !now.bad, sane = load && fabsf(now.vs) <= FLT_MAX;
+                const bool load = now.wanted && !now.bad;
+                const bool sane = load && fabsf(now.ks) <= FLT_MAX && fabsf(now.vs) <= FLT_MAX;
                 if (now.bad) atomicOr(a.err, FO_DEVERR_PAGED);
                 // (That of a page that no row sees is never used.)
                 const float ks = !now.wanted ? 1.0f : !sane ? NAN : now.ks, vs = sane ? now.vs : 0.0f;

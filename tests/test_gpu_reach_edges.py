@@ -12,7 +12,7 @@ torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 from test_gpu_paged import Cache, dev, rows_of  # noqa: E402
-from test_gpu_reach import check_rows, seen_of  # noqa: E402
+from test_gpu_reach import SharedCache, check_rows, seen_of  # noqa: E402
 
 
 def attend_window(cache, rows, q, window, first, scale=None, ctx=None):
@@ -85,3 +85,118 @@ def test_sums_of_long_sequences(fmt, dim, call, rows, positions):
     bound = 2.0 ** -22 + 2.0 ** -21 + 2.0 ** -22 + 6 * steps ** 0.5 * 2.0 ** -24 + (64 * 2.0 ** -23 / 2 if rows > 48 else 0)
     got = out.view(seqs, rows, heads, dim)[:, -1].double()  # the rows that see all
     assert float((got / (total / n) - 1).abs().max()) <= bound
+
+
+# Shared beginnings, by what computes them: the few rows' kernel both times; the many rows' for the beginning and the few
+# rows' for the rest, of single rows and of more; the many rows' both times; each sequence over all it sees.
+FORMS = {"few": (4, 1, 2, False), "many and few": (40, 1, 2, False), "many and few, rows": (4, 20, 1, False),
+         "many": (4, 20, 1, True), "alone": (4, 70, 1, False)}
+
+
+def positive_keys(cache):
+    if cache.fmt == "i8":
+        cache.codes[0] = np.abs(cache.codes[0].view(np.int8)).view(np.uint8)
+    else:
+        cache.codes[0] &= 0x7F
+
+
+class SharedForm:
+    """Sequences of one group over a beginning of 3 1/2 pages, the third shorter than it.  (`below`: all scores below 0.)"""
+
+    def __init__(self, form, seed, fmt, dim, dtype, below=False):
+        self.seqs, self.n, self.group, wide = FORMS[form]
+        rng, page = np.random.default_rng(seed), 128 if wide else 16
+        self.page, self.shared = page, 3 * page + page // 2
+        lens = [self.shared + self.n + 9 * b % 40 for b in range(self.seqs)]
+        lens[2] = page + page // 2 + self.n // 2
+        self.cache = SharedCache(rng, fmt, dim, page, 1, lens, [0, self.seqs], [self.shared])
+        if wide:  # more positions than the few rows' kernel takes with several rows
+            table = np.full((self.seqs, 8192 // page + 1), -7, np.int32)
+            table[:, :self.cache.table.shape[1]] = self.cache.table
+            self.cache.table = table
+        if below:
+            positive_keys(self.cache)
+        self.kv = self.cache.on_device()
+        self.values = [(self.cache.values(0, b), self.cache.values(1, b)) for b in range(self.seqs)]
+        self.q, _ = rows_of(rng, self.seqs * self.n, self.group, dim, dtype)
+        if below:
+            self.q = -self.q.abs()
+        self.places = np.concatenate([np.arange(n - self.n, n) for n in lens])
+        self.dtype, self.scale = dtype, dim ** -0.5
+
+    def attend(self, scale=None, ctx=None):
+        groups = F.PagedGroups(dev(np.array([0, self.seqs], np.int32)), dev(np.array([self.shared], np.int32)))
+        out, lse = torch.full_like(self.q, 9.0), torch.full(self.q.shape[:2], 9.0, device="cuda")
+        F.paged_prefix_attention(self.kv, self.cache.batch([self.n] * self.seqs, False), groups, self.q, out, lse=lse,
+                                 scale=scale, ctx=ctx)
+        return out, lse
+
+    def check(self, out, lse, rows, scale=None):
+        """The rows whose numbers are given against the float64 form."""
+        check_rows(out, lse, self.q.double().cpu().numpy(), [self.n] * self.seqs, self.cache.lens,
+                   lambda b: self.values[b], lambda p: seen_of(p, 0, 0), None, self.scale if scale is None else scale,
+                   self.dtype, only={(int(r) // self.n, int(r) % self.n) for r in rows})
+
+
+WHAT = ["number", "k inf", "k -inf", "k nan", "v inf", "v -inf", "v nan"]
+
+
+def damage(cache, seq, page, what):
+    """A page number outside the pool, or a scale that is not finite (on the device; the cache keeps what was there)."""
+    if what == "number":
+        cache.table[seq, page] = 1 << 30
+    else:
+        cache.dev[2 if what[0] == "k" else 3][int(cache.table[seq, page])] = float(what[2:])
+
+
+@pytest.mark.parametrize("fmt,dim,dtype", [("i8", 64, "bf16"), ("e4m3", 128, "f32")])
+@pytest.mark.parametrize("what", WHAT)
+@pytest.mark.parametrize("rows", [1, 12, 20, 60])
+def test_a_lost_page_in_windows(fmt, dim, dtype, what, rows):
+    """Rows that see the page give NaN, scores below 0 or not, and the others what they give without it."""
+    for n, window, first in ((70, 1000, 1), (120, 30, 50)):
+        rng = np.random.default_rng(4)
+        cache = Cache(rng, fmt, dim, 16, 1, [n])
+        positive_keys(cache)
+        values, kv = [cache.values(i, 0) for i in range(2)], cache.on_device()
+        damage(cache, 0, 3, what)
+        q, _ = rows_of(rng, rows, 2, dim, dtype)
+        q = -q.abs()
+        ctx = F.Context(0)
+        out, lse = torch.full_like(q, 9.0), torch.full((rows, 2), 9.0, device="cuda")
+        F.paged_window_attention(kv, cache.batch([rows], False), q, out, window=window, first=first, lse=lse, ctx=ctx)
+        sees = np.arange(n - rows, n) >= 48  # by the first positions, or a window longer than the sequence
+        if what == "number":
+            with pytest.raises(F.FoError, match="page table"):
+                ctx.synchronize()
+        ctx.synchronize()
+        ctx.close()
+        assert out[torch.from_numpy(sees).cuda()].isnan().all() and lse[torch.from_numpy(sees).cuda()].isnan().all()
+        check_rows(out, lse, q.double().cpu().numpy(), [rows], [n], lambda b: values, lambda p: seen_of(p, window, first),
+                   None, dim ** -0.5, dtype, only={(0, int(r)) for r in np.nonzero(~sees)[0]})
+
+
+@pytest.mark.parametrize("fmt,dim,dtype", [("i8", 64, "bf16"), ("e4m3", 128, "f32")])
+@pytest.mark.parametrize("what", WHAT)
+@pytest.mark.parametrize("form", list(FORMS))
+@pytest.mark.parametrize("where", ["beginning", "behind one", "own"])
+def test_a_lost_page_of_shared_beginnings(form, where, what, fmt, dim, dtype):
+    """Of the beginning: lost to the rows of all sequences that come to it (one ends before its third page).  Of one
+    sequence's own: to its rows alone."""
+    f = SharedForm(form, 5, fmt, dim, dtype, below=True)
+    seq, page = {"beginning": (0, 1), "behind one": (0, 2), "own": (1, f.shared // f.page)}[where]
+    damage(f.cache, seq, page, what)
+    ctx = F.Context(0)
+    out, lse = f.attend(ctx=ctx)
+    if what == "number":
+        with pytest.raises(F.FoError, match="page table"):
+            ctx.synchronize()
+    ctx.synchronize()
+    ctx.close()
+    sees = f.places >= page * f.page
+    if where == "own":
+        sees = (np.arange(len(f.places)) // f.n == 1) & (f.places >= f.shared)
+    assert sees.any()
+    at = torch.from_numpy(sees).cuda()
+    assert out[at].isnan().all() and lse[at].isnan().all()
+    f.check(out, lse, np.nonzero(~sees)[0])
