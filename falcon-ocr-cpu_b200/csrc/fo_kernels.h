@@ -284,7 +284,10 @@ struct fo_paged_attention_launch {
 };
 #define FO_PAGED_QUERIES 48  // queries that a block holds at most
 cudaError_t fo_launch_paged_attention(const fo_paged_attention_launch *args, int sms, cudaStream_t stream);
-// The same kernel with a reach (paged_attention_reach.cu).
+// The same with a page's number outside the pool, or its scale that is not finite, lost
+// to the rows that see the page alone (paged_attention_window.cu).
+cudaError_t fo_launch_paged_attention_window(const fo_paged_attention_launch *args, int sms, cudaStream_t stream);
+// That with a reach (paged_attention_reach.cu).
 cudaError_t fo_launch_paged_attention_reach(const fo_paged_attention_launch *args, int sms, cudaStream_t stream);
 
 // Attention of many query rows over the paged cache on the 5th-generation

@@ -5,5 +5,5 @@
 #include "paged_attention.cuh"
 
 extern "C" cudaError_t fo_launch_paged_attention(const fo_paged_attention_launch *args, int sms, cudaStream_t stream) {
-    return fo::launch_attention<false>(*args, sms, stream);
+    return fo::launch_attention<false, false>(*args, sms, stream);
 }

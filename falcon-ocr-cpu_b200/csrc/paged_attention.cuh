@@ -69,11 +69,16 @@
 // TB/s.  A call of one short sequence takes 9.7 us, a chain of launch, length, page
 // number, tile and join.  Spills: 0 to 88 bytes of stores in a variant.
 //
-// With REACH (paged_attention_reach.cu; the variants without it are unchanged
-// by it) a row also sees a few first positions behind its window, whose tiles
-// come before the window's in the line.  64 sequences in a window of 4,096 with
-// 16 first positions, 2 query rows to each of 8 KV heads of 64: 60 us against a
-// floor of 41; a unit's change costs some 3 us and a unit here is short.
+// With LOST (paged_attention_window.cu) a page whose number is outside the pool, or
+// that has a scale that is not finite, makes NaN of the rows that see it and of no
+// others; without, a page number does of all rows of its unit.  (A flag in the
+// arguments in place of the variant: one short sequence 9.8 us for 9.6, a serving
+// step 31.7 for 30.8.)  64 sequences in a window of 4,096, 2 query rows to each of
+// 8 KV heads of 64, int8: 55 us either way.
+// With REACH too (paged_attention_reach.cu) a row also sees a few first positions
+// behind its window, whose tiles come before the window's in the line.  Those 64
+// sequences with 16 first positions: 57.4 us against a floor of 41; a unit's change
+// costs some 3 us and a unit here is short.
 #pragma once
 
 #include "paged.cuh"
@@ -595,7 +600,7 @@ __device__ __forceinline__ void pa_epilogue(const fo_paged_attention_launch &a, 
     }
 }
 
-template <int D, int FORMAT, bool F32, bool REACH>
+template <int D, int FORMAT, bool F32, bool REACH, bool LOST>
 __global__ void __launch_bounds__(PA_THREADS, 1)
     paged_attention_kernel(const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
                            const __grid_constant__ fo_paged_attention_launch a) {
@@ -835,13 +840,13 @@ __global__ void __launch_bounds__(PA_THREADS, 1)
                 if (here) {
                     // A page number outside the pool gives NaN; a page that no row
                     // sees has scales of 0.
-                    if constexpr (REACH) {
+                    if constexpr (LOST) {
                         // Like values that are not finite, by the scores: rows that do not see the page are
                         // not changed by it.
                         const bool lost = now.bad || !(fabsf(now.ks) <= FLT_MAX && fabsf(now.vs) <= FLT_MAX);
                         sh.scales[slot][j] = lost ? NAN : now.ks;
                         sh.scales[slot][8 + j] = lost ? 0.0f : now.vs;
-                        if (now.bad) {
+                        if (FORMAT == FO_PAGED_E4M3 && now.bad) {  // (what is there may be NaN)
                             uint4 *vt = reinterpret_cast<uint4 *>(tiles + slot * Shape::STAGE + Shape::TILE_BYTES + j * bytes);
                             for (uint32_t x = 0; x < bytes / 16; x++) vt[x] = make_uint4(0, 0, 0, 0);
                             sm100::fence_proxy_async_smem();  // these before the next copy
@@ -1310,9 +1315,9 @@ inline bool pa_map(CUtensorMap *map, const void *codes, const fo_paged_kv &kv) {
               CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int D, int FORMAT, bool F32, bool REACH>
+template <int D, int FORMAT, bool F32, bool REACH, bool LOST>
 cudaError_t launch_attention(const fo_paged_attention_launch &a, unsigned grid, cudaStream_t stream) {
-    auto *kernel = paged_attention_kernel<D, FORMAT, F32, REACH>;
+    auto *kernel = paged_attention_kernel<D, FORMAT, F32, REACH, LOST>;
     using Shape = PaShape<D, FORMAT, F32>;
     static_assert(Shape::smem(PA_CONSUMERS / 2) + sizeof(PaShared) <= 227 * 1024, "shared memory");
     // The attribute belongs to each device's context: set once per device.
@@ -1337,16 +1342,16 @@ cudaError_t launch_attention(const fo_paged_attention_launch &a, unsigned grid, 
     return launch(kernel, dim3(grid), dim3(PA_THREADS), Shape::smem(a.queries / 8), stream, k_map, v_map, a);
 }
 
-template <int D, bool REACH>
+template <int D, bool REACH, bool LOST>
 cudaError_t launch_attention(const fo_paged_attention_launch &a, unsigned grid, cudaStream_t stream) {
     if (a.q.dtype == FO_DT_F32)
-        return a.kv.format == FO_PAGED_I8 ? launch_attention<D, FO_PAGED_I8, true, REACH>(a, grid, stream)
-                                          : launch_attention<D, FO_PAGED_E4M3, true, REACH>(a, grid, stream);
-    return a.kv.format == FO_PAGED_I8 ? launch_attention<D, FO_PAGED_I8, false, REACH>(a, grid, stream)
-                                      : launch_attention<D, FO_PAGED_E4M3, false, REACH>(a, grid, stream);
+        return a.kv.format == FO_PAGED_I8 ? launch_attention<D, FO_PAGED_I8, true, REACH, LOST>(a, grid, stream)
+                                          : launch_attention<D, FO_PAGED_E4M3, true, REACH, LOST>(a, grid, stream);
+    return a.kv.format == FO_PAGED_I8 ? launch_attention<D, FO_PAGED_I8, false, REACH, LOST>(a, grid, stream)
+                                      : launch_attention<D, FO_PAGED_E4M3, false, REACH, LOST>(a, grid, stream);
 }
 
-template <bool REACH>
+template <bool REACH, bool LOST>
 cudaError_t launch_attention(const fo_paged_attention_launch &args, int sms, cudaStream_t stream) {
     fo_paged_attention_launch a = args;
     if (a.batch.total_rows <= 0) return cudaSuccess;
@@ -1375,7 +1380,8 @@ cudaError_t launch_attention(const fo_paged_attention_launch &args, int sms, cud
     if (a.whole_units) blocks = std::max(blocks, units);
     const unsigned grid = (unsigned)std::max<int64_t>(1, blocks);
     if (most > INT32_MAX) return cudaErrorInvalidValue;
-    return a.kv.head_dim == 64 ? launch_attention<64, REACH>(a, grid, stream) : launch_attention<128, REACH>(a, grid, stream);
+    return a.kv.head_dim == 64 ? launch_attention<64, REACH, LOST>(a, grid, stream)
+                               : launch_attention<128, REACH, LOST>(a, grid, stream);
 }
 
 }  // namespace fo

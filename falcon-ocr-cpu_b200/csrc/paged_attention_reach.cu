@@ -5,5 +5,5 @@
 
 extern "C" cudaError_t fo_launch_paged_attention_reach(const fo_paged_attention_launch *args, int sms,
                                                        cudaStream_t stream) {
-    return fo::launch_attention<true>(*args, sms, stream);
+    return fo::launch_attention<true, true>(*args, sms, stream);
 }

@@ -630,7 +630,8 @@ int fo_paged_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch 
  * prompt's): the row at position p sees the positions j <= p with j < first or
  * p - j < window (window 0: all of them).  Pages that no row sees are not read.
  * Rows that see nothing, and rows that are not finite, as there; a page number
- * outside the pool and a scale that is not finite give NaN.
+ * outside the pool and a scale that is not finite give NaN to the rows that see
+ * the page, and to no others.
  *
  * Few query rows of a KV head (a sequence's rows times the query heads of one:
  * up to 48 with a head_dim of 64, up to 24 with 128; beside longer sequences up

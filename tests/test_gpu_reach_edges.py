@@ -178,6 +178,44 @@ def test_a_lost_page_in_windows(fmt, dim, dtype, what, rows):
 
 @pytest.mark.parametrize("fmt,dim,dtype", [("i8", 64, "bf16"), ("e4m3", 128, "f32")])
 @pytest.mark.parametrize("what", WHAT)
+@pytest.mark.parametrize("window,first", [(0, 0), (20, 0), (0, 7), (20, 7)])
+@pytest.mark.parametrize("call,rows", [("window", 12), ("window", 20), ("window", 60), ("no groups", 12)])
+def test_a_lost_page_whatever_the_window(fmt, dim, dtype, what, window, first, call, rows):
+    """Rows before the page, and those whose window is behind it, with and without first positions."""
+    if call == "no groups" and (window or first):
+        pytest.skip("a beginning that nothing shares has no window")
+    rng, n = np.random.default_rng(6), 90
+    cache = Cache(rng, fmt, dim, 16, 1, [n])
+    values, kv = [cache.values(i, 0) for i in range(2)], cache.on_device()
+    lost = (n - rows // 2) // 16  # the page that the rows come to half way
+    damage(cache, 0, lost, what)
+    q, _ = rows_of(rng, rows, 2, dim, dtype)
+    out, lse, ctx = torch.full_like(q, 9.0), torch.full((rows, 2), 9.0, device="cuda"), F.Context(0)
+    if call == "window":
+        F.paged_window_attention(kv, cache.batch([rows], False), q, out, window=window, first=first, lse=lse, ctx=ctx)
+    else:
+        groups = F.PagedGroups(dev(np.array([0], np.int32)), torch.empty(0, dtype=torch.int32, device="cuda"))
+        F.paged_prefix_attention(kv, cache.batch([rows], False), groups, q, out, lse=lse, ctx=ctx)
+    if what == "number":
+        with pytest.raises(F.FoError, match="page table"):
+            ctx.synchronize()
+    ctx.synchronize()
+    ctx.close()
+    place = np.arange(n - rows, n)
+    sees = place >= 16 * lost
+    if window:
+        sees &= place - (16 * lost + 15) < window
+    assert sees.any()
+    others = {(0, int(r)) for r in np.nonzero(~sees)[0]}
+    check_rows(out, lse, q.double().cpu().numpy(), [rows], [n], lambda b: values, lambda p: seen_of(p, window, first), None,
+               dim ** -0.5, dtype, only=others)
+    at = torch.from_numpy(sees).cuda()
+    # (A key scale of infinity: some of a row's scores are above 0.)
+    assert out[at].isnan().all() and lse[at].isnan().all()
+
+
+@pytest.mark.parametrize("fmt,dim,dtype", [("i8", 64, "bf16"), ("e4m3", 128, "f32")])
+@pytest.mark.parametrize("what", WHAT)
 @pytest.mark.parametrize("form", list(FORMS))
 @pytest.mark.parametrize("where", ["beginning", "behind one", "own"])
 def test_a_lost_page_of_shared_beginnings(form, where, what, fmt, dim, dtype):
