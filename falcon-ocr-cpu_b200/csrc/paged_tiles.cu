@@ -520,8 +520,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                         *place(lane, x + CHUNKS / 2) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                     }
                 }
-                // Zeros, and rows of no query, have scores of 0 at any scale; at this one they go the short way.
-                if (most == 0) q_scale = a.scale * REACH_LOG2E;
+                // Zeros, rows of no query and those that see nothing have scores of 0 at any scale; at this one
+                // they go the short way.
+                if (most == 0 || high < 0) q_scale = a.scale * REACH_LOG2E;
                 if (!pair) sh.q_scale[r] = q_scale;
                 fence_proxy_async_smem();
             }
@@ -608,8 +609,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 int tile_top = meta.top;
                 const int hi = min(high, meta.to - 1), lo = max(low, meta.from);
                 // The scores' factors will multiply -infinity too, of which a product that underflows to 0
-                // would make NaN.
-                const bool plain = __all_sync(0xffffffffu, meta.least * q_scale >= FLT_MIN);
+                // would make NaN.  (Rows that are not finite are NaN either way, and do not send the others
+                // round about, where their scores are rounded once more.)
+                const bool plain = __all_sync(0xffffffffu, !(meta.least * q_scale < FLT_MIN));
                 const bool all = hi - tile >= PT_TILE - 1 && (lo <= tile || a.reach.first - tile >= PT_TILE);
                 if (!__all_sync(0xffffffffu, plain && all)) {
                     // Scores of keys that the row does not see become -infinity in tensor memory, 32 keys

@@ -178,12 +178,10 @@ def test_a_lost_page_in_windows(fmt, dim, dtype, what, rows):
 
 @pytest.mark.parametrize("fmt,dim,dtype", [("i8", 64, "bf16"), ("e4m3", 128, "f32")])
 @pytest.mark.parametrize("what", WHAT)
-@pytest.mark.parametrize("window,first", [(0, 0), (20, 0), (0, 7), (20, 7)])
-@pytest.mark.parametrize("call,rows", [("window", 12), ("window", 20), ("window", 60), ("no groups", 12)])
-def test_a_lost_page_whatever_the_window(fmt, dim, dtype, what, window, first, call, rows):
+@pytest.mark.parametrize("call,rows,window,first", [("window", rows, *reach) for rows in (12, 20, 60)
+                                                    for reach in ((0, 0), (20, 0), (0, 7), (20, 7))] + [("no groups", 12, 0, 0)])
+def test_a_lost_page_whatever_the_window(fmt, dim, dtype, what, call, rows, window, first):
     """Rows before the page, and those whose window is behind it, with and without first positions."""
-    if call == "no groups" and (window or first):
-        pytest.skip("a beginning that nothing shares has no window")
     rng, n = np.random.default_rng(6), 90
     cache = Cache(rng, fmt, dim, 16, 1, [n])
     values, kv = [cache.values(i, 0) for i in range(2)], cache.on_device()
@@ -238,3 +236,26 @@ def test_a_lost_page_of_shared_beginnings(form, where, what, fmt, dim, dtype):
     at = torch.from_numpy(sees).cuda()
     assert out[at].isnan().all() and lse[at].isnan().all()
     f.check(out, lse, np.nonzero(~sees)[0])
+
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("form", list(FORMS))
+@pytest.mark.parametrize("scale", [None, -0.3, 0.0, 1e-3])
+def test_queries_of_shared_beginnings(form, dtype, scale):
+    """Rows of zeros, tiny and large ones beside ordinary ones; rows that are not finite are NaN and alone."""
+    for fmt, dim in (("i8", 64), ("e4m3", 128)):
+        f = SharedForm(form, 10, fmt, dim, dtype)
+        total = len(f.places)
+        f.q[0::4] = 0
+        f.q[1::4] *= 1e-30
+        f.q[2::4] *= 8
+        out, lse = f.attend(scale)
+        f.check(out, lse, range(0, total, max(total // 40, 1)), scale)
+        bad = [1, 2, total - 1] if total > 4 else [1, 2]
+        f.q[bad[0]], f.q[bad[1], 0, 3], f.q[bad[-1], -1, 9] = np.nan, np.inf, -np.inf
+        again, lse_again = f.attend(scale)
+        heads = torch.ones(total, f.group, dtype=torch.bool, device="cuda")
+        heads[bad[0]], heads[bad[1], 0], heads[bad[-1], -1] = False, False, False
+        assert torch.equal(again[heads], out[heads]) and torch.equal(lse_again[heads], lse[heads])
+        assert again[~heads].isnan().all() and lse_again[~heads].isnan().all()
