@@ -12,7 +12,7 @@ torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
 from test_gpu_paged import Cache, dev, rows_of  # noqa: E402
-from test_gpu_reach import SharedCache, check_rows, seen_of  # noqa: E402
+from test_gpu_reach import SharedCache, check_rows, prefix_case, seen_of, window_case  # noqa: E402
 
 
 def attend_window(cache, rows, q, window, first, scale=None, ctx=None):
@@ -259,3 +259,91 @@ def test_queries_of_shared_beginnings(form, dtype, scale):
         heads[bad[0]], heads[bad[1], 0], heads[bad[-1], -1] = False, False, False
         assert torch.equal(again[heads], out[heads]) and torch.equal(lse_again[heads], lse[heads])
         assert again[~heads].isnan().all() and lse_again[~heads].isnan().all()
+
+
+# ------------------------------------------------ both sides of the kernels' limits
+@pytest.mark.parametrize("rows", [20, 60])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_scales_of_queries_in_every_kernel(rows, dim):
+    """Two query heads: 40 rows of a KV head of 64 are the few rows' kernel's, of 128, and 120, the many rows'."""
+    window_case(7, "i8", dim, 32, 2, 2, "f32", [500], [rows], q_scale=1e-6, scale=1e5)
+    window_case(7, "i8", dim, 32, 2, 2, "bf16", [500], [rows], q_scale=2.0 ** 20, scale=2.0 ** -21)
+    window_case(8, "e4m3", dim, 32, 2, 2, "f32", [500], [rows], scale=3.0)
+    for dtype in ("f32", "bf16"):
+        window_case(9, "i8", dim, 32, 2, 2, dtype, [70], [rows], q_scale=0.0, window=30, first=3)
+        window_case(9, "e4m3", dim, 32, 2, 2, dtype, [70], [rows], scale=-0.3, window=30, first=3)
+        window_case(9, "i8", dim, 32, 2, 2, dtype, [300], [rows], scale=0.0)
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_a_prompt_at_once_and_in_short_pieces(fmt, dtype):
+    """The many rows' kernel for 120 rows, and the few rows' for the same in calls of 12: each is within its bound of
+    the float64 form, so they are within twice that of each other."""
+    rng = np.random.default_rng(11)
+    n, rows, piece = 700, 120, 12
+    for dim, window, first in ((64, 0, 0), (64, 100, 20), (128, 100, 20)):
+        cache = Cache(rng, fmt, dim, 32, 2, [n])
+        kv = cache.on_device()
+        q, _ = rows_of(rng, rows, 4, dim, dtype)
+        whole, lse = torch.full_like(q, 9.0), torch.full((rows, 4), 9.0, device="cuda")
+        F.paged_window_attention(kv, cache.batch([rows], False), q, whole, window=window, first=first, lse=lse)
+        pieces, lses = torch.full_like(q, 9.0), torch.full((rows, 4), 9.0, device="cuda")
+        for r in range(0, rows, piece):
+            batch = F.PagedBatch(dev(cache.table), dev(np.array([n - rows + r + piece], np.int32)), rows=piece)
+            F.paged_window_attention(kv, batch, q[r:r + piece], pieces[r:r + piece], window=window, first=first,
+                                     lse=lses[r:r + piece])
+        values = [(cache.values(0, 0), cache.values(1, 0))]
+        for out, z in ((whole, lse), (pieces, lses)):
+            check_rows(out, z, q.double().cpu().numpy(), [rows], [n], lambda b: values[b],
+                       lambda p: seen_of(p, window, first), None, dim ** -0.5, dtype)
+        k, v = values[0]
+        size = max(float((np.abs(k[h // 2]) @ np.abs(q[:, h].double().cpu().numpy().T)).max()) for h in range(4)) * dim ** -0.5
+        d, top = 2.0 ** -17 * size, np.abs(v).max()
+        bound = 2 * (4 * d + 2.0 ** -18 + (2.0 ** -11 if dtype == "bf16" else 2.0 ** -22)) * top
+        if dtype == "bf16":
+            bound += 2 * torch.finfo(torch.bfloat16).eps / 2 * top  # each rounded once
+        assert float((whole.double() - pieces.double()).abs().max()) <= bound
+
+
+@pytest.mark.parametrize("dim,dtype", [(64, "bf16"), (128, "f32")])
+@pytest.mark.parametrize("prompt", [200, 900])
+def test_a_decode_step_beside_a_prompt_over_shared_beginnings(dim, dtype, prompt):
+    """Groups of several sequences, single rows beside prompts: below and above 64 query rows on average, in and out of
+    groups."""
+    rows = [1, 1, prompt, 1, 1, 0, 2, 1, 1, 70]
+    own = [5, 40, prompt + 3, 1, 130, 2, 2, 9, 64, 90]
+    some = {(b, r) for b, n in enumerate(rows) for r in range(n) if r < 3 or r % 61 == 0 or r == n - 1}
+    prefix_case(12, "e4m3", dim, 32, 2, 2, dtype, [1, 5, 8], [333, 128], own, rows, ragged=True, only=some)
+    prefix_case(13, "i8", dim, 16, 1, 4, dtype, [0, 10], [150], own, rows, ragged=True, only=some)
+
+
+@pytest.mark.parametrize("group", [40, 100, 300])
+@pytest.mark.parametrize("dim,dtype", [(64, "bf16"), (128, "f32")])
+def test_many_query_heads(group, dim, dtype):
+    """Units that end inside a row's heads, rows that are several units."""
+    window_case(14, "i8", dim, 32, 1, group, dtype, [90, 3, 0, 200], [1] * 4, window=50, first=3)
+    window_case(14, "e4m3", dim, 16, 2, group, dtype, [90, 40], [3, 0], ragged=True)
+    prefix_case(15, "i8", dim, 32, 1, group, dtype, [0, 3], [100], [1, 30, 70], [1] * 3)
+    prefix_case(15, "e4m3", dim, 16, 2, group, dtype, [0, 2, 3], [40, 16], [9, 30, 5], [2, 0, 5], ragged=True)
+
+
+@pytest.mark.parametrize("form", list(FORMS))
+def test_sinks_that_take_nothing_and_all(form):
+    """Terms of 0 and of infinity; those of large sinks are exp(80)."""
+    f = SharedForm(form, 16, "i8", 64, "f32")
+    groups = F.PagedGroups(dev(np.array([0, f.seqs], np.int32)), dev(np.array([f.shared], np.int32)))
+    batch, without = f.cache.batch([f.n] * f.seqs, False), f.attend()[0]
+    for sink in (-np.inf, np.inf, 80.0):
+        out, lse = torch.full_like(f.q, 9.0), torch.full(f.q.shape[:2], 9.0, device="cuda")
+        F.paged_prefix_attention(f.kv, batch, groups, f.q, out, sinks=torch.full((f.group,), sink, device="cuda"), lse=lse)
+        if sink == -np.inf:
+            assert torch.equal(out, without)
+        elif sink == np.inf:
+            assert (out == 0).all()
+        else:
+            # out / without = e^lse / (e^lse + e^80): the exponent (some 116 in log2 units) is held to 2^-17, the
+            # rest to 2^-18.
+            expected = without.double() * (1 / (1 + torch.exp(80.0 - lse.double())))[..., None]
+            assert ((out.double() - expected).abs() <= expected.abs() * (2.0 ** -16 + 2.0 ** -18)).all()
+        assert lse[torch.from_numpy(f.places >= 0).cuda()].isfinite().all()
