@@ -347,3 +347,64 @@ def test_sinks_that_take_nothing_and_all(form):
             expected = without.double() * (1 / (1 + torch.exp(80.0 - lse.double())))[..., None]
             assert ((out.double() - expected).abs() <= expected.abs() * (2.0 ** -16 + 2.0 ** -18)).all()
         assert lse[torch.from_numpy(f.places >= 0).cuda()].isfinite().all()
+
+
+# ------------------------------------------------------------------ far positions, large pools
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+@pytest.mark.parametrize("rows", [1, 12, 60])
+@pytest.mark.parametrize("first", [0, 20])
+def test_windows_near_two_to_the_31(fmt, rows, first):
+    """A table with room for nearly 2^31 positions whose pages between the first positions and the window are gone."""
+    page, dim, window = 16, 64, 50
+    room = (2 ** 31 - 1) // page
+    n, near = room * page, 8 * page  # positions; those whose pages are there at the end
+    rng = np.random.default_rng(20)
+    cache = Cache(rng, fmt, dim, page, 2, [10 * page])
+    table = torch.full((1, room), -1, dtype=torch.int32, device="cuda")
+    table[0, :2] = dev(cache.table[0, :2])
+    table[0, -8:] = dev(cache.table[0, 2:])
+    kv = cache.on_device()
+    q, _ = rows_of(rng, rows, 4, dim, "f32")
+    out, lse, ctx = torch.full_like(q, 9.0), torch.full((rows, 4), 9.0, device="cuda"), F.Context(0)
+    batch = F.PagedBatch(table, dev(np.array([n], np.int32)), rows=rows)
+    F.paged_window_attention(kv, batch, q, out, window=window, first=first, lse=lse, ctx=ctx)
+    ctx.synchronize()
+    ctx.close()
+    values = (cache.values(0, 0), cache.values(1, 0))
+
+    def seen(p):  # of the pages that are there
+        return np.concatenate((np.arange(first), np.arange(p + 1 - window, p + 1)))
+
+    check_rows(out, lse, q.double().cpu().numpy(), [rows], [2 * page + near], lambda b: values, seen, None, dim ** -0.5, "f32")
+
+
+@pytest.mark.parametrize("fmt", ["i8", "e4m3"])
+def test_offsets_beyond_32_bits(fmt):
+    """The last pages of a pool of more than 2^32 bytes, by every kernel of the two calls."""
+    page, kv_heads, dim, held = 128, 8, 128, 500
+    pages = (1 << 32) // (page * kv_heads * dim) + 40
+    rng = np.random.default_rng(21)
+    small = Cache(rng, fmt, dim, page, kv_heads, [held])
+    small.on_device()
+    pool = [torch.zeros(pages, kv_heads, page, dim, dtype=torch.int8, device="cuda") for _ in range(2)]
+    scales = [torch.zeros(pages, kv_heads, device="cuda") for _ in range(2)]
+    ids = np.arange(pages - 1, pages - 5, -1, dtype=np.int32)
+    for i in range(2):
+        for j, at in enumerate(ids):
+            pool[i][int(at)] = small.dev[i][int(small.table[0, j])].view(torch.int8)
+            scales[i][int(at)] = small.dev[2 + i][int(small.table[0, j])]
+    kind = torch.int8 if fmt == "i8" else torch.float8_e4m3fn
+    kv, values = F.PagedKv(*(c.view(kind) for c in pool), *scales), (small.values(0, 0), small.values(1, 0))
+    for seqs, rows in ((1, 1), (40, 1), (2, 40), (1, 100)):  # (of shared beginnings, each in a form of its own)
+        q, _ = rows_of(rng, seqs * rows, kv_heads, dim, "f32")
+        batch = F.PagedBatch(dev(np.repeat(ids[None], seqs, 0)), dev(np.full(seqs, held, np.int32)), rows=rows)
+        groups = F.PagedGroups(dev(np.array([0, seqs], np.int32)), dev(np.array([300], np.int32)))
+        only = {(b, r) for b in range(0, seqs, 13) for r in range(0, rows, 9)}
+        for call in ("window", "prefix"):
+            out, lse = torch.full_like(q, 9.0), torch.full(q.shape[:2], 9.0, device="cuda")
+            if call == "window":
+                F.paged_window_attention(kv, batch, q, out, window=200, first=7, lse=lse)
+            else:
+                F.paged_prefix_attention(kv, batch, groups, q, out, lse=lse)
+            check_rows(out, lse, q.double().cpu().numpy(), [rows] * seqs, [held] * seqs, lambda b: values,
+                       lambda p: seen_of(p, 200, 7) if call == "window" else seen_of(p, 0, 0), None, dim ** -0.5, "f32", only)
