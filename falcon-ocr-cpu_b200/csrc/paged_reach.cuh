@@ -1,7 +1,7 @@
 // paged_reach.cuh -- what a row of a paged attention sees when that is more
 // than "its sequence's newest positions": groups of sequences that share their
 // beginnings, and rows that are joined from two attentions over different
-// positions.  Device helpers of paged_attention.cuh and paged_tiles.cu.
+// positions.  Device helpers of paged_tiles.cu and paged_few.cu.
 #pragma once
 
 #include "paged.cuh"

@@ -636,11 +636,13 @@ int fo_paged_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch 
  * Few query rows of a KV head (a sequence's rows times the query heads of one:
  * up to 48 with a head_dim of 64, up to 24 with 128; beside longer sequences up
  * to 8, or 16 where a KV head has more than 8 query heads, and only if the batch
- * can hold eight such) are computed as fo_paged_attention's; more as FP16 products with FP32 sums: codes are exact, a
- * query element is held to 2^-11 (FP32 rows: 2^-22) of itself, which BF16 rows'
- * are exactly, or to 2^-39 of the largest of its row and head; a probability to
- * 2^-11 (2^-22) of itself, or to 2^-35 of its row's largest.  The sum of
- * probabilities has no such rounding.
+ * can hold eight such) are computed as fo_paged_attention's; more as FP16
+ * products with FP32 sums: codes are exact, a query element is held to 2^-11
+ * (FP32 rows: 2^-22) of itself, which BF16 rows' are exactly, or to 2^-39 of the
+ * largest of its row and head; a probability to 2^-11 (2^-22) of itself, or to
+ * 2^-35 of its row's largest.  The sum of probabilities has no such rounding.
+ * Calls with the same contents give the same bits; with other sequences or rows
+ * beside it, a row may be rounded elsewhere within these bounds.
  *
  * A sequence's rows times the query heads of a KV head are at most 2^31 - 1,
  * and so are the tiles of 8 KB of keys that the page tables have room for, of
@@ -655,21 +657,28 @@ int fo_paged_window_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged
  * in the page table; what the others have there is not read, but for the page
  * that position lens[g] falls into, where each has its own from that position
  * on.  Sequences before the first group and behind the last share nothing.
- * Starts that do not ascend within the batch and lengths beyond the page table are
- * reported by the error word; what the rows of such groups hold is undefined. */
+ * Starts that do not ascend within the batch and lengths beyond the page table
+ * are reported by the error word; what the rows of such groups hold is
+ * undefined. */
 typedef struct {
     const int32_t *seq_start; /* [n_groups + 1] */
     const int32_t *lens;      /* [n_groups] */
     int64_t n_groups;
 } fo_paged_groups;
 
-/* Attention of rows whose sequences share their beginnings, which are read once
- * for all rows of a group: the row at position p sees positions 0 .. p, as in
- * fo_paged_attention without a window.  Limits as in fo_paged_window_attention,
- * rounding as of many query rows there.  Where a KV head has fewer than 64 query rows of a
- * sequence on average, unfinished rows wait in the context's scratch, total_rows *
- * n_heads * (head_dim + 4) floats: a call that needs more of it than any before
- * makes it, which a graph's capture refuses (what graphs use is kept). */
+/* Attention of rows whose sequences share their beginnings: the row at position
+ * p sees positions 0 .. p, as in fo_paged_attention without a window.  Limits and
+ * lost pages as in fo_paged_window_attention, rounding as of many query rows
+ * there (n_groups 0: as there).
+ *
+ * Where a KV head has fewer than 64 query rows of a sequence on average over the
+ * batch's sequences (empty ones among them), a beginning is read once for all
+ * rows of its group, and unfinished rows wait in the context's scratch,
+ * total_rows * n_heads * (head_dim + 4) floats: a call that needs more of it than
+ * any before makes it, which a graph's capture refuses (what graphs use is kept).
+ * With more, each sequence reads its beginning by itself.  A long prompt among
+ * single rows is better off in a call of its own: 63 rows and a prompt of 2,048
+ * over 16,384 positions take 1,424 us in one call, 39 and 315 in two. */
 int fo_paged_prefix_attention(fo_ctx *ctx, const fo_paged_kv *kv, const fo_paged_batch *batch,
                               const fo_paged_groups *groups, const fo_rows *q, const float *sinks, float scale,
                               const fo_rows *out, float *lse);
