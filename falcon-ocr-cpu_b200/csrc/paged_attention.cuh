@@ -175,9 +175,11 @@ __device__ __forceinline__ uint32_t pa_transpose(uint32_t x) {
     asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
+// (The largest number in place of infinity: of maxima beyond 2^27, 2^10 less is
+// rounded to 2^16 less, for which FP16 has no room.)
 __device__ __forceinline__ uint32_t pa_f16x2(float lo, float hi) {
     uint32_t r;
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    asm("cvt.rn.satfinite.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
 

@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(PF_THREADS, F32 && NT == 2 ? 1 : 2)
                 const int p = pos + g + 8 * (e >> 1);
                 const bool seen = p >= from && p <= place[x][e & 1];
                 c[x][e] = seen ? c[x][e] * (now.ks * q_scale[x][e & 1]) : -INFINITY;
-                moves |= c[x][e] > m[x][e & 1] + PF_SLACK || (seen && step_top > top[x][e & 1]);
+                moves |= c[x][e] - m[x][e & 1] > PF_SLACK || (seen && step_top > top[x][e & 1]);
             }
         if (__any_sync(0xffffffffu, moves)) {
             float factor[NT][2];

@@ -123,10 +123,10 @@ struct PtSegment {
     int part;                 // scratch of an unfinished unit's part, -1: the unit is whole
 };
 
-struct PtMeta {
+struct alignas(8) PtMeta {  // (its scales are read in pairs)
     float ks[8], vs[8];  // keys' and values' scales of each 16 positions' page
     int top;             // exponent bits of a power of two above the values' scales
-    float least;         // the least of the keys' scales, 0: one is not a number above 0
+    float least, most;   // the least of the keys' scales, 0: one is not a number above 0; and the largest
     int base;            // the tile's first position
     int from, to;        // positions [from, to) that rows may see of it
     unsigned pages;      // pages that were copied
@@ -610,9 +610,11 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 int tile_top = meta.top;
                 const int hi = min(high, meta.to - 1), lo = max(low, meta.from);
                 // The scores' factors will multiply -infinity too, of which a product that underflows to 0
-                // would make NaN.  (Rows that are not finite are NaN either way, and do not send the others
-                // round about, where their scores are rounded once more.)
-                const bool plain = __all_sync(0xffffffffu, !(meta.least * q_scale < FLT_MIN));
+                // would make NaN; and scores that may pass 2^25 (sums of D products below 2^15 448, times their
+                // factor) are rounded before their maximum is taken from them, or what is left, exact, could
+                // be more than P has room for.  (Rows that are not finite are NaN either way, and do not send
+                // the others round about, where their scores are rounded once more.)
+                const bool plain = __all_sync(0xffffffffu, !(meta.least * q_scale < FLT_MIN || meta.most * q_scale > 0x1p-6f));
                 const bool all = hi - tile >= PT_TILE - 1 && (lo <= tile || a.reach.first - tile >= PT_TILE);
                 if (!__all_sync(0xffffffffu, plain && all)) {
                     // Scores of keys that the row does not see become -infinity in tensor memory, 32 keys
@@ -685,7 +687,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 if (!any) {
                     m = mx;
                     top = tile_top;
-                } else if (__any_sync(0xffffffffu, mx > m + PT_SLACK || tile_top > top)) {
+                } else if (__any_sync(0xffffffffu, mx - m > PT_SLACK || tile_top > top)) {
                     const float next = fmaxf(m, mx);
                     const float alpha = next == -INFINITY ? 1.0f : ex2(m - next);
                     l *= alpha;
@@ -1133,7 +1135,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 }
                 // (Numbers above 0 are in their bits' order.)
                 const float least = __uint_as_float(__reduce_min_sync(0xffffffffu, ks > 0.0f ? __float_as_uint(ks) : 0u));
-                if (lane == 8) meta.top = pt_above(most), meta.least = least;
+                const float largest =
+                    __uint_as_float(__reduce_max_sync(0xffffffffu, now.wanted && ks > 0.0f ? __float_as_uint(ks) : 0u));
+                if (lane == 8) meta.top = pt_above(most), meta.least = least, meta.most = largest;
                 if (lane == 9) meta.base = now.base;
                 if (lane == 10) meta.pages = mask;
                 if (lane == 11) meta.from = now.from, meta.to = now.to;

@@ -408,3 +408,38 @@ def test_offsets_beyond_32_bits(fmt):
                 F.paged_prefix_attention(kv, batch, groups, q, out, lse=lse)
             check_rows(out, lse, q.double().cpu().numpy(), [rows] * seqs, [held] * seqs, lambda b: values,
                        lambda p: seen_of(p, 200, 7) if call == "window" else seen_of(p, 0, 0), None, dim ** -0.5, "f32", only)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("fmt,dim", [("i8", 64), ("e4m3", 128)])
+@pytest.mark.parametrize("factor", [2.0 ** 20, 2.0 ** 24, 2.0 ** 30, 2.0 ** 60])
+def test_scores_beyond_what_fp32_tells_apart(fmt, dim, dtype, factor):
+    """Scores of 1e7 to 1e20, whose steps in FP32 are larger than a softmax's whole range: which positions win goes by
+    rounding, and what comes out is a mean of values that the row sees (held to 2^-8 of the largest), never NaN."""
+    rng = np.random.default_rng(22)
+    cases = []
+    for rows, window, first in ((4, 0, 0), (4, 60, 5), (100, 0, 0), (100, 60, 5), (300, 0, 0)):
+        cache = Cache(rng, fmt, dim, 16, 1, [700, 320])
+        q, _ = rows_of(rng, 2 * rows, 2, dim, dtype)
+        q *= factor
+        out, lse = attend_window(cache, [rows] * 2, q, window, first, 1.0)
+        sequences = [(np.arange(n - rows, n), cache.values(1, b)) for b, n in enumerate(cache.lens)]
+        cases.append((out, lse, sequences, window, first))
+        if rows == 4:  # the older call's kernel is the same
+            out, lse = torch.full_like(q, 9.0), torch.full(q.shape[:2], 9.0, device="cuda")
+            F.paged_attention(cache.on_device(), cache.batch([rows] * 2, False), q, out, window=window, scale=1.0, lse=lse)
+            cases.append((out, lse, sequences, window, 0))
+    for form in FORMS:
+        f = SharedForm(form, 23, fmt, dim, dtype)
+        f.q *= factor
+        out, lse = f.attend(1.0)
+        cases.append((out, lse, [(f.places[b * f.n:(b + 1) * f.n], f.values[b][1]) for b in range(f.seqs)], 0, 0))
+    for out, lse, sequences, window, first in cases:
+        got, at = out.double().cpu().numpy(), 0
+        for places, v in sequences:
+            for p in places:
+                seen = seen_of(int(p), window, first)
+                top = np.abs(v[:, seen]).max(initial=0.0)
+                assert (np.abs(got[at]) <= top * (1 + 2.0 ** -8)).all(), (p, got[at])
+                at += 1
+        assert not lse.isnan().any()
