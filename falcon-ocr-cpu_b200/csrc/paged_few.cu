@@ -34,7 +34,7 @@ namespace fo {
 
 constexpr int PF_WARPS = 8, PF_THREADS = 32 * PF_WARPS;  // of a block at most
 constexpr int PF_LOWEST = 12;       // exponent bits of the least power of two that scales are relative to
-constexpr float PF_SLACK = 4.0f;    // log2: what a score may pass the maximum by before that moves
+constexpr float PF_SLACK = 4.0f;    // log2: what a score may pass the maximum by before that moves (no more: rounded down)
 
 __device__ __forceinline__ uint32_t pf_cluster_rank() {
     uint32_t r;
@@ -328,7 +328,7 @@ __global__ void __launch_bounds__(PF_THREADS, F32 && NT == 2 ? 1 : 2)
                 const int p = pos + g + 8 * (e >> 1);
                 const bool seen = p >= from && p <= place[x][e & 1];
                 c[x][e] = seen ? c[x][e] * (now.ks * q_scale[x][e & 1]) : -INFINITY;
-                moves |= c[x][e] - m[x][e & 1] > PF_SLACK || (seen && step_top > top[x][e & 1]);
+                moves |= c[x][e] > __fadd_rd(m[x][e & 1], PF_SLACK) || (seen && step_top > top[x][e & 1]);
             }
         if (__any_sync(0xffffffffu, moves)) {
             float factor[NT][2];

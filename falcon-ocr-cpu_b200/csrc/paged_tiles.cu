@@ -94,8 +94,9 @@ __device__ __forceinline__ int pt_above(float x) {
     return min(max((int)(__float_as_uint(x) >> 23 & 255u) + 1, PT_LOWEST), 253);
 }
 
-// A row's maximum moves only when a score passes it by more than 2^4: P stays
-// below 2^15, FP16's range.
+// A row's maximum moves only when a score passes it by more than 2^4 (the sum of
+// both rounded down, so by no more beyond 2^25 either): P stays below 2^15, FP16's
+// range.
 constexpr float PT_SLACK = 4.0f;
 
 template <int D, bool F32>
@@ -687,7 +688,7 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 if (!any) {
                     m = mx;
                     top = tile_top;
-                } else if (__any_sync(0xffffffffu, mx - m > PT_SLACK || tile_top > top)) {
+                } else if (__any_sync(0xffffffffu, mx > __fadd_rd(m, PT_SLACK) || tile_top > top)) {
                     const float next = fmaxf(m, mx);
                     const float alpha = next == -INFINITY ? 1.0f : ex2(m - next);
                     l *= alpha;
