@@ -522,9 +522,9 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                         *place(lane, x + CHUNKS / 2) = make_uint4(lo[0], lo[1], lo[2], lo[3]);
                     }
                 }
-                // Zeros, rows of no query and those that see nothing have scores of 0 at any scale; at this one
-                // they go the short way.
-                if (most == 0 || high < 0) q_scale = a.scale * REACH_LOG2E;
+                // Zeros, rows of no query and those that see nothing have scores of 0, or none, at any scale; at
+                // this one they go the short way.
+                if (most == 0 || high < 0) q_scale = 0x1p-30f;
                 if (!pair) sh.q_scale[r] = q_scale;
                 fence_proxy_async_smem();
             }
@@ -611,11 +611,12 @@ __global__ void __launch_bounds__(PT_THREADS, 1) paged_tiles_kernel(const __grid
                 int tile_top = meta.top;
                 const int hi = min(high, meta.to - 1), lo = max(low, meta.from);
                 // The scores' factors will multiply -infinity too, of which a product that underflows to 0
-                // would make NaN; and scores that may pass 2^25 (sums of D products below 2^15 448, times their
-                // factor) are rounded before their maximum is taken from them, or what is left, exact, could
-                // be more than P has room for.  (Rows that are not finite are NaN either way, and do not send
-                // the others round about, where their scores are rounded once more.)
-                const bool plain = __all_sync(0xffffffffu, !(meta.least * q_scale < FLT_MIN || meta.most * q_scale > 0x1p-6f));
+                // would make NaN; and scores that may pass 2^25 are rounded before their maximum is taken
+                // from them, or what is left, exact, could be more than P has room for.  (Rows that are not
+                // finite are NaN either way, and do not send the others round about, where their scores are
+                // rounded once more.)
+                constexpr float MOST = 0x1p25f / (0x1p15f * (FORMAT == FO_PAGED_I8 ? 128.0f : 448.0f) * D);
+                const bool plain = __all_sync(0xffffffffu, !(meta.least * q_scale < FLT_MIN || meta.most * q_scale > MOST));
                 const bool all = hi - tile >= PT_TILE - 1 && (lo <= tile || a.reach.first - tile >= PT_TILE);
                 if (!__all_sync(0xffffffffu, plain && all)) {
                     // Scores of keys that the row does not see become -infinity in tensor memory, 32 keys

@@ -443,3 +443,24 @@ def test_scores_beyond_what_fp32_tells_apart(fmt, dim, dtype, factor):
                 assert (np.abs(got[at]) <= top * (1 + 2.0 ** -8)).all(), (p, got[at])
                 at += 1
         assert not lse.isnan().any()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("fmt,dim", [("i8", 64), ("e4m3", 128)])
+@pytest.mark.parametrize("scale", [3e38, -3e38, 1e-30, 1e-40])
+@pytest.mark.parametrize("keys", [1.0, 1e4])
+def test_queries_of_zeros_at_any_scale(fmt, dim, dtype, scale, keys):
+    """Scores of 0, whatever the scale argument and the keys' scales: the mean of what is in sight."""
+    rng = np.random.default_rng(24)
+    for rows, window, first in ((4, 60, 5), (100, 60, 5), (100, 0, 0)):
+        cache = Cache(rng, fmt, dim, 16, 1, [300])
+        cache.scales[0] *= np.float32(keys)
+        q, _ = rows_of(rng, rows, 2, dim, dtype)
+        q.zero_()
+        out, lse = attend_window(cache, [rows], q, window, first, scale)
+        check_rows(out, lse, q.double().cpu().numpy(), [rows], [300], lambda b: (cache.values(0, 0), cache.values(1, 0)),
+                   lambda p: seen_of(p, window, first), None, scale, dtype)
+    for form in FORMS:
+        f = SharedForm(form, 25, fmt, dim, dtype)
+        f.q.zero_()
+        f.check(*f.attend(scale), range(0, len(f.places), max(len(f.places) // 30, 1)), scale)
