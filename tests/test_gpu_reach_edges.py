@@ -7,12 +7,13 @@ import numpy as np
 import pytest
 
 import fo_cuda as F
+import paged_reference as R
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
 
-from test_gpu_paged import Cache, dev, rows_of  # noqa: E402
-from test_gpu_reach import SharedCache, check_rows, prefix_case, seen_of, window_case  # noqa: E402
+from test_gpu_paged import Cache, dev, rows_of, within  # noqa: E402
+from test_gpu_reach import SharedCache, attend, check_rows, prefix_case, seen_of, window_case  # noqa: E402
 
 
 def attend_window(cache, rows, q, window, first, scale=None, ctx=None):
@@ -464,3 +465,65 @@ def test_queries_of_zeros_at_any_scale(fmt, dim, dtype, scale, keys):
         f = SharedForm(form, 25, fmt, dim, dtype)
         f.q.zero_()
         f.check(*f.attend(scale), range(0, len(f.places), max(len(f.places) // 30, 1)), scale)
+
+
+# ------------------------------------------------------------------ the most there can be
+@pytest.mark.parametrize("call", ["window", "window of few", "prefix", "prefix of one"])
+def test_the_most_sequences(call):
+    """65,535 of them, of 0 to 40 positions in pages that they share, some with many rows; as many groups."""
+    rng = np.random.default_rng(26)
+    n, page, dim = 65535, 16, 64
+    cache = Cache(rng, "i8", dim, page, 1, [page] * 90)
+    kv = cache.on_device()
+    ids = cache.table[:, 0]
+    table = ids[rng.integers(0, 90, (n, 3))].astype(np.int32)
+    lens = rng.integers(0, 41, n).astype(np.int32)
+    rows = np.minimum(1, lens) if call in ("window of few", "prefix") else np.where(rng.random(n) < 0.002, lens, np.minimum(lens, 1))
+    start = np.concatenate(([0], np.cumsum(rows))).astype(np.int32)
+    batch = F.PagedBatch(dev(table), dev(lens), rows=max(int(rows.max()), 1), row_start=dev(start))
+    q, qv = rows_of(rng, int(start[-1]), 2, dim, "f32")
+    out, lse, ctx = torch.full_like(q, 9.0), torch.full(q.shape[:2], 9.0, device="cuda"), F.Context(0)
+    shared = np.zeros(n, np.int32)
+    if call.startswith("window"):
+        F.paged_window_attention(kv, batch, q, out, window=20, first=3, lse=lse, ctx=ctx)
+    elif call == "prefix":  # every sequence a group of its own, over some of its positions
+        shared = rng.integers(0, 41, n).astype(np.int32)
+        groups = F.PagedGroups(dev(np.arange(n + 1, dtype=np.int32)), dev(shared))
+        F.paged_prefix_attention(kv, batch, groups, q, out, lse=lse, ctx=ctx)
+    else:  # one group of nearly all
+        groups = F.PagedGroups(dev(np.array([1, n - 1], np.int32)), dev(np.array([page], np.int32)))
+        table[1:n - 1, 0] = table[1, 0]
+        F.paged_prefix_attention(kv, batch, groups, q, out, lse=lse, ctx=ctx)
+    ctx.synchronize()
+    ctx.close()
+    got, got_lse = out.double().cpu().numpy(), lse.double().cpu().numpy()
+    assert np.isfinite(got).all() and not np.isnan(got_lse).any()
+    k, v = (R.decode(cache.codes[i], "i8") * cache.scales[i].astype(np.float64)[..., None, None] for i in range(2))
+    some = set(rng.integers(0, n, 300).tolist()) | set(np.nonzero(rows > 1)[0].tolist()) | {0, 1, n - 2, n - 1}
+    for b in sorted(some):
+        kk, vv = (x[table[b]].transpose(1, 0, 2, 3).reshape(1, -1, dim)[:, :lens[b]] for x in (k, v))
+        for r in range(rows[b]):
+            at, p = start[b] + r, lens[b] - rows[b] + r
+            seen = seen_of(int(p), 20, 3) if call.startswith("window") else seen_of(int(p), 0, 0)
+            o, z, size, top = attend(qv[at], kk, vv, seen, None, dim ** -0.5)
+            d = 2.0 ** -17 * size
+            assert within(got[at], o, 4 * d * top + (2.0 ** -18 + 2.0 ** -22) * top, "f32")
+            assert (np.abs(got_lse[at] - z) <= d + 2.0 ** -20 * (1 + np.abs(z))).all()
+
+
+def test_a_beginning_of_a_sequence_without_positions():
+    """The first of a group need only have the pages: its own length and rows may be none."""
+    for form in ("few", "many and few", "many and few, rows", "many", "alone"):
+        f = SharedForm(form, 27, "e4m3", 64, "bf16")
+        lens, rows = list(f.cache.lens), [f.n] * f.seqs
+        lens[0], rows[0] = 0, 0
+        start = dev(np.concatenate(([0], np.cumsum(rows))).astype(np.int32))
+        batch = F.PagedBatch(dev(f.cache.table), dev(np.array(lens, np.int32)), rows=f.n, row_start=start)
+        groups = F.PagedGroups(dev(np.array([0, f.seqs], np.int32)), dev(np.array([f.shared], np.int32)))
+        q = f.q[f.n:]
+        out, lse, ctx = torch.full_like(q, 9.0), torch.full(q.shape[:2], 9.0, device="cuda"), F.Context(0)
+        F.paged_prefix_attention(f.kv, batch, groups, q, out, lse=lse, ctx=ctx)
+        ctx.synchronize()
+        ctx.close()
+        check_rows(out, lse, q.double().cpu().numpy(), rows, lens, lambda b: f.values[b], lambda p: seen_of(p, 0, 0), None,
+                   0.125, "bf16", only={(b, r) for b in range(1, f.seqs) for r in range(0, f.n, 7)})
