@@ -13,8 +13,8 @@
 // warps, which is what long ranges want: 52 us for 64 uneven sequences of 1 to
 // 1,024 positions where this one takes 27, profiled and cold.  In FP32 on CUDA
 // cores this kernel took 36.)  Measured (CUDA graph, both parts): 8 readings of 6,544
-// positions 20.4 us; 64 continuations of 16,384, the shared part by paged_tiles.cu,
-// 50.0.
+// positions 20.5 us; 64 continuations of 16,384, the shared part by paged_tiles.cu,
+// 50.2.
 // Codes become FP16, which holds them exactly, in registers, where they lie as they
 // are loaded: 16 adjacent dimensions of a key to a lane are four k steps of
 // m16n8k16 products if the query's elements are taken in the same order, and of
@@ -554,7 +554,7 @@ cudaError_t launch_few(const fo_paged_few_launch &in, int sms, cudaStream_t stre
     int blocks = 1;
     while (blocks < 8 && 2 * blocks * busy <= 2 * sms) blocks *= 2;
     // Sixteen, which want that many SMs next to each other, for no more units than there are such
-    // neighbourhoods: 8 units over 6,544 positions 20.4 us with sixteen, 23.2 with eight; 16 units
+    // neighbourhoods: 8 units over 6,544 positions 20.5 us with sixteen, 23.2 with eight; 16 units
     // 37.0 and 33.2.
     if (blocks == 8 && 16 * busy <= sms) blocks = 16;
     a.warps = busy > 2 * sms ? 4 : 8;

@@ -44,9 +44,9 @@
 // Measured (CUDA graph): a prompt of 6,544 rows in windows of 1,024 with 64 first
 // positions, 2 query heads to each of 8 KV heads of 64, int8: 106 us, 0.15 of the
 // measured FP16 peak; 16 ragged prompts of up to 4,096 rows, 4 query heads to each of
-// 8 of 128, windows of 2,048 with 128, e4m3: 2,352 us, 0.36; 48 questions of up to 96
-// rows to 4 documents of up to 9,001, the same heads: 655 us, 0.26; FP32 rows, the
-// page's prompt 150 us, the ragged ones 5,227.  Of the
+// 8 of 128, windows of 2,048 with 128, e4m3: 2,366 us, 0.36; 48 questions of up to 96
+// rows to 4 documents of up to 9,001, the same heads: 657 us, 0.26; FP32 rows, the
+// page's prompt 150 us, the ragged ones 5,302.  Of the
 // prompt, profiled: 47.1 M warp instructions, 1.8 a cycle and SM, 92 % of the
 // instructions found in the instruction cache.  With heads of 128 a pair of tiles
 // takes 6,000 cycles, of which the products are 2,050: a stream waits 1,850 for its S,
